@@ -10,6 +10,8 @@ Public API (mirrors of the reference ``heimdall`` package):
   delta_rule_gqa                     heimdall/motor.py:70-102
   delta_rule_step                    heimdall/kernels.py:132-138
   window_attention                   heimdall/hibrit.py:336-361 (the math of _window_fp32)
+  prompt_attention                   heimdall/hibrit.py:275-290 (a kept layer's causal attention, packed prompts)
+  PagedKV                            a kept layer's cache in 8-bit pages: append, attend, fork, free, compact
   BifrostLayer.student               heimdall/hibrit.py:363-424 (HybridAttention._student)
   BifrostLayer.mem_inputs            heimdall/hibrit.py:327-334
   BifrostLayer.student_host          _student for host (pinned) inputs, copies overlapped with the layer
@@ -20,9 +22,11 @@ Public API (mirrors of the reference ``heimdall`` package):
   sp.student_sp                      one layer prefill of a sequence split over GPUs (sequence parallelism)
   plugin.prepare / install           the kernels.prepare plug-in convention (heimdall/kernels.py:158-188)
 """
-from .functional import delta_rule, delta_rule_gqa, delta_rule_step, delta_rule_step_gqa, window_attention  # noqa: F401
+from .functional import delta_rule, delta_rule_gqa, delta_rule_step, delta_rule_step_gqa  # noqa: F401
+from .functional import prompt_attention, window_attention  # noqa: F401
 from .layer import BifrostLayer  # noqa: F401
+from .paged import PagedKV  # noqa: F401
 from .attention import BifrostAttention  # noqa: F401
 
 __all__ = ["delta_rule", "delta_rule_gqa", "delta_rule_step", "delta_rule_step_gqa", "window_attention",
-           "BifrostLayer", "BifrostAttention"]
+           "prompt_attention", "BifrostLayer", "BifrostAttention", "PagedKV"]

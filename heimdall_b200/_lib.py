@@ -52,6 +52,12 @@ SIGNATURES = {
     "bf_ret_summarize": [_P, _L, _I, _I, _I, _I, _I, _I, _I, _P, _P, _L, _P],
     "bf_ret_decode_workspace": [_I, _I, _I, _I, _I, _I, _I, _I, _I],
     "bf_ret_decode": [_P, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P],
+    "bf_prompt_attn_fwd": [_P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, ctypes.c_float, _P,
+                           _P, _P],
+    "bf_paged_append": [_P, _I, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _I, _I, _P],
+    "bf_paged_attend_workspace": [_I, _I, _I, _I, _I],
+    "bf_paged_attend": [_P, _I, _P, _L, _L, _L, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P, _P, _Z, _P],
+    "bf_paged_pages": [_P, _P, _I, _P, _I, _P, _I, _P, _I, _P],
     "bf_llama_state_floats": [_I, _I, _I, _I],
     "bf_llama_state_pack": [_P, _P, _I, _I, _I, _I, _I, _P, _L, _P],
     "bf_llama_state_unpack": [_P, _L, _P, _I, _I, _I, _I, _I, _P, _P],
@@ -60,7 +66,7 @@ _RESTYPE = {"bf_strerror": ctypes.c_char_p, "bf_last_cuda_error": ctypes.c_char_
             "bf_gdn_chunk_workspace": _Z, "bf_window_workspace": _Z, "bf_layer_prefill_workspace": _Z,
             "bf_layer_prefill_sp_workspace": _Z,
             "bf_gdn_segment_workspace": _Z, "bf_llama_state_floats": _Z,
-            "bf_ret_decode_workspace": _Z, "bf_gdn_bwd_workspace": _Z}
+            "bf_ret_decode_workspace": _Z, "bf_paged_attend_workspace": _Z, "bf_gdn_bwd_workspace": _Z}
 
 _lock = threading.Lock()
 _lib = None

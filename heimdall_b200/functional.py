@@ -212,6 +212,89 @@ def window_attention(qr, ext_k, ext_v, qpos0: int, kpos0: int, klo: int, window:
     return o, lse
 
 
+def refuse_grad(name: str, *ts) -> None:
+    """The serving operators have no backward: a call that autograd would have to follow is refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise NotImplementedError(f"heimdall_b200 {name} has no backward: call it under torch.no_grad()")
+
+
+def same_device(*ts) -> torch.device:
+    dev = next(t.device for t in ts if t is not None)
+    if any(t is not None and t.device != dev for t in ts):
+        raise ValueError("all tensors must be on one device")
+    return dev
+
+
+def heads_16bit(name: str, t) -> torch.Tensor:
+    """t [..., D] with its last dimension contiguous and every row on a 16-byte boundary (copied when it is not)."""
+    if t.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"{name} is {t.dtype}: built for bfloat16 and float16")
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def strides(t) -> tuple:
+    """Element strides of all but the last dimension (0 for a dimension of one, whose stride means nothing)."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape))
+
+
+def kernel_dtype(t) -> int:
+    return 1 if t.dtype == torch.bfloat16 else 2
+
+
+def score_scale(scale, D: int) -> float:
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError("scale must be positive and finite")
+    return scale
+
+
+def int32_on(dev, name: str, t) -> torch.Tensor:
+    """An index tensor as contiguous int32 on ``dev`` (values above 31 bits are the caller's error)."""
+    if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be a one-dimensional int32 or int64 tensor")
+    return t.to(device=dev, dtype=torch.int32).contiguous()
+
+
+def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, with_lse: bool = False):
+    """Causal attention of packed prompts: the full attention of a kept layer (``HybridAttention._teacher``,
+    hibrit.py:275-290) for sequences of different lengths in one call.
+
+    q [T,H,D]; k, v [Tk,G,D] (bf16 or fp16, any strides; H a multiple of G); cu_seqlens [n+1] cumulative query counts
+    and cu_seqlens_k [n+1] cumulative key counts (None: the same), int tensors with entries that do not descend
+    (an entry below the one before it counts as equal to it, one beyond T as T).  Query i of a sequence with nq
+    queries and nk keys sees its keys j <= i + nk - nq: the queries are the sequence's last tokens.
+    Returns o [T,H,D] in q's dtype and lse [H,T] fp32 (None unless ``with_lse``); a query that sees no key and the
+    rows behind the last sequence have o = 0 and lse = -inf.  ``scale`` (default D^-1/2) must be positive.
+    """
+    check_cuda(q, k, v)
+    refuse_grad("prompt_attention", q, k, v)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[-1] != q.shape[-1]:
+        raise ValueError("prompt_attention takes q [T,H,D] and k, v [Tk,G,D]")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError("q, k and v must have one dtype")
+    (T, H, D), (Tk, G, _) = q.shape, k.shape
+    if D != 256:
+        raise NotImplementedError("prompt_attention is built for head dim 256")
+    if H % G:
+        raise ValueError("the query heads must be a multiple of the KV heads")
+    if cu_seqlens_k is None and Tk != T:
+        raise ValueError("keys and queries differ in number: cu_seqlens_k is needed")
+    dev = same_device(q, k, v)
+    scale = score_scale(scale, D)
+    with torch.cuda.device(dev):
+        cu = int32_on(dev, "cu_seqlens", cu_seqlens)
+        cuk = None if cu_seqlens_k is None else int32_on(dev, "cu_seqlens_k", cu_seqlens_k)
+        if cu.numel() < 1 or (cuk is not None and cuk.numel() != cu.numel()):
+            raise ValueError("cu_seqlens and cu_seqlens_k need one entry more than there are sequences")
+        q, k, v = heads_16bit("q", q), heads_16bit("k", k), heads_16bit("v", v)
+        o = torch.empty(T, H, D, device=dev, dtype=q.dtype)
+        lse = torch.empty(H, T, device=dev, dtype=torch.float32) if with_lse else None
+        _lib.call("bf_prompt_attn_fwd", ptr(q), *strides(q), ptr(k), *strides(k), ptr(v), *strides(v), ptr(cu), ptr(cuk),
+                  cu.numel() - 1, T, Tk, H, G, D, kernel_dtype(q), scale, ptr(o), ptr(lse), stream_handle())
+    return o, lse
+
+
 def segment_transform(k, v, g, beta, s0=None):
     """State map of one segment of the write stream, for sequence parallelism of the delta rule.
 

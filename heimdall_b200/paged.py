@@ -1,0 +1,384 @@
+"""An 8-bit cache in pages for the kept (not converted) full-attention layers.
+
+The reference's server keeps the full-attention layers' keys and values in 8 bits and copies and removes sequences of
+its cache (llamacpp/README.md:77-78).  Here a pool of pages of ``page`` tokens holds e4m3 codes with one power-of-two
+scale per (layer, page, KV head), for keys and for values; the host gives out pages (lowest index first, with reference
+counts) and the device holds the page table and the lengths, so that ``append`` and ``attend`` read nothing from the
+host and can be captured into a CUDA graph:
+
+    c = PagedKV(layers=4, pages=4096, heads=4, slots=64, max_len=131072)
+    c.reserve(slots, 1)                       # host: room for the next token of each sequence, once per step
+    for layer in range(4):
+        c.append(layer, k, v, slot_ids)       # device
+        o, _ = c.attend(layer, q, slot_ids)   # device
+
+``fork`` shares pages between sequences, ``free`` and ``truncate`` give them back, ``compact`` closes the pool up.
+Calls on one cache belong on one stream, or on streams that the caller orders.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import numpy as np
+import torch
+
+from . import _lib
+from .functional import (check_cuda, heads_16bit, int32_on, kernel_dtype, prompt_attention, ptr, refuse_grad, same_device,
+                         score_scale, stream_handle, strides)
+from .structs import BfPagePool
+
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+class PageTable:
+    """The host's side of the cache: which slot holds which pages.  Every method returns what the device has to do, as
+    the int32 lists of ``bf_paged_pages``; a call that raises has changed nothing.
+
+    Only the last page of a sequence can be partly filled, and a partly filled page belongs to one sequence."""
+
+    def __init__(self, pages: int, slots: int, page: int, width: int):
+        self.pages, self.slots, self.page, self.width = pages, slots, page, width
+        self.refs = np.zeros(pages, np.int32)
+        self.table = np.full((slots, width), -1, np.int32)
+        self.lens = np.zeros(slots, np.int64)
+        self.n_free = pages
+        self._low = 0                        # no free page below this one
+
+    def _slots(self, slots, distinct=True) -> np.ndarray:
+        s = np.atleast_1d(np.asarray(slots))
+        if s.size == 0:
+            return np.zeros(0, np.int64)
+        if s.ndim != 1 or not np.issubdtype(s.dtype, np.integer):
+            raise ValueError("slots must be a list of whole numbers")
+        if s.min() < 0 or s.max() >= self.slots:
+            raise ValueError(f"a slot is outside [0, {self.slots})")
+        if distinct and np.unique(s).size != s.size:
+            raise ValueError("a slot is named twice")
+        return s.astype(np.int64)
+
+    def _counts(self, n, like) -> np.ndarray:
+        n = np.asarray(n)
+        if not np.issubdtype(n.dtype, np.integer) or (n.ndim and n.shape != like.shape):
+            raise ValueError("one whole number, or one for each slot, is needed")
+        n = np.broadcast_to(n, like.shape).astype(np.int64)
+        if n.size and n.min() < 0:
+            raise ValueError("a number of tokens is negative")
+        return n
+
+    def _held(self, lens):
+        return -(-lens // self.page)
+
+    def _take(self, n: int) -> np.ndarray:
+        """The n lowest free pages (the caller has checked that there are so many)."""
+        out, at, step = [], self._low, max(1024, 2 * n)
+        left = n
+        while left > 0:
+            got = np.flatnonzero(self.refs[at:at + step] == 0)[:left] + at
+            out.append(got)
+            left -= got.size
+            at += step
+        pages = np.concatenate(out) if out else np.zeros(0, np.int64)
+        if n:
+            self.refs[pages] = 1
+            self.n_free -= n
+            self._low = int(pages[-1]) + 1
+        return pages
+
+    def _drop(self, pages: np.ndarray) -> None:
+        np.subtract.at(self.refs, pages, 1)
+        gone = np.unique(pages[self.refs[pages] == 0])
+        self.n_free += gone.size
+        if gone.size:
+            self._low = min(self._low, int(gone[0]))
+
+    def _need(self, n: int, free: int) -> None:
+        if n > free:
+            raise RuntimeError(f"heimdall_b200: the page pool is full ({n} pages needed, {free} of {self.pages} free)")
+
+    def reserve(self, slots, n) -> dict:
+        s = self._slots(slots)
+        n = self._counts(n, s)
+        old = self.lens[s]
+        new = old + n
+        if s.size and new.max() > self.width * self.page:
+            raise ValueError(f"a sequence would be longer than the cache's max_len ({self.width * self.page})")
+        have = self._held(old)
+        more = self._held(new) - have
+        total = int(more.sum())
+        self._need(total, self.n_free)
+        pages = self._take(total)
+        row = np.repeat(s, more)
+        col = np.arange(total) - np.repeat(np.cumsum(more) - more, more) + np.repeat(have, more)
+        self.table[row, col] = pages
+        self.lens[s] = new
+        at = np.concatenate([row * self.width + col, self.slots * self.width + s])
+        return {"set": np.stack([at, np.concatenate([pages, new])], 1)}
+
+    def free(self, slots) -> dict:
+        s = self._slots(slots)
+        rows = self.table[s]
+        self._drop(rows[rows >= 0])
+        self.table[s] = -1
+        self.lens[s] = 0
+        return {"release": s}
+
+    def fork(self, src, dst) -> dict:
+        a, b = self._slots(src, distinct=False), self._slots(dst)
+        if a.size != b.size:
+            raise ValueError("fork needs as many slots to fill as slots to take from")
+        if np.intersect1d(a, b).size:
+            raise ValueError("a slot is both taken from and filled")
+        if (self.lens[b] > 0).any():
+            raise ValueError("a slot to fill holds a sequence: free it first")
+        lens = self.lens[a]
+        part = lens % self.page > 0
+        self._need(int(part.sum()), self.n_free)
+        last = np.maximum(self._held(lens) - 1, 0)
+        old = np.where(part, self.table[a, last], -1)
+        new = np.full(a.size, -1, np.int64)
+        new[part] = self._take(int(part.sum()))
+        rows = self.table[a]
+        rows[part, last[part]] = new[part]
+        shared = rows.copy()
+        shared[part, last[part]] = -1
+        np.add.at(self.refs, shared[shared >= 0], 1)
+        self.table[b] = rows
+        self.lens[b] = lens
+        return {"fork": np.stack([a, b, lens, old, new], 1)}
+
+    def truncate(self, slots, lens) -> dict:
+        s = self._slots(slots)
+        new = self._counts(lens, s)
+        if (new > self.lens[s]).any():
+            raise ValueError("truncate cannot lengthen a sequence")
+        keep = self._held(new)
+        rows = self.table[s]
+        col = np.arange(self.width)[None]
+        tail = (col >= keep[:, None]) & (rows >= 0)
+        last = np.maximum(keep - 1, 0)
+        end = rows[np.arange(s.size), last] if s.size else np.zeros(0, np.int32)
+        part = (new % self.page > 0)
+        # references left once the tails are given back: a partly filled page that others still hold is copied, slot by
+        # slot (the last holder keeps it)
+        refs = self.refs.copy()
+        np.subtract.at(refs, rows[tail], 1)
+        copied = np.zeros(s.size, bool)
+        for i in np.flatnonzero(part):
+            if refs[end[i]] > 1:
+                refs[end[i]] -= 1
+                copied[i] = True
+        n = int(copied.sum())
+        self._need(n, int((refs == 0).sum()))
+        self._drop(rows[tail])
+        pages = self._take(n)
+        self._drop(end[copied])
+        r, c = np.nonzero(tail)
+        self.table[s[r], c] = -1
+        self.table[s[copied], last[copied]] = pages
+        self.lens[s] = new
+        out = {"fork": np.stack([s[copied], s[copied], new[copied], end[copied], pages], 1)}
+        at = np.concatenate([s[r] * self.width + c, self.slots * self.width + s])
+        out["set"] = np.stack([at, np.concatenate([np.full(r.size, -1), new])], 1)
+        return out
+
+    def compact(self) -> dict:
+        n = self.pages - self.n_free
+        src = np.flatnonzero(self.refs[n:]) + n
+        dst = np.flatnonzero(self.refs[:n] == 0)
+        to = np.arange(self.pages, dtype=np.int32)
+        to[src] = dst
+        self.refs[dst] = self.refs[src]
+        self.refs[src] = 0
+        self.table = np.where(self.table >= 0, to[self.table], self.table)
+        self._low = n
+        return {"move": np.stack([src, dst], 1)}
+
+
+class PagedKV:
+    """Keys and values of ``layers`` kept layers in 8-bit pages (see the module's docstring).
+
+    ``pages`` of ``page`` tokens (16, 32, 64 or 128) for ``slots`` sequences of up to ``max_len`` tokens (default: the whole
+    pool), ``heads`` KV heads of 256.  Device tensors, for reading: ``k_pages``, ``v_pages`` [layers,pages,heads,page,256]
+    float8_e4m3fn, ``k_scale``, ``v_scale`` [layers,pages,heads] fp32 (value = code * scale), ``table`` [slots,width] int32
+    (-1: no page), ``lens`` [slots] int32."""
+
+    def __init__(self, layers: int, pages: int, heads: int, slots: int, page: int = 64, dim: int = 256, max_len=None,
+                 device="cuda"):
+        if dim != 256:
+            raise NotImplementedError("PagedKV is built for head dim 256")
+        if page not in PAGE_SIZES:
+            raise NotImplementedError(f"PagedKV has pages of {', '.join(map(str, PAGE_SIZES))} tokens")
+        if min(layers, pages, heads, slots) < 1 or (max_len is not None and max_len < 1):
+            raise ValueError("layers, pages, heads, slots and max_len must be positive")
+        max_len = pages * page if max_len is None else max_len
+        width = -(-max_len // page)
+        if slots * (width + 1) >= 2 ** 31 or pages * heads * page >= 2 ** 31 or layers * heads > 65535:
+            raise ValueError("the cache is too large for 32-bit row numbers")
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise RuntimeError("heimdall_b200 runs on CUDA tensors only (there is no CPU fallback)")
+        self.layers, self.heads, self.page, self.dim = layers, heads, page, dim
+        self.host = PageTable(pages, slots, page, width)
+        code = lambda: torch.zeros(layers, pages, heads, page, dim, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+        self.k_pages, self.v_pages = code(), code()
+        self.device = self.k_pages.device
+        self.k_scale = torch.zeros(layers, pages, heads, device=dev)
+        self.v_scale = torch.zeros(layers, pages, heads, device=dev)
+        self.table = torch.full((slots, width), -1, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(slots, dtype=torch.int32, device=dev)
+        self._pool = BfPagePool(ptr(self.k_pages), ptr(self.v_pages), ptr(self.k_scale), ptr(self.v_scale), ptr(self.table),
+                                ptr(self.lens), layers, pages, heads, page, dim, slots, width)
+        import ctypes
+        self._pool_ptr = ctypes.addressof(self._pool)
+
+    # -------------------------------------------------------------------------------------------- sequences and pages
+    @property
+    def free_pages(self) -> int:
+        return self.host.n_free
+
+    def length(self, slot: int) -> int:
+        """Tokens of a slot, as the host knows them (no device read)."""
+        return int(self.host.lens[slot])
+
+    def _apply(self, change, *args) -> None:
+        """The host's change, then the device's.  Not for a capture: a replay would not repeat the host's part."""
+        with torch.cuda.device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("heimdall_b200: pages are given out on the host: reserve, fork, free, truncate and compact "
+                                   "cannot be captured into a CUDA graph")
+            todo = change(*args)
+            lists = []
+            for name in ("release", "fork", "move", "set"):
+                x = np.ascontiguousarray(todo[name], np.int32) if name in todo else np.zeros((0, 1), np.int32)
+                lists.append(x)
+            if any(x.shape[0] for x in lists):
+                flat = [y for x in lists for y in (x.ctypes.data, x.shape[0])]
+                _lib.call("bf_paged_pages", self._pool_ptr, *flat, stream_handle())
+
+    def reserve(self, slots, n) -> None:
+        """Room for n more tokens (one number, or one per slot) of each slot; they belong to the sequences from here on.
+        Raises RuntimeError, with nothing changed, when the pool has too few free pages."""
+        self._apply(self.host.reserve, slots, n)
+
+    def free(self, slots) -> None:
+        """End the sequences of these slots: their pages return to the pool unless another sequence shares them."""
+        self._apply(self.host.free, slots)
+
+    def fork(self, src, dst) -> None:
+        """The (empty) slots dst continue the sequences of src: full pages are shared, the tokens of a partly filled last
+        page are copied, in every layer."""
+        self._apply(self.host.fork, src, dst)
+
+    def truncate(self, slots, lens) -> None:
+        """Shorten the sequences of these slots to lens tokens (rejected drafts); a shared page that becomes partly filled
+        is copied.  The scale of the page that is cut stays as it is."""
+        self._apply(self.host.truncate, slots, lens)
+
+    def compact(self) -> int:
+        """Move the live pages at or above their number into the holes below it (both in ascending order), so that the
+        pool is in use from page 0 on.  Returns the number of live pages."""
+        self._apply(self.host.compact)
+        return self.host.pages - self.host.n_free
+
+    # -------------------------------------------------------------------------------------------- keys and values
+    def _layer(self, layer: int) -> int:
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} is outside [0, {self.layers})")
+        return int(layer)
+
+    def _ids(self, slots, B: int):
+        if slots is None:
+            if B > self.host.slots:
+                raise ValueError("more sequences than the cache has slots")
+            return None
+        check_cuda(slots)
+        same_device(self.k_pages, slots)
+        slots = int32_on(self.device, "slots", slots)
+        if slots.numel() != B:
+            raise ValueError("slots needs one entry per sequence")
+        return slots
+
+    def append(self, layer: int, k, v, slots=None, cu_seqlens=None) -> None:
+        """Write the newest tokens of each sequence, already reserved: k, v [B,t,G,D], or [T,G,D] packed with cu_seqlens
+        [B+1].  Sequence b (slot slots[b], an int tensor on the device; None: slot b) gets its n_b tokens at the positions
+        lens - n_b .. lens - 1.  A page's scale covers what was written to it; earlier codes of a page whose scale grows are
+        rounded to the new one.  Infinities are stored as the largest code, NaN as NaN."""
+        check_cuda(k, v)
+        refuse_grad("PagedKV.append", k, v)
+        layer = self._layer(layer)
+        packed = cu_seqlens is not None
+        if k.shape != v.shape or k.dtype != v.dtype or k.dim() != (3 if packed else 4):
+            raise ValueError("append takes k and v alike: [B,t,G,D], or [T,G,D] with cu_seqlens")
+        if k.shape[-2] != self.heads or k.shape[-1] != self.dim:
+            raise ValueError(f"append takes {self.heads} heads of {self.dim}")
+        same_device(self.k_pages, k, v)
+        with torch.cuda.device(self.device):
+            cu = int32_on(self.device, "cu_seqlens", cu_seqlens) if packed else None
+            B = cu.numel() - 1 if packed else k.shape[0]
+            if B < 0:
+                raise ValueError("cu_seqlens needs one entry more than there are sequences")
+            ids = self._ids(slots, B)
+            k, v = heads_16bit("k", k), heads_16bit("v", v)
+            ks, vs = strides(k), strides(v)
+            if packed:
+                ks, vs = (0,) + ks, (0,) + vs
+            _lib.call("bf_paged_append", self._pool_ptr, layer, ptr(k), *ks, ptr(v), *vs, ptr(ids), ptr(cu), B, k.shape[-3],
+                      kernel_dtype(k), stream_handle())
+
+    def attend(self, layer: int, q, slots=None, scale=None, with_lse: bool = False):
+        """Attention of each sequence's last t tokens over its pages: q [B,t,H,D] (bf16 or fp16; H a multiple of the KV
+        heads) at the positions lens - t .. lens - 1, each seeing the positions up to its own.  Returns o [B,t,H,D] in q's
+        dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf."""
+        check_cuda(q)
+        refuse_grad("PagedKV.attend", q)
+        layer = self._layer(layer)
+        if q.dim() != 4 or q.shape[-1] != self.dim or q.shape[2] % self.heads or q.shape[2] < 1:
+            raise ValueError(f"attend takes q [B,t,H,{self.dim}] with H a multiple of {self.heads}")
+        B, t, H, D = q.shape
+        if H // self.heads > 24:
+            raise NotImplementedError("attend takes at most 24 query heads per KV head")
+        same_device(self.k_pages, q)
+        scale = score_scale(scale, D)
+        with torch.cuda.device(self.device):
+            ids = self._ids(slots, B)
+            q = heads_16bit("q", q)
+            o = torch.empty(B, t, H, D, device=self.device, dtype=q.dtype)
+            lse = torch.empty(B, H, t, device=self.device, dtype=torch.float32) if with_lse else None
+            nws = _lib.size("bf_paged_attend_workspace", B, t, H, self.heads, D)
+            ws = torch.empty(max(nws, 16), dtype=torch.uint8, device=self.device)
+            _lib.call("bf_paged_attend", self._pool_ptr, layer, ptr(q), *strides(q), ptr(ids), B, t, H, kernel_dtype(q), scale,
+                      ptr(o), ptr(lse), ptr(ws), ws.numel(), stream_handle())
+        return o, lse
+
+    def layer(self, layer: int) -> "PagedLayer":
+        """This cache as one kept layer's ``cache`` argument of ``retrieval.teacher`` (slots 0 .. B-1 in step)."""
+        return PagedLayer(self, self._layer(layer))
+
+
+class PagedLayer:
+    """One layer of a ``PagedKV`` as the cache of ``retrieval.teacher``: a batch of B sequences in the slots 0 .. B-1, all
+    layers of the cache called in the same order every step.  The first layer that needs room reserves it."""
+
+    def __init__(self, cache: PagedKV, layer: int):
+        self.cache, self.index, self.n = cache, layer, 0
+
+    def teacher(self, qr, kr, v, retrieval=None):
+        c, (B, H, t, D) = self.cache, qr.shape
+        n = self.n + t
+        if retrieval is not None and (t == 1 or retrieval.get("prefill")) and \
+                n - retrieval["sinks"] - retrieval["window"] >= retrieval["k"] * retrieval["block"]:
+            raise NotImplementedError("heimdall_b200 retrieval: block selection over 8-bit pages is not built")
+        if B > c.host.slots:
+            raise ValueError("more sequences than the cache has slots")
+        if (c.host.lens[:B] == self.n).all():
+            c.reserve(np.arange(B), t)
+        if not (c.host.lens[:B] == n).all():
+            raise ValueError("the layers of a paged cache must take the same tokens in step")
+        dt = kr.dtype if kr.dtype == torch.float16 else torch.bfloat16
+        q, k, v = qr.transpose(1, 2).to(dt), kr.transpose(1, 2).to(dt), v.to(dt)
+        c.append(self.index, k, v)
+        first, self.n = self.n == 0, n
+        if not first:
+            return c.attend(self.index, q)[0].to(qr.dtype)
+        # a whole prompt: attention over the keys and values as they are, not over their codes
+        cu = torch.arange(B + 1, device=qr.device, dtype=torch.int32) * t
+        o, _ = prompt_attention(q.reshape(B * t, H, D), k.reshape(B * t, -1, D), v.reshape(B * t, -1, D), cu)
+        return o.reshape(B, t, H, D).to(qr.dtype)

@@ -9,7 +9,8 @@ with retrieval on and enough history (n - sinks - window >= k * block) runs ``bf
 the summaries, top-k selection, exact attention over sinks + selected blocks + window); every other call is
 causal attention over the whole cache on the window kernel (``bf_window_attn_fwd`` with the window as long as
 the sequence).  Retrieval in prefill (``prefill=True`` with t > 1, a different selection per query) is not
-built and raises.  There is no CPU path.
+built and raises.  A ``PagedKV.layer(i)`` in the place of the cache dict keeps the keys and values in 8-bit pages:
+the prompt runs on ``prompt_attention``, later calls on ``PagedKV.attend``.  There is no CPU path.
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ import torch
 
 from . import _lib
 from .functional import check_cuda, ptr, stream_handle, window_attention
+from .paged import PagedLayer
 
 
 def _grow(cache: dict, B: int, G: int, D: int, n_new: int, dev, dtype, block: int) -> None:
@@ -44,9 +46,11 @@ def _grow(cache: dict, B: int, G: int, D: int, n_new: int, dev, dtype, block: in
 
 def teacher(qr, kr, v, cache=None, retrieval=None):
     """HybridAttention._teacher (hibrit.py:275-290): qr [B,H,t,D], kr [B,G,t,D], v [B,t,G,D] (bf16 on CUDA) ->
-    o [B,t,H,D] in qr's dtype.  ``cache`` (or None) keeps "k", "v" [B,G,n,D]; ``retrieval`` is the dict that
-    ``set_retrieval`` stores (k, block, window, sinks, prefill) or None."""
+    o [B,t,H,D] in qr's dtype.  ``cache`` (or None) keeps "k", "v" [B,G,n,D], or is a ``PagedKV.layer(i)``; ``retrieval``
+    is the dict that ``set_retrieval`` stores (k, block, window, sinks, prefill) or None."""
     check_cuda(qr, kr, v)
+    if isinstance(cache, PagedLayer):
+        return cache.teacher(qr, kr, v, retrieval)
     B, H, t, D = qr.shape
     G = kr.shape[1]
     dev, bf = qr.device, torch.bfloat16

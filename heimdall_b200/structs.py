@@ -14,3 +14,9 @@ class BfRingCache(ctypes.Structure):
     _fields_ = [("ring_k", _P), ("ring_v", _P), ("ring_km", _P), ("ring_g", _P), ("ring_beta", _P),
                 ("ring_pos", _P), ("ring_pos_bstride", ctypes.c_longlong), ("sink_k", _P), ("sink_v", _P),
                 ("ns", ctypes.c_int), ("S", _P)]
+
+
+class BfPagePool(ctypes.Structure):
+    _fields_ = [("k_pages", _P), ("v_pages", _P), ("k_scale", _P), ("v_scale", _P), ("table", _P), ("lens", _P),
+                ("layers", ctypes.c_int), ("pages", ctypes.c_int), ("heads", ctypes.c_int), ("page", ctypes.c_int),
+                ("dim", ctypes.c_int), ("slots", ctypes.c_int), ("width", ctypes.c_int)]

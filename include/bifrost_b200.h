@@ -345,6 +345,70 @@ int bf_llama_state_pack(const bf_ring_cache* cache, const int64_t* next_pos, int
 int bf_llama_state_unpack(const float* rows, long long row_stride, const int64_t* next_pos, int B, int G, int D,
                           int window, int sinks, bf_ring_cache* cache, bf_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Causal attention of packed prompts with grouped query heads (the prompt of the kept layers' full attention,
+ * HybridAttention._teacher, heimdall/hibrit.py:275-290, for sequences of different lengths in one call).
+ * Sequence b has queries cu_q[b] .. cu_q[b+1] - 1 and keys cu_k[b] .. cu_k[b+1] - 1 (cu_k NULL: cu_q); its query i
+ * of nq sees its keys j <= i + nk - nq, the rest is masked; softmax of scale * q.k in fp32.
+ *   q [T,H,D], k, v [Tk,G,D]: dtype BF_BF16 or BF_F16, element strides per token and head given (multiples of 8, a
+ *   head's D elements contiguous); cu_q, cu_k [n_seq + 1] int32 on the device, ascending: every entry is clamped
+ *   into [previous, T] (or Tk); o [T,H,D] contiguous in dtype; lse [H,T] fp32 or NULL.
+ * A query that sees no key, and every row behind the last sequence, gets o = 0 and lse = -inf.
+ * D = 256, scale > 0.
+ */
+int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void* k, long long k_st, long long k_sh,
+                       const void* v, long long v_st, long long v_sh, const int32_t* cu_q, const int32_t* cu_k,
+                       int n_seq, int T, int Tk, int H, int G, int D, int dtype, float scale, void* o, float* lse,
+                       bf_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * A cache of keys and values in 8 bits, in pages of L tokens, with one scale per (layer, page, KV head) for the keys
+ * and one for the values: value = code (e4m3) * scale, scale = 2^e.
+ *   k_pages, v_pages [layers,P,G,L,D] one byte per code, 16-byte aligned; k_scale, v_scale [layers,P,G] fp32;
+ *   table [slots,width] int32: the page of tokens [jL, (j+1)L) of a slot (an entry outside [0, P) is no page);
+ *   lens [slots] int32: tokens of each slot, those of the current call included.
+ * L is 16, 32, 64 or 128; D = 256.
+ *
+ * bf_paged_append: writes sequence b's n_b new tokens (n_b = t, or cu[b+1] - cu[b]) to the positions
+ *   lens - n_b .. lens - 1 of slot slots[b] (slots NULL: slot b) of one layer.  k, v: dtype BF_BF16 or BF_F16 with element strides per
+ *   batch, token and head (multiples of 8; with cu the batch stride is not used and t is the packed token count).
+ *   A (page, head)'s scale is the smallest power of two s >= 2^-64 with amax / s <= 448 over the finite values written
+ *   and, where the page held tokens before, at least the scale it had: the codes of those tokens are rounded again to
+ *   a grown scale.  Infinities are stored as +-448 s, NaN as NaN.  Tokens without a page are not stored; a slot named
+ *   twice is written by the first.
+ * bf_paged_attend: the last t tokens of each sequence against its pages: q [B,t,H,D] (dtype; element strides per batch,
+ *   token and head) is at positions lens - t .. lens - 1 and token i sees the positions <= its own whose page is in the
+ *   table.  o [B,t,H,D] contiguous in dtype, lse [B,H,t] fp32 or NULL; a row that sees nothing gets 0 and -inf.
+ *   Workspace: bf_paged_attend_workspace().  H / G <= 24.
+ * bf_paged_pages: page bookkeeping and copies on the device; every list is HOST memory, read before the call returns.
+ *   release [n_release]: slots whose table rows become -1 and lens 0;
+ *   fork [n_fork][5] = (from slot, to slot, tokens, from page, to page): the row and length of `from`, and, where
+ *     to page >= 0, that page in the place of the last one, with the scales and the first tokens % L rows of from page;
+ *   move [n_move][2] = (from page, to page): the whole page (codes and scales, every layer), then every table entry
+ *     equal to `from` becomes `to`; `from` ascending, no page both source and target;
+ *   set [n_set][2] = (index, value): index < slots * width is a table entry, slots * width + s is lens[s].
+ *   In this order: release, fork, move, set.
+ */
+typedef struct bf_page_pool {
+  void* k_pages;
+  void* v_pages;
+  float* k_scale;
+  float* v_scale;
+  int32_t* table;
+  int32_t* lens;
+  int layers, pages, heads, page, dim, slots, width;
+} bf_page_pool;
+
+int bf_paged_append(const bf_page_pool* pool, int layer, const void* k, long long k_sb, long long k_st, long long k_sh,
+                    const void* v, long long v_sb, long long v_st, long long v_sh, const int32_t* slots,
+                    const int32_t* cu, int B, int t, int dtype, bf_stream_t stream);
+size_t bf_paged_attend_workspace(int B, int t, int H, int G, int D);
+int bf_paged_attend(const bf_page_pool* pool, int layer, const void* q, long long q_sb, long long q_st, long long q_sh,
+                    const int32_t* slots, int B, int t, int H, int dtype, float scale, void* o, float* lse, void* ws,
+                    size_t ws_bytes, bf_stream_t stream);
+int bf_paged_pages(const bf_page_pool* pool, const int32_t* release, int n_release, const int32_t* fork, int n_fork,
+                   const int32_t* move, int n_move, const int32_t* set, int n_set, bf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
