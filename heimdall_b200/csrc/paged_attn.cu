@@ -3,71 +3,640 @@
 //   o = sum_j p_j sv_j c^v_j,  p = softmax_j(scale sk_j q . c^k_j)  over the positions j <= the token's own that have a page,
 //   with the e4m3 codes c and the scales sk, sv of each (page, KV head).
 //
-// One warp per (sequence, token, query head): lane l holds dims 8l .. 8l+7.
+// A decode step reads every code once and computes little with it, so what bounds it is HBM: 512 bytes per (token, KV
+// head).  Turning the codes into 16-bit operands in registers would cost two conversions and a shared-memory round trip
+// per byte pair; instead the codes go from HBM by TMA into shared memory and from there, untouched, into the 5th-gen
+// tensor core (kind::f8f6f4).  The other operand of each product, which is small, is split into three e4m3 parts of 4
+// significant bits each (x = (x0 + x1 / 16 + x2 / 256) / 2^k, every part scaled into the code's upper range), each part a column of its own:
+//   S^T[token, part x row] = K Q^T    M = 128 tokens, N = 3 RP, K = 256 dims   (a bf16 or fp16 query is exact in three parts)
+//   O^T[dim, part x row]   = V^T P^T  M = 2 x 128 dims, N = 3 RP, K = 128 tokens (P is off by at most 2^-12 of itself, or
+//                                     2^-26 of the tile's largest weight)
+// with a row = (token of the call, query head of the KV head's group), RP rows at a time.  P is taken relative to its own
+// tile's maximum, so that a tile of small weights keeps its bits, and the tile's O^T leaves TMEM for fp32 registers that
+// carry the running maximum: nothing is rescaled in TMEM.  V's scales go into P (as their ratio to the tile's largest).
+//
+// Work: the tiles of 128 tokens of all (sequence, token chunk, KV head) segments in one line, cut into equal runs, one per CTA
+// (one CTA per SM), whatever the lengths.  A segment inside one run is finished there; of a cut one each CTA writes its
+// partial (at most two per CTA), and paged_combine_kernel merges them in order, so results do not depend on timing.
+// Warps (384 threads): 0 TMA of the codes (a ring of 32 KB units K0 V0 K1 V1 ...); 1 MMA; 2 the next segment's Q parts; 3 the
+// tiles' scales; 4-7 softmax (thread = token); 8-11 the accumulators (thread = dims d and d + 128) and the output.
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
 #include "paged_kv.h"
+#include "tmap.h"
 
 namespace bfb {
+
+constexpr int kPA_Threads = 384;
+constexpr int kPA_Tile = 128;                        // tokens per tile
+constexpr int kPA_Unit = kPA_Tile * kPG_D;           // bytes of one K or V tile
+constexpr int kPA_MaxCtas = 160;
+constexpr int kPA_MaxRows = 24;
+constexpr int kPA_Part = kPG_D + 2;                  // floats of a row's partial: accumulator, maximum, sum
 
 struct PagedAttnArgs {
   PagePool p;
   const void* q;
   long long q_sb, q_st, q_sh;
   const int32_t* slots;
-  int B, t, H;
-  float c2;
+  int B, t, H, R;
+  int tc, nqc;          // tokens per chunk, chunks
+  float c2;             // scale * log2(e)
   void* o;
   float* lse;
+  int4* desc;           // [ctas] (first CTA of the cut segment that ends here or -1, b, chunk, KV head)
+  float* part;          // [ctas][2][RP][kPA_Part]
+  unsigned int* err;
 };
 
-__device__ __forceinline__ void codes8(const uint8_t* at, float (&x)[8]) {
-  const uint2 u = *reinterpret_cast<const uint2*>(at);
+template <int RP>
+struct PagedCfg {
+  static constexpr int NP = (3 * RP + 15) / 16 * 16;       // MMA N: three parts of RP rows, padded to 16
+  static constexpr int Units = RP == 8 ? 6 : 5;            // ring units that fit beside Q and P
+  static constexpr int TmemCols = 6 * NP <= 256 ? 256 : 512;   // S[2], O[2][2 halves]
+  static constexpr int QBytes = NP * kPG_D, PBytes = NP * kPA_Tile;
+  static constexpr int Smem = Units * kPA_Unit + 2 * QBytes + 2 * PBytes + 4096 + 1024;
+};
+
+__device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
+  const int slot = a.slots ? a.slots[b] : b;
+  if (slot < 0 || slot >= a.p.slots) return 0;
+  return (int)max(0LL, min((long long)a.p.lens[slot], (long long)a.p.width * a.p.page));
+}
+// tiles of a sequence: at least one, so that a segment that sees nothing has a CTA that writes its zeros
+__device__ __forceinline__ int paged_tiles(int len) { return max(1, (len + kPA_Tile - 1) / kPA_Tile); }
+
+// a CTA's walk over its run of tiles
+struct PagedWalk {
+  int b, c, g, tile, ntiles, len;
+  __device__ __forceinline__ void next(const PagedAttnArgs& a) {
+    if (++tile < ntiles) return;
+    tile = 0;
+    if (++g < a.p.heads) return;
+    g = 0;
+    if (++c < a.nqc) return;
+    c = 0;
+    if (++b < a.B) {
+      len = paged_len(a, b);
+      ntiles = paged_tiles(len);
+    }
+  }
+};
+
+// x = (x0 + x1 / 16 + x2 / 256) with e4m3 parts, for |x| <= 256; two values at a time
+__device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 of_e4m3x2(uint16_t c) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
+  return __half22float2(*reinterpret_cast<__half2*>(&h));
+}
+__device__ __forceinline__ void split3(float a, float b, uint16_t (&part)[3]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = i < 2 ? u.x : u.y;
-    uint32_t h;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (16 * (i & 1)))));
-    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&h));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+  for (int i = 0; i < 3; ++i) {
+    part[i] = to_e4m3x2(a, b);
+    const float2 f = of_e4m3x2(part[i]);
+    a = (a - f.x) * 16.f;
+    b = (b - f.y) * 16.f;
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(128) paged_attn_kernel(PagedAttnArgs a) {
-  const int b = blockIdx.x / a.t, i = blockIdx.x % a.t, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (h >= a.H) return;
-  const int slot = a.slots ? a.slots[b] : b, g = h / (a.H / a.p.heads);
-  const int len = slot >= 0 && slot < a.p.slots ? (int)min((long long)a.p.lens[slot], (long long)a.p.width * a.p.page) : 0;
-  const int n = len - a.t + 1 + i;
-  float q[8], acc[8] = {}, m = -INFINITY, l = 0.f;
-  const T* qp = static_cast<const T*>(a.q) + b * a.q_sb + i * a.q_st + h * a.q_sh + 8 * lane;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = (float)qp[e];
-  for (int j = 0; j < n; ++j) {
-    const int page = a.p.table[(size_t)slot * a.p.width + j / a.p.page];
-    if (page < 0 || page >= a.p.pages) continue;
-    const size_t pg = (size_t)page * a.p.heads + g, at = (pg * a.p.page + j % a.p.page) * kPG_D + 8 * lane;
-    float x[8], s = 0.f;
-    codes8(a.p.k + at, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(q[e], x[e], s);
-    s = warp_sum(s) * (a.c2 * a.p.ks[pg]);
-    const float mn = fmaxf(m, s);
-    const float w = exp2f(s - mn), al = m == -INFINITY ? 0.f : exp2f(m - mn), wv = w * a.p.vs[pg];
-    codes8(a.p.v + at, x);
-    l = l * al + w;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], al, wv * x[e]);
-    m = mn;
+template <typename T, int RP>
+__global__ void __launch_bounds__(kPA_Threads, 1)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PagedAttnArgs a) {
+  using C = PagedCfg<RP>;
+  constexpr int NP = C::NP, NU = C::Units;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem;
+  uint8_t* sQ = ring + NU * kPA_Unit;          // [2][2 atoms][NP][128]
+  uint8_t* sP = sQ + 2 * C::QBytes;            // [2][NP][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * C::PBytes);
+  uint64_t *full = bars, *empty = bars + 6, *s_full = bars + 12, *s_free = bars + 14, *p_full = bars + 16, *o_full = bars + 18,
+           *o_free = bars + 20, *q_full = bars + 22, *q_free = bars + 24, *sc_full = bars + 26, *sc_free = bars + 30, *red = bars + 34,
+           *seg_full = bars + 35, *seg_free = bars + 37;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 40);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 41);
+  long long* s_sum = reinterpret_cast<long long*>(bars + 42);       // [12] per-warp totals of the tile count
+  int* s_start = reinterpret_cast<int*>(bars + 54);                 // b, tiles into it
+  float* s_qs = reinterpret_cast<float*>(bars + 56);                // [2][RP] scale of the Q rows
+  float* s_fac = s_qs + 2 * kPA_MaxRows;                            // [2][RP][2] factors of the tile's O^T and the accumulators
+  float* s_red = s_fac + 4 * kPA_MaxRows;                           // [2][4][RP] the warps' maxima
+  float* s_seg = s_red + 8 * kPA_MaxRows;                           // [2][5][RP] a segment's sums per warp, its maximum
+  float* s_sc = s_seg + 10 * kPA_MaxRows;                           // [4][20] scales of a tile's pages: 8 K, 8 V ratios, V's largest, mask
+  static_assert(56 * 8 + (2 + 4 + 8 + 10) * kPA_MaxRows * 4 + 80 * 4 <= 4096, "barriers and exchanges");
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int i = 0; i < NU; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 1);
+      mbar_init(s_free + i, 4);
+      mbar_init(p_full + i, 4);
+      mbar_init(o_full + i, 1);
+      mbar_init(o_free + i, 4);
+      mbar_init(q_full + i, 1);
+      mbar_init(q_free + i, 5);
+      mbar_init(seg_full + i, 4);
+      mbar_init(seg_free + i, 4);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(sc_full + i, 1);
+      mbar_init(sc_free + i, 4);
+    }
+    mbar_init(red, 4);
+    *abort_flag = 0;
+    fence_barrier_init();
   }
-  T out[8];
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TmemCols);
+    tmem_relinquish();
+  }
+  // this CTA's run of tiles: the sequences' tile counts summed over the block, thread i holding per consecutive ones
+  const int per = (a.B + kPA_Threads - 1) / kPA_Threads;
+  const int segs = a.nqc * a.p.heads;
+  long long mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = tid * per + i;
+    if (b < a.B) mine += (long long)paged_tiles(paged_len(a, b)) * segs;
+  }
+  long long incl = mine;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) out[e] = (T)(l > 0.f || l != l ? acc[e] / l : 0.f);
-  *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (((size_t)b * a.t + i) * a.H + h) * kPG_D + 8 * lane) = *reinterpret_cast<uint4*>(out);
-  if (a.lse && lane == 0) a.lse[((size_t)b * a.H + h) * a.t + i] = l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) s_sum[warp] = incl;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  long long total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kPA_Threads / 32; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  // with fewer tiles than CTAs the first `total` CTAs take one each: no CTA between two parts of a segment is idle
+  const long long ctas = total < gridDim.x ? total : gridDim.x, x0 = min((long long)blockIdx.x, ctas);
+  const long long u0 = total * x0 / ctas, u1 = total * min(x0 + 1, ctas) / ctas;
+  if (u0 < u1 && before <= u0 && u0 < before + mine) {
+    long long at = before;
+    for (int b = tid * per;; ++b) {
+      const long long n = (long long)paged_tiles(paged_len(a, b)) * segs;
+      if (u0 < at + n) {
+        s_start[0] = b;
+        s_start[1] = (int)((u0 - at) / paged_tiles(paged_len(a, b)));
+        s_start[2] = (int)((u0 - at) % paged_tiles(paged_len(a, b)));
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem = *tmem_slot;
+  const int count = (int)(u1 - u0);
+  PagedWalk w{};
+  if (count > 0) {
+    w.b = s_start[0];
+    w.c = s_start[1] / a.p.heads;
+    w.g = s_start[1] % a.p.heads;
+    w.tile = s_start[2];
+    w.len = paged_len(a, w.b);
+    w.ntiles = paged_tiles(w.len);
+  }
+  const int L = a.p.page, ppt = kPA_Tile / L;       // pages per tile
+  // the page of this tile's page number `i`, -1 where there is none
+  auto page_of = [&](const PagedWalk& x, int i) -> int {
+    const int j = x.tile * ppt + i;
+    if (i >= ppt || (long long)j * L >= x.len) return -1;
+    const int slot = a.slots ? a.slots[x.b] : x.b;
+    const int page = a.p.table[(size_t)slot * a.p.width + j];
+    return page >= 0 && page < a.p.pages ? page : -1;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ codes
+    if (lane == 0) {
+      tma_prefetch(&kmap);
+      tma_prefetch(&vmap);
+    }
+    int unit = 0;
+    bool ok = true;
+    int page = count > 0 ? page_of(w, lane) : -1;
+    for (int j = 0; j < count && ok; ++j) {
+      const int g = w.g, now = page;
+      if (j + 1 < count) {       // the next tile's page numbers, on their way during this one's loads
+        w.next(a);
+        page = page_of(w, lane);
+      }
+      const unsigned have = __ballot_sync(0xffffffffu, now >= 0);
+      for (int kv = 0; kv < 2 && ok; ++kv, ++unit) {
+        const int u = unit % NU, round = unit / NU;
+        if (round > 0) ok = mbar_wait_warp(empty + u, (round - 1) & 1, abort_flag, a.err, 0x60);
+        if (!ok) break;
+        if (lane == 0) {
+          if (have) mbar_expect_tx(full + u, (uint32_t)__popc(have) * L * kPG_D); else mbar_arrive(full + u);
+        }
+        __syncwarp();
+        if (now >= 0) {
+          const int row = (now * a.p.heads + g) * L;
+          uint8_t* dst = ring + u * kPA_Unit + lane * L * 128;
+          tma_load_2d(dst, kv ? &vmap : &kmap, full + u, 0, row);
+          tma_load_2d(dst + kPA_Tile * 128, kv ? &vmap : &kmap, full + u, 128, row);
+        }
+      }
+    }
+    // every load issued has landed before the CTA may exit
+    for (int i = unit > NU ? unit - NU : 0; i < unit; ++i) mbar_wait(full + i % NU, (i / NU) & 1, nullptr, a.err, 0x61);
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc_e4m3(kPA_Tile, NP), id_o = idesc_e4m3(128, NP) | kIdescAMn;
+      int seg = 0;
+      bool ok = true, first = true;
+      auto pv = [&](int j) -> bool {
+        const int u = (2 * j + 1) % NU, s = j & 1;
+        if (!mbar_wait(p_full + s, (j >> 1) & 1, abort_flag, a.err, 0x62)) return false;
+        if (!mbar_wait(full + u, ((2 * j + 1) / NU) & 1, abort_flag, a.err, 0x63)) return false;
+        if (j >= 2 && !mbar_wait(o_free + s, ((j >> 1) - 1) & 1, abort_flag, a.err, 0x64)) return false;
+        tc_fence_after();
+        const uint32_t v = smem_u32(ring + u * kPA_Unit), p = smem_u32(sP + s * C::PBytes);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_f8_ss(tmem + 2 * NP + (2 * s + half) * NP, sdesc_sw128_mn(v + half * 16384 + ks * 4096, 16384),
+                       sdesc_kstep(p, NP, ks), id_o, ks > 0);
+        umma_commit(o_full + s);
+        umma_commit(empty + u);
+        return true;
+      };
+      for (int j = 0; j < count && ok; ++j) {
+        const int u = (2 * j) % NU, s = j & 1;
+        if (first && !(ok = mbar_wait(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, a.err, 0x65))) break;
+        if (!(ok = mbar_wait(full + u, ((2 * j) / NU) & 1, abort_flag, a.err, 0x66))) break;
+        if (j >= 2 && !(ok = mbar_wait(s_free + s, ((j >> 1) - 1) & 1, abort_flag, a.err, 0x67))) break;
+        tc_fence_after();
+        const uint32_t k = smem_u32(ring + u * kPA_Unit), q = smem_u32(sQ + (seg & 1) * C::QBytes);
+#pragma unroll
+        for (int ks = 0; ks < kPG_D / 32; ++ks)
+          umma_f8_ss(tmem + s * NP, sdesc_kstep(k, kPA_Tile, ks), sdesc_kstep(q, NP, ks), id_s, ks > 0);
+        umma_commit(s_full + s);
+        umma_commit(empty + u);
+        first = w.tile + 1 == w.ntiles;
+        if (first || j + 1 == count) {
+          umma_commit(q_free + (seg & 1));
+          ++seg;
+        }
+        w.next(a);
+        if (j >= 1) ok = pv(j - 1);
+      }
+      if (ok && count > 0) pv(count - 1);
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ Q parts of each segment
+    bool ok = true;
+    int seg = 0;
+    for (int j = 0; j < count && ok;) {
+      if (seg >= 2 && !(ok = mbar_wait_warp(q_free + (seg & 1), ((seg >> 1) - 1) & 1, abort_flag, a.err, 0x68))) break;
+      uint8_t* dst = sQ + (seg & 1) * C::QBytes;
+      const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
+#pragma unroll 4
+      for (int r = 0; r < RP; ++r) {
+        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows)
+          raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + w.b * a.q_sb + (long long)(i0 + r / a.R) * a.q_st +
+                                                     (long long)(w.g * a.R + r % a.R) * a.q_sh + 8 * lane));
+        const T* e = reinterpret_cast<const T*>(&raw);
+        float x[8], m = 0.f;
+        bool fin = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = (float)e[i];
+          fin = fin && fabsf(x[i]) < INFINITY;
+          m = fmaxf(m, fabsf(x[i]));
+        }
+        m = warp_max(m);
+        fin = __all_sync(0xffffffffu, fin);
+        // the row's largest value to [128, 256): x * 2^k, k = 7 - exponent
+        const int ex = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 16) : 127;
+        const float up = fin ? __uint_as_float((uint32_t)(254 + 7 - ex) << 23) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fin ? x[i] * up : 0.f;
+        uint16_t c[4][3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split3(x[2 * i], x[2 * i + 1], c[i]);
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+          const int n = part * RP + r;
+          const uint32_t chunk = ((lane & 15) >> 1) ^ (n & 7);
+          *reinterpret_cast<uint2*>(dst + (lane >> 4) * (NP * 128) + n * 128 + chunk * 16 + (lane & 1) * 8) =
+              make_uint2(c[0][part] | ((uint32_t)c[1][part] << 16), c[2][part] | ((uint32_t)c[3][part] << 16));
+        }
+        // a row with a value that is not finite has no finite scores
+        if (lane == 0) s_qs[(seg & 1) * RP + r] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + (seg & 1));
+      ++seg;
+      const int left = w.ntiles - w.tile;        // on to the next segment
+      j += left;
+      w.tile = w.ntiles - 1;
+      w.next(a);
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ scales of each tile's pages
+    bool ok = true;
+    int page = count > 0 ? page_of(w, lane) : -1;
+    for (int j = 0; j < count && ok; ++j) {
+      const int s = j & 3, now = page, g = w.g;
+      float ks = 0.f, vs = 0.f;
+      if (now >= 0) {
+        ks = a.p.ks[(size_t)now * a.p.heads + g];
+        vs = a.p.vs[(size_t)now * a.p.heads + g];
+      }
+      if (j + 1 < count) {
+        w.next(a);
+        page = page_of(w, lane);
+      }
+      const float top = warp_max(vs);
+      const unsigned have = __ballot_sync(0xffffffffu, now >= 0);
+      if (j >= 4 && !(ok = mbar_wait_warp(sc_free + s, ((j >> 2) - 1) & 1, abort_flag, a.err, 0x69))) break;
+      if (lane < 8) {
+        s_sc[s * 20 + lane] = ks;
+        s_sc[s * 20 + 8 + lane] = top > 0.f ? vs / top : 0.f;      // powers of two: exact
+      }
+      if (lane == 0) {
+        s_sc[s * 20 + 16] = top;
+        s_sc[s * 20 + 17] = __uint_as_float(have);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sc_full + s);
+    }
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ softmax: thread = token of the tile
+    const int wq = warp & 3, tok = wq * 32 + lane;
+    const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16);
+    float m_run[RP], l[RP], qs[RP];
+    int lim[RP];
+    bool ok = true, first = true;
+    int seg = 0, rows = 0;
+    for (int j = 0; j < count; ++j) {
+      const int s = j & 1;
+      if (first) {
+        if (!(ok = mbar_wait_warp(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, a.err, 0x6a))) break;
+        const int i0 = w.c * a.tc;
+        rows = min(a.tc, a.t - i0) * a.R;
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          m_run[r] = -INFINITY;
+          l[r] = 0.f;
+          qs[r] = s_qs[(seg & 1) * RP + r];
+          lim[r] = r < rows ? w.len - a.t + i0 + r / a.R : -1;     // the row's last visible position
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_free + (seg & 1));
+      }
+      const bool last = w.tile + 1 == w.ntiles, end = last || j + 1 == count;
+      if (!(ok = mbar_wait_warp(sc_full + (j & 3), (j >> 2) & 1, abort_flag, a.err, 0x6b))) break;
+      const float* sc = s_sc + (j & 3) * 20;
+      const int pi = tok / L;
+      const float ks = sc[pi], vr = sc[8 + pi], top = sc[16];
+      const bool there = (__float_as_uint(sc[17]) >> pi) & 1u;
+      const int pos = w.tile * kPA_Tile + tok;
+      const bool valid = there && pos < w.len;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sc_free + (j & 3));
+      if (!(ok = mbar_wait_warp(s_full + s, (j >> 1) & 1, abort_flag, a.err, 0x6c))) break;
+      tc_fence_after();
+      uint32_t raw[3 * RP];
+#pragma unroll
+      for (int c = 0; c < 3 * RP; c += 8) tmem_ld8(trow + s * NP + c, raw + c);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free + s);
+      float x[RP];
+      float* rd = s_red + s * 4 * RP;
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        const float d = __uint_as_float(raw[r]) + (__uint_as_float(raw[RP + r]) + __uint_as_float(raw[2 * RP + r]) * 0.0625f) * 0.0625f;
+        x[r] = valid && pos <= lim[r] ? d * (ks * qs[r]) : -INFINITY;
+        float mx;
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(mx) : "f"(x[r]));
+        if (lane == 0) rd[wq * RP + r] = mx;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(red);
+      if (!(ok = mbar_wait_warp(red, j & 1, abort_flag, a.err, 0x6d))) break;
+      // P of the tile before the last but one has been read, and so have its factors
+      if (j >= 2 && !(ok = mbar_wait_warp(o_free + s, ((j >> 1) - 1) & 1, abort_flag, a.err, 0x6e))) break;
+      uint8_t* pd = sP + s * C::PBytes;
+#pragma unroll
+      for (int r = 0; r < RP; r += 2) {
+        float y[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float mt = fmaxf(fmaxf(rd[r + e], rd[RP + r + e]), fmaxf(rd[2 * RP + r + e], rd[3 * RP + r + e]));
+          const float mn = fmaxf(m_run[r + e], mt);
+          const float al = m_run[r + e] == -INFINITY ? 0.f : ex2_approx(m_run[r + e] - mn);
+          const float f = mt == -INFINITY ? 0.f : ex2_approx(mt - mn);
+          // masked scores are -inf and give 0; a NaN stays one, whatever the others are
+          const float p = x[r + e] == -INFINITY ? 0.f : ex2_approx(x[r + e] - (mt == -INFINITY ? 0.f : mt));
+          l[r + e] = l[r + e] * al + (p != p ? p : p * f);
+          m_run[r + e] = mn;
+          y[e] = p * (vr * 256.f);
+          if (tok == 0) {
+            s_fac[(s * RP + r + e) * 2] = al;
+            s_fac[(s * RP + r + e) * 2 + 1] = f * top * (1.f / 256.f);
+          }
+        }
+        uint16_t c[3];
+        split3(y[0], y[1], c);
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int n = part * RP + r + e;
+            pd[n * 128 + (((tok >> 4) ^ (n & 7)) << 4) + (tok & 15)] = (uint8_t)(c[part] >> (8 * e));
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, !valid)) {
+        // the values of tokens that are not there may be anything (a weight of 0 times NaN would be NaN): zeros
+        const int u = (2 * j + 1) % NU;
+        if (!(ok = mbar_wait_warp(full + u, ((2 * j + 1) / NU) & 1, abort_flag, a.err, 0x6f))) break;
+        if (!valid) {
+          uint4* row = reinterpret_cast<uint4*>(ring + u * kPA_Unit + tok * 128);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) row[i] = row[kPA_Tile * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + s);
+      if (end) {
+        if (seg >= 2 && !(ok = mbar_wait_warp(seg_free + (seg & 1), ((seg >> 1) - 1) & 1, abort_flag, a.err, 0x70))) break;
+        float* sg = s_seg + (seg & 1) * 5 * RP;
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          const float sum = warp_sum(l[r]);
+          if (lane == 0) sg[wq * RP + r] = sum;
+          if (tok == 0) sg[4 * RP + r] = m_run[r];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(seg_full + (seg & 1));
+        ++seg;
+      }
+      first = last;
+      w.next(a);
+    }
+  } else {
+    // ------------------------------------------------------------------ accumulators: thread = dims d and d + 128
+    const int wq = warp & 3, d = wq * 32 + lane;
+    const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + 2 * NP;
+    float acc[2][RP];
+    bool ok = true, from_start = w.tile == 0;
+    int seg = 0;
+    int4 desc = make_int4(-1, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < RP; ++r) acc[0][r] = acc[1][r] = 0.f;
+    for (int j = 0; j < count; ++j) {
+      const int s = j & 1;
+      if (!(ok = mbar_wait_warp(p_full + s, (j >> 1) & 1, abort_flag, a.err, 0x73))) break;   // the factors
+      if (!(ok = mbar_wait_warp(o_full + s, (j >> 1) & 1, abort_flag, a.err, 0x71))) break;
+      tc_fence_after();
+      float fac[RP][2];
+#pragma unroll
+      for (int r = 0; r < RP; ++r) {
+        fac[r][0] = s_fac[(s * RP + r) * 2];
+        fac[r][1] = s_fac[(s * RP + r) * 2 + 1];
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t raw[3 * RP];
+#pragma unroll
+        for (int c = 0; c < 3 * RP; c += 8) tmem_ld8(trow + (2 * s + half) * NP + c, raw + c);
+        tmem_wait_ld();
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          const float x = __uint_as_float(raw[r]) + (__uint_as_float(raw[RP + r]) + __uint_as_float(raw[2 * RP + r]) * 0.0625f) * 0.0625f;
+          acc[half][r] = acc[half][r] * fac[r][0] + x * fac[r][1];
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free + s);
+      const bool last = w.tile + 1 == w.ntiles;
+      if (last || j + 1 == count) {
+        if (!(ok = mbar_wait_warp(seg_full + (seg & 1), (seg >> 1) & 1, abort_flag, a.err, 0x72))) break;
+        const float* sg = s_seg + (seg & 1) * 5 * RP;
+        const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
+        const bool whole = from_start && last;
+        float* part = a.part + ((size_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * RP * kPA_Part;
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          if (r < rows) {
+            const float sum = (sg[r] + sg[RP + r]) + (sg[2 * RP + r] + sg[3 * RP + r]), m = sg[4 * RP + r];
+            if (whole) {
+              const int i = i0 + r / a.R, h = w.g * a.R + r % a.R;
+              const float inv = sum == 0.f ? 0.f : 1.f / sum;       // nothing seen: zeros
+              T* o = static_cast<T*>(a.o) + (((size_t)w.b * a.t + i) * a.H + h) * kPG_D;
+              o[d] = (T)(acc[0][r] * inv);
+              o[d + 128] = (T)(acc[1][r] * inv);
+              if (a.lse && d == 0) a.lse[((size_t)w.b * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+            } else {
+              part[r * kPA_Part + d] = acc[0][r];
+              part[r * kPA_Part + d + 128] = acc[1][r];
+              if (d == 0) {
+                part[r * kPA_Part + kPG_D] = m;
+                part[r * kPA_Part + kPG_D + 1] = sum;
+              }
+            }
+          }
+          acc[0][r] = acc[1][r] = 0.f;
+        }
+        // a cut segment that ends here: the CTA that holds its first tile
+        if (last && !from_start) {
+          const long long t0 = u0 + j - (w.ntiles - 1);
+          desc = make_int4((int)(((t0 + 1) * ctas - 1) / total), w.b, w.c, w.g);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(seg_free + (seg & 1));
+        ++seg;
+        from_start = true;
+      }
+      w.next(a);
+    }
+    if (d == 0) a.desc[blockIdx.x] = ok ? desc : make_int4(-1, 0, 0, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TmemCols);
+  }
+}
+
+// Block (x, r): row r of the cut segment that ends in CTA x, if there is one: the partials of the CTAs first .. x, in order
+template <typename T, int RP>
+__global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttnArgs a) {
+  const int x = blockIdx.x, r = blockIdx.y, d = threadIdx.x;
+  const int4 desc = a.desc[x];
+  if (desc.x < 0) return;
+  const int i0 = desc.z * a.tc;
+  if (r >= min(a.tc, a.t - i0) * a.R) return;
+  auto part = [&](int c) { return a.part + (((size_t)c * 2 + (c == desc.x ? 1 : 0)) * RP + r) * kPA_Part; };
+  float m = -INFINITY, sum = 0.f, acc = 0.f;
+  for (int c0 = desc.x; c0 <= x; c0 += 8) {
+    float mv[8], lv[8], av[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float* p = part(min(c0 + i, x));
+      const bool in = c0 + i <= x;
+      av[i] = in ? p[d] : 0.f;
+      mv[i] = in ? p[kPG_D] : -INFINITY;
+      lv[i] = in ? p[kPG_D + 1] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float mn = fmaxf(m, mv[i]);
+      const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = mv[i] == -INFINITY ? 1.f : ex2_approx(mv[i] - mn);
+      acc = acc * al + av[i] * f;       // a partial without a maximum holds zeros, or NaN to be passed on
+      sum = sum * al + lv[i] * f;
+      m = mn;
+    }
+  }
+  const int i = i0 + r / a.R, h = desc.w * a.R + r % a.R;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  static_cast<T*>(a.o)[(((size_t)desc.y * a.t + i) * a.H + h) * kPG_D + d] = (T)(acc * inv);
+  if (a.lse && d == 0) a.lse[((size_t)desc.y * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+}
+
+// rows at a time for t tokens of R query heads: as many whole tokens as 24 rows hold, in equal chunks
+static void paged_chunks(int t, int R, int* tc, int* nqc, int* rp) {
+  const int most = t < kPA_MaxRows / R ? t : kPA_MaxRows / R;
+  *nqc = (t + most - 1) / most;
+  *tc = (t + *nqc - 1) / *nqc;
+  *rp = (*tc * R + 7) / 8 * 8;
+}
+
+template <typename T, int RP>
+static int launch_paged(const CUtensorMap& kmap, const CUtensorMap& vmap, const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
+  int rc = ensure_smem_attr((const void*)paged_attn_kernel<T, RP>, PagedCfg<RP>::Smem);
+  if (rc) return rc;
+  paged_attn_kernel<T, RP><<<ctas, kPA_Threads, PagedCfg<RP>::Smem, stream>>>(kmap, vmap, a);
+  if ((rc = launch_status())) return rc;
+  paged_combine_kernel<T, RP><<<dim3(ctas, a.tc * a.R), 256, 0, stream>>>(a);
+  return launch_status();
 }
 
 }  // namespace bfb
@@ -77,7 +646,10 @@ using namespace bfb;
 extern "C" {
 
 size_t bf_paged_attend_workspace(int B, int t, int H, int G, int D) {
-  return B > 0 && t > 0 && H > 0 && G > 0 && D == kPG_D ? 16 : 0;
+  if (B <= 0 || t <= 0 || H <= 0 || G <= 0 || H % G || H / G > kPA_MaxRows || D != kPG_D) return 0;
+  int tc, nqc, rp;
+  paged_chunks(t, H / G, &tc, &nqc, &rp);
+  return (size_t)kPA_MaxCtas * (sizeof(int4) + (size_t)2 * rp * kPA_Part * 4);
 }
 
 int bf_paged_attend(const bf_page_pool* pool, int layer, const void* q, long long q_sb, long long q_st, long long q_sh,
@@ -88,26 +660,40 @@ int bf_paged_attend(const bf_page_pool* pool, int layer, const void* q, long lon
   if (rc) return rc;
   if (B < 0 || t < 0 || H <= 0 || H % a.p.heads || (!slots && B > a.p.slots) || !(scale > 0.f) || scale > 3e38f)
     return BF_ERR_INVALID_ARGUMENT;
-  if ((dtype != BF_BF16 && dtype != BF_F16) || H / a.p.heads > 24) return BF_ERR_UNSUPPORTED;
+  if ((dtype != BF_BF16 && dtype != BF_F16) || H / a.p.heads > kPA_MaxRows) return BF_ERR_UNSUPPORTED;
   if (B == 0 || t == 0) return BF_OK;
   if (!q || !o) return BF_ERR_INVALID_ARGUMENT;
   if (!aligned16(q) || !aligned16(o) || ((q_sb | q_st | q_sh) & 7)) return BF_ERR_ALIGNMENT;
-  if (ws_bytes < bf_paged_attend_workspace(B, t, H, a.p.heads, kPG_D) || !ws) return BF_ERR_WORKSPACE;
+  if (!ws || ws_bytes < bf_paged_attend_workspace(B, t, H, a.p.heads, kPG_D)) return BF_ERR_WORKSPACE;
+  if (!aligned16(ws)) return BF_ERR_ALIGNMENT;
   DeviceState st;
   if ((rc = device_state(&st))) return rc;
   a.q = q;
   a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
   a.slots = slots;
-  a.B = B; a.t = t; a.H = H;
+  a.B = B; a.t = t; a.H = H; a.R = H / a.p.heads;
+  int rp;
+  paged_chunks(t, a.R, &a.tc, &a.nqc, &rp);
   a.c2 = scale * kLog2e;
   a.o = o;
   a.lse = lse;
-  const dim3 grid(B * t, (H + 3) / 4);
-  if (dtype == BF_BF16)
-    paged_attn_kernel<__nv_bfloat16><<<grid, 128, 0, stream>>>(a);
-  else
-    paged_attn_kernel<__half><<<grid, 128, 0, stream>>>(a);
-  return launch_status();
+  a.desc = static_cast<int4*>(ws);
+  a.part = reinterpret_cast<float*>(a.desc + kPA_MaxCtas);
+  a.err = st.err;
+  CUtensorMap kmap, vmap;
+  const uint64_t dims[2] = {(uint64_t)kPG_D, (uint64_t)a.p.pages * a.p.heads * a.p.page}, strides[1] = {(uint64_t)kPG_D};
+  const uint32_t box[2] = {128, (uint32_t)a.p.page};
+  if ((rc = make_tmap(&kmap, a.p.k, kTmapU8, 2, dims, strides, box, true))) return rc;
+  if ((rc = make_tmap(&vmap, a.p.v, kTmapU8, 2, dims, strides, box, true))) return rc;
+  const int ctas = st.sm_count < kPA_MaxCtas ? st.sm_count : kPA_MaxCtas;
+  if (dtype == BF_BF16) {
+    if (rp == 8) return launch_paged<__nv_bfloat16, 8>(kmap, vmap, a, ctas, stream);
+    if (rp == 16) return launch_paged<__nv_bfloat16, 16>(kmap, vmap, a, ctas, stream);
+    return launch_paged<__nv_bfloat16, 24>(kmap, vmap, a, ctas, stream);
+  }
+  if (rp == 8) return launch_paged<__half, 8>(kmap, vmap, a, ctas, stream);
+  if (rp == 16) return launch_paged<__half, 16>(kmap, vmap, a, ctas, stream);
+  return launch_paged<__half, 24>(kmap, vmap, a, ctas, stream);
 }
 
 }  // extern "C"

@@ -35,6 +35,7 @@ int make_tmap(CUtensorMap* map, const void* base, int dtype, int rank, const uin
     if (strides_bytes[i] & 15u) return BF_ERR_ALIGNMENT;
   CUtensorMapDataType t = dtype == BF_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                           : dtype == BF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                          : dtype == kTmapU8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   cuuint64_t d[5];
   cuuint64_t s[4];

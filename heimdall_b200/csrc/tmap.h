@@ -3,6 +3,7 @@
 #include <stdint.h>
 
 namespace bfb {
+constexpr int kTmapU8 = 16;   // element type of 8-bit codes, beside the BF_* types
 // rank-N tiled map with optional 128-byte swizzle (dims/box innermost first, strides in bytes for dims 1..N-1)
 int make_tmap(CUtensorMap* map, const void* base, int dtype, int rank, const uint64_t* dims,
               const uint64_t* strides_bytes, const uint32_t* box, bool swizzle128);

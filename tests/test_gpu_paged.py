@@ -194,8 +194,8 @@ def test_attend_longer_and_slots_in_any_order():
     _fill(c, 1)
     _poison(c)
     q = _rand(7, 1, 12, D, seed=5)
-    o = _check_attend(c, q, [4, 0, 2, 5, 4, 1, 9], layer=1)       # one slot twice, an empty one, one that is not there
-    assert torch.equal(_check_attend(c, q[:1], [4], layer=1), o[:1])
+    _check_attend(c, q, [4, 0, 2, 5, 4, 1, 9], layer=1)           # one slot twice, an empty one, one that is not there
+    _check_attend(c, q[:1], [4], layer=1)      # in another batch a sequence is cut elsewhere: the same to rounding, not to the bit
     _check_attend(c, q[:2] * 6, [4, 2], scale=0.3, layer=1)
 
 
