@@ -2,73 +2,462 @@
 //
 //   o_i = sum_j p_ij v_j,  p_i = softmax_j(scale q_i . k_j),  keys j <= i + nk - nq of the query's own sequence.
 //
-// One warp per (token, query head): lane l holds dims 8l .. 8l+7 of the query and of the output, the keys of the
-// sequence pass one by one with the running maximum and sum of the softmax in registers.
+// Bound by the tensor core: 4 D flops per visible (query, key, head) against 2 D bytes per key.  With D = 256 an output tile of
+// 128 rows takes half of TMEM, so an SM works on one tile of 128 queries; fed by one CTA alone each 128-key tile is 128 KB
+// from L2 per 1.5 us and SM, as much as L2 delivers.  So two CTAs form a pair (cta_group::2, M = 256): each holds its own 128
+// query rows and half of the keys' rows and of the values' columns, 64 KB per key tile and SM, which leaves room for two stages of each.
+// The pair's two row tiles are two query heads of one KV head on the same 128 tokens (the same keys, the same causal edge), or,
+// with an odd number of heads per KV head, two neighbouring tiles of 128 tokens of one head.
+//   S_j = Q K_j^T    M256 N128 K256 (A and B in shared memory)                        -> TMEM S buffer (tile parity)
+//   O  += P_j V_j    M256 N256 K128 (A = P_j in TMEM over S_j, B = V_j as it lies: N-major)
+//   TMEM of each CTA: S/P buffers at columns 0 and 128, O at 256..511.
+// P is rounded to the inputs' type (a step of the type, half of it at most, per weight: as large as the output's own rounding, and averaged over the keys);
+// its sum is taken before.  Scores are in the log2 domain; O is rescaled only when a row's maximum grows by more than 2^8.
+//
+// A cluster takes `per` items (head pairs, or heads) of one (token block, KV head) in turn; blocks go from the last to the first, so
+// the long ones start first, and KV head by KV head, so the clusters that run together share one head's keys in L2.
+// Warps (512 threads): 0 Q and K loads; 1 MMA (in the first CTA of the pair); 2 V loads; 4-11 softmax, two warpgroups, each for
+// 64 of a tile's 128 keys and 128 of O's columns; 12-15 the outputs, while the next item's products run.
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
+#include "tmap.h"
 
 namespace bfb {
 
-constexpr int kPA_D = 256;
+constexpr int kPR_D = 256;
+constexpr int kPR_M = 128;        // query rows per CTA
+constexpr int kPR_N = 128;        // keys per tile
+constexpr int kPR_Threads = 512;
+// register split (setmaxnreg) of the 128 per thread at launch
+constexpr uint32_t kPR_RegsCtl = 96, kPR_RegsSoftmax = 168, kPR_RegsEpi = 80;
+static_assert(128 * kPR_RegsCtl + 256 * kPR_RegsSoftmax + 128 * kPR_RegsEpi == kPR_Threads * 128, "register split");
+constexpr int kPR_SmemQ = kPR_M * kPR_D * 2;          // 64 KB
+constexpr int kPR_SmemK = kPR_N / 2 * kPR_D * 2;      // 32 KB: this CTA's half of the keys
+constexpr int kPR_SmemV = kPR_N * kPR_D / 2 * 2;      // 32 KB: this CTA's half of the columns
+constexpr int kPR_Tiles = kPR_SmemQ + 2 * kPR_SmemK + 2 * kPR_SmemV;
+constexpr int kPR_Smem = kPR_Tiles + 256 + 5120 + 1024;
+constexpr uint32_t kPR_TmO = 256;
+constexpr float kPR_Rescale = 8.0f;
 
 struct PromptArgs {
-  const void *q, *k, *v;
-  long long q_st, q_sh, k_st, k_sh, v_st, v_sh;
   const int32_t *cu_q, *cu_k;
   int n_seq, T, Tk, H, G;
-  float c2;   // scale * log2(e)
+  int qb;                 // tokens per block: 128 (two heads) or 256 (two tiles of one head)
+  int nblk, hsplit, per;  // blocks, clusters per (block, KV head), items per cluster
+  float c2;               // scale * log2(e)
   void* o;
   float* lse;
+  unsigned int* err;
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-  const T* t = reinterpret_cast<const T*>(&u);
+// the block's sequence: tokens q0 .. q0 + nq - 1, keys k0 .. k0 + nk - 1, the block's first token i0 in it
+struct PromptBlock {
+  int q0, nq, k0, nk, i0;
+};
+
+// Block number blk of the call.  The rows are cut into n_seq + 2 parts: those before the first sequence, the sequences, those
+// behind the last; the first and the last part have no keys.  Part p, from row s on, owns the block numbers s / qb + p and up,
+// at least as many as it has blocks.  Cumulative lengths are clamped into [previous, T] and [previous, Tk].  A warp
+// looks at 32 parts at a time.
+__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, int blk, int lane) {
+  PromptBlock r{0, 0, 0, 0, 0};
+  int carry_q = 0, carry_k = 0;
+  for (int c = 0; c < a.n_seq + 2; c += 32) {
+    const int p = c + lane;
+    const bool from = p >= 1 && p <= a.n_seq + 1 && a.cu_q, to = p <= a.n_seq && a.cu_q;
+    int q = from ? min(max(a.cu_q[p - 1], 0), a.T) : 0, k = from ? min(max(a.cu_k[p - 1], 0), a.Tk) : 0;
+    int qn = to ? min(max(a.cu_q[p], 0), a.T) : a.T, kn = to ? min(max(a.cu_k[p], 0), a.Tk) : 0;
+    q = max(q, carry_q);
+    k = max(k, carry_k);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (float)t[e];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, q, o), y = __shfl_up_sync(0xffffffffu, k, o);
+      if (lane >= o) {
+        q = max(q, x);
+        k = max(k, y);
+      }
+    }
+    qn = max(q, qn);
+    kn = p >= 1 && to ? max(k, kn) : k;
+    carry_q = __shfl_sync(0xffffffffu, q, 31);
+    carry_k = __shfl_sync(0xffffffffu, k, 31);
+    const int base = q / a.qb + p;
+    const unsigned ok = __ballot_sync(0xffffffffu, p < a.n_seq + 2 && base <= blk);
+    if (ok == 0u) break;
+    const int at = 31 - __clz(ok);
+    r.q0 = __shfl_sync(0xffffffffu, q, at);
+    r.nq = __shfl_sync(0xffffffffu, qn, at) - r.q0;
+    r.k0 = __shfl_sync(0xffffffffu, k, at);
+    r.nk = __shfl_sync(0xffffffffu, kn, at) - r.k0;
+    r.i0 = (blk - __shfl_sync(0xffffffffu, base, at)) * a.qb;
+    if (at < 31) break;
+  }
+  return r;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(128) prompt_attn_kernel(PromptArgs a) {
-  const int tok = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (h >= a.H) return;
-  // the sequence of this token, the cumulative lengths clamped into [previous, T] and [previous, Tk]
-  int q0 = 0, k0 = 0, k1 = 0, q1 = 0, found = 0;
-  for (int b = 0; b < a.n_seq && !found; ++b) {
-    q0 = b ? q1 : min(max(a.cu_q[0], 0), a.T);
-    k0 = b ? k1 : min(max(a.cu_k[0], 0), a.Tk);
-    q1 = min(max(a.cu_q[b + 1], q0), a.T);
-    k1 = min(max(a.cu_k[b + 1], k0), a.Tk);
-    found = tok >= q0 && tok < q1;
+__device__ __forceinline__ uint32_t pack16(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// TMEM column of the P operand for key step ks (16 keys) of an S buffer: each softmax half writes the weights of its 64
+// keys into the first 32 columns of its own 64 score columns
+__device__ __forceinline__ uint32_t prompt_pcol(int ks) { return (uint32_t)((ks >> 2) * 64 + (ks & 3) * 8); }
+
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
+    prompt_attn_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap, PromptArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                        // [4 atoms][128 rows][128 B]
+  uint8_t* sK = sQ + kPR_SmemQ;              // [2][4 atoms][64 keys][128 B]
+  uint8_t* sV = sK + 2 * kPR_SmemK;          // [2][2 atoms][128 keys][128 B]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPR_Tiles);
+  // in the first CTA, for both: one arrival and the bytes of each CTA, or one arrival per warp of both
+  uint64_t *q_full = bars, *k_full = bars + 1 /*[2]*/, *v_full = bars + 3 /*[2]*/, *p_full = bars + 5 /*[2]*/, *o_free = bars + 7;
+  // in each CTA, by commits of the first
+  uint64_t *q_free = bars + 8, *k_empty = bars + 9 /*[2]*/, *v_empty = bars + 11 /*[2]*/, *s_full = bars + 13 /*[2]*/, *o_fin = bars + 15;
+  // within a CTA
+  uint64_t *pair = bars + 16 /*[4]*/, *stats = bars + 20 /*[2]*/, *sfree = bars + 22 /*[2]*/, *v_own = bars + 24;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 26);
+  float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);   // [2 tile parities][2 halves][128] maxima
+  float* xl = xch + 512;                                                           // [2 slots][2 halves][128] row sums
+  float* xmx = xl + 512;                                                           // [2 slots][128] row maxima
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_rank();
+  int cl = blockIdx.x >> 1;
+  const int hs = cl % a.hsplit;
+  cl /= a.hsplit;
+  const int g = cl / a.nblk;
+  const PromptBlock blk = prompt_block(a, a.nblk - 1 - cl % a.nblk, lane);
+  if (blk.i0 >= blk.nq) return;              // both CTAs of the pair: a block number that no sequence uses
+  const int R = a.H / a.G, two = a.qb == kPR_M;            // two: the pair's tiles are two heads
+  const int off = blk.nk - blk.nq;                         // query i sees keys j <= i + off
+  const int i0 = blk.i0 + (two ? 0 : (int)rank * kPR_M);   // this CTA's first token
+  const int items = min(a.per, (two ? R / 2 : R) - hs * a.per);
+  const int last = min(blk.i0 + a.qb, blk.nq) - 1 + off;   // last key that the pair sees
+  const int n = last >= 0 ? last / kPR_N + 1 : 0;          // key tiles
+  auto head = [&](int it) { return g * R + (two ? 2 * (hs * a.per + it) + (int)rank : hs * a.per + it); };
+
+  if (tid == 0) {
+    mbar_init(q_full, 2);
+    mbar_init(o_free, 8);
+    mbar_init(q_free, 1);
+    mbar_init(o_fin, 1);
+    mbar_init(v_own, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + i, 2);
+      mbar_init(v_full + i, 2);
+      mbar_init(p_full + i, 16);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(stats + i, 8);
+      mbar_init(sfree + i, 4);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(pair + i, 2);
+    *abort_flag = 0;
+    fence_barrier_init();
   }
-  const int nk = found ? min(k1 - k0, tok - q0 + 1 + (k1 - k0) - (q1 - q0)) : 0;
-  float q[8], acc[8] = {};
-  load8(static_cast<const T*>(a.q) + tok * a.q_st + h * a.q_sh + 8 * lane, q);
-  const int g = h / (a.H / a.G);
-  const T* k = static_cast<const T*>(a.k) + k0 * a.k_st + g * a.k_sh + 8 * lane;
-  const T* v = static_cast<const T*>(a.v) + k0 * a.v_st + g * a.v_sh + 8 * lane;
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < nk; ++j) {
-    float x[8], s = 0.f;
-    load8(k + j * a.k_st, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(q[e], x[e], s);
-    s = warp_sum(s) * a.c2;
-    const float mn = fmaxf(m, s);
-    const float w = mn == -INFINITY && s == -INFINITY ? 0.f : exp2f(s - mn), al = m == -INFINITY ? 0.f : exp2f(m - mn);
-    load8(v + j * a.v_st, x);
-    l = l * al + w;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], al, w * x[e]);
-    m = mn;
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
   }
-  T out[8];
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPR_RegsCtl));
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------------- Q and K
+      tma_prefetch(&qmap);
+      tma_prefetch(&kmap);
+      const uint32_t qf = cluster_addr(q_full, 0), kf[2] = {cluster_addr(k_full, 0), cluster_addr(k_full + 1, 0)};
+      int t = 0;
+      bool ok = true;
+      for (int it = 0; it < items && ok; ++it) {
+        if (it >= 1 && !(ok = mbar_wait(q_free, (it - 1) & 1, abort_flag, a.err, 0x80))) break;
+        mbar_expect_tx_cluster(qf, kPR_SmemQ);
+        tma_load_4d_pair(sQ, &qmap, qf, 0, blk.q0 + i0, 0, head(it));
+        for (int j = 0; j < n; ++j, ++t) {
+          const int s = t & 1;
+          if (t >= 2 && !(ok = mbar_wait(k_empty + s, ((t >> 1) - 1) & 1, abort_flag, a.err, 0x81))) break;
+          mbar_expect_tx_cluster(kf[s], kPR_SmemK);
+          tma_load_4d_pair(sK + s * kPR_SmemK, &kmap, kf[s], 0, blk.k0 + j * kPR_N + (int)rank * (kPR_N / 2), 0, g);
+        }
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- V
+      if (lane == 0) tma_prefetch(&vmap);
+      const uint32_t vf[2] = {cluster_addr(v_full, 0), cluster_addr(v_full + 1, 0)};
+      int t = 0, own = 0;
+      bool ok = true;
+      for (int it = 0; it < items && ok; ++it) {
+        for (int j = 0; j < n; ++j, ++t) {
+          const int s = t & 1, rows = blk.nk - j * kPR_N;   // rows of the tile that are this sequence's
+          if (t >= 2 && !(ok = mbar_wait_warp(v_empty + s, ((t >> 1) - 1) & 1, abort_flag, a.err, 0x82))) break;
+          uint8_t* dst = sV + s * kPR_SmemV;
+          const bool whole = rows >= kPR_N;
+          if (lane == 0) {
+            if (whole) mbar_expect_tx_cluster(vf[s], kPR_SmemV); else mbar_expect_tx(v_own, kPR_SmemV);
+            tma_load_4d_pair(dst, &vmap, whole ? vf[s] : smem_u32(v_own), 0, blk.k0 + j * kPR_N, 2 * (int)rank, g);
+          }
+          __syncwarp();
+          if (!whole) {
+            // the rows behind the sequence belong to others: their weights are 0, but 0 times NaN would not be
+            if (!(ok = mbar_wait_warp(v_own, own & 1, abort_flag, a.err, 0x83))) break;
+            ++own;
+            for (int i = lane; i < (kPR_N - rows) * 8; i += 32) {
+              uint4* p = reinterpret_cast<uint4*>(dst + rows * 128) + i;
+              p[0] = p[kPR_N * 8] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(vf[s]);
+          }
+        }
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      // ---------------------------------------------------------------- MMA
+      constexpr int is_bf16 = sizeof(T) == 2 && !__is_same(T, __half);
+      constexpr uint32_t id_s = idesc_f16(2 * kPR_M, kPR_N, is_bf16), id_o = idesc_f16(2 * kPR_M, kPR_D, is_bf16) | kIdescBMn;
+      const uint32_t aQ = smem_u32(sQ);
+      int t = 0;
+      bool ok = true;
+      for (int it = 0; it < items && ok; ++it) {
+        if (!(ok = mbar_wait(q_full, it & 1, abort_flag, a.err, 0x84))) break;
+        auto pv = [&](int j, int tt) -> bool {
+          const int s = tt & 1;
+          if (!mbar_wait(p_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x85)) return false;
+          if (!mbar_wait(v_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x86)) return false;
+          if (j == 0 && it >= 1 && !mbar_wait(o_free, (it - 1) & 1, abort_flag, a.err, 0x87)) return false;
+          fence_acquire_cluster();
+          tc_fence_after();
+          const uint32_t bV = smem_u32(sV + s * kPR_SmemV);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) out[e] = (T)(l > 0.f || l != l ? acc[e] / l : 0.f);
-  *reinterpret_cast<uint4*>(static_cast<T*>(a.o) + ((size_t)tok * a.H + h) * kPA_D + 8 * lane) = *reinterpret_cast<uint4*>(out);
-  if (a.lse && lane == 0) a.lse[(size_t)h * a.T + tok] = l > 0.f || l != l ? (m + log2f(l)) * kLn2 : -INFINITY;
+          for (int ks = 0; ks < kPR_N / 16; ++ks)
+            umma_f16_ts_pair(tmem + kPR_TmO, tmem + s * kPR_N + prompt_pcol(ks), sdesc_sw128_mn(bV + ks * 2048, kPR_N * 128), id_o,
+                             (j | ks) > 0 ? 1u : 0u);
+          umma_commit_pair(v_empty + s);
+          return true;
+        };
+        for (int j = 0; j < n && ok; ++j) {
+          const int tt = t + j, s = tt & 1;
+          if (!(ok = mbar_wait(k_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x88))) break;
+          tc_fence_after();
+          const uint32_t bK = smem_u32(sK + s * kPR_SmemK);
+#pragma unroll
+          for (int ks = 0; ks < kPR_D / 16; ++ks)
+            umma_f16_ss_pair(tmem + s * kPR_N, sdesc_kstep(aQ, kPR_M, ks), sdesc_kstep(bK, kPR_N / 2, ks), id_s, ks > 0);
+          umma_commit_pair(k_empty + s);
+          umma_commit_pair(s_full + s);
+          if (j == n - 1) umma_commit_pair(q_free);
+          if (j >= 1 && !(ok = pv(j - 1, tt - 1))) break;
+        }
+        if (!ok) break;
+        if (n > 0) {
+          if (!(ok = pv(n - 1, t + n - 1))) break;
+        } else {
+          // O counts as complete only once the item before has been drained, products or not
+          if (it >= 1 && !(ok = mbar_wait(o_free, (it - 1) & 1, abort_flag, a.err, 0x87))) break;
+          umma_commit_pair(q_free);
+        }
+        umma_commit_pair(o_fin);
+        t += n;
+      }
+    }
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPR_RegsSoftmax));
+    // ------------------------------------------------------------------ softmax (warps 4..11)
+    const int q4 = warp & 3, hh = (warp - 4) >> 2;
+    const int r = q4 * 32 + lane;                 // row of the tile == TMEM lane
+    const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16);
+    constexpr int NH = kPR_N / 2;                 // 64 keys per half
+    const uint32_t pf[2] = {cluster_addr(p_full, 0), cluster_addr(p_full + 1, 0)};
+    uint32_t pair_phase = 0;
+    const int lim = i0 + r + off;                 // last key that this row sees
+    const int lim_all = i0 + off;                 // last key that every row of this CTA sees
+    bool alive = true;
+    int t = 0;
+    for (int it = 0; it < items && alive; ++it) {
+      float m_ref = -INFINITY, l = 0.f;           // running maximum (log2 domain) and this half's sum
+      for (int j = 0; j < n; ++j) {
+        const int tt = t + j, s = tt & 1;
+        if (!mbar_wait_warp(s_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x89)) { alive = false; break; }
+        tc_fence_after();
+        float uu[NH];
+        {
+          uint32_t w0[32], w1[32];
+          tmem_ld32(trow + s * kPR_N + hh * NH, w0);
+          tmem_ld32(trow + s * kPR_N + hh * NH + 32, w1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            uu[e] = __uint_as_float(w0[e]);
+            uu[e + 32] = __uint_as_float(w1[e]);
+          }
+        }
+        if (j * kPR_N + kPR_N - 1 > lim_all) {
+          const int hi = lim - j * kPR_N - hh * NH;
+#pragma unroll
+          for (int e = 0; e < NH; ++e) uu[e] = e <= hi ? uu[e] : -INFINITY;
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < NH; e += 8) {
+          mx0 = max3(mx0, uu[e], uu[e + 1]);
+          mx1 = max3(mx1, uu[e + 2], uu[e + 3]);
+          mx2 = max3(mx2, uu[e + 4], uu[e + 5]);
+          mx3 = max3(mx3, uu[e + 6], uu[e + 7]);
+        }
+        const float mown = max3(mx0, mx1, fmaxf(mx2, mx3));
+        float* xm = xch + s * 256;
+        xm[hh * 128 + r] = mown;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pair[q4]);
+        if (!mbar_wait_warp(&pair[q4], pair_phase++ & 1, abort_flag, a.err, 0x8a)) { alive = false; break; }
+        const float mt = fmaxf(mown, xm[(1 - hh) * 128 + r]) * a.c2;
+        float factor = 1.f;
+        bool rescale = false;
+        if (m_ref == -INFINITY) {
+          m_ref = mt;   // nothing accumulated yet
+        } else if (mt > m_ref + kPR_Rescale) {
+          factor = ex2_approx(m_ref - mt);
+          rescale = true;
+          m_ref = mt;
+          l *= factor;
+        }
+        uint32_t pk[NH / 2];
+        {
+          // a row that has seen nothing: scores of -inf against 0 give weights of 0, and a NaN stays one
+          const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
+          float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < NH; c += 2) {
+            const float e0 = ex2_approx(fmaf(uu[c], a.c2, nm)), e1 = ex2_approx(fmaf(uu[c + 1], a.c2, nm));
+            ls[(c >> 1) & 3] += e0 + e1;
+            pk[c / 2] = pack16<T>(e0, e1);
+          }
+          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        }
+        // O rescale (warp-collective), from the item's second tile on: after O += P_{j-1} V_{j-1} has finished
+        if (j >= 1 && __any_sync(0xffffffffu, rescale)) {
+          if (!mbar_wait_warp(v_empty + ((tt - 1) & 1), ((tt - 1) >> 1) & 1, abort_flag, a.err, 0x8b)) { alive = false; break; }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = hh * 128; c < hh * 128 + 128; c += 32) {
+            uint32_t ow[32];
+            tmem_ld32(trow + kPR_TmO + c, ow);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * factor);
+            tmem_st32(trow + kPR_TmO + c, ow);
+          }
+        }
+        tmem_st32(trow + s * kPR_N + hh * NH, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(pf[s]);
+      }
+      if (!alive) break;
+      t += n;
+      // the row's statistics for the output warps (slot it & 1, free once they read item it - 2's)
+      const int slot = it & 1;
+      if (it >= 2 && !(alive = mbar_wait_warp(&sfree[slot], ((it >> 1) - 1) & 1, abort_flag, a.err, 0x8c))) break;
+      xl[slot * 256 + hh * 128 + r] = l;
+      if (hh == 0) xmx[slot * 128 + r] = m_ref;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&stats[slot]);
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPR_RegsEpi));
+    // ------------------------------------------------------------------ outputs (warps 12..15)
+    const int q4 = warp & 3, r = q4 * 32 + lane;
+    const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16);
+    const uint32_t of = cluster_addr(o_free, 0);
+    const bool store = i0 + r < blk.nq;
+    for (int it = 0; it < items; ++it) {
+      if (!mbar_wait_warp(o_fin, it & 1, abort_flag, a.err, 0x8d)) break;
+      const int slot = it & 1;
+      if (!mbar_wait_warp(&stats[slot], (it >> 1) & 1, abort_flag, a.err, 0x8e)) break;
+      const float l = xl[slot * 256 + r] + xl[slot * 256 + 128 + r], m = xmx[slot * 128 + r];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sfree[slot]);
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;        // nothing seen: zeros
+      const int h = head(it);
+      const size_t row = (size_t)blk.q0 + i0 + r;
+      if (store && a.lse) a.lse[(size_t)h * a.T + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (row * a.H + h) * kPR_D);
+#pragma unroll 1
+      for (int c = 0; c < kPR_D; c += 32) {
+        uint32_t ow[32];
+        if (n > 0) {
+          tmem_ld32(trow + kPR_TmO + c, ow);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) ow[e] = 0u;
+        }
+        uint32_t v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = pack16<T>(__uint_as_float(ow[2 * e]) * inv, __uint_as_float(ow[2 * e + 1]) * inv);
+        if (store) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[c / 8 + e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(of);
+    }
+  }
+  if (*abort_flag) {   // a wait gave up: time for the copies and products in flight to end
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000ull) {
+    }
+  }
+  // neither CTA leaves while the other's products may read its shared memory or arrive on its barriers
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+template <typename T>
+static int launch_prompt(const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap, const PromptArgs& a,
+                         long long clusters, cudaStream_t stream) {
+  const int rc = ensure_smem_attr((const void*)prompt_attn_kernel<T>, kPR_Smem);
+  if (rc) return rc;
+  prompt_attn_kernel<T><<<(unsigned)(2 * clusters), kPR_Threads, kPR_Smem, stream>>>(qmap, kmap, vmap, a);
+  return launch_status();
 }
 
 }  // namespace bfb
@@ -83,22 +472,48 @@ int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void
                        bf_stream_t stream) {
   if (T < 0 || Tk < 0 || n_seq < 0 || H <= 0 || G <= 0 || H % G || !(scale > 0.f) || scale > 3e38f)
     return BF_ERR_INVALID_ARGUMENT;
-  if (D != kPA_D || (dtype != BF_BF16 && dtype != BF_F16)) return BF_ERR_UNSUPPORTED;
+  if (D != kPR_D || (dtype != BF_BF16 && dtype != BF_F16)) return BF_ERR_UNSUPPORTED;
   if (T == 0) return BF_OK;
   if (!q || !o || (Tk > 0 && (!k || !v)) || (n_seq > 0 && !cu_q)) return BF_ERR_INVALID_ARGUMENT;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || ((q_st | q_sh | k_st | k_sh | v_st | v_sh) & 7))
     return BF_ERR_ALIGNMENT;
+  if ((T > 1 && q_st <= 0) || (H > 1 && q_sh <= 0) || (Tk > 1 && (k_st <= 0 || v_st <= 0)) || (G > 1 && (k_sh <= 0 || v_sh <= 0)))
+    return BF_ERR_INVALID_ARGUMENT;
   DeviceState st;
   int rc = device_state(&st);
   if (rc) return rc;
-  PromptArgs a{q, k, v, q_st, q_sh, k_st, k_sh, v_st, v_sh, cu_q, cu_k ? cu_k : cu_q, n_seq, T, Tk, H, G,
-               scale * kLog2e, o, lse};
-  const dim3 grid(T, (H + 3) / 4);
-  if (dtype == BF_BF16)
-    prompt_attn_kernel<__nv_bfloat16><<<grid, 128, 0, stream>>>(a);
-  else
-    prompt_attn_kernel<__half><<<grid, 128, 0, stream>>>(a);
-  return launch_status();
+  PromptArgs a{};
+  a.cu_q = cu_q;
+  a.cu_k = cu_k ? cu_k : cu_q;
+  a.n_seq = n_seq; a.T = T; a.Tk = Tk; a.H = H; a.G = G;
+  a.c2 = scale * kLog2e;
+  a.o = o;
+  a.lse = lse;
+  a.err = st.err;
+  const int R = H / G;
+  a.qb = R % 2 == 0 ? kPR_M : 2 * kPR_M;
+  const int all = R % 2 == 0 ? R / 2 : R;
+  const long long nblk = (long long)T / a.qb + n_seq + 2;
+  if (nblk > 0x7fffffffLL) return BF_ERR_UNSUPPORTED;
+  a.nblk = (int)nblk;
+  a.per = nblk * G >= 2LL * st.sm_count ? all : 1;
+  a.hsplit = (all + a.per - 1) / a.per;
+  const long long clusters = nblk * G * a.hsplit;
+  if (clusters > 0x3fffffffLL) return BF_ERR_UNSUPPORTED;
+  // (64 dims, tokens, 4 groups of 64 dims, heads); a stride of a dimension of one means nothing, and the encoder wants a positive one
+  auto map = [&](CUtensorMap* m, const void* x, int rows, int heads, long long st_, long long sh_, uint32_t box_rows, uint32_t atoms) {
+    const uint64_t dims[4] = {64, (uint64_t)rows, 4, (uint64_t)heads};
+    const uint64_t str[3] = {(uint64_t)(st_ > 0 ? st_ : kPR_D) * 2, 128, (uint64_t)(sh_ > 0 ? sh_ : kPR_D) * 2};
+    const uint32_t box[4] = {64, box_rows, atoms, 1};
+    return make_tmap(m, x, dtype, 4, dims, str, box, true);
+  };
+  CUtensorMap qmap, kmap, vmap;
+  if ((rc = map(&qmap, q, T, H, q_st, q_sh, kPR_M, 4))) return rc;
+  // without a key no tile is loaded: any map will do
+  if ((rc = map(&kmap, Tk ? k : q, Tk ? Tk : T, Tk ? G : H, Tk ? k_st : q_st, Tk ? k_sh : q_sh, kPR_N / 2, 4))) return rc;
+  if ((rc = map(&vmap, Tk ? v : q, Tk ? Tk : T, Tk ? G : H, Tk ? v_st : q_st, Tk ? v_sh : q_sh, kPR_N, 2))) return rc;
+  return dtype == BF_BF16 ? launch_prompt<__nv_bfloat16>(qmap, kmap, vmap, a, clusters, stream)
+                          : launch_prompt<__half>(qmap, kmap, vmap, a, clusters, stream);
 }
 
 }  // extern "C"

@@ -226,10 +226,12 @@ def same_device(*ts) -> torch.device:
 
 
 def heads_16bit(name: str, t) -> torch.Tensor:
-    """t [..., D] with its last dimension contiguous and every row on a 16-byte boundary (copied when it is not)."""
+    """t [..., D] with its last dimension contiguous, every row on a 16-byte boundary and no dimension expanded (copied when it is
+    not so)."""
     if t.dtype not in (torch.bfloat16, torch.float16):
         raise NotImplementedError(f"{name} is {t.dtype}: built for bfloat16 and float16")
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+        all(s > 0 and s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -265,7 +267,7 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, with_ls
     (an entry below the one before it counts as equal to it, one beyond T as T).  Query i of a sequence with nq
     queries and nk keys sees its keys j <= i + nk - nq: the queries are the sequence's last tokens.
     Returns o [T,H,D] in q's dtype and lse [H,T] fp32 (None unless ``with_lse``); a query that sees no key and the
-    rows behind the last sequence have o = 0 and lse = -inf.  ``scale`` (default D^-1/2) must be positive.
+    rows of no sequence (before the first, behind the last) have o = 0 and lse = -inf.  ``scale`` (default D^-1/2) must be positive.
     """
     check_cuda(q, k, v)
     refuse_grad("prompt_attention", q, k, v)

@@ -350,10 +350,10 @@ int bf_llama_state_unpack(const float* rows, long long row_stride, const int64_t
  * HybridAttention._teacher, heimdall/hibrit.py:275-290, for sequences of different lengths in one call).
  * Sequence b has queries cu_q[b] .. cu_q[b+1] - 1 and keys cu_k[b] .. cu_k[b+1] - 1 (cu_k NULL: cu_q); its query i
  * of nq sees its keys j <= i + nk - nq, the rest is masked; softmax of scale * q.k in fp32.
- *   q [T,H,D], k, v [Tk,G,D]: dtype BF_BF16 or BF_F16, element strides per token and head given (multiples of 8, a
- *   head's D elements contiguous); cu_q, cu_k [n_seq + 1] int32 on the device, ascending: every entry is clamped
+ *   q [T,H,D], k, v [Tk,G,D]: dtype BF_BF16 or BF_F16, element strides per token and head given (positive multiples
+ *   of 8, a head's D elements contiguous); cu_q, cu_k [n_seq + 1] int32 on the device, ascending: every entry is clamped
  *   into [previous, T] (or Tk); o [T,H,D] contiguous in dtype; lse [H,T] fp32 or NULL.
- * A query that sees no key, and every row behind the last sequence, gets o = 0 and lse = -inf.
+ * A query that sees no key, and every row of no sequence, gets o = 0 and lse = -inf.
  * D = 256, scale > 0.
  */
 int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void* k, long long k_st, long long k_sh,

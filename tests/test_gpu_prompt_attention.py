@@ -103,6 +103,9 @@ def test_lengths_beyond_the_tensors_are_cut():
     _check(o, lse, q, k, v, [0, 60, 100])
     o, lse = _run(q, k, v, [0, 60, 40, 100])       # a descending entry counts as the one before it
     _check(o, lse, q, k, v, [0, 60, 60, 100])
+    o, lse = _run(q, k, v, [20, 60, 90])           # rows before the first sequence belong to none
+    _check(o[20:90], lse[:, 20:90], q[20:90], k[20:90], v[20:90], [0, 40, 70])
+    assert (o[:20] == 0).all() and (o[90:] == 0).all() and (lse[:, :20] == -float("inf")).all()
     o, lse = _run(q, k, v, [-7, 60, 100])
     _check(o, lse, q, k, v, [0, 60, 100])
 
@@ -186,6 +189,18 @@ def test_refusals():
     for s in (0.0, -1.0, float("nan"), float("inf")):
         with pytest.raises(ValueError):
             prompt_attention(q, k, v, cu, scale=s)
+
+
+def test_many_sequences():
+    """More sequences than a warp has lanes, most of them short, some empty."""
+    lens = [(11 * i) % 23 for i in range(100)] + [200] + [(7 * i) % 5 for i in range(40)]
+    T = sum(lens)
+    q, k, v = _inputs(T, T, 3, 1, torch.bfloat16, 12)
+    o, lse = _run(q, k, v, _cu(lens))
+    _check(o, lse, q, k, v, _cu(lens))
+    q, k, v = _inputs(T, T, 4, 2, torch.bfloat16, 13)
+    o, lse = _run(q, k, v, _cu(lens))
+    _check(o, lse, q, k, v, _cu(lens))
 
 
 def test_no_tokens():
