@@ -18,8 +18,11 @@
 // Work: the tiles of 128 tokens of all (sequence, token chunk, KV head) segments in one line, cut into equal runs, one per CTA
 // (one CTA per SM), whatever the lengths.  A segment inside one run is finished there; of a cut one each CTA writes its
 // partial (at most two per CTA), and paged_combine_kernel merges them in order, so results do not depend on timing.
-// Warps (384 threads): 0 TMA of the codes (a ring of 32 KB units K0 V0 K1 V1 ...); 1 MMA; 2 the next segment's Q parts; 3 the
-// tiles' scales; 4-7 softmax (thread = token); 8-11 the accumulators (thread = dims d and d + 128) and the output.
+// Warps (640 threads): 0 TMA of the codes (a ring of 32 KB units K0 V0 K1 V1 ...); 1 MMA; 2 the next segment's Q parts; 3 the
+// tiles' scales; 4-11 softmax (thread = token and the even or the odd rows); 12-19 the accumulators (thread = dim) and the output.
+// With one softmax warp per scheduler a tile took 6100 cycles, most of them the latency of that warp's own chain of
+// instructions; the rows are therefore dealt to two warpgroups, and what is the same for all tokens (a row's maximum and its
+// two factors) is computed by one lane per row and passed by shuffles.
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -28,7 +31,7 @@
 
 namespace bfb {
 
-constexpr int kPA_Threads = 384;
+constexpr int kPA_Threads = 640;
 constexpr int kPA_Tile = 128;                        // tokens per tile
 constexpr int kPA_Unit = kPA_Tile * kPG_D;           // bytes of one K or V tile
 constexpr int kPA_MaxCtas = 160;
@@ -84,26 +87,31 @@ struct PagedWalk {
   }
 };
 
-// x = (x0 + x1 / 16 + x2 / 256) with e4m3 parts, for |x| <= 256; two values at a time
-__device__ __forceinline__ uint16_t to_e4m3x2(float lo, float hi) {
+// x = (x0 + x1 / 16 + x2 / 256) with e4m3 parts, for |x| <= 256; two values at a time.  x is first rounded to fp16, whose 11
+// bits the parts hold exactly; the remainders are exact in fp16.
+__device__ __forceinline__ uint16_t to_e4m3x2(uint32_t h2) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h2));
   return r;
 }
-__device__ __forceinline__ float2 of_e4m3x2(uint16_t c) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(c));
-  return __half22float2(*reinterpret_cast<__half2*>(&h));
-}
 __device__ __forceinline__ void split3(float a, float b, uint16_t (&part)[3]) {
+  const __half2 m16 = __floats2half2_rn(-16.f, -16.f), p16 = __floats2half2_rn(16.f, 16.f);
+  __half2 x = __floats2half2_rn(a, b);
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    part[i] = to_e4m3x2(a, b);
-    const float2 f = of_e4m3x2(part[i]);
-    a = (a - f.x) * 16.f;
-    b = (b - f.y) * 16.f;
+    part[i] = to_e4m3x2(*reinterpret_cast<uint32_t*>(&x));
+    if (i < 2) {
+      uint32_t f;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f) : "h"(part[i]));
+      x = __hfma2(*reinterpret_cast<__half2*>(&f), m16, __hmul2(x, p16));   // 16 (x - part)
+    }
   }
 }
+// the RP rows lie in the order even rows, odd rows: row r in column row_col(r) of each part
+template <int RP>
+__device__ __forceinline__ constexpr int row_col(int r) { return (r & 1) * (RP / 2) + (r >> 1); }
+template <int RP>
+__device__ __forceinline__ constexpr int col_row(int c) { return 2 * (c % (RP / 2)) + c / (RP / 2); }
 
 template <typename T, int RP>
 __global__ void __launch_bounds__(kPA_Threads, 1)
@@ -118,17 +126,17 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * C::PBytes);
   uint64_t *full = bars, *empty = bars + 6, *s_full = bars + 12, *s_free = bars + 14, *p_full = bars + 16, *o_full = bars + 18,
            *o_free = bars + 20, *q_full = bars + 22, *q_free = bars + 24, *sc_full = bars + 26, *sc_free = bars + 30, *red = bars + 34,
-           *seg_full = bars + 35, *seg_free = bars + 37;
+           *seg_full = bars + 36, *seg_free = bars + 38;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 40);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 41);
-  long long* s_sum = reinterpret_cast<long long*>(bars + 42);       // [12] per-warp totals of the tile count
-  int* s_start = reinterpret_cast<int*>(bars + 54);                 // b, tiles into it
-  float* s_qs = reinterpret_cast<float*>(bars + 56);                // [2][RP] scale of the Q rows
+  long long* s_sum = reinterpret_cast<long long*>(bars + 42);       // [20] per-warp totals of the tile count
+  int* s_start = reinterpret_cast<int*>(bars + 62);                 // b, segment of it, tile of that
+  float* s_qs = reinterpret_cast<float*>(bars + 64);                // [2][RP] scale of the Q rows
   float* s_fac = s_qs + 2 * kPA_MaxRows;                            // [2][RP][2] factors of the tile's O^T and the accumulators
   float* s_red = s_fac + 4 * kPA_MaxRows;                           // [2][4][RP] the warps' maxima
   float* s_seg = s_red + 8 * kPA_MaxRows;                           // [2][5][RP] a segment's sums per warp, its maximum
   float* s_sc = s_seg + 10 * kPA_MaxRows;                           // [4][20] scales of a tile's pages: 8 K, 8 V ratios, V's largest, mask
-  static_assert(56 * 8 + (2 + 4 + 8 + 10) * kPA_MaxRows * 4 + 80 * 4 <= 4096, "barriers and exchanges");
+  static_assert(64 * 8 + (2 + 4 + 8 + 10) * kPA_MaxRows * 4 + 80 * 4 <= 4096, "barriers and exchanges");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
@@ -138,20 +146,20 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(s_free + i, 4);
-      mbar_init(p_full + i, 4);
+      mbar_init(s_free + i, 8);
+      mbar_init(p_full + i, 8);
       mbar_init(o_full + i, 1);
-      mbar_init(o_free + i, 4);
+      mbar_init(o_free + i, 8);
       mbar_init(q_full + i, 1);
-      mbar_init(q_free + i, 5);
-      mbar_init(seg_full + i, 4);
-      mbar_init(seg_free + i, 4);
+      mbar_init(q_free + i, 9);
+      mbar_init(seg_full + i, 8);
+      mbar_init(seg_free + i, 8);
+      mbar_init(red + i, 4);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(sc_full + i, 1);
-      mbar_init(sc_free + i, 4);
+      mbar_init(sc_free + i, 8);
     }
-    mbar_init(red, 4);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -335,13 +343,13 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         for (int i = 0; i < 4; ++i) split3(x[2 * i], x[2 * i + 1], c[i]);
 #pragma unroll
         for (int part = 0; part < 3; ++part) {
-          const int n = part * RP + r;
+          const int n = part * RP + row_col<RP>(r);
           const uint32_t chunk = ((lane & 15) >> 1) ^ (n & 7);
           *reinterpret_cast<uint2*>(dst + (lane >> 4) * (NP * 128) + n * 128 + chunk * 16 + (lane & 1) * 8) =
               make_uint2(c[0][part] | ((uint32_t)c[1][part] << 16), c[2][part] | ((uint32_t)c[3][part] << 16));
         }
         // a row with a value that is not finite has no finite scores
-        if (lane == 0) s_qs[(seg & 1) * RP + r] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
+        if (lane == 0) s_qs[(seg & 1) * RP + row_col<RP>(r)] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
       }
       fence_async_smem();
       __syncwarp();
@@ -381,26 +389,28 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_full + s);
     }
-  } else if (warp < 8) {
-    // ------------------------------------------------------------------ softmax: thread = token of the tile
-    const int wq = warp & 3, tok = wq * 32 + lane;
-    const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16);
-    float m_run[RP], l[RP], qs[RP];
-    int lim[RP];
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ softmax: thread = token of the tile, rows 2 i + hh
+    constexpr int RH = RP / 2;
+    const int wq = warp & 3, hh = (warp - 4) >> 2, tok = wq * 32 + lane;
+    const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + hh * RH;
+    float l[RH], qs[RH];
+    int lim[RH];
+    float m_run = -INFINITY;             // of row 2 lane + hh, in lanes < RH
     bool ok = true, first = true;
-    int seg = 0, rows = 0;
+    int seg = 0;
     for (int j = 0; j < count; ++j) {
       const int s = j & 1;
       if (first) {
         if (!(ok = mbar_wait_warp(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, a.err, 0x6a))) break;
-        const int i0 = w.c * a.tc;
-        rows = min(a.tc, a.t - i0) * a.R;
+        const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
+        m_run = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          m_run[r] = -INFINITY;
-          l[r] = 0.f;
-          qs[r] = s_qs[(seg & 1) * RP + r];
-          lim[r] = r < rows ? w.len - a.t + i0 + r / a.R : -1;     // the row's last visible position
+        for (int i = 0; i < RH; ++i) {
+          const int r = 2 * i + hh;
+          l[i] = 0.f;
+          qs[i] = s_qs[(seg & 1) * RP + hh * RH + i];
+          lim[i] = r < rows ? w.len - a.t + i0 + r / a.R : -1;     // the row's last visible position
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(q_free + (seg & 1));
@@ -409,7 +419,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       if (!(ok = mbar_wait_warp(sc_full + (j & 3), (j >> 2) & 1, abort_flag, a.err, 0x6b))) break;
       const float* sc = s_sc + (j & 3) * 20;
       const int pi = tok / L;
-      const float ks = sc[pi], vr = sc[8 + pi], top = sc[16];
+      const float ks = sc[pi], vr = sc[8 + pi] * 256.f, top = sc[16];
       const bool there = (__float_as_uint(sc[17]) >> pi) & 1u;
       const int pos = w.tile * kPA_Tile + tok;
       const bool valid = there && pos < w.len;
@@ -417,47 +427,54 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       if (lane == 0) mbar_arrive(sc_free + (j & 3));
       if (!(ok = mbar_wait_warp(s_full + s, (j >> 1) & 1, abort_flag, a.err, 0x6c))) break;
       tc_fence_after();
-      uint32_t raw[3 * RP];
+      uint32_t raw[3 * RH];
 #pragma unroll
-      for (int c = 0; c < 3 * RP; c += 8) tmem_ld8(trow + s * NP + c, raw + c);
+      for (int part = 0; part < 3; ++part) {
+#pragma unroll
+        for (int c = 0; c + 8 <= RH; c += 8) tmem_ld8(trow + s * NP + part * RP + c, raw + part * RH + c);
+        if (RH % 8) tmem_ld4(trow + s * NP + part * RP + RH / 8 * 8, raw + part * RH + RH / 8 * 8);
+      }
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free + s);
-      float x[RP];
-      float* rd = s_red + s * 4 * RP;
+      float x[RH], mine = -INFINITY;
+      float* rd = s_red + s * 4 * RP + hh * RH;
 #pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        const float d = __uint_as_float(raw[r]) + (__uint_as_float(raw[RP + r]) + __uint_as_float(raw[2 * RP + r]) * 0.0625f) * 0.0625f;
-        x[r] = valid && pos <= lim[r] ? d * (ks * qs[r]) : -INFINITY;
+      for (int i = 0; i < RH; ++i) {
+        const float d = __uint_as_float(raw[i]) + (__uint_as_float(raw[RH + i]) + __uint_as_float(raw[2 * RH + i]) * 0.0625f) * 0.0625f;
+        x[i] = valid && pos <= lim[i] ? d * (ks * qs[i]) : -INFINITY;
         float mx;
-        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(mx) : "f"(x[r]));
-        if (lane == 0) rd[wq * RP + r] = mx;
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(mx) : "f"(x[i]));
+        if (lane == i) mine = mx;
       }
+      if (lane < RH) rd[wq * RP + lane] = mine;
       __syncwarp();
-      if (lane == 0) mbar_arrive(red);
-      if (!(ok = mbar_wait_warp(red, j & 1, abort_flag, a.err, 0x6d))) break;
+      if (lane == 0) mbar_arrive(red + hh);
+      if (!(ok = mbar_wait_warp(red + hh, j & 1, abort_flag, a.err, 0x6d))) break;
+      // lane i: row 2 i + hh's maximum of the tile, and the factors of what was before and of this tile
+      float mt = -INFINITY;
+      if (lane < RH) mt = fmaxf(fmaxf(rd[lane], rd[RP + lane]), fmaxf(rd[2 * RP + lane], rd[3 * RP + lane]));
+      const float mn = fmaxf(m_run, mt);
+      const float al = m_run == -INFINITY ? 0.f : ex2_approx(m_run - mn);
+      const float f = mt == -INFINITY ? 0.f : ex2_approx(mt - mn);
+      m_run = mn;
+      mt = mt == -INFINITY ? 0.f : mt;
       // P of the tile before the last but one has been read, and so have its factors
       if (j >= 2 && !(ok = mbar_wait_warp(o_free + s, ((j >> 1) - 1) & 1, abort_flag, a.err, 0x6e))) break;
+      if (wq == 0 && lane < RH)
+        *reinterpret_cast<float2*>(s_fac + (s * RP + hh * RH + lane) * 2) = make_float2(al, f * top * (1.f / 256.f));
       uint8_t* pd = sP + s * C::PBytes;
 #pragma unroll
-      for (int r = 0; r < RP; r += 2) {
+      for (int i = 0; i < RH; i += 2) {
         float y[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float mt = fmaxf(fmaxf(rd[r + e], rd[RP + r + e]), fmaxf(rd[2 * RP + r + e], rd[3 * RP + r + e]));
-          const float mn = fmaxf(m_run[r + e], mt);
-          const float al = m_run[r + e] == -INFINITY ? 0.f : ex2_approx(m_run[r + e] - mn);
-          const float f = mt == -INFINITY ? 0.f : ex2_approx(mt - mn);
           // masked scores are -inf and give 0; a NaN stays one, whatever the others are
-          const float p = x[r + e] == -INFINITY ? 0.f : ex2_approx(x[r + e] - (mt == -INFINITY ? 0.f : mt));
-          l[r + e] = l[r + e] * al + (p != p ? p : p * f);
-          m_run[r + e] = mn;
-          y[e] = p * (vr * 256.f);
-          if (tok == 0) {
-            s_fac[(s * RP + r + e) * 2] = al;
-            s_fac[(s * RP + r + e) * 2 + 1] = f * top * (1.f / 256.f);
-          }
+          const float p = ex2_approx(x[i + e] - __shfl_sync(0xffffffffu, mt, i + e));
+          const float fi = __shfl_sync(0xffffffffu, f, i + e);
+          l[i + e] = fmaf(l[i + e], __shfl_sync(0xffffffffu, al, i + e), p * fi);
+          y[e] = p * vr;
         }
         uint16_t c[3];
         split3(y[0], y[1], c);
@@ -465,8 +482,8 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         for (int part = 0; part < 3; ++part) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int n = part * RP + r + e;
-            pd[n * 128 + (((tok >> 4) ^ (n & 7)) << 4) + (tok & 15)] = (uint8_t)(c[part] >> (8 * e));
+            const int n7 = (part * RP + hh * RH + i + e) & 7, n = part * RP + hh * RH + i + e;
+            pd[n * 128 + (tok ^ (n7 << 4))] = (uint8_t)(c[part] >> (8 * e));
           }
         }
       }
@@ -475,9 +492,9 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         const int u = (2 * j + 1) % NU;
         if (!(ok = mbar_wait_warp(full + u, ((2 * j + 1) / NU) & 1, abort_flag, a.err, 0x6f))) break;
         if (!valid) {
-          uint4* row = reinterpret_cast<uint4*>(ring + u * kPA_Unit + tok * 128);
+          uint4* row = reinterpret_cast<uint4*>(ring + u * kPA_Unit + hh * (kPA_Tile * 128) + tok * 128);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) row[i] = row[kPA_Tile * 8 + i] = make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
         }
       }
       fence_async_smem();
@@ -485,13 +502,13 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       if (lane == 0) mbar_arrive(p_full + s);
       if (end) {
         if (seg >= 2 && !(ok = mbar_wait_warp(seg_free + (seg & 1), ((seg >> 1) - 1) & 1, abort_flag, a.err, 0x70))) break;
-        float* sg = s_seg + (seg & 1) * 5 * RP;
+        float* sg = s_seg + (seg & 1) * 5 * RP + hh * RH;
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float sum = warp_sum(l[r]);
-          if (lane == 0) sg[wq * RP + r] = sum;
-          if (tok == 0) sg[4 * RP + r] = m_run[r];
+        for (int i = 0; i < RH; ++i) {
+          const float sum = warp_sum(l[i]);
+          if (lane == 0) sg[wq * RP + i] = sum;
         }
+        if (wq == 0 && lane < RH) sg[4 * RP + lane] = m_run;
         __syncwarp();
         if (lane == 0) mbar_arrive(seg_full + (seg & 1));
         ++seg;
@@ -500,37 +517,29 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       w.next(a);
     }
   } else {
-    // ------------------------------------------------------------------ accumulators: thread = dims d and d + 128
-    const int wq = warp & 3, d = wq * 32 + lane;
-    const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + 2 * NP;
-    float acc[2][RP];
+    // ------------------------------------------------------------------ accumulators: thread = dim d of every row
+    const int wq = warp & 3, half = (warp - 12) >> 2, d = half * 128 + wq * 32 + lane;
+    const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + (2 + half) * NP;
+    float acc[RP];
     bool ok = true, from_start = w.tile == 0;
     int seg = 0;
     int4 desc = make_int4(-1, 0, 0, 0);
 #pragma unroll
-    for (int r = 0; r < RP; ++r) acc[0][r] = acc[1][r] = 0.f;
+    for (int c = 0; c < RP; ++c) acc[c] = 0.f;
     for (int j = 0; j < count; ++j) {
       const int s = j & 1;
       if (!(ok = mbar_wait_warp(p_full + s, (j >> 1) & 1, abort_flag, a.err, 0x73))) break;   // the factors
       if (!(ok = mbar_wait_warp(o_full + s, (j >> 1) & 1, abort_flag, a.err, 0x71))) break;
       tc_fence_after();
-      float fac[RP][2];
+      uint32_t raw[3 * RP];
 #pragma unroll
-      for (int r = 0; r < RP; ++r) {
-        fac[r][0] = s_fac[(s * RP + r) * 2];
-        fac[r][1] = s_fac[(s * RP + r) * 2 + 1];
-      }
+      for (int c = 0; c < 3 * RP; c += 8) tmem_ld8(trow + 2 * s * NP + c, raw + c);
+      tmem_wait_ld();
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t raw[3 * RP];
-#pragma unroll
-        for (int c = 0; c < 3 * RP; c += 8) tmem_ld8(trow + (2 * s + half) * NP + c, raw + c);
-        tmem_wait_ld();
-#pragma unroll
-        for (int r = 0; r < RP; ++r) {
-          const float x = __uint_as_float(raw[r]) + (__uint_as_float(raw[RP + r]) + __uint_as_float(raw[2 * RP + r]) * 0.0625f) * 0.0625f;
-          acc[half][r] = acc[half][r] * fac[r][0] + x * fac[r][1];
-        }
+      for (int c = 0; c < RP; ++c) {
+        const float2 fac = *reinterpret_cast<const float2*>(s_fac + (s * RP + c) * 2);
+        const float x = __uint_as_float(raw[c]) + (__uint_as_float(raw[RP + c]) + __uint_as_float(raw[2 * RP + c]) * 0.0625f) * 0.0625f;
+        acc[c] = acc[c] * fac.x + x * fac.y;
       }
       tc_fence_before();
       __syncwarp();
@@ -543,26 +552,24 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         const bool whole = from_start && last;
         float* part = a.part + ((size_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * RP * kPA_Part;
 #pragma unroll
-        for (int r = 0; r < RP; ++r) {
+        for (int c = 0; c < RP; ++c) {
+          const int r = col_row<RP>(c);
           if (r < rows) {
-            const float sum = (sg[r] + sg[RP + r]) + (sg[2 * RP + r] + sg[3 * RP + r]), m = sg[4 * RP + r];
+            const float sum = (sg[c] + sg[RP + c]) + (sg[2 * RP + c] + sg[3 * RP + c]), m = sg[4 * RP + c];
             if (whole) {
               const int i = i0 + r / a.R, h = w.g * a.R + r % a.R;
               const float inv = sum == 0.f ? 0.f : 1.f / sum;       // nothing seen: zeros
-              T* o = static_cast<T*>(a.o) + (((size_t)w.b * a.t + i) * a.H + h) * kPG_D;
-              o[d] = (T)(acc[0][r] * inv);
-              o[d + 128] = (T)(acc[1][r] * inv);
+              static_cast<T*>(a.o)[(((size_t)w.b * a.t + i) * a.H + h) * kPG_D + d] = (T)(acc[c] * inv);
               if (a.lse && d == 0) a.lse[((size_t)w.b * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
             } else {
-              part[r * kPA_Part + d] = acc[0][r];
-              part[r * kPA_Part + d + 128] = acc[1][r];
+              part[r * kPA_Part + d] = acc[c];
               if (d == 0) {
                 part[r * kPA_Part + kPG_D] = m;
                 part[r * kPA_Part + kPG_D + 1] = sum;
               }
             }
           }
-          acc[0][r] = acc[1][r] = 0.f;
+          acc[c] = 0.f;
         }
         // a cut segment that ends here: the CTA that holds its first tile
         if (last && !from_start) {

@@ -254,7 +254,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           if (!mbar_wait(p_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x85)) return false;
           if (!mbar_wait(v_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x86)) return false;
           if (j == 0 && it >= 1 && !mbar_wait(o_free, (it - 1) & 1, abort_flag, a.err, 0x87)) return false;
-          fence_acquire_cluster();
           tc_fence_after();
           const uint32_t bV = smem_u32(sV + s * kPR_SmemV);
 #pragma unroll
