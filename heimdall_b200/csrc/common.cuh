@@ -44,6 +44,13 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 // wait limit for any single mbarrier wait: 200 ms of wall time (legitimate waits last microseconds)
 constexpr uint64_t kWaitLimitNs = 200ull * 1000ull * 1000ull;
 
+// one lane of a converged warp; what runs under it keeps warp-uniform operands (descriptors, addresses) in uniform registers
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -106,6 +113,33 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
                                                unsigned int site) {
   const bool ok = mbar_wait(bar, parity, abort, err, site);
   return __all_sync(0xffffffffu, ok) != 0;
+}
+
+// The same two waits in a few instructions, for kernels of many roles, whose loops would otherwise not stay in the instruction
+// cache: limited by a number of tries (each one suspends the thread for a while itself), a wait that gives up leaves its site in
+// the CTA's abort word, and the kernel's end reports that (report_abort).
+constexpr uint32_t kWaitTries = 1u << 20;
+__device__ __forceinline__ bool mbar_wait_small(uint64_t* bar, uint32_t parity, volatile int* abort, unsigned int site) {
+  const uint32_t a = smem_u32(bar);
+#pragma unroll 1
+  for (uint32_t n = 0; !mbar_try_wait(a, parity); ++n) {
+    if (n == kWaitTries || *abort) {
+      if (n == kWaitTries) *abort = (int)site;
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ bool mbar_wait_warp_small(uint64_t* bar, uint32_t parity, volatile int* abort, unsigned int site) {
+  return __all_sync(0xffffffffu, mbar_wait_small(bar, parity, abort, site)) != 0;
+}
+// by one thread after the CTA's last barrier; gives copies and products in flight time to end before the CTA does
+__device__ __forceinline__ void report_abort(volatile int* abort, unsigned int* err) {
+  if (*abort == 0) return;
+  record_error(err, (unsigned)*abort);
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 1000000ull) {
+  }
 }
 
 // ----------------------------------------------------------------------------------------------

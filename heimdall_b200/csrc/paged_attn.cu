@@ -16,13 +16,16 @@
 // carry the running maximum: nothing is rescaled in TMEM.  V's scales go into P (as their ratio to the tile's largest).
 //
 // Work: the tiles of 128 tokens of all (sequence, token chunk, KV head) segments in one line, cut into equal runs, one per CTA
-// (one CTA per SM), whatever the lengths.  A segment inside one run is finished there; of a cut one each CTA writes its
+// (one CTA per SM), whatever the lengths; a segment's start counts as one tile more, as its queries and its output take about that long.  A segment inside one run is finished there; of a cut one each CTA writes its
 // partial (at most two per CTA), and paged_combine_kernel merges them in order, so results do not depend on timing.
-// Warps (640 threads): 0 TMA of the codes (a ring of 32 KB units K0 V0 K1 V1 ...); 1 MMA; 2 the next segment's Q parts; 3 the
-// tiles' scales; 4-11 softmax (thread = token and the even or the odd rows); 12-19 the accumulators (thread = dim) and the output.
+// Warps (640 threads): 0 TMA of the codes (a ring of 32 KB units K0 V0 K1 V1 ...) and the tiles' scales; 1 the products S; 2 the
+// next segment's Q parts; 3 the products O; 4-11 softmax (thread = token and the even or the odd rows); 12-19 the accumulators
+// (thread = dim) and the output.
 // With one softmax warp per scheduler a tile took 6100 cycles, most of them the latency of that warp's own chain of
 // instructions; the rows are therefore dealt to two warpgroups, and what is the same for all tokens (a row's maximum and its
-// two factors) is computed by one lane per row and passed by shuffles.
+// two factors) is computed by one lane per row and passed by shuffles.  The products are small, so issuing them is what costs:
+// one thread of a diverged warp took 4400 cycles per tile for both (every descriptor on its way through vector registers); two
+// warps that stay converged and elect the issuing lane do not bound it.
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -45,6 +48,9 @@ struct PagedAttnArgs {
   const int32_t* slots;
   int B, t, H, R;
   int tc, nqc;          // tokens per chunk, chunks
+  int cap;              // tokens that the table has room for
+  int page_log;         // log2 of the page's tokens
+  unsigned by_r;        // 2^16 / R, rounded up: r / R = r * by_r >> 16 for rows r < 24
   float c2;             // scale * log2(e)
   void* o;
   float* lse;
@@ -59,20 +65,37 @@ struct PagedCfg {
   static constexpr int Units = RP == 8 ? 6 : 5;            // ring units that fit beside Q and P
   static constexpr int TmemCols = 6 * NP <= 256 ? 256 : 512;   // S[2], O[2][2 halves]
   static constexpr int QBytes = NP * kPG_D, PBytes = NP * kPA_Tile;
-  static constexpr int Smem = Units * kPA_Unit + 2 * QBytes + 2 * PBytes + 4096 + 1024;
+  static constexpr int Smem = Units * kPA_Unit + 2 * QBytes + 2 * PBytes + 5120 + 1024;
 };
 
-__device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
+// slot (-1: none) and visible length of sequence b
+__device__ __forceinline__ int2 paged_seq(const PagedAttnArgs& a, int b) {
   const int slot = a.slots ? a.slots[b] : b;
-  if (slot < 0 || slot >= a.p.slots) return 0;
-  return (int)max(0LL, min((long long)a.p.lens[slot], (long long)a.p.width * a.p.page));
+  const bool ok = slot >= 0 && slot < a.p.slots;
+  return make_int2(ok ? slot : -1, ok ? max(0, min(a.p.lens[slot], a.cap)) : 0);
 }
 // tiles of a sequence: at least one, so that a segment that sees nothing has a CTA that writes its zeros
 __device__ __forceinline__ int paged_tiles(int len) { return max(1, (len + kPA_Tile - 1) / kPA_Tile); }
 
-// a CTA's walk over its run of tiles
+// a row's token of the chunk and its query head of the group
+__device__ __forceinline__ int2 paged_row(const PagedAttnArgs& a, int r) {
+  const int i = (int)(r * a.by_r >> 16);
+  return make_int2(i, r - i * a.R);
+}
+
+// a CTA's walk over its run of tiles; the run's first kPA_Seqs sequences are in shared memory, a load from L2 on every warp's
+// way to the next sequence would cost as much as half a tile
+constexpr int kPA_Seqs = 192;
 struct PagedWalk {
-  int b, c, g, tile, ntiles, len;
+  int b, c, g, tile, ntiles, len, slot;
+  int b0;
+  const int2* seqs;      // (slot, length) of sequences b0, b0 + 1, ...
+  __device__ __forceinline__ void enter(const PagedAttnArgs& a) {
+    const int2 x = b - b0 < kPA_Seqs ? seqs[b - b0] : paged_seq(a, b);
+    slot = x.x;
+    len = x.y;
+    ntiles = paged_tiles(len);
+  }
   __device__ __forceinline__ void next(const PagedAttnArgs& a) {
     if (++tile < ntiles) return;
     tile = 0;
@@ -80,10 +103,7 @@ struct PagedWalk {
     g = 0;
     if (++c < a.nqc) return;
     c = 0;
-    if (++b < a.B) {
-      len = paged_len(a, b);
-      ntiles = paged_tiles(len);
-    }
+    if (++b < a.B) enter(a);
   }
 };
 
@@ -129,16 +149,17 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
            *seg_full = bars + 36, *seg_free = bars + 38;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 40);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 41);
-  long long* s_sum = reinterpret_cast<long long*>(bars + 42);       // [20] per-warp totals of the tile count
-  int* s_start = reinterpret_cast<int*>(bars + 62);                 // b, segment of it, tile of that
-  float* s_qs = reinterpret_cast<float*>(bars + 64);                // [2][RP] scale of the Q rows
+  long long* s_sum = reinterpret_cast<long long*>(bars + 42);       // [20] per-warp totals of the unit count
+  int* s_start = reinterpret_cast<int*>(bars + 63);                 // b, segment of it, tile of that
+  float* s_qs = reinterpret_cast<float*>(bars + 65);                // [2][RP] scale of the Q rows
   float* s_fac = s_qs + 2 * kPA_MaxRows;                            // [2][RP][2] factors of the tile's O^T and the accumulators
   float* s_red = s_fac + 4 * kPA_MaxRows;                           // [2][4][RP] the warps' maxima
   float* s_seg = s_red + 8 * kPA_MaxRows;                           // [2][5][RP] a segment's sums per warp, its maximum
   float* s_sc = s_seg + 10 * kPA_MaxRows;                           // [4][20] scales of a tile's pages: 8 K, 8 V ratios, V's largest, mask
-  static_assert(64 * 8 + (2 + 4 + 8 + 10) * kPA_MaxRows * 4 + 80 * 4 <= 4096, "barriers and exchanges");
+  int2* s_seqs = reinterpret_cast<int2*>(s_sc + 80);                 // [kPA_Seqs]
+  static_assert(66 * 8 + (2 + 4 + 8 + 10) * kPA_MaxRows * 4 + 80 * 4 + kPA_Seqs * 8 <= 5120, "barriers and exchanges");
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < NU; ++i) {
       mbar_init(full + i, 1);
@@ -167,13 +188,14 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     tmem_alloc(tmem_slot, C::TmemCols);
     tmem_relinquish();
   }
-  // this CTA's run of tiles: the sequences' tile counts summed over the block, thread i holding per consecutive ones
+  // this CTA's run: every segment is one unit and one for each of its tiles.  The sequences' units are summed over the block,
+  // thread i holding `per` consecutive sequences
   const int per = (a.B + kPA_Threads - 1) / kPA_Threads;
   const int segs = a.nqc * a.p.heads;
   long long mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
-    if (b < a.B) mine += (long long)paged_tiles(paged_len(a, b)) * segs;
+    if (b < a.B) mine += (long long)(paged_tiles(paged_seq(a, b).y) + 1) * segs;
   }
   long long incl = mine;
 #pragma unroll
@@ -191,41 +213,56 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
   }
-  // with fewer tiles than CTAs the first `total` CTAs take one each: no CTA between two parts of a segment is idle
   const long long ctas = total < gridDim.x ? total : gridDim.x, x0 = min((long long)blockIdx.x, ctas);
   const long long u0 = total * x0 / ctas, u1 = total * min(x0 + 1, ctas) / ctas;
+  // the sequence, segment and tile of the first unit u0, and how many of the run's units are tiles
   if (u0 < u1 && before <= u0 && u0 < before + mine) {
     long long at = before;
     for (int b = tid * per;; ++b) {
-      const long long n = (long long)paged_tiles(paged_len(a, b)) * segs;
-      if (u0 < at + n) {
+      const int n = paged_tiles(paged_seq(a, b).y) + 1;
+      if (u0 < at + (long long)n * segs) {
         s_start[0] = b;
-        s_start[1] = (int)((u0 - at) / paged_tiles(paged_len(a, b)));
-        s_start[2] = (int)((u0 - at) % paged_tiles(paged_len(a, b)));
+        s_start[1] = (int)((u0 - at) / n);
+        s_start[2] = (int)((u0 - at) % n);
         break;
       }
-      at += n;
+      at += (long long)n * segs;
     }
   }
   __syncthreads();
-  const uint32_t tmem = *tmem_slot;
-  const int count = (int)(u1 - u0);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   PagedWalk w{};
-  if (count > 0) {
-    w.b = s_start[0];
+  int count = 0;                  // tiles of the run
+  if (u0 < u1) {
+    for (int i = tid; i < kPA_Seqs && s_start[0] + i < a.B; i += kPA_Threads) {
+      s_seqs[i] = paged_seq(a, s_start[0] + i);
+    }
+  }
+  __syncthreads();
+  if (u0 < u1) {
+    w.seqs = s_seqs;
+    w.b = w.b0 = s_start[0];
     w.c = s_start[1] / a.p.heads;
     w.g = s_start[1] % a.p.heads;
-    w.tile = s_start[2];
-    w.len = paged_len(a, w.b);
-    w.ntiles = paged_tiles(w.len);
+    w.enter(a);
+    w.tile = max(s_start[2] - 1, 0);
+    // walk the run's segments: the units of each that are tiles
+    PagedWalk x = w;
+    for (long long u = u0 - s_start[2]; u < u1;) {
+      const long long lo = max(u + 1, u0), hi = min(u + 1 + x.ntiles, u1);
+      if (hi > lo) count += (int)(hi - lo);
+      u += x.ntiles + 1;
+      x.tile = x.ntiles - 1;
+      x.next(a);
+    }
   }
-  const int L = a.p.page, ppt = kPA_Tile / L;       // pages per tile
+  count = __shfl_sync(0xffffffffu, count, 0);
+  const int L = a.p.page, ppt = kPA_Tile >> a.page_log;       // pages per tile
   // the page of this tile's page number `i`, -1 where there is none
   auto page_of = [&](const PagedWalk& x, int i) -> int {
     const int j = x.tile * ppt + i;
     if (i >= ppt || (long long)j * L >= x.len) return -1;
-    const int slot = a.slots ? a.slots[x.b] : x.b;
-    const int page = a.p.table[(size_t)slot * a.p.width + j];
+    const int page = a.p.table[(size_t)x.slot * a.p.width + j];
     return page >= 0 && page < a.p.pages ? page : -1;
   };
 
@@ -235,20 +272,25 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       tma_prefetch(&kmap);
       tma_prefetch(&vmap);
     }
-    int unit = 0;
+    int unit = 0, u = 0, uphase = 1;      // uphase: the parity of the round before
     bool ok = true;
     int page = count > 0 ? page_of(w, lane) : -1;
+#pragma unroll 1
     for (int j = 0; j < count && ok; ++j) {
       const int g = w.g, now = page;
+      float ks = 0.f, vs = 0.f;
+      if (now >= 0) {
+        ks = a.p.ks[(size_t)now * a.p.heads + g];
+        vs = a.p.vs[(size_t)now * a.p.heads + g];
+      }
       if (j + 1 < count) {       // the next tile's page numbers, on their way during this one's loads
         w.next(a);
         page = page_of(w, lane);
       }
       const unsigned have = __ballot_sync(0xffffffffu, now >= 0);
-      for (int kv = 0; kv < 2 && ok; ++kv, ++unit) {
-        const int u = unit % NU, round = unit / NU;
-        if (round > 0) ok = mbar_wait_warp(empty + u, (round - 1) & 1, abort_flag, a.err, 0x60);
-        if (!ok) break;
+#pragma unroll 1
+      for (int kv = 0; kv < 2; ++kv, ++unit) {
+        if (unit >= NU && !(ok = mbar_wait_warp_small(empty + u, uphase, abort_flag, 0x60))) break;
         if (lane == 0) {
           if (have) mbar_expect_tx(full + u, (uint32_t)__popc(have) * L * kPG_D); else mbar_arrive(full + u);
         }
@@ -259,125 +301,16 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
           tma_load_2d(dst, kv ? &vmap : &kmap, full + u, 0, row);
           tma_load_2d(dst + kPA_Tile * 128, kv ? &vmap : &kmap, full + u, 128, row);
         }
-      }
-    }
-    // every load issued has landed before the CTA may exit
-    for (int i = unit > NU ? unit - NU : 0; i < unit; ++i) mbar_wait(full + i % NU, (i / NU) & 1, nullptr, a.err, 0x61);
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc_e4m3(kPA_Tile, NP), id_o = idesc_e4m3(128, NP) | kIdescAMn;
-      int seg = 0;
-      bool ok = true, first = true;
-      auto pv = [&](int j) -> bool {
-        const int u = (2 * j + 1) % NU, s = j & 1;
-        if (!mbar_wait(p_full + s, (j >> 1) & 1, abort_flag, a.err, 0x62)) return false;
-        if (!mbar_wait(full + u, ((2 * j + 1) / NU) & 1, abort_flag, a.err, 0x63)) return false;
-        if (j >= 2 && !mbar_wait(o_free + s, ((j >> 1) - 1) & 1, abort_flag, a.err, 0x64)) return false;
-        tc_fence_after();
-        const uint32_t v = smem_u32(ring + u * kPA_Unit), p = smem_u32(sP + s * C::PBytes);
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            umma_f8_ss(tmem + 2 * NP + (2 * s + half) * NP, sdesc_sw128_mn(v + half * 16384 + ks * 4096, 16384),
-                       sdesc_kstep(p, NP, ks), id_o, ks > 0);
-        umma_commit(o_full + s);
-        umma_commit(empty + u);
-        return true;
-      };
-      for (int j = 0; j < count && ok; ++j) {
-        const int u = (2 * j) % NU, s = j & 1;
-        if (first && !(ok = mbar_wait(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, a.err, 0x65))) break;
-        if (!(ok = mbar_wait(full + u, ((2 * j) / NU) & 1, abort_flag, a.err, 0x66))) break;
-        if (j >= 2 && !(ok = mbar_wait(s_free + s, ((j >> 1) - 1) & 1, abort_flag, a.err, 0x67))) break;
-        tc_fence_after();
-        const uint32_t k = smem_u32(ring + u * kPA_Unit), q = smem_u32(sQ + (seg & 1) * C::QBytes);
-#pragma unroll
-        for (int ks = 0; ks < kPG_D / 32; ++ks)
-          umma_f8_ss(tmem + s * NP, sdesc_kstep(k, kPA_Tile, ks), sdesc_kstep(q, NP, ks), id_s, ks > 0);
-        umma_commit(s_full + s);
-        umma_commit(empty + u);
-        first = w.tile + 1 == w.ntiles;
-        if (first || j + 1 == count) {
-          umma_commit(q_free + (seg & 1));
-          ++seg;
+        if (++u == NU) {
+          u = 0;
+          uphase ^= 1;
         }
-        w.next(a);
-        if (j >= 1) ok = pv(j - 1);
       }
-      if (ok && count > 0) pv(count - 1);
-    }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------------ Q parts of each segment
-    bool ok = true;
-    int seg = 0;
-    for (int j = 0; j < count && ok;) {
-      if (seg >= 2 && !(ok = mbar_wait_warp(q_free + (seg & 1), ((seg >> 1) - 1) & 1, abort_flag, a.err, 0x68))) break;
-      uint8_t* dst = sQ + (seg & 1) * C::QBytes;
-      const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
-#pragma unroll 4
-      for (int r = 0; r < RP; ++r) {
-        uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows)
-          raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + w.b * a.q_sb + (long long)(i0 + r / a.R) * a.q_st +
-                                                     (long long)(w.g * a.R + r % a.R) * a.q_sh + 8 * lane));
-        const T* e = reinterpret_cast<const T*>(&raw);
-        float x[8], m = 0.f;
-        bool fin = true;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = (float)e[i];
-          fin = fin && fabsf(x[i]) < INFINITY;
-          m = fmaxf(m, fabsf(x[i]));
-        }
-        m = warp_max(m);
-        fin = __all_sync(0xffffffffu, fin);
-        // the row's largest value to [128, 256): x * 2^k, k = 7 - exponent
-        const int ex = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 16) : 127;
-        const float up = fin ? __uint_as_float((uint32_t)(254 + 7 - ex) << 23) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fin ? x[i] * up : 0.f;
-        uint16_t c[4][3];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) split3(x[2 * i], x[2 * i + 1], c[i]);
-#pragma unroll
-        for (int part = 0; part < 3; ++part) {
-          const int n = part * RP + row_col<RP>(r);
-          const uint32_t chunk = ((lane & 15) >> 1) ^ (n & 7);
-          *reinterpret_cast<uint2*>(dst + (lane >> 4) * (NP * 128) + n * 128 + chunk * 16 + (lane & 1) * 8) =
-              make_uint2(c[0][part] | ((uint32_t)c[1][part] << 16), c[2][part] | ((uint32_t)c[3][part] << 16));
-        }
-        // a row with a value that is not finite has no finite scores
-        if (lane == 0) s_qs[(seg & 1) * RP + row_col<RP>(r)] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full + (seg & 1));
-      ++seg;
-      const int left = w.ntiles - w.tile;        // on to the next segment
-      j += left;
-      w.tile = w.ntiles - 1;
-      w.next(a);
-    }
-  } else if (warp == 3) {
-    // ------------------------------------------------------------------ scales of each tile's pages
-    bool ok = true;
-    int page = count > 0 ? page_of(w, lane) : -1;
-    for (int j = 0; j < count && ok; ++j) {
-      const int s = j & 3, now = page, g = w.g;
-      float ks = 0.f, vs = 0.f;
-      if (now >= 0) {
-        ks = a.p.ks[(size_t)now * a.p.heads + g];
-        vs = a.p.vs[(size_t)now * a.p.heads + g];
-      }
-      if (j + 1 < count) {
-        w.next(a);
-        page = page_of(w, lane);
-      }
+      if (!ok) break;
+      // the tile's scales, their loads as old as its TMA's
+      const int s = j & 3;
       const float top = warp_max(vs);
-      const unsigned have = __ballot_sync(0xffffffffu, now >= 0);
-      if (j >= 4 && !(ok = mbar_wait_warp(sc_free + s, ((j >> 2) - 1) & 1, abort_flag, a.err, 0x69))) break;
+      if (j >= 4 && !(ok = mbar_wait_warp_small(sc_free + s, ((j >> 2) - 1) & 1, abort_flag, 0x69))) break;
       if (lane < 8) {
         s_sc[s * 20 + lane] = ks;
         s_sc[s * 20 + 8 + lane] = top > 0.f ? vs / top : 0.f;      // powers of two: exact
@@ -389,6 +322,142 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_full + s);
     }
+    // every load issued has landed before the CTA may exit: the products have read it, or it is waited for here
+    if (*abort_flag) {
+      for (int i = unit > NU ? unit - NU : 0; i < unit; ++i) mbar_wait(full + i % NU, (i / NU) & 1, nullptr, a.err, 0x61);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ S = K Q^T
+    constexpr uint32_t id_s = idesc_e4m3(kPA_Tile, NP);
+    const uint64_t dk0 = sdesc_sw128(smem_u32(ring)), dq0 = sdesc_sw128(smem_u32(sQ));
+    int seg = 0, u = 0, uphase = 0;
+    bool first = true;
+#pragma unroll 1
+    for (int j = 0; j < count; ++j) {
+      const int s = j & 1;
+      if (first && !mbar_wait_warp_small(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, 0x65)) break;
+      if (!mbar_wait_warp_small(full + u, uphase, abort_flag, 0x66)) break;
+      if (j >= 2 && !mbar_wait_warp_small(s_free + s, ((j >> 1) - 1) & 1, abort_flag, 0x67)) break;
+      tc_fence_after();
+      first = w.tile + 1 == w.ntiles;
+      const bool end = first || j + 1 == count;
+      if (elect_one()) {
+        const uint64_t dk = dk0 + (uint32_t)(u * (kPA_Unit >> 4)), dq = dq0 + (uint32_t)((seg & 1) * (C::QBytes >> 4));
+#pragma unroll
+        for (int ks = 0; ks < kPG_D / 32; ++ks)
+          umma_f8_ss(tmem + s * NP, dk + ((ks >> 2) * (kPA_Tile * 128) + (ks & 3) * 32) / 16,
+                     dq + ((ks >> 2) * (NP * 128) + (ks & 3) * 32) / 16, id_s, ks > 0);
+        umma_commit(s_full + s);
+        umma_commit(empty + u);
+        if (end) umma_commit(q_free + (seg & 1));
+      }
+      __syncwarp();
+      seg += end;
+      w.next(a);
+      u += 2;
+      if (u >= NU) {
+        u -= NU;
+        uphase ^= 1;
+      }
+    }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ O = V^T P^T
+    constexpr uint32_t id_o = idesc_e4m3(128, NP) | kIdescAMn;
+    const uint64_t dv0 = sdesc_sw128_mn(smem_u32(ring), 16384), dp0 = sdesc_sw128(smem_u32(sP));
+    int u = 1, uphase = 0;
+#pragma unroll 1
+    for (int j = 0; j < count; ++j) {
+      const int s = j & 1;
+      if (!mbar_wait_warp_small(full + u, uphase, abort_flag, 0x63)) break;
+      if (!mbar_wait_warp_small(p_full + s, (j >> 1) & 1, abort_flag, 0x62)) break;
+      if (j >= 2 && !mbar_wait_warp_small(o_free + s, ((j >> 1) - 1) & 1, abort_flag, 0x64)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t dv = dv0 + (uint32_t)(u * (kPA_Unit >> 4)), dp = dp0 + (uint32_t)(s * (C::PBytes >> 4));
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+            umma_f8_ss(tmem + 2 * NP + (2 * s + half) * NP, dv + (half * 16384 + ks * 4096) / 16, dp + ks * 32 / 16, id_o, ks > 0);
+        umma_commit(o_full + s);
+        umma_commit(empty + u);
+      }
+      __syncwarp();
+      u += 2;
+      if (u >= NU) {
+        u -= NU;
+        uphase ^= 1;
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ Q parts of each segment
+    bool ok = true;
+    int seg = 0;
+#pragma unroll 1
+    for (int j = 0; j < count && ok;) {
+      if (seg >= 2 && !(ok = mbar_wait_warp_small(q_free + (seg & 1), ((seg >> 1) - 1) & 1, abort_flag, 0x68))) break;
+      uint8_t* dst = sQ + (seg & 1) * C::QBytes;
+      const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
+      // two rows at a time, 16 lanes each, every load of four rows before their arithmetic; rows from `rows` on stay as they are,
+      // nothing reads their scores
+      const int r2 = lane >> 4, dim = (lane & 15) * 16;
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 4) {
+        uint4 raw[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = min(r0 + 2 * i + r2, rows - 1);
+          const int2 ih = paged_row(a, r);
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + w.b * a.q_sb + (long long)(i0 + ih.x) * a.q_st +
+                                                            (long long)(w.g * a.R + ih.y) * a.q_sh + dim);
+          raw[i][0] = __ldg(src);
+          raw[i][1] = __ldg(src + 1);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = min(r0 + 2 * i + r2, rows - 1);       // the last row may be written twice, with the same values
+          const T* e = reinterpret_cast<const T*>(raw[i]);
+          float m = 0.f;
+          bool fin = true;
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const float x = fabsf((float)e[q]);
+            fin = fin && x < INFINITY;
+            m = fmaxf(m, x);
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          fin = ((__ballot_sync(0xffffffffu, fin) >> (lane & 16)) & 0xffffu) == 0xffffu;
+          // the row's largest value to [128, 256): x * 2^k, k = 7 - exponent
+          const int ex = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 16) : 127;
+          const float up = fin ? __uint_as_float((uint32_t)(254 + 7 - ex) << 23) : 0.f;
+          uint32_t word[3][4];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            uint16_t c[3];
+            split3(fin ? (float)e[2 * q] * up : 0.f, fin ? (float)e[2 * q + 1] * up : 0.f, c);
+#pragma unroll
+            for (int part = 0; part < 3; ++part) word[part][q >> 1] = q & 1 ? word[part][q >> 1] | ((uint32_t)c[part] << 16) : c[part];
+          }
+#pragma unroll
+          for (int part = 0; part < 3; ++part) {
+            const int n = part * RP + row_col<RP>(r);
+            *reinterpret_cast<uint4*>(dst + (dim >> 7) * (NP * 128) + n * 128 + ((((dim & 127) >> 4) ^ (n & 7)) << 4)) =
+                make_uint4(word[part][0], word[part][1], word[part][2], word[part][3]);
+          }
+          // a row with a value that is not finite has no finite scores
+          if ((lane & 15) == 0) s_qs[(seg & 1) * RP + row_col<RP>(r)] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + (seg & 1));
+      ++seg;
+      const int left = w.ntiles - w.tile;        // on to the next segment
+      j += left;
+      w.tile = w.ntiles - 1;
+      w.next(a);
+    }
   } else if (warp < 12) {
     // ------------------------------------------------------------------ softmax: thread = token of the tile, rows 2 i + hh
     constexpr int RH = RP / 2;
@@ -399,10 +468,11 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     float m_run = -INFINITY;             // of row 2 lane + hh, in lanes < RH
     bool ok = true, first = true;
     int seg = 0;
+#pragma unroll 1
     for (int j = 0; j < count; ++j) {
       const int s = j & 1;
       if (first) {
-        if (!(ok = mbar_wait_warp(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, a.err, 0x6a))) break;
+        if (!(ok = mbar_wait_warp_small(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, 0x6a))) break;
         const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
         m_run = -INFINITY;
 #pragma unroll
@@ -410,22 +480,22 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
           const int r = 2 * i + hh;
           l[i] = 0.f;
           qs[i] = s_qs[(seg & 1) * RP + hh * RH + i];
-          lim[i] = r < rows ? w.len - a.t + i0 + r / a.R : -1;     // the row's last visible position
+          lim[i] = r < rows ? w.len - a.t + i0 + paged_row(a, r).x : -1;     // the row's last visible position
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(q_free + (seg & 1));
       }
       const bool last = w.tile + 1 == w.ntiles, end = last || j + 1 == count;
-      if (!(ok = mbar_wait_warp(sc_full + (j & 3), (j >> 2) & 1, abort_flag, a.err, 0x6b))) break;
+      if (!(ok = mbar_wait_warp_small(sc_full + (j & 3), (j >> 2) & 1, abort_flag, 0x6b))) break;
       const float* sc = s_sc + (j & 3) * 20;
-      const int pi = tok / L;
+      const int pi = tok >> a.page_log;
       const float ks = sc[pi], vr = sc[8 + pi] * 256.f, top = sc[16];
       const bool there = (__float_as_uint(sc[17]) >> pi) & 1u;
       const int pos = w.tile * kPA_Tile + tok;
       const bool valid = there && pos < w.len;
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_free + (j & 3));
-      if (!(ok = mbar_wait_warp(s_full + s, (j >> 1) & 1, abort_flag, a.err, 0x6c))) break;
+      if (!(ok = mbar_wait_warp_small(s_full + s, (j >> 1) & 1, abort_flag, 0x6c))) break;
       tc_fence_after();
       uint32_t raw[3 * RH];
 #pragma unroll
@@ -451,7 +521,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       if (lane < RH) rd[wq * RP + lane] = mine;
       __syncwarp();
       if (lane == 0) mbar_arrive(red + hh);
-      if (!(ok = mbar_wait_warp(red + hh, j & 1, abort_flag, a.err, 0x6d))) break;
+      if (!(ok = mbar_wait_warp_small(red + hh, j & 1, abort_flag, 0x6d))) break;
       // lane i: row 2 i + hh's maximum of the tile, and the factors of what was before and of this tile
       float mt = -INFINITY;
       if (lane < RH) mt = fmaxf(fmaxf(rd[lane], rd[RP + lane]), fmaxf(rd[2 * RP + lane], rd[3 * RP + lane]));
@@ -461,7 +531,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       m_run = mn;
       mt = mt == -INFINITY ? 0.f : mt;
       // P of the tile before the last but one has been read, and so have its factors
-      if (j >= 2 && !(ok = mbar_wait_warp(o_free + s, ((j >> 1) - 1) & 1, abort_flag, a.err, 0x6e))) break;
+      if (j >= 2 && !(ok = mbar_wait_warp_small(o_free + s, ((j >> 1) - 1) & 1, abort_flag, 0x6e))) break;
       if (wq == 0 && lane < RH)
         *reinterpret_cast<float2*>(s_fac + (s * RP + hh * RH + lane) * 2) = make_float2(al, f * top * (1.f / 256.f));
       uint8_t* pd = sP + s * C::PBytes;
@@ -490,7 +560,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       if (__any_sync(0xffffffffu, !valid)) {
         // the values of tokens that are not there may be anything (a weight of 0 times NaN would be NaN): zeros
         const int u = (2 * j + 1) % NU;
-        if (!(ok = mbar_wait_warp(full + u, ((2 * j + 1) / NU) & 1, abort_flag, a.err, 0x6f))) break;
+        if (!(ok = mbar_wait_warp_small(full + u, ((2 * j + 1) / NU) & 1, abort_flag, 0x6f))) break;
         if (!valid) {
           uint4* row = reinterpret_cast<uint4*>(ring + u * kPA_Unit + hh * (kPA_Tile * 128) + tok * 128);
 #pragma unroll
@@ -501,7 +571,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full + s);
       if (end) {
-        if (seg >= 2 && !(ok = mbar_wait_warp(seg_free + (seg & 1), ((seg >> 1) - 1) & 1, abort_flag, a.err, 0x70))) break;
+        if (seg >= 2 && !(ok = mbar_wait_warp_small(seg_free + (seg & 1), ((seg >> 1) - 1) & 1, abort_flag, 0x70))) break;
         float* sg = s_seg + (seg & 1) * 5 * RP + hh * RH;
 #pragma unroll
         for (int i = 0; i < RH; ++i) {
@@ -523,13 +593,15 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     float acc[RP];
     bool ok = true, from_start = w.tile == 0;
     int seg = 0;
+    long long unit = u0 + (count > 0 && s_start[2] == 0 ? 1 : 0);      // the tile's
     int4 desc = make_int4(-1, 0, 0, 0);
 #pragma unroll
     for (int c = 0; c < RP; ++c) acc[c] = 0.f;
+#pragma unroll 1
     for (int j = 0; j < count; ++j) {
       const int s = j & 1;
-      if (!(ok = mbar_wait_warp(p_full + s, (j >> 1) & 1, abort_flag, a.err, 0x73))) break;   // the factors
-      if (!(ok = mbar_wait_warp(o_full + s, (j >> 1) & 1, abort_flag, a.err, 0x71))) break;
+      if (!(ok = mbar_wait_warp_small(p_full + s, (j >> 1) & 1, abort_flag, 0x73))) break;   // the factors
+      if (!(ok = mbar_wait_warp_small(o_full + s, (j >> 1) & 1, abort_flag, 0x71))) break;
       tc_fence_after();
       uint32_t raw[3 * RP];
 #pragma unroll
@@ -546,83 +618,105 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       if (lane == 0) mbar_arrive(o_free + s);
       const bool last = w.tile + 1 == w.ntiles;
       if (last || j + 1 == count) {
-        if (!(ok = mbar_wait_warp(seg_full + (seg & 1), (seg >> 1) & 1, abort_flag, a.err, 0x72))) break;
+        if (!(ok = mbar_wait_warp_small(seg_full + (seg & 1), (seg >> 1) & 1, abort_flag, 0x72))) break;
         const float* sg = s_seg + (seg & 1) * 5 * RP;
         const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
         const bool whole = from_start && last;
         float* part = a.part + ((size_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * RP * kPA_Part;
-#pragma unroll
+        // one copy of the code for all rows: the accumulators move up by one per row
+#pragma unroll 1
         for (int c = 0; c < RP; ++c) {
           const int r = col_row<RP>(c);
           if (r < rows) {
             const float sum = (sg[c] + sg[RP + c]) + (sg[2 * RP + c] + sg[3 * RP + c]), m = sg[4 * RP + c];
             if (whole) {
-              const int i = i0 + r / a.R, h = w.g * a.R + r % a.R;
+              const int2 ih = paged_row(a, r);
+              const int i = i0 + ih.x, h = w.g * a.R + ih.y;
               const float inv = sum == 0.f ? 0.f : 1.f / sum;       // nothing seen: zeros
-              static_cast<T*>(a.o)[(((size_t)w.b * a.t + i) * a.H + h) * kPG_D + d] = (T)(acc[c] * inv);
+              static_cast<T*>(a.o)[(((size_t)w.b * a.t + i) * a.H + h) * kPG_D + d] = (T)(acc[0] * inv);
               if (a.lse && d == 0) a.lse[((size_t)w.b * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
             } else {
-              part[r * kPA_Part + d] = acc[c];
+              part[r * kPA_Part + d] = acc[0];
               if (d == 0) {
                 part[r * kPA_Part + kPG_D] = m;
                 part[r * kPA_Part + kPG_D + 1] = sum;
               }
             }
           }
-          acc[c] = 0.f;
+#pragma unroll
+          for (int k = 0; k + 1 < RP; ++k) acc[k] = acc[k + 1];
+          acc[RP - 1] = 0.f;
         }
         // a cut segment that ends here: the CTA that holds its first tile
         if (last && !from_start) {
-          const long long t0 = u0 + j - (w.ntiles - 1);
+          const long long t0 = unit - (w.ntiles - 1);
           desc = make_int4((int)(((t0 + 1) * ctas - 1) / total), w.b, w.c, w.g);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(seg_free + (seg & 1));
         ++seg;
         from_start = true;
+        ++unit;                  // the next segment's start
       }
+      ++unit;
       w.next(a);
     }
     if (d == 0) a.desc[blockIdx.x] = ok ? desc : make_int4(-1, 0, 0, 0);
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0) report_abort(abort_flag, a.err);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TmemCols);
   }
 }
 
-// Block (x, r): row r of the cut segment that ends in CTA x, if there is one: the partials of the CTAs first .. x, in order
+// Block (x, r, z): dims 64 z .. 64 z + 63 of row r of the cut segment that ends in CTA x, if there is one: the partials of the
+// CTAs first .. x, a quarter of them per group of 64 threads, then the four groups' results, always in the same order
 template <typename T, int RP>
 __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttnArgs a) {
-  const int x = blockIdx.x, r = blockIdx.y, d = threadIdx.x;
+  __shared__ float s_m[4], s_l[4], s_acc[4][64];
+  const int x = blockIdx.x, r = blockIdx.y, grp = threadIdx.x >> 6, d = blockIdx.z * 64 + (threadIdx.x & 63);
   const int4 desc = a.desc[x];
   if (desc.x < 0) return;
   const int i0 = desc.z * a.tc;
   if (r >= min(a.tc, a.t - i0) * a.R) return;
+  const int n = x - desc.x + 1, each = (n + 3) / 4, c_end = min(desc.x + (grp + 1) * each, x + 1);
   auto part = [&](int c) { return a.part + (((size_t)c * 2 + (c == desc.x ? 1 : 0)) * RP + r) * kPA_Part; };
   float m = -INFINITY, sum = 0.f, acc = 0.f;
-  for (int c0 = desc.x; c0 <= x; c0 += 8) {
-    float mv[8], lv[8], av[8];
+  // a partial without a maximum holds zeros, or NaN to be passed on
+  auto add = [&](float mv, float lv, float av) {
+    const float mn = fmaxf(m, mv);
+    const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = mv == -INFINITY ? 1.f : ex2_approx(mv - mn);
+    acc = acc * al + av * f;
+    sum = sum * al + lv * f;
+    m = mn;
+  };
+  for (int c0 = desc.x + grp * each; c0 < c_end; c0 += 16) {
+    float mv[16], lv[16], av[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
       const float* p = part(min(c0 + i, x));
-      const bool in = c0 + i <= x;
+      const bool in = c0 + i < c_end;
       av[i] = in ? p[d] : 0.f;
       mv[i] = in ? p[kPG_D] : -INFINITY;
       lv[i] = in ? p[kPG_D + 1] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float mn = fmaxf(m, mv[i]);
-      const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = mv[i] == -INFINITY ? 1.f : ex2_approx(mv[i] - mn);
-      acc = acc * al + av[i] * f;       // a partial without a maximum holds zeros, or NaN to be passed on
-      sum = sum * al + lv[i] * f;
-      m = mn;
-    }
+    for (int i = 0; i < 16; ++i) add(mv[i], lv[i], av[i]);
   }
-  const int i = i0 + r / a.R, h = desc.w * a.R + r % a.R;
+  s_acc[grp][threadIdx.x & 63] = acc;
+  if ((threadIdx.x & 63) == 0) {
+    s_m[grp] = m;
+    s_l[grp] = sum;
+  }
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) add(s_m[i], s_l[i], s_acc[i][threadIdx.x]);
+  const int2 ih = paged_row(a, r);
+  const int i = i0 + ih.x, h = desc.w * a.R + ih.y;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   static_cast<T*>(a.o)[(((size_t)desc.y * a.t + i) * a.H + h) * kPG_D + d] = (T)(acc * inv);
   if (a.lse && d == 0) a.lse[((size_t)desc.y * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
@@ -642,7 +736,7 @@ static int launch_paged(const CUtensorMap& kmap, const CUtensorMap& vmap, const 
   if (rc) return rc;
   paged_attn_kernel<T, RP><<<ctas, kPA_Threads, PagedCfg<RP>::Smem, stream>>>(kmap, vmap, a);
   if ((rc = launch_status())) return rc;
-  paged_combine_kernel<T, RP><<<dim3(ctas, a.tc * a.R), 256, 0, stream>>>(a);
+  paged_combine_kernel<T, RP><<<dim3(ctas, a.tc * a.R, kPG_D / 64), 256, 0, stream>>>(a);
   return launch_status();
 }
 
@@ -681,6 +775,9 @@ int bf_paged_attend(const bf_page_pool* pool, int layer, const void* q, long lon
   a.B = B; a.t = t; a.H = H; a.R = H / a.p.heads;
   int rp;
   paged_chunks(t, a.R, &a.tc, &a.nqc, &rp);
+  a.page_log = a.p.page == 16 ? 4 : a.p.page == 32 ? 5 : a.p.page == 64 ? 6 : 7;
+  a.cap = (int)((long long)a.p.width * a.p.page < 0x7fffffffLL ? (long long)a.p.width * a.p.page : 0x7fffffffLL);
+  a.by_r = (65536u + a.R - 1) / a.R;
   a.c2 = scale * kLog2e;
   a.o = o;
   a.lse = lse;

@@ -199,12 +199,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       int t = 0;
       bool ok = true;
       for (int it = 0; it < items && ok; ++it) {
-        if (it >= 1 && !(ok = mbar_wait(q_free, (it - 1) & 1, abort_flag, a.err, 0x80))) break;
+        if (it >= 1 && !(ok = mbar_wait_small(q_free, (it - 1) & 1, abort_flag, 0x80))) break;
         mbar_expect_tx_cluster(qf, kPR_SmemQ);
         tma_load_4d_pair(sQ, &qmap, qf, 0, blk.q0 + i0, 0, head(it));
         for (int j = 0; j < n; ++j, ++t) {
           const int s = t & 1;
-          if (t >= 2 && !(ok = mbar_wait(k_empty + s, ((t >> 1) - 1) & 1, abort_flag, a.err, 0x81))) break;
+          if (t >= 2 && !(ok = mbar_wait_small(k_empty + s, ((t >> 1) - 1) & 1, abort_flag, 0x81))) break;
           mbar_expect_tx_cluster(kf[s], kPR_SmemK);
           tma_load_4d_pair(sK + s * kPR_SmemK, &kmap, kf[s], 0, blk.k0 + j * kPR_N + (int)rank * (kPR_N / 2), 0, g);
         }
@@ -218,7 +218,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       for (int it = 0; it < items && ok; ++it) {
         for (int j = 0; j < n; ++j, ++t) {
           const int s = t & 1, rows = blk.nk - j * kPR_N;   // rows of the tile that are this sequence's
-          if (t >= 2 && !(ok = mbar_wait_warp(v_empty + s, ((t >> 1) - 1) & 1, abort_flag, a.err, 0x82))) break;
+          if (t >= 2 && !(ok = mbar_wait_warp_small(v_empty + s, ((t >> 1) - 1) & 1, abort_flag, 0x82))) break;
           uint8_t* dst = sV + s * kPR_SmemV;
           const bool whole = rows >= kPR_N;
           if (lane == 0) {
@@ -228,7 +228,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           __syncwarp();
           if (!whole) {
             // the rows behind the sequence belong to others: their weights are 0, but 0 times NaN would not be
-            if (!(ok = mbar_wait_warp(v_own, own & 1, abort_flag, a.err, 0x83))) break;
+            if (!(ok = mbar_wait_warp_small(v_own, own & 1, abort_flag, 0x83))) break;
             ++own;
             for (int i = lane; i < (kPR_N - rows) * 8; i += 32) {
               uint4* p = reinterpret_cast<uint4*>(dst + rows * 128) + i;
@@ -248,12 +248,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       int t = 0;
       bool ok = true;
       for (int it = 0; it < items && ok; ++it) {
-        if (!(ok = mbar_wait(q_full, it & 1, abort_flag, a.err, 0x84))) break;
+        if (!(ok = mbar_wait_small(q_full, it & 1, abort_flag, 0x84))) break;
         auto pv = [&](int j, int tt) -> bool {
           const int s = tt & 1;
-          if (!mbar_wait(p_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x85)) return false;
-          if (!mbar_wait(v_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x86)) return false;
-          if (j == 0 && it >= 1 && !mbar_wait(o_free, (it - 1) & 1, abort_flag, a.err, 0x87)) return false;
+          if (!mbar_wait_small(p_full + s, (tt >> 1) & 1, abort_flag, 0x85)) return false;
+          if (!mbar_wait_small(v_full + s, (tt >> 1) & 1, abort_flag, 0x86)) return false;
+          if (j == 0 && it >= 1 && !mbar_wait_small(o_free, (it - 1) & 1, abort_flag, 0x87)) return false;
           tc_fence_after();
           const uint32_t bV = smem_u32(sV + s * kPR_SmemV);
 #pragma unroll
@@ -265,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
         };
         for (int j = 0; j < n && ok; ++j) {
           const int tt = t + j, s = tt & 1;
-          if (!(ok = mbar_wait(k_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x88))) break;
+          if (!(ok = mbar_wait_small(k_full + s, (tt >> 1) & 1, abort_flag, 0x88))) break;
           tc_fence_after();
           const uint32_t bK = smem_u32(sK + s * kPR_SmemK);
 #pragma unroll
@@ -281,7 +281,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           if (!(ok = pv(n - 1, t + n - 1))) break;
         } else {
           // O counts as complete only once the item before has been drained, products or not
-          if (it >= 1 && !(ok = mbar_wait(o_free, (it - 1) & 1, abort_flag, a.err, 0x87))) break;
+          if (it >= 1 && !(ok = mbar_wait_small(o_free, (it - 1) & 1, abort_flag, 0x87))) break;
           umma_commit_pair(q_free);
         }
         umma_commit_pair(o_fin);
@@ -305,7 +305,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       float m_ref = -INFINITY, l = 0.f;           // running maximum (log2 domain) and this half's sum
       for (int j = 0; j < n; ++j) {
         const int tt = t + j, s = tt & 1;
-        if (!mbar_wait_warp(s_full + s, (tt >> 1) & 1, abort_flag, a.err, 0x89)) { alive = false; break; }
+        if (!mbar_wait_warp_small(s_full + s, (tt >> 1) & 1, abort_flag, 0x89)) { alive = false; break; }
         tc_fence_after();
         float uu[NH];
         {
@@ -337,7 +337,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
         xm[hh * 128 + r] = mown;
         __syncwarp();
         if (lane == 0) mbar_arrive(&pair[q4]);
-        if (!mbar_wait_warp(&pair[q4], pair_phase++ & 1, abort_flag, a.err, 0x8a)) { alive = false; break; }
+        if (!mbar_wait_warp_small(&pair[q4], pair_phase++ & 1, abort_flag, 0x8a)) { alive = false; break; }
         const float mt = fmaxf(mown, xm[(1 - hh) * 128 + r]) * a.c2;
         float factor = 1.f;
         bool rescale = false;
@@ -364,7 +364,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
         }
         // O rescale (warp-collective), from the item's second tile on: after O += P_{j-1} V_{j-1} has finished
         if (j >= 1 && __any_sync(0xffffffffu, rescale)) {
-          if (!mbar_wait_warp(v_empty + ((tt - 1) & 1), ((tt - 1) >> 1) & 1, abort_flag, a.err, 0x8b)) { alive = false; break; }
+          if (!mbar_wait_warp_small(v_empty + ((tt - 1) & 1), ((tt - 1) >> 1) & 1, abort_flag, 0x8b)) { alive = false; break; }
           tc_fence_after();
 #pragma unroll 1
           for (int c = hh * 128; c < hh * 128 + 128; c += 32) {
@@ -386,7 +386,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       t += n;
       // the row's statistics for the output warps (slot it & 1, free once they read item it - 2's)
       const int slot = it & 1;
-      if (it >= 2 && !(alive = mbar_wait_warp(&sfree[slot], ((it >> 1) - 1) & 1, abort_flag, a.err, 0x8c))) break;
+      if (it >= 2 && !(alive = mbar_wait_warp_small(&sfree[slot], ((it >> 1) - 1) & 1, abort_flag, 0x8c))) break;
       xl[slot * 256 + hh * 128 + r] = l;
       if (hh == 0) xmx[slot * 128 + r] = m_ref;
       __syncwarp();
@@ -400,9 +400,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
     const uint32_t of = cluster_addr(o_free, 0);
     const bool store = i0 + r < blk.nq;
     for (int it = 0; it < items; ++it) {
-      if (!mbar_wait_warp(o_fin, it & 1, abort_flag, a.err, 0x8d)) break;
+      if (!mbar_wait_warp_small(o_fin, it & 1, abort_flag, 0x8d)) break;
       const int slot = it & 1;
-      if (!mbar_wait_warp(&stats[slot], (it >> 1) & 1, abort_flag, a.err, 0x8e)) break;
+      if (!mbar_wait_warp_small(&stats[slot], (it >> 1) & 1, abort_flag, 0x8e)) break;
       const float l = xl[slot * 256 + r] + xl[slot * 256 + 128 + r], m = xmx[slot * 128 + r];
       __syncwarp();
       if (lane == 0) mbar_arrive(&sfree[slot]);
@@ -435,14 +435,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       if (lane == 0) mbar_arrive_cluster(of);
     }
   }
-  if (*abort_flag) {   // a wait gave up: time for the copies and products in flight to end
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < 1000000ull) {
-    }
-  }
   // neither CTA leaves while the other's products may read its shared memory or arrive on its barriers
   tc_fence_before();
   __syncthreads();
+  if (tid == 0) report_abort(abort_flag, a.err);
   cluster_sync();
   if (warp == 1) {
     tc_fence_after();
