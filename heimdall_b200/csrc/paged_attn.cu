@@ -274,20 +274,41 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     }
     int unit = 0, u = 0, uphase = 1;      // uphase: the parity of the round before
     bool ok = true;
-    int page = count > 0 ? page_of(w, lane) : -1;
+    // each lane a page of the tile: page numbers are loaded two tiles ahead, scales one, so that no load is waited for here
+    int now = -1, next = -1, g = 0, g_next = 0, ahead = 0;
+    float ks_next = 0.f, vs_next = 0.f;
+    auto step = [&]() {                   // the walk's next tile into (next, g_next)
+      next = -1;
+      if (ahead < count) {
+        g_next = w.g;
+        next = page_of(w, lane);
+        w.next(a);
+      }
+      ++ahead;
+    };
+    auto scales = [&]() {
+      ks_next = vs_next = 0.f;
+      if (now >= 0) {
+        ks_next = a.p.ks[(size_t)now * a.p.heads + g];
+        vs_next = a.p.vs[(size_t)now * a.p.heads + g];
+      }
+    };
+    step();
+    int after = next, g_after = g_next;   // tile j + 1's page, loaded before tile j's turn
+    step();
+    now = after;
+    g = g_after;
+    scales();
 #pragma unroll 1
     for (int j = 0; j < count && ok; ++j) {
-      const int g = w.g, now = page;
-      float ks = 0.f, vs = 0.f;
-      if (now >= 0) {
-        ks = a.p.ks[(size_t)now * a.p.heads + g];
-        vs = a.p.vs[(size_t)now * a.p.heads + g];
-      }
-      if (j + 1 < count) {       // the next tile's page numbers, on their way during this one's loads
-        w.next(a);
-        page = page_of(w, lane);
-      }
-      const unsigned have = __ballot_sync(0xffffffffu, now >= 0);
+      const float ks = ks_next, vs = vs_next;
+      const int page = now, head = g;
+      now = next;
+      g = g_next;
+      step();
+      scales();
+      const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+      const int first_row = page >= 0 ? (page * a.p.heads + head) * L : 0;
 #pragma unroll 1
       for (int kv = 0; kv < 2; ++kv, ++unit) {
         if (unit >= NU && !(ok = mbar_wait_warp_small(empty + u, uphase, abort_flag, 0x60))) break;
@@ -295,11 +316,17 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
           if (have) mbar_expect_tx(full + u, (uint32_t)__popc(have) * L * kPG_D); else mbar_arrive(full + u);
         }
         __syncwarp();
-        if (now >= 0) {
-          const int row = (now * a.p.heads + g) * L;
-          uint8_t* dst = ring + u * kPA_Unit + lane * L * 128;
-          tma_load_2d(dst, kv ? &vmap : &kmap, full + u, 0, row);
-          tma_load_2d(dst + kPA_Tile * 128, kv ? &vmap : &kmap, full + u, 128, row);
+        // page by page with operands that all lanes agree on: eight lanes issuing their own pages took 150 cycles per copy
+        const void* map = kv ? &vmap : &kmap;
+#pragma unroll 1
+        for (int i = 0; i < ppt; ++i) {
+          const int row = __shfl_sync(0xffffffffu, first_row, i);
+          if (((have >> i) & 1u) && elect_one()) {
+            uint8_t* dst = ring + u * kPA_Unit + i * L * 128;
+            tma_load_2d(dst, map, full + u, 0, row);
+            tma_load_2d(dst + kPA_Tile * 128, map, full + u, 128, row);
+          }
+          __syncwarp();
         }
         if (++u == NU) {
           u = 0;
