@@ -58,6 +58,11 @@ SIGNATURES = {
     "bf_paged_attend_workspace": [_I, _I, _I, _I, _I],
     "bf_paged_attend": [_P, _I, _P, _L, _L, _L, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P, _P, _Z, _P],
     "bf_paged_pages": [_P, _P, _I, _P, _I, _P, _I, _P, _I, _P],
+    "bf_page_table_reserve": [_P, _P, _P, _I, _P, _P, _P],
+    "bf_page_table_free": [_P, _P, _I, _P],
+    "bf_page_table_fork": [_P, _P, _P, _I, _P, _P],
+    "bf_page_table_truncate": [_P, _P, _P, _I, _P, _P, _P, _P, _P],
+    "bf_page_table_compact": [_P, _P, _P],
     "bf_llama_state_floats": [_I, _I, _I, _I],
     "bf_llama_state_pack": [_P, _P, _I, _I, _I, _I, _I, _P, _L, _P],
     "bf_llama_state_unpack": [_P, _L, _P, _I, _I, _I, _I, _I, _P, _P],
@@ -102,11 +107,11 @@ def strerror(code: int) -> str:
 
 def size(name: str, *args) -> int:
     """Call a size query (returns size_t)."""
-    return int(getattr(load(), name)(*args))
+    return getattr(_lib or load(), name)(*args)
 
 
 def call(name: str, *args) -> None:
-    rc = getattr(load(), name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc != 0:
         msg = strerror(rc)
         if rc == 5:   # BF_ERR_CUDA: add the CUDA error behind it

@@ -6,6 +6,8 @@ made contiguous; q/k/v may be fp32 or bf16 where the kernel accepts both.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 
 from . import _lib
@@ -18,7 +20,8 @@ def check_cuda(*ts) -> None:
 
 
 def stream_handle() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device (torch.cuda.current_stream() builds an object around it: 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def ptr(t) -> int:
@@ -220,9 +223,15 @@ def refuse_grad(name: str, *ts) -> None:
 
 def same_device(*ts) -> torch.device:
     dev = next(t.device for t in ts if t is not None)
-    if any(t is not None and t.device != dev for t in ts):
-        raise ValueError("all tensors must be on one device")
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device")
     return dev
+
+
+def on_device(dev: torch.device):
+    """The tensors' device as the current one (no guard where it is already: the guard costs a few microseconds)."""
+    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def heads_16bit(name: str, t) -> torch.Tensor:
@@ -230,14 +239,16 @@ def heads_16bit(name: str, t) -> torch.Tensor:
     not so)."""
     if t.dtype not in (torch.bfloat16, torch.float16):
         raise NotImplementedError(f"{name} is {t.dtype}: built for bfloat16 and float16")
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
-        all(s > 0 and s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1)
+    st = t.stride()
+    ok = st[-1] == 1 and t.data_ptr() % 16 == 0
+    for s, n in zip(st[:-1], t.shape):
+        ok = ok and (n < 2 or (s > 0 and s % 8 == 0))
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def strides(t) -> tuple:
     """Element strides of all but the last dimension (0 for a dimension of one, whose stride means nothing)."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape))
+    return tuple([s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)])
 
 
 def kernel_dtype(t) -> int:
@@ -255,6 +266,8 @@ def int32_on(dev, name: str, t) -> torch.Tensor:
     """An index tensor as contiguous int32 on ``dev`` (values above 31 bits are the caller's error)."""
     if t.dim() != 1 or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be a one-dimensional int32 or int64 tensor")
+    if t.dtype == torch.int32 and t.device == dev and t.is_contiguous():
+        return t
     return t.to(device=dev, dtype=torch.int32).contiguous()
 
 
@@ -284,7 +297,7 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, with_ls
         raise ValueError("keys and queries differ in number: cu_seqlens_k is needed")
     dev = same_device(q, k, v)
     scale = score_scale(scale, D)
-    with torch.cuda.device(dev):
+    with on_device(dev):
         cu = int32_on(dev, "cu_seqlens", cu_seqlens)
         cuk = None if cu_seqlens_k is None else int32_on(dev, "cu_seqlens_k", cu_seqlens_k)
         if cu.numel() < 1 or (cuk is not None and cuk.numel() != cu.numel()):

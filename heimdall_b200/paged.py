@@ -17,179 +17,108 @@ Calls on one cache belong on one stream, or on streams that the caller orders.  
 """
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import torch
 
 from . import _lib
-from .functional import (check_cuda, heads_16bit, int32_on, kernel_dtype, prompt_attention, ptr, refuse_grad, same_device,
-                         score_scale, stream_handle, strides)
-from .structs import BfPagePool
+from .functional import (check_cuda, heads_16bit, int32_on, kernel_dtype, on_device, prompt_attention, ptr, refuse_grad,
+                         same_device, score_scale, stream_handle, strides)
+from .structs import BfPagePool, BfPageTable
 
 PAGE_SIZES = (16, 32, 64, 128)
 
 
-class PageTable:
-    """The host's side of the cache: which slot holds which pages.  Every method returns what the device has to do, as
-    the int32 lists of ``bf_paged_pages``; a call that raises has changed nothing.
+_REASONS = {1: "a slot is outside [0, {slots})", 2: "a slot is named twice", 3: "a number of tokens is negative",
+            4: "a sequence would be longer than the cache's max_len ({tokens})", 5: "a slot is both taken from and filled",
+            6: "a slot to fill holds a sequence: free it first", 7: "truncate cannot lengthen a sequence"}
 
-    Only the last page of a sequence can be partly filled, and a partly filled page belongs to one sequence."""
+
+class PageTable:
+    """The host's side of the cache: which slot holds which pages (``bf_page_table_*``, over numpy arrays).  Every method
+    returns what the device has to do, as the int32 lists of ``bf_paged_pages``, good until the next call; a call that raises has
+    changed nothing."""
 
     def __init__(self, pages: int, slots: int, page: int, width: int):
         self.pages, self.slots, self.page, self.width = pages, slots, page, width
         self.refs = np.zeros(pages, np.int32)
         self.table = np.full((slots, width), -1, np.int32)
         self.lens = np.zeros(slots, np.int64)
-        self.n_free = pages
-        self._low = 0                        # no free page below this one
+        self._mark = np.zeros(slots, np.int32)
+        self._set = np.empty((slots * (width + 1), 2), np.int32)
+        self._fork = np.empty((slots, 5), np.int32)
+        self._move = np.empty((pages, 2), np.int32)
+        self._out = np.zeros(8, np.int32)                   # [0:3] info, [4] and [5] list lengths
+        self._state = BfPageTable(*(x.ctypes.data for x in (self.refs, self.table, self.lens, self._mark)), pages, slots, page,
+                                  width, pages, 0, 0)
+        self._lib = _lib.load()
+        # addresses of what stays where it is
+        self._t, self._info = ctypes.addressof(self._state), self._out.ctypes.data
+        self._n0, self._n1 = self._info + 16, self._info + 20
+        self._to_set, self._to_fork, self._to_move = (x.ctypes.data for x in (self._set, self._fork, self._move))
 
-    def _slots(self, slots, distinct=True) -> np.ndarray:
-        s = np.atleast_1d(np.asarray(slots))
-        if s.size == 0:
-            return np.zeros(0, np.int64)
-        if s.ndim != 1 or not np.issubdtype(s.dtype, np.integer):
+    @property
+    def n_free(self) -> int:
+        return self._state.n_free
+
+    def _whole(self, x, like=None) -> np.ndarray:
+        """x as int64 [n], or, beside slots, one number for each of them."""
+        x = np.asarray(x)
+        if x.dtype.kind not in "iu" and x.size:
+            raise ValueError("whole numbers are needed")
+        if like is not None:
+            if x.ndim == 0:
+                return np.full(like.shape, x, np.int64)
+            if x.shape != like.shape:
+                raise ValueError("one whole number, or one for each slot, is needed")
+        elif x.ndim > 1:
             raise ValueError("slots must be a list of whole numbers")
-        if s.min() < 0 or s.max() >= self.slots:
-            raise ValueError(f"a slot is outside [0, {self.slots})")
-        if distinct and np.unique(s).size != s.size:
-            raise ValueError("a slot is named twice")
-        return s.astype(np.int64)
+        return np.ascontiguousarray(x.reshape(-1), np.int64)
 
-    def _counts(self, n, like) -> np.ndarray:
-        n = np.asarray(n)
-        if not np.issubdtype(n.dtype, np.integer) or (n.ndim and n.shape != like.shape):
-            raise ValueError("one whole number, or one for each slot, is needed")
-        n = np.broadcast_to(n, like.shape).astype(np.int64)
-        if n.size and n.min() < 0:
-            raise ValueError("a number of tokens is negative")
-        return n
-
-    def _held(self, lens):
-        return -(-lens // self.page)
-
-    def _take(self, n: int) -> np.ndarray:
-        """The n lowest free pages (the caller has checked that there are so many)."""
-        out, at, step = [], self._low, max(1024, 2 * n)
-        left = n
-        while left > 0:
-            got = np.flatnonzero(self.refs[at:at + step] == 0)[:left] + at
-            out.append(got)
-            left -= got.size
-            at += step
-        pages = np.concatenate(out) if out else np.zeros(0, np.int64)
-        if n:
-            self.refs[pages] = 1
-            self.n_free -= n
-            self._low = int(pages[-1]) + 1
-        return pages
-
-    def _drop(self, pages: np.ndarray) -> None:
-        np.subtract.at(self.refs, pages, 1)
-        gone = np.unique(pages[self.refs[pages] == 0])
-        self.n_free += gone.size
-        if gone.size:
-            self._low = min(self._low, int(gone[0]))
-
-    def _need(self, n: int, free: int) -> None:
-        if n > free:
-            raise RuntimeError(f"heimdall_b200: the page pool is full ({n} pages needed, {free} of {self.pages} free)")
+    def _call(self, name, *args) -> None:
+        rc = getattr(self._lib, name)(self._t, *args)
+        if rc:
+            reason = int(self._out[0])
+            if reason == 8:
+                raise RuntimeError(f"heimdall_b200: the page pool is full ({self._out[1]} pages needed, {self._out[2]} of "
+                                   f"{self.pages} free)")
+            raise ValueError(_REASONS[reason].format(slots=self.slots, tokens=self.width * self.page))
 
     def reserve(self, slots, n) -> dict:
-        s = self._slots(slots)
-        n = self._counts(n, s)
-        old = self.lens[s]
-        new = old + n
-        if s.size and new.max() > self.width * self.page:
-            raise ValueError(f"a sequence would be longer than the cache's max_len ({self.width * self.page})")
-        have = self._held(old)
-        more = self._held(new) - have
-        total = int(more.sum())
-        self._need(total, self.n_free)
-        pages = self._take(total)
-        row = np.repeat(s, more)
-        col = np.arange(total) - np.repeat(np.cumsum(more) - more, more) + np.repeat(have, more)
-        self.table[row, col] = pages
-        self.lens[s] = new
-        at = np.concatenate([row * self.width + col, self.slots * self.width + s])
-        return {"set": np.stack([at, np.concatenate([pages, new])], 1)}
+        s = self._whole(slots)
+        n = self._whole(n, s)
+        if s.size > self.slots:
+            raise ValueError(_REASONS[2])
+        self._call("bf_page_table_reserve", s.ctypes.data, n.ctypes.data, s.size, self._to_set, self._n0, self._info)
+        return {"set": self._set[:self._out[4]]}
 
     def free(self, slots) -> dict:
-        s = self._slots(slots)
-        rows = self.table[s]
-        self._drop(rows[rows >= 0])
-        self.table[s] = -1
-        self.lens[s] = 0
-        return {"release": s}
+        s = self._whole(slots)
+        self._call("bf_page_table_free", s.ctypes.data, s.size, self._info)
+        return {"release": s.astype(np.int32)}
 
     def fork(self, src, dst) -> dict:
-        a, b = self._slots(src, distinct=False), self._slots(dst)
+        a, b = self._whole(src), self._whole(dst)
         if a.size != b.size:
             raise ValueError("fork needs as many slots to fill as slots to take from")
-        if np.intersect1d(a, b).size:
-            raise ValueError("a slot is both taken from and filled")
-        if (self.lens[b] > 0).any():
-            raise ValueError("a slot to fill holds a sequence: free it first")
-        lens = self.lens[a]
-        part = lens % self.page > 0
-        self._need(int(part.sum()), self.n_free)
-        last = np.maximum(self._held(lens) - 1, 0)
-        old = np.where(part, self.table[a, last], -1)
-        new = np.full(a.size, -1, np.int64)
-        new[part] = self._take(int(part.sum()))
-        rows = self.table[a]
-        rows[part, last[part]] = new[part]
-        shared = rows.copy()
-        shared[part, last[part]] = -1
-        np.add.at(self.refs, shared[shared >= 0], 1)
-        self.table[b] = rows
-        self.lens[b] = lens
-        return {"fork": np.stack([a, b, lens, old, new], 1)}
+        if b.size > self.slots:
+            raise ValueError(_REASONS[2])
+        self._call("bf_page_table_fork", a.ctypes.data, b.ctypes.data, a.size, self._to_fork, self._info)
+        return {"fork": self._fork[:a.size]}
 
     def truncate(self, slots, lens) -> dict:
-        s = self._slots(slots)
-        new = self._counts(lens, s)
-        if (new > self.lens[s]).any():
-            raise ValueError("truncate cannot lengthen a sequence")
-        keep = self._held(new)
-        rows = self.table[s]
-        col = np.arange(self.width)[None]
-        tail = (col >= keep[:, None]) & (rows >= 0)
-        last = np.maximum(keep - 1, 0)
-        end = rows[np.arange(s.size), last] if s.size else np.zeros(0, np.int32)
-        part = (new % self.page > 0)
-        # references left once the tails are given back: a partly filled page that others still hold is copied, slot by
-        # slot (the last holder keeps it)
-        refs = self.refs.copy()
-        np.subtract.at(refs, rows[tail], 1)
-        copied = np.zeros(s.size, bool)
-        for i in np.flatnonzero(part):
-            if refs[end[i]] > 1:
-                refs[end[i]] -= 1
-                copied[i] = True
-        n = int(copied.sum())
-        self._need(n, int((refs == 0).sum()))
-        self._drop(rows[tail])
-        pages = self._take(n)
-        self._drop(end[copied])
-        r, c = np.nonzero(tail)
-        self.table[s[r], c] = -1
-        self.table[s[copied], last[copied]] = pages
-        self.lens[s] = new
-        out = {"fork": np.stack([s[copied], s[copied], new[copied], end[copied], pages], 1)}
-        at = np.concatenate([s[r] * self.width + c, self.slots * self.width + s])
-        out["set"] = np.stack([at, np.concatenate([np.full(r.size, -1), new])], 1)
-        return out
+        s = self._whole(slots)
+        n = self._whole(lens, s)
+        if s.size > self.slots:
+            raise ValueError(_REASONS[2])
+        self._call("bf_page_table_truncate", s.ctypes.data, n.ctypes.data, s.size, self._to_fork, self._n0, self._to_set,
+                   self._n1, self._info)
+        return {"fork": self._fork[:self._out[4]], "set": self._set[:self._out[5]]}
 
     def compact(self) -> dict:
-        n = self.pages - self.n_free
-        src = np.flatnonzero(self.refs[n:]) + n
-        dst = np.flatnonzero(self.refs[:n] == 0)
-        to = np.arange(self.pages, dtype=np.int32)
-        to[src] = dst
-        self.refs[dst] = self.refs[src]
-        self.refs[src] = 0
-        self.table = np.where(self.table >= 0, to[self.table], self.table)
-        self._low = n
-        return {"move": np.stack([src, dst], 1)}
+        self._call("bf_page_table_compact", self._to_move, self._n0)
+        return {"move": self._move[:self._out[4]]}
 
 
 class PagedKV:
@@ -226,7 +155,6 @@ class PagedKV:
         self.lens = torch.zeros(slots, dtype=torch.int32, device=dev)
         self._pool = BfPagePool(ptr(self.k_pages), ptr(self.v_pages), ptr(self.k_scale), ptr(self.v_scale), ptr(self.table),
                                 ptr(self.lens), layers, pages, heads, page, dim, slots, width)
-        import ctypes
         self._pool_ptr = ctypes.addressof(self._pool)
 
     # -------------------------------------------------------------------------------------------- sequences and pages
@@ -240,17 +168,18 @@ class PagedKV:
 
     def _apply(self, change, *args) -> None:
         """The host's change, then the device's.  Not for a capture: a replay would not repeat the host's part."""
-        with torch.cuda.device(self.device):
+        with on_device(self.device):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("heimdall_b200: pages are given out on the host: reserve, fork, free, truncate and compact "
                                    "cannot be captured into a CUDA graph")
             todo = change(*args)
-            lists = []
+            flat, some = [], 0
             for name in ("release", "fork", "move", "set"):
-                x = np.ascontiguousarray(todo[name], np.int32) if name in todo else np.zeros((0, 1), np.int32)
-                lists.append(x)
-            if any(x.shape[0] for x in lists):
-                flat = [y for x in lists for y in (x.ctypes.data, x.shape[0])]
+                x = todo.get(name)
+                n = 0 if x is None else x.shape[0]
+                flat += (x.ctypes.data, n) if n else (0, 0)
+                some += n
+            if some:
                 _lib.call("bf_paged_pages", self._pool_ptr, *flat, stream_handle())
 
     def reserve(self, slots, n) -> None:
@@ -310,7 +239,7 @@ class PagedKV:
         if k.shape[-2] != self.heads or k.shape[-1] != self.dim:
             raise ValueError(f"append takes {self.heads} heads of {self.dim}")
         same_device(self.k_pages, k, v)
-        with torch.cuda.device(self.device):
+        with on_device(self.device):
             cu = int32_on(self.device, "cu_seqlens", cu_seqlens) if packed else None
             B = cu.numel() - 1 if packed else k.shape[0]
             if B < 0:
@@ -337,7 +266,7 @@ class PagedKV:
             raise NotImplementedError("attend takes at most 24 query heads per KV head")
         same_device(self.k_pages, q)
         scale = score_scale(scale, D)
-        with torch.cuda.device(self.device):
+        with on_device(self.device):
             ids = self._ids(slots, B)
             q = heads_16bit("q", q)
             o = torch.empty(B, t, H, D, device=self.device, dtype=q.dtype)

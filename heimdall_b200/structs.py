@@ -20,3 +20,9 @@ class BfPagePool(ctypes.Structure):
     _fields_ = [("k_pages", _P), ("v_pages", _P), ("k_scale", _P), ("v_scale", _P), ("table", _P), ("lens", _P),
                 ("layers", ctypes.c_int), ("pages", ctypes.c_int), ("heads", ctypes.c_int), ("page", ctypes.c_int),
                 ("dim", ctypes.c_int), ("slots", ctypes.c_int), ("width", ctypes.c_int)]
+
+
+class BfPageTable(ctypes.Structure):
+    _fields_ = [("refs", _P), ("table", _P), ("lens", _P), ("mark", _P), ("pages", ctypes.c_int), ("slots", ctypes.c_int),
+                ("page", ctypes.c_int), ("width", ctypes.c_int), ("n_free", ctypes.c_int), ("low", ctypes.c_int),
+                ("epoch", ctypes.c_int)]

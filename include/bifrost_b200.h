@@ -399,6 +399,34 @@ typedef struct bf_page_pool {
   int layers, pages, heads, page, dim, slots, width;
 } bf_page_pool;
 
+/* The host's side: which slot holds which pages.  All arrays are the caller's host memory: refs [pages], table [slots,width], lens
+ * [slots], mark [slots]; before the first call refs, lens, mark, epoch and low are 0, every table entry -1, n_free = pages.  Pages are given out
+ * lowest first, in the order of the slots; only a sequence's last page can be partly filled, and then no other holds it.  A
+ * refused call changes nothing: BF_ERR_INVALID_ARGUMENT with info[0] = the reason (BF_PAGES_FULL: info[1] pages needed,
+ * info[2] free).  The lists written are what bf_paged_pages takes (its release list is the slots freed):
+ *   reserve: n[i] more tokens for slots[i]; set has room for 2 * (pages given out + count), at most 2 * slots * (width + 1);
+ *   fork: slots dst continue the sequences of src, full pages shared; fork [count][5];
+ *   truncate: slots keep lens[i] tokens; fork has room for [count][5], set as for reserve;
+ *   compact: the live pages at or above their number move into the holes below; move has room for [pages][2]. */
+enum {
+  BF_PAGES_SLOT_RANGE = 1, BF_PAGES_SLOT_TWICE = 2, BF_PAGES_NEGATIVE = 3, BF_PAGES_TOO_LONG = 4, BF_PAGES_BOTH = 5,
+  BF_PAGES_HELD = 6, BF_PAGES_LENGTHEN = 7, BF_PAGES_FULL = 8
+};
+typedef struct bf_page_table {
+  int32_t* refs;
+  int32_t* table;
+  int64_t* lens;
+  int32_t* mark;
+  int pages, slots, page, width, n_free, low, epoch;
+} bf_page_table;
+int bf_page_table_reserve(bf_page_table* t, const int64_t* slots, const int64_t* n, int count, int32_t* set, int* n_set,
+                          int* info);
+int bf_page_table_free(bf_page_table* t, const int64_t* slots, int count, int* info);
+int bf_page_table_fork(bf_page_table* t, const int64_t* src, const int64_t* dst, int count, int32_t* fork, int* info);
+int bf_page_table_truncate(bf_page_table* t, const int64_t* slots, const int64_t* lens, int count, int32_t* fork, int* n_fork,
+                           int32_t* set, int* n_set, int* info);
+int bf_page_table_compact(bf_page_table* t, int32_t* move, int* n_move);
+
 int bf_paged_append(const bf_page_pool* pool, int layer, const void* k, long long k_sb, long long k_st, long long k_sh,
                     const void* v, long long v_sb, long long v_st, long long v_sh, const int32_t* slots,
                     const int32_t* cu, int B, int t, int dtype, bf_stream_t stream);
