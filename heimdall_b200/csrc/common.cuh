@@ -335,6 +335,47 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 __device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// messages between the CTAs of a cluster through ordinary shared memory: store, release-arrive; acquire-wait, load
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t x) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint64_t* bar, uint32_t parity, volatile int* abort, unsigned int site) {
+  if (!mbar_wait_small(bar, parity, abort, site)) return false;
+  uint32_t ok;     // complete: this try only adds the scope
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Cluster launch control: ask for a cluster of the grid that has not started yet, to do its work here.  The 16-byte answer
+// completes on `bar`; the first CTA index of the cluster, or -1 when none is left (then nothing may be asked again)
+__device__ __forceinline__ void clc_try_cancel(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ int clc_answer(const void* answer) {
+  uint32_t x, got;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "mov.u32 %0, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, h;\n\t}"
+      : "=&r"(x), "=&r"(got)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return got ? (int)x : -1;
+}
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
                : "memory");

@@ -14,10 +14,13 @@
 // P is rounded to the inputs' type (a step of the type, half of it at most, per weight: as large as the output's own rounding, and averaged over the keys);
 // its sum is taken before.  Scores are in the log2 domain; O is rescaled only when a row's maximum grows by more than 2^8.
 //
-// A cluster takes `per` items (head pairs, or heads) of one (token block, KV head) in turn; blocks go from the last to the first, so
-// the long ones start first, and KV head by KV head, so the clusters that run together share one head's keys in L2.
-// Warps (512 threads): 0 Q and K loads; 1 MMA (in the first CTA of the pair); 2 V loads; 4-11 softmax, two warpgroups, each for
-// 64 of a tile's 128 keys and 128 of O's columns; 12-15 the outputs, while the next item's products run.
+// Work items are (token block, KV head, head pair or head), one cluster of the grid each, from the last block of the call to the
+// first: a sequence's long blocks start first.  A cluster that has done its own item asks the hardware for one that has not
+// started (cluster launch control) and goes on with that: the start of a CTA pair (barriers, TMEM, the first loads) costs about 9 us,
+// as much as six key tiles, and the next item's loads and first products run under the end of the last one.
+// Warps (512 threads): 0 Q and K loads; 1 MMA (in the first CTA of the pair); 2 V loads; 3 the next items (the first CTA asks and
+// passes the answer on); 4-11 softmax, two warpgroups, each for 64 of a tile's 128 keys and 128 of O's columns; 12-15 the outputs,
+// while the next item's products run.
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -36,7 +39,8 @@ constexpr int kPR_SmemQ = kPR_M * kPR_D * 2;          // 64 KB
 constexpr int kPR_SmemK = kPR_N / 2 * kPR_D * 2;      // 32 KB: this CTA's half of the keys
 constexpr int kPR_SmemV = kPR_N * kPR_D / 2 * 2;      // 32 KB: this CTA's half of the columns
 constexpr int kPR_Tiles = kPR_SmemQ + 2 * kPR_SmemK + 2 * kPR_SmemV;
-constexpr int kPR_Smem = kPR_Tiles + 256 + 5120 + 1024;
+constexpr int kPR_Items = 3;      // items known ahead
+constexpr int kPR_Smem = kPR_Tiles + 512 + 5120 + 1024;
 constexpr uint32_t kPR_TmO = 256;
 constexpr float kPR_Rescale = 8.0f;
 
@@ -44,7 +48,7 @@ struct PromptArgs {
   const int32_t *cu_q, *cu_k;
   int n_seq, T, Tk, H, G;
   int qb;                 // tokens per block: 128 (two heads) or 256 (two tiles of one head)
-  int nblk, hsplit, per;  // blocks, clusters per (block, KV head), items per cluster
+  int nblk, hsplit;       // blocks, items per (block, KV head)
   float c2;               // scale * log2(e)
   void* o;
   float* lse;
@@ -54,6 +58,12 @@ struct PromptArgs {
 // the block's sequence: tokens q0 .. q0 + nq - 1, keys k0 .. k0 + nk - 1, the block's first token i0 in it
 struct PromptBlock {
   int q0, nq, k0, nk, i0;
+};
+
+// What a CTA has to do for an item: its rows of q and o (row0 and up, `rows` of them stored), keys k0 and up of which nk are the
+// sequence's, n key tiles (-1: no more items), row r of the tile sees keys up to lim + r
+struct __align__(16) PromptItem {
+  int row0, rows, k0, nk, n, lim, h, g;
 };
 
 // Block number blk of the call.  The rows are cut into n_seq + 2 parts: those before the first sequence, the sequences, those
@@ -137,27 +147,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   uint64_t *q_free = bars + 8, *k_empty = bars + 9 /*[2]*/, *v_empty = bars + 11 /*[2]*/, *s_full = bars + 13 /*[2]*/, *o_fin = bars + 15;
   // within a CTA
   uint64_t *pair = bars + 16 /*[4]*/, *stats = bars + 20 /*[2]*/, *sfree = bars + 22 /*[2]*/, *v_own = bars + 24;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 26);
-  float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 256);   // [2 tile parities][2 halves][128] maxima
+  uint64_t *item_full = bars + 25 /*[3]*/, *item_free = bars + 28 /*[3]*/, *clc = bars + 31, *msg_full = bars + 32, *msg_free = bars + 33;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 35);
+  uint8_t* answer = reinterpret_cast<uint8_t*>(bars + 36);                         // 16 bytes
+  volatile int* msg = reinterpret_cast<volatile int*>(bars + 38);
+  PromptItem* s_items = reinterpret_cast<PromptItem*>(bars + 40);                  // [kPR_Items]
+  static_assert(40 * 8 + kPR_Items * sizeof(PromptItem) <= 512, "barriers and items");
+  float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);   // [2 tile parities][2 halves][128] maxima
   float* xl = xch + 512;                                                           // [2 slots][2 halves][128] row sums
   float* xmx = xl + 512;                                                           // [2 slots][128] row maxima
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
-  int cl = blockIdx.x >> 1;
-  const int hs = cl % a.hsplit;
-  cl /= a.hsplit;
-  const int g = cl / a.nblk;
-  const PromptBlock blk = prompt_block(a, a.nblk - 1 - cl % a.nblk, lane);
-  if (blk.i0 >= blk.nq) return;              // both CTAs of the pair: a block number that no sequence uses
   const int R = a.H / a.G, two = a.qb == kPR_M;            // two: the pair's tiles are two heads
-  const int off = blk.nk - blk.nq;                         // query i sees keys j <= i + off
-  const int i0 = blk.i0 + (two ? 0 : (int)rank * kPR_M);   // this CTA's first token
-  const int items = min(a.per, (two ? R / 2 : R) - hs * a.per);
-  const int last = min(blk.i0 + a.qb, blk.nq) - 1 + off;   // last key that the pair sees
-  const int n = last >= 0 ? last / kPR_N + 1 : 0;          // key tiles
-  auto head = [&](int it) { return g * R + (two ? 2 * (hs * a.per + it) + (int)rank : hs * a.per + it); };
+  // item `it`, by one lane (lanes = 1) or a whole warp; false when there are no more, or a wait gave up
+  auto item = [&](int it, bool whole_warp, PromptItem& x) -> bool {
+    const int s = it % kPR_Items;
+    const bool ok = whole_warp ? mbar_wait_warp_small(item_full + s, (it / kPR_Items) & 1, abort_flag, 0x90)
+                               : mbar_wait_small(item_full + s, (it / kPR_Items) & 1, abort_flag, 0x90);
+    if (!ok) return false;
+    x = s_items[s];
+    if (whole_warp) __syncwarp();
+    if (!whole_warp || lane == 0) mbar_arrive(item_free + s);
+    return x.n >= 0;
+  };
 
   if (tid == 0) {
     mbar_init(q_full, 2);
@@ -165,6 +179,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
     mbar_init(q_free, 1);
     mbar_init(o_fin, 1);
     mbar_init(v_own, 1);
+    mbar_init(clc, 1);
+    mbar_init(msg_full, 1);
+    mbar_init(msg_free, 1);
+    for (int i = 0; i < kPR_Items; ++i) {
+      mbar_init(item_full + i, 1);
+      mbar_init(item_free + i, rank == 0 ? 15 : 14);       // Q and K, V, softmax 8, outputs 4, and the products
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full + i, 2);
       mbar_init(v_full + i, 2);
@@ -198,15 +219,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       const uint32_t qf = cluster_addr(q_full, 0), kf[2] = {cluster_addr(k_full, 0), cluster_addr(k_full + 1, 0)};
       int t = 0;
       bool ok = true;
-      for (int it = 0; it < items && ok; ++it) {
+      PromptItem x;
+      for (int it = 0; ok && item(it, false, x); ++it) {
         if (it >= 1 && !(ok = mbar_wait_small(q_free, (it - 1) & 1, abort_flag, 0x80))) break;
         mbar_expect_tx_cluster(qf, kPR_SmemQ);
-        tma_load_4d_pair(sQ, &qmap, qf, 0, blk.q0 + i0, 0, head(it));
-        for (int j = 0; j < n; ++j, ++t) {
+        tma_load_4d_pair(sQ, &qmap, qf, 0, x.row0, 0, x.h);
+        for (int j = 0; j < x.n; ++j, ++t) {
           const int s = t & 1;
           if (t >= 2 && !(ok = mbar_wait_small(k_empty + s, ((t >> 1) - 1) & 1, abort_flag, 0x81))) break;
           mbar_expect_tx_cluster(kf[s], kPR_SmemK);
-          tma_load_4d_pair(sK + s * kPR_SmemK, &kmap, kf[s], 0, blk.k0 + j * kPR_N + (int)rank * (kPR_N / 2), 0, g);
+          tma_load_4d_pair(sK + s * kPR_SmemK, &kmap, kf[s], 0, x.k0 + j * kPR_N + (int)rank * (kPR_N / 2), 0, x.g);
         }
       }
     } else if (warp == 2) {
@@ -215,15 +237,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       const uint32_t vf[2] = {cluster_addr(v_full, 0), cluster_addr(v_full + 1, 0)};
       int t = 0, own = 0;
       bool ok = true;
-      for (int it = 0; it < items && ok; ++it) {
-        for (int j = 0; j < n; ++j, ++t) {
-          const int s = t & 1, rows = blk.nk - j * kPR_N;   // rows of the tile that are this sequence's
+      PromptItem x;
+      for (int it = 0; ok && item(it, true, x); ++it) {
+        for (int j = 0; j < x.n; ++j, ++t) {
+          const int s = t & 1, rows = x.nk - j * kPR_N;   // rows of the tile that are this sequence's
           if (t >= 2 && !(ok = mbar_wait_warp_small(v_empty + s, ((t >> 1) - 1) & 1, abort_flag, 0x82))) break;
           uint8_t* dst = sV + s * kPR_SmemV;
           const bool whole = rows >= kPR_N;
           if (lane == 0) {
             if (whole) mbar_expect_tx_cluster(vf[s], kPR_SmemV); else mbar_expect_tx(v_own, kPR_SmemV);
-            tma_load_4d_pair(dst, &vmap, whole ? vf[s] : smem_u32(v_own), 0, blk.k0 + j * kPR_N, 2 * (int)rank, g);
+            tma_load_4d_pair(dst, &vmap, whole ? vf[s] : smem_u32(v_own), 0, x.k0 + j * kPR_N, 2 * (int)rank, x.g);
           }
           __syncwarp();
           if (!whole) {
@@ -240,6 +263,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           }
         }
       }
+    } else if (warp == 3) {
+      // ---------------------------------------------------------------- items
+      const uint32_t peer_msg = cluster_addr((const void*)msg, 1), peer_full = cluster_addr(msg_full, 1), lead_free = cluster_addr(msg_free, 0);
+      int it = 0, asked = 0;
+      int cta = (int)(blockIdx.x & ~1u);
+      for (bool ok = true; ok;) {
+        PromptItem x{0, 0, 0, 0, -1, 0, 0, 0};
+        if (cta >= 0) {
+          int cl = cta >> 1;
+          const int hs = cl % a.hsplit;
+          cl /= a.hsplit;
+          const PromptBlock b = prompt_block(a, a.nblk - 1 - cl / a.G, lane);
+          const int off = b.nk - b.nq;                                // query i sees keys j <= i + off
+          const int i0 = b.i0 + (two ? 0 : (int)rank * kPR_M);        // this CTA's first token
+          const int last = min(b.i0 + a.qb, b.nq) - 1 + off;          // last key that the pair sees
+          x.g = cl % a.G;
+          x.h = x.g * R + (two ? 2 * hs + (int)rank : hs);
+          x.row0 = b.q0 + i0;
+          x.rows = b.nq - i0;
+          x.k0 = b.k0;
+          x.nk = b.nk;
+          x.n = last >= 0 ? last / kPR_N + 1 : 0;
+          x.lim = i0 + off;
+          if (b.i0 >= b.nq) x.n = -2;                                 // a block number that no sequence uses
+        }
+        if (x.n != -2) {
+          const int s = it % kPR_Items;
+          if (it >= kPR_Items && !mbar_wait_warp_small(item_free + s, (it / kPR_Items - 1) & 1, abort_flag, 0x91)) break;
+          if (lane == 0) {
+            s_items[s] = x;
+            mbar_arrive(item_full + s);
+          }
+          __syncwarp();
+          ++it;
+        }
+        if (cta < 0) break;
+        // the next one: the first CTA of the pair asks, and tells the other
+        if (rank == 0) {
+          if (lane == 0) {
+            mbar_expect_tx(clc, 16);
+            clc_try_cancel(answer, clc);
+          }
+          __syncwarp();
+          ok = mbar_wait_warp_small(clc, asked & 1, abort_flag, 0x92);
+          if (ok && asked >= 1) ok = __all_sync(0xffffffffu, mbar_wait_acquire_cluster(msg_free, (asked - 1) & 1, abort_flag, 0x93));
+          if (!ok) break;
+          cta = clc_answer(answer);
+          fence_async_smem();          // the answer has been read before the next one is written over it
+          if (lane == 0) {
+            st_cluster_u32(peer_msg, (uint32_t)cta);
+            mbar_arrive_release_cluster(peer_full);
+          }
+          __syncwarp();
+        } else {
+          ok = __all_sync(0xffffffffu, mbar_wait_acquire_cluster(msg_full, asked & 1, abort_flag, 0x94));
+          if (!ok) break;
+          cta = *msg;
+          __syncwarp();
+          if (lane == 0) mbar_arrive_release_cluster(lead_free);
+        }
+        ++asked;
+      }
     } else if (warp == 1 && lane == 0 && rank == 0) {
       // ---------------------------------------------------------------- MMA
       constexpr int is_bf16 = sizeof(T) == 2 && !__is_same(T, __half);
@@ -247,7 +332,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       const uint32_t aQ = smem_u32(sQ);
       int t = 0;
       bool ok = true;
-      for (int it = 0; it < items && ok; ++it) {
+      PromptItem x;
+      for (int it = 0; ok && item(it, false, x); ++it) {
+        const int n = x.n;
         if (!(ok = mbar_wait_small(q_full, it & 1, abort_flag, 0x84))) break;
         auto pv = [&](int j, int tt) -> bool {
           const int s = tt & 1;
@@ -297,11 +384,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
     constexpr int NH = kPR_N / 2;                 // 64 keys per half
     const uint32_t pf[2] = {cluster_addr(p_full, 0), cluster_addr(p_full + 1, 0)};
     uint32_t pair_phase = 0;
-    const int lim = i0 + r + off;                 // last key that this row sees
-    const int lim_all = i0 + off;                 // last key that every row of this CTA sees
     bool alive = true;
     int t = 0;
-    for (int it = 0; it < items && alive; ++it) {
+    PromptItem x;
+    for (int it = 0; alive && item(it, true, x); ++it) {
+      const int n = x.n, lim_all = x.lim, lim = x.lim + r;   // last key that every row of this CTA sees, and this row
       float m_ref = -INFINITY, l = 0.f;           // running maximum (log2 domain) and this half's sum
       for (int j = 0; j < n; ++j) {
         const int tt = t + j, s = tt & 1;
@@ -398,8 +485,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
     const int q4 = warp & 3, r = q4 * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16);
     const uint32_t of = cluster_addr(o_free, 0);
-    const bool store = i0 + r < blk.nq;
-    for (int it = 0; it < items; ++it) {
+    PromptItem x;
+    for (int it = 0; item(it, true, x); ++it) {
+      const bool store = r < x.rows;
+      const int n = x.n;
       if (!mbar_wait_warp_small(o_fin, it & 1, abort_flag, 0x8d)) break;
       const int slot = it & 1;
       if (!mbar_wait_warp_small(&stats[slot], (it >> 1) & 1, abort_flag, 0x8e)) break;
@@ -408,8 +497,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       if (lane == 0) mbar_arrive(&sfree[slot]);
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : 1.f / l;        // nothing seen: zeros
-      const int h = head(it);
-      const size_t row = (size_t)blk.q0 + i0 + r;
+      const int h = x.h;
+      const size_t row = (size_t)x.row0 + r;
       if (store && a.lse) a.lse[(size_t)h * a.T + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
       uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (row * a.H + h) * kPR_D);
 #pragma unroll 1
@@ -487,12 +576,10 @@ int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void
   a.err = st.err;
   const int R = H / G;
   a.qb = R % 2 == 0 ? kPR_M : 2 * kPR_M;
-  const int all = R % 2 == 0 ? R / 2 : R;
   const long long nblk = (long long)T / a.qb + n_seq + 2;
   if (nblk > 0x7fffffffLL) return BF_ERR_UNSUPPORTED;
   a.nblk = (int)nblk;
-  a.per = nblk * G >= 2LL * st.sm_count ? all : 1;
-  a.hsplit = (all + a.per - 1) / a.per;
+  a.hsplit = R % 2 == 0 ? R / 2 : R;
   const long long clusters = nblk * G * a.hsplit;
   if (clusters > 0x3fffffffLL) return BF_ERR_UNSUPPORTED;
   // (64 dims, tokens, 4 groups of 64 dims, heads); a stride of a dimension of one means nothing, and the encoder wants a positive one
