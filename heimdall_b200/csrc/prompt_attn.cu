@@ -14,8 +14,7 @@
 // P is rounded to the inputs' type (a step of the type, half of it at most, per weight: as large as the output's own rounding, and averaged over the keys);
 // its sum is taken before.  Scores are in the log2 domain; O is rescaled only when a row's maximum grows by more than 2^8.
 //
-// Work items are (token block, KV head, head pair or head), one cluster of the grid each, from the last block of the call to the
-// first: a sequence's long blocks start first.  A cluster that has done its own item asks the hardware for one that has not
+// Work items are (token block, KV head, head pair or head), one cluster of the grid each, those with the most key tiles first.  A cluster that has done its own item asks the hardware for one that has not
 // started (cluster launch control) and goes on with that: the start of a CTA pair (barriers, TMEM, the first loads) costs about 9 us,
 // as much as six key tiles, and the next item's loads and first products run under the end of the last one.
 // Warps (512 threads): 0 Q and K loads; 1 MMA (in the first CTA of the pair); 2 V loads; 3 the next items (the first CTA asks and
@@ -40,6 +39,7 @@ constexpr int kPR_SmemK = kPR_N / 2 * kPR_D * 2;      // 32 KB: this CTA's half 
 constexpr int kPR_SmemV = kPR_N * kPR_D / 2 * 2;      // 32 KB: this CTA's half of the columns
 constexpr int kPR_Tiles = kPR_SmemQ + 2 * kPR_SmemK + 2 * kPR_SmemV;
 constexpr int kPR_Items = 3;      // items known ahead
+constexpr int kPR_Ask = 4;        // the next item is asked for this many key tiles before the loads of the last one end
 constexpr int kPR_Smem = kPR_Tiles + 512 + 5120 + 1024;
 constexpr uint32_t kPR_TmO = 256;
 constexpr float kPR_Rescale = 8.0f;
@@ -66,41 +66,81 @@ struct __align__(16) PromptItem {
   int row0, rows, k0, nk, n, lim, h, g;
 };
 
-// Block number blk of the call.  The rows are cut into n_seq + 2 parts: those before the first sequence, the sequences, those
-// behind the last; the first and the last part have no keys.  Part p, from row s on, owns the block numbers s / qb + p and up,
-// at least as many as it has blocks.  Cumulative lengths are clamped into [previous, T] and [previous, Tk].  A warp
-// looks at 32 parts at a time.
-__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, int blk, int lane) {
-  PromptBlock r{0, 0, 0, 0, 0};
+// The rows are cut into n_seq + 2 parts: those before the first sequence, the sequences, those behind the last; the first and the
+// last part have no keys.  Cumulative lengths are clamped into [previous, T] and [previous, Tk].  Lane's part c + lane, given the
+// greatest entries before part c:
+struct PromptPart {
+  int q0, nq, k0, nk;
+};
+__device__ __forceinline__ PromptPart prompt_part(const PromptArgs& a, int c, int lane, int& carry_q, int& carry_k) {
+  const int p = c + lane;
+  const bool from = p >= 1 && p <= a.n_seq + 1 && a.cu_q, to = p <= a.n_seq && a.cu_q;
+  int q = from ? min(max(a.cu_q[p - 1], 0), a.T) : 0, k = from ? min(max(a.cu_k[p - 1], 0), a.Tk) : 0;
+  int qn = to ? min(max(a.cu_q[p], 0), a.T) : a.T, kn = to ? min(max(a.cu_k[p], 0), a.Tk) : 0;
+  q = max(q, carry_q);
+  k = max(k, carry_k);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, q, o), y = __shfl_up_sync(0xffffffffu, k, o);
+    if (lane >= o) {
+      q = max(q, x);
+      k = max(k, y);
+    }
+  }
+  qn = max(q, qn);
+  kn = p >= 1 && to ? max(k, kn) : k;
+  carry_q = __shfl_sync(0xffffffffu, q, 31);
+  carry_k = __shfl_sync(0xffffffffu, k, 31);
+  return PromptPart{q, qn - q, k, kn - k};
+}
+__device__ __forceinline__ PromptBlock prompt_of_lane(const PromptPart& p, int i0, int at) {
+  return PromptBlock{__shfl_sync(0xffffffffu, p.q0, at), __shfl_sync(0xffffffffu, p.nq, at), __shfl_sync(0xffffffffu, p.k0, at),
+                     __shfl_sync(0xffffffffu, p.nk, at), __shfl_sync(0xffffffffu, i0, at)};
+}
+
+// The block of rank `rank` by key tiles, the most first.  With a part per lane (up to 30 sequences): the largest number of tiles t
+// that more than `rank` blocks have at least, by bisection; of a part with nb blocks those with t tiles or more are its last ones.
+// The last blocks to start decide how long the call takes: chunks of 512 tokens after 8192, 1000, 2048 and 4096 earlier ones
+// took 164 us in the order of the sequences.
+// With more parts than lanes: in the reverse order of the rows, 32 parts at a time; part p owns the block numbers q0 / qb + p and up.
+__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, int rank, int lane) {
   int carry_q = 0, carry_k = 0;
-  for (int c = 0; c < a.n_seq + 2; c += 32) {
-    const int p = c + lane;
-    const bool from = p >= 1 && p <= a.n_seq + 1 && a.cu_q, to = p <= a.n_seq && a.cu_q;
-    int q = from ? min(max(a.cu_q[p - 1], 0), a.T) : 0, k = from ? min(max(a.cu_k[p - 1], 0), a.Tk) : 0;
-    int qn = to ? min(max(a.cu_q[p], 0), a.T) : a.T, kn = to ? min(max(a.cu_k[p], 0), a.Tk) : 0;
-    q = max(q, carry_q);
-    k = max(k, carry_k);
+  if (a.n_seq + 2 <= 32) {
+    const PromptPart p = prompt_part(a, 0, lane, carry_q, carry_k);
+    const int qlog = a.qb == 256 ? 8 : 7, nb = lane < a.n_seq + 2 ? (p.nq + a.qb - 1) >> qlog : 0, off = p.nk - p.nq;
+    auto at_least = [&](int t) {      // blocks of this part with t tiles or more
+      const int key = (t - 1) * kPR_N;                       // the first key of the last tile
+      if (t <= 0 || nb == 0) return nb;
+      if (p.nk <= key) return 0;
+      return nb - min(max(((key + 1 - off + a.qb - 1) >> qlog) - 1, 0), nb - 1);
+    };
+    auto sum = [](int x) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)x); };
+    int lo = 0, hi = (int)__reduce_max_sync(0xffffffffu, nb ? (unsigned)((p.nk + kPR_N - 1) / kPR_N) : 0u);
+    if (sum(nb) <= rank) return PromptBlock{0, 0, 0, 0, 0};
+    while (lo < hi) {                  // the answer is in [lo, hi]
+      const int mid = (lo + hi + 1) >> 1;
+      if (sum(at_least(mid)) > rank) lo = mid; else hi = mid - 1;
+    }
+    const int more = at_least(lo + 1), here = at_least(lo) - more;
+    int incl = here;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, q, o), y = __shfl_up_sync(0xffffffffu, k, o);
-      if (lane >= o) {
-        q = max(q, x);
-        k = max(k, y);
-      }
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
     }
-    qn = max(q, qn);
-    kn = p >= 1 && to ? max(k, kn) : k;
-    carry_q = __shfl_sync(0xffffffffu, q, 31);
-    carry_k = __shfl_sync(0xffffffffu, k, 31);
-    const int base = q / a.qb + p;
-    const unsigned ok = __ballot_sync(0xffffffffu, p < a.n_seq + 2 && base <= blk);
+    const int idx = rank - sum(more);
+    const int at = __ffs(__ballot_sync(0xffffffffu, incl > idx)) - 1;
+    return prompt_of_lane(p, (nb - more - here + idx - (incl - here)) * a.qb, at);
+  }
+  PromptBlock r{0, 0, 0, 0, 0};
+  const int blk = a.nblk - 1 - rank;
+  for (int c = 0; c < a.n_seq + 2; c += 32) {
+    const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
+    const int base = p.q0 / a.qb + c + lane;
+    const unsigned ok = __ballot_sync(0xffffffffu, c + lane < a.n_seq + 2 && base <= blk);
     if (ok == 0u) break;
     const int at = 31 - __clz(ok);
-    r.q0 = __shfl_sync(0xffffffffu, q, at);
-    r.nq = __shfl_sync(0xffffffffu, qn, at) - r.q0;
-    r.k0 = __shfl_sync(0xffffffffu, k, at);
-    r.nk = __shfl_sync(0xffffffffu, kn, at) - r.k0;
-    r.i0 = (blk - __shfl_sync(0xffffffffu, base, at)) * a.qb;
+    r = prompt_of_lane(p, (blk - base) * a.qb, at);
     if (at < 31) break;
   }
   return r;
@@ -147,7 +187,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   uint64_t *q_free = bars + 8, *k_empty = bars + 9 /*[2]*/, *v_empty = bars + 11 /*[2]*/, *s_full = bars + 13 /*[2]*/, *o_fin = bars + 15;
   // within a CTA
   uint64_t *pair = bars + 16 /*[4]*/, *stats = bars + 20 /*[2]*/, *sfree = bars + 22 /*[2]*/, *v_own = bars + 24;
-  uint64_t *item_full = bars + 25 /*[3]*/, *item_free = bars + 28 /*[3]*/, *clc = bars + 31, *msg_full = bars + 32, *msg_free = bars + 33;
+  uint64_t *item_full = bars + 25 /*[3]*/, *item_free = bars + 28 /*[3]*/, *clc = bars + 31, *msg_full = bars + 32, *msg_free = bars + 33,
+           *ask = bars + 39;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 35);
   uint8_t* answer = reinterpret_cast<uint8_t*>(bars + 36);                         // 16 bytes
@@ -180,6 +221,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
     mbar_init(o_fin, 1);
     mbar_init(v_own, 1);
     mbar_init(clc, 1);
+    mbar_init(ask, 1);
     mbar_init(msg_full, 1);
     mbar_init(msg_free, 1);
     for (int i = 0; i < kPR_Items; ++i) {
@@ -224,8 +266,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
         if (it >= 1 && !(ok = mbar_wait_small(q_free, (it - 1) & 1, abort_flag, 0x80))) break;
         mbar_expect_tx_cluster(qf, kPR_SmemQ);
         tma_load_4d_pair(sQ, &qmap, qf, 0, x.row0, 0, x.h);
+        if (x.n == 0 && rank == 0) mbar_arrive(ask);
         for (int j = 0; j < x.n; ++j, ++t) {
           const int s = t & 1;
+          if (j == max(x.n - kPR_Ask, 0) && rank == 0) mbar_arrive(ask);
           if (t >= 2 && !(ok = mbar_wait_small(k_empty + s, ((t >> 1) - 1) & 1, abort_flag, 0x81))) break;
           mbar_expect_tx_cluster(kf[s], kPR_SmemK);
           tma_load_4d_pair(sK + s * kPR_SmemK, &kmap, kf[s], 0, x.k0 + j * kPR_N + (int)rank * (kPR_N / 2), 0, x.g);
@@ -274,7 +318,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           int cl = cta >> 1;
           const int hs = cl % a.hsplit;
           cl /= a.hsplit;
-          const PromptBlock b = prompt_block(a, a.nblk - 1 - cl / a.G, lane);
+          const PromptBlock b = prompt_block(a, cl / a.G, lane);
           const int off = b.nk - b.nq;                                // query i sees keys j <= i + off
           const int i0 = b.i0 + (two ? 0 : (int)rank * kPR_M);        // this CTA's first token
           const int last = min(b.i0 + a.qb, b.nq) - 1 + off;          // last key that the pair sees
@@ -299,8 +343,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           ++it;
         }
         if (cta < 0) break;
-        // the next one: the first CTA of the pair asks, and tells the other
+        // the next one: the first CTA of the pair asks, when the loads of the item before it near their end (a cluster that
+        // asked earlier would keep an item waiting that another could start), and tells the other
         if (rank == 0) {
+          if (it > 0 && x.n != -2 && !(ok = mbar_wait_warp_small(ask, (it - 1) & 1, abort_flag, 0x95))) break;
           if (lane == 0) {
             mbar_expect_tx(clc, 16);
             clc_try_cancel(answer, clc);
