@@ -103,10 +103,10 @@ __device__ __forceinline__ PromptBlock prompt_of_lane(const PromptPart& p, int i
 // The last blocks to start decide how long the call takes: chunks of 512 tokens after 8192, 1000, 2048 and 4096 earlier ones
 // took 164 us in the order of the sequences.
 // With more parts than lanes: in the reverse order of the rows, 32 parts at a time; part p owns the block numbers q0 / qb + p and up.
-__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, int rank, int lane) {
-  int carry_q = 0, carry_k = 0;
-  if (a.n_seq + 2 <= 32) {
-    const PromptPart p = prompt_part(a, 0, lane, carry_q, carry_k);
+__device__ __forceinline__ bool prompt_few(const PromptArgs& a) { return a.n_seq + 2 <= 32; }
+__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, const PromptPart& first, int rank, int lane) {
+  if (prompt_few(a)) {
+    const PromptPart p = first;
     const int qlog = a.qb == 256 ? 8 : 7, nb = lane < a.n_seq + 2 ? (p.nq + a.qb - 1) >> qlog : 0, off = p.nk - p.nq;
     auto at_least = [&](int t) {      // blocks of this part with t tiles or more
       const int key = (t - 1) * kPR_N;                       // the first key of the last tile
@@ -132,6 +132,7 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, int ran
     const int at = __ffs(__ballot_sync(0xffffffffu, incl > idx)) - 1;
     return prompt_of_lane(p, (nb - more - here + idx - (incl - here)) * a.qb, at);
   }
+  int carry_q = 0, carry_k = 0;
   PromptBlock r{0, 0, 0, 0, 0};
   const int blk = a.nblk - 1 - rank;
   for (int c = 0; c < a.n_seq + 2; c += 32) {
@@ -310,7 +311,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
     } else if (warp == 3) {
       // ---------------------------------------------------------------- items
       const uint32_t peer_msg = cluster_addr((const void*)msg, 1), peer_full = cluster_addr(msg_full, 1), lead_free = cluster_addr(msg_free, 0);
-      int it = 0, asked = 0;
+      int it = 0, asked = 0, carry_q = 0, carry_k = 0;
+      const PromptPart first = prompt_few(a) ? prompt_part(a, 0, lane, carry_q, carry_k) : PromptPart{0, 0, 0, 0};
       int cta = (int)(blockIdx.x & ~1u);
       for (bool ok = true; ok;) {
         PromptItem x{0, 0, 0, 0, -1, 0, 0, 0};
@@ -318,7 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           int cl = cta >> 1;
           const int hs = cl % a.hsplit;
           cl /= a.hsplit;
-          const PromptBlock b = prompt_block(a, cl / a.G, lane);
+          const PromptBlock b = prompt_block(a, first, cl / a.G, lane);
           const int off = b.nk - b.nq;                                // query i sees keys j <= i + off
           const int i0 = b.i0 + (two ? 0 : (int)rank * kPR_M);        // this CTA's first token
           const int last = min(b.i0 + a.qb, b.nq) - 1 + off;          // last key that the pair sees
