@@ -40,14 +40,15 @@ constexpr int kPR_SmemV = kPR_N * kPR_D / 2 * 2;      // 32 KB: this CTA's half 
 constexpr int kPR_Tiles = kPR_SmemQ + 2 * kPR_SmemK + 2 * kPR_SmemV;
 constexpr int kPR_Items = 3;      // items known ahead
 constexpr int kPR_Ask = 4;        // the next item is asked for this many key tiles before the loads of the last one end
-constexpr int kPR_Smem = kPR_Tiles + 512 + 5120 + 1024;
+constexpr int kPR_Parts = 1022;   // parts of a call whose first rows and keys fit into shared memory
+constexpr int kPR_Smem = kPR_Tiles + 512 + 5120 + 8192 + 4 * 2048 + 1024;
 constexpr uint32_t kPR_TmO = 256;
 constexpr float kPR_Rescale = 8.0f;
 
 struct PromptArgs {
   const int32_t *cu_q, *cu_k;
   int n_seq, T, Tk, H, G;
-  int qb;                 // tokens per block: 128 (two heads) or 256 (two tiles of one head)
+  int qb, qlog;           // tokens per block: 128 (two heads) or 256 (two tiles of one head), and its log2
   int nblk, hsplit;       // blocks, items per (block, KV head)
   float c2;               // scale * log2(e)
   void* o;
@@ -102,12 +103,14 @@ __device__ __forceinline__ PromptBlock prompt_of_lane(const PromptPart& p, int i
 // that more than `rank` blocks have at least, by bisection; of a part with nb blocks those with t tiles or more are its last ones.
 // The last blocks to start decide how long the call takes: chunks of 512 tokens after 8192, 1000, 2048 and 4096 earlier ones
 // took 164 us in the order of the sequences.
-// With more parts than lanes: in the reverse order of the rows, 32 parts at a time; part p owns the block numbers q0 / qb + p and up.
+// With more parts than lanes: in the reverse order of the rows; part p owns the block numbers q0 / qb + p and up, at least as many as
+// it has blocks, and is found by bisection in shared memory (starts: first row and key of each part, and the ends), or, with more
+// than fit there, by going through all parts again.
 __device__ __forceinline__ bool prompt_few(const PromptArgs& a) { return a.n_seq + 2 <= 32; }
-__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, const PromptPart& first, int rank, int lane) {
+__device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, const PromptPart& first, const int2* starts, int rank, int lane) {
   if (prompt_few(a)) {
     const PromptPart p = first;
-    const int qlog = a.qb == 256 ? 8 : 7, nb = lane < a.n_seq + 2 ? (p.nq + a.qb - 1) >> qlog : 0, off = p.nk - p.nq;
+    const int qlog = a.qlog, nb = lane < a.n_seq + 2 ? (p.nq + a.qb - 1) >> qlog : 0, off = p.nk - p.nq;
     auto at_least = [&](int t) {      // blocks of this part with t tiles or more
       const int key = (t - 1) * kPR_N;                       // the first key of the last tile
       if (t <= 0 || nb == 0) return nb;
@@ -132,12 +135,22 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, const P
     const int at = __ffs(__ballot_sync(0xffffffffu, incl > idx)) - 1;
     return prompt_of_lane(p, (nb - more - here + idx - (incl - here)) * a.qb, at);
   }
-  int carry_q = 0, carry_k = 0;
   PromptBlock r{0, 0, 0, 0, 0};
   const int blk = a.nblk - 1 - rank;
+  if (a.n_seq + 2 <= kPR_Parts) {
+    int lo = 0, hi = a.n_seq + 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((starts[mid].x >> a.qlog) + mid <= blk) lo = mid; else hi = mid - 1;
+    }
+    const int2 s = starts[lo], e = starts[lo + 1];
+    const bool keys = lo >= 1 && lo <= a.n_seq;
+    return PromptBlock{s.x, e.x - s.x, s.y, keys ? e.y - s.y : 0, (blk - (s.x >> a.qlog) - lo) << a.qlog};
+  }
+  int carry_q = 0, carry_k = 0;
   for (int c = 0; c < a.n_seq + 2; c += 32) {
     const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
-    const int base = p.q0 / a.qb + c + lane;
+    const int base = (p.q0 >> a.qlog) + c + lane;
     const unsigned ok = __ballot_sync(0xffffffffu, c + lane < a.n_seq + 2 && base <= blk);
     if (ok == 0u) break;
     const int at = 31 - __clz(ok);
@@ -199,6 +212,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);   // [2 tile parities][2 halves][128] maxima
   float* xl = xch + 512;                                                           // [2 slots][2 halves][128] row sums
   float* xmx = xl + 512;                                                           // [2 slots][128] row maxima
+  int2* s_starts = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(bars) + 512 + 5120);   // [kPR_Parts + 1], one warp's
+  uint8_t* s_out = reinterpret_cast<uint8_t*>(bars) + 512 + 5120 + 8192;          // [4 output warps][32 rows][128 B]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
@@ -312,7 +327,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       // ---------------------------------------------------------------- items
       const uint32_t peer_msg = cluster_addr((const void*)msg, 1), peer_full = cluster_addr(msg_full, 1), lead_free = cluster_addr(msg_free, 0);
       int it = 0, asked = 0, carry_q = 0, carry_k = 0;
-      const PromptPart first = prompt_few(a) ? prompt_part(a, 0, lane, carry_q, carry_k) : PromptPart{0, 0, 0, 0};
+      PromptPart first{0, 0, 0, 0};
+      if (prompt_few(a)) {
+        first = prompt_part(a, 0, lane, carry_q, carry_k);
+      } else if (a.n_seq + 2 <= kPR_Parts) {
+        for (int c = 0; c < a.n_seq + 2; c += 32) {
+          const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
+          if (c + lane < a.n_seq + 2) s_starts[c + lane] = make_int2(p.q0, p.k0);
+          if (c + lane == a.n_seq + 1) s_starts[a.n_seq + 2] = make_int2(p.q0 + p.nq, p.k0 + p.nk);
+        }
+        __syncwarp();
+      }
       int cta = (int)(blockIdx.x & ~1u);
       for (bool ok = true; ok;) {
         PromptItem x{0, 0, 0, 0, -1, 0, 0, 0};
@@ -320,7 +345,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           int cl = cta >> 1;
           const int hs = cl % a.hsplit;
           cl /= a.hsplit;
-          const PromptBlock b = prompt_block(a, first, cl / a.G, lane);
+          const PromptBlock b = prompt_block(a, first, s_starts, cl / a.G, lane);
           const int off = b.nk - b.nq;                                // query i sees keys j <= i + off
           const int i0 = b.i0 + (two ? 0 : (int)rank * kPR_M);        // this CTA's first token
           const int last = min(b.i0 + a.qb, b.nq) - 1 + off;          // last key that the pair sees
@@ -548,7 +573,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       const int h = x.h;
       const size_t row = (size_t)x.row0 + r;
       if (store && a.lse) a.lse[(size_t)h * a.T + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-      uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (row * a.H + h) * kPR_D);
+      // 32 columns at a time through shared memory (16-byte chunks, swizzled by the row), so that a store instruction writes whole
+      // 64-byte pieces of eight rows instead of 16 bytes of 32
+      uint8_t* stage = s_out + (warp - 12) * 2048;
+      const int r8 = lane >> 2, chunk = lane & 3;
+      T* out = static_cast<T*>(a.o) + ((size_t)(x.row0 + q4 * 32) * a.H + h) * kPR_D + chunk * 8;
 #pragma unroll 1
       for (int c = 0; c < kPR_D; c += 32) {
         uint32_t ow[32];
@@ -559,17 +588,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) ow[e] = 0u;
         }
-        uint32_t v[16];
+        if (c + 32 == kPR_D) {           // O is free as soon as the last of it is in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(of);
+        }
+        __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = pack16<T>(__uint_as_float(ow[2 * e]) * inv, __uint_as_float(ow[2 * e + 1]) * inv);
-        if (store) {
+        for (int e = 0; e < 4; ++e) {
+          uint32_t v[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out[c / 8 + e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          for (int i = 0; i < 4; ++i) v[i] = pack16<T>(__uint_as_float(ow[8 * e + 2 * i]) * inv, __uint_as_float(ow[8 * e + 2 * i + 1]) * inv);
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rr = 8 * i + r8;
+          if (q4 * 32 + rr < x.rows)
+            *reinterpret_cast<uint4*>(out + (size_t)rr * a.H * kPR_D + c) =
+                *reinterpret_cast<const uint4*>(stage + rr * 64 + ((chunk ^ ((rr >> 1) & 3)) << 4));
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(of);
     }
   }
   // neither CTA leaves while the other's products may read its shared memory or arrive on its barriers
@@ -627,6 +667,7 @@ int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void
   const long long nblk = (long long)T / a.qb + n_seq + 2;
   if (nblk > 0x7fffffffLL) return BF_ERR_UNSUPPORTED;
   a.nblk = (int)nblk;
+  a.qlog = a.qb == kPR_M ? 7 : 8;
   a.hsplit = R % 2 == 0 ? R / 2 : R;
   const long long clusters = nblk * G * a.hsplit;
   if (clusters > 0x3fffffffLL) return BF_ERR_UNSUPPORTED;
