@@ -335,24 +335,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 __device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// messages between the CTAs of a cluster through ordinary shared memory: store, release-arrive; acquire-wait, load
-__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t x) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint64_t* bar, uint32_t parity, volatile int* abort, unsigned int site) {
-  if (!mbar_wait_small(bar, parity, abort, site)) return false;
-  uint32_t ok;     // complete: this try only adds the scope
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
+// a word for another CTA's shared memory, completing 4 bytes on a barrier there (a release-arrive after an ordinary store waits
+// for every memory operation of the thread first: 5900 cycles beside a busy kernel's other warps)
+__device__ __forceinline__ void st_async_u32(uint32_t addr, uint32_t x, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(addr), "r"(x), "r"(bar)
+               : "memory");
 }
 // Cluster launch control: ask for a cluster of the grid that has not started yet, to do its work here.  The 16-byte answer
 // completes on `bar`; the first CTA index of the cluster, or -1 when none is left (then nothing may be asked again)

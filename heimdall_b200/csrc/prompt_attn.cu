@@ -380,21 +380,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           }
           __syncwarp();
           ok = mbar_wait_warp_small(clc, asked & 1, abort_flag, 0x92);
-          if (ok && asked >= 1) ok = __all_sync(0xffffffffu, mbar_wait_acquire_cluster(msg_free, (asked - 1) & 1, abort_flag, 0x93));
+          if (ok && asked >= 1) ok = mbar_wait_warp_small(msg_free, (asked - 1) & 1, abort_flag, 0x93);
           if (!ok) break;
           cta = clc_answer(answer);
           fence_async_smem();          // the answer has been read before the next one is written over it
-          if (lane == 0) {
-            st_cluster_u32(peer_msg, (uint32_t)cta);
-            mbar_arrive_release_cluster(peer_full);
-          }
+          if (lane == 0) st_async_u32(peer_msg, (uint32_t)cta, peer_full);
           __syncwarp();
         } else {
-          ok = __all_sync(0xffffffffu, mbar_wait_acquire_cluster(msg_full, asked & 1, abort_flag, 0x94));
-          if (!ok) break;
-          cta = *msg;
+          if (lane == 0) mbar_expect_tx(msg_full, 4);
           __syncwarp();
-          if (lane == 0) mbar_arrive_release_cluster(lead_free);
+          if (!(ok = mbar_wait_warp_small(msg_full, asked & 1, abort_flag, 0x94))) break;
+          cta = __shfl_sync(0xffffffffu, *msg, 0);
+          if (lane == 0) mbar_arrive_cluster(lead_free);       // the word has been read
         }
         ++asked;
       }
