@@ -18,8 +18,9 @@
 // Work: the tiles of 128 tokens of all (sequence, token chunk, KV head) segments in one line, cut into equal runs, one per CTA
 // (one CTA per SM), whatever the lengths; a segment's start counts as one tile more, as its queries and its output take about that long.  A segment inside one run is finished there; of a cut one each CTA writes its
 // partial (at most two per CTA), and paged_combine_kernel merges them in order, so results do not depend on timing.
-// Warps (640 threads): 0 TMA of the codes (a ring of 32 KB units K0 V0 K1 V1 ...) and the tiles' scales; 1 the products S; 2 the
-// next segment's Q parts; 3 the products O; 4-11 softmax (thread = token and the even or the odd rows); 12-19 the accumulators
+// Warps (640 threads): 0 and 2 TMA of the codes (K and V, each its own ring of 32 KB units), 0 also the tiles' scales;
+// 1 the products S; 3 the products O; 4-11 softmax (thread = token and the even or the odd rows) and, at the start of a segment,
+// the next one's Q parts (loaded a segment before; a warp of its own for them took 9000 cycles for 24 rows); 12-19 the accumulators
 // (thread = dim) and the output.
 // With one softmax warp per scheduler a tile took 6100 cycles, most of them the latency of that warp's own chain of
 // instructions; the rows are therefore dealt to two warpgroups, and what is the same for all tokens (a row's maximum and its
@@ -62,7 +63,8 @@ struct PagedAttnArgs {
 template <int RP>
 struct PagedCfg {
   static constexpr int NP = (3 * RP + 15) / 16 * 16;       // MMA N: three parts of RP rows, padded to 16
-  static constexpr int Units = RP == 8 ? 6 : 5;            // ring units that fit beside Q and P
+  static constexpr int KUnits = 3, VUnits = RP == 8 ? 3 : 2;   // ring units that fit beside Q and P
+  static constexpr int Units = KUnits + VUnits;
   static constexpr int TmemCols = 6 * NP <= 256 ? 256 : 512;   // S[2], O[2][2 halves]
   static constexpr int QBytes = NP * kPG_D, PBytes = NP * kPA_Tile;
   static constexpr int Smem = Units * kPA_Unit + 2 * QBytes + 2 * PBytes + 5120 + 1024;
@@ -105,6 +107,13 @@ struct PagedWalk {
     c = 0;
     if (++b < a.B) enter(a);
   }
+  // on to the next segment; returns this one's tiles from `tile` on
+  __device__ __forceinline__ int skip(const PagedAttnArgs& a) {
+    const int n = ntiles - tile;
+    tile = ntiles - 1;
+    next(a);
+    return n;
+  }
 };
 
 // x = (x0 + x1 / 16 + x2 / 256) with e4m3 parts, for |x| <= 256; two values at a time.  x is first rounded to fp16, whose 11
@@ -137,7 +146,7 @@ template <typename T, int RP>
 __global__ void __launch_bounds__(kPA_Threads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PagedAttnArgs a) {
   using C = PagedCfg<RP>;
-  constexpr int NP = C::NP, NU = C::Units;
+  constexpr int NP = C::NP, NU = C::Units, NK = C::KUnits, NV = C::VUnits;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem;
@@ -171,7 +180,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       mbar_init(p_full + i, 8);
       mbar_init(o_full + i, 1);
       mbar_init(o_free + i, 8);
-      mbar_init(q_full + i, 1);
+      mbar_init(q_full + i, 8);
       mbar_init(q_free + i, 9);
       mbar_init(seg_full + i, 8);
       mbar_init(seg_free + i, 8);
@@ -266,13 +275,15 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     return page >= 0 && page < a.p.pages ? page : -1;
   };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ codes
-    if (lane == 0) {
-      tma_prefetch(&kmap);
-      tma_prefetch(&vmap);
-    }
-    int unit = 0, u = 0, uphase = 1;      // uphase: the parity of the round before
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------------ codes: K (warp 0), V (warp 2)
+    const bool is_v = warp == 2;
+    const void* map = is_v ? &vmap : &kmap;
+    if (lane == 0) tma_prefetch(map);
+    // each ring has one producer, which waits for its slots' rounds one by one (with K and V in one ring of an odd number of slots, a
+    // producer could meet a slot two rounds behind and take the parity of the round before for its own)
+    const int units = is_v ? NV : NK, base = is_v ? NK : 0;
+    int u = 0, uphase = 1;                // the unit's slot of the ring; the parity of the round before
     bool ok = true;
     // each lane a page of the tile: page numbers are loaded two tiles ahead, scales one, so that no load is waited for here
     int now = -1, next = -1, g = 0, g_next = 0, ahead = 0;
@@ -288,19 +299,18 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     };
     auto scales = [&]() {
       ks_next = vs_next = 0.f;
-      if (now >= 0) {
+      if (now >= 0 && !is_v) {
         ks_next = a.p.ks[(size_t)now * a.p.heads + g];
         vs_next = a.p.vs[(size_t)now * a.p.heads + g];
       }
     };
     step();
-    int after = next, g_after = g_next;   // tile j + 1's page, loaded before tile j's turn
+    now = next;
+    g = g_next;
     step();
-    now = after;
-    g = g_after;
     scales();
 #pragma unroll 1
-    for (int j = 0; j < count && ok; ++j) {
+    for (int j = 0; j < count; ++j) {
       const float ks = ks_next, vs = vs_next;
       const int page = now, head = g;
       now = next;
@@ -309,31 +319,27 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       scales();
       const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
       const int first_row = page >= 0 ? (page * a.p.heads + head) * L : 0;
+      if (j >= units && !(ok = mbar_wait_warp_small(empty + base + u, uphase, abort_flag, 0x60))) break;
+      if (lane == 0) {
+        if (have) mbar_expect_tx(full + base + u, (uint32_t)__popc(have) * L * kPG_D); else mbar_arrive(full + base + u);
+      }
+      __syncwarp();
+      // page by page with operands that all lanes agree on: eight lanes issuing their own pages took 150 cycles per copy
 #pragma unroll 1
-      for (int kv = 0; kv < 2; ++kv, ++unit) {
-        if (unit >= NU && !(ok = mbar_wait_warp_small(empty + u, uphase, abort_flag, 0x60))) break;
-        if (lane == 0) {
-          if (have) mbar_expect_tx(full + u, (uint32_t)__popc(have) * L * kPG_D); else mbar_arrive(full + u);
+      for (int i = 0; i < ppt; ++i) {
+        const int row = __shfl_sync(0xffffffffu, first_row, i);
+        if (((have >> i) & 1u) && elect_one()) {
+          uint8_t* dst = ring + (base + u) * kPA_Unit + i * L * 128;
+          tma_load_2d(dst, map, full + base + u, 0, row);
+          tma_load_2d(dst + kPA_Tile * 128, map, full + base + u, 128, row);
         }
         __syncwarp();
-        // page by page with operands that all lanes agree on: eight lanes issuing their own pages took 150 cycles per copy
-        const void* map = kv ? &vmap : &kmap;
-#pragma unroll 1
-        for (int i = 0; i < ppt; ++i) {
-          const int row = __shfl_sync(0xffffffffu, first_row, i);
-          if (((have >> i) & 1u) && elect_one()) {
-            uint8_t* dst = ring + u * kPA_Unit + i * L * 128;
-            tma_load_2d(dst, map, full + u, 0, row);
-            tma_load_2d(dst + kPA_Tile * 128, map, full + u, 128, row);
-          }
-          __syncwarp();
-        }
-        if (++u == NU) {
-          u = 0;
-          uphase ^= 1;
-        }
       }
-      if (!ok) break;
+      if (++u == units) {
+        u = 0;
+        uphase ^= 1;
+      }
+      if (is_v) continue;
       // the tile's scales, their loads as old as its TMA's
       const int s = j & 3;
       const float top = warp_max(vs);
@@ -349,10 +355,8 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_full + s);
     }
-    // every load issued has landed before the CTA may exit: the products have read it, or it is waited for here
-    if (*abort_flag) {
-      for (int i = unit > NU ? unit - NU : 0; i < unit; ++i) mbar_wait(full + i % NU, (i / NU) & 1, nullptr, a.err, 0x61);
-    }
+    // every load issued has landed before the CTA may exit: the products have read it, or, with a wait that gave up, report_abort
+    // gives it time
   } else if (warp == 1) {
     // ------------------------------------------------------------------ S = K Q^T
     constexpr uint32_t id_s = idesc_e4m3(kPA_Tile, NP);
@@ -381,9 +385,8 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       __syncwarp();
       seg += end;
       w.next(a);
-      u += 2;
-      if (u >= NU) {
-        u -= NU;
+      if (++u == NK) {
+        u = 0;
         uphase ^= 1;
       }
     }
@@ -391,99 +394,29 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     // ------------------------------------------------------------------ O = V^T P^T
     constexpr uint32_t id_o = idesc_e4m3(128, NP) | kIdescAMn;
     const uint64_t dv0 = sdesc_sw128_mn(smem_u32(ring), 16384), dp0 = sdesc_sw128(smem_u32(sP));
-    int u = 1, uphase = 0;
+    int u = 0, uphase = 0;
 #pragma unroll 1
     for (int j = 0; j < count; ++j) {
       const int s = j & 1;
-      if (!mbar_wait_warp_small(full + u, uphase, abort_flag, 0x63)) break;
+      if (!mbar_wait_warp_small(full + NK + u, uphase, abort_flag, 0x63)) break;
       if (!mbar_wait_warp_small(p_full + s, (j >> 1) & 1, abort_flag, 0x62)) break;
       if (j >= 2 && !mbar_wait_warp_small(o_free + s, ((j >> 1) - 1) & 1, abort_flag, 0x64)) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t dv = dv0 + (uint32_t)(u * (kPA_Unit >> 4)), dp = dp0 + (uint32_t)(s * (C::PBytes >> 4));
+        const uint64_t dv = dv0 + (uint32_t)((NK + u) * (kPA_Unit >> 4)), dp = dp0 + (uint32_t)(s * (C::PBytes >> 4));
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
             umma_f8_ss(tmem + 2 * NP + (2 * s + half) * NP, dv + (half * 16384 + ks * 4096) / 16, dp + ks * 32 / 16, id_o, ks > 0);
         umma_commit(o_full + s);
-        umma_commit(empty + u);
+        umma_commit(empty + NK + u);
       }
       __syncwarp();
-      u += 2;
-      if (u >= NU) {
-        u -= NU;
+      if (++u == NV) {
+        u = 0;
         uphase ^= 1;
       }
-    }
-  } else if (warp == 2) {
-    // ------------------------------------------------------------------ Q parts of each segment
-    bool ok = true;
-    int seg = 0;
-#pragma unroll 1
-    for (int j = 0; j < count && ok;) {
-      if (seg >= 2 && !(ok = mbar_wait_warp_small(q_free + (seg & 1), ((seg >> 1) - 1) & 1, abort_flag, 0x68))) break;
-      uint8_t* dst = sQ + (seg & 1) * C::QBytes;
-      const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
-      // two rows at a time, 16 lanes each, every load of four rows before their arithmetic; rows from `rows` on stay as they are,
-      // nothing reads their scores
-      const int r2 = lane >> 4, dim = (lane & 15) * 16;
-#pragma unroll 1
-      for (int r0 = 0; r0 < rows; r0 += 4) {
-        uint4 raw[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = min(r0 + 2 * i + r2, rows - 1);
-          const int2 ih = paged_row(a, r);
-          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + w.b * a.q_sb + (long long)(i0 + ih.x) * a.q_st +
-                                                            (long long)(w.g * a.R + ih.y) * a.q_sh + dim);
-          raw[i][0] = __ldg(src);
-          raw[i][1] = __ldg(src + 1);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = min(r0 + 2 * i + r2, rows - 1);       // the last row may be written twice, with the same values
-          const T* e = reinterpret_cast<const T*>(raw[i]);
-          float m = 0.f;
-          bool fin = true;
-#pragma unroll
-          for (int q = 0; q < 16; ++q) {
-            const float x = fabsf((float)e[q]);
-            fin = fin && x < INFINITY;
-            m = fmaxf(m, x);
-          }
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          fin = ((__ballot_sync(0xffffffffu, fin) >> (lane & 16)) & 0xffffu) == 0xffffu;
-          // the row's largest value to [128, 256): x * 2^k, k = 7 - exponent
-          const int ex = m > 0.f ? max((int)(__float_as_uint(m) >> 23), 16) : 127;
-          const float up = fin ? __uint_as_float((uint32_t)(254 + 7 - ex) << 23) : 0.f;
-          uint32_t word[3][4];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            uint16_t c[3];
-            split3(fin ? (float)e[2 * q] * up : 0.f, fin ? (float)e[2 * q + 1] * up : 0.f, c);
-#pragma unroll
-            for (int part = 0; part < 3; ++part) word[part][q >> 1] = q & 1 ? word[part][q >> 1] | ((uint32_t)c[part] << 16) : c[part];
-          }
-#pragma unroll
-          for (int part = 0; part < 3; ++part) {
-            const int n = part * RP + row_col<RP>(r);
-            *reinterpret_cast<uint4*>(dst + (dim >> 7) * (NP * 128) + n * 128 + ((((dim & 127) >> 4) ^ (n & 7)) << 4)) =
-                make_uint4(word[part][0], word[part][1], word[part][2], word[part][3]);
-          }
-          // a row with a value that is not finite has no finite scores
-          if ((lane & 15) == 0) s_qs[(seg & 1) * RP + row_col<RP>(r)] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
-        }
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full + (seg & 1));
-      ++seg;
-      const int left = w.ntiles - w.tile;        // on to the next segment
-      j += left;
-      w.tile = w.ntiles - 1;
-      w.next(a);
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------------ softmax: thread = token of the tile, rows 2 i + hh
@@ -495,22 +428,87 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     float m_run = -INFINITY;             // of row 2 lane + hh, in lanes < RH
     bool ok = true, first = true;
     int seg = 0;
+    // the queries: warp w of the eight takes rows w, w + 8, w + 16, lane l dims 8 l .. 8 l + 7
+    PagedWalk nx = w;                    // the segment whose queries are in `raw`
+    int nx_at = 0, nx_rows = 0;          // its first tile in the run
+    uint4 qraw[RP / 8];
+    auto q_load = [&]() {
+      const int i0 = nx.c * a.tc;
+      nx_rows = min(a.tc, a.t - i0) * a.R;
+#pragma unroll
+      for (int i = 0; i < RP / 8; ++i) {
+        const int r = warp - 4 + 8 * i;
+        const int2 ih = paged_row(a, r);
+        if (r < nx_rows)
+          qraw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + nx.b * a.q_sb + (long long)(i0 + ih.x) * a.q_st +
+                                                         (long long)(nx.g * a.R + ih.y) * a.q_sh + 8 * lane));
+      }
+    };
+    auto q_store = [&](int buf) {        // rows from nx_rows on stay as they are, nothing reads their scores
+      uint8_t* dst = sQ + buf * C::QBytes + (lane >> 4) * (NP * 128) + (lane & 1) * 8;
+#pragma unroll
+      for (int i = 0; i < RP / 8; ++i) {
+        const int r = warp - 4 + 8 * i;
+        if (r >= nx_rows) break;
+        const uint32_t u[4] = {qraw[i].x, qraw[i].y, qraw[i].z, qraw[i].w};
+        // the largest value of the row, as 16-bit patterns without their sign
+        const uint32_t m2 = __vmaxu2(__vmaxu2(u[0] & 0x7fff7fffu, u[1] & 0x7fff7fffu), __vmaxu2(u[2] & 0x7fff7fffu, u[3] & 0x7fff7fffu));
+        const uint32_t m = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
+        const uint16_t m16 = (uint16_t)m;
+        const float mf = (float)*reinterpret_cast<const T*>(&m16);
+        const bool fin = mf < INFINITY;          // false for NaN too
+        // to [128, 256): x * 2^k, k = 7 - exponent
+        const int ex = mf > 0.f ? max((int)(__float_as_uint(mf) >> 23), 16) : 127;
+        const float up = fin ? __uint_as_float((uint32_t)(254 + 7 - ex) << 23) : 0.f;
+        uint16_t c[4][3];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const T* e = reinterpret_cast<const T*>(&u[q]);
+          split3(fin ? (float)e[0] * up : 0.f, fin ? (float)e[1] * up : 0.f, c[q]);
+        }
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+          const int n = part * RP + row_col<RP>(r);
+          *reinterpret_cast<uint2*>(dst + n * 128 + ((((lane & 15) >> 1) ^ (n & 7)) << 4)) =
+              make_uint2(c[0][part] | ((uint32_t)c[1][part] << 16), c[2][part] | ((uint32_t)c[3][part] << 16));
+        }
+        // a row with a value that is not finite has no finite scores
+        if (lane == 0) s_qs[buf * RP + row_col<RP>(r)] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + buf);
+      nx_at += nx.skip(a);
+      if (nx_at < count) q_load();
+    };
+    if (count > 0) q_load();
 #pragma unroll 1
     for (int j = 0; j < count; ++j) {
       const int s = j & 1;
       if (first) {
-        if (!(ok = mbar_wait_warp_small(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, 0x6a))) break;
-        const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
-        m_run = -INFINITY;
+        // store the next segment's queries (and, at the run's start, this one's before them)
+#pragma unroll 1
+        for (int k = j ? 1 : 0; k < 2 && ok; ++k) {
+          if (k) {
+            if (!(ok = mbar_wait_warp_small(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, 0x6a))) break;
+            const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
+            m_run = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < RH; ++i) {
-          const int r = 2 * i + hh;
-          l[i] = 0.f;
-          qs[i] = s_qs[(seg & 1) * RP + hh * RH + i];
-          lim[i] = r < rows ? w.len - a.t + i0 + paged_row(a, r).x : -1;     // the row's last visible position
+            for (int i = 0; i < RH; ++i) {
+              const int r = 2 * i + hh;
+              l[i] = 0.f;
+              qs[i] = s_qs[(seg & 1) * RP + hh * RH + i];
+              lim[i] = r < rows ? w.len - a.t + i0 + paged_row(a, r).x : -1;     // the row's last visible position
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_free + (seg & 1));
+          }
+          if (nx_at < count) {
+            if (k && seg >= 1 && !(ok = mbar_wait_warp_small(q_free + ((seg + 1) & 1), (((seg + 1) >> 1) - 1) & 1, abort_flag, 0x68))) break;
+            q_store((seg + k) & 1);
+          }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_free + (seg & 1));
+        if (!ok) break;
       }
       const bool last = w.tile + 1 == w.ntiles, end = last || j + 1 == count;
       if (!(ok = mbar_wait_warp_small(sc_full + (j & 3), (j >> 2) & 1, abort_flag, 0x6b))) break;
@@ -586,8 +584,8 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       }
       if (__any_sync(0xffffffffu, !valid)) {
         // the values of tokens that are not there may be anything (a weight of 0 times NaN would be NaN): zeros
-        const int u = (2 * j + 1) % NU;
-        if (!(ok = mbar_wait_warp_small(full + u, ((2 * j + 1) / NU) & 1, abort_flag, 0x6f))) break;
+        const int u = NK + j % NV;
+        if (!(ok = mbar_wait_warp_small(full + u, (j / NV) & 1, abort_flag, 0x6f))) break;
         if (!valid) {
           uint4* row = reinterpret_cast<uint4*>(ring + u * kPA_Unit + hh * (kPA_Tile * 128) + tok * 128);
 #pragma unroll

@@ -199,6 +199,16 @@ def test_attend_longer_and_slots_in_any_order():
     _check_attend(c, q[:2] * 6, [4, 2], scale=0.3, layer=1)
 
 
+@pytest.mark.parametrize("H,t,page", [(6, 4, 16), (6, 2, 64), (12, 2, 32), (5, 3, 128)])
+def test_attend_several_tokens_over_long_and_short_sequences(H, t, page):
+    """Rows in every size of block (16 and 24 at a time), runs of many tiles and of many segments in one CTA."""
+    lens = [7000, 4, 130, 40, 2900] + [5 + 3 * i for i in range(40)] + [1500]
+    c = _cache(1, sum(-(-n // page) for n in lens), 1, len(lens), page=page, max_len=7040)
+    c.reserve(range(len(lens)), lens)
+    _fill(c, 9)
+    _check_attend(c, _rand(len(lens), t, H, D, seed=11, dtype=torch.float16), None)
+
+
 def test_attend_many_sequences():
     n = 150
     lens = [(37 * i) % 200 for i in range(n)]
