@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 41);
   long long* s_sum = reinterpret_cast<long long*>(bars + 42);       // [20] per-warp totals of the unit count
   int* s_start = reinterpret_cast<int*>(bars + 63);                 // b, segment of it, tile of that
-  float* s_qs = reinterpret_cast<float*>(bars + 65);                // [2][RP] scale of the Q rows
+  float* s_qs = reinterpret_cast<float*>(bars + 66);                // [2][RP] scale of the Q rows
   float* s_fac = s_qs + 2 * kPA_MaxRows;                            // [2][RP][2] factors of the tile's O^T and the accumulators
   float* s_red = s_fac + 4 * kPA_MaxRows;                           // [2][4][RP] the warps' maxima
   float* s_seg = s_red + 8 * kPA_MaxRows;                           // [2][5][RP] a segment's sums per warp, its maximum
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     const int wq = warp & 3, hh = (warp - 4) >> 2, tok = wq * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + hh * RH;
     float l[RH], qs[RH];
-    int lim[RH];
+    int rows = 0, first_pos = 0;         // of the chunk; the position of its first token
     float m_run = -INFINITY;             // of row 2 lane + hh, in lanes < RH
     bool ok = true, first = true;
     int seg = 0;
@@ -491,14 +491,13 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         for (int k = j ? 1 : 0; k < 2 && ok; ++k) {
           if (k) {
             if (!(ok = mbar_wait_warp_small(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, 0x6a))) break;
-            const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
+            rows = min(a.tc, a.t - w.c * a.tc) * a.R;
+            first_pos = w.len - a.t + w.c * a.tc;
             m_run = -INFINITY;
 #pragma unroll
             for (int i = 0; i < RH; ++i) {
-              const int r = 2 * i + hh;
               l[i] = 0.f;
               qs[i] = s_qs[(seg & 1) * RP + hh * RH + i];
-              lim[i] = r < rows ? w.len - a.t + i0 + paged_row(a, r).x : -1;     // the row's last visible position
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(q_free + (seg & 1));
@@ -518,6 +517,9 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       const bool there = (__float_as_uint(sc[17]) >> pi) & 1u;
       const int pos = w.tile * kPA_Tile + tok;
       const bool valid = there && pos < w.len;
+      // bit r: row r's token is at or behind this position (the first of them is that many tokens into the chunk)
+      const unsigned later = (unsigned)min(max(pos - first_pos, 0) * a.R, 31);
+      const unsigned sees = valid ? (((1u << rows) - 1u) >> later << later) >> hh : 0u;
       __syncwarp();
       if (lane == 0) mbar_arrive(sc_free + (j & 3));
       if (!(ok = mbar_wait_warp_small(s_full + s, (j >> 1) & 1, abort_flag, 0x6c))) break;
@@ -538,7 +540,10 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
 #pragma unroll
       for (int i = 0; i < RH; ++i) {
         const float d = __uint_as_float(raw[i]) + (__uint_as_float(raw[RH + i]) + __uint_as_float(raw[2 * RH + i]) * 0.0625f) * 0.0625f;
-        x[i] = valid && pos <= lim[i] ? d * (ks * qs[i]) : -INFINITY;
+        x[i] = (sees >> (2 * i)) & 1u ? d * (ks * qs[i]) : -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < RH; ++i) {
         float mx;
         asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(mx) : "f"(x[i]));
         if (lane == i) mine = mx;
@@ -628,15 +633,19 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       if (!(ok = mbar_wait_warp_small(p_full + s, (j >> 1) & 1, abort_flag, 0x73))) break;   // the factors
       if (!(ok = mbar_wait_warp_small(o_full + s, (j >> 1) & 1, abort_flag, 0x71))) break;
       tc_fence_after();
-      uint32_t raw[3 * RP];
+      // eight rows at a time (all of RP = 24 at once would not fit the registers)
 #pragma unroll
-      for (int c = 0; c < 3 * RP; c += 8) tmem_ld8(trow + 2 * s * NP + c, raw + c);
-      tmem_wait_ld();
+      for (int c0 = 0; c0 < RP; c0 += 8) {
+        uint32_t raw[24];
 #pragma unroll
-      for (int c = 0; c < RP; ++c) {
-        const float2 fac = *reinterpret_cast<const float2*>(s_fac + (s * RP + c) * 2);
-        const float x = __uint_as_float(raw[c]) + (__uint_as_float(raw[RP + c]) + __uint_as_float(raw[2 * RP + c]) * 0.0625f) * 0.0625f;
-        acc[c] = acc[c] * fac.x + x * fac.y;
+        for (int part = 0; part < 3; ++part) tmem_ld8(trow + 2 * s * NP + part * RP + c0, raw + part * 8);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 fac = *reinterpret_cast<const float2*>(s_fac + (s * RP + c0 + i) * 2);
+          const float x = __uint_as_float(raw[i]) + (__uint_as_float(raw[8 + i]) + __uint_as_float(raw[16 + i]) * 0.0625f) * 0.0625f;
+          acc[c0 + i] = acc[c0 + i] * fac.x + x * fac.y;
+        }
       }
       tc_fence_before();
       __syncwarp();
