@@ -16,8 +16,9 @@
 // carry the running maximum: nothing is rescaled in TMEM.  V's scales go into P (as their ratio to the tile's largest).
 //
 // Work: the tiles of 128 tokens of all (sequence, token chunk, KV head) segments in one line, cut into equal runs, one per CTA
-// (one CTA per SM), whatever the lengths; a segment's start counts as one tile more, as its queries and its output take about that long.  A segment inside one run is finished there; of a cut one each CTA writes its
-// partial (at most two per CTA), and paged_combine_kernel merges them in order, so results do not depend on timing.
+// (one CTA per SM), whatever the lengths; a segment's start counts as two or three tiles, as its queries and its
+// output take about that long.  A segment inside one run is finished there; of a cut one each CTA writes its partial (at most two
+// per CTA), and paged_combine_kernel merges them in order, so results do not depend on timing.
 // Warps (640 threads): 0 and 2 TMA of the codes (K and V, each its own ring of 32 KB units), 0 also the tiles' scales;
 // 1 the products S; 3 the products O; 4-11 softmax (thread = token and the even or the odd rows) and, at the start of a segment,
 // the next one's Q parts (loaded a segment before; a warp of its own for them took 9000 cycles for 24 rows); 12-19 the accumulators
@@ -65,6 +66,9 @@ struct PagedCfg {
   static constexpr int NP = (3 * RP + 15) / 16 * 16;       // MMA N: three parts of RP rows, padded to 16
   static constexpr int KUnits = 3, VUnits = RP == 8 ? 3 : 2;   // ring units that fit beside Q and P
   static constexpr int Units = KUnits + VUnits;
+  // what a segment's start counts, in tiles.  64 sequences of 1 to 16384 tokens, 8 rows: 67, 59 and 59 us with 1, 2 and 3, 32 of 3000 to
+  // 6100: 71, 70 and 72; 32 of 4 to 32768 tokens, 24 rows: 143, 122 and 117 us
+  static constexpr int Start = RP == 8 ? 2 : 3;
   static constexpr int TmemCols = 6 * NP <= 256 ? 256 : 512;   // S[2], O[2][2 halves]
   static constexpr int QBytes = NP * kPG_D, PBytes = NP * kPA_Tile;
   static constexpr int Smem = Units * kPA_Unit + 2 * QBytes + 2 * PBytes + 5120 + 1024;
@@ -197,14 +201,14 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     tmem_alloc(tmem_slot, C::TmemCols);
     tmem_relinquish();
   }
-  // this CTA's run: every segment is one unit and one for each of its tiles.  The sequences' units are summed over the block,
+  // this CTA's run: every segment is Start units and one for each of its tiles.  The sequences' units are summed over the block,
   // thread i holding `per` consecutive sequences
   const int per = (a.B + kPA_Threads - 1) / kPA_Threads;
   const int segs = a.nqc * a.p.heads;
   long long mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
-    if (b < a.B) mine += (long long)(paged_tiles(paged_seq(a, b).y) + 1) * segs;
+    if (b < a.B) mine += (long long)(paged_tiles(paged_seq(a, b).y) + C::Start) * segs;
   }
   long long incl = mine;
 #pragma unroll
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
   if (u0 < u1 && before <= u0 && u0 < before + mine) {
     long long at = before;
     for (int b = tid * per;; ++b) {
-      const int n = paged_tiles(paged_seq(a, b).y) + 1;
+      const int n = paged_tiles(paged_seq(a, b).y) + C::Start;
       if (u0 < at + (long long)n * segs) {
         s_start[0] = b;
         s_start[1] = (int)((u0 - at) / n);
@@ -254,13 +258,13 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     w.c = s_start[1] / a.p.heads;
     w.g = s_start[1] % a.p.heads;
     w.enter(a);
-    w.tile = max(s_start[2] - 1, 0);
+    w.tile = max(s_start[2] - C::Start, 0);
     // walk the run's segments: the units of each that are tiles
     PagedWalk x = w;
     for (long long u = u0 - s_start[2]; u < u1;) {
-      const long long lo = max(u + 1, u0), hi = min(u + 1 + x.ntiles, u1);
+      const long long lo = max(u + C::Start, u0), hi = min(u + C::Start + x.ntiles, u1);
       if (hi > lo) count += (int)(hi - lo);
-      u += x.ntiles + 1;
+      u += x.ntiles + C::Start;
       x.tile = x.ntiles - 1;
       x.next(a);
     }
@@ -623,7 +627,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     float acc[RP];
     bool ok = true, from_start = w.tile == 0;
     int seg = 0;
-    long long unit = u0 + (count > 0 && s_start[2] == 0 ? 1 : 0);      // the tile's
+    long long unit = count > 0 ? u0 + max(C::Start - s_start[2], 0) : 0;      // the tile's
     int4 desc = make_int4(-1, 0, 0, 0);
 #pragma unroll
     for (int c = 0; c < RP; ++c) acc[c] = 0.f;
@@ -690,7 +694,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         if (lane == 0) mbar_arrive(seg_free + (seg & 1));
         ++seg;
         from_start = true;
-        ++unit;                  // the next segment's start
+        unit += C::Start;
       }
       ++unit;
       w.next(a);
