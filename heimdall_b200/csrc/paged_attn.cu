@@ -41,7 +41,7 @@ constexpr int kPA_Tile = 128;                        // tokens per tile
 constexpr int kPA_Unit = kPA_Tile * kPG_D;           // bytes of one K or V tile
 constexpr int kPA_MaxCtas = 160;
 constexpr int kPA_MaxRows = 24;
-constexpr int kPA_Part = kPG_D + 2;                  // floats of a row's partial: accumulator, maximum, sum
+constexpr int kPA_Part = kPG_D + 4;                  // floats of a row's partial: accumulator, maximum, sum, two to keep it aligned
 
 struct PagedAttnArgs {
   PagePool p;
@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     *abort_flag = 0;
     fence_barrier_init();
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TmemCols);
     tmem_relinquish();
@@ -710,54 +711,69 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
   }
 }
 
-// Block (x, r, z): dims 64 z .. 64 z + 63 of row r of the cut segment that ends in CTA x, if there is one: the partials of the
-// CTAs first .. x, a quarter of them per group of 64 threads, then the four groups' results, always in the same order
+// Block (x, y): a quarter of the rows and dims of the cut segment that ends in CTA x, if there is one: the partials of the CTAs
+// first .. x, added in order, four dims per thread.  Up to eight partials are loaded at once; more are dealt to the block's eight warps,
+// whose results are added in order.  (One block per row and 64 dims took 12 us for 8 rows and 32 us for 24, most of it block starts.)
 template <typename T, int RP>
 __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttnArgs a) {
-  __shared__ float s_m[4], s_l[4], s_acc[4][64];
-  const int x = blockIdx.x, r = blockIdx.y, grp = threadIdx.x >> 6, d = blockIdx.z * 64 + (threadIdx.x & 63);
+  __shared__ float4 s_acc[8][32];
+  __shared__ float2 s_ml[8][32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int x = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int4 desc = a.desc[x];
   if (desc.x < 0) return;
-  const int i0 = desc.z * a.tc;
-  if (r >= min(a.tc, a.t - i0) * a.R) return;
-  const int n = x - desc.x + 1, each = (n + 3) / 4, c_end = min(desc.x + (grp + 1) * each, x + 1);
-  auto part = [&](int c) { return a.part + (((size_t)c * 2 + (c == desc.x ? 1 : 0)) * RP + r) * kPA_Part; };
-  float m = -INFINITY, sum = 0.f, acc = 0.f;
-  // a partial without a maximum holds zeros, or NaN to be passed on
-  auto add = [&](float mv, float lv, float av) {
-    const float mn = fmaxf(m, mv);
-    const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = mv == -INFINITY ? 1.f : ex2_approx(mv - mn);
-    acc = acc * al + av * f;
-    sum = sum * al + lv * f;
-    m = mn;
-  };
-  for (int c0 = desc.x + grp * each; c0 < c_end; c0 += 16) {
-    float mv[16], lv[16], av[16];
+  const int i0 = desc.z * a.tc, items = min(a.tc, a.t - i0) * a.R * (kPG_D / 4);
+  const int n = x - desc.x + 1, lo = (int)((long long)items * blockIdx.y / gridDim.y), hi = (int)((long long)items * (blockIdx.y + 1) / gridDim.y);
+  const bool few = n <= 8;
+  const int each = few ? n : (n + 7) / 8, c_lo = few ? 0 : min(warp * each, n), c_hi = few ? n : min(c_lo + each, n);
+  for (int it0 = lo; it0 < hi; it0 += few ? 256 : 32) {
+    const int it = it0 + (few ? tid : lane), r = min(it, hi - 1) / (kPG_D / 4), d = (min(it, hi - 1) % (kPG_D / 4)) * 4;
+    float m = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // a partial without a maximum holds zeros, or NaN to be passed on
+    auto add = [&](float mv, float lv, const float4& v) {
+      const float mn = fmaxf(m, mv);
+      const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = mv == -INFINITY ? 1.f : ex2_approx(mv - mn);
+      acc.x = acc.x * al + v.x * f;
+      acc.y = acc.y * al + v.y * f;
+      acc.z = acc.z * al + v.z * f;
+      acc.w = acc.w * al + v.w * f;
+      sum = sum * al + lv * f;
+      m = mn;
+    };
+    for (int c0 = c_lo; c0 < c_hi; c0 += 8) {
+      float4 v[8];
+      float2 ml[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float* p = part(min(c0 + i, x));
-      const bool in = c0 + i < c_end;
-      av[i] = in ? p[d] : 0.f;
-      mv[i] = in ? p[kPG_D] : -INFINITY;
-      lv[i] = in ? p[kPG_D + 1] : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const int c = desc.x + min(c0 + i, c_hi - 1);
+        const float* p = a.part + (((size_t)c * 2 + (c == desc.x ? 1 : 0)) * RP + r) * kPA_Part;
+        v[i] = *reinterpret_cast<const float4*>(p + d);
+        ml[i] = *reinterpret_cast<const float2*>(p + kPG_D);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i < c_hi) add(ml[i].x, ml[i].y, v[i]);
     }
+    if (!few) {
+      __syncthreads();
+      s_acc[warp][lane] = acc;
+      s_ml[warp][lane] = make_float2(m, sum);
+      __syncthreads();
+      if (warp == 0) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) add(mv[i], lv[i], av[i]);
+        for (int k = 1; k < 8; ++k) add(s_ml[k][lane].x, s_ml[k][lane].y, s_acc[k][lane]);
+      }
+    }
+    if (it < hi && (few || warp == 0)) {
+      const int2 ih = paged_row(a, r);
+      const int i = i0 + ih.x, h = desc.w * a.R + ih.y;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      T o[4] = {(T)(acc.x * inv), (T)(acc.y * inv), (T)(acc.z * inv), (T)(acc.w * inv)};
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + (((size_t)desc.y * a.t + i) * a.H + h) * kPG_D + d) = *reinterpret_cast<uint2*>(o);
+      if (a.lse && d == 0) a.lse[((size_t)desc.y * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+    }
   }
-  s_acc[grp][threadIdx.x & 63] = acc;
-  if ((threadIdx.x & 63) == 0) {
-    s_m[grp] = m;
-    s_l[grp] = sum;
-  }
-  __syncthreads();
-  if (grp) return;
-#pragma unroll
-  for (int i = 1; i < 4; ++i) add(s_m[i], s_l[i], s_acc[i][threadIdx.x]);
-  const int2 ih = paged_row(a, r);
-  const int i = i0 + ih.x, h = desc.w * a.R + ih.y;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  static_cast<T*>(a.o)[(((size_t)desc.y * a.t + i) * a.H + h) * kPG_D + d] = (T)(acc * inv);
-  if (a.lse && d == 0) a.lse[((size_t)desc.y * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
 }
 
 // rows at a time for t tokens of R query heads: as many whole tokens as 24 rows hold, in equal chunks
@@ -774,8 +790,18 @@ static int launch_paged(const CUtensorMap& kmap, const CUtensorMap& vmap, const 
   if (rc) return rc;
   paged_attn_kernel<T, RP><<<ctas, kPA_Threads, PagedCfg<RP>::Smem, stream>>>(kmap, vmap, a);
   if ((rc = launch_status())) return rc;
-  paged_combine_kernel<T, RP><<<dim3(ctas, a.tc * a.R, kPG_D / 64), 256, 0, stream>>>(a);
-  return launch_status();
+  // may start while the last CTAs of the first kernel run, and waits for their results itself
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas, 4);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_combine_kernel<T, RP>, a);
+  return e == cudaSuccess ? BF_OK : cuda_fail(e);
 }
 
 }  // namespace bfb
