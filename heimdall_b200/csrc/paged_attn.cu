@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
            *seg_full = bars + 36, *seg_free = bars + 38;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 40);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 41);
-  long long* s_sum = reinterpret_cast<long long*>(bars + 42);       // [20] per-warp totals of the unit count
+  int* s_sum = reinterpret_cast<int*>(bars + 42);                   // [20] per-warp totals of the unit count
   int* s_start = reinterpret_cast<int*>(bars + 63);                 // b, segment of it, tile of that
   float* s_qs = reinterpret_cast<float*>(bars + 66);                // [2][RP] scale of the Q rows
   float* s_fac = s_qs + 2 * kPA_MaxRows;                            // [2][RP][2] factors of the tile's O^T and the accumulators
@@ -203,68 +203,70 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     tmem_relinquish();
   }
   // this CTA's run: every segment is Start units and one for each of its tiles.  The sequences' units are summed over the block,
-  // thread i holding `per` consecutive sequences
+  // thread i holding `per` consecutive sequences (the caller has made sure that 32 bits hold the sum)
   const int per = (a.B + kPA_Threads - 1) / kPA_Threads;
   const int segs = a.nqc * a.p.heads;
-  long long mine = 0;
+  const bool known = a.B <= kPA_Seqs;          // all sequences fit into s_seqs
+  int mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
-    if (b < a.B) mine += (long long)(paged_tiles(paged_seq(a, b).y) + C::Start) * segs;
+    if (b < a.B) {
+      const int2 q = paged_seq(a, b);
+      mine += (paged_tiles(q.y) + C::Start) * segs;
+      if (known) s_seqs[b] = q;
+    }
   }
-  long long incl = mine;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+    const int x = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += x;
   }
   if (lane == 31) s_sum[warp] = incl;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  long long total = 0, before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < kPA_Threads / 32; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
-  const long long ctas = total < gridDim.x ? total : gridDim.x, x0 = min((long long)blockIdx.x, ctas);
-  const long long u0 = total * x0 / ctas, u1 = total * min(x0 + 1, ctas) / ctas;
+  int total = lane < kPA_Threads / 32 ? s_sum[lane] : 0, before = lane < warp ? total : 0;
+  total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
+  before = (int)__reduce_add_sync(0xffffffffu, (unsigned)before) + incl - mine;
+  // with fewer units than CTAs the first `total` CTAs take one each; the first `more` runs are one unit longer than the others
+  const int ctas = min(total, (int)gridDim.x), each = total / ctas, more = total - each * ctas;
+  const int u0 = min((int)blockIdx.x, ctas) * each + min((int)blockIdx.x, more);
+  const int u1 = u0 + ((int)blockIdx.x < ctas ? each + ((int)blockIdx.x < more ? 1 : 0) : 0);
   // the sequence, segment and tile of the first unit u0, and how many of the run's units are tiles
   if (u0 < u1 && before <= u0 && u0 < before + mine) {
-    long long at = before;
+    int at = before;
     for (int b = tid * per;; ++b) {
-      const int n = paged_tiles(paged_seq(a, b).y) + C::Start;
-      if (u0 < at + (long long)n * segs) {
+      const int n = paged_tiles(known ? s_seqs[b].y : paged_seq(a, b).y) + C::Start;
+      if (u0 < at + n * segs) {
         s_start[0] = b;
-        s_start[1] = (int)((u0 - at) / n);
-        s_start[2] = (int)((u0 - at) % n);
+        s_start[1] = (u0 - at) / n;
+        s_start[2] = (u0 - at) - s_start[1] * n;
         break;
       }
-      at += (long long)n * segs;
+      at += n * segs;
     }
   }
   __syncthreads();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   PagedWalk w{};
   int count = 0;                  // tiles of the run
-  if (u0 < u1) {
-    for (int i = tid; i < kPA_Seqs && s_start[0] + i < a.B; i += kPA_Threads) {
-      s_seqs[i] = paged_seq(a, s_start[0] + i);
-    }
+  if (!known) {
+    for (int i = tid; u0 < u1 && i < kPA_Seqs && s_start[0] + i < a.B; i += kPA_Threads) s_seqs[i] = paged_seq(a, s_start[0] + i);
+    __syncthreads();
   }
-  __syncthreads();
   if (u0 < u1) {
     w.seqs = s_seqs;
-    w.b = w.b0 = s_start[0];
+    w.b = s_start[0];
+    w.b0 = known ? 0 : w.b;
     w.c = s_start[1] / a.p.heads;
     w.g = s_start[1] % a.p.heads;
     w.enter(a);
     w.tile = max(s_start[2] - C::Start, 0);
     // walk the run's segments: the units of each that are tiles
     PagedWalk x = w;
-    for (long long u = u0 - s_start[2]; u < u1;) {
-      const long long lo = max(u + C::Start, u0), hi = min(u + C::Start + x.ntiles, u1);
-      if (hi > lo) count += (int)(hi - lo);
+    for (int u = u0 - s_start[2]; u < u1;) {
+      count += max(min(u + C::Start + x.ntiles, u1) - max(u + C::Start, u0), 0);
       u += x.ntiles + C::Start;
       x.tile = x.ntiles - 1;
       x.next(a);
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         if (!valid) {
           uint4* row = reinterpret_cast<uint4*>(ring + u * kPA_Unit + hh * (kPA_Tile * 128) + tok * 128);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) row[i] = make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < 8; ++i) row[(i + tok) & 7] = make_uint4(0u, 0u, 0u, 0u);     // (rows are 128 bytes: eight banks' lanes at once)
         }
       }
       fence_async_smem();
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     float acc[RP];
     bool ok = true, from_start = w.tile == 0;
     int seg = 0;
-    long long unit = count > 0 ? u0 + max(C::Start - s_start[2], 0) : 0;      // the tile's
+    int unit = count > 0 ? u0 + max(C::Start - s_start[2], 0) : 0;      // the tile's
     int4 desc = make_int4(-1, 0, 0, 0);
 #pragma unroll
     for (int c = 0; c < RP; ++c) acc[c] = 0.f;
@@ -662,25 +664,31 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
         const bool whole = from_start && last;
         float* part = a.part + ((size_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * RP * kPA_Part;
+        // lane c: row of column c, its sum, maximum and place in the output
+        const int rc = col_row<RP>(min(lane, RP - 1));
+        const int2 ih = paged_row(a, rc);
+        const bool mine_row = lane < RP && rc < rows;
+        float sum = 0.f, m = -INFINITY;
+        if (mine_row) {
+          sum = (sg[lane] + sg[RP + lane]) + (sg[2 * RP + lane] + sg[3 * RP + lane]);
+          m = sg[4 * RP + lane];
+        }
+        const int row = ((w.b * a.t + i0 + ih.x) * a.H) + w.g * a.R + ih.y;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;       // nothing seen: zeros
+        if (mine_row && warp == 12) {
+          if (!whole)
+            *reinterpret_cast<float2*>(part + rc * kPA_Part + kPG_D) = make_float2(m, sum);
+          else if (a.lse)
+            a.lse[((size_t)w.b * a.H + w.g * a.R + ih.y) * a.t + i0 + ih.x] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+        }
         // one copy of the code for all rows: the accumulators move up by one per row
+        T* out = static_cast<T*>(a.o) + d;
 #pragma unroll 1
         for (int c = 0; c < RP; ++c) {
-          const int r = col_row<RP>(c);
+          const float f = __shfl_sync(0xffffffffu, inv, c);
+          const int to = __shfl_sync(0xffffffffu, row, c), r = __shfl_sync(0xffffffffu, rc, c);
           if (r < rows) {
-            const float sum = (sg[c] + sg[RP + c]) + (sg[2 * RP + c] + sg[3 * RP + c]), m = sg[4 * RP + c];
-            if (whole) {
-              const int2 ih = paged_row(a, r);
-              const int i = i0 + ih.x, h = w.g * a.R + ih.y;
-              const float inv = sum == 0.f ? 0.f : 1.f / sum;       // nothing seen: zeros
-              static_cast<T*>(a.o)[(((size_t)w.b * a.t + i) * a.H + h) * kPG_D + d] = (T)(acc[0] * inv);
-              if (a.lse && d == 0) a.lse[((size_t)w.b * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
-            } else {
-              part[r * kPA_Part + d] = acc[0];
-              if (d == 0) {
-                part[r * kPA_Part + kPG_D] = m;
-                part[r * kPA_Part + kPG_D + 1] = sum;
-              }
-            }
+            if (whole) out[(size_t)to * kPG_D] = (T)(acc[0] * f); else part[r * kPA_Part + d] = acc[0];
           }
 #pragma unroll
           for (int k = 0; k + 1 < RP; ++k) acc[k] = acc[k + 1];
@@ -688,8 +696,8 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         }
         // a cut segment that ends here: the CTA that holds its first tile
         if (last && !from_start) {
-          const long long t0 = unit - (w.ntiles - 1);
-          desc = make_int4((int)(((t0 + 1) * ctas - 1) / total), w.b, w.c, w.g);
+          const int t0 = unit - (w.ntiles - 1), longer = more * (each + 1);
+          desc = make_int4(t0 < longer ? t0 / (each + 1) : more + (t0 - longer) / each, w.b, w.c, w.g);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(seg_free + (seg & 1));
@@ -842,6 +850,9 @@ int bf_paged_attend(const bf_page_pool* pool, int layer, const void* q, long lon
   a.page_log = a.p.page == 16 ? 4 : a.p.page == 32 ? 5 : a.p.page == 64 ? 6 : 7;
   a.cap = (int)((long long)a.p.width * a.p.page < 0x7fffffffLL ? (long long)a.p.width * a.p.page : 0x7fffffffLL);
   a.by_r = (65536u + a.R - 1) / a.R;
+  // the tiles of all segments are counted, and the output's rows numbered, in 32 bits
+  if ((long long)B * a.nqc * a.p.heads * (a.cap / kPA_Tile + 4) > 0x7fffffffLL || (long long)B * t * H > 0x7fffffffLL)
+    return BF_ERR_UNSUPPORTED;
   a.c2 = scale * kLog2e;
   a.o = o;
   a.lse = lse;
