@@ -18,8 +18,8 @@
 // started (cluster launch control) and goes on with that: the start of a CTA pair (barriers, TMEM, the first loads) costs about 9 us,
 // as much as six key tiles, and the next item's loads and first products run under the end of the last one.
 // Warps (512 threads): 0 Q and K loads; 1 MMA (in the first CTA of the pair); 2 V loads; 3 the next items (the first CTA asks and
-// passes the answer on); 4-11 softmax, two warpgroups, each for 64 of a tile's 128 keys and 128 of O's columns; 12-15 the outputs,
-// while the next item's products run.
+// passes the answer on); 4-11 softmax, two warpgroups, every other tile each; 12-15 the outputs, while the next item's
+// products run.
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -41,7 +41,7 @@ constexpr int kPR_Tiles = kPR_SmemQ + 2 * kPR_SmemK + 2 * kPR_SmemV;
 constexpr int kPR_Items = 3;      // items known ahead
 constexpr int kPR_Ask = 4;        // the next item is asked for this many key tiles before the loads of the last one end
 constexpr int kPR_Parts = 1022;   // parts of a call whose first rows and keys fit into shared memory
-constexpr int kPR_Smem = kPR_Tiles + 512 + 5120 + 8192 + 4 * 2048 + 1024;
+constexpr int kPR_Smem = kPR_Tiles + 640 + 5120 + 8192 + 4 * 2048 + 1024;
 constexpr uint32_t kPR_TmO = 256;
 constexpr float kPR_Rescale = 8.0f;
 
@@ -175,10 +175,6 @@ __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
   return r;
 }
 
-// TMEM column of the P operand for key step ks (16 keys) of an S buffer: each softmax half writes the weights of its 64
-// keys into the first 32 columns of its own 64 score columns
-__device__ __forceinline__ uint32_t prompt_pcol(int ks) { return (uint32_t)((ks >> 2) * 64 + (ks & 3) * 8); }
-
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -200,20 +196,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   // in each CTA, by commits of the first
   uint64_t *q_free = bars + 8, *k_empty = bars + 9 /*[2]*/, *v_empty = bars + 11 /*[2]*/, *s_full = bars + 13 /*[2]*/, *o_fin = bars + 15;
   // within a CTA
-  uint64_t *pair = bars + 16 /*[4]*/, *stats = bars + 20 /*[2]*/, *sfree = bars + 22 /*[2]*/, *v_own = bars + 24;
+  uint64_t *mref = bars + 46 /*[2][4]*/, *stats = bars + 20 /*[2]*/, *sfree = bars + 22 /*[2]*/, *v_own = bars + 24;
   uint64_t *item_full = bars + 25 /*[3]*/, *item_free = bars + 28 /*[3]*/, *clc = bars + 31, *msg_full = bars + 32, *msg_free = bars + 33,
            *ask = bars + 39;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 34);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 35);
   uint8_t* answer = reinterpret_cast<uint8_t*>(bars + 36);                         // 16 bytes
   volatile int* msg = reinterpret_cast<volatile int*>(bars + 38);
-  PromptItem* s_items = reinterpret_cast<PromptItem*>(bars + 40);                  // [kPR_Items]
-  static_assert(40 * 8 + kPR_Items * sizeof(PromptItem) <= 512, "barriers and items");
-  float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 512);   // [2 tile parities][2 halves][128] maxima
-  float* xl = xch + 512;                                                           // [2 slots][2 halves][128] row sums
-  float* xmx = xl + 512;                                                           // [2 slots][128] row maxima
-  int2* s_starts = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(bars) + 512 + 5120);   // [kPR_Parts + 1], one warp's
-  uint8_t* s_out = reinterpret_cast<uint8_t*>(bars) + 512 + 5120 + 8192;          // [4 output warps][32 rows][128 B]
+  PromptItem* s_items = reinterpret_cast<PromptItem*>(bars + 54);                  // [kPR_Items]
+  static_assert(54 * 8 + kPR_Items * sizeof(PromptItem) <= 640, "barriers and items");
+  float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 640);   // [2 tile parities][128] references
+  float* xl = xch + 256;                                                           // [2 slots][2 warpgroups][128] row sums
+  float* xmx = xl + 512;                                                           // [2 slots][2 warpgroups][128] their references
+  int2* s_starts = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(bars) + 640 + 5120);   // [kPR_Parts + 1], one warp's
+  uint8_t* s_out = reinterpret_cast<uint8_t*>(bars) + 640 + 5120 + 8192;          // [4 output warps][32 rows][128 B]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_rank();
@@ -247,14 +243,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full + i, 2);
       mbar_init(v_full + i, 2);
-      mbar_init(p_full + i, 16);
+      mbar_init(p_full + i, 8);
       mbar_init(k_empty + i, 1);
       mbar_init(v_empty + i, 1);
       mbar_init(s_full + i, 1);
       mbar_init(stats + i, 8);
       mbar_init(sfree + i, 4);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(pair + i, 2);
+    for (int i = 0; i < 8; ++i) mbar_init(mref + i, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -365,6 +361,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           if (lane == 0) {
             s_items[s] = x;
             mbar_arrive(item_full + s);
+            if (it > 0 && x.n > 0) tma_prefetch_tile_4d(&qmap, 0, x.row0, 0, x.h);     // its queries into L2 meanwhile
           }
           __syncwarp();
           ++it;
@@ -415,7 +412,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           const uint32_t bV = smem_u32(sV + s * kPR_SmemV);
 #pragma unroll
           for (int ks = 0; ks < kPR_N / 16; ++ks)
-            umma_f16_ts_pair(tmem + kPR_TmO, tmem + s * kPR_N + prompt_pcol(ks), sdesc_sw128_mn(bV + ks * 2048, kPR_N * 128), id_o,
+            umma_f16_ts_pair(tmem + kPR_TmO, tmem + s * kPR_N + ks * 8, sdesc_sw128_mn(bV + ks * 2048, kPR_N * 128), id_o,
                              (j | ks) > 0 ? 1u : 0u);
           umma_commit_pair(v_empty + s);
           return true;
@@ -448,104 +445,97 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPR_RegsSoftmax));
     // ------------------------------------------------------------------ softmax (warps 4..11)
-    const int q4 = warp & 3, hh = (warp - 4) >> 2;
+    // Warpgroup w takes the tiles of parity w, thread = row, all 128 keys of it.  (Two warpgroups on the halves of each tile's keys
+    // ran in step, loading, comparing, exponentiating together, 3300 cycles a tile; taking turns, one's exponentials run beside
+    // the other's loads and comparisons.)  A tile's reference, what O and P are relative to, is the tile before's, unless the tile's
+    // maximum exceeds it by more than 2^kPR_Rescale; it is passed on as soon as the maximum is known.
+    const int q4 = warp & 3, w = (warp - 4) >> 2;
     const int r = q4 * 32 + lane;                 // row of the tile == TMEM lane
-    const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16);
-    constexpr int NH = kPR_N / 2;                 // 64 keys per half
-    const uint32_t pf[2] = {cluster_addr(p_full, 0), cluster_addr(p_full + 1, 0)};
-    uint32_t pair_phase = 0;
+    const uint32_t trow = tmem + ((uint32_t)(q4 * 32) << 16), srow = trow + w * kPR_N;
+    const uint32_t pf = cluster_addr(p_full + w, 0);
     bool alive = true;
     int t = 0;
     PromptItem x;
     for (int it = 0; alive && item(it, true, x); ++it) {
       const int n = x.n, lim_all = x.lim, lim = x.lim + r;   // last key that every row of this CTA sees, and this row
-      float m_ref = -INFINITY, l = 0.f;           // running maximum (log2 domain) and this half's sum
-      for (int j = 0; j < n; ++j) {
-        const int tt = t + j, s = tt & 1;
-        if (!mbar_wait_warp_small(s_full + s, (tt >> 1) & 1, abort_flag, 0x89)) { alive = false; break; }
+      float m_own = -INFINITY, l = 0.f;           // this warpgroup's last reference (log2 domain), its sum relative to that
+      for (int j = (t & 1) ^ w; j < n; j += 2) {
+        const int tt = t + j, ph = (tt >> 1) & 1;
+        if (!mbar_wait_warp_small(s_full + w, ph, abort_flag, 0x89)) { alive = false; break; }
         tc_fence_after();
-        float uu[NH];
+        float uu[kPR_N];
         {
-          uint32_t w0[32], w1[32];
-          tmem_ld32(trow + s * kPR_N + hh * NH, w0);
-          tmem_ld32(trow + s * kPR_N + hh * NH + 32, w1);
-          tmem_wait_ld();
+          uint32_t(&raw)[4][32] = reinterpret_cast<uint32_t(&)[4][32]>(uu);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            uu[e] = __uint_as_float(w0[e]);
-            uu[e + 32] = __uint_as_float(w1[e]);
-          }
+          for (int c = 0; c < 4; ++c) tmem_ld32(srow + c * 32, raw[c]);
+          tmem_wait_ld();
         }
         if (j * kPR_N + kPR_N - 1 > lim_all) {
-          const int hi = lim - j * kPR_N - hh * NH;
+          const int hi = lim - j * kPR_N;
 #pragma unroll
-          for (int e = 0; e < NH; ++e) uu[e] = e <= hi ? uu[e] : -INFINITY;
+          for (int e = 0; e < kPR_N; ++e) uu[e] = e <= hi ? uu[e] : -INFINITY;
         }
         float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < NH; e += 8) {
+        for (int e = 0; e < kPR_N; e += 8) {
           mx0 = max3(mx0, uu[e], uu[e + 1]);
           mx1 = max3(mx1, uu[e + 2], uu[e + 3]);
           mx2 = max3(mx2, uu[e + 4], uu[e + 5]);
           mx3 = max3(mx3, uu[e + 6], uu[e + 7]);
         }
-        const float mown = max3(mx0, mx1, fmaxf(mx2, mx3));
-        float* xm = xch + s * 256;
-        xm[hh * 128 + r] = mown;
+        const float mt = max3(mx0, mx1, fmaxf(mx2, mx3)) * a.c2;
+        // the reference of the tile before (which also says that it has been taken over from there)
+        if (tt >= 1 && !mbar_wait_warp_small(mref + (1 - w) * 4 + q4, ((tt - 1) >> 1) & 1, abort_flag, 0x8a)) { alive = false; break; }
+        const float prev = j >= 1 ? xch[(1 - w) * 128 + r] : -INFINITY;
+        const bool grown = prev != -INFINITY && mt > prev + kPR_Rescale;
+        const float m = prev == -INFINITY || grown ? mt : prev;
+        xch[w * 128 + r] = m;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&pair[q4]);
-        if (!mbar_wait_warp_small(&pair[q4], pair_phase++ & 1, abort_flag, 0x8a)) { alive = false; break; }
-        const float mt = fmaxf(mown, xm[(1 - hh) * 128 + r]) * a.c2;
-        float factor = 1.f;
-        bool rescale = false;
-        if (m_ref == -INFINITY) {
-          m_ref = mt;   // nothing accumulated yet
-        } else if (mt > m_ref + kPR_Rescale) {
-          factor = ex2_approx(m_ref - mt);
-          rescale = true;
-          m_ref = mt;
-          l *= factor;
-        }
-        uint32_t pk[NH / 2];
-        {
-          // a row that has seen nothing: scores of -inf against 0 give weights of 0, and a NaN stays one
-          const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
-          float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < NH; c += 2) {
-            const float e0 = ex2_approx(fmaf(uu[c], a.c2, nm)), e1 = ex2_approx(fmaf(uu[c + 1], a.c2, nm));
-            ls[(c >> 1) & 3] += e0 + e1;
-            pk[c / 2] = pack16<T>(e0, e1);
-          }
-          l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-        }
+        if (lane == 0) mbar_arrive(mref + w * 4 + q4);
+        l *= m_own == -INFINITY ? 1.f : ex2_approx(m_own - m);
+        m_own = m;
         // O rescale (warp-collective), from the item's second tile on: after O += P_{j-1} V_{j-1} has finished
-        if (j >= 1 && __any_sync(0xffffffffu, rescale)) {
+        if (j >= 1 && __any_sync(0xffffffffu, grown)) {
           if (!mbar_wait_warp_small(v_empty + ((tt - 1) & 1), ((tt - 1) >> 1) & 1, abort_flag, 0x8b)) { alive = false; break; }
           tc_fence_after();
+          const float factor = grown ? ex2_approx(prev - m) : 1.f;
 #pragma unroll 1
-          for (int c = hh * 128; c < hh * 128 + 128; c += 32) {
-            uint32_t ow[32];
-            tmem_ld32(trow + kPR_TmO + c, ow);
+          for (int c = 0; c < kPR_D; c += 16) {
+            uint32_t ow[16];
+            tmem_ld16(trow + kPR_TmO + c, ow);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * factor);
-            tmem_st32(trow + kPR_TmO + c, ow);
+            for (int e = 0; e < 16; ++e) ow[e] = __float_as_uint(__uint_as_float(ow[e]) * factor);
+            tmem_st16(trow + kPR_TmO + c, ow);
           }
         }
-        tmem_st32(trow + s * kPR_N + hh * NH, pk);
+        // a row that has seen nothing: scores of -inf against 0 give weights of 0, and a NaN stays one
+        const float nm = m == -INFINITY ? 0.f : -m;
+        float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kPR_N; c += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float e0 = ex2_approx(fmaf(uu[c + e], a.c2, nm)), e1 = ex2_approx(fmaf(uu[c + e + 1], a.c2, nm));
+            ls[(e >> 1) & 3] += e0 + e1;
+            pk[e / 2] = pack16<T>(e0, e1);
+          }
+          tmem_st16(srow + c / 2, pk);
+        }
+        l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(pf[s]);
+        if (lane == 0) mbar_arrive_cluster(pf);
       }
       if (!alive) break;
       t += n;
       // the row's statistics for the output warps (slot it & 1, free once they read item it - 2's)
       const int slot = it & 1;
       if (it >= 2 && !(alive = mbar_wait_warp_small(&sfree[slot], ((it >> 1) - 1) & 1, abort_flag, 0x8c))) break;
-      xl[slot * 256 + hh * 128 + r] = l;
-      if (hh == 0) xmx[slot * 128 + r] = m_ref;
+      xl[slot * 256 + w * 128 + r] = l;
+      xmx[slot * 256 + w * 128 + r] = m_own;
       __syncwarp();
       if (lane == 0) mbar_arrive(&stats[slot]);
     }
@@ -562,7 +552,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       if (!mbar_wait_warp_small(o_fin, it & 1, abort_flag, 0x8d)) break;
       const int slot = it & 1;
       if (!mbar_wait_warp_small(&stats[slot], (it >> 1) & 1, abort_flag, 0x8e)) break;
-      const float l = xl[slot * 256 + r] + xl[slot * 256 + 128 + r], m = xmx[slot * 128 + r];
+      // the warpgroups' sums on the later reference, which is the greater
+      const float m0 = xmx[slot * 256 + r], m1 = xmx[slot * 256 + 128 + r], m = fmaxf(m0, m1);
+      const float l = xl[slot * 256 + r] * (m0 == -INFINITY ? 1.f : ex2_approx(m0 - m)) +
+                      xl[slot * 256 + 128 + r] * (m1 == -INFINITY ? 1.f : ex2_approx(m1 - m));
       __syncwarp();
       if (lane == 0) mbar_arrive(&sfree[slot]);
       tc_fence_after();
