@@ -29,6 +29,8 @@ __device__ __forceinline__ float scale_for(float amax) {
   if (u < 0x00800000u) e = -64;   // zero and subnormal values
   return __uint_as_float((uint32_t)(max(e, -64) + 127) << 23);
 }
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t inf16() { return sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u; }
 __device__ __forceinline__ float pow2_inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }
 
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {   // saturating, NaN stays NaN
@@ -45,24 +47,30 @@ __device__ __forceinline__ void from_e4m3x4(uint32_t u, float (&x)[4]) {
   x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
 
-// One CTA per (sequence, page it writes, KV head, keys or values); thread i takes 16 elements (chunk i % 16) of rows
-// i / 16, i / 16 + 16, ...: all of its loads are in flight before the block's maximum is known, so the new tokens are
-// read once.  Bound by HBM (2 bytes in and 1 out per element) for prompts, by latency for a decode step.
+// One CTA per (sequence, page it writes, KV head), keys and values; thread i takes 16 elements (chunk i % 16) of rows i / 16,
+// i / 16 + 16, ...: all of its loads are in flight before the block's maxima are known, so the new tokens are read once.  Bound by HBM
+// (2 bytes in and 1 out per element) for prompts, where the way to the first load (cumulative lengths, slot and length, page) is what a
+// CTA mostly waits for: with keys and values in CTAs of their own 32143 tokens took 47 us, now 33 (0.92 of HBM) in pages of 64, where
+// three CTAs share an SM (two: 46 us), and 38, 38 and 44 in pages of 16, 32 and 128 (bounding their registers too made these slower).
+// A decode step is bound by latency: 5 us.
 template <typename T, int L>
-__global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(256, L == 64 ? 3 : 1) paged_append_kernel(AppendArgs a) {
   constexpr int PASS = L / 16;
-  __shared__ float s_max[8];
+  __shared__ float s_max[2][8];
   __shared__ int s_dup;
-  const int tid = threadIdx.x, kv = blockIdx.z, g = blockIdx.y;
+  const int tid = threadIdx.x, g = blockIdx.y;
   int b, ord, tok0 = 0, n = a.t;
   if (a.cu) {
-    // sequence b owns the items cu[b] / L + 2 b ...: at least one more than the pages that its tokens can touch
-    int lo = 0, hi = a.B - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (min(max(a.cu[mid], 0), a.t) / L + 2 * mid <= (int)blockIdx.x) lo = mid; else hi = mid - 1;
+    // sequence b owns the items cu[b] / L + 2 b ...: at least one more than the pages that its tokens can touch.  Every warp looks
+    // through 32 sequences at a time
+    b = 0;
+    for (int c = 0; c < a.B; c += 32) {
+      const int i = c + (tid & 31);
+      const unsigned ok = __ballot_sync(0xffffffffu, i < a.B && min(max(a.cu[min(i, a.B)], 0), a.t) / L + 2 * i <= (int)blockIdx.x);
+      if (ok == 0u) break;
+      b = c + 31 - __clz(ok);
+      if (ok != 0xffffffffu) break;
     }
-    b = lo;
     tok0 = min(max(a.cu[b], 0), a.t);
     n = min(max(a.cu[b + 1], tok0), a.t) - tok0;
     ord = (int)blockIdx.x - (tok0 / L + 2 * b);
@@ -90,72 +98,99 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
   const int lo = max(start, pi * L), had = lo - pi * L, rows = min(len, (pi + 1) * L) - lo;
   const int skip = n - (end - lo);   // this page's first new token among the sequence's
   if (rows <= 0) return;
-  const T* src = static_cast<const T*>(kv ? a.x[1] : a.x[0]) + g * (kv ? a.sh[1] : a.sh[0]) +
-                 (a.cu ? (long long)(tok0 + skip) * (kv ? a.st[1] : a.st[0])
-                       : b * (kv ? a.sb[1] : a.sb[0]) + (long long)skip * (kv ? a.st[1] : a.st[0]));
-  const long long st = kv ? a.st[1] : a.st[0];
   const size_t pg = (size_t)page * a.p.heads + g;
-  uint8_t* dst = (kv ? a.p.v : a.p.k) + pg * L * kPG_D;
-  float* scale = (kv ? a.p.vs : a.p.ks) + pg;
-  const float told = had ? *scale : 0.f;
   const int chunk = (tid & 15) * 16, r0 = tid >> 4;
-  uint4 w[PASS][2];
+  uint4 w[2][PASS][2];
+  float told[2];
 #pragma unroll
-  for (int i = 0; i < PASS; ++i) {
-    const int r = r0 + 16 * i;
-    w[i][0] = w[i][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (r < rows) {
-      const uint4* s = reinterpret_cast<const uint4*>(src + r * st + chunk);
-      w[i][0] = __ldg(s);
-      w[i][1] = __ldg(s + 1);
+  for (int kv = 0; kv < 2; ++kv) {
+    const T* src = static_cast<const T*>(a.x[kv]) + g * a.sh[kv] + chunk +
+                   (a.cu ? (long long)(tok0 + skip) * a.st[kv] : b * a.sb[kv] + (long long)skip * a.st[kv]);
+    told[kv] = had ? (kv ? a.p.vs : a.p.ks)[pg] : 0.f;
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const int r = r0 + 16 * i;
+      w[kv][i][0] = w[kv][i][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows) {
+        const uint4* s = reinterpret_cast<const uint4*>(src + r * a.st[kv]);
+        w[kv][i][0] = __ldg(s);
+        w[kv][i][1] = __ldg(s + 1);
+      }
     }
   }
-  float amax = 0.f;
+  float amax[2];
 #pragma unroll
-  for (int i = 0; i < PASS; ++i) {
-    const T* e = reinterpret_cast<const T*>(w[i]);
+  for (int kv = 0; kv < 2; ++kv) {
+    // the largest of the 16-bit patterns without their signs, which are in the order of the values; non-finite ones are left out in a
+    // second look
+    uint32_t m2 = 0u;
 #pragma unroll
-    for (int c = 0; c < 16; ++c) {
-      const float x = fabsf((float)e[c]);
-      amax = x < INFINITY ? fmaxf(amax, x) : amax;
+    for (int i = 0; i < PASS; ++i) {
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(w[kv][i]);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) m2 = __vmaxu2(m2, u[c] & 0x7fff7fffu);
     }
+    uint32_t top = max(m2 & 0xffffu, m2 >> 16);
+    if (top >= inf16<T>()) {
+      top = 0u;
+#pragma unroll
+      for (int i = 0; i < PASS; ++i) {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(w[kv][i]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t x = u[c] & 0x7fffu, y = (u[c] >> 16) & 0x7fffu;
+          top = max(top, max(x < inf16<T>() ? x : 0u, y < inf16<T>() ? y : 0u));
+        }
+      }
+    }
+    const uint16_t t16 = (uint16_t)top;
+    float m = (float)*reinterpret_cast<const T*>(&t16);
+    m = warp_max(m);
+    if ((tid & 31) == 0) s_max[kv][tid >> 5] = m;
   }
-  amax = warp_max(amax);
-  if ((tid & 31) == 0) s_max[tid >> 5] = amax;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, s_max[i]);
-  const float s = had ? fmaxf(scale_for(amax), told) : scale_for(amax);
-  const float inv = pow2_inverse(s);
+  for (int kv = 0; kv < 2; ++kv) {
+    amax[kv] = s_max[kv][0];
 #pragma unroll
-  for (int i = 0; i < PASS; ++i) {
-    const int r = r0 + 16 * i;
-    if (r < rows) {
-      const T* e = reinterpret_cast<const T*>(w[i]);
-      uint32_t c[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        c[q] = e4m3x4((float)e[4 * q] * inv, (float)e[4 * q + 1] * inv, (float)e[4 * q + 2] * inv, (float)e[4 * q + 3] * inv);
-      *reinterpret_cast<uint4*>(dst + (size_t)(had + r) * kPG_D + chunk) = make_uint4(c[0], c[1], c[2], c[3]);
-    }
+    for (int i = 1; i < 8; ++i) amax[kv] = fmaxf(amax[kv], s_max[kv][i]);
   }
-  if (had && s > told) {   // the page's earlier tokens on the grown scale
-    const float ratio = told * inv;
-    for (int r = r0; r < had; r += 16) {
-      uint4* at = reinterpret_cast<uint4*>(dst + (size_t)r * kPG_D + chunk);
-      const uint4 o = *at;
-      const uint32_t u[4] = {o.x, o.y, o.z, o.w};
-      uint32_t c[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float x[4];
-        from_e4m3x4(u[q], x);
-        c[q] = e4m3x4(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio);
+  for (int kv = 0; kv < 2; ++kv) {
+    uint8_t* dst = (kv ? a.p.v : a.p.k) + pg * L * kPG_D + chunk;
+    const float s = had ? fmaxf(scale_for(amax[kv]), told[kv]) : scale_for(amax[kv]);
+    const float inv = pow2_inverse(s);
+#pragma unroll
+    for (int i = 0; i < PASS; ++i) {
+      const int r = r0 + 16 * i;
+      if (r < rows) {
+        const T* e = reinterpret_cast<const T*>(w[kv][i]);
+        uint32_t c[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          c[q] = e4m3x4((float)e[4 * q] * inv, (float)e[4 * q + 1] * inv, (float)e[4 * q + 2] * inv, (float)e[4 * q + 3] * inv);
+        *reinterpret_cast<uint4*>(dst + (size_t)(had + r) * kPG_D) = make_uint4(c[0], c[1], c[2], c[3]);
       }
-      *at = make_uint4(c[0], c[1], c[2], c[3]);
     }
+    if (had && s > told[kv]) {   // the page's earlier tokens on the grown scale
+      const float ratio = told[kv] * inv;
+#pragma unroll 1
+      for (int r = r0; r < had; r += 16) {
+        uint4* at = reinterpret_cast<uint4*>(dst + (size_t)r * kPG_D);
+        const uint4 o = *at;
+        const uint32_t u[4] = {o.x, o.y, o.z, o.w};
+        uint32_t c[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float x[4];
+          from_e4m3x4(u[q], x);
+          c[q] = e4m3x4(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio);
+        }
+        *at = make_uint4(c[0], c[1], c[2], c[3]);
+      }
+    }
+    if (tid == 0) (kv ? a.p.vs : a.p.ks)[pg] = s;
   }
-  if (tid == 0) *scale = s;
 }
 
 // ------------------------------------------------------------------------------------------------ pages
@@ -300,7 +335,7 @@ int bf_paged_append(const bf_page_pool* pool, int layer, const void* k, long lon
   a.cu = cu;
   a.B = B;
   a.t = t;
-  const dim3 grid((unsigned)items, a.p.heads, 2);
+  const dim3 grid((unsigned)items, a.p.heads);
   auto go = [&](auto type) {
     using E = decltype(type);
     if (L == 16) paged_append_kernel<E, 16><<<grid, 256, 0, stream>>>(a);

@@ -191,6 +191,19 @@ def test_refusals():
             prompt_attention(q, k, v, cu, scale=s)
 
 
+@pytest.mark.parametrize("H,G", [(6, 1), (4, 2), (3, 1)])
+@pytest.mark.parametrize("nq,nk", [([5, 130], [3000, 2100]), ([1], [5000]), ([260, 3, 40], [2304, 0, 1999]), ([300], [2200])])
+def test_few_queries_of_many_keys(nq, nk, H, G):
+    """Blocks of many key tiles beside short ones, rows that see nothing and rows of no sequence."""
+    T, Tk = sum(nq) + 7, sum(nk) + 9
+    q, k, v = _inputs(T, Tk, H, G, torch.bfloat16, 14)
+    o, lse = _run(q, k, v, _cu(nq), _cu(nk))
+    _check(o[:-7], lse[:, :-7], q[:-7], k, v, _cu(nq), _cu(nk))
+    assert (o[-7:] == 0).all() and (lse[:, -7:] == -float("inf")).all()
+    o2, lse2 = _run(q, k, v, _cu(nq), _cu(nk))
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
 def test_many_sequences():
     """More sequences than a warp has lanes, most of them short, some empty."""
     lens = [(11 * i) % 23 for i in range(100)] + [200] + [(7 * i) % 5 for i in range(40)]
