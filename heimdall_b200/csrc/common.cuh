@@ -116,15 +116,18 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
 }
 
 // The same two waits in a few instructions, for kernels of many roles, whose loops would otherwise not stay in the instruction
-// cache: limited by a number of tries (each one suspends the thread for a while itself), a wait that gives up leaves its site in
-// the CTA's abort word, and the kernel's end reports that (report_abort).
-constexpr uint32_t kWaitTries = 1u << 20;
+// cache: limited by the SM's clock (about a second: a wait can be as long as a work item, 16 ms for a million keys); a wait that gives
+// up leaves its site in the CTA's abort word, and the kernel's end reports that (report_abort).
+constexpr long long kWaitCycles = 2000000000ll;
 __device__ __forceinline__ bool mbar_wait_small(uint64_t* bar, uint32_t parity, volatile int* abort, unsigned int site) {
   const uint32_t a = smem_u32(bar);
+  if (mbar_try_wait(a, parity)) return true;
+  const long long t0 = clock64();
 #pragma unroll 1
-  for (uint32_t n = 0; !mbar_try_wait(a, parity); ++n) {
-    if (n == kWaitTries || *abort) {
-      if (n == kWaitTries) *abort = (int)site;
+  while (!mbar_try_wait(a, parity)) {
+    if (*abort) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      *abort = (int)site;
       return false;
     }
   }

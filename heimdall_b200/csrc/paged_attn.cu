@@ -848,7 +848,7 @@ int bf_paged_attend(const bf_page_pool* pool, int layer, const void* q, long lon
   int rp;
   paged_chunks(t, a.R, &a.tc, &a.nqc, &rp);
   a.page_log = a.p.page == 16 ? 4 : a.p.page == 32 ? 5 : a.p.page == 64 ? 6 : 7;
-  a.cap = (int)((long long)a.p.width * a.p.page < 0x7fffffffLL ? (long long)a.p.width * a.p.page : 0x7fffffffLL);
+  a.cap = (int)((long long)a.p.width * a.p.page < 0x7fffff00LL ? (long long)a.p.width * a.p.page : 0x7fffff00LL);
   a.by_r = (65536u + a.R - 1) / a.R;
   // the tiles of all segments are counted, and the output's rows numbered, in 32 bits
   if ((long long)B * a.nqc * a.p.heads * (a.cap / kPA_Tile + 4) > 0x7fffffffLL || (long long)B * t * H > 0x7fffffffLL)

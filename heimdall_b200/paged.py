@@ -139,7 +139,7 @@ class PagedKV:
             raise ValueError("layers, pages, heads, slots and max_len must be positive")
         max_len = pages * page if max_len is None else max_len
         width = -(-max_len // page)
-        if slots * (width + 1) >= 2 ** 31 or pages * heads * page >= 2 ** 31 or layers * heads > 65535:
+        if slots * (width + 1) >= 2 ** 31 or width * page >= 2 ** 31 - 256 or pages * heads * page >= 2 ** 31 or layers * heads > 65535:
             raise ValueError("the cache is too large for 32-bit row numbers")
         dev = torch.device(device)
         if dev.type != "cuda":
