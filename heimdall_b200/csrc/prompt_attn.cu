@@ -211,7 +211,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   int2* s_starts = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(bars) + 640 + 5120);   // [kPR_Parts + 1], one warp's
   uint8_t* s_out = reinterpret_cast<uint8_t*>(bars) + 640 + 5120 + 8192;          // [4 output warps][32 rows][128 B]
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const uint32_t rank = cluster_rank();
   const int R = a.H / a.G, two = a.qb == kPR_M;            // two: the pair's tiles are two heads
   // item `it`, by one lane (lanes = 1) or a whole warp; false when there are no more, or a wait gave up
@@ -262,7 +262,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   __syncthreads();
   cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPR_RegsCtl));
@@ -392,53 +392,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
         }
         ++asked;
       }
-    } else if (warp == 1 && lane == 0 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
       // ---------------------------------------------------------------- MMA
-      constexpr int is_bf16 = sizeof(T) == 2 && !__is_same(T, __half);
+      // The warp stays converged and elects the issuing lane, so that descriptors stay in uniform registers: one lane of a diverged
+      // warp took 1300 cycles to issue the 16 steps of S and 700 for the 8 of O, longer than the tensor core for them.
+      constexpr int is_bf16 = !__is_same(T, __half);
       constexpr uint32_t id_s = idesc_f16(2 * kPR_M, kPR_N, is_bf16), id_o = idesc_f16(2 * kPR_M, kPR_D, is_bf16) | kIdescBMn;
-      const uint32_t aQ = smem_u32(sQ);
+      const uint64_t dq = sdesc_sw128(smem_u32(sQ)), dk0 = sdesc_sw128(smem_u32(sK)), dv0 = sdesc_sw128_mn(smem_u32(sV), kPR_N * 128);
       int t = 0;
       bool ok = true;
       PromptItem x;
-      for (int it = 0; ok && item(it, false, x); ++it) {
+#pragma unroll 1
+      for (int it = 0; ok && item(it, true, x); ++it) {
         const int n = x.n;
-        if (!(ok = mbar_wait_small(q_full, it & 1, abort_flag, 0x84))) break;
-        auto pv = [&](int j, int tt) -> bool {
-          const int s = tt & 1;
-          if (!mbar_wait_small(p_full + s, (tt >> 1) & 1, abort_flag, 0x85)) return false;
-          if (!mbar_wait_small(v_full + s, (tt >> 1) & 1, abort_flag, 0x86)) return false;
-          if (j == 0 && it >= 1 && !mbar_wait_small(o_free, (it - 1) & 1, abort_flag, 0x87)) return false;
-          tc_fence_after();
-          const uint32_t bV = smem_u32(sV + s * kPR_SmemV);
+        if (!(ok = mbar_wait_warp_small(q_full, it & 1, abort_flag, 0x84))) break;
+        // O += P_j V_j of tile j = jj - 1 follows the issue of S_jj; jj = n closes the item
+#pragma unroll 1
+        for (int jj = 0; jj <= n; ++jj) {
+          if (jj < n) {
+            const int tt = t + jj, s = tt & 1;
+            if (!(ok = mbar_wait_warp_small(k_full + s, (tt >> 1) & 1, abort_flag, 0x88))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t dk = dk0 + (uint32_t)(s * (kPR_SmemK >> 4));
 #pragma unroll
-          for (int ks = 0; ks < kPR_N / 16; ++ks)
-            umma_f16_ts_pair(tmem + kPR_TmO, tmem + s * kPR_N + ks * 8, sdesc_sw128_mn(bV + ks * 2048, kPR_N * 128), id_o,
-                             (j | ks) > 0 ? 1u : 0u);
-          umma_commit_pair(v_empty + s);
-          return true;
-        };
-        for (int j = 0; j < n && ok; ++j) {
-          const int tt = t + j, s = tt & 1;
-          if (!(ok = mbar_wait_small(k_full + s, (tt >> 1) & 1, abort_flag, 0x88))) break;
-          tc_fence_after();
-          const uint32_t bK = smem_u32(sK + s * kPR_SmemK);
+              for (int ks = 0; ks < kPR_D / 16; ++ks)
+                umma_f16_ss_pair(tmem + s * kPR_N, dq + ((ks >> 2) * (kPR_M * 128) + (ks & 3) * 32) / 16,
+                                 dk + ((ks >> 2) * (kPR_N / 2 * 128) + (ks & 3) * 32) / 16, id_s, ks > 0);
+              umma_commit_pair(s_full + s);
+              umma_commit_pair(k_empty + s);
+              if (jj == n - 1) umma_commit_pair(q_free);
+            }
+            __syncwarp();
+          }
+          if (jj >= 1) {
+            const int tt = t + jj - 1, s = tt & 1;
+            if (!(ok = mbar_wait_warp_small(v_full + s, (tt >> 1) & 1, abort_flag, 0x86))) break;
+            if (jj == 1 && it >= 1 && !(ok = mbar_wait_warp_small(o_free, (it - 1) & 1, abort_flag, 0x87))) break;
+            if (!(ok = mbar_wait_warp_small(p_full + s, (tt >> 1) & 1, abort_flag, 0x85))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t dv = dv0 + (uint32_t)(s * (kPR_SmemV >> 4));
 #pragma unroll
-          for (int ks = 0; ks < kPR_D / 16; ++ks)
-            umma_f16_ss_pair(tmem + s * kPR_N, sdesc_kstep(aQ, kPR_M, ks), sdesc_kstep(bK, kPR_N / 2, ks), id_s, ks > 0);
-          umma_commit_pair(k_empty + s);
-          umma_commit_pair(s_full + s);
-          if (j == n - 1) umma_commit_pair(q_free);
-          if (j >= 1 && !(ok = pv(j - 1, tt - 1))) break;
+              for (int ks = 0; ks < kPR_N / 16; ++ks)
+                umma_f16_ts_pair(tmem + kPR_TmO, tmem + s * kPR_N + ks * 8, dv + ks * (2048 / 16), id_o, (jj > 1 || ks > 0) ? 1u : 0u);
+              umma_commit_pair(v_empty + s);
+            }
+            __syncwarp();
+          }
         }
         if (!ok) break;
-        if (n > 0) {
-          if (!(ok = pv(n - 1, t + n - 1))) break;
-        } else {
-          // O counts as complete only once the item before has been drained, products or not
-          if (it >= 1 && !(ok = mbar_wait_small(o_free, (it - 1) & 1, abort_flag, 0x87))) break;
-          umma_commit_pair(q_free);
+        // O counts as complete only once the item before has been drained, products or not
+        if (n == 0 && it >= 1 && !(ok = mbar_wait_warp_small(o_free, (it - 1) & 1, abort_flag, 0x87))) break;
+        if (elect_one()) {
+          if (n == 0) umma_commit_pair(q_free);
+          umma_commit_pair(o_fin);
         }
-        umma_commit_pair(o_fin);
+        __syncwarp();
         t += n;
       }
     }
