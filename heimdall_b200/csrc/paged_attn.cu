@@ -7,7 +7,8 @@
 // head).  Turning the codes into 16-bit operands in registers would cost two conversions and a shared-memory round trip
 // per byte pair; instead the codes go from HBM by TMA into shared memory and from there, untouched, into the 5th-gen
 // tensor core (kind::f8f6f4).  The other operand of each product, which is small, is split into three e4m3 parts of 4
-// significant bits each (x = (x0 + x1 / 16 + x2 / 256) / 2^k, every part scaled into the code's upper range), each part a column of its own:
+// significant bits each (x = (x0 + x1 / 16 + x2 / 256) / 2^k, every part scaled into the code's upper range), each part a column of
+// its own:
 //   S^T[token, part x row] = K Q^T    M = 128 tokens, N = 3 RP, K = 256 dims   (a bf16 or fp16 query is exact in three parts)
 //   O^T[dim, part x row]   = V^T P^T  M = 2 x 128 dims, N = 3 RP, K = 128 tokens (P is off by at most 2^-12 of itself, or
 //                                     2^-26 of the tile's largest weight)
@@ -16,18 +17,22 @@
 // carry the running maximum: nothing is rescaled in TMEM.  V's scales go into P (as their ratio to the tile's largest).
 //
 // Work: the tiles of 128 tokens of all (sequence, token chunk, KV head) segments in one line, cut into equal runs, one per CTA
-// (one CTA per SM), whatever the lengths; a segment's start counts as two or three tiles, as its queries and its
-// output take about that long.  A segment inside one run is finished there; of a cut one each CTA writes its partial (at most two
-// per CTA), and paged_combine_kernel merges them in order, so results do not depend on timing.
-// Warps (640 threads): 0 and 2 TMA of the codes (K and V, each its own ring of 32 KB units), 0 also the tiles' scales;
-// 1 the products S; 3 the products O; 4-11 softmax (thread = token and the even or the odd rows) and, at the start of a segment,
-// the next one's Q parts (loaded a segment before; a warp of its own for them took 9000 cycles for 24 rows); 12-19 the accumulators
-// (thread = dim) and the output.
-// With one softmax warp per scheduler a tile took 6100 cycles, most of them the latency of that warp's own chain of
-// instructions; the rows are therefore dealt to two warpgroups, and what is the same for all tokens (a row's maximum and its
-// two factors) is computed by one lane per row and passed by shuffles.  The products are small, so issuing them is what costs:
-// one thread of a diverged warp took 4400 cycles per tile for both (every descriptor on its way through vector registers); two
-// warps that stay converged and elect the issuing lane do not bound it.
+// (one CTA per SM), whatever the lengths; a segment's start counts as two or three tiles, as its queries and its output take about
+// that long.  A segment inside one run is finished there; of a cut one each CTA writes its partial (at most two per CTA), and
+// paged_combine_kernel merges them in order, so results do not depend on timing.
+// Warps (640 threads): 0 and 2 TMA of the codes (K and V, each its own ring of 32 KB units), 0 also the tiles' scales; 1 the products
+// S; 3 the products O; 4-11 softmax (thread = token and the even or the odd rows) and, at the start of a segment, the next one's Q
+// parts (loaded a segment before; a warp of its own for them took 9000 cycles for 24 rows); 12-19 the accumulators (thread = dim)
+// and the output.
+// A tile has 2900 cycles at HBM's rate, so what counts is each role's chain of instructions.  With one softmax warp per scheduler a
+// tile took 6100 cycles; the rows are therefore dealt to two warpgroups, and what is the same for all tokens (a row's maximum
+// and its two factors) is computed by one lane per row and passed by shuffles.  The products are small, so issuing them is what
+// costs: one thread of a diverged warp took 4400 cycles per tile for both (every descriptor on its way through vector registers); two
+// warps that stay converged and elect the issuing lane do not bound it.  The roles together have to stay in the instruction
+// cache: waits and loops are written for few instructions (106 KB of code took a third longer than 72 KB).
+// Measured (24 query heads, 4 KV heads, pages of 64): 64 sequences of 16384 tokens 326 us, all that the measured copy rate allows
+// (331 us); 64 of 1 to 16384 tokens 52 us (floor 36); one of 777 tokens 10.5 us.  24 rows (four tokens): 4600 cycles a tile, bound by
+// the softmax warps' instructions: 32 sequences of 16384 tokens 275 us (floor 166).
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -601,7 +606,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         if (!valid) {
           uint4* row = reinterpret_cast<uint4*>(ring + u * kPA_Unit + hh * (kPA_Tile * 128) + tok * 128);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) row[(i + tok) & 7] = make_uint4(0u, 0u, 0u, 0u);     // (rows are 128 bytes: eight banks' lanes at once)
+          for (int i = 0; i < 8; ++i) row[(i + tok) & 7] = make_uint4(0u, 0u, 0u, 0u);     // a chunk per lane: rows are as long as all banks
         }
       }
       fence_async_smem();

@@ -3,23 +3,29 @@
 //   o_i = sum_j p_ij v_j,  p_i = softmax_j(scale q_i . k_j),  keys j <= i + nk - nq of the query's own sequence.
 //
 // Bound by the tensor core: 4 D flops per visible (query, key, head) against 2 D bytes per key.  With D = 256 an output tile of
-// 128 rows takes half of TMEM, so an SM works on one tile of 128 queries; fed by one CTA alone each 128-key tile is 128 KB
+// 128 rows takes half of TMEM, so an SM works on one tile of 128 queries; fed by one CTA alone, a 128-key tile is 128 KB
 // from L2 per 1.5 us and SM, as much as L2 delivers.  So two CTAs form a pair (cta_group::2, M = 256): each holds its own 128
-// query rows and half of the keys' rows and of the values' columns, 64 KB per key tile and SM, which leaves room for two stages of each.
-// The pair's two row tiles are two query heads of one KV head on the same 128 tokens (the same keys, the same causal edge), or,
-// with an odd number of heads per KV head, two neighbouring tiles of 128 tokens of one head.
+// query rows and half of the keys' rows and of the values' columns, 64 KB per key tile and SM, which leaves room for two stages
+// of each.  The pair's two row tiles are two query heads of one KV head on the same 128 tokens (the same keys, the same causal
+// edge), or, with an odd number of heads per KV head, two neighbouring tiles of 128 tokens of one head.
 //   S_j = Q K_j^T    M256 N128 K256 (A and B in shared memory)                        -> TMEM S buffer (tile parity)
 //   O  += P_j V_j    M256 N256 K128 (A = P_j in TMEM over S_j, B = V_j as it lies: N-major)
 //   TMEM of each CTA: S/P buffers at columns 0 and 128, O at 256..511.
-// P is rounded to the inputs' type (a step of the type, half of it at most, per weight: as large as the output's own rounding, and averaged over the keys);
-// its sum is taken before.  Scores are in the log2 domain; O is rescaled only when a row's maximum grows by more than 2^8.
+// P is rounded to the inputs' type, which moves a weight by half a step of the type at most: as much as the output's own rounding,
+// and it averages over the keys.  Its sum is taken before.  Scores are in the log2 domain; O is rescaled only when a row's
+// maximum grows by more than 2^8.
 //
-// Work items are (token block, KV head, head pair or head), one cluster of the grid each, those with the most key tiles first.  A cluster that has done its own item asks the hardware for one that has not
-// started (cluster launch control) and goes on with that: the start of a CTA pair (barriers, TMEM, the first loads) costs about 9 us,
-// as much as six key tiles, and the next item's loads and first products run under the end of the last one.
+// Work items are (token block, KV head, head pair or head), one cluster of the grid each, those with the most key tiles first.
+// A cluster that has done its own item asks the hardware for one that has not started (cluster launch control) and goes on with
+// that: the start of a CTA pair (barriers, TMEM, the first loads) costs about 9 us, and the next item's loads and first products
+// run under the end of the last one.
 // Warps (512 threads): 0 Q and K loads; 1 MMA (in the first CTA of the pair); 2 V loads; 3 the next items (the first CTA asks and
-// passes the answer on); 4-11 softmax, two warpgroups, every other tile each; 12-15 the outputs, while the next item's
-// products run.
+// passes the answer on); 4-11 softmax, two warpgroups, every other tile each; 12-15 the outputs, while the next item's products run.
+//
+// Measured (24 query heads, 4 KV heads, bf16): 32768 tokens 9.13 ms = 1446 TFLOP/s, above the library product's rate under the power
+// limit (1406) and 0.87 of its burst; 8192 tokens 538 us = 1534 (0.92 of burst); 2300 cycles per key tile against the tensor core's
+// 2048.  Between items 3700 cycles are lost, most of them for the next item's queries, 64 KB that only fit once the last product has
+// read the ones before: eight prompts of 1 to 4095 tokens run at 1274.
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -455,9 +461,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPR_RegsSoftmax));
     // ------------------------------------------------------------------ softmax (warps 4..11)
-    // Warpgroup w takes the tiles of parity w, thread = row, all 128 keys of it.  (Two warpgroups on the halves of each tile's keys
-    // ran in step, loading, comparing, exponentiating together, 3300 cycles a tile; taking turns, one's exponentials run beside
-    // the other's loads and comparisons.)  A tile's reference, what O and P are relative to, is the tile before's, unless the tile's
+    // Warpgroup w takes the tiles of parity w, thread = row, all 128 keys of it, in 2200 cycles (1400 for the exponentials), so one's
+    // exponentials run beside the other's loads and comparisons.  (On the halves of each tile's keys the two would run in step, with
+    // an exchange of maxima in between.)  A tile's reference, what O and P are relative to, is the tile before's, unless the tile's
     // maximum exceeds it by more than 2^kPR_Rescale; it is passed on as soon as the maximum is known.
     const int q4 = warp & 3, w = (warp - 4) >> 2;
     const int r = q4 * 32 + lane;                 // row of the tile == TMEM lane

@@ -1,7 +1,7 @@
 """An 8-bit cache in pages for the kept (not converted) full-attention layers.
 
-The reference's server keeps the full-attention layers' keys and values in 8 bits and copies and removes sequences of
-its cache (llamacpp/README.md:77-78).  Here a pool of pages of ``page`` tokens holds e4m3 codes with one power-of-two
+The reference quotes its decode figures with an 8-bit key and value cache (README.md:15, 60), and its port copies and removes
+sequences of the cache (llamacpp/README.md:77-78).  Here a pool of pages of ``page`` tokens holds e4m3 codes with one power-of-two
 scale per (layer, page, KV head), for keys and for values; the host gives out pages (lowest index first, with reference
 counts) and the device holds the page table and the lengths, so that ``append`` and ``attend`` read nothing from the
 host and can be captured into a CUDA graph:
@@ -13,7 +13,8 @@ host and can be captured into a CUDA graph:
         o, _ = c.attend(layer, q, slot_ids)   # device
 
 ``fork`` shares pages between sequences, ``free`` and ``truncate`` give them back, ``compact`` closes the pool up.
-Calls on one cache belong on one stream, or on streams that the caller orders.  There is no CPU path.
+Calls on one cache belong on one stream, or on streams that the caller orders, and on one host thread at a time.  There is no
+CPU path.
 """
 from __future__ import annotations
 
@@ -255,7 +256,8 @@ class PagedKV:
     def attend(self, layer: int, q, slots=None, scale=None, with_lse: bool = False):
         """Attention of each sequence's last t tokens over its pages: q [B,t,H,D] (bf16 or fp16; H a multiple of the KV
         heads) at the positions lens - t .. lens - 1, each seeing the positions up to its own.  Returns o [B,t,H,D] in q's
-        dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf."""
+        dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf.  What the pages hold
+        behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t tokens."""
         check_cuda(q)
         refuse_grad("PagedKV.attend", q)
         layer = self._layer(layer)
