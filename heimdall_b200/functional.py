@@ -215,17 +215,20 @@ def window_attention(qr, ext_k, ext_v, qpos0: int, kpos0: int, klo: int, window:
     return o, lse
 
 
-def refuse_grad(name: str, *ts) -> None:
-    """The serving operators have no backward: a call that autograd would have to follow is refused."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise NotImplementedError(f"heimdall_b200 {name} has no backward: call it under torch.no_grad()")
-
-
-def same_device(*ts) -> torch.device:
-    dev = next(t.device for t in ts if t is not None)
+def serving_inputs(name: str, *ts) -> torch.device:
+    """The one CUDA device of these tensors.  The serving operators have no backward: a call that autograd would have to follow is
+    refused.  (One pass over the tensors: these calls are a few microseconds on the device.)"""
+    dev, grad = None, False
     for t in ts:
-        if t is not None and t.device != dev:
+        if not t.is_cuda:
+            check_cuda(t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
             raise ValueError("all tensors must be on one device")
+        grad = grad or t.requires_grad
+    if grad and torch.is_grad_enabled():
+        raise NotImplementedError(f"heimdall_b200 {name} has no backward: call it under torch.no_grad()")
     return dev
 
 
@@ -234,21 +237,22 @@ def on_device(dev: torch.device):
     return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
-def heads_16bit(name: str, t) -> torch.Tensor:
-    """t [..., D] with its last dimension contiguous, every row on a 16-byte boundary and no dimension expanded (copied when it is
-    not so)."""
-    if t.dtype not in (torch.bfloat16, torch.float16):
+def heads_16bit(name: str, t):
+    """t [..., D] as a kernel takes it: (tensor, address, element strides of all but the last dimension), the last dimension
+    contiguous, every row on a 16-byte boundary and no dimension expanded (copied when it is not so; the stride of a
+    dimension of one means nothing and is given as 0).  The tensor is returned to be kept alive over the launch."""
+    if t.dtype != torch.bfloat16 and t.dtype != torch.float16:
         raise NotImplementedError(f"{name} is {t.dtype}: built for bfloat16 and float16")
-    st = t.stride()
-    ok = st[-1] == 1 and t.data_ptr() % 16 == 0
+    at, st = t.data_ptr(), t.stride()
+    ok = st[-1] == 1 and at % 16 == 0
+    out = []
     for s, n in zip(st[:-1], t.shape):
-        ok = ok and (n < 2 or (s > 0 and s % 8 == 0))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
-
-
-def strides(t) -> tuple:
-    """Element strides of all but the last dimension (0 for a dimension of one, whose stride means nothing)."""
-    return tuple([s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)])
+        if n < 2:
+            s = 0
+        elif s <= 0 or s % 8:
+            ok = False
+        out.append(s)
+    return (t, at, out) if ok else heads_16bit(name, t.clone(memory_format=torch.contiguous_format))
 
 
 def kernel_dtype(t) -> int:
@@ -256,7 +260,9 @@ def kernel_dtype(t) -> int:
 
 
 def score_scale(scale, D: int) -> float:
-    scale = D ** -0.5 if scale is None else float(scale)
+    if scale is None:
+        return D ** -0.5
+    scale = float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError("scale must be positive and finite")
     return scale
@@ -285,31 +291,34 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, with_ls
     NaN of earlier queries of its own sequence in the same block of 128 keys (a weight of 0 times it).  No backward: the
     kept layers are frozen and their outputs enter training precomputed (motor.py:126-146).
     """
-    check_cuda(q, k, v)
-    refuse_grad("prompt_attention", q, k, v)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[-1] != q.shape[-1]:
+    dev = serving_inputs("prompt_attention", q, k, v)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or ks != v.shape or ks[2] != qs[2]:
         raise ValueError("prompt_attention takes q [T,H,D] and k, v [Tk,G,D]")
-    if q.dtype != k.dtype or q.dtype != v.dtype:
+    dt = q.dtype
+    if dt != k.dtype or dt != v.dtype:
         raise ValueError("q, k and v must have one dtype")
-    (T, H, D), (Tk, G, _) = q.shape, k.shape
+    (T, H, D), (Tk, G, _) = qs, ks
     if D != 256:
         raise NotImplementedError("prompt_attention is built for head dim 256")
-    if H % G:
+    if G < 1 or H < 1 or H % G:
         raise ValueError("the query heads must be a multiple of the KV heads")
     if cu_seqlens_k is None and Tk != T:
         raise ValueError("keys and queries differ in number: cu_seqlens_k is needed")
-    dev = same_device(q, k, v)
     scale = score_scale(scale, D)
     with on_device(dev):
         cu = int32_on(dev, "cu_seqlens", cu_seqlens)
         cuk = None if cu_seqlens_k is None else int32_on(dev, "cu_seqlens_k", cu_seqlens_k)
-        if cu.numel() < 1 or (cuk is not None and cuk.numel() != cu.numel()):
+        n = cu.numel()
+        if n < 1 or (cuk is not None and cuk.numel() != n):
             raise ValueError("cu_seqlens and cu_seqlens_k need one entry more than there are sequences")
-        q, k, v = heads_16bit("q", q), heads_16bit("k", k), heads_16bit("v", v)
-        o = torch.empty(T, H, D, device=dev, dtype=q.dtype)
-        lse = torch.empty(H, T, device=dev, dtype=torch.float32) if with_lse else None
-        _lib.call("bf_prompt_attn_fwd", ptr(q), *strides(q), ptr(k), *strides(k), ptr(v), *strides(v), ptr(cu), ptr(cuk),
-                  cu.numel() - 1, T, Tk, H, G, D, kernel_dtype(q), scale, ptr(o), ptr(lse), stream_handle())
+        q, qp, qst = heads_16bit("q", q)
+        k, kp, kst = heads_16bit("k", k)
+        v, vp, vst = heads_16bit("v", v)
+        o = q.new_empty(qs)
+        lse = q.new_empty((H, T), dtype=torch.float32) if with_lse else None
+        _lib.call("bf_prompt_attn_fwd", qp, *qst, kp, *kst, vp, *vst, cu.data_ptr(), ptr(cuk), n - 1, T, Tk, H, G, D,
+                  kernel_dtype(q), scale, o.data_ptr(), ptr(lse), stream_handle())
     return o, lse
 
 

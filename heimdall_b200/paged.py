@@ -24,8 +24,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from .functional import (check_cuda, heads_16bit, int32_on, kernel_dtype, on_device, prompt_attention, ptr, refuse_grad,
-                         same_device, score_scale, stream_handle, strides)
+from .functional import (heads_16bit, int32_on, kernel_dtype, on_device, prompt_attention, ptr, score_scale, serving_inputs,
+                         stream_handle)
 from .structs import BfPagePool, BfPageTable
 
 PAGE_SIZES = (16, 32, 64, 128)
@@ -157,6 +157,7 @@ class PagedKV:
         self._pool = BfPagePool(ptr(self.k_pages), ptr(self.v_pages), ptr(self.k_scale), ptr(self.v_scale), ptr(self.table),
                                 ptr(self.lens), layers, pages, heads, page, dim, slots, width)
         self._pool_ptr = ctypes.addressof(self._pool)
+        self._ws = {}                       # workspace bytes by (B, t, H)
 
     # -------------------------------------------------------------------------------------------- sequences and pages
     @property
@@ -219,8 +220,7 @@ class PagedKV:
             if B > self.host.slots:
                 raise ValueError("more sequences than the cache has slots")
             return None
-        check_cuda(slots)
-        same_device(self.k_pages, slots)
+        serving_inputs("PagedKV", self.k_pages, slots)
         slots = int32_on(self.device, "slots", slots)
         if slots.numel() != B:
             raise ValueError("slots needs one entry per sequence")
@@ -231,52 +231,49 @@ class PagedKV:
         [B+1].  Sequence b (slot slots[b], an int tensor on the device; None: slot b) gets its n_b tokens at the positions
         lens - n_b .. lens - 1.  A page's scale covers what was written to it; earlier codes of a page whose scale grows are
         rounded to the new one.  Infinities are stored as the largest code, NaN as NaN."""
-        check_cuda(k, v)
-        refuse_grad("PagedKV.append", k, v)
-        layer = self._layer(layer)
-        packed = cu_seqlens is not None
-        if k.shape != v.shape or k.dtype != v.dtype or k.dim() != (3 if packed else 4):
+        dev = serving_inputs("PagedKV.append", self.k_pages, k, v)
+        layer, shape, packed = self._layer(layer), k.shape, cu_seqlens is not None
+        if shape != v.shape or k.dtype != v.dtype or len(shape) != (3 if packed else 4):
             raise ValueError("append takes k and v alike: [B,t,G,D], or [T,G,D] with cu_seqlens")
-        if k.shape[-2] != self.heads or k.shape[-1] != self.dim:
+        if shape[-2] != self.heads or shape[-1] != self.dim:
             raise ValueError(f"append takes {self.heads} heads of {self.dim}")
-        same_device(self.k_pages, k, v)
-        with on_device(self.device):
-            cu = int32_on(self.device, "cu_seqlens", cu_seqlens) if packed else None
-            B = cu.numel() - 1 if packed else k.shape[0]
+        with on_device(dev):
+            cu = int32_on(dev, "cu_seqlens", cu_seqlens) if packed else None
+            B = cu.numel() - 1 if packed else shape[0]
             if B < 0:
                 raise ValueError("cu_seqlens needs one entry more than there are sequences")
             ids = self._ids(slots, B)
-            k, v = heads_16bit("k", k), heads_16bit("v", v)
-            ks, vs = strides(k), strides(v)
+            k, kp, ks = heads_16bit("k", k)
+            v, vp, vs = heads_16bit("v", v)
             if packed:
-                ks, vs = (0,) + ks, (0,) + vs
-            _lib.call("bf_paged_append", self._pool_ptr, layer, ptr(k), *ks, ptr(v), *vs, ptr(ids), ptr(cu), B, k.shape[-3],
-                      kernel_dtype(k), stream_handle())
+                ks, vs = [0] + ks, [0] + vs
+            _lib.call("bf_paged_append", self._pool_ptr, layer, kp, *ks, vp, *vs, ptr(ids), ptr(cu), B, shape[-3], kernel_dtype(k),
+                      stream_handle())
 
     def attend(self, layer: int, q, slots=None, scale=None, with_lse: bool = False):
         """Attention of each sequence's last t tokens over its pages: q [B,t,H,D] (bf16 or fp16; H a multiple of the KV
         heads) at the positions lens - t .. lens - 1, each seeing the positions up to its own.  Returns o [B,t,H,D] in q's
         dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf.  What the pages hold
         behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t tokens."""
-        check_cuda(q)
-        refuse_grad("PagedKV.attend", q)
-        layer = self._layer(layer)
-        if q.dim() != 4 or q.shape[-1] != self.dim or q.shape[2] % self.heads or q.shape[2] < 1:
+        dev = serving_inputs("PagedKV.attend", self.k_pages, q)
+        layer, shape = self._layer(layer), q.shape
+        if len(shape) != 4 or shape[3] != self.dim or shape[2] % self.heads or shape[2] < 1:
             raise ValueError(f"attend takes q [B,t,H,{self.dim}] with H a multiple of {self.heads}")
-        B, t, H, D = q.shape
+        B, t, H, D = shape
         if H // self.heads > 24:
             raise NotImplementedError("attend takes at most 24 query heads per KV head")
-        same_device(self.k_pages, q)
         scale = score_scale(scale, D)
-        with on_device(self.device):
+        with on_device(dev):
             ids = self._ids(slots, B)
-            q = heads_16bit("q", q)
-            o = torch.empty(B, t, H, D, device=self.device, dtype=q.dtype)
-            lse = torch.empty(B, H, t, device=self.device, dtype=torch.float32) if with_lse else None
-            nws = _lib.size("bf_paged_attend_workspace", B, t, H, self.heads, D)
-            ws = torch.empty(max(nws, 16), dtype=torch.uint8, device=self.device)
-            _lib.call("bf_paged_attend", self._pool_ptr, layer, ptr(q), *strides(q), ptr(ids), B, t, H, kernel_dtype(q), scale,
-                      ptr(o), ptr(lse), ptr(ws), ws.numel(), stream_handle())
+            q, qp, qs = heads_16bit("q", q)
+            o = q.new_empty(shape)
+            lse = q.new_empty((B, H, t), dtype=torch.float32) if with_lse else None
+            nws = self._ws.get((B, t, H))
+            if nws is None:
+                nws = self._ws[B, t, H] = max(_lib.size("bf_paged_attend_workspace", B, t, H, self.heads, D), 16)
+            ws = q.new_empty((nws,), dtype=torch.uint8)
+            _lib.call("bf_paged_attend", self._pool_ptr, layer, qp, *qs, ptr(ids), B, t, H, kernel_dtype(q), scale, o.data_ptr(),
+                      ptr(lse), ws.data_ptr(), nws, stream_handle())
         return o, lse
 
     def layer(self, layer: int) -> "PagedLayer":
