@@ -20,12 +20,12 @@
 // (one CTA per SM), whatever the lengths; a segment's start counts as two or three tiles, as its queries and its output take about
 // that long.  A segment inside one run is finished there; of a cut one each CTA writes its partial (at most two per CTA), and
 // paged_combine_kernel merges them in order, so results do not depend on timing.
-// Warps (640 threads): 0 and 2 TMA of the codes (K and V, each its own ring of 32 KB units), 0 also the tiles' scales; 1 the products
-// S; 3 the products O; 4-11 softmax (thread = token and the even or the odd rows) and, at the start of a segment, the next one's Q
-// parts (loaded a segment before; a warp of its own for them took 9000 cycles for 24 rows); 12-19 the accumulators (thread = dim)
-// and the output.
+// Warps: 0 and 2 TMA of the codes (K and V, each its own ring of 32 KB units), 0 also the tiles' scales; 1 the products S; 3 the
+// products O; then two (24 rows: three) warpgroups of softmax (thread = token and every second, or third, row), which at the start of
+// a segment also make the next one's Q parts (loaded a segment before; a warp of its own for them took 9000 cycles for 24 rows);
+// the last two warpgroups the accumulators (thread = dim) and the output.
 // A tile has 2900 cycles at HBM's rate, so what counts is each role's chain of instructions.  With one softmax warp per scheduler a
-// tile took 6100 cycles; the rows are therefore dealt to two warpgroups, and what is the same for all tokens (a row's maximum
+// tile took 6100 cycles; the rows are therefore dealt to several warpgroups, and what is the same for all tokens (a row's maximum
 // and its two factors) is computed by one lane per row and passed by shuffles.  The products are small, so issuing them is what
 // costs: one thread of a diverged warp took 4400 cycles per tile for both (every descriptor on its way through vector registers); two
 // warps that stay converged and elect the issuing lane do not bound it.  The roles together have to stay in the instruction
@@ -41,7 +41,6 @@
 
 namespace bfb {
 
-constexpr int kPA_Threads = 640;
 constexpr int kPA_Tile = 128;                        // tokens per tile
 constexpr int kPA_Unit = kPA_Tile * kPG_D;           // bytes of one K or V tile
 constexpr int kPA_MaxCtas = 160;
@@ -69,6 +68,8 @@ struct PagedAttnArgs {
 template <int RP>
 struct PagedCfg {
   static constexpr int NP = (3 * RP + 15) / 16 * 16;       // MMA N: three parts of RP rows, padded to 16
+  static constexpr int Groups = RP == 24 ? 3 : 2;          // softmax warpgroups: row r is of group r % Groups
+  static constexpr int Threads = (4 + 4 * Groups + 8) * 32;
   static constexpr int KUnits = 3, VUnits = RP == 8 ? 3 : 2;   // ring units that fit beside Q and P
   static constexpr int Units = KUnits + VUnits;
   // what a segment's start counts, in tiles.  64 sequences of 1 to 16384 tokens, 8 rows: 67, 59 and 59 us with 1, 2 and 3, 32 of 3000 to
@@ -145,17 +146,20 @@ __device__ __forceinline__ void split3(float a, float b, uint16_t (&part)[3]) {
     }
   }
 }
-// the RP rows lie in the order even rows, odd rows: row r in column row_col(r) of each part
+// the RP rows lie group by group of the softmax warps: row r in column row_col(r) of each part
 template <int RP>
-__device__ __forceinline__ constexpr int row_col(int r) { return (r & 1) * (RP / 2) + (r >> 1); }
+__device__ __forceinline__ constexpr int row_col(int r) { return r % PagedCfg<RP>::Groups * (RP / PagedCfg<RP>::Groups) + r / PagedCfg<RP>::Groups; }
 template <int RP>
-__device__ __forceinline__ constexpr int col_row(int c) { return 2 * (c % (RP / 2)) + c / (RP / 2); }
+__device__ __forceinline__ constexpr int col_row(int c) {
+  constexpr int n = RP / PagedCfg<RP>::Groups;
+  return c % n * PagedCfg<RP>::Groups + c / n;
+}
 
 template <typename T, int RP>
-__global__ void __launch_bounds__(kPA_Threads, 1)
+__global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PagedAttnArgs a) {
   using C = PagedCfg<RP>;
-  constexpr int NP = C::NP, NU = C::Units, NK = C::KUnits, NV = C::VUnits;
+  constexpr int NP = C::NP, NU = C::Units, NK = C::KUnits, NV = C::VUnits, SG = C::Groups;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring = smem;
@@ -164,11 +168,11 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * C::PBytes);
   uint64_t *full = bars, *empty = bars + 6, *s_full = bars + 12, *s_free = bars + 14, *p_full = bars + 16, *o_full = bars + 18,
            *o_free = bars + 20, *q_full = bars + 22, *q_free = bars + 24, *sc_full = bars + 26, *sc_free = bars + 30, *red = bars + 34,
-           *seg_full = bars + 36, *seg_free = bars + 38;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 40);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 41);
-  int* s_sum = reinterpret_cast<int*>(bars + 42);                   // [20] per-warp totals of the unit count
-  int* s_start = reinterpret_cast<int*>(bars + 63);                 // b, segment of it, tile of that
+           *seg_full = bars + 37, *seg_free = bars + 39;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 41);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 42);
+  int* s_sum = reinterpret_cast<int*>(bars + 43);                   // [24] per-warp totals of the unit count
+  int* s_start = reinterpret_cast<int*>(bars + 56);                 // b, segment of it, tile of that
   float* s_qs = reinterpret_cast<float*>(bars + 66);                // [2][RP] scale of the Q rows
   float* s_fac = s_qs + 2 * kPA_MaxRows;                            // [2][RP][2] factors of the tile's O^T and the accumulators
   float* s_red = s_fac + 4 * kPA_MaxRows;                           // [2][4][RP] the warps' maxima
@@ -185,19 +189,19 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(s_free + i, 8);
-      mbar_init(p_full + i, 8);
+      mbar_init(s_free + i, 4 * SG);
+      mbar_init(p_full + i, 4 * SG);
       mbar_init(o_full + i, 1);
       mbar_init(o_free + i, 8);
-      mbar_init(q_full + i, 8);
-      mbar_init(q_free + i, 9);
-      mbar_init(seg_full + i, 8);
+      mbar_init(q_full + i, 4 * SG);
+      mbar_init(q_free + i, 4 * SG + 1);
+      mbar_init(seg_full + i, 4 * SG);
       mbar_init(seg_free + i, 8);
-      mbar_init(red + i, 4);
     }
+    for (int i = 0; i < SG; ++i) mbar_init(red + i, 4);
     for (int i = 0; i < 4; ++i) {
       mbar_init(sc_full + i, 1);
-      mbar_init(sc_free + i, 8);
+      mbar_init(sc_free + i, 4 * SG);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
   }
   // this CTA's run: every segment is Start units and one for each of its tiles.  The sequences' units are summed over the block,
   // thread i holding `per` consecutive sequences (the caller has made sure that 32 bits hold the sum)
-  const int per = (a.B + kPA_Threads - 1) / kPA_Threads;
+  const int per = (a.B + C::Threads - 1) / C::Threads;
   const int segs = a.nqc * a.p.heads;
   const bool known = a.B <= kPA_Seqs;          // all sequences fit into s_seqs
   int mine = 0;
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  int total = lane < kPA_Threads / 32 ? s_sum[lane] : 0, before = lane < warp ? total : 0;
+  int total = lane < C::Threads / 32 ? s_sum[lane] : 0, before = lane < warp ? total : 0;
   total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
   before = (int)__reduce_add_sync(0xffffffffu, (unsigned)before) + incl - mine;
   // with fewer units than CTAs the first `total` CTAs take one each; the first `more` runs are one unit longer than the others
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
   PagedWalk w{};
   int count = 0;                  // tiles of the run
   if (!known) {
-    for (int i = tid; u0 < u1 && i < kPA_Seqs && s_start[0] + i < a.B; i += kPA_Threads) s_seqs[i] = paged_seq(a, s_start[0] + i);
+    for (int i = tid; u0 < u1 && i < kPA_Seqs && s_start[0] + i < a.B; i += C::Threads) s_seqs[i] = paged_seq(a, s_start[0] + i);
     __syncthreads();
   }
   if (u0 < u1) {
@@ -430,26 +434,27 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         uphase ^= 1;
       }
     }
-  } else if (warp < 12) {
-    // ------------------------------------------------------------------ softmax: thread = token of the tile, rows 2 i + hh
-    constexpr int RH = RP / 2;
+  } else if (warp < 4 + 4 * SG) {
+    // ------------------------------------------------------------------ softmax: thread = token of the tile, rows SG i + hh
+    constexpr int RH = RP / SG;
     const int wq = warp & 3, hh = (warp - 4) >> 2, tok = wq * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + hh * RH;
     float l[RH], qs[RH];
     int rows = 0, first_pos = 0;         // of the chunk; the position of its first token
-    float m_run = -INFINITY;             // of row 2 lane + hh, in lanes < RH
+    float m_run = -INFINITY;             // of row SG lane + hh, in lanes < RH
     bool ok = true, first = true;
     int seg = 0;
-    // the queries: warp w of the eight takes rows w, w + 8, w + 16, lane l dims 8 l .. 8 l + 7
+    // the queries: warp w of the 4 SG takes rows w, w + 4 SG, ..., lane l dims 8 l .. 8 l + 7
+    constexpr int QW = 4 * SG;
     PagedWalk nx = w;                    // the segment whose queries are in `raw`
     int nx_at = 0, nx_rows = 0;          // its first tile in the run
-    uint4 qraw[RP / 8];
+    uint4 qraw[RP / QW];
     auto q_load = [&]() {
       const int i0 = nx.c * a.tc;
       nx_rows = min(a.tc, a.t - i0) * a.R;
 #pragma unroll
-      for (int i = 0; i < RP / 8; ++i) {
-        const int r = warp - 4 + 8 * i;
+      for (int i = 0; i < RP / QW; ++i) {
+        const int r = warp - 4 + QW * i;
         const int2 ih = paged_row(a, r);
         if (r < nx_rows)
           qraw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + nx.b * a.q_sb + (long long)(i0 + ih.x) * a.q_st +
@@ -459,8 +464,8 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     auto q_store = [&](int buf) {        // rows from nx_rows on stay as they are, nothing reads their scores
       uint8_t* dst = sQ + buf * C::QBytes + (lane >> 4) * (NP * 128) + (lane & 1) * 8;
 #pragma unroll
-      for (int i = 0; i < RP / 8; ++i) {
-        const int r = warp - 4 + 8 * i;
+      for (int i = 0; i < RP / QW; ++i) {
+        const int r = warp - 4 + QW * i;
         if (r >= nx_rows) break;
         const uint32_t u[4] = {qraw[i].x, qraw[i].y, qraw[i].z, qraw[i].w};
         // the largest value of the row, as 16-bit patterns without their sign
@@ -552,7 +557,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
 #pragma unroll
       for (int i = 0; i < RH; ++i) {
         const float d = __uint_as_float(raw[i]) + (__uint_as_float(raw[RH + i]) + __uint_as_float(raw[2 * RH + i]) * 0.0625f) * 0.0625f;
-        x[i] = (sees >> (2 * i)) & 1u ? d * (ks * qs[i]) : -INFINITY;
+        x[i] = (sees >> (SG * i)) & 1u ? d * (ks * qs[i]) : -INFINITY;
       }
 #pragma unroll
       for (int i = 0; i < RH; ++i) {
@@ -564,7 +569,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(red + hh);
       if (!(ok = mbar_wait_warp_small(red + hh, j & 1, abort_flag, 0x6d))) break;
-      // lane i: row 2 i + hh's maximum of the tile, and the factors of what was before and of this tile
+      // lane i: row SG i + hh's maximum of the tile, and the factors of what was before and of this tile
       float mt = -INFINITY;
       if (lane < RH) mt = fmaxf(fmaxf(rd[lane], rd[RP + lane]), fmaxf(rd[2 * RP + lane], rd[3 * RP + lane]));
       const float mn = fmaxf(m_run, mt);
@@ -603,7 +608,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         // the values of tokens that are not there may be anything (a weight of 0 times NaN would be NaN): zeros
         const int u = NK + j % NV;
         if (!(ok = mbar_wait_warp_small(full + u, (j / NV) & 1, abort_flag, 0x6f))) break;
-        if (!valid) {
+        if (!valid && hh < 2) {
           uint4* row = reinterpret_cast<uint4*>(ring + u * kPA_Unit + hh * (kPA_Tile * 128) + tok * 128);
 #pragma unroll
           for (int i = 0; i < 8; ++i) row[(i + tok) & 7] = make_uint4(0u, 0u, 0u, 0u);     // a chunk per lane: rows are as long as all banks
@@ -630,7 +635,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
     }
   } else {
     // ------------------------------------------------------------------ accumulators: thread = dim d of every row
-    const int wq = warp & 3, half = (warp - 12) >> 2, d = half * 128 + wq * 32 + lane;
+    const int wq = warp & 3, half = (warp - 4 - 4 * SG) >> 2, d = half * 128 + wq * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + (2 + half) * NP;
     float acc[RP];
     bool ok = true, from_start = w.tile == 0;
@@ -680,7 +685,7 @@ __global__ void __launch_bounds__(kPA_Threads, 1)
         }
         const int row = ((w.b * a.t + i0 + ih.x) * a.H) + w.g * a.R + ih.y;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;       // nothing seen: zeros
-        if (mine_row && warp == 12) {
+        if (mine_row && warp == 4 + 4 * SG) {
           if (!whole)
             *reinterpret_cast<float2*>(part + rc * kPA_Part + kPG_D) = make_float2(m, sum);
           else if (a.lse)
@@ -801,7 +806,7 @@ template <typename T, int RP>
 static int launch_paged(const CUtensorMap& kmap, const CUtensorMap& vmap, const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   int rc = ensure_smem_attr((const void*)paged_attn_kernel<T, RP>, PagedCfg<RP>::Smem);
   if (rc) return rc;
-  paged_attn_kernel<T, RP><<<ctas, kPA_Threads, PagedCfg<RP>::Smem, stream>>>(kmap, vmap, a);
+  paged_attn_kernel<T, RP><<<ctas, PagedCfg<RP>::Threads, PagedCfg<RP>::Smem, stream>>>(kmap, vmap, a);
   if ((rc = launch_status())) return rc;
   // may start while the last CTAs of the first kernel run, and waits for their results itself
   cudaLaunchConfig_t cfg{};
