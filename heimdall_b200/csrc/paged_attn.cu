@@ -385,6 +385,9 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
       if (first && !mbar_wait_warp_small(q_full + (seg & 1), (seg >> 1) & 1, abort_flag, 0x65)) break;
       if (!mbar_wait_warp_small(full + u, uphase, abort_flag, 0x66)) break;
       if (j >= 2 && !mbar_wait_warp_small(s_free + s, ((j >> 1) - 1) & 1, abort_flag, 0x67)) break;
+      // the accumulators have taken over tile j - 2, so its P, its factors and its O may be written over once S of this tile is there:
+      // waited for here, where it costs nothing, and not again on the way of the softmax warps and of O
+      if (j >= 2 && !mbar_wait_warp_small(o_free + s, ((j >> 1) - 1) & 1, abort_flag, 0x64)) break;
       tc_fence_after();
       first = w.tile + 1 == w.ntiles;
       const bool end = first || j + 1 == count;
@@ -416,7 +419,6 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
       const int s = j & 1;
       if (!mbar_wait_warp_small(full + NK + u, uphase, abort_flag, 0x63)) break;
       if (!mbar_wait_warp_small(p_full + s, (j >> 1) & 1, abort_flag, 0x62)) break;
-      if (j >= 2 && !mbar_wait_warp_small(o_free + s, ((j >> 1) - 1) & 1, abort_flag, 0x64)) break;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t dv = dv0 + (uint32_t)((NK + u) * (kPA_Unit >> 4)), dp = dp0 + (uint32_t)(s * (C::PBytes >> 4));
@@ -577,8 +579,6 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
       const float f = mt == -INFINITY ? 0.f : ex2_approx(mt - mn);
       m_run = mn;
       mt = mt == -INFINITY ? 0.f : mt;
-      // P of the tile before the last but one has been read, and so have its factors
-      if (j >= 2 && !(ok = mbar_wait_warp_small(o_free + s, ((j >> 1) - 1) & 1, abort_flag, 0x6e))) break;
       if (wq == 0 && lane < RH)
         *reinterpret_cast<float2*>(s_fac + (s * RP + hh * RH + lane) * 2) = make_float2(al, f * top * (1.f / 256.f));
       uint8_t* pd = sP + s * C::PBytes;
