@@ -219,6 +219,34 @@ def test_attend_many_sequences():
     _check_attend(c, _rand(n, 1, 2, D, seed=6), None)
 
 
+def test_attend_more_sequences_than_threads():
+    """Slots in any order, as 64-bit numbers, more sequences than a CTA has threads; the longest is cut over many CTAs."""
+    n = 900
+    lens = [(37 * i) % 60 for i in range(n)]
+    lens[700] = 4000
+    c = _cache(1, 1200, 1, n, page=64, max_len=4096)
+    c.reserve(range(n), lens)
+    _fill(c, 12)
+    _poison(c)
+    slots = [(i * 7) % n for i in range(n)]
+    _check_attend(c, _rand(n, 1, 2, D, seed=13), slots)
+
+
+def test_append_many_sequences():
+    n = 75
+    news = [(11 * i) % 40 for i in range(n)]
+    c = _cache(1, 200, 1, n + 2, page=32, max_len=96)
+    slots = [(i * 2 + 1) % (n + 2) for i in range(n)]
+    c.reserve(slots, [i % 7 for i in range(n)])
+    c.reserve(slots, news)
+    _fill(c, 14)
+    T = sum(news)
+    k, v = _rand(T, 1, D, seed=15) * 5, _rand(T, 1, D, seed=16)
+    before = _host(c)
+    c.append(0, k.cuda(), v.cuda(), torch.tensor(slots, device="cuda"), torch.tensor([0] + news).cumsum(0).cuda())
+    _check_append(c, before, slots, news, k, v)
+
+
 def test_attend_one_heavy_key_among_many():
     """A weight near one beside thousands near 2^-13: their sum counts."""
     c = _cache(1, 64, 1, 1, page=128, max_len=8192)

@@ -216,6 +216,14 @@ def test_many_sequences():
     _check(o, lse, q, k, v, _cu(lens))
 
 
+def test_more_sequences_than_shared_memory_lists():
+    lens = [(5 * i) % 4 for i in range(1200)]
+    T = sum(lens)
+    q, k, v = _inputs(T, T, 2, 1, torch.bfloat16, 15)
+    o, lse = _run(q, k, v, _cu(lens))
+    _check(o, lse, q, k, v, _cu(lens))
+
+
 def test_no_tokens():
     dev = _dev()
     from heimdall_b200 import prompt_attention
