@@ -61,15 +61,16 @@ __global__ void __launch_bounds__(256, L == 64 ? 3 : 1) paged_append_kernel(Appe
   const int tid = threadIdx.x, g = blockIdx.y;
   int b, ord, tok0 = 0, n = a.t;
   if (a.cu) {
-    // sequence b owns the items cu[b] / L + 2 b ...: at least one more than the pages that its tokens can touch.  Every warp looks
-    // through 32 sequences at a time
+    // sequence b owns the items cu[b] / L + 2 b ...: at least one more than the pages that its tokens can touch.  Every warp cuts
+    // the range that b is in, n sequences from b on, into 32 pieces at a time
     b = 0;
-    for (int c = 0; c < a.B; c += 32) {
-      const int i = c + (tid & 31);
-      const unsigned ok = __ballot_sync(0xffffffffu, i < a.B && min(max(a.cu[min(i, a.B)], 0), a.t) / L + 2 * i <= (int)blockIdx.x);
-      if (ok == 0u) break;
-      b = c + 31 - __clz(ok);
-      if (ok != 0xffffffffu) break;
+    for (int n_in = a.B, step = a.B; step > 1;) {
+      step = (n_in + 31) / 32;
+      const int i = (tid & 31) * step;
+      const unsigned ok = __ballot_sync(0xffffffffu, i < n_in && min(max(a.cu[b + min(i, n_in)], 0), a.t) / L + 2 * (b + i) <= (int)blockIdx.x);
+      const int at = ok ? (31 - __clz(ok)) * step : 0;
+      b += at;
+      n_in = min(step, n_in - at);
     }
     tok0 = min(max(a.cu[b], 0), a.t);
     n = min(max(a.cu[b + 1], tok0), a.t) - tok0;

@@ -47,6 +47,9 @@ constexpr int kPR_Tiles = kPR_SmemQ + 2 * kPR_SmemK + 2 * kPR_SmemV;
 constexpr int kPR_Items = 3;      // items known ahead
 constexpr int kPR_Ask = 4;        // the next item is asked for this many key tiles before the loads of the last one end
 constexpr int kPR_Parts = 1022;   // parts of a call whose first rows and keys fit into shared memory
+// Limits: the waits give up after about a second, an item of 2^25 keys takes a third of that, and the first look through 2^20 sequences
+// a few hundredths
+constexpr int kPR_MaxKeys = 1 << 25, kPR_MaxSeqs = 1 << 20;
 constexpr int kPR_Smem = kPR_Tiles + 640 + 5120 + 8192 + 4 * 2048 + 1024;
 constexpr uint32_t kPR_TmO = 256;
 constexpr float kPR_Rescale = 8.0f;
@@ -110,9 +113,14 @@ __device__ __forceinline__ PromptBlock prompt_of_lane(const PromptPart& p, int i
 // The last blocks to start decide how long the call takes: chunks of 512 tokens after 8192, 1000, 2048 and 4096 earlier ones
 // took 164 us in the order of the sequences.
 // With more parts than lanes: in the reverse order of the rows; part p owns the block numbers q0 / qb + p and up, at least as many as
-// it has blocks, and is found by bisection in shared memory (starts: first row and key of each part, and the ends), or, with more
-// than fit there, by going through all parts again.
+// it has blocks, and is found by bisection in shared memory (starts: first row and key of each part, and the ends).  With more
+// parts than fit there, starts holds every step-th one's (step = 32 or more) and the parts from that one on are gone through.
 __device__ __forceinline__ bool prompt_few(const PromptArgs& a) { return a.n_seq + 2 <= 32; }
+__device__ __forceinline__ int prompt_step(const PromptArgs& a) {
+  int step = 32;
+  while ((a.n_seq + 2) / step >= kPR_Parts) step *= 2;
+  return step;
+}
 __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, const PromptPart& first, const int2* starts, int rank, int lane) {
   if (prompt_few(a)) {
     const PromptPart p = first;
@@ -153,8 +161,14 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, const P
     const bool keys = lo >= 1 && lo <= a.n_seq;
     return PromptBlock{s.x, e.x - s.x, s.y, keys ? e.y - s.y : 0, (blk - (s.x >> a.qlog) - lo) << a.qlog};
   }
-  int carry_q = 0, carry_k = 0;
-  for (int c = 0; c < a.n_seq + 2; c += 32) {
+  const int step = prompt_step(a);
+  int lo = 0, hi = (a.n_seq + 1) / step;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((starts[mid].x >> a.qlog) + mid * step <= blk) lo = mid; else hi = mid - 1;
+  }
+  int carry_q = starts[lo].x, carry_k = starts[lo].y;
+  for (int c = lo * step; c < a.n_seq + 2; c += 32) {
     const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
     const int base = (p.q0 >> a.qlog) + c + lane;
     const unsigned ok = __ballot_sync(0xffffffffu, c + lane < a.n_seq + 2 && base <= blk);
@@ -337,6 +351,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
           if (c + lane < a.n_seq + 2) s_starts[c + lane] = make_int2(p.q0, p.k0);
           if (c + lane == a.n_seq + 1) s_starts[a.n_seq + 2] = make_int2(p.q0 + p.nq, p.k0 + p.nk);
+        }
+        __syncwarp();
+      } else {
+        const int step = prompt_step(a);
+        for (int c = 0; c < a.n_seq + 2; c += 32) {
+          const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
+          if (c % step == 0 && lane == 0) s_starts[c / step] = make_int2(p.q0, p.k0);
         }
         __syncwarp();
       }
@@ -651,6 +672,7 @@ int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void
   if (T < 0 || Tk < 0 || n_seq < 0 || H <= 0 || G <= 0 || H % G || !(scale > 0.f) || scale > 3e38f)
     return BF_ERR_INVALID_ARGUMENT;
   if (D != kPR_D || (dtype != BF_BF16 && dtype != BF_F16)) return BF_ERR_UNSUPPORTED;
+  if (Tk > kPR_MaxKeys || n_seq > kPR_MaxSeqs) return BF_ERR_UNSUPPORTED;
   if (T == 0) return BF_OK;
   if (!q || !o || (Tk > 0 && (!k || !v)) || (n_seq > 0 && !cu_q)) return BF_ERR_INVALID_ARGUMENT;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || ((q_st | q_sh | k_st | k_sh | v_st | v_sh) & 7))

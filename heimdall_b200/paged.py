@@ -166,6 +166,8 @@ class PagedKV:
 
     def length(self, slot: int) -> int:
         """Tokens of a slot, as the host knows them (no device read)."""
+        if not 0 <= slot < self.host.slots:
+            raise ValueError(_REASONS[1].format(slots=self.host.slots))
         return int(self.host.lens[slot])
 
     def _apply(self, change, *args) -> None:
@@ -254,7 +256,8 @@ class PagedKV:
         """Attention of each sequence's last t tokens over its pages: q [B,t,H,D] (bf16 or fp16; H a multiple of the KV
         heads) at the positions lens - t .. lens - 1, each seeing the positions up to its own.  Returns o [B,t,H,D] in q's
         dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf.  What the pages hold
-        behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t tokens."""
+        behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t tokens.  A token's weight times its V scale is held to
+        2^-26 of (largest weight) * (largest V scale) among the 128 tokens of its tile."""
         dev = serving_inputs("PagedKV.attend", self.k_pages, q)
         layer, shape = self._layer(layer), q.shape
         if len(shape) != 4 or shape[3] != self.dim or shape[2] % self.heads or shape[2] < 1:
@@ -308,5 +311,5 @@ class PagedLayer:
             return c.attend(self.index, q)[0].to(qr.dtype)
         # a whole prompt: attention over the keys and values as they are, not over their codes
         cu = torch.arange(B + 1, device=qr.device, dtype=torch.int32) * t
-        o, _ = prompt_attention(q.reshape(B * t, H, D), k.reshape(B * t, -1, D), v.reshape(B * t, -1, D), cu)
+        o, _ = prompt_attention(q.reshape(B * t, H, D), k.reshape(B * t, c.heads, D), v.reshape(B * t, c.heads, D), cu)
         return o.reshape(B, t, H, D).to(qr.dtype)

@@ -354,7 +354,7 @@ int bf_llama_state_unpack(const float* rows, long long row_stride, const int64_t
  *   of 8, a head's D elements contiguous); cu_q, cu_k [n_seq + 1] int32 on the device, ascending: every entry is clamped
  *   into [previous, T] (or Tk); o [T,H,D] contiguous in dtype; lse [H,T] fp32 or NULL.
  * A query that sees no key, and every row of no sequence, gets o = 0 and lse = -inf.
- * D = 256, scale > 0.
+ * D = 256, scale > 0, at most 2^25 keys and 2^20 sequences.
  */
 int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void* k, long long k_st, long long k_sh,
                        const void* v, long long v_st, long long v_sh, const int32_t* cu_q, const int32_t* cu_k,
@@ -379,7 +379,8 @@ int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void
  * bf_paged_attend: the last t tokens of each sequence against its pages: q [B,t,H,D] (dtype; element strides per batch,
  *   token and head) is at positions lens - t .. lens - 1 and token i sees the positions <= its own whose page is in the
  *   table.  o [B,t,H,D] contiguous in dtype, lse [B,H,t] fp32 or NULL; a row that sees nothing gets 0 and -inf.
- *   Workspace: bf_paged_attend_workspace().  H / G <= 24.
+ *   Workspace: bf_paged_attend_workspace().  H / G <= 24; B t H and B G ceil(t / floor(24 G / H)) (width L / 128 + 4) below 2^31.
+ *   A token's weight times its V scale is held to 2^-26 of (largest weight) * (largest V scale) among the 128 tokens of its tile.
  * bf_paged_pages: page bookkeeping and copies on the device; every list is HOST memory, read before the call returns.
  *   release [n_release]: slots whose table rows become -1 and lens 0;
  *   fork [n_fork][5] = (from slot, to slot, tokens, from page, to page): the row and length of `from`, and, where

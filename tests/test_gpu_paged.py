@@ -232,11 +232,11 @@ def test_attend_more_sequences_than_threads():
     _check_attend(c, _rand(n, 1, 2, D, seed=13), slots)
 
 
-def test_append_many_sequences():
-    n = 75
-    news = [(11 * i) % 40 for i in range(n)]
-    c = _cache(1, 200, 1, n + 2, page=32, max_len=96)
-    slots = [(i * 2 + 1) % (n + 2) for i in range(n)]
+@pytest.mark.parametrize("n,page", [(75, 32), (1100, 16), (33, 128)])
+def test_append_many_sequences(n, page):
+    news = [(11 * i) % 40 * (n < 100 or i % 5 == 0) for i in range(n)]
+    c = _cache(1, n * 3, 1, n + 2, page=page, max_len=max(page, 96))
+    slots = [(i * 2 + 1) % (n + 2 if n % 2 else n + 1) for i in range(n)]
     c.reserve(slots, [i % 7 for i in range(n)])
     c.reserve(slots, news)
     _fill(c, 14)
@@ -245,6 +245,25 @@ def test_append_many_sequences():
     before = _host(c)
     c.append(0, k.cuda(), v.cuda(), torch.tensor(slots, device="cuda"), torch.tensor([0] + news).cumsum(0).cuda())
     _check_append(c, before, slots, news, k, v)
+
+
+def test_calls_without_sequences_or_tokens():
+    c = _cache(1, 4, 2, 2, page=16, max_len=32)
+    c.reserve([0], 3)
+    c.reserve([], 1), c.free([]), c.fork([], []), c.truncate([], 0)
+    before = _host(c)
+    none, cu = torch.zeros(0, dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    k = torch.zeros(0, 2, D, dtype=torch.bfloat16, device="cuda")
+    c.append(0, k, k, none, cu)
+    c.append(0, k[None], k[None])
+    c.append(0, k.view(0, 1, 2, D), k.view(0, 1, 2, D))
+    for B, t in ((0, 1), (2, 0), (0, 0)):
+        o, lse = c.attend(0, torch.zeros(B, t, 4, D, dtype=torch.bfloat16, device="cuda"), none if B == 0 else None, with_lse=True)
+        assert o.shape == (B, t, 4, D) and lse.shape == (B, 4, t)
+    assert all(_same(x, y) for x, y in zip(_host(c), before)) and c.length(0) == 3
+    for slot in (-1, 2):
+        with pytest.raises(ValueError):
+            c.length(slot)
 
 
 def test_attend_one_heavy_key_among_many():

@@ -224,6 +224,14 @@ def test_more_sequences_than_shared_memory_lists():
     _check(o, lse, q, k, v, _cu(lens))
 
 
+def test_very_many_sequences_few_of_them_with_tokens():
+    lens = [(1 + i % 3) * (i % 97 == 5) for i in range(40000)] + [130]
+    T = sum(lens)
+    q, k, v = _inputs(T, T, 3, 1, torch.float16, 16)
+    o, lse = _run(q, k, v, _cu(lens))
+    _check(o, lse, q, k, v, _cu(lens))
+
+
 def test_no_tokens():
     dev = _dev()
     from heimdall_b200 import prompt_attention

@@ -195,6 +195,7 @@ def test_c_entries_check_their_arguments_before_a_launch():
         "bf_prompt_attn_fwd", q, st, 256, P, 1024, 256, P, 1024, 256, cu, 0, n, T, Tk, H, G, D, dt, scale, o, 0, 0)
     assert prompt(q=0) == 1 and prompt(o=0) == 1 and prompt(cu=0) == 1 and prompt(T=-1) == 1 and prompt(H=23) == 1
     assert prompt(scale=0.0) == 1 and prompt(scale=float("nan")) == 1 and prompt(scale=float("inf")) == 1
+    assert prompt(Tk=2 ** 25 + 1) == 2 and prompt(n=2 ** 20 + 1) == 2
     assert prompt(D=128) == 2 and prompt(dt=0) == 2 and prompt(q=P + 8) == 3 and prompt(st=6140) == 3
     keep = []
 
