@@ -206,11 +206,14 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
     *abort_flag = 0;
     fence_barrier_init();
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  let_next_start();
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TmemCols);
     tmem_relinquish();
   }
+  if (warp == 0 && lane == 0) tma_prefetch(&kmap);
+  if (warp == 2 && lane == 0) tma_prefetch(&vmap);
+  wait_for_stream();
   // this CTA's run: every segment is Start units and one for each of its tiles.  The sequences' units are summed over the block,
   // thread i holding `per` consecutive sequences (the caller has made sure that 32 bits hold the sum)
   const int per = (a.B + C::Threads - 1) / C::Threads;
@@ -295,7 +298,6 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
     // ------------------------------------------------------------------ codes: K (warp 0), V (warp 2)
     const bool is_v = warp == 2;
     const void* map = is_v ? &vmap : &kmap;
-    if (lane == 0) tma_prefetch(map);
     // each ring has one producer, which waits for its slots' rounds one by one (with K and V in one ring of an odd number of slots, a
     // producer could meet a slot two rounds behind and take the parity of the round before for its own)
     const int units = is_v ? NV : NK, base = is_v ? NK : 0;
@@ -736,7 +738,8 @@ template <typename T, int RP>
 __global__ void __launch_bounds__(256) paged_combine_kernel(PagedAttnArgs a) {
   __shared__ float4 s_acc[8][32];
   __shared__ float2 s_ml[8][32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  let_next_start();
+  wait_for_stream();
   const int x = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int4 desc = a.desc[x];
   if (desc.x < 0) return;
@@ -806,20 +809,8 @@ template <typename T, int RP>
 static int launch_paged(const CUtensorMap& kmap, const CUtensorMap& vmap, const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
   int rc = ensure_smem_attr((const void*)paged_attn_kernel<T, RP>, PagedCfg<RP>::Smem);
   if (rc) return rc;
-  paged_attn_kernel<T, RP><<<ctas, PagedCfg<RP>::Threads, PagedCfg<RP>::Smem, stream>>>(kmap, vmap, a);
-  if ((rc = launch_status())) return rc;
-  // may start while the last CTAs of the first kernel run, and waits for their results itself
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, 4);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_combine_kernel<T, RP>, a);
-  return e == cudaSuccess ? BF_OK : cuda_fail(e);
+  rc = launch_early(paged_attn_kernel<T, RP>, dim3(ctas), PagedCfg<RP>::Threads, PagedCfg<RP>::Smem, stream, kmap, vmap, a);
+  return rc ? rc : launch_early(paged_combine_kernel<T, RP>, dim3(ctas, 4), 256, 0, stream, a);
 }
 
 }  // namespace bfb

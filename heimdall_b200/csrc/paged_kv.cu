@@ -58,19 +58,21 @@ __global__ void __launch_bounds__(256, L == 64 ? 3 : 1) paged_append_kernel(Appe
   constexpr int PASS = L / 16;
   __shared__ float s_max[2][8];
   __shared__ int s_dup;
+  let_next_start();
+  wait_for_stream();
   const int tid = threadIdx.x, g = blockIdx.y;
   int b, ord, tok0 = 0, n = a.t;
   if (a.cu) {
     // sequence b owns the items cu[b] / L + 2 b ...: at least one more than the pages that its tokens can touch.  Every warp cuts
-    // the range that b is in, n sequences from b on, into 32 pieces at a time
+    // the range that b is in into 32 pieces of `step` sequences at a time
     b = 0;
-    for (int n_in = a.B, step = a.B; step > 1;) {
-      step = (n_in + 31) / 32;
-      const int i = (tid & 31) * step;
-      const unsigned ok = __ballot_sync(0xffffffffu, i < n_in && min(max(a.cu[b + min(i, n_in)], 0), a.t) / L + 2 * (b + i) <= (int)blockIdx.x);
-      const int at = ok ? (31 - __clz(ok)) * step : 0;
-      b += at;
-      n_in = min(step, n_in - at);
+    int step = 1;
+    while (32 * step < a.B) step *= 32;
+#pragma unroll 1
+    for (; step > 0; step >>= 5) {
+      const int i = b + (tid & 31) * step;
+      const unsigned ok = __ballot_sync(0xffffffffu, i < a.B && min(max(a.cu[min(i, a.B)], 0), a.t) / L + 2 * i <= (int)blockIdx.x);
+      if (ok) b += (31 - __clz(ok)) * step;
     }
     tok0 = min(max(a.cu[b], 0), a.t);
     n = min(max(a.cu[b + 1], tok0), a.t) - tok0;
@@ -339,13 +341,10 @@ int bf_paged_append(const bf_page_pool* pool, int layer, const void* k, long lon
   const dim3 grid((unsigned)items, a.p.heads);
   auto go = [&](auto type) {
     using E = decltype(type);
-    if (L == 16) paged_append_kernel<E, 16><<<grid, 256, 0, stream>>>(a);
-    if (L == 32) paged_append_kernel<E, 32><<<grid, 256, 0, stream>>>(a);
-    if (L == 64) paged_append_kernel<E, 64><<<grid, 256, 0, stream>>>(a);
-    if (L == 128) paged_append_kernel<E, 128><<<grid, 256, 0, stream>>>(a);
+    return launch_early(L == 16 ? paged_append_kernel<E, 16> : L == 32 ? paged_append_kernel<E, 32>
+                        : L == 64 ? paged_append_kernel<E, 64> : paged_append_kernel<E, 128>, grid, 256, 0, stream, a);
   };
-  if (dtype == BF_BF16) go(__nv_bfloat16()); else go(__half());
-  return launch_status();
+  return dtype == BF_BF16 ? go(__nv_bfloat16()) : go(__half());
 }
 
 int bf_paged_pages(const bf_page_pool* pool, const int32_t* release, int n_release, const int32_t* fork, int n_fork,
