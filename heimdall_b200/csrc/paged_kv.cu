@@ -238,6 +238,8 @@ __device__ __forceinline__ void copy_page(const PagePool& p, int from, int to, i
 }
 
 __global__ void __launch_bounds__(256) pages_release_kernel(PagePool p, const __grid_constant__ PageList list) {
+  let_next_start();
+  wait_for_stream();
   const int slot = list.v[blockIdx.x];
   for (int i = threadIdx.x; i < p.width; i += 256) p.table[(size_t)slot * p.width + i] = -1;
   if (threadIdx.x == 0) p.lens[slot] = 0;
@@ -245,6 +247,8 @@ __global__ void __launch_bounds__(256) pages_release_kernel(PagePool p, const __
 
 template <int L>
 __global__ void __launch_bounds__(256) pages_fork_kernel(PagePool p, const __grid_constant__ PageList list) {
+  let_next_start();
+  wait_for_stream();
   const int* f = list.v + 5 * blockIdx.x;
   const int from = f[0], to = f[1], len = f[2];
   if (blockIdx.y == 0 && blockIdx.z == 0) {
@@ -257,11 +261,15 @@ __global__ void __launch_bounds__(256) pages_fork_kernel(PagePool p, const __gri
 
 template <int L>
 __global__ void __launch_bounds__(256) pages_move_kernel(PagePool p, const __grid_constant__ PageList list) {
+  let_next_start();
+  wait_for_stream();
   copy_page<L>(p, list.v[2 * blockIdx.x], list.v[2 * blockIdx.x + 1], L);
 }
 
 // table entries by binary search in the list's ascending sources
 __global__ void __launch_bounds__(256) pages_remap_kernel(PagePool p, const __grid_constant__ PageList list) {
+  let_next_start();
+  wait_for_stream();
   const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (size_t)p.slots * p.width) return;
   const int page = p.table[i];
@@ -274,6 +282,8 @@ __global__ void __launch_bounds__(256) pages_remap_kernel(PagePool p, const __gr
 }
 
 __global__ void __launch_bounds__(256) pages_set_kernel(PagePool p, const __grid_constant__ PageList list) {
+  let_next_start();
+  wait_for_stream();
   for (int i = threadIdx.x; i < list.n; i += 256) {
     const long long at = list.v[2 * i], cells = (long long)p.slots * p.width;
     if (at < cells) p.table[at] = list.v[2 * i + 1]; else p.lens[at - cells] = list.v[2 * i + 1];
@@ -379,33 +389,26 @@ int bf_paged_pages(const bf_page_pool* pool, const int32_t* release, int n_relea
       PageList l;
       l.n = n - at < most ? n - at : most;
       for (int i = 0; i < l.n * ints; ++i) l.v[i] = from[(size_t)at * ints + i];
-      launch(l);
-      const int e = launch_status();
+      const int e = launch(l);
       if (e) return e;
     }
     return BF_OK;
   };
   const unsigned lh = (unsigned)(p.layers * p.heads);
-  rc = pieces(release, n_release, 1, [&](const PageList& l) { pages_release_kernel<<<l.n, 256, 0, stream>>>(p, l); });
+  rc = pieces(release, n_release, 1, [&](const PageList& l) { return launch_early(pages_release_kernel, dim3(l.n), 256, 0, stream, p, l); });
   if (rc) return rc;
   rc = pieces(fork, n_fork, 5, [&](const PageList& l) {
-    const dim3 grid(l.n, lh, 2);
-    if (p.page == 16) pages_fork_kernel<16><<<grid, 256, 0, stream>>>(p, l);
-    if (p.page == 32) pages_fork_kernel<32><<<grid, 256, 0, stream>>>(p, l);
-    if (p.page == 64) pages_fork_kernel<64><<<grid, 256, 0, stream>>>(p, l);
-    if (p.page == 128) pages_fork_kernel<128><<<grid, 256, 0, stream>>>(p, l);
+    return launch_early(p.page == 16 ? pages_fork_kernel<16> : p.page == 32 ? pages_fork_kernel<32> : p.page == 64 ? pages_fork_kernel<64>
+                        : pages_fork_kernel<128>, dim3(l.n, lh, 2), 256, 0, stream, p, l);
   });
   if (rc) return rc;
   rc = pieces(move, n_move, 2, [&](const PageList& l) {
-    const dim3 grid(l.n, lh, 2);
-    if (p.page == 16) pages_move_kernel<16><<<grid, 256, 0, stream>>>(p, l);
-    if (p.page == 32) pages_move_kernel<32><<<grid, 256, 0, stream>>>(p, l);
-    if (p.page == 64) pages_move_kernel<64><<<grid, 256, 0, stream>>>(p, l);
-    if (p.page == 128) pages_move_kernel<128><<<grid, 256, 0, stream>>>(p, l);
-    pages_remap_kernel<<<(unsigned)((cells + 255) / 256), 256, 0, stream>>>(p, l);
+    const int e = launch_early(p.page == 16 ? pages_move_kernel<16> : p.page == 32 ? pages_move_kernel<32> : p.page == 64 ? pages_move_kernel<64>
+                               : pages_move_kernel<128>, dim3(l.n, lh, 2), 256, 0, stream, p, l);
+    return e ? e : launch_early(pages_remap_kernel, dim3((unsigned)((cells + 255) / 256)), 256, 0, stream, p, l);
   });
   if (rc) return rc;
-  return pieces(set, n_set, 2, [&](const PageList& l) { pages_set_kernel<<<1, 256, 0, stream>>>(p, l); });
+  return pieces(set, n_set, 2, [&](const PageList& l) { return launch_early(pages_set_kernel, dim3(1), 256, 0, stream, p, l); });
 }
 
 }  // extern "C"
