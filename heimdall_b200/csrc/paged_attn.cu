@@ -36,6 +36,7 @@
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
+#include "launch_early.h"
 #include "paged_kv.h"
 #include "tmap.h"
 

@@ -29,6 +29,7 @@
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
+#include "launch_early.h"
 #include "tmap.h"
 
 namespace bfb {
@@ -46,7 +47,7 @@ constexpr int kPR_SmemV = kPR_N * kPR_D / 2 * 2;      // 32 KB: this CTA's half 
 constexpr int kPR_Tiles = kPR_SmemQ + 2 * kPR_SmemK + 2 * kPR_SmemV;
 constexpr int kPR_Items = 3;      // items known ahead
 constexpr int kPR_Ask = 4;        // the next item is asked for this many key tiles before the loads of the last one end
-constexpr int kPR_Parts = 1022;   // parts of a call whose first rows and keys fit into shared memory
+constexpr int kPR_Parts = 1024;   // parts whose first rows and keys fit into shared memory
 // Limits: the waits give up after about a second, an item of 2^25 keys takes a third of that, and the first look through 2^20 sequences
 // a few hundredths
 constexpr int kPR_MaxKeys = 1 << 25, kPR_MaxSeqs = 1 << 20;
@@ -59,6 +60,7 @@ struct PromptArgs {
   int n_seq, T, Tk, H, G;
   int qb, qlog;           // tokens per block: 128 (two heads) or 256 (two tiles of one head), and its log2
   int nblk, hsplit;       // blocks, items per (block, KV head)
+  int step_log;
   float c2;               // scale * log2(e)
   void* o;
   float* lse;
@@ -113,14 +115,9 @@ __device__ __forceinline__ PromptBlock prompt_of_lane(const PromptPart& p, int i
 // The last blocks to start decide how long the call takes: chunks of 512 tokens after 8192, 1000, 2048 and 4096 earlier ones
 // took 164 us in the order of the sequences.
 // With more parts than lanes: in the reverse order of the rows; part p owns the block numbers q0 / qb + p and up, at least as many as
-// it has blocks, and is found by bisection in shared memory (starts: first row and key of each part, and the ends).  With more
-// parts than fit there, starts holds every step-th one's (step = 32 or more) and the parts from that one on are gone through.
+// it has blocks, and is found by bisection in shared memory, where starts holds the first row and key of every 2^step_log-th part (of
+// each one, if they fit), and by going through the parts from that one on.
 __device__ __forceinline__ bool prompt_few(const PromptArgs& a) { return a.n_seq + 2 <= 32; }
-__device__ __forceinline__ int prompt_step(const PromptArgs& a) {
-  int step = 32;
-  while ((a.n_seq + 2) / step >= kPR_Parts) step *= 2;
-  return step;
-}
 __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, const PromptPart& first, const int2* starts, int rank, int lane) {
   if (prompt_few(a)) {
     const PromptPart p = first;
@@ -151,24 +148,13 @@ __device__ __forceinline__ PromptBlock prompt_block(const PromptArgs& a, const P
   }
   PromptBlock r{0, 0, 0, 0, 0};
   const int blk = a.nblk - 1 - rank;
-  if (a.n_seq + 2 <= kPR_Parts) {
-    int lo = 0, hi = a.n_seq + 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((starts[mid].x >> a.qlog) + mid <= blk) lo = mid; else hi = mid - 1;
-    }
-    const int2 s = starts[lo], e = starts[lo + 1];
-    const bool keys = lo >= 1 && lo <= a.n_seq;
-    return PromptBlock{s.x, e.x - s.x, s.y, keys ? e.y - s.y : 0, (blk - (s.x >> a.qlog) - lo) << a.qlog};
-  }
-  const int step = prompt_step(a);
-  int lo = 0, hi = (a.n_seq + 1) / step;
+  int lo = 0, hi = (a.n_seq + 1) >> a.step_log;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if ((starts[mid].x >> a.qlog) + mid * step <= blk) lo = mid; else hi = mid - 1;
+    if ((starts[mid].x >> a.qlog) + (mid << a.step_log) <= blk) lo = mid; else hi = mid - 1;
   }
   int carry_q = starts[lo].x, carry_k = starts[lo].y;
-  for (int c = lo * step; c < a.n_seq + 2; c += 32) {
+  for (int c = lo << a.step_log; c < a.n_seq + 2; c += 32) {
     const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
     const int base = (p.q0 >> a.qlog) + c + lane;
     const unsigned ok = __ballot_sync(0xffffffffu, c + lane < a.n_seq + 2 && base <= blk);
@@ -228,7 +214,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   float* xch = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(bars) + 640);   // [2 tile parities][128] references
   float* xl = xch + 256;                                                           // [2 slots][2 warpgroups][128] row sums
   float* xmx = xl + 512;                                                           // [2 slots][2 warpgroups][128] their references
-  int2* s_starts = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(bars) + 640 + 5120);   // [kPR_Parts + 1], one warp's
+  int2* s_starts = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(bars) + 640 + 5120);   // [kPR_Parts], one warp's
   uint8_t* s_out = reinterpret_cast<uint8_t*>(bars) + 640 + 5120 + 8192;          // [4 output warps][32 rows][128 B]
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -283,6 +269,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  wait_for_stream();
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPR_RegsCtl));
@@ -346,18 +333,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       PromptPart first{0, 0, 0, 0};
       if (prompt_few(a)) {
         first = prompt_part(a, 0, lane, carry_q, carry_k);
-      } else if (a.n_seq + 2 <= kPR_Parts) {
-        for (int c = 0; c < a.n_seq + 2; c += 32) {
-          const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
-          if (c + lane < a.n_seq + 2) s_starts[c + lane] = make_int2(p.q0, p.k0);
-          if (c + lane == a.n_seq + 1) s_starts[a.n_seq + 2] = make_int2(p.q0 + p.nq, p.k0 + p.nk);
-        }
-        __syncwarp();
       } else {
-        const int step = prompt_step(a);
         for (int c = 0; c < a.n_seq + 2; c += 32) {
           const PromptPart p = prompt_part(a, c, lane, carry_q, carry_k);
-          if (c % step == 0 && lane == 0) s_starts[c / step] = make_int2(p.q0, p.k0);
+          const int at = (c + lane) >> a.step_log;
+          if (c + lane < a.n_seq + 2 && at << a.step_log == c + lane) s_starts[at] = make_int2(p.q0, p.k0);
         }
         __syncwarp();
       }
@@ -655,8 +635,7 @@ static int launch_prompt(const CUtensorMap& qmap, const CUtensorMap& kmap, const
                          long long clusters, cudaStream_t stream) {
   const int rc = ensure_smem_attr((const void*)prompt_attn_kernel<T>, kPR_Smem);
   if (rc) return rc;
-  prompt_attn_kernel<T><<<(unsigned)(2 * clusters), kPR_Threads, kPR_Smem, stream>>>(qmap, kmap, vmap, a);
-  return launch_status();
+  return launch_early(prompt_attn_kernel<T>, dim3((unsigned)(2 * clusters)), kPR_Threads, kPR_Smem, stream, qmap, kmap, vmap, a);
 }
 
 }  // namespace bfb
@@ -697,6 +676,7 @@ int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void
   a.nblk = (int)nblk;
   a.qlog = a.qb == kPR_M ? 7 : 8;
   a.hsplit = R % 2 == 0 ? R / 2 : R;
+  while ((n_seq + 1) >> a.step_log >= kPR_Parts) ++a.step_log;
   const long long clusters = nblk * G * a.hsplit;
   if (clusters > 0x3fffffffLL) return BF_ERR_UNSUPPORTED;
   // (64 dims, tokens, 4 groups of 64 dims, heads); a stride of a dimension of one means nothing, and the encoder wants a positive one
