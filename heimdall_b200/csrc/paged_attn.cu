@@ -31,8 +31,10 @@
 // warps that stay converged and elect the issuing lane do not bound it.  The roles together have to stay in the instruction
 // cache: waits and loops are written for few instructions (106 KB of code took a third longer than 72 KB).
 // Measured (24 query heads, 4 KV heads, pages of 64): 64 sequences of 16384 tokens 326 us, all that the measured copy rate allows
-// (331 us); 64 of 1 to 16384 tokens 52 us (floor 36); one of 777 tokens 10.5 us.  24 rows (four tokens): 4600 cycles a tile, bound by
-// the softmax warps' instructions: 32 sequences of 16384 tokens 275 us (floor 166).
+// (331 us); 64 of 1 to 16384 tokens 51 us (floor 36); one of 777 tokens 9.6 us.  24 rows (four tokens): 3550 cycles a tile, bound by
+// the softmax warps' way through a tile: 32 sequences of 16384 tokens 225 us (floor 166), with pages of 16 tokens 247 (eight copies
+// per tile and half).  There 80 registers per thread are all there are, and what does not fit costs: 244 us with 28 bytes spilled.
+// (Taking a tile's scores before the weights of the one before, so that nobody waits for the maxima, made it 267 us.)
 #include "bifrost_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -444,19 +446,16 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
     constexpr int RH = RP / SG;
     const int wq = warp & 3, hh = (warp - 4) >> 2, tok = wq * 32 + lane;
     const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + hh * RH;
-    float l[RH], qs[RH];
+    float l[RH];
     int rows = 0, first_pos = 0;         // of the chunk; the position of its first token
     float m_run = -INFINITY;             // of row SG lane + hh, in lanes < RH
     bool ok = true, first = true;
     int seg = 0;
     // the queries: warp w of the 4 SG takes rows w, w + 4 SG, ..., lane l dims 8 l .. 8 l + 7
     constexpr int QW = 4 * SG;
-    PagedWalk nx = w;                    // the segment whose queries are in `raw`
-    int nx_at = 0, nx_rows = 0;          // its first tile in the run
     uint4 qraw[RP / QW];
-    auto q_load = [&]() {
-      const int i0 = nx.c * a.tc;
-      nx_rows = min(a.tc, a.t - i0) * a.R;
+    auto q_load = [&](const PagedWalk& nx) {
+      const int i0 = nx.c * a.tc, nx_rows = min(a.tc, a.t - i0) * a.R;
 #pragma unroll
       for (int i = 0; i < RP / QW; ++i) {
         const int r = warp - 4 + QW * i;
@@ -466,7 +465,10 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
                                                          (long long)(nx.g * a.R + ih.y) * a.q_sh + 8 * lane));
       }
     };
-    auto q_store = [&](int buf) {        // rows from nx_rows on stay as they are, nothing reads their scores
+    // the queries in qraw, of segment nx, which begins with tile `at` of the run; then nx and qraw are the next segment's.  Rows from
+    // nx_rows on stay as they are, nothing reads their scores
+    auto q_store = [&](PagedWalk& nx, int& at, int buf) {
+      const int nx_rows = min(a.tc, a.t - nx.c * a.tc) * a.R;
       uint8_t* dst = sQ + buf * C::QBytes + (lane >> 4) * (NP * 128) + (lane & 1) * 8;
 #pragma unroll
       for (int i = 0; i < RP / QW; ++i) {
@@ -500,15 +502,18 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full + buf);
-      nx_at += nx.skip(a);
-      if (nx_at < count) q_load();
+      at += nx.skip(a);
+      if (at < count) q_load(nx);
     };
-    if (count > 0) q_load();
+    if (count > 0) q_load(w);
 #pragma unroll 1
     for (int j = 0; j < count; ++j) {
       const int s = j & 1;
       if (first) {
         // store the next segment's queries (and, at the run's start, this one's before them)
+        PagedWalk nx = w;
+        int at = j;
+        if (j) at += nx.skip(a);
 #pragma unroll 1
         for (int k = j ? 1 : 0; k < 2 && ok; ++k) {
           if (k) {
@@ -517,21 +522,25 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
             first_pos = w.len - a.t + w.c * a.tc;
             m_run = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < RH; ++i) {
-              l[i] = 0.f;
-              qs[i] = s_qs[(seg & 1) * RP + hh * RH + i];
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(q_free + (seg & 1));
+            for (int i = 0; i < RH; ++i) l[i] = 0.f;
           }
-          if (nx_at < count) {
+          if (at < count) {
             if (k && seg >= 1 && !(ok = mbar_wait_warp_small(q_free + ((seg + 1) & 1), (((seg + 1) >> 1) - 1) & 1, abort_flag, 0x68))) break;
-            q_store((seg + k) & 1);
+            q_store(nx, at, (seg + k) & 1);
           }
         }
         if (!ok) break;
       }
       const bool last = w.tile + 1 == w.ntiles, end = last || j + 1 == count;
+      // the scores, four rows at a time (more registers there are not for 24 rows), the first of them on their way while the mask is made
+      if (!(ok = mbar_wait_warp_small(s_full + s, (j >> 1) & 1, abort_flag, 0x6c))) break;
+      tc_fence_after();
+      uint32_t raw[12];
+      auto load4 = [&](int c) {
+#pragma unroll
+        for (int part = 0; part < 3; ++part) tmem_ld4(trow + s * NP + part * RP + c, raw + part * 4);
+      };
+      load4(0);
       if (!(ok = mbar_wait_warp_small(sc_full + (j & 3), (j >> 2) & 1, abort_flag, 0x6b))) break;
       const float* sc = s_sc + (j & 3) * 20;
       const int pi = tok >> a.page_log;
@@ -542,27 +551,25 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
       // bit r: row r's token is at or behind this position (the first of them is that many tokens into the chunk)
       const unsigned later = (unsigned)min(max(pos - first_pos, 0) * a.R, 31);
       const unsigned sees = valid ? (((1u << rows) - 1u) >> later << later) >> hh : 0u;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sc_free + (j & 3));
-      if (!(ok = mbar_wait_warp_small(s_full + s, (j >> 1) & 1, abort_flag, 0x6c))) break;
-      tc_fence_after();
-      uint32_t raw[3 * RH];
-#pragma unroll
-      for (int part = 0; part < 3; ++part) {
-#pragma unroll
-        for (int c = 0; c + 8 <= RH; c += 8) tmem_ld8(trow + s * NP + part * RP + c, raw + part * RH + c);
-        if (RH % 8) tmem_ld4(trow + s * NP + part * RP + RH / 8 * 8, raw + part * RH + RH / 8 * 8);
-      }
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_free + s);
       float x[RH], mine = -INFINITY;
+      const float* qs = s_qs + (seg & 1) * RP + hh * RH;
       float* rd = s_red + s * 4 * RP + hh * RH;
 #pragma unroll
-      for (int i = 0; i < RH; ++i) {
-        const float d = __uint_as_float(raw[i]) + (__uint_as_float(raw[RH + i]) + __uint_as_float(raw[2 * RH + i]) * 0.0625f) * 0.0625f;
-        x[i] = (sees >> (SG * i)) & 1u ? d * (ks * qs[i]) : -INFINITY;
+      for (int c = 0; c < RH; c += 4) {
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float d = __uint_as_float(raw[i]) + (__uint_as_float(raw[4 + i]) + __uint_as_float(raw[8 + i]) * 0.0625f) * 0.0625f;
+          x[c + i] = (sees >> (SG * (c + i))) & 1u ? d * (ks * qs[c + i]) : -INFINITY;
+        }
+        if (c + 4 < RH) load4(c + 4);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(s_free + s);
+        mbar_arrive(sc_free + (j & 3));
+        if (end) mbar_arrive(q_free + (seg & 1));
       }
 #pragma unroll
       for (int i = 0; i < RH; ++i) {
