@@ -17,7 +17,7 @@
 // carry the running maximum: nothing is rescaled in TMEM.  V's scales go into P (as their ratio to the tile's largest).
 //
 // Work: the tiles of 128 tokens of all (sequence, token chunk, KV head) segments in one line, cut into equal runs, one per CTA
-// (one CTA per SM), whatever the lengths; a segment's start counts as two or three tiles, as its queries and its output take about
+// (one CTA per SM), whatever the lengths; a segment's start counts as one or two tiles, as its queries and its output take about
 // that long.  A segment inside one run is finished there; of a cut one each CTA writes its partial (at most two per CTA), and
 // paged_combine_kernel merges them in order, so results do not depend on timing.
 // Warps: 0 and 2 TMA of the codes (K and V, each its own ring of 32 KB units), 0 also the tiles' scales; 1 the products S; 3 the
@@ -31,7 +31,7 @@
 // warps that stay converged and elect the issuing lane do not bound it.  The roles together have to stay in the instruction
 // cache: waits and loops are written for few instructions (106 KB of code took a third longer than 72 KB).
 // Measured (24 query heads, 4 KV heads, pages of 64): 64 sequences of 16384 tokens 326 us, all that the measured copy rate allows
-// (331 us); 64 of 1 to 16384 tokens 51 us (floor 36); one of 777 tokens 9.6 us.  24 rows (four tokens): 3550 cycles a tile, bound by
+// (331 us); 64 of 1 to 16384 tokens 48 us (floor 36); one of 777 tokens 9.6 us.  24 rows (four tokens): 3550 cycles a tile, bound by
 // the softmax warps' way through a tile: 32 sequences of 16384 tokens 225 us (floor 166), with pages of 16 tokens 247 (eight copies
 // per tile and half).  There 80 registers per thread are all there are, and what does not fit costs: 244 us with 28 bytes spilled.
 // (Taking a tile's scores before the weights of the one before, so that nobody waits for the maxima, made it 267 us.)
@@ -75,9 +75,9 @@ struct PagedCfg {
   static constexpr int Threads = (4 + 4 * Groups + 8) * 32;
   static constexpr int KUnits = 3, VUnits = RP == 8 ? 3 : 2;   // ring units that fit beside Q and P
   static constexpr int Units = KUnits + VUnits;
-  // what a segment's start counts, in tiles.  64 sequences of 1 to 16384 tokens, 8 rows: 67, 59 and 59 us with 1, 2 and 3, 32 of 3000 to
-  // 6100: 71, 70 and 72; 32 of 4 to 32768 tokens, 24 rows: 143, 122 and 117 us
-  static constexpr int Start = RP == 8 ? 2 : 3;
+  // what a segment's start counts, in tiles.  64 sequences of 1 to 16384 tokens, 8 rows: 60, 48 and 51 us with 0, 1 and 2, 64 of 700: 56 to
+  // 57 with each; 32 of 4 to 32768 tokens, 24 rows: 95, 88 and 90 us with 1, 2 and 3, 64 of 100 to 3000, 16 rows: 59, 57 and 58
+  static constexpr int Start = RP == 8 ? 1 : 2;
   static constexpr int TmemCols = 6 * NP <= 256 ? 256 : 512;   // S[2], O[2][2 halves]
   static constexpr int QBytes = NP * kPG_D, PBytes = NP * kPA_Tile;
   static constexpr int Smem = Units * kPA_Unit + 2 * QBytes + 2 * PBytes + 5120 + 1024;
