@@ -48,20 +48,25 @@ __device__ __forceinline__ void from_e4m3x4(uint32_t u, float (&x)[4]) {
   x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
 }
 
-// One CTA per (sequence, page it writes, KV head), keys and values; thread i takes 16 elements (chunk i % 16) of rows i / 16,
-// i / 16 + 16, ...: all of its loads are in flight before the block's maxima are known, so the new tokens are read once.  Bound by HBM
-// (2 bytes in and 1 out per element) for prompts, where the way to the first load (cumulative lengths, slot and length, page) is what a
-// CTA mostly waits for: with keys and values in CTAs of their own 32143 tokens took 47 us, now 33 (0.92 of HBM) in pages of 64, where
-// three CTAs share an SM (two: 46 us), and 38, 38 and 44 in pages of 16, 32 and 128 (bounding their registers too made these slower).
-// A decode step is bound by latency: 5 us.
-template <typename T, int L>
-__global__ void __launch_bounds__(256, L == 64 ? 3 : 1) paged_append_kernel(AppendArgs a) {
-  constexpr int PASS = L / 16;
-  __shared__ float s_max[2][8];
+// One CTA per (sequence, page it writes, NH KV heads), keys and values; thread i takes 16 elements (chunk i % 16) of rows i / 16,
+// i / 16 + threads / 16, ...: all of its loads are in flight before the block's maxima are known, so the new tokens are read once.  Bound
+// by HBM (2 bytes in and 1 out per element) for prompts, where the way to the first load (cumulative lengths, slot and length, page) is
+// what a CTA mostly waits for, so a CTA takes 64 KB where it can: with keys and values in CTAs of their own 32143 tokens of 4 heads took
+// 47 us in pages of 64, now 34 (0.9 of HBM; with two CTAs per SM instead of three 46); pages of 16 and 32 with a head per CTA 44 and 43,
+// with four and two 38 and 36; pages of 128 with 256 threads, which fill an SM's registers, 44, with 512 42.
+// A decode step is bound by latency, 4 to 9 us, and takes a head per CTA (16 tokens: 3.8 us instead of 5.5).
+template <int L>
+struct AppendCfg {
+  static constexpr int Threads = L == 128 ? 512 : 256, Ctas = L == 128 ? 1 : 3;
+};
+template <typename T, int L, int NH>
+__global__ void __launch_bounds__(AppendCfg<L>::Threads, AppendCfg<L>::Ctas) paged_append_kernel(AppendArgs a) {
+  constexpr int NT = AppendCfg<L>::Threads, RP = NT / 16, PASS = L / RP;     // rows per pass, heads, passes per head
+  __shared__ float s_max[2][NH][NT / 32], s_told[2][NH];
   __shared__ int s_dup;
   let_next_start();
   wait_for_stream();
-  const int tid = threadIdx.x, g = blockIdx.y;
+  const int tid = threadIdx.x, g0 = blockIdx.y * NH;
   int b, ord, tok0 = 0, n = a.t;
   if (a.cu) {
     // sequence b owns the items cu[b] / L + 2 b ...: at least one more than the pages that its tokens can touch.  Every warp cuts
@@ -88,7 +93,7 @@ __global__ void __launch_bounds__(256, L == 64 ? 3 : 1) paged_append_kernel(Appe
   if (a.slots) {   // a slot named twice: the first sequence writes
     if (tid == 0) s_dup = 0;
     __syncthreads();
-    for (int i = tid; i < b; i += 256)
+    for (int i = tid; i < b; i += NT)
       if (a.slots[i] == slot) s_dup = 1;
     __syncthreads();
     if (s_dup) return;
@@ -102,99 +107,111 @@ __global__ void __launch_bounds__(256, L == 64 ? 3 : 1) paged_append_kernel(Appe
   const int lo = max(start, pi * L), had = lo - pi * L, rows = min(len, (pi + 1) * L) - lo;
   const int skip = n - (end - lo);   // this page's first new token among the sequence's
   if (rows <= 0) return;
-  const size_t pg = (size_t)page * a.p.heads + g;
-  const int chunk = (tid & 15) * 16, r0 = tid >> 4;
-  uint4 w[2][PASS][2];
-  float told[2];
-#pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const T* src = static_cast<const T*>(a.x[kv]) + g * a.sh[kv] + chunk +
-                   (a.cu ? (long long)(tok0 + skip) * a.st[kv] : b * a.sb[kv] + (long long)skip * a.st[kv]);
-    told[kv] = had ? (kv ? a.p.vs : a.p.ks)[pg] : 0.f;
-#pragma unroll
-    for (int i = 0; i < PASS; ++i) {
-      const int r = r0 + 16 * i;
-      w[kv][i][0] = w[kv][i][1] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows) {
-        const uint4* s = reinterpret_cast<const uint4*>(src + r * a.st[kv]);
-        w[kv][i][0] = __ldg(s);
-        w[kv][i][1] = __ldg(s + 1);
-      }
-    }
+  const size_t pg = (size_t)page * a.p.heads + g0;
+  const int chunk = (tid & 15) * 16, r0 = tid >> 4, heads = NH == 1 ? 1 : min(NH, a.p.heads - g0);
+  // the scales so far, in registers for one head (from shared memory a page of 64 took 40 us instead of 34 of the prompts above)
+  float told1[2] = {0.f, 0.f};
+  if (NH > 1 && tid < 2 * NH) {
+    const int kv = tid / NH, h = tid % NH;
+    s_told[kv][h] = had && h < heads ? (kv ? a.p.vs : a.p.ks)[pg + h] : 0.f;
   }
-  float amax[2];
+  uint4 w[2][NH][PASS][2];
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
-    // the largest of the 16-bit patterns without their signs, which are in the order of the values; non-finite ones are left out in a
-    // second look
-    uint32_t m2 = 0u;
+    const T* src = static_cast<const T*>(a.x[kv]) + g0 * a.sh[kv] + chunk +
+                   (a.cu ? (long long)(tok0 + skip) * a.st[kv] : b * a.sb[kv] + (long long)skip * a.st[kv]);
+    if (NH == 1) told1[kv] = had ? (kv ? a.p.vs : a.p.ks)[pg] : 0.f;
 #pragma unroll
-    for (int i = 0; i < PASS; ++i) {
-      const uint32_t* u = reinterpret_cast<const uint32_t*>(w[kv][i]);
-#pragma unroll
-      for (int c = 0; c < 8; ++c) m2 = __vmaxu2(m2, u[c] & 0x7fff7fffu);
-    }
-    uint32_t top = max(m2 & 0xffffu, m2 >> 16);
-    if (top >= inf16<T>()) {
-      top = 0u;
+    for (int h = 0; h < NH; ++h)
 #pragma unroll
       for (int i = 0; i < PASS; ++i) {
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(w[kv][i]);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint32_t x = u[c] & 0x7fffu, y = (u[c] >> 16) & 0x7fffu;
-          top = max(top, max(x < inf16<T>() ? x : 0u, y < inf16<T>() ? y : 0u));
+        const int r = r0 + RP * i;
+        w[kv][h][i][0] = w[kv][h][i][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows && h < heads) {
+          const uint4* s = reinterpret_cast<const uint4*>(src + h * a.sh[kv] + r * a.st[kv]);
+          w[kv][h][i][0] = __ldg(s);
+          w[kv][h][i][1] = __ldg(s + 1);
         }
       }
-    }
-    const uint16_t t16 = (uint16_t)top;
-    float m = (float)*reinterpret_cast<const T*>(&t16);
-    m = warp_max(m);
-    if ((tid & 31) == 0) s_max[kv][tid >> 5] = m;
   }
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      // the largest of the 16-bit patterns without their signs, which are in the order of the values; non-finite ones are left out in
+      // a second look
+      uint32_t m2 = 0u;
+#pragma unroll
+      for (int i = 0; i < PASS; ++i) {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(w[kv][h][i]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) m2 = __vmaxu2(m2, u[c] & 0x7fff7fffu);
+      }
+      uint32_t top = max(m2 & 0xffffu, m2 >> 16);
+      if (top >= inf16<T>()) {
+        top = 0u;
+#pragma unroll
+        for (int i = 0; i < PASS; ++i) {
+          const uint32_t* u = reinterpret_cast<const uint32_t*>(w[kv][h][i]);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t x = u[c] & 0x7fffu, y = (u[c] >> 16) & 0x7fffu;
+            top = max(top, max(x < inf16<T>() ? x : 0u, y < inf16<T>() ? y : 0u));
+          }
+        }
+      }
+      const uint16_t t16 = (uint16_t)top;
+      const float m = warp_max((float)*reinterpret_cast<const T*>(&t16));
+      if ((tid & 31) == 0) s_max[kv][h][tid >> 5] = m;
+    }
   __syncthreads();
+  auto maximum = [&](int kv, int h) {
+    float m = s_max[kv][h][0];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    amax[kv] = s_max[kv][0];
+    for (int i = 1; i < NT / 32; ++i) m = fmaxf(m, s_max[kv][h][i]);
+    return m;
+  };
+  const float amax1[2] = {NH == 1 ? maximum(0, 0) : 0.f, NH == 1 ? maximum(1, 0) : 0.f};
 #pragma unroll
-    for (int i = 1; i < 8; ++i) amax[kv] = fmaxf(amax[kv], s_max[kv][i]);
-  }
+  for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    uint8_t* dst = (kv ? a.p.v : a.p.k) + pg * L * kPG_D + chunk;
-    const float s = had ? fmaxf(scale_for(amax[kv]), told[kv]) : scale_for(amax[kv]);
-    const float inv = pow2_inverse(s);
+    for (int h = 0; h < NH; ++h) {
+      if (h >= heads) break;
+      const float amax = NH == 1 ? amax1[kv] : maximum(kv, h), told = NH == 1 ? told1[kv] : s_told[kv][h];
+      uint8_t* dst = (kv ? a.p.v : a.p.k) + (pg + h) * L * kPG_D + chunk;
+      const float s = had ? fmaxf(scale_for(amax), told) : scale_for(amax);
+      const float inv = pow2_inverse(s);
 #pragma unroll
-    for (int i = 0; i < PASS; ++i) {
-      const int r = r0 + 16 * i;
-      if (r < rows) {
-        const T* e = reinterpret_cast<const T*>(w[kv][i]);
-        uint32_t c[4];
+      for (int i = 0; i < PASS; ++i) {
+        const int r = r0 + RP * i;
+        if (r < rows) {
+          const T* e = reinterpret_cast<const T*>(w[kv][h][i]);
+          uint32_t c[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          c[q] = e4m3x4((float)e[4 * q] * inv, (float)e[4 * q + 1] * inv, (float)e[4 * q + 2] * inv, (float)e[4 * q + 3] * inv);
-        *reinterpret_cast<uint4*>(dst + (size_t)(had + r) * kPG_D) = make_uint4(c[0], c[1], c[2], c[3]);
-      }
-    }
-    if (had && s > told[kv]) {   // the page's earlier tokens on the grown scale
-      const float ratio = told[kv] * inv;
-#pragma unroll 1
-      for (int r = r0; r < had; r += 16) {
-        uint4* at = reinterpret_cast<uint4*>(dst + (size_t)r * kPG_D);
-        const uint4 o = *at;
-        const uint32_t u[4] = {o.x, o.y, o.z, o.w};
-        uint32_t c[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float x[4];
-          from_e4m3x4(u[q], x);
-          c[q] = e4m3x4(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio);
+          for (int q = 0; q < 4; ++q)
+            c[q] = e4m3x4((float)e[4 * q] * inv, (float)e[4 * q + 1] * inv, (float)e[4 * q + 2] * inv, (float)e[4 * q + 3] * inv);
+          *reinterpret_cast<uint4*>(dst + (size_t)(had + r) * kPG_D) = make_uint4(c[0], c[1], c[2], c[3]);
         }
-        *at = make_uint4(c[0], c[1], c[2], c[3]);
       }
+      if (had && s > told) {   // the page's earlier tokens on the grown scale
+        const float ratio = told * inv;
+#pragma unroll 1
+        for (int r = r0; r < had; r += RP) {
+          uint4* at = reinterpret_cast<uint4*>(dst + (size_t)r * kPG_D);
+          const uint4 o = *at;
+          const uint32_t u[4] = {o.x, o.y, o.z, o.w};
+          uint32_t c[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float x[4];
+            from_e4m3x4(u[q], x);
+            c[q] = e4m3x4(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio);
+          }
+          *at = make_uint4(c[0], c[1], c[2], c[3]);
+        }
+      }
+      if (tid == 0) (kv ? a.p.vs : a.p.ks)[pg + h] = s;
     }
-    if (tid == 0) (kv ? a.p.vs : a.p.ks)[pg] = s;
-  }
 }
 
 // ------------------------------------------------------------------------------------------------ pages
@@ -349,11 +366,18 @@ int bf_paged_append(const bf_page_pool* pool, int layer, const void* k, long lon
   a.cu = cu;
   a.B = B;
   a.t = t;
-  const dim3 grid((unsigned)items, a.p.heads);
+  const bool many = ((long long)(cu ? t : (long long)B * t) / L + B) * a.p.heads > 3LL * st.sm_count;
   auto go = [&](auto type) {
     using E = decltype(type);
-    return launch_early(L == 16 ? paged_append_kernel<E, 16> : L == 32 ? paged_append_kernel<E, 32>
-                        : L == 64 ? paged_append_kernel<E, 64> : paged_append_kernel<E, 128>, grid, 256, 0, stream, a);
+    auto with = [&](auto kernel, int threads, int heads) {
+      return launch_early(kernel, dim3((unsigned)items, (a.p.heads + heads - 1) / heads), threads, 0, stream, a);
+    };
+    if (L == 16 && many) return with(paged_append_kernel<E, 16, 4>, 256, 4);
+    if (L == 16) return with(paged_append_kernel<E, 16, 1>, 256, 1);
+    if (L == 32 && many) return with(paged_append_kernel<E, 32, 2>, 256, 2);
+    if (L == 32) return with(paged_append_kernel<E, 32, 1>, 256, 1);
+    if (L == 64) return with(paged_append_kernel<E, 64, 1>, 256, 1);
+    return with(paged_append_kernel<E, 128, 1>, AppendCfg<128>::Threads, 1);
   };
   return dtype == BF_BF16 ? go(__nv_bfloat16()) : go(__half());
 }

@@ -247,6 +247,23 @@ def test_append_many_sequences(n, page):
     _check_append(c, before, slots, news, k, v)
 
 
+@pytest.mark.parametrize("page,G", [(16, 5), (16, 4), (32, 3), (32, 2), (128, 3)])
+def test_append_long_prompts_of_several_heads(page, G):
+    """So many pages that a CTA takes several heads of a page, whose number need not go into theirs; pages half full and values of
+    which a page's scale grows among them."""
+    lens, had = [page * 70 + 5, 1, page * 55 - 3, 0, page * 30], [3, page - 1, page // 2, 7, 0]
+    c = _cache(1, 200, G, 5, page=page, max_len=page * 80)
+    c.reserve(range(5), had)
+    k = _rand(1, 1, 1, D, seed=17).expand(5, page, G, D)
+    c.append(0, k.cuda(), k.cuda())
+    c.reserve(range(5), lens)
+    T = sum(lens)
+    k, v = (_rand(T, G, D, seed=18 + i) * torch.logspace(-3, 3, G)[:, None].to(torch.bfloat16) for i in range(2))
+    before = _host(c)
+    c.append(0, k.cuda(), v.cuda(), cu_seqlens=torch.tensor([0] + lens).cumsum(0).cuda())
+    _check_append(c, before, range(5), lens, k, v)
+
+
 def test_calls_without_sequences_or_tokens():
     c = _cache(1, 4, 2, 2, page=16, max_len=32)
     c.reserve([0], 3)
