@@ -482,6 +482,49 @@ def test_serving_steps_captured_and_replayed():
         assert _same(x, y)
 
 
+def test_calls_in_a_row_without_waiting():
+    """Kernels start under the end of the one before: what they enqueue back to back is what they do one by one."""
+    from heimdall_b200 import prompt_attention
+    dev = _dev()
+    g = torch.Generator().manual_seed(3)
+    G, H, n = 2, 12, 12
+    ks = [torch.randn(2, 1, G, D, generator=g).to(torch.bfloat16).to(dev) for _ in range(n)]
+    qs = [torch.randn(2, 1, H, D, generator=g).to(torch.bfloat16).to(dev) for _ in range(n)]
+    x = torch.randn(300, G, D, generator=g).to(torch.bfloat16).to(dev)
+    cu = torch.tensor([0, 300], device=dev, dtype=torch.int32)
+
+    def steps(wait):
+        c = _cache(1, 120, G, 4, page=16, max_len=700)
+        c.reserve([0, 1], 300)
+        out, q = [], torch.empty_like(qs[0])
+        for i in range(n):
+            for b in (0, 1):
+                if i == 0:
+                    c.append(0, x, x, torch.tensor([b], device=dev), cu)
+                    wait()
+            c.reserve([0, 1], 1)
+            wait()
+            q.copy_(qs[i])
+            c.append(0, ks[i], ks[i])
+            wait()
+            out.append(c.attend(0, q)[0])
+            wait()
+            c.fork([0], [2]), wait()
+            out.append(c.attend(0, q[:1], torch.tensor([2], device=dev))[0])
+            wait()
+            out.append(prompt_attention(torch.cat([q[0]] * 40), torch.cat([x] * 2)[:40], torch.cat([x] * 2)[:40], cu.clamp(max=40))[0])
+            c.free([2]), wait()
+            if i % 3 == 2:
+                c.truncate([1], c.length(1) - 2), wait()
+                c.compact(), wait()
+        torch.cuda.synchronize()
+        return out, _host(c)
+    a, pa = steps(torch.cuda.synchronize)
+    for _ in range(3):
+        b, pb = steps(lambda: None)
+        assert all(torch.equal(u, w) for u, w in zip(a, b)) and all(_same(u, w) for u, w in zip(pa, pb))
+
+
 def test_two_captured_graphs_side_by_side():
     dev = _dev()
     cs = [_cache(1, 200, 2, 2, page=32) for _ in range(2)]
