@@ -287,9 +287,10 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, with_ls
     queries and nk keys sees its keys j <= i + nk - nq: the queries are the sequence's last tokens.
     Returns o [T,H,D] in q's dtype and lse [H,T] fp32 (None unless ``with_lse``); a query that sees no key and the
     rows of no sequence (before the first, behind the last) have o = 0 and lse = -inf.  ``scale`` (default D^-1/2) must be
-    positive.  Other sequences' values have no part in a sequence's output, whatever they are; a value that is not finite can make
-    NaN of earlier queries of its own sequence in the same block of 128 keys (a weight of 0 times it).  No backward: the
-    kept layers are frozen and their outputs enter training precomputed (motor.py:126-146).
+    positive; at most 2^25 keys and 2^20 sequences.  Other sequences' values have no part in a sequence's output, whatever
+    they are; a value that is not finite can make NaN of earlier queries of its own sequence in the same block of 128 keys
+    (a weight of 0 times it).  No backward: the kept layers are frozen and their outputs enter training precomputed
+    (motor.py:126-146).
     """
     dev = serving_inputs("prompt_attention", q, k, v)
     qs, ks = q.shape, k.shape

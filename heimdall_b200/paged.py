@@ -231,8 +231,10 @@ class PagedKV:
     def append(self, layer: int, k, v, slots=None, cu_seqlens=None) -> None:
         """Write the newest tokens of each sequence, already reserved: k, v [B,t,G,D], or [T,G,D] packed with cu_seqlens
         [B+1].  Sequence b (slot slots[b], an int tensor on the device; None: slot b) gets its n_b tokens at the positions
-        lens - n_b .. lens - 1.  A page's scale covers what was written to it; earlier codes of a page whose scale grows are
-        rounded to the new one.  Infinities are stored as the largest code, NaN as NaN."""
+        lens - n_b .. lens - 1, which are to be its own: tokens from before a fork may lie in pages that it shares.
+        A page's scale covers what was written to it; earlier codes of a page whose scale grows are rounded to the new one.
+        Infinities are stored as the largest code, NaN as NaN.  A slot named twice is written by its first sequence, a
+        number outside the cache's slots by none."""
         dev = serving_inputs("PagedKV.append", self.k_pages, k, v)
         layer, shape, packed = self._layer(layer), k.shape, cu_seqlens is not None
         if shape != v.shape or k.dtype != v.dtype or len(shape) != (3 if packed else 4):
@@ -255,9 +257,10 @@ class PagedKV:
     def attend(self, layer: int, q, slots=None, scale=None, with_lse: bool = False):
         """Attention of each sequence's last t tokens over its pages: q [B,t,H,D] (bf16 or fp16; H a multiple of the KV
         heads) at the positions lens - t .. lens - 1, each seeing the positions up to its own.  Returns o [B,t,H,D] in q's
-        dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf.  What the pages hold
-        behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t tokens.  A token's weight times its V scale is held to
-        2^-26 of (largest weight) * (largest V scale) among the 128 tokens of its tile."""
+        dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf.  What the
+        pages hold behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t
+        tokens.  A token's weight times its V scale is held to 2^-26 of (largest weight) * (largest V scale) among the 128
+        tokens of its tile."""
         dev = serving_inputs("PagedKV.attend", self.k_pages, q)
         layer, shape = self._layer(layer), q.shape
         if len(shape) != 4 or shape[3] != self.dim or shape[2] % self.heads or shape[2] < 1:

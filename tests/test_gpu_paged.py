@@ -525,6 +525,51 @@ def test_calls_in_a_row_without_waiting():
         assert all(torch.equal(u, w) for u, w in zip(a, b)) and all(_same(u, w) for u, w in zip(pa, pb))
 
 
+def test_captured_behind_copies_and_other_streams():
+    """What comes before a call in a graph may be a copy from the host, a memset or work of another stream: it is waited for."""
+    from heimdall_b200 import prompt_attention
+    dev = _dev()
+    c = _cache(1, 40, 2, 2, page=64)
+    c.reserve([0, 1], [300, 65])
+    _fill(c, 20)
+    host = [_rand(2, 1, h, D, seed=21 + h).pin_memory() for h in (2, 8)]
+    k, q = (x.to(dev) for x in host)
+    big, slots = _rand(1 << 24, seed=22).to(dev), torch.tensor([0, 1], device=dev, dtype=torch.int32)
+    cu = torch.tensor([0, 1, 2], device=dev, dtype=torch.int32)
+    side = torch.cuda.Stream()
+
+    def calls():
+        k.copy_(host[0], non_blocking=True)                     # a copy node, then append
+        c.append(0, k, k, slots)
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):                           # something slow on the other stream, which q waits for
+            big.mul_(1.0)
+            q.copy_(host[1], non_blocking=True)
+        slots.zero_()
+        slots[1:].fill_(1)
+        main.wait_stream(side)
+        o = c.attend(0, q, slots)[0]
+        q.copy_(host[1], non_blocking=True)
+        return o, prompt_attention(q.view(2, 8, D), k.view(2, 2, D), k.view(2, 2, D), cu)[0]
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for i in range(5):
+        for j, x in enumerate(host):
+            x.copy_(_rand(*x.shape, seed=30 + 2 * i + j) * 3)
+        k.zero_(), q.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        held = [x.clone() for x in got]
+        want = calls()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(held, want)), i
+
+
 def test_two_captured_graphs_side_by_side():
     dev = _dev()
     cs = [_cache(1, 200, 2, 2, page=32) for _ in range(2)]
