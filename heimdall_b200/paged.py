@@ -158,6 +158,8 @@ class PagedKV:
                                 ptr(self.lens), layers, pages, heads, page, dim, slots, width)
         self._pool_ptr = ctypes.addressof(self._pool)
         self._ws = {}                       # workspace bytes by (B, t, H)
+        self._appended = set()              # layers that the caller's own append has written, for as long as no layer() is out
+        self._progress = None               # what retrieval.teacher has written, from the first layer() on
 
     # -------------------------------------------------------------------------------------------- sequences and pages
     @property
@@ -194,16 +196,22 @@ class PagedKV:
     def free(self, slots) -> None:
         """End the sequences of these slots: their pages return to the pool unless another sequence shares them."""
         self._apply(self.host.free, slots)
+        if self._progress is not None:
+            self._progress.free(slots)
 
     def fork(self, src, dst) -> None:
         """The (empty) slots dst continue the sequences of src: full pages are shared, the tokens of a partly filled last
         page are copied, in every layer."""
         self._apply(self.host.fork, src, dst)
+        if self._progress is not None:
+            self._progress.fork(src, dst)
 
     def truncate(self, slots, lens) -> None:
         """Shorten the sequences of these slots to lens tokens (rejected drafts); a shared page that becomes partly filled
         is copied.  The scale of the page that is cut stays as it is."""
         self._apply(self.host.truncate, slots, lens)
+        if self._progress is not None:
+            self._progress.truncate(slots, lens)
 
     def compact(self) -> int:
         """Move the live pages at or above their number into the holes below it (both in ascending order), so that the
@@ -235,6 +243,13 @@ class PagedKV:
         A page's scale covers what was written to it; earlier codes of a page whose scale grows are rounded to the new one.
         Infinities are stored as the largest code, NaN as NaN.  A slot named twice is written by its first sequence, a
         number outside the cache's slots by none."""
+        B = self._append(layer, k, v, slots, cu_seqlens)
+        if self._progress is None:
+            self._appended.add(layer)
+        else:
+            self._progress.appended(int(layer), slots, B)
+
+    def _append(self, layer: int, k, v, slots=None, cu_seqlens=None) -> int:
         dev = serving_inputs("PagedKV.append", self.k_pages, k, v)
         layer, shape, packed = self._layer(layer), k.shape, cu_seqlens is not None
         if shape != v.shape or k.dtype != v.dtype or len(shape) != (3 if packed else 4):
@@ -253,6 +268,7 @@ class PagedKV:
                 ks, vs = [0] + ks, [0] + vs
             _lib.call("bf_paged_append", self._pool_ptr, layer, kp, *ks, vp, *vs, ptr(ids), ptr(cu), B, shape[-3], kernel_dtype(k),
                       stream_handle())
+        return B
 
     def attend(self, layer: int, q, slots=None, scale=None, with_lse: bool = False):
         """Attention of each sequence's last t tokens over its pages: q [B,t,H,D] (bf16 or fp16; H a multiple of the KV
@@ -283,34 +299,93 @@ class PagedKV:
         return o, lse
 
     def layer(self, layer: int) -> "PagedLayer":
-        """This cache as one kept layer's ``cache`` argument of ``retrieval.teacher`` (slots 0 .. B-1 in step)."""
+        """This cache as one kept layer's ``cache`` argument of ``retrieval.teacher`` (slots 0 .. B-1).  How far the layer
+        is belongs to the cache: fetched once or for every call, a layer goes on where it was."""
         return PagedLayer(self, self._layer(layer))
 
 
+class _Progress:
+    """What ``retrieval.teacher`` has written: the tokens of each slot in each layer, -1 where the host cannot tell, because the caller's
+    own ``append`` may have written a sequence's newest tokens there."""
+
+    def __init__(self, cache: PagedKV):
+        self.host = cache.host
+        self.n = np.zeros((cache.layers, self.host.slots), np.int64)
+        self.room = np.zeros(self.host.slots, np.int64)     # a slot's length when teacher last made room in it
+        for layer in cache._appended:
+            self.n[layer, self.host.lens > 0] = -1
+
+    def free(self, slots) -> None:
+        s = self.host._whole(slots)
+        self.n[:, s] = self.room[s] = 0
+
+    def fork(self, src, dst) -> None:
+        a, b = self.host._whole(src), self.host._whole(dst)
+        self.n[:, b], self.room[b] = self.n[:, a], self.room[a]
+
+    def truncate(self, slots, lens) -> None:
+        s = self.host._whole(slots)
+        m = self.host._whole(lens, s)
+        self.n[:, s], self.room[s] = np.minimum(self.n[:, s], m), np.minimum(self.room[s], m)
+        self.n[:, s[m == 0]] = 0
+
+    def appended(self, layer: int, slots, B: int) -> None:
+        """The caller's own append of B sequences to a layer: what was reserved by the caller, and not by teacher, may be written now.  (Which
+        slots it named is read back from the device where that matters, but not in a capture.)"""
+        n, lens = self.n[layer], self.host.lens
+        may = (n >= 0) & (n < lens) & (lens != self.room)
+        if slots is None:
+            may[B:] = False
+        elif may.any() and not (slots.is_cuda and torch.cuda.is_current_stream_capturing()):
+            named = np.asarray(slots.tolist(), np.int64)
+            may &= np.isin(np.arange(n.size), named)
+        n[may] = -1
+
+
 class PagedLayer:
-    """One layer of a ``PagedKV`` as the cache of ``retrieval.teacher``: a batch of B sequences in the slots 0 .. B-1, all
-    layers of the cache called in the same order every step.  The first layer that needs room reserves it."""
+    """One layer of a ``PagedKV`` as the cache of ``retrieval.teacher``: every call brings the next t tokens of each of the
+    sequences in the slots 0 .. B-1.  The first layer that needs room reserves it (or the caller has, for exactly these tokens), and
+    every layer takes the same tokens.  ``free``, ``truncate`` and ``fork`` of the cache are followed.  A sequence whose tokens were
+    written to the layer with ``append`` is not gone on with: ``attend`` is the call for those.  Replays of a captured call are
+    not seen by the host; what was captured goes on by replays, or anew after ``free``."""
 
     def __init__(self, cache: PagedKV, layer: int):
-        self.cache, self.index, self.n = cache, layer, 0
+        self.cache, self.index = cache, layer
+        if cache._progress is None:
+            cache._progress = _Progress(cache)
+
+    @property
+    def n(self) -> int:
+        """Tokens of the longest sequence that this layer holds.  Setting it says that the layer holds n tokens of each sequence."""
+        return max(int(self.cache._progress.n[self.index].max()), 0)
+
+    @n.setter
+    def n(self, tokens: int) -> None:
+        p = self.cache._progress
+        p.n[self.index, p.host.lens > 0] = tokens
 
     def teacher(self, qr, kr, v, retrieval=None):
         c, (B, H, t, D) = self.cache, qr.shape
-        n = self.n + t
+        if B > c.host.slots:
+            raise ValueError("more sequences than the cache has slots")
+        p, lens = c._progress, c.host.lens[:B]
+        had = p.n[self.index, :B].copy()
+        n = int(had.max(initial=0)) + t
         if retrieval is not None and (t == 1 or retrieval.get("prefill")) and \
                 n - retrieval["sinks"] - retrieval["window"] >= retrieval["k"] * retrieval["block"]:
             raise NotImplementedError("heimdall_b200 retrieval: block selection over 8-bit pages is not built")
-        if B > c.host.slots:
-            raise ValueError("more sequences than the cache has slots")
-        if (c.host.lens[:B] == self.n).all():
+        if (had < 0).any():
+            raise ValueError("a sequence's tokens in this layer were written with append: attend goes on from there, not teacher")
+        if (lens == had).all():
             c.reserve(np.arange(B), t)
-        if not (c.host.lens[:B] == n).all():
+            p.room[:B] = lens
+        if not (lens == had + t).all():
             raise ValueError("the layers of a paged cache must take the same tokens in step")
         dt = kr.dtype if kr.dtype == torch.float16 else torch.bfloat16
         q, k, v = qr.transpose(1, 2).to(dt), kr.transpose(1, 2).to(dt), v.to(dt)
-        c.append(self.index, k, v)
-        first, self.n = self.n == 0, n
-        if not first:
+        c._append(self.index, k, v)
+        p.n[self.index, :B] = lens
+        if had.any():
             return c.attend(self.index, q)[0].to(qr.dtype)
         # a whole prompt: attention over the keys and values as they are, not over their codes
         cu = torch.arange(B + 1, device=qr.device, dtype=torch.int32) * t

@@ -223,3 +223,45 @@ def test_c_entries_check_their_arguments_before_a_launch():
     assert pages(release=[3]) == 1 and pages(release=[-1]) == 1 and pages(fork=[0, 3, 1, 0, 1]) == 1 and pages(fork=[0, 1, 300, 0, 1]) == 1
     assert pages(fork=[0, 1, 5, 8, 1]) == 1 and pages(fork=[0, 1, 5, 1, 1]) == 1 and pages(move=[8, 1]) == 1 and pages(move=[5, 1, 4, 0]) == 1
     assert pages(set_=[15, 0]) == 1 and pages(set_=[-1, 0]) == 1
+
+
+def test_a_layers_progress_follows_the_page_table():
+    """What teacher has written of each slot, as the sequences are forked, cut and ended, and where the host cannot tell."""
+    from heimdall_b200.paged import _Progress
+
+    class Cache:
+        layers, host, _appended = 3, PageTable(40, 4, 16, 6), {1}
+    host = Cache.host
+    host.reserve([3], 5)                                    # written directly in layer 1 before the first layer()
+    p = _Progress(Cache)
+    assert p.n.tolist() == [[0] * 4, [0, 0, 0, -1], [0] * 4]
+
+    def teacher(layer, B, t):
+        if (host.lens[:B] == p.n[layer, :B]).all():
+            host.reserve(range(B), t)
+            p.room[:B] = host.lens[:B]
+        assert (host.lens[:B] == p.n[layer, :B] + t).all()
+        p.n[layer, :B] = host.lens[:B]
+    for layer in (0, 1, 2):
+        teacher(layer, 2, 20)
+    host.truncate([0, 1], [18, 0])
+    p.truncate([0, 1], [18, 0])
+    assert p.n[:, :2].tolist() == [[18, 0]] * 3
+    host.fork([0, 3], [1, 2])
+    p.fork([0, 3], [1, 2])
+    assert p.n.tolist() == [[18, 18, 0, 0], [18, 18, -1, -1], [18, 18, 0, 0]]
+    teacher(0, 2, 1)
+    p.appended(1, torch.tensor([2, 3]), 2)                  # teacher's own room is not in doubt
+    p.appended(1, None, 4)
+    assert p.n[1].tolist() == [18, 18, -1, -1]
+    teacher(1, 2, 1), teacher(2, 2, 1)
+    host.reserve([0, 1], 2)                                 # the caller's is
+    p.appended(0, torch.tensor([1, 9, -1]), 3)
+    assert p.n[0].tolist() == [19, -1, 0, 0]
+    p.appended(2, None, 1)
+    assert p.n[2].tolist() == [-1, 19, 0, 0]
+    host.truncate([1], 0)
+    p.truncate([1], 0)
+    host.free([0, 3])
+    p.free([0, 3])
+    assert p.n[:, [0, 1, 3]].tolist() == [[0] * 3] * 3
