@@ -29,6 +29,7 @@ from .functional import (heads_16bit, int32_on, kernel_dtype, on_device, prompt_
 from .structs import BfPagePool, BfPageTable
 
 PAGE_SIZES = (16, 32, 64, 128)
+MAX_GROUP = 24                  # query heads per KV head of attend
 
 
 _REASONS = {1: "a slot is outside [0, {slots})", 2: "a slot is named twice", 3: "a number of tokens is negative",
@@ -282,8 +283,8 @@ class PagedKV:
         if len(shape) != 4 or shape[3] != self.dim or shape[2] % self.heads or shape[2] < 1:
             raise ValueError(f"attend takes q [B,t,H,{self.dim}] with H a multiple of {self.heads}")
         B, t, H, D = shape
-        if H // self.heads > 24:
-            raise NotImplementedError("attend takes at most 24 query heads per KV head")
+        if H // self.heads > MAX_GROUP:
+            raise NotImplementedError(f"attend takes at most {MAX_GROUP} query heads per KV head")
         scale = score_scale(scale, D)
         with on_device(dev):
             ids = self._ids(slots, B)
@@ -365,7 +366,14 @@ class PagedLayer:
         p.n[self.index, p.host.lens > 0] = tokens
 
     def teacher(self, qr, kr, v, retrieval=None):
-        c, (B, H, t, D) = self.cache, qr.shape
+        c = self.cache
+        # what the calls below would refuse, before room is given out
+        serving_inputs("retrieval.teacher over pages", c.k_pages, qr, kr, v)
+        if qr.dim() != 4 or v.shape != (qr.shape[0], qr.shape[2], c.heads, c.dim) or \
+                kr.shape != (qr.shape[0], c.heads, qr.shape[2], c.dim) or qr.shape[3] != c.dim or qr.shape[1] % c.heads or qr.shape[1] < 1:
+            raise ValueError(f"teacher over pages takes qr [B,H,t,{c.dim}], kr [B,{c.heads},t,{c.dim}] and v [B,t,{c.heads},{c.dim}] "
+                             f"with H a multiple of {c.heads}")
+        B, H, t, D = qr.shape
         if B > c.host.slots:
             raise ValueError("more sequences than the cache has slots")
         p, lens = c._progress, c.host.lens[:B]
@@ -374,18 +382,31 @@ class PagedLayer:
         if retrieval is not None and (t == 1 or retrieval.get("prefill")) and \
                 n - retrieval["sinks"] - retrieval["window"] >= retrieval["k"] * retrieval["block"]:
             raise NotImplementedError("heimdall_b200 retrieval: block selection over 8-bit pages is not built")
+        if had.any() and H // c.heads > MAX_GROUP:
+            raise NotImplementedError(f"attend takes at most {MAX_GROUP} query heads per KV head")
         if (had < 0).any():
             raise ValueError("a sequence's tokens in this layer were written with append: attend goes on from there, not teacher")
-        if (lens == had).all():
+        make_room = bool((lens == had).all())
+        if not make_room and not (lens == had + t).all():
+            raise ValueError("the layers of a paged cache must take the same tokens in step")
+        if make_room:
             c.reserve(np.arange(B), t)
             p.room[:B] = lens
-        if not (lens == had + t).all():
-            raise ValueError("the layers of a paged cache must take the same tokens in step")
+        try:
+            o = self._attend(qr, kr, v, had.any())
+        except BaseException:
+            if make_room:                 # what only a kernel's entry refuses: the room goes back
+                c.truncate(np.arange(B), had)
+            raise
+        p.n[self.index, :B] = lens
+        return o
+
+    def _attend(self, qr, kr, v, later: bool):
+        c, (B, H, t, D) = self.cache, qr.shape
         dt = kr.dtype if kr.dtype == torch.float16 else torch.bfloat16
         q, k, v = qr.transpose(1, 2).to(dt), kr.transpose(1, 2).to(dt), v.to(dt)
         c._append(self.index, k, v)
-        p.n[self.index, :B] = lens
-        if had.any():
+        if later:
             return c.attend(self.index, q)[0].to(qr.dtype)
         # a whole prompt: attention over the keys and values as they are, not over their codes
         cu = torch.arange(B + 1, device=qr.device, dtype=torch.int32) * t

@@ -140,3 +140,38 @@ def test_room_for_all_sequences_reserved_at_once():
         assert _same(c, twin), i
         if i:
             assert torch.equal(o, twin.attend(0, qr[:2].transpose(1, 2))[0]), i
+
+
+def test_a_refused_call_leaves_the_cache_as_it_was(monkeypatch):
+    """What a call refuses it refuses before room is given out; what only a kernel's entry refuses is taken back."""
+    import heimdall_b200.paged as paged
+    c = _cache(2)
+    layers = [c.layer(0), c.layer(1)]
+    qr, kr, v = _qkv(2, 20, 0)
+    for x in layers:
+        _teacher(qr, kr, v, x, None)
+    before = _state(c)
+    qr, kr, v = _qkv(2, 3, 1)
+    wide = torch.cat([qr] * 7, 1)                              # 28 query heads per KV head
+    for kind, a in ((NotImplementedError, (qr, kr.clone().requires_grad_(), v)), (NotImplementedError, (qr.clone().requires_grad_(), kr, v)),
+                    (NotImplementedError, (wide, kr, v)), (ValueError, (qr, kr[:, :1], v[:, :, :1])), (ValueError, (qr, kr[:, :, :2], v)),
+                    (ValueError, (qr[:, :7], kr, v)), (ValueError, (qr[..., :128], kr[..., :128], v[..., :128]))):
+        for x in layers:
+            with pytest.raises(kind):
+                _teacher(*a, x, None)
+            assert _same(before, c) and c.length(0) == 20 and x.n == 20 and c.free_pages == 60 - 4
+    real = paged._lib.call
+
+    def failing(name, *a):
+        if name == "bf_paged_append":
+            raise RuntimeError("append")
+        return real(name, *a)
+    with monkeypatch.context() as m:
+        m.setattr(paged._lib, "call", failing)
+        with pytest.raises(RuntimeError, match="append"):
+            _teacher(qr, kr, v, layers[0], None)
+    assert _same(before, c) and c.length(1) == 20 and layers[0].n == 20
+    qr, kr, v = _qkv(2, 5, 2)                                  # another number of tokens than the refused call's
+    for x in layers:
+        _teacher(qr, kr, v, x, None)
+    assert c.lens.tolist() == [25, 25] and layers[1].n == 25
