@@ -159,6 +159,7 @@ class PagedKV:
                                 ptr(self.lens), layers, pages, heads, page, dim, slots, width)
         self._pool_ptr = ctypes.addressof(self._pool)
         self._ws = {}                       # workspace bytes by (B, t, H)
+        self._ended = False                 # a change has reached the host's table and not the device's
         self._appended = set()              # layers that the caller's own append has written, for as long as no layer() is out
         self._progress = None               # what retrieval.teacher has written, from the first layer() on
 
@@ -174,12 +175,15 @@ class PagedKV:
         return int(self.host.lens[slot])
 
     def _apply(self, change, *args) -> None:
-        """The host's change, then the device's.  Not for a capture: a replay would not repeat the host's part."""
+        """The host's change, then the device's.  Not for a capture: a replay would not repeat the host's part.  A change that
+        fails on the device leaves its table behind the host's, so the cache ends there."""
+        self._check()
         with on_device(self.device):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("heimdall_b200: pages are given out on the host: reserve, fork, free, truncate and compact "
                                    "cannot be captured into a CUDA graph")
             todo = change(*args)
+            self._ended = True
             flat, some = [], 0
             for name in ("release", "fork", "move", "set"):
                 x = todo.get(name)
@@ -188,6 +192,12 @@ class PagedKV:
                 some += n
             if some:
                 _lib.call("bf_paged_pages", self._pool_ptr, *flat, stream_handle())
+            self._ended = False
+
+    def _check(self) -> None:
+        if self._ended:
+            raise RuntimeError("heimdall_b200: a change of pages failed on the device, whose table is behind the host's: this "
+                               "cache cannot be used any more")
 
     def reserve(self, slots, n) -> None:
         """Room for n more tokens (one number, or one per slot) of each slot; they belong to the sequences from here on.
@@ -251,6 +261,7 @@ class PagedKV:
             self._progress.appended(int(layer), slots, B)
 
     def _append(self, layer: int, k, v, slots=None, cu_seqlens=None) -> int:
+        self._check()
         dev = serving_inputs("PagedKV.append", self.k_pages, k, v)
         layer, shape, packed = self._layer(layer), k.shape, cu_seqlens is not None
         if shape != v.shape or k.dtype != v.dtype or len(shape) != (3 if packed else 4):
@@ -278,6 +289,7 @@ class PagedKV:
         pages hold behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t
         tokens.  A token's weight times its V scale is held to 2^-26 of (largest weight) * (largest V scale) among the 128
         tokens of its tile."""
+        self._check()
         dev = serving_inputs("PagedKV.attend", self.k_pages, q)
         layer, shape = self._layer(layer), q.shape
         if len(shape) != 4 or shape[3] != self.dim or shape[2] % self.heads or shape[2] < 1:

@@ -622,3 +622,25 @@ def test_teacher_over_pages():
     layers[0].n -= 2
     with pytest.raises(ValueError, match="in step"):
         teacher(qr, kr, v, layers[0])
+
+
+def test_a_change_of_pages_that_fails_on_the_device_ends_the_cache(monkeypatch):
+    """The host's table would be ahead of the device's: no later call goes on from there."""
+    import heimdall_b200.paged as paged
+    c = _cache(1, 8, 2, 3, page=16, max_len=32)
+    c.reserve([0], 20)
+    real = paged._lib.call
+
+    def failing(name, *a):
+        if name == "bf_paged_pages":
+            raise RuntimeError("the launch failed")
+        return real(name, *a)
+    k = _rand(1, 1, 2, D).cuda()
+    with monkeypatch.context() as m:
+        m.setattr(paged._lib, "call", failing)
+        with pytest.raises(RuntimeError, match="the launch failed"):
+            c.fork([0], [1])
+    for call in (lambda: c.reserve([0], 1), lambda: c.free([1]), lambda: c.fork([0], [2]), lambda: c.truncate([0], 3), c.compact,
+                 lambda: c.append(0, k, k), lambda: c.attend(0, k)):
+        with pytest.raises(RuntimeError, match="cannot be used any more"):
+            call()
