@@ -13,7 +13,9 @@
 //   TMEM of each CTA: S/P buffers at columns 0 and 128, O at 256..511.
 // P is rounded to the inputs' type, which moves a weight by half a step of the type at most: as much as the output's own rounding,
 // and it averages over the keys.  Its sum is taken before.  Scores are in the log2 domain; O is rescaled only when a row's
-// maximum grows by more than 2^8.
+// maximum grows by more than 2^8.  In fp16 that leaves 2^7 of the type's range above the weights, so they enter 2^7 times as large:
+// fp16 is exact to half a step of the weight only down to 2^-14, thus down to 2^-21 of the row's reference, and below that to 2^-32
+// of it (without the factor 2^-25: a key of weight 2^-20 beside one of nearly 1 was off by 2^-6 of itself).
 //
 // Work items are (token block, KV head, head pair or head), one cluster of the grid each, those with the most key tiles first.
 // A cluster that has done its own item asks the hardware for one that has not started (cluster launch control) and goes on with
@@ -54,6 +56,9 @@ constexpr int kPR_MaxKeys = 1 << 25, kPR_MaxSeqs = 1 << 20;
 constexpr int kPR_Smem = kPR_Tiles + 640 + 5120 + 8192 + 4 * 2048 + 1024;
 constexpr uint32_t kPR_TmO = 256;
 constexpr float kPR_Rescale = 8.0f;
+// log2 of what P is multiplied by: the largest weight, 2^kPR_Rescale times that, has to stay below fp16's 65504
+template <typename T>
+__device__ __forceinline__ constexpr float prompt_up() { return __is_same(T, __half) ? 7.f : 0.f; }
 
 struct PromptArgs {
   const int32_t *cu_q, *cu_k;
@@ -504,7 +509,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
         // the reference of the tile before (which also says that it has been taken over from there)
         if (tt >= 1 && !mbar_wait_warp_small(mref + (1 - w) * 4 + q4, ((tt - 1) >> 1) & 1, abort_flag, 0x8a)) { alive = false; break; }
         const float prev = j >= 1 ? xch[(1 - w) * 128 + r] : -INFINITY;
-        const bool grown = prev != -INFINITY && mt > prev + kPR_Rescale;
+        // (in fp16 less may be left standing where the scores are so large that their own last bit is a power of two or more)
+        const float leave = prompt_up<T>() > 0.f ? fmaxf(fmaf(fabsf(mt), -0x1p-20f, kPR_Rescale), 0.f) : kPR_Rescale;
+        const bool grown = prev != -INFINITY && mt > prev + leave;
         const float m = prev == -INFINITY || grown ? mt : prev;
         xch[w * 128 + r] = m;
         __syncwarp();
@@ -527,7 +534,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
           }
         }
         // a row that has seen nothing: scores of -inf against 0 give weights of 0, and a NaN stays one
-        const float nm = m == -INFINITY ? 0.f : -m;
+        const float nm = m == -INFINITY ? 0.f : prompt_up<T>() - m;
         float ls[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < kPR_N; c += 32) {
@@ -579,7 +586,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPR_Threads, 1)
       const float inv = l == 0.f ? 0.f : 1.f / l;        // nothing seen: zeros
       const int h = x.h;
       const size_t row = (size_t)x.row0 + r;
-      if (store && a.lse) a.lse[(size_t)h * a.T + row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      if (store && a.lse) a.lse[(size_t)h * a.T + row] = l == 0.f ? -INFINITY : (m - prompt_up<T>() + log2f(l)) * kLn2;
       // 32 columns at a time through shared memory (16-byte chunks, swizzled by the row), so that a store instruction writes whole
       // 64-byte pieces of eight rows instead of 16 bytes of 32
       uint8_t* stage = s_out + (warp - 12) * 2048;

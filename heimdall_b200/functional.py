@@ -289,7 +289,8 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, with_ls
     rows of no sequence (before the first, behind the last) have o = 0 and lse = -inf.  ``scale`` (default D^-1/2) must be
     positive; at most 2^25 keys and 2^20 sequences.  Other sequences' values have no part in a sequence's output, whatever
     they are; a value that is not finite can make NaN of earlier queries of its own sequence in the same block of 128 keys
-    (a weight of 0 times it).  No backward: the kept layers are frozen and their outputs enter training precomputed
+    (a weight of 0 times it).  Scores, maxima, sums and the accumulator are fp32; a weight is rounded to q's dtype for the product with
+    v (half a step of the type; in fp16, where that is more, 2^-32 of the row's largest weight).  No backward: the kept layers are frozen and their outputs enter training precomputed
     (motor.py:126-146).
     """
     dev = serving_inputs("prompt_attention", q, k, v)

@@ -353,7 +353,8 @@ int bf_llama_state_unpack(const float* rows, long long row_stride, const int64_t
  *   q [T,H,D], k, v [Tk,G,D]: dtype BF_BF16 or BF_F16, element strides per token and head given (positive multiples
  *   of 8, a head's D elements contiguous); cu_q, cu_k [n_seq + 1] int32 on the device, ascending: every entry is clamped
  *   into [previous, T] (or Tk); o [T,H,D] contiguous in dtype; lse [H,T] fp32 or NULL.
- * A query that sees no key, and every row of no sequence, gets o = 0 and lse = -inf.
+ * A query that sees no key, and every row of no sequence, gets o = 0 and lse = -inf.  Weights are rounded to dtype for the product with
+ * v (half a step of the type; BF_F16, where that is more: 2^-32 of the row's largest weight), all else is fp32.
  * D = 256, scale > 0, at most 2^25 keys and 2^20 sequences.
  */
 int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void* k, long long k_st, long long k_sh,

@@ -271,3 +271,44 @@ def test_two_streams_and_a_captured_call():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(x, prompt_attention(*a, ca)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("below", [5, 9, 11, 13, 15, 16.5])
+@pytest.mark.parametrize("n", [2, 300, 2500])
+def test_one_heavy_key_beside_light_ones(n, below, dtype):
+    """A key of weight near one whose value is zero: the output is what the others, each of weight e^-below, bring.
+
+    Their weights are rounded to q's type.  In bf16 that is half a step of each, whatever its size.  fp16 has steps of 2^-24 below
+    2^-14, and a weight enters as 2^7 times itself relative to a reference that is at most the row's maximum: off by at most u of itself
+    or by 2^-25 / 2^7 = 2^-32 of the largest weight."""
+    q, k, v = torch.zeros(1, 2, D), torch.zeros(n, 1, D), torch.ones(n, 1, D)
+    q[..., 0], k[:, 0, 0] = 16.0, -below
+    at = n // 3
+    k[at], v[at] = 0.0, 0.0
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    o, lse = _run(q, k, v, [0, 1], [0, n])
+    ro, rl, mag, big = opk.prompt_attention(q, k, v, [0, 1], [0, n])
+    u = U[dtype]
+    top = torch.exp(-rl).T[..., None]                     # the heavy key's weight
+    tol = (2 * u + 2.0 ** -15 * big[..., None] + 2.0 ** -18) * mag + (2.0 ** -32 * top * (n - 1) + 2.0 ** -25 if dtype == torch.float16 else 0.0)
+    off = (o.cpu().double() - ro).abs()
+    assert (off <= tol).all(), (off / ro).max()
+    assert ((lse.cpu().double() - rl).abs() <= 2.0 ** -16 * big.T + 2.0 ** -18 * (1 + rl.abs())).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("e", [0, 12, 16, 20, 24])
+def test_large_scores_that_grow_from_tile_to_tile(e, dtype):
+    """Maxima that rise a little with every tile of keys, at scores from one to 2^24: weights are at most one, so an output is between the
+    smallest and the largest value; rounded weights and their sum, each off by u, and the output's own rounding leave 4 u of that."""
+    n = 900
+    q, k = torch.zeros(n, 2, D), torch.zeros(n, 1, D)
+    q[..., 0] = 2.0 ** (e // 2)
+    k[:, 0, 0] = 2.0 ** (e - e // 2)
+    q[..., 1], k[:, 0, 1] = 1.0, torch.arange(n) // 100 * 4.0
+    v = 1.0 + (torch.arange(n)[:, None, None] % 7).expand(n, 1, D) / 8.0
+    o, lse = _run(q.to(dtype), k.to(dtype), v.to(dtype), [0, n], scale=1.0)
+    o = o.cpu().double()
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+    assert (o >= 1.0 - 4 * U[dtype]).all() and (o <= 1.75 * (1 + 4 * U[dtype])).all()
