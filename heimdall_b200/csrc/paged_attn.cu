@@ -9,7 +9,8 @@
 // tensor core (kind::f8f6f4).  The other operand of each product, which is small, is split into three e4m3 parts of 4
 // significant bits each (x = (x0 + x1 / 16 + x2 / 256) / 2^k, every part scaled into the code's upper range), each part a column of
 // its own:
-//   S^T[token, part x row] = K Q^T    M = 128 tokens, N = 3 RP, K = 256 dims   (a bf16 or fp16 query is exact in three parts)
+//   S^T[token, part x row] = K Q^T    M = 128 tokens, N = 3 RP, K = 256 dims   (a query component is exact in three parts while it is not
+//                                     far below its row's largest, and off by at most 2^-25 of the largest: the parts end there)
 //   O^T[dim, part x row]   = V^T P^T  M = 2 x 128 dims, N = 3 RP, K = 128 tokens (P is off by at most 2^-12 of itself, or
 //                                     2^-26 of the tile's largest weight)
 // with a row = (token of the call, query head of the KV head's group), RP rows at a time.  P is taken relative to its own

@@ -287,7 +287,8 @@ class PagedKV:
         heads) at the positions lens - t .. lens - 1, each seeing the positions up to its own.  Returns o [B,t,H,D] in q's
         dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf.  What the
         pages hold behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t
-        tokens.  A token's weight times its V scale is held to 2^-26 of (largest weight) * (largest V scale) among the 128
+        tokens.  A component of q is held to 2^-25 of the largest of its row and head (exactly, where it is above about 2^-14 of
+        that).  A token's weight times its V scale is held to 2^-26 of (largest weight) * (largest V scale) among the 128
         tokens of its tile."""
         self._check()
         dev = serving_inputs("PagedKV.attend", self.k_pages, q)

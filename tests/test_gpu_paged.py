@@ -644,3 +644,34 @@ def test_a_change_of_pages_that_fails_on_the_device_ends_the_cache(monkeypatch):
                  lambda: c.append(0, k, k), lambda: c.attend(0, k)):
         with pytest.raises(RuntimeError, match="cannot be used any more"):
             call()
+
+
+@pytest.mark.parametrize("t,H", [(1, 2), (4, 6)])
+@pytest.mark.parametrize("dtype,e", [(torch.bfloat16, 8), (torch.bfloat16, 16), (torch.bfloat16, 20), (torch.bfloat16, 30),
+                                     (torch.float16, 8), (torch.float16, 15)])
+def test_attend_query_rows_of_a_wide_range(dtype, e, t, H):
+    """One component of 2^e among others of order one, against keys that are zero there.
+
+    The parts of a query end at 2^-17 of a row scaled to [128, 256): a component is off by at most half of that, 2^-18 / 128 = 2^-25 of
+    the row's largest, a score by that times scale * sum |k|, a weight by twice that relatively, as long as it is small."""
+    c = _cache(1, 20, 1, 1, page=64)
+    c.reserve([0], 700)
+    _fill(c, 23)
+    c.k_pages[0, :, :, :, 37] = 0.0
+    c.k_scale.fill_(2.0 ** -7)
+    q = _rand(1, t, H, D, seed=24, dtype=dtype)
+    q[..., 37] = 2.0 ** e
+    q[:, -1, -1] = _rand(D, seed=25, dtype=dtype)                  # and a row without one
+    o, lse = c.attend(0, q.cuda(), with_lse=True)
+    kc, ks, vc, vs = _host(c)
+    ro, rl, mag, big = opk.attend(kc, ks, vc, vs, c.table[0].tolist(), 700, q[0], None)
+    span = D ** -0.5 * float((kc * ks[..., None, None]).abs().sum(-1).max())
+    lost = 2.0 ** -25 * span * q[0].abs().amax(-1).double()        # [t, H]
+    known = lost < 2.0 ** -4                                       # 2 x is a bound of e^x - 1 and 1 - e^-x well beyond that
+    assert known[-1, -1] and (known.all() or e > 16)
+    assert torch.isfinite(o).all()
+    top = float((vc.abs().amax((2, 3)) * vs).max())
+    tol = (U[dtype] + 2.0 ** -11 + 2.0 ** -12 * big[..., None] + 2 * 2 * lost[..., None]) * mag + 2.0 ** -19 * top
+    assert ((o[0].cpu().double() - ro).abs() <= tol)[known].all()
+    off, tol = (lse[0].cpu().double() - rl).abs(), 2.0 ** -13 * big.T + lost.T + 2.0 ** -16 * (1 + rl.abs())
+    assert (off <= tol)[known.T].all(), (off - tol).max()
