@@ -69,8 +69,9 @@ __global__ void __launch_bounds__(AppendCfg<L>::Threads, AppendCfg<L>::Ctas) pag
   const int tid = threadIdx.x, g0 = blockIdx.y * NH;
   int b, ord, tok0 = 0, n = a.t;
   if (a.cu) {
-    // sequence b owns the items cu[b] / L + 2 b ...: at least one more than the pages that its tokens can touch.  Every warp cuts
-    // the range that b is in into 32 pieces of `step` sequences at a time
+    // sequence b owns the items cu[b] / L + 2 b ...: at least as many as the pages that its tokens can touch.  Every warp cuts
+    // the range that b is in into 32 pieces of `step` sequences at a time, which takes cu to ascend: where it does not, items of a
+    // sequence go to another, whose tokens are then written more than once or not all, at positions of its own
     b = 0;
     int step = 1;
     while (32 * step < a.B) step *= 32;

@@ -249,7 +249,8 @@ class PagedKV:
 
     def append(self, layer: int, k, v, slots=None, cu_seqlens=None) -> None:
         """Write the newest tokens of each sequence, already reserved: k, v [B,t,G,D], or [T,G,D] packed with cu_seqlens
-        [B+1].  Sequence b (slot slots[b], an int tensor on the device; None: slot b) gets its n_b tokens at the positions
+        [B+1], whose entries must not descend (one below 0 counts as 0, one beyond T as T; after a descending one, which
+        prompt_attention takes for the one before it, not all tokens may be written).  Sequence b (slot slots[b], an int tensor on the device; None: slot b) gets its n_b tokens at the positions
         lens - n_b .. lens - 1, which are to be its own: tokens from before a fork may lie in pages that it shares.
         A page's scale covers what was written to it; earlier codes of a page whose scale grows are rounded to the new one.
         Infinities are stored as the largest code, NaN as NaN.  A slot named twice is written by its first sequence, a

@@ -372,7 +372,8 @@ int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void
  *
  * bf_paged_append: writes sequence b's n_b new tokens (n_b = t, or cu[b+1] - cu[b]) to the positions
  *   lens - n_b .. lens - 1 of slot slots[b] (slots NULL: slot b) of one layer.  k, v: dtype BF_BF16 or BF_F16 with element strides per
- *   batch, token and head (multiples of 8; with cu the batch stride is not used and t is the packed token count).
+ *   batch, token and head (multiples of 8; with cu the batch stride is not used and t is the packed token count; cu must not
+ *   descend, entries are clamped into [0, t]).
  *   A (page, head)'s scale is the smallest power of two s >= 2^-64 with amax / s <= 448 over the finite values written
  *   and, where the page held tokens before, at least the scale it had: the codes of those tokens are rounded again to
  *   a grown scale.  Infinities are stored as +-448 s, NaN as NaN.  Tokens without a page are not stored; a slot named

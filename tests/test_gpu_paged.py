@@ -675,3 +675,27 @@ def test_attend_query_rows_of_a_wide_range(dtype, e, t, H):
     assert ((o[0].cpu().double() - ro).abs() <= tol)[known].all()
     off, tol = (lse[0].cpu().double() - rl).abs(), 2.0 ** -13 * big.T + lost.T + 2.0 ** -16 * (1 + rl.abs())
     assert (off <= tol)[known.T].all(), (off - tol).max()
+
+
+def test_append_cumulative_lengths_beyond_the_tensors_and_out_of_order():
+    """Entries are clamped into [0, T].  Out of order they do not say which tokens are whose: what is written then lies in the named
+    sequences' newest positions and nowhere else."""
+    k, v = _rand(50, 2, D, seed=40), _rand(50, 2, D, seed=41)
+    c = _cache(1, 30, 2, 4, page=16, max_len=160)
+    c.reserve(range(4), [20, 40, 11, 7])
+    _fill(c, 42)
+    before = _host(c)
+    c.append(0, k.cuda(), v.cuda(), torch.tensor([0, 1, 2], device="cuda"), torch.tensor([-3, 5, 42, 90], device="cuda"))
+    _check_append(c, before, [0, 1, 2], [5, 37, 8], k, v)
+    x = torch.full((50, 2, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    keep = [y.clone() for y in (c.k_pages, c.v_pages)]
+    c.append(0, x, x, torch.tensor([0, 1, 2], device="cuda"), torch.tensor([0, 45, 9, 50], device="cuda"))
+    for old, new in zip(keep, (c.k_pages, c.v_pages)):
+        for slot, most in ((0, 20), (1, 5), (2, 41), (3, 0)):
+            n = int(c.lens[slot])
+            for j, p in enumerate(c.table[slot].tolist()[:-(-n // 16)]):
+                a, b = old[0, p].view(torch.uint8), new[0, p].view(torch.uint8)
+                assert torch.equal(a[:, max(n - j * 16, 0):], b[:, max(n - j * 16, 0):])          # behind the sequence's end
+                if (j + 1) * 16 <= n - most or most == 0:           # pages of none of its newest tokens
+                    assert torch.equal(a, b)
+        assert torch.equal(old[0, 10:].view(torch.uint8), new[0, 10:].view(torch.uint8))       # pages of no sequence
