@@ -11,8 +11,8 @@
 // its own:
 //   S^T[token, part x row] = K Q^T    M = 128 tokens, N = 3 RP, K = 256 dims   (a query component is exact in three parts while it is not
 //                                     far below its row's largest, and off by at most 2^-25 of the largest: the parts end there)
-//   O^T[dim, part x row]   = V^T P^T  M = 2 x 128 dims, N = 3 RP, K = 128 tokens (P is off by at most 2^-12 of itself, or
-//                                     2^-26 of the tile's largest weight)
+//   O^T[dim, part x row]   = V^T P^T  M = 2 x 128 dims, N = 3 RP, K = 128 tokens (P is rounded to fp16's 11 bits, which the parts
+//                                     hold: off by at most 2^-11 of itself, or 2^-26 of the tile's largest weight)
 // with a row = (token of the call, query head of the KV head's group), RP rows at a time.  P is taken relative to its own
 // tile's maximum, so that a tile of small weights keeps its bits, and the tile's O^T leaves TMEM for fp32 registers that
 // carry the running maximum: nothing is rescaled in TMEM.  V's scales go into P (as their ratio to the tile's largest).

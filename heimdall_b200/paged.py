@@ -126,8 +126,8 @@ class PageTable:
 class PagedKV:
     """Keys and values of ``layers`` kept layers in 8-bit pages (see the module's docstring).
 
-    ``pages`` of ``page`` tokens (16, 32, 64 or 128) for ``slots`` sequences of up to ``max_len`` tokens (default: the whole
-    pool), ``heads`` KV heads of 256.  Device tensors, for reading: ``k_pages``, ``v_pages`` [layers,pages,heads,page,256]
+    ``pages`` of ``page`` tokens (16, 32, 64 or 128) for ``slots`` sequences of up to ``max_len`` tokens, rounded up to whole
+    pages (default: the whole pool), ``heads`` KV heads of 256.  Device tensors, for reading: ``k_pages``, ``v_pages`` [layers,pages,heads,page,256]
     float8_e4m3fn, ``k_scale``, ``v_scale`` [layers,pages,heads] fp32 (value = code * scale), ``table`` [slots,width] int32
     (-1: no page), ``lens`` [slots] int32."""
 
@@ -289,8 +289,9 @@ class PagedKV:
         dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf.  What the
         pages hold behind a sequence's last token has no part in it; a NaN among a sequence's stored values reaches all t
         tokens.  A component of q is held to 2^-25 of the largest of its row and head (exactly, where it is above about 2^-14 of
-        that).  A token's weight times its V scale is held to 2^-26 of (largest weight) * (largest V scale) among the 128
-        tokens of its tile."""
+        that).  A token's weight times its V scale is held to 2^-11 of itself or 2^-26 of (largest weight) * (largest V scale) among
+        the 128 tokens of its tile, whichever is more.  Made for decode steps and drafts: 24 rows (tokens times query heads per KV
+        head) share one way through the pages, so t tokens take as long as t / floor(24 / (H / G)) of them."""
         self._check()
         dev = serving_inputs("PagedKV.attend", self.k_pages, q)
         layer, shape = self._layer(layer), q.shape

@@ -383,7 +383,8 @@ int bf_prompt_attn_fwd(const void* q, long long q_st, long long q_sh, const void
  *   table.  o [B,t,H,D] contiguous in dtype, lse [B,H,t] fp32 or NULL; a row that sees nothing gets 0 and -inf.
  *   Workspace: bf_paged_attend_workspace().  H / G <= 24; B t H and B G ceil(t / floor(24 G / H)) (width L / 128 + 4) below 2^31.
  *   A component of q is held to 2^-25 of the largest of its row (exactly, where it is above about 2^-14 of that).
- *   A token's weight times its V scale is held to 2^-26 of (largest weight) * (largest V scale) among the 128 tokens of its tile.
+ *   A token's weight times its V scale is held to 2^-11 of itself or 2^-26 of (largest weight) * (largest V scale) among the 128 tokens of
+ *   its tile, whichever is more.  24 rows (tokens times query heads per KV head) share one way through the pages.
  * bf_paged_pages: page bookkeeping and copies on the device; every list is HOST memory, read before the call returns.
  *   release [n_release]: slots whose table rows become -1 and lens 0;
  *   fork [n_fork][5] = (from slot, to slot, tokens, from page, to page): the row and length of `from`, and, where

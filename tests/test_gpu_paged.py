@@ -699,3 +699,55 @@ def test_append_cumulative_lengths_beyond_the_tensors_and_out_of_order():
                 if (j + 1) * 16 <= n - most or most == 0:           # pages of none of its newest tokens
                     assert torch.equal(a, b)
         assert torch.equal(old[0, 10:].view(torch.uint8), new[0, 10:].view(torch.uint8))       # pages of no sequence
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("apart", [4, 10, 16, 22])
+def test_attend_small_scales_with_the_weight_beside_large_ones(apart, page):
+    """Nearly all weight on pages whose V scale is 2^-apart of another's in the same tile; the largest scale of the last tile is on a page
+    that the first tokens of the call do not see.  A weight times its V scale is held to 2^-26 of the tile's largest weight times its
+    largest V scale: that times sum |code|, tile by tile, is the whole of the absolute term."""
+    G, H, t, n = 2, 4, 3, 15 * 16 + 1
+    c = _cache(1, 16, G, 1, page=page, max_len=256)
+    c.reserve([0], n)
+    _fill(c, 43)
+    row = c.table[0].tolist()[:-(-n // page)]
+    big = [row[j] for j in range(1, len(row), 4)] + [row[-1]]
+    c.k_scale.fill_(2.0 ** -7)
+    c.v_scale.fill_(2.0 ** -apart)
+    c.v_scale[0, big, 1] = 0.5
+    c.v_scale[0, big, 0] = 1.0
+    c.k_pages[0, :, :, :, 0] = 256.0
+    c.k_pages[0, big, :, :, 0] = -256.0
+    q = _rand(1, t, H, D, seed=44)
+    q[..., 0] = 80.0                                          # scores of 10 and -10 from this component
+    o, _ = c.attend(0, q.cuda())
+    kc, ks, vc, vs = _host(c)
+    ro, _, mag, size = opk.attend(kc, ks, vc, vs, c.table[0].tolist(), n, q[0])
+    for h in range(H):
+        g = h // (H // G)
+        k = (kc[row, g] * ks[row, g][:, None, None]).reshape(-1, D)[:n]
+        code, scale = vc[row, g].reshape(-1, D)[:n].abs(), vs[row, g].repeat_interleave(page)[:n]
+        for i in range(t):
+            m = n - t + 1 + i
+            p = torch.softmax(k[:m] @ q[0, i, h].double() / 16, 0)
+            floor = torch.zeros(D, dtype=torch.float64)
+            for a in range(0, m, 128):
+                floor += 2.0 ** -26 * p[a:a + 128].max() * scale[a:a + 128].max() * code[a:min(m, a + 128)].sum(0)
+            tol = (U[q.dtype] + 2.0 ** -11 + 2.0 ** -12 * size[i, h]) * mag[i, h] + floor
+            off = (o[0, i, h].cpu().double() - ro[i, h]).abs()
+            assert (off <= tol).all(), (h, i, (off - tol).max())
+            w = p * scale[:m]
+            assert w[scale[:m] < 0.25].sum() > 0.5 * w.sum() and floor.max() < 0.5 * mag[i, h].max()   # so that their part cannot be missing
+
+
+@pytest.mark.parametrize("t", [25, 130, 600])
+@pytest.mark.parametrize("H,G,page", [(3, 1, 16), (2, 2, 64)])
+def test_attend_of_many_tokens_at_once(t, H, G, page):
+    """A chunk of a prompt over the pages: many blocks of rows of one sequence, the last one not full, and tokens before the first."""
+    lens = [t + 45, 100]
+    c = _cache(1, sum(-(-n // page) for n in lens) + 1, G, 2, page=page, max_len=704)
+    c.reserve([0, 1], lens)
+    _fill(c, 45)
+    _poison(c)
+    _check_attend(c, _rand(2, t, H, D, seed=46, dtype=torch.float16 if t == 130 else torch.bfloat16), None)
