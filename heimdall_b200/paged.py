@@ -321,15 +321,17 @@ class PagedKV:
 
 
 class _Progress:
-    """What ``retrieval.teacher`` has written: the tokens of each slot in each layer, -1 where the host cannot tell, because the caller's
-    own ``append`` may have written a sequence's newest tokens there."""
+    """What ``retrieval.teacher`` has written: the tokens of each slot in each layer, UNKNOWN where the host cannot tell, because the
+    caller's own ``append`` may have written a sequence's newest tokens there."""
+
+    UNKNOWN = -2 ** 40              # so far below any length that no number of new tokens makes one of it
 
     def __init__(self, cache: PagedKV):
         self.host = cache.host
         self.n = np.zeros((cache.layers, self.host.slots), np.int64)
         self.room = np.zeros(self.host.slots, np.int64)     # a slot's length when teacher last made room in it
         for layer in cache._appended:
-            self.n[layer, self.host.lens > 0] = -1
+            self.n[layer, self.host.lens > 0] = self.UNKNOWN
 
     def free(self, slots) -> None:
         s = self.host._whole(slots)
@@ -355,7 +357,7 @@ class _Progress:
         elif may.any() and not (slots.is_cuda and torch.cuda.is_current_stream_capturing()):
             named = np.asarray(slots.tolist(), np.int64)
             may &= np.isin(np.arange(n.size), named)
-        n[may] = -1
+        n[may] = self.UNKNOWN
 
 
 class PagedLayer:
@@ -382,38 +384,38 @@ class PagedLayer:
 
     def teacher(self, qr, kr, v, retrieval=None):
         c = self.cache
-        # what the calls below would refuse, before room is given out
-        serving_inputs("retrieval.teacher over pages", c.k_pages, qr, kr, v)
-        if qr.dim() != 4 or v.shape != (qr.shape[0], qr.shape[2], c.heads, c.dim) or \
-                kr.shape != (qr.shape[0], c.heads, qr.shape[2], c.dim) or qr.shape[3] != c.dim or qr.shape[1] % c.heads or qr.shape[1] < 1:
+        B, H, t, D = qr.shape
+        # what would be refused after the keys and values are written (append refuses kr and v before that)
+        if qr.device != c.device or (qr.requires_grad and torch.is_grad_enabled()):
+            serving_inputs("retrieval.teacher over pages", c.k_pages, qr)
+        if v.shape != (B, t, c.heads, c.dim) or D != c.dim or H % c.heads or H < 1:
             raise ValueError(f"teacher over pages takes qr [B,H,t,{c.dim}], kr [B,{c.heads},t,{c.dim}] and v [B,t,{c.heads},{c.dim}] "
                              f"with H a multiple of {c.heads}")
-        B, H, t, D = qr.shape
         if B > c.host.slots:
             raise ValueError("more sequences than the cache has slots")
         p, lens = c._progress, c.host.lens[:B]
-        had = p.n[self.index, :B].copy()
-        n = int(had.max(initial=0)) + t
+        had = p.n[self.index, :B]
+        later = bool(had.any())
         if retrieval is not None and (t == 1 or retrieval.get("prefill")) and \
-                n - retrieval["sinks"] - retrieval["window"] >= retrieval["k"] * retrieval["block"]:
+                int(had.max(initial=0)) + t - retrieval["sinks"] - retrieval["window"] >= retrieval["k"] * retrieval["block"]:
             raise NotImplementedError("heimdall_b200 retrieval: block selection over 8-bit pages is not built")
-        if had.any() and H // c.heads > MAX_GROUP:
+        if later and H // c.heads > MAX_GROUP:
             raise NotImplementedError(f"attend takes at most {MAX_GROUP} query heads per KV head")
-        if (had < 0).any():
-            raise ValueError("a sequence's tokens in this layer were written with append: attend goes on from there, not teacher")
-        make_room = bool((lens == had).all())
-        if not make_room and not (lens == had + t).all():
-            raise ValueError("the layers of a paged cache must take the same tokens in step")
+        make_room = had.tobytes() == lens.tobytes()            # (a fifth of the time of comparing the arrays)
         if make_room:
             c.reserve(np.arange(B), t)
             p.room[:B] = lens
+        elif (had + t).tobytes() != lens.tobytes():
+            if (had < 0).any():
+                raise ValueError("a sequence's tokens in this layer were written with append: attend goes on from there, not teacher")
+            raise ValueError("the layers of a paged cache must take the same tokens in step")
         try:
-            o = self._attend(qr, kr, v, had.any())
+            o = self._attend(qr, kr, v, later)
         except BaseException:
-            if make_room:                 # what only a kernel's entry refuses: the room goes back
-                c.truncate(np.arange(B), had)
+            if make_room:                 # nothing of the sequences has changed but their room
+                c.truncate(np.arange(B), had.copy())
             raise
-        p.n[self.index, :B] = lens
+        had[:] = lens
         return o
 
     def _attend(self, qr, kr, v, later: bool):

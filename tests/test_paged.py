@@ -231,10 +231,10 @@ def test_a_layers_progress_follows_the_page_table():
 
     class Cache:
         layers, host, _appended = 3, PageTable(40, 4, 16, 6), {1}
-    host = Cache.host
+    host, no = Cache.host, _Progress.UNKNOWN
     host.reserve([3], 5)                                    # written directly in layer 1 before the first layer()
     p = _Progress(Cache)
-    assert p.n.tolist() == [[0] * 4, [0, 0, 0, -1], [0] * 4]
+    assert p.n.tolist() == [[0] * 4, [0, 0, 0, no], [0] * 4]
 
     def teacher(layer, B, t):
         if (host.lens[:B] == p.n[layer, :B]).all():
@@ -249,17 +249,17 @@ def test_a_layers_progress_follows_the_page_table():
     assert p.n[:, :2].tolist() == [[18, 0]] * 3
     host.fork([0, 3], [1, 2])
     p.fork([0, 3], [1, 2])
-    assert p.n.tolist() == [[18, 18, 0, 0], [18, 18, -1, -1], [18, 18, 0, 0]]
+    assert p.n.tolist() == [[18, 18, 0, 0], [18, 18, no, no], [18, 18, 0, 0]]
     teacher(0, 2, 1)
     p.appended(1, torch.tensor([2, 3]), 2)                  # teacher's own room is not in doubt
     p.appended(1, None, 4)
-    assert p.n[1].tolist() == [18, 18, -1, -1]
+    assert p.n[1].tolist() == [18, 18, no, no]
     teacher(1, 2, 1), teacher(2, 2, 1)
     host.reserve([0, 1], 2)                                 # the caller's is
     p.appended(0, torch.tensor([1, 9, -1]), 3)
-    assert p.n[0].tolist() == [19, -1, 0, 0]
+    assert p.n[0].tolist() == [19, no, 0, 0]
     p.appended(2, None, 1)
-    assert p.n[2].tolist() == [-1, 19, 0, 0]
+    assert p.n[2].tolist() == [no, 19, 0, 0]
     host.truncate([1], 0)
     p.truncate([1], 0)
     host.free([0, 3])
