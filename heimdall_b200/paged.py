@@ -127,8 +127,8 @@ class PagedKV:
     """Keys and values of ``layers`` kept layers in 8-bit pages (see the module's docstring).
 
     ``pages`` of ``page`` tokens (16, 32, 64 or 128) for ``slots`` sequences of up to ``max_len`` tokens, rounded up to whole
-    pages (default: the whole pool), ``heads`` KV heads of 256.  Device tensors, for reading: ``k_pages``, ``v_pages`` [layers,pages,heads,page,256]
-    float8_e4m3fn, ``k_scale``, ``v_scale`` [layers,pages,heads] fp32 (value = code * scale), ``table`` [slots,width] int32
+    pages (default: the whole pool), ``heads`` KV heads of 256.  Device tensors, for reading: ``k_pages``, ``v_pages``
+    [layers,pages,heads,page,256] float8_e4m3fn, ``k_scale``, ``v_scale`` [layers,pages,heads] fp32 (value = code * scale), ``table`` [slots,width] int32
     (-1: no page), ``lens`` [slots] int32."""
 
     def __init__(self, layers: int, pages: int, heads: int, slots: int, page: int = 64, dim: int = 256, max_len=None,
@@ -250,15 +250,16 @@ class PagedKV:
     def append(self, layer: int, k, v, slots=None, cu_seqlens=None) -> None:
         """Write the newest tokens of each sequence, already reserved: k, v [B,t,G,D], or [T,G,D] packed with cu_seqlens
         [B+1], whose entries must not descend (one below 0 counts as 0, one beyond T as T; after a descending one, which
-        prompt_attention takes for the one before it, not all tokens may be written).  Sequence b (slot slots[b], an int tensor on the device; None: slot b) gets its n_b tokens at the positions
-        lens - n_b .. lens - 1, which are to be its own: tokens from before a fork may lie in pages that it shares.
+        prompt_attention takes for the one before it, not all tokens may be written).  Sequence b (slot
+        slots[b], an int tensor on the device; None: slot b) gets its n_b tokens at the positions lens - n_b .. lens - 1,
+        which are to be its own: tokens from before a fork may lie in pages that it shares.
         A page's scale covers what was written to it; earlier codes of a page whose scale grows are rounded to the new one.
         Infinities are stored as the largest code, NaN as NaN.  A slot named twice is written by its first sequence, a
         number outside the cache's slots by none."""
         B = self._append(layer, k, v, slots, cu_seqlens)
-        if self._progress is None:
+        if B and self._progress is None:
             self._appended.add(layer)
-        else:
+        elif B:
             self._progress.appended(int(layer), slots, B)
 
     def _append(self, layer: int, k, v, slots=None, cu_seqlens=None) -> int:
@@ -281,7 +282,7 @@ class PagedKV:
                 ks, vs = [0] + ks, [0] + vs
             _lib.call("bf_paged_append", self._pool_ptr, layer, kp, *ks, vp, *vs, ptr(ids), ptr(cu), B, shape[-3], kernel_dtype(k),
                       stream_handle())
-        return B
+        return B if shape[-3] else 0        # the sequences that tokens may have been written of
 
     def attend(self, layer: int, q, slots=None, scale=None, with_lse: bool = False):
         """Attention of each sequence's last t tokens over its pages: q [B,t,H,D] (bf16 or fp16; H a multiple of the KV
@@ -348,8 +349,8 @@ class _Progress:
         self.n[:, s[m == 0]] = 0
 
     def appended(self, layer: int, slots, B: int) -> None:
-        """The caller's own append of B sequences to a layer: what was reserved by the caller, and not by teacher, may be written now.  (Which
-        slots it named is read back from the device where that matters, but not in a capture.)"""
+        """The caller's own append of B sequences to a layer: what was reserved by the caller, and not by teacher, may be
+        written now.  (Which slots it named is read back from the device where that matters, but not in a capture.)"""
         n, lens = self.n[layer], self.host.lens
         may = (n >= 0) & (n < lens) & (lens != self.room)
         if slots is None:

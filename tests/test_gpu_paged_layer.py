@@ -175,3 +175,16 @@ def test_a_refused_call_leaves_the_cache_as_it_was(monkeypatch):
     for x in layers:
         _teacher(qr, kr, v, x, None)
     assert c.lens.tolist() == [25, 25] and layers[1].n == 25
+
+
+def test_appends_of_nothing_leave_no_doubt():
+    """A call without sequences or tokens has written nothing, before the first layer() and after it."""
+    c = _cache(1)
+    qr, kr, v = _qkv(2, 3, 0)
+    c.reserve([0, 1], 3)
+    none = lambda: (c.append(0, kr.transpose(1, 2)[:0], v[:0]), c.append(0, kr.transpose(1, 2)[:, :0], v[:, :0]))
+    none()
+    layer = c.layer(0)
+    none()
+    _teacher(qr, kr, v, layer, None)
+    assert c.lens.tolist() == [3, 3] and layer.n == 3
