@@ -31,10 +31,11 @@
 // costs: one thread of a diverged warp took 4400 cycles per tile for both (every descriptor on its way through vector registers); two
 // warps that stay converged and elect the issuing lane do not bound it.  The roles together have to stay in the instruction
 // cache: waits and loops are written for few instructions (106 KB of code took a third longer than 72 KB).
-// Measured (24 query heads, 4 KV heads, pages of 64): 64 sequences of 16384 tokens 326 us, all that the measured copy rate allows
-// (331 us); 64 of 1 to 16384 tokens 48 us (floor 36); one of 777 tokens 9.6 us.  24 rows (four tokens): 3550 cycles a tile, bound by
-// the softmax warps' way through a tile: 32 sequences of 16384 tokens 225 us (floor 166), with pages of 16 tokens 247 (eight copies
-// per tile and half).  There 80 registers per thread are all there are, and what does not fit costs: 244 us with 28 bytes spilled.
+// Measured (24 query heads, 4 KV heads, pages of 64): 64 sequences of 16384 tokens 326 us, 6.6 TB/s (the measured rate of a copy, which
+// also writes, is 6.5; 16 of 131072 take 622 us repeated, 676 to 734 with other passes in between); 64 of 1 to 16384 tokens 48 us
+// (floor 36); one of 777 tokens 9.6 us.  24 rows (four tokens): 3550 cycles a tile, bound by the softmax warps' way through a tile: 32
+// sequences of 16384 tokens 225 us (floor 166), with pages of 16 tokens 247 (eight copies per tile and half).  There 80 registers per
+// thread are all there are, and what does not fit costs: 244 us with 28 bytes spilled.
 // (Taking a tile's scores before the weights of the one before, so that nobody waits for the maxima, made it 267 us.)
 #include "bifrost_b200.h"
 #include "capi_internal.h"

@@ -24,8 +24,9 @@
 // Warps (512 threads): 0 Q and K loads; 1 MMA (in the first CTA of the pair); 2 V loads; 3 the next items (the first CTA asks and
 // passes the answer on); 4-11 softmax, two warpgroups, every other tile each; 12-15 the outputs, while the next item's products run.
 //
-// Measured (24 query heads, 4 KV heads, bf16): 32768 tokens 9.13 ms = 1446 TFLOP/s, above the library product's rate under the power
-// limit (1406) and 0.87 of its burst; 8192 tokens 538 us = 1534 (0.92 of burst); 2300 cycles per key tile against the tensor core's
+// Measured (24 query heads, 4 KV heads, bf16), repeated on one input: 32768 tokens 9.13 ms = 1446 TFLOP/s on one GPU, 9.3 to 9.6 ms on
+// others and with other inputs in every pass (1375 to 1420; the library product's rate under the power limit is 1406, its burst
+// 1666); 8192 tokens 538 us = 1534 before the power limit sets in, 600 in a longer loop; 2300 cycles per key tile against the tensor core's
 // 2048.  Between items 3700 cycles are lost, most of them for the next item's queries, 64 KB that only fit once the last product has
 // read the ones before: eight prompts of 1 to 4095 tokens run at 1274.
 #include "bifrost_b200.h"
