@@ -365,8 +365,9 @@ class PagedLayer:
     """One layer of a ``PagedKV`` as the cache of ``retrieval.teacher``: every call brings the next t tokens of each of the
     sequences in the slots 0 .. B-1.  The first layer that needs room reserves it (or the caller has, for exactly these tokens), and
     every layer takes the same tokens.  ``free``, ``truncate`` and ``fork`` of the cache are followed.  A sequence whose tokens were
-    written to the layer with ``append`` is not gone on with: ``attend`` is the call for those.  Replays of a captured call are
-    not seen by the host; what was captured goes on by replays, or anew after ``free``."""
+    written to the layer with ``append`` is not gone on with: ``attend`` is the call for those.  (Beside
+    teacher, an ``append`` to sequences whose room the caller reserved waits for its slot numbers to be read back.)  Replays of a captured
+    call are not seen by the host; what was captured goes on by replays, or anew after ``free``."""
 
     def __init__(self, cache: PagedKV, layer: int):
         self.cache, self.index = cache, layer
