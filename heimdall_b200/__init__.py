@@ -11,6 +11,7 @@ Public API (mirrors of the reference ``heimdall`` package):
   delta_rule_step                    heimdall/kernels.py:132-138
   window_attention                   heimdall/hibrit.py:336-361 (the math of _window_fp32)
   prompt_attention                   heimdall/hibrit.py:275-290 (a kept layer's causal attention, packed prompts)
+  norm_rope_heads                    heimdall/hibrit.py:254-268 (_proj's norm and rotation, positions on several axes)
   PagedKV                            a kept layer's cache in 8-bit pages: append, attend, fork, free, compact
   BifrostLayer.student               heimdall/hibrit.py:363-424 (HybridAttention._student)
   BifrostLayer.mem_inputs            heimdall/hibrit.py:327-334
@@ -23,10 +24,10 @@ Public API (mirrors of the reference ``heimdall`` package):
   plugin.prepare / install           the kernels.prepare plug-in convention (heimdall/kernels.py:158-188)
 """
 from .functional import delta_rule, delta_rule_gqa, delta_rule_step, delta_rule_step_gqa  # noqa: F401
-from .functional import prompt_attention, window_attention  # noqa: F401
+from .functional import norm_rope_heads, prompt_attention, rope_axes, window_attention  # noqa: F401
 from .layer import BifrostLayer  # noqa: F401
 from .paged import PagedKV  # noqa: F401
 from .attention import BifrostAttention  # noqa: F401
 
 __all__ = ["delta_rule", "delta_rule_gqa", "delta_rule_step", "delta_rule_step_gqa", "window_attention",
-           "prompt_attention", "BifrostLayer", "BifrostAttention", "PagedKV"]
+           "prompt_attention", "norm_rope_heads", "rope_axes", "BifrostLayer", "BifrostAttention", "PagedKV"]

@@ -44,6 +44,7 @@ SIGNATURES = {
     "bf_bifrost_layer_prefill": [_P, _P, _P, _P, _P, _P, _P, _L, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _Z, _P],
     "bf_attn_prologue": [_P, _P, _P, _P, _P, _I, ctypes.c_float, _L, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P],
     "bf_attn_epilogue": [_P, _P, _I, _I, _I, _I, _I, _P, _P],
+    "bf_norm_rope": [_P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _I, _P, _I, _P, _I, ctypes.c_float] + [_I] * 6 + [_P] * 5,
     "bf_gdn_segment_workspace": [_I, _I, _I, _I],
     "bf_gdn_segment_transform": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P],
     "bf_gdn_apply_prefix": [_P, _P, _I, _P, _P, _I, _I, _I, _P],

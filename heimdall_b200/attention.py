@@ -14,7 +14,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
-from .functional import check_cuda, ptr, stream_handle
+from .functional import check_cuda, norm_rope_heads, ptr, rope_axes, stream_handle
 from .layer import BifrostLayer
 
 
@@ -25,10 +25,12 @@ class BifrostAttention:
     ``k_w``/``v_w`` [G*D, d], ``o_w`` [d, H*D], optional biases, ``q_norm_w``/``k_norm_w`` [D] (zero-centred
     ZNorm weights), RoPE on the first ``rot`` dims with base ``theta``, norm ``eps``; ``layer`` the converted
     core (``BifrostLayer``).  ``mode``: "student" (window + memory) or "window" (the reference's memoryless mode).
+    ``rope_sections``: rotary frequencies per axis (time, height, width) for calls with ``positions`` on several axes.
     """
 
     def __init__(self, q_w, k_w, v_w, o_w, q_norm_w, k_norm_w, layer: BifrostLayer, rot: int, theta: float,
-                 eps: float = 1e-6, gated: bool = True, q_b=None, k_b=None, v_b=None, o_b=None, mode: str = "student"):
+                 eps: float = 1e-6, gated: bool = True, q_b=None, k_b=None, v_b=None, o_b=None, mode: str = "student",
+                 rope_sections=None):
         dev = layer.device
         bf = torch.bfloat16
         cvt = lambda t: None if t is None else t.detach().to(device=dev, dtype=bf).contiguous()
@@ -43,12 +45,15 @@ class BifrostAttention:
         H, G, D = layer.H, layer.G, layer.D
         if tuple(self.q_w.shape) != (H * D * (2 if gated else 1), layer.d) or tuple(self.k_w.shape) != (G * D, layer.d):
             raise ValueError("projection shapes do not match the layer")
+        if rope_sections is not None and sum(rope_sections) * 2 != self.rot:
+            raise ValueError("rope_sections must add up to rot / 2 frequencies")
+        self.axes = None if rope_sections is None else rope_axes(rope_sections)
         # inverse RoPE frequencies exactly as the reference computes them (heimdall/kernels.py:44), in fp32
         d_rot = max(self.rot, 2)
         self.inv_freq = (1.0 / (self.theta ** (torch.arange(0, d_rot, 2, dtype=torch.float32) / d_rot))).to(dev)
 
     @classmethod
-    def from_module(cls, attn, device=None) -> "BifrostAttention":
+    def from_module(cls, attn, device=None, rope_sections=None) -> "BifrostAttention":
         """From a converted reference ``HybridAttention`` (its projections, norms, RoPE config and new parameters)."""
         c = attn.c
         layer = BifrostLayer.from_module(attn, device)
@@ -56,12 +61,13 @@ class BifrostAttention:
         return cls(attn.q_proj.weight, attn.k_proj.weight, attn.v_proj.weight, attn.o_proj.weight,
                    attn.q_norm.weight, attn.k_norm.weight, layer, c.rot, c.rope_theta, c.eps, c.gate,
                    bias(attn.q_proj), bias(attn.k_proj), bias(attn.v_proj), bias(attn.o_proj),
-                   mode="window" if attn.mode == "window" else "student")
+                   mode="window" if attn.mode == "window" else "student", rope_sections=rope_sections)
 
-    def project(self, x, start: int = 0):
+    def project(self, x, start: int = 0, positions=None):
         """``HybridAttention._proj`` (heimdall/hibrit.py:254-268): x [B,t,d] -> (q, k, v, qr, kr, qg) with q
         [B,t,H,D], k/v [B,t,G,D] (ZNorm'd), qr [B,H,t,D], kr [B,G,t,D] (partial RoPE) in bf16, and qg the query
-        projection [B,t,H,(2 if gated) D] holding the output gate."""
+        projection [B,t,H,(2 if gated) D] holding the output gate.  ``positions`` (int [B,t], or [axes,B,t] with the layer's
+        ``rope_sections``): the rotation's positions of every token, in the place of start, start + 1, ... (``norm_rope_heads``)."""
         check_cuda(x)
         L = self.layer
         B, t = x.shape[:2]
@@ -70,6 +76,11 @@ class BifrostAttention:
         qg = F.linear(xb, self.q_w, self.q_b).contiguous()
         kl = F.linear(xb, self.k_w, self.k_b).contiguous()
         v = F.linear(xb, self.v_w, self.v_b).view(B, t, G, D)
+        if positions is not None:
+            q, k, qr, kr = norm_rope_heads(qg.view(B, t, H, -1), kl.view(B, t, G, D), self.q_norm_w, self.k_norm_w, positions,
+                                           self.inv_freq if self.rot else None, self.axes if positions.dim() == 3 else None, self.eps,
+                                           self.gated)
+            return q, k, v.contiguous(), qr, kr, qg
         dev = x.device
         q = torch.empty(B, t, H, D, device=dev, dtype=torch.bfloat16)
         k = torch.empty(B, t, G, D, device=dev, dtype=torch.bfloat16)
@@ -89,10 +100,11 @@ class BifrostAttention:
                   stream_handle())
         return F.linear(y, self.o_w, self.o_b)
 
-    def forward(self, x, cache=None, start: int = 0):
+    def forward(self, x, cache=None, start: int = 0, positions=None):
         """``HybridAttention.forward`` of a converted layer (heimdall/hibrit.py:426-432): x [B,t,d] -> [B,t,d] bf16,
-        with the reference's cache dict (prefill for t > 1, the decode step for t == 1 with a cache)."""
-        q, k, v, qr, kr, qg = self.project(x, start)
+        with the reference's cache dict (prefill for t > 1, the decode step for t == 1 with a cache).
+        ``positions`` turn the heads (``project``); the window and the memory go by the tokens' order, from ``start`` on."""
+        q, k, v, qr, kr, qg = self.project(x, start, positions)
         o = self.layer.student(x, q, k, v, qr, kr, int(start), cache, memory=self.mode != "window")
         o = o.reshape(*x.shape[:2], self.layer.H, self.layer.D)
         return self.output(o, qg, x)

@@ -324,6 +324,64 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, scale=None, with_ls
     return o, lse
 
 
+def rope_axes(sections) -> list:
+    """The axis of each rotary frequency for ``sections`` (frequencies per axis, as (11, 11, 10) for time, height and width):
+    frequencies are dealt to the axes in turn, and an axis that has all of its own leaves the rest to the first."""
+    n, F = len(sections), sum(sections)
+    if not 1 <= n <= 4 or min(sections) < 0:
+        raise ValueError("sections are the frequencies of one to four axes")
+    axes = [f % n if f < n * sections[f % n] else 0 for f in range(F)]
+    if [axes.count(a) for a in range(n)] != list(sections):
+        raise ValueError(f"sections {tuple(sections)} cannot be dealt in turn")
+    return axes
+
+
+def norm_rope_heads(qg, kl, q_norm_w, k_norm_w, positions, inv_freq, axes=None, eps: float = 1e-6, gated: bool = True,
+                    memory: bool = True):
+    """The norm and the partial rotation of ``HybridAttention._proj`` (hibrit.py:254-268) with every token's own positions, on one
+    axis or several (time, height and width of images).
+
+    qg [B,t,H,(2 if gated) D] (query projection, the output gate behind each head's query) and kl [B,t,G,D], bf16 or fp16, any
+    strides; q_norm_w, k_norm_w [D] zero-centred norm weights; positions [B,t] or [n,B,t] (int32 or int64, n <= 4 axes); inv_freq [F] fp32
+    or None; ``axes``: the axis of each frequency (``rope_axes``; None: the first).  Returns (q [B,t,H,D], k [B,t,G,D], qr [B,H,t,D],
+    kr [B,G,t,D]) in qg's dtype: y = x / sqrt(mean x^2 + eps) * (1 + w), and y with the dims f and f + F turned by positions[axes[f]] *
+    inv_freq[f]; q and k are None without ``memory`` (a kept layer has no memory path).  Each output is rounded once (the one-axis prologue of
+    ``BifrostAttention.project`` rounds y before it turns it, as the reference does), and angles are computed in 64 bits."""
+    dev = serving_inputs("norm_rope_heads", qg, kl, q_norm_w, k_norm_w)
+    if qg.dim() != 4 or kl.dim() != 4 or qg.shape[:2] != kl.shape[:2] or qg.dtype != kl.dtype:
+        raise ValueError("norm_rope_heads takes qg [B,t,H,(2) D] and kl [B,t,G,D] of one dtype")
+    B, t, H, _ = qg.shape
+    G, D = kl.shape[2], kl.shape[3]
+    if D != 256:
+        raise NotImplementedError("norm_rope_heads is built for head dim 256")
+    if qg.shape[3] != (2 * D if gated else D) or q_norm_w.shape != (D,) or k_norm_w.shape != (D,) or H < 1 or G < 1:
+        raise ValueError("the heads' and norm weights' shapes do not match")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape[-2:] != (B, t) or positions.dim() not in (2, 3):
+        raise ValueError("positions must be an int32 or int64 tensor [B,t] or [axes,B,t]")
+    n = positions.shape[0] if positions.dim() == 3 else 1
+    F = 0 if inv_freq is None else inv_freq.numel()
+    if not 1 <= n <= 4 or (axes is None and n > 1):
+        raise ValueError("positions have one to four axes, and with more than one the axis of each frequency is needed")
+    if F % 8 or F > D // 2:
+        raise NotImplementedError("norm_rope_heads turns a multiple of 16 dims, at most all of them")
+    code = bytes(F) if axes is None else bytes(axes)
+    if len(code) != F or (F and max(code) >= n):
+        raise ValueError("axes needs one of the positions' axes for each frequency")
+    with on_device(dev):
+        on = lambda x, dt: x if x.dtype == dt and x.device == dev and x.is_contiguous() else x.to(device=dev, dtype=dt).contiguous()
+        q_norm_w, k_norm_w = on(q_norm_w, torch.float32), on(k_norm_w, torch.float32)
+        inv_freq = None if not F else on(inv_freq, torch.float32)
+        positions = on(positions, positions.dtype)
+        qg, qp, qs = heads_16bit("qg", qg)
+        kl, kp, ks = heads_16bit("kl", kl)
+        q, k = (qg.new_empty((B, t, H, D)), qg.new_empty((B, t, G, D))) if memory else (None, None)
+        qr, kr = qg.new_empty((B, H, t, D)), qg.new_empty((B, G, t, D))
+        _lib.call("bf_norm_rope", qp, *qs, kp, *ks, ptr(q_norm_w), ptr(k_norm_w), ptr(inv_freq), F, code, n, ptr(positions),
+                  int(positions.dtype == torch.int64), eps, B, t, H, G, D, kernel_dtype(qg), ptr(q), ptr(k), ptr(qr), ptr(kr),
+                  stream_handle())
+    return q, k, qr, kr
+
+
 def segment_transform(k, v, g, beta, s0=None):
     """State map of one segment of the write stream, for sequence parallelism of the delta rule.
 

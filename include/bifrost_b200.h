@@ -260,6 +260,21 @@ int bf_attn_epilogue(const float* o, const void* qg, int gated, int B, int T, in
                      bf_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * The prologue's norm and rotation with positions given per token on several axes (time, height, width of an image's
+ * patches; text counts on all axes alike), for batches whose sequences are each at their own position.
+ *   qg [B,T,H,...], kl [B,T,G,...]: dtype BF_BF16 or BF_F16, element strides per batch, token and head given (multiples of 8),
+ *   the first D elements of each row are the head; q_norm_w, k_norm_w [D] fp32; inv_freq [freqs] fp32; axes [freqs] HOST
+ *   bytes: the axis of each frequency, below n_axes (1 to 4); pos [n_axes,B,T] int32, or int64 when pos64
+ *   -> y = x rsqrt(mean x^2 + eps) (1 + w); q [B,T,H,D], k [B,T,G,D] (y, both NULL: not written); qr [B,H,T,D], kr [B,G,T,D]
+ *   (y with dims f and f + freqs turned by the angle pos[axes[f]] * inv_freq[f]), contiguous, each rounded to dtype once.  The
+ *   angle is computed in 64 bits.  D = 256, freqs a multiple of 8, at most 128.
+ */
+int bf_norm_rope(const void* qg, long long q_sb, long long q_st, long long q_sh, const void* kl, long long k_sb, long long k_st,
+                 long long k_sh, const float* q_norm_w, const float* k_norm_w, const float* inv_freq, int freqs,
+                 const uint8_t* axes, int n_axes, const void* pos, int pos64, float eps, int B, int T, int H, int G, int D,
+                 int dtype, void* q, void* k, void* qr, void* kr, bf_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Sequence parallelism of the delta rule (a long sequence split into consecutive segments, one per
  * GPU).  A segment of the write stream maps any incoming state S to S_out = M (S - s0) + N, where N
  * is the final state from s0 (zero state when s0 is NULL).  These two entry points replace the
