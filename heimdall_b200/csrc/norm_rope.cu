@@ -5,10 +5,14 @@
 //   frequency.  y itself goes out too where the memory path reads it.
 //
 // What bounds it is HBM: 512 bytes read and 512 or 1024 written per (token, head).  The angles are the same for all heads of a token, so
-// a CTA makes the sines and cosines of its tokens once, in shared memory; the product and its reduction by 2 pi are done in 64 bits (in
+// a CTA makes the sines and cosines of its tokens once, in shared memory; the product and its reduction to one turn are done in 64 bits (in
 // fp32 an angle of position 100000 is off by up to 2^-8, as much as the output's rounding).  A warp takes four heads of one token at a
-// time (lane l: dims 8 l .. 8 l + 7), so that enough loads are in flight; the rotation's partner dims are F / 8 lanes away.  The rotated
-// heads are made from y in fp32, so each output is rounded once.
+// time, with the next four on their way.  Lane l < F / 4 has the dims 4 l .. 4 l + 3 and their partners F further on, the other lanes eight dims that
+// are not turned (cos 1, sin 0): no value changes lanes, at the price of 8-byte accesses.  The rotated heads are made from y in fp32, so
+// each output is rounded once.
+// The instructions of a head come next to HBM as a bound: with the partner's values by shuffles and 64-bit divisions for every four heads it
+// took 75 us for 8191 tokens of 24 + 4 heads and 446 for 65536 without q and k, now 65 (5.4 TB/s) and 345 (5.5).  Two heads at a time on three or
+// four CTAs per SM, which costs spills, 72 to 80 and 394 to 426; 16 tokens per CTA 65 and 350.
 #include "capi_internal.h"
 #include "common.cuh"
 #include "launch_early.h"
@@ -17,7 +21,7 @@ namespace bfb {
 
 constexpr int kNR_D = 256;
 constexpr int kNR_Heads = 4;       // heads per warp at a time
-constexpr int kNR_Tokens = 8;      // most tokens per CTA
+constexpr int kNR_Tokens = 32;     // most tokens per CTA
 
 struct NormRopeArgs {
   const void *qg, *kl;
@@ -32,106 +36,143 @@ struct NormRopeArgs {
   void *q, *k, *qr, *kr;
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&f)[8]) {
-  const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = (float)e[j];
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 template <typename T>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  uint4 u;
-  T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) e[j] = (T)f[j];
-  return u;
+__device__ __forceinline__ uint64_t widen(uint32_t u) {      // two 16-bit values as fp32
+  const T* e = reinterpret_cast<const T*>(&u);
+  return pair2((float)e[0], (float)e[1]);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t narrow(uint64_t x);
+template <>
+__device__ __forceinline__ uint32_t narrow<__nv_bfloat16>(uint64_t x) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo_hi(x, 0), lo_hi(x, 1));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t narrow<__half>(uint64_t x) {
+  return pack_half2(lo_hi(x, 0), lo_hi(x, 1));
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) norm_rope_kernel(NormRopeArgs a) {
-  __shared__ float2 s_cs[kNR_Tokens][kNR_D / 2];
+__global__ void __launch_bounds__(256, 2) norm_rope_kernel(NormRopeArgs a) {
+  __shared__ __align__(16) float s_cos[kNR_Tokens][kNR_D / 2], s_sin[kNR_Tokens][kNR_D / 2];
+  __shared__ long long s_at[kNR_Tokens][4];        // elements of q and k behind which a token's heads begin; its rows of q and k turned
   let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   wait_for_stream();
   const long long n0 = (long long)blockIdx.x * a.tokens;
   const int tokens = (int)(a.BT - n0 < a.tokens ? a.BT - n0 : a.tokens), F = a.F;
-  for (int i = tid; i < tokens * F; i += 256) {
-    const int t = i / F, f = i % F, ax = (a.axis[f >> 4] >> (2 * (f & 15))) & 3;
-    const long long at = ax * a.BT + n0 + t;
-    const double p = a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at] : (double)static_cast<const int32_t*>(a.pos)[at];
-    const double ang = p * (double)a.inv_freq[f], turns = rint(ang * 0.15915494309189535);
-    float sn, cs;
-    sincosf((float)fma(turns, -6.283185307179586, ang), &sn, &cs);
-    s_cs[t][f] = make_float2(cs, sn);
-  }
-  float wq[8], wk[8];
-  {
-    const float4* w = reinterpret_cast<const float4*>(a.q_w) + 2 * lane;
-    const float4* v = reinterpret_cast<const float4*>(a.k_w) + 2 * lane;
-    const float4 w0 = __ldg(w), w1 = __ldg(w + 1), v0 = __ldg(v), v1 = __ldg(v + 1);
-    const float x[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w}, y[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      wq[e] = 1.f + x[e];
-      wk[e] = 1.f + y[e];
-    }
+  if (tid < tokens) {
+    const long long b = (n0 + tid) / a.T, t = (n0 + tid) - b * a.T;
+    s_at[tid][0] = b * a.q_sb + t * a.q_st;
+    s_at[tid][1] = b * a.k_sb + t * a.k_st;
+    s_at[tid][2] = b * a.H * a.T + t;
+    s_at[tid][3] = b * a.G * a.T + t;
   }
   __syncthreads();
-  const int qn = (a.H + kNR_Heads - 1) / kNR_Heads, kn = (a.G + kNR_Heads - 1) / kNR_Heads;
-  const int off = F >> 3;                                   // the partner's distance in lanes
-  const bool turned = 4 * lane < F, first = lane < off;     // 8 lane < 2 F
-  const int partner = turned ? (first ? lane + off : lane - off) : lane;
-  for (int it = warp; it < tokens * (qn + kn); it += 8) {
-    const int t = it / (qn + kn), j = it % (qn + kn);
+  // a warp's items: four heads of a token, j of the token's qn + kn groups of heads
+  const int qn = (a.H + kNR_Heads - 1) / kNR_Heads, per = qn + (a.G + kNR_Heads - 1) / kNR_Heads;
+  const bool turned = 4 * lane < F;
+  const int d0 = turned ? 4 * lane : F + 4 * lane, d1 = turned ? F + 4 * lane : 128 + 4 * lane;      // dims d0 .. d0 + 3 and d1 .. d1 + 3
+  uint2 raw[kNR_Heads][2];
+  auto load = [&](int t, int j) {
     const bool isq = j < qn;
-    const int h0 = (isq ? j : j - qn) * kNR_Heads, heads = isq ? a.H : a.G, m = min(kNR_Heads, heads - h0);
-    const long long n = n0 + t, b = n / a.T, tt = n % a.T;
-    const T* src = static_cast<const T*>(isq ? a.qg : a.kl) + b * (isq ? a.q_sb : a.k_sb) + tt * (isq ? a.q_st : a.k_st) + 8 * lane;
+    const int h0 = (isq ? j : j - qn) * kNR_Heads, m = (isq ? a.H : a.G) - h0;
     const long long sh = isq ? a.q_sh : a.k_sh;
-    uint4 raw[kNR_Heads];
+    const T* src = static_cast<const T*>(isq ? a.qg : a.kl) + s_at[t][isq ? 0 : 1] + h0 * sh;
 #pragma unroll
-    for (int i = 0; i < kNR_Heads; ++i) raw[i] = i < m ? __ldcs(reinterpret_cast<const uint4*>(src + (h0 + i) * sh)) : make_uint4(0u, 0u, 0u, 0u);
-    float2 cs[8];
-    if (turned) {
-      const float4* c = reinterpret_cast<const float4*>(&s_cs[t][8 * (first ? lane : lane - off)]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 x = c[e];
-        cs[2 * e] = make_float2(x.x, first ? -x.y : x.y);
-        cs[2 * e + 1] = make_float2(x.z, first ? -x.w : x.w);
+    for (int i = 0; i < kNR_Heads; ++i) {
+      raw[i][0] = raw[i][1] = make_uint2(0u, 0u);
+      if (i < m) {
+        raw[i][0] = __ldcs(reinterpret_cast<const uint2*>(src + d0));
+        raw[i][1] = __ldcs(reinterpret_cast<const uint2*>(src + d1));
       }
+      src += sh;
     }
+  };
+  int t = 0, j = warp;
+  auto settle = [&](int& t, int& j) {
+    while (j >= per) {
+      j -= per;
+      ++t;
+    }
+  };
+  settle(t, j);
+  if (t < tokens) load(t, j);
+  for (int i = tid; i < tokens * F; i += 256) {
+    const int k = i / F, f = i % F, ax = (a.axis[f >> 4] >> (2 * (f & 15))) & 3;
+    const long long at = ax * a.BT + n0 + k;
+    const double p = a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at] : (double)static_cast<const int32_t*>(a.pos)[at];
+    const double turns = p * (double)a.inv_freq[f] * 0.15915494309189535;
+    sincospif((float)(2. * (turns - rint(turns))), &s_sin[k][f], &s_cos[k][f]);
+  }
+  uint64_t wq[4], wk[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int d = (e < 2 ? d0 : d1) + 2 * (e & 1);
+    wq[e] = pair2(1.f + a.q_w[d], 1.f + a.q_w[d + 1]);
+    wk[e] = pair2(1.f + a.k_w[d], 1.f + a.k_w[d + 1]);
+  }
+  __syncthreads();
+  while (t < tokens) {
+    const bool isq = j < qn;
+    const int h0 = (isq ? j : j - qn) * kNR_Heads, heads = isq ? a.H : a.G, m = heads - h0, now_t = t;
+    uint2 now[kNR_Heads][2];
+#pragma unroll
+    for (int i = 0; i < kNR_Heads; ++i) {
+      now[i][0] = raw[i][0];
+      now[i][1] = raw[i][1];
+    }
+    j += 8;
+    settle(t, j);
+    if (t < tokens) load(t, j);
+    uint64_t c0 = pair2(1.f, 1.f), c1 = c0, s0 = 0, s1 = 0;
+    if (turned) {
+      const float4 c = *reinterpret_cast<const float4*>(&s_cos[now_t][4 * lane]), s = *reinterpret_cast<const float4*>(&s_sin[now_t][4 * lane]);
+      c0 = pair2(c.x, c.y);
+      c1 = pair2(c.z, c.w);
+      s0 = pair2(s.x, s.y);
+      s1 = pair2(s.z, s.w);
+    }
+    const uint64_t minus = pair2(-1.f, -1.f), n0_ = mul2(s0, minus), n1_ = mul2(s1, minus);
     float ss[kNR_Heads];
 #pragma unroll
     for (int i = 0; i < kNR_Heads; ++i) {
-      float x[8];
-      unpack8<T>(raw[i], x);
-      ss[i] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss[i] = fmaf(x[e], x[e], ss[i]);
+      uint64_t x = widen<T>(now[i][0].x), sum = mul2(x, x);
+      x = widen<T>(now[i][0].y), sum = fma2(x, x, sum);
+      x = widen<T>(now[i][1].x), sum = fma2(x, x, sum);
+      x = widen<T>(now[i][1].y), sum = fma2(x, x, sum);
+      ss[i] = lo_hi(sum, 0) + lo_hi(sum, 1);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
       for (int i = 0; i < kNR_Heads; ++i) ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
     T* plain = static_cast<T*>(isq ? a.q : a.k);
-    T* rot = static_cast<T*>(isq ? a.qr : a.kr);
+    if (plain) plain += ((n0 + now_t) * heads + h0) * kNR_D;
+    T* rot = static_cast<T*>(isq ? a.qr : a.kr) + (s_at[now_t][isq ? 2 : 3] + (long long)h0 * a.T) * kNR_D;
 #pragma unroll
     for (int i = 0; i < kNR_Heads; ++i) {
-      float x[8], o8[8];
-      unpack8<T>(raw[i], x);
       const float inv = rsqrtf(ss[i] * (1.f / kNR_D) + a.eps);
+      const uint64_t inv2 = pair2(inv, inv);
+      uint64_t y[4] = {widen<T>(now[i][0].x), widen<T>(now[i][0].y), widen<T>(now[i][1].x), widen<T>(now[i][1].y)};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (isq ? wq[e] : wk[e]);
-      if (plain && i < m) __stcs(reinterpret_cast<uint4*>(plain + (n * heads + h0 + i) * kNR_D) + lane, pack8<T>(x));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o8[e] = __shfl_sync(0xffffffffu, x[e], partner);
-      if (turned) {
-        // first half: x cos - partner sin, second: x cos + partner sin (the sign is in cs)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = fmaf(o8[e], cs[e].y, x[e] * cs[e].x);
+      for (int e = 0; e < 4; ++e) y[e] = mul2(mul2(y[e], inv2), isq ? wq[e] : wk[e]);
+      if (i < m) {
+        if (plain) {
+          __stcs(reinterpret_cast<uint2*>(plain + d0), make_uint2(narrow<T>(y[0]), narrow<T>(y[1])));
+          __stcs(reinterpret_cast<uint2*>(plain + d1), make_uint2(narrow<T>(y[2]), narrow<T>(y[3])));
+        }
+        __stcs(reinterpret_cast<uint2*>(rot + d0), make_uint2(narrow<T>(fma2(y[2], n0_, mul2(y[0], c0))), narrow<T>(fma2(y[3], n1_, mul2(y[1], c1)))));
+        __stcs(reinterpret_cast<uint2*>(rot + d1), make_uint2(narrow<T>(fma2(y[0], s0, mul2(y[2], c0))), narrow<T>(fma2(y[1], s1, mul2(y[3], c1)))));
       }
-      if (i < m) __stcs(reinterpret_cast<uint4*>(rot + ((b * heads + h0 + i) * a.T + tt) * kNR_D) + lane, pack8<T>(x));
+      if (plain) plain += kNR_D;
+      rot += (long long)a.T * kNR_D;
     }
   }
 }
