@@ -13,6 +13,7 @@ Public API (mirrors of the reference ``heimdall`` package):
   prompt_attention                   heimdall/hibrit.py:275-290 (a kept layer's causal attention, packed prompts)
   norm_rope_heads                    heimdall/hibrit.py:254-268 (_proj's norm and rotation, positions on several axes)
   PagedKV                            a kept layer's cache in 8-bit pages: append, attend, fork, free, compact
+  Adapters                           low-rank adapters of many requests beside a shared projection
   BifrostLayer.student               heimdall/hibrit.py:363-424 (HybridAttention._student)
   BifrostLayer.mem_inputs            heimdall/hibrit.py:327-334
   BifrostLayer.student_host          _student for host (pinned) inputs, copies overlapped with the layer
@@ -27,7 +28,9 @@ from .functional import delta_rule, delta_rule_gqa, delta_rule_step, delta_rule_
 from .functional import norm_rope_heads, prompt_attention, rope_axes, window_attention  # noqa: F401
 from .layer import BifrostLayer  # noqa: F401
 from .paged import PagedKV  # noqa: F401
+from .adapters import Adapters  # noqa: F401
 from .attention import BifrostAttention  # noqa: F401
 
 __all__ = ["delta_rule", "delta_rule_gqa", "delta_rule_step", "delta_rule_step_gqa", "window_attention",
-           "prompt_attention", "norm_rope_heads", "rope_axes", "BifrostLayer", "BifrostAttention", "PagedKV"]
+           "prompt_attention", "norm_rope_heads", "rope_axes", "BifrostLayer", "BifrostAttention", "PagedKV",
+           "Adapters"]

@@ -45,6 +45,8 @@ SIGNATURES = {
     "bf_attn_prologue": [_P, _P, _P, _P, _P, _I, ctypes.c_float, _L, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P],
     "bf_attn_epilogue": [_P, _P, _I, _I, _I, _I, _I, _P, _P],
     "bf_norm_rope": [_P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _I, _P, _I, _P, _I, ctypes.c_float] + [_I] * 6 + [_P] * 5,
+    "bf_adapter_workspace": [_I, _I, _I, _I],
+    "bf_adapter_add": [_P, _L, _P, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _L, _P, _L, _I, _P, _Z, _P],
     "bf_gdn_segment_workspace": [_I, _I, _I, _I],
     "bf_gdn_segment_transform": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P],
     "bf_gdn_apply_prefix": [_P, _P, _I, _P, _P, _I, _I, _I, _P],
@@ -72,7 +74,8 @@ _RESTYPE = {"bf_strerror": ctypes.c_char_p, "bf_last_cuda_error": ctypes.c_char_
             "bf_gdn_chunk_workspace": _Z, "bf_window_workspace": _Z, "bf_layer_prefill_workspace": _Z,
             "bf_layer_prefill_sp_workspace": _Z,
             "bf_gdn_segment_workspace": _Z, "bf_llama_state_floats": _Z,
-            "bf_ret_decode_workspace": _Z, "bf_paged_attend_workspace": _Z, "bf_gdn_bwd_workspace": _Z}
+            "bf_ret_decode_workspace": _Z, "bf_paged_attend_workspace": _Z, "bf_gdn_bwd_workspace": _Z,
+            "bf_adapter_workspace": _Z}
 
 _lock = threading.Lock()
 _lib = None

@@ -25,12 +25,13 @@ class BifrostAttention:
     ``k_w``/``v_w`` [G*D, d], ``o_w`` [d, H*D], optional biases, ``q_norm_w``/``k_norm_w`` [D] (zero-centred
     ZNorm weights), RoPE on the first ``rot`` dims with base ``theta``, norm ``eps``; ``layer`` the converted
     core (``BifrostLayer``).  ``mode``: "student" (window + memory) or "window" (the reference's memoryless mode).
-    ``rope_sections``: rotary frequencies per axis (time, height, width) for calls with ``positions`` on several axes.
+    ``rope_sections``: rotary frequencies per axis (time, height, width) for calls with ``positions`` on several axes.  ``adapters``: the
+    requests' low-rank adapters, {"q": Adapters, "k": ..., "v": ..., "o": ...} for any of the projections, for calls with ``adapter_ids``.
     """
 
     def __init__(self, q_w, k_w, v_w, o_w, q_norm_w, k_norm_w, layer: BifrostLayer, rot: int, theta: float,
                  eps: float = 1e-6, gated: bool = True, q_b=None, k_b=None, v_b=None, o_b=None, mode: str = "student",
-                 rope_sections=None):
+                 rope_sections=None, adapters=None):
         dev = layer.device
         bf = torch.bfloat16
         cvt = lambda t: None if t is None else t.detach().to(device=dev, dtype=bf).contiguous()
@@ -48,12 +49,17 @@ class BifrostAttention:
         if rope_sections is not None and sum(rope_sections) * 2 != self.rot:
             raise ValueError("rope_sections must add up to rot / 2 frequencies")
         self.axes = None if rope_sections is None else rope_axes(rope_sections)
+        self.adapters = dict(adapters or {})
+        for name, ad in self.adapters.items():
+            w = {"q": self.q_w, "k": self.k_w, "v": self.v_w, "o": self.o_w}.get(name)
+            if w is None or (ad.d_out, ad.d_in) != tuple(w.shape) or ad.dtype != bf or ad.device != w.device:
+                raise ValueError(f"the adapters of {name!r} do not match a projection of this layer (q, k, v or o, bf16, its shape and device)")
         # inverse RoPE frequencies exactly as the reference computes them (heimdall/kernels.py:44), in fp32
         d_rot = max(self.rot, 2)
         self.inv_freq = (1.0 / (self.theta ** (torch.arange(0, d_rot, 2, dtype=torch.float32) / d_rot))).to(dev)
 
     @classmethod
-    def from_module(cls, attn, device=None, rope_sections=None) -> "BifrostAttention":
+    def from_module(cls, attn, device=None, rope_sections=None, adapters=None) -> "BifrostAttention":
         """From a converted reference ``HybridAttention`` (its projections, norms, RoPE config and new parameters)."""
         c = attn.c
         layer = BifrostLayer.from_module(attn, device)
@@ -61,21 +67,32 @@ class BifrostAttention:
         return cls(attn.q_proj.weight, attn.k_proj.weight, attn.v_proj.weight, attn.o_proj.weight,
                    attn.q_norm.weight, attn.k_norm.weight, layer, c.rot, c.rope_theta, c.eps, c.gate,
                    bias(attn.q_proj), bias(attn.k_proj), bias(attn.v_proj), bias(attn.o_proj),
-                   mode="window" if attn.mode == "window" else "student", rope_sections=rope_sections)
+                   mode="window" if attn.mode == "window" else "student", rope_sections=rope_sections,
+                   adapters=adapters)
 
-    def project(self, x, start: int = 0, positions=None):
+    def _linear(self, name: str, x, ids):
+        """The projection ``name`` of x with its bias and, for calls with adapter ids [B] or [B,t], its adapters."""
+        y = F.linear(x, getattr(self, name + "_w"), getattr(self, name + "_b"))
+        if ids is None or name not in self.adapters:
+            return y
+        if ids.dim() == 1 and x.dim() == 3:
+            ids = ids[:, None].expand(x.shape[:2])
+        return self.adapters[name].add(y, x, ids, out=y)
+
+    def project(self, x, start: int = 0, positions=None, adapter_ids=None):
         """``HybridAttention._proj`` (heimdall/hibrit.py:254-268): x [B,t,d] -> (q, k, v, qr, kr, qg) with q
         [B,t,H,D], k/v [B,t,G,D] (ZNorm'd), qr [B,H,t,D], kr [B,G,t,D] (partial RoPE) in bf16, and qg the query
         projection [B,t,H,(2 if gated) D] holding the output gate.  ``positions`` (int [B,t], or [axes,B,t] with the layer's
-        ``rope_sections``): the rotation's positions of every token, in the place of start, start + 1, ... (``norm_rope_heads``)."""
+        ``rope_sections``): the rotation's positions of every token, in the place of start, start + 1, ... (``norm_rope_heads``).
+        ``adapter_ids`` (int [B] or [B,t]): each sequence's or token's adapter in the layer's ``adapters``; a number that names none: none."""
         check_cuda(x)
         L = self.layer
         B, t = x.shape[:2]
         H, G, D = L.H, L.G, L.D
         xb = x.to(torch.bfloat16)
-        qg = F.linear(xb, self.q_w, self.q_b).contiguous()
-        kl = F.linear(xb, self.k_w, self.k_b).contiguous()
-        v = F.linear(xb, self.v_w, self.v_b).view(B, t, G, D)
+        qg = self._linear("q", xb, adapter_ids).contiguous()
+        kl = self._linear("k", xb, adapter_ids).contiguous()
+        v = self._linear("v", xb, adapter_ids).view(B, t, G, D)
         if positions is not None:
             q, k, qr, kr = norm_rope_heads(qg.view(B, t, H, -1), kl.view(B, t, G, D), self.q_norm_w, self.k_norm_w, positions,
                                            self.inv_freq if self.rot else None, self.axes if positions.dim() == 3 else None, self.eps,
@@ -91,22 +108,24 @@ class BifrostAttention:
                   1 if self.gated else 0, ptr(q), ptr(k), ptr(qr), ptr(kr), stream_handle())
         return q, k, v.contiguous(), qr, kr, qg
 
-    def output(self, o, qg, x):
-        """``HybridAttention._out`` (heimdall/hibrit.py:270-272): o [B,t,H,D] fp32 -> o_proj(o * sigmoid(gate))."""
+    def output(self, o, qg, x, adapter_ids=None):
+        """``HybridAttention._out`` (heimdall/hibrit.py:270-272): o [B,t,H,D] fp32 -> o_proj(o * sigmoid(gate)), with the adapters of o_proj
+        for ``adapter_ids``."""
         L = self.layer
         B, t = x.shape[:2]
         y = torch.empty(B, t, L.H * L.D, device=x.device, dtype=torch.bfloat16)
         _lib.call("bf_attn_epilogue", ptr(o.contiguous()), ptr(qg), 1 if self.gated else 0, B, t, L.H, L.D, ptr(y),
                   stream_handle())
-        return F.linear(y, self.o_w, self.o_b)
+        return self._linear("o", y.view(B, t, L.H * L.D), adapter_ids)
 
-    def forward(self, x, cache=None, start: int = 0, positions=None):
+    def forward(self, x, cache=None, start: int = 0, positions=None, adapter_ids=None):
         """``HybridAttention.forward`` of a converted layer (heimdall/hibrit.py:426-432): x [B,t,d] -> [B,t,d] bf16,
         with the reference's cache dict (prefill for t > 1, the decode step for t == 1 with a cache).
-        ``positions`` turn the heads (``project``); the window and the memory go by the tokens' order, from ``start`` on."""
-        q, k, v, qr, kr, qg = self.project(x, start, positions)
+        ``positions`` turn the heads (``project``); the window and the memory go by the tokens' order, from ``start`` on.
+        ``adapter_ids``: the requests' adapters (``project``)."""
+        q, k, v, qr, kr, qg = self.project(x, start, positions, adapter_ids)
         o = self.layer.student(x, q, k, v, qr, kr, int(start), cache, memory=self.mode != "window")
         o = o.reshape(*x.shape[:2], self.layer.H, self.layer.D)
-        return self.output(o, qg, x)
+        return self.output(o, qg, x, adapter_ids)
 
     __call__ = forward
