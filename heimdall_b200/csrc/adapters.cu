@@ -9,12 +9,13 @@
 // Tokens are taken in groups of one adapter, so that an adapter is read once for many tokens:
 //   * few tokens (up to kAD_Few, a decode step): every token stands for a possible group of 16; a CTA compares all ids with its token's
 //     and goes on if its token is the first of a group.  No pass over the ids before, two launches.
-//   * more: adapter_route_kernel sorts the tokens by adapter and lists groups of 64.
-// h = A x is split over d_in so that every SM has work; each split's sums are written on their own and added in order.  h enters the second
-// product as two 16-bit parts of its row's power-of-two scale (hi + lo, 16 bits of bf16, 22 of fp16), so that the only rounding of consequence
-// is that of out.  The order of a group's tokens, which the sort leaves to chance, has no part in their values.
-// The products run on mma.sync: the first has 8 r FLOPs for the 2 bytes of an x value, the second 16 r for the 4 bytes of a y and an out, which
-// its rate covers up to r = 64, and its fragments come from registers (weights) or shared memory without a layout change.
+//   * more: adapter_route_kernel sorts the tokens by adapter and lists groups of 128, one M = 128 tile of the tensor core (tcgen05).
+// h = A x is split over d_in so that every SM has work; each split's sums are written on their own and added in order.  For many tokens h enters the
+// second product as two 16-bit parts of its row's power-of-two scale (hi + lo, 16 bits of bf16, 22 of fp16), so that the only rounding of
+// consequence is that of out; for few it stays fp32.  The order of a group's tokens, which the sort leaves to chance, has no part in
+// their values.
+// (With mma.sync in the place of tcgen05 both kernels of many tokens were bound by its rate, about 32 cycles per m16n8k16 and scheduler:
+// 25480 tokens 6144 -> 5120, rank 64: 148 + 324 us.)
 #include "capi_internal.h"
 #include "common.cuh"
 #include "launch_early.h"
@@ -25,7 +26,7 @@ constexpr int kAD_Few = 256;       // tokens up to which every CTA looks for its
 constexpr int kAD_MaxRank = 128;
 constexpr int kAD_MaxAdapters = 4096;
 constexpr int kAD_KFew = 1024;     // d_in per CTA for few tokens
-constexpr int kAD_Group = 64;      // tokens per group of many
+constexpr int kAD_Group = 128;     // tokens per group of many: the M of a tcgen05 product
 
 struct AdapterArgs {
   const void *x, *y;
@@ -36,11 +37,17 @@ struct AdapterArgs {
   const float* scale;              // [n]
   const void *A, *B;               // A [row[n]][d_in]; B: adapter a's [d_out][r_a] from element row[a] d_out on
   int n, T, d_in, d_out, rmax, splits, kper, units;
+  unsigned int* err;
   float* h;                        // [splits][T][rmax]
   int32_t* perm;                   // [T] tokens by adapter
   int4* groups;                    // (adapter or n, first of perm, tokens, -)
   int32_t* n_groups;
 };
+
+template <typename T>
+constexpr int kIsBf16 = 0;
+template <>
+constexpr int kIsBf16<__nv_bfloat16> = 1;
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
@@ -54,13 +61,10 @@ __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uin
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {      // 16 bytes into shared memory, zeros where there are none
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ uint4 ldg_stream(const uint4* p) { return __ldcs(p); }
+__device__ __forceinline__ uint4 ldg_stream(const uint4* p) { return __ldcs(p); }      // read once
 
 // an adapter's number, n for none
 __device__ __forceinline__ int adapter_of(const AdapterArgs& a, int id) { return id >= 0 && id < a.n ? id : a.n; }
@@ -137,36 +141,55 @@ __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(AdapterArgs a) 
   }
 }
 
-// The sorted list of many tokens and their groups, by one CTA.  A thread takes consecutive tokens, whose adapters come in runs, and
-// counts whole runs.
+// The sorted list of many tokens and their groups, by one CTA.  The adapters' numbers go through shared memory, so that a thread can take
+// consecutive tokens, whose adapters come in runs, and count whole runs; a warp whose tokens are all of one adapter counts at once.  (With
+// each thread reading and writing its own tokens in global memory, 25480 tokens took 26 us.)
+constexpr int kAD_RoutePer = 32;                                        // tokens per thread at a time, at most
+constexpr int kAD_RouteIds = 1024 * (kAD_RoutePer + 2) * 2;              // bytes of their adapters' numbers, two more per thread against bank conflicts
 __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   extern __shared__ int s_dyn[];
   int* s_at = s_dyn;                  // [n + 2] count, then first place in perm of each adapter (n: none)
   int* s_grp = s_dyn + a.n + 2;       // [n + 2] first group
+  uint16_t* s_id = reinterpret_cast<uint16_t*>(s_dyn + 2 * (a.n + 2));
   __shared__ int2 s_warp[32];
+  __shared__ int s_base[1024];
   wait_for_stream();
   let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, buckets = a.n + 1;
   for (int i = tid; i < buckets + 1; i += 1024) s_at[i] = 0;
-  __syncthreads();
-  const int per = min((a.T + 1023) / 1024, 32);
-  auto runs = [&](auto&& done) {
-    for (int t0 = 0; t0 < a.T; t0 += 1024 * per) {
-      const int first = t0 + tid * per, n = min(per, a.T - first);
-      int v[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = i < n ? adapter_of(a, __ldg(a.ids + first + i)) : -1;
-      int begin = 0;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (i < n && (i + 1 == n || v[i + 1 < 32 ? i + 1 : 31] != v[i])) {
-          done(v[i], first + begin, i + 1 - begin);
+  const int per = min((a.T + 1023) / 1024, kAD_RoutePer);
+  auto load = [&](int t0) {
+    const int n = min(a.T - t0, 1024 * per);
+    __syncthreads();
+    for (int i = tid; i < n; i += 1024) s_id[i / per * (kAD_RoutePer + 2) + i % per] = (uint16_t)adapter_of(a, __ldg(a.ids + t0 + i));
+    __syncthreads();
+  };
+  const uint16_t* mine_id = s_id + tid * (kAD_RoutePer + 2);
+  // this thread's tokens: how many, and whether the warp's are all of one adapter
+  auto whole = [&](int t0, int& n) {
+    n = max(0, min(per, a.T - t0 - tid * per));
+    const int first = n > 0 ? mine_id[0] : -1, of_warp = __shfl_sync(0xffffffffu, first, 0);
+    bool same = n > 0 && first == of_warp;
+    for (int i = 1; i < n; ++i) same = same && mine_id[i] == first;
+    return __all_sync(0xffffffffu, same) ? of_warp : -1;
+  };
+  auto warp_total = [&](int n) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)n); };
+  for (int t0 = 0; t0 < a.T; t0 += 1024 * per) {
+    load(t0);
+    int n;
+    const int one = whole(t0, n);
+    if (one >= 0) {
+      const int sum = warp_total(n);
+      if (lane == 0) atomicAdd(&s_at[one], sum);
+    } else {
+      for (int i = 0, begin = 0; i < n; ++i) {
+        if (i + 1 == n || mine_id[i + 1] != mine_id[i]) {
+          atomicAdd(&s_at[mine_id[i]], i + 1 - begin);
           begin = i + 1;
         }
       }
     }
-  };
-  runs([&](int b, int, int n) { atomicAdd(&s_at[b], n); });
+  }
   __syncthreads();
   // both running sums over the adapters, thread i holding `each` of them
   const int each = (buckets + 1023) / 1024, lo = min(tid * each, buckets), hi = min(lo + each, buckets);
@@ -215,234 +238,434 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   }
   if (tid == 0) *a.n_groups = total;
   __syncthreads();
-  runs([&](int b, int first, int n) {
-    const int to = atomicAdd(&s_at[b], n);
-    for (int i = 0; i < n; ++i) a.perm[to + i] = first + i;
-  });
+  for (int t0 = 0; t0 < a.T; t0 += 1024 * per) {
+    if (a.T > 1024 * per) load(t0);
+    int n;
+    const int one = whole(t0, n);
+    int base = -1;
+    if (one >= 0) {
+      const int sum = warp_total(n);
+      if (lane == 0) base = atomicAdd(&s_at[one], sum);
+      base = __shfl_sync(0xffffffffu, base, 0) + lane * per;      // only the last lane with tokens can have fewer
+    } else {
+      const int first = t0 + tid * per;
+      for (int i = 0, begin = 0; i < n; ++i) {
+        if (i + 1 == n || mine_id[i + 1] != mine_id[i]) {
+          const int to = atomicAdd(&s_at[mine_id[i]], i + 1 - begin);
+          for (int j = begin; j <= i; ++j) a.perm[to + j - begin] = first + j;
+          begin = i + 1;
+        }
+      }
+    }
+    s_base[tid] = base;
+    __syncthreads();
+    // the tokens of whole warps, in their order
+    for (int i = tid; i < min(a.T - t0, 1024 * per); i += 1024) {
+      const int to = s_base[i / per];
+      if (to >= 0) a.perm[to + i % per] = t0 + i;
+    }
+  }
 }
 
-// h of a group of 64 tokens: CTA = (group, part of d_in); x rows and A rows come 64 values at a time through a ring in shared memory
-// (rows of 128 bytes, 16-byte pieces at (piece ^ row)); warps 0 - 3 take 16 tokens and the first half of the 64 values, warps 4 - 7
-// the second, added at the end.
+// h of a group of 128 tokens: CTA = (group, part of d_in).  x rows (gathered) and A rows come 64 values at a time through a ring in shared memory
+// (K-major, 128-byte swizzle), all threads copying; one thread issues the products of a stage, D in TMEM is the group's h.
 template <typename T, int RM, int ST>
 __global__ void __launch_bounds__(256) adapter_shrink_kernel(AdapterArgs a) {
-  constexpr int kStage = (kAD_Group + RM) * 128;
-  extern __shared__ __align__(128) uint8_t s_ring[];
+  constexpr int kStage = (kAD_Group + RM) * 128, kCols = RM < 32 ? 32 : RM;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int s_tok[kAD_Group];
+  __shared__ uint64_t s_bar[ST];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  volatile int* abort = &s_abort;
   wait_for_stream();
   let_next_start();
   if ((int)blockIdx.x >= *a.n_groups) return;
   const int4 grp = a.groups[blockIdx.x];
   if (grp.x == a.n) return;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3, m = grp.z;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, m = grp.z;
   const int r0 = a.row[grp.x], rank = a.row[grp.x + 1] - r0;
   if (tid < kAD_Group) s_tok[tid] = a.perm[grp.y + min(tid, m - 1)];
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(s_bar + i, 1);
+    s_abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&s_tmem, kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
   __syncthreads();
-  const int k0 = blockIdx.y * a.kper, k1 = min(k0 + a.kper, a.d_in), steps = (k1 - k0 + 63) / 64;
-  const uint32_t ring = smem_u32(s_ring);
-  // a thread's pieces: piece tid & 7 of rows tid / 8 + 32 i, x rows first
+  tc_fence_after();
+  const uint32_t tmem = s_tmem, ring_at = smem_u32(ring);
+  const int k0 = blockIdx.y * a.kper, k1 = min(k0 + a.kper, a.d_in), stages = (k1 - k0 + 63) / 64;
+  // a thread's pieces of 16 bytes: piece tid % 8 of the rows tid / 8 + 32 i, x rows first.  Rows of tokens that are not there repeat the last one
   const int piece = tid & 7, prow = tid >> 3;
-  const T* src[2 + RM / 32];
+  const T* src[(kAD_Group + RM) / 32];
 #pragma unroll
-  for (int i = 0; i < 2 + RM / 32; ++i) {
+  for (int i = 0; i < (kAD_Group + RM) / 32; ++i) {
     const int r = prow + 32 * i;
-    src[i] = (i < 2 ? static_cast<const T*>(a.x) + (long long)s_tok[r] * a.x_st
-                    : static_cast<const T*>(a.A) + (long long)(r0 + min(r - kAD_Group, rank - 1)) * a.d_in) + 8 * piece;
+    src[i] = (r < kAD_Group ? static_cast<const T*>(a.x) + (long long)s_tok[r] * a.x_st
+                            : static_cast<const T*>(a.A) + (long long)(r0 + min(r - kAD_Group, rank - 1)) * a.d_in) + 8 * piece;
   }
   auto fetch = [&](int s) {
-    if (s < steps) {
+    if (s < stages) {
       const int k = k0 + 64 * s;
       const bool in = k + 8 * piece < k1;
-      const uint32_t dst = ring + (s % ST) * kStage;
+      const uint32_t dst = ring_at + (s % ST) * kStage + prow * 128 + ((piece ^ (prow & 7)) << 4);
 #pragma unroll
-      for (int i = 0; i < 2 + RM / 32; ++i) {
-        const int r = prow + 32 * i;
-        if (i < 2 ? r < m : r - kAD_Group < rank) copy16(dst + r * 128 + ((piece ^ (r & 7)) << 4), in ? src[i] + k : src[i], in);
-      }
+      for (int i = 0; i < (kAD_Group + RM) / 32; ++i)
+        if (32 * i + prow < kAD_Group + rank) copy16(dst + i * 4096, in ? src[i] + k : src[i], in);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // rows of tokens that are not there: zeros, once (their products are not written, but may not be read uninitialised)
-  for (int i = tid; i < (kAD_Group - m) * 8 * ST; i += 256) {
-    const int s = i / ((kAD_Group - m) * 8), j = i % ((kAD_Group - m) * 8);
-    *reinterpret_cast<uint4*>(s_ring + s * kStage + m * 128 + j * 16) = make_uint4(0u, 0u, 0u, 0u);
-  }
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) fetch(s);
-  float acc[RM / 8][4] = {};
-  const int wr = (warp & 3) * 16, half = warp >> 2;
-  for (int s = 0; s < steps; ++s) {
+  const uint32_t idesc = idesc_f16(128, rank, kIsBf16<T>);
+  bool ok = true;
+  for (int s = 0; s < stages && ok; ++s) {
     asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+    fence_async_smem();
     __syncthreads();
+    if (tid == 0) {
+      tc_fence_after();
+      const uint32_t xs = ring_at + (s % ST) * kStage;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        umma_f16_ss(tmem, sdesc_sw128(xs + ks * 32), sdesc_sw128(xs + kAD_Group * 128 + ks * 32), idesc, s > 0 || ks > 0);
+      umma_commit(s_bar + s % ST);
+    }
+    // stage s + ST - 1 takes the place of s - 1, whose products were issued a stage ago
+    if (s > 0 && s + ST - 1 < stages) ok = mbar_wait_small(s_bar + (s - 1) % ST, ((s - 1) / ST) & 1, abort, 0x80);
     fetch(s + ST - 1);
-    const uint32_t xs = ring + (s % ST) * kStage, ws = xs + kAD_Group * 128;
+  }
+  ok = ok && mbar_wait_small(s_bar + (stages - 1) % ST, ((stages - 1) / ST) & 1, abort, 0x81);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  ok = __all_sync(0xffffffffu, ok) != 0;
+  tc_fence_after();
+  if (warp < 4 && ok) {
+    const int r = 32 * warp + lane;
+    float* to = a.h + ((size_t)blockIdx.y * a.T + s_tok[r]) * a.rmax;
+#pragma unroll 1
+    for (int c = 0; c < rank; c += 16) {
+      uint32_t v[16];
+      tmem_ld16(tmem + ((uint32_t)(32 * warp) << 16) + c, v);
+      tmem_wait_ld();
+      if (r < m) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const int p = half * 4 + ks * 2;           // the 16-byte piece at which these 16 values begin
-      uint32_t x[4];
-      const int xr = wr + (lane & 15);
-      ldsm4(x, xs + xr * 128 + (((p + (lane >> 4)) ^ (xr & 7)) << 4));
-#pragma unroll
-      for (int j = 0; j < RM / 16; ++j) {
-        if (16 * j < rank) {
-          uint32_t w[4];
-          const int r = 16 * j + (lane & 7) + ((lane >> 4) << 3);
-          ldsm4(w, ws + r * 128 + (((p + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
-          mma16816<T>(acc[2 * j], x[0], x[1], x[2], x[3], w[0], w[1]);
-          mma16816<T>(acc[2 * j + 1], x[0], x[1], x[2], x[3], w[2], w[3]);
-        }
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(to + c)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       }
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  tc_fence_before();
   __syncthreads();
-  float* s_half = reinterpret_cast<float*>(s_ring);      // [64][RM + 2]
-  if (half) {
-#pragma unroll
-    for (int j = 0; j < RM / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<float2*>(s_half + (wr + g + 8 * e) * (RM + 2) + 8 * j + 2 * c) = make_float2(acc[j][2 * e], acc[j][2 * e + 1]);
+  if (tid == 0) report_abort(abort, a.err);
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kCols);
   }
-  __syncthreads();
-  if (!half) {
+}
+
+// out of a few tokens: CTA = (group, `units` times 512 columns).  A lane has two columns, whose rows of B (r values) it loads whole, 16 bytes at a
+// time and the next 16 ranks ahead, and up to four of the group's tokens: with one token per adapter most of a tensor-core tile would be empty, and
+// fp32 products of up to 16 tokens cost no more than mma.sync of two parts.
+template <typename T, int M>       // M: 1 or 4 tokens at most
+__device__ __forceinline__ void expand_few(const AdapterArgs& a, const T* w, int rank, int m, const int* s_tok, const float* s_h, float scale, int col0,
+                                           int units) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int u = 0; u < units; ++u) {
+    const int col = col0 + 512 * u + 2 * lane;
+    if (col >= a.d_out) return;
+    uint32_t y[M];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = wr + g + 8 * e;
-      if (r >= m) continue;
-      float* to = a.h + ((size_t)blockIdx.y * a.T + s_tok[r]) * a.rmax;
+    for (int t = 0; t < M; ++t)
+      if (t < m) y[t] = __ldcs(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.y) + (long long)s_tok[t] * a.y_st + col));
+    uint64_t acc[M][2];
 #pragma unroll
-      for (int j = 0; j < RM / 8; ++j) {
-        if (8 * j >= rank) break;
-        const float2 o = *reinterpret_cast<const float2*>(s_half + r * (RM + 2) + 8 * j + 2 * c);
-        *reinterpret_cast<float2*>(to + 8 * j + 2 * c) = make_float2(acc[j][2 * e] + o.x, acc[j][2 * e + 1] + o.y);
+    for (int t = 0; t < M; ++t) acc[t][0] = acc[t][1] = 0;
+    const uint4* p = reinterpret_cast<const uint4*>(w + (long long)col * rank);
+    const uint4* q = reinterpret_cast<const uint4*>(w + (long long)(col + 1) * rank);
+    uint4 b[4] = {ldg_stream(p), ldg_stream(p + 1), ldg_stream(q), ldg_stream(q + 1)};
+#pragma unroll 1
+    for (int r = 0; r < rank; r += 16) {
+      uint4 now[4] = {b[0], b[1], b[2], b[3]};
+      if (r + 16 < rank) {
+        p += 2;
+        q += 2;
+        b[0] = ldg_stream(p), b[1] = ldg_stream(p + 1), b[2] = ldg_stream(q), b[3] = ldg_stream(q + 1);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint64_t wf[2][4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const T* e = reinterpret_cast<const T*>(&now[2 * k + i]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) wf[k][x] = pair2((float)e[2 * x], (float)e[2 * x + 1]);
+        }
+#pragma unroll
+        for (int t = 0; t < M; ++t) {
+          if (t < m) {
+            const ulonglong2* h = reinterpret_cast<const ulonglong2*>(s_h + t * kAD_MaxRank + r + 8 * i);
+            const ulonglong2 h0 = h[0], h1 = h[1];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              acc[t][k] = fma2(wf[k][3], h1.y, fma2(wf[k][2], h1.x, fma2(wf[k][1], h0.y, fma2(wf[k][0], h0.x, acc[t][k]))));
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < M; ++t) {
+      if (t < m) {
+        T* e = reinterpret_cast<T*>(&y[t]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) e[k] = (T)fmaf(lo_hi(acc[t][k], 0) + lo_hi(acc[t][k], 1), scale, (float)e[k]);
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (long long)s_tok[t] * a.o_st + col) = y[t];
       }
     }
   }
 }
 
-// out of a group: CTA = (group, `units` times 256 columns), a warp 32 columns at a time.  B's fragments come straight from memory: in step
-// ks lane (g, c) loads the 8 bytes of ranks 16 ks + 4 c .. + 3 of the columns that it stands for, and reads the same ranks of h's rows g and
-// g + 8.  Column n of product j is column 8 (n / 2) + 2 j + n % 2 of the 32, so that a lane ends with 8 consecutive columns of two
-// rows: 16-byte accesses to y and out.
-template <typename T, int GT>      // GT: 16 (few tokens) or 64 tokens per group
-__global__ void __launch_bounds__(256) adapter_expand_kernel(AdapterArgs a) {
-  constexpr int KS = 4;            // steps of 16 ranks whose weights stay in registers
-  constexpr int kRow = kAD_MaxRank * 4 + 32;       // bytes: hi and lo parts of a row of h; 32 more spread the rows over the banks
-  extern __shared__ __align__(16) uint8_t s_h[];
-  __shared__ int s_tok[GT];
-  __shared__ float s_scale[GT];
+template <typename T>
+__global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs a) {
+  __shared__ __align__(16) float s_h[16 * kAD_MaxRank];
+  __shared__ int s_tok[16];
   __shared__ unsigned s_mask[8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  let_next_start();
+  int id;
+  // the ids are older than the kernel before this one, which began by waiting for what was before it
+  const int m = few_group(a, blockIdx.x, s_tok, s_mask, id);
+  if (m == 0 || (id == a.n && a.out == a.y)) return;
+  const int col0 = blockIdx.y * a.units * 512 + warp * 64;
+  if (id == a.n) {
+    wait_for_stream();
+    for (int u = 0; u < a.units; ++u) {
+      const int col = col0 + 512 * u + 2 * lane;
+      if (col >= a.d_out) break;
+      for (int t = 0; t < m; ++t)
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (long long)s_tok[t] * a.o_st + col) =
+            *reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.y) + (long long)s_tok[t] * a.y_st + col);
+    }
+    return;
+  }
+  const int r0 = a.row[id], rank = a.row[id + 1] - r0;
+  const float scale = a.scale[id];
+  const T* w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
+  // the CTA's weights on their way to L2
+  for (int u = 0; u < a.units; ++u) {
+    const int col = col0 + 512 * u + 2 * lane;
+    if (col < a.d_out)
+      for (int r = 0; r < 2 * rank; r += 64) prefetch_l2(w + (long long)col * rank + r);
+  }
+  wait_for_stream();
+  for (int i = tid; i < m * rank; i += 256) {
+    const int t = i / rank, r = i - t * rank;
+    float v = 0.f;
+    for (int s = 0; s < a.splits; ++s) v += a.h[((size_t)s * a.T + s_tok[t]) * a.rmax + r];
+    s_h[t * kAD_MaxRank + r] = v;
+  }
+  __syncthreads();
+  if (m == 1) expand_few<T, 1>(a, w, rank, 1, s_tok, s_h, scale, col0, a.units);
+  else
+    for (int t = 0; t < m; t += 4) expand_few<T, 4>(a, w, rank, min(4, m - t), s_tok + t, s_h + t * kAD_MaxRank, scale, col0, a.units);
+}
+
+// out of a group of 128 tokens: CTA = (group, `units` tiles of 128 columns).  h's two parts are made once in shared memory (A operand, K-major); the tiles'
+// rows of B (N operand) come through a ring of three, D alternates between two halves of 256 TMEM columns, and the next tile's y is in
+// registers while this one's sums leave TMEM.  TMEM is read 16 lanes by 64 columns at a time, where a thread has two columns of every eight: the
+// rows of B are dealt so that column n = 8 k + 2 c + e of such a block is column 16 c + 2 k + e of y, and a thread ends with 16 consecutive
+// columns of a row, four threads with 128 bytes.
+constexpr int kAD_Tile = 128;
+template <typename T, int RM>
+struct ExpandCfg {
+  static constexpr int Atoms = RM <= 64 ? 1 : 2;                  // of 64 ranks
+  static constexpr int HBytes = 2 * Atoms * kAD_Group * 128, BBytes = Atoms * kAD_Tile * 128, Ring = 3;
+  static constexpr int Smem = HBytes + Ring * BBytes + 1024;
+};
+
+template <typename T, int RM>
+__global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(AdapterArgs a) {
+  using C = ExpandCfg<T, RM>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* s_h = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ int s_tok[kAD_Group];
+  __shared__ float s_scale[kAD_Group];
+  __shared__ uint64_t s_bar[2];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  volatile int* abort = &s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   let_next_start();
-  int m, id;
-  // the ids and groups are older than the kernel before this one, which began by waiting for what was before it
-  if constexpr (GT == 16) {
-    m = few_group(a, blockIdx.x, s_tok, s_mask, id);
-    if (m == 0) return;
-  } else {
-    if ((int)blockIdx.x >= *a.n_groups) return;
-    const int4 grp = a.groups[blockIdx.x];
-    id = grp.x;
-    m = grp.z;
-    if (tid < m) s_tok[tid] = a.perm[grp.y + tid];
-  }
+  // the groups are older than the kernel before this one, which began by waiting for what was before it
+  if ((int)blockIdx.x >= *a.n_groups) return;
+  const int4 grp = a.groups[blockIdx.x];
+  const int id = grp.x, m = grp.z;
   if (id == a.n && a.out == a.y) return;
-  const int r0 = id < a.n ? a.row[id] : 0, rank = id < a.n ? a.row[id + 1] - r0 : 0;
+  if (tid < m) s_tok[tid] = a.perm[grp.y + tid];
+  if (tid == 0) {
+    mbar_init(s_bar, 1);
+    mbar_init(s_bar + 1, 1);
+    s_abort = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  const int r0 = id < a.n ? a.row[id] : 0, rank = id < a.n ? a.row[id + 1] - r0 : 0, steps = rank / 16;
+  const int col0 = blockIdx.y * a.units * kAD_Tile, tiles = min(a.units, (a.d_out - col0 + kAD_Tile - 1) / kAD_Tile);
   const T* w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
-  const int col0 = blockIdx.y * a.units * 256 + warp * 32, steps = rank / 16;
-  uint2 b[KS][4];
-  auto weights = [&](int cu, int k0) {
+  const uint32_t hs = smem_u32(s_h), bs = hs + C::HBytes;
+  // B's rows of a tile: row n of the operand is column 64 (n / 64) + 16 c + 2 k + e of the tile, n % 64 = 8 k + 2 c + e
+  const int pieces = rank / 8;             // of 16 bytes in a row: two threads to a row, each every second piece
+  const int brow = tid >> 1, bcol = (brow & 64) + 16 * ((brow >> 1) & 3) + 2 * ((brow >> 3) & 7) + (brow & 1);
+  auto fetch = [&](int j) {
+    if (j < tiles) {
+      const int col = col0 + j * kAD_Tile + bcol;
+      const bool in = col < a.d_out;
+      const T* src = w + (long long)(in ? col : 0) * rank;
+      const uint32_t dst = bs + (j % C::Ring) * C::BBytes + brow * 128;
+      for (int p = tid & 1; p < pieces; p += 2) copy16(dst + (p >> 3) * (kAD_Tile * 128) + (((p & 7) ^ (brow & 7)) << 4), src + 8 * p, in);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // a thread's part of y: rows 32 (warp % 4) + 16 i + 8 e + g, columns 64 (warp / 4) + 16 c .. + 15
+  const int wr = 32 * (warp & 3), wc = 64 * (warp >> 2) + 16 * c;
+  uint4 yv[2][2][2], y_next[2][2][2];
+  auto load_y = [&](int j) {
+    const int col = col0 + j * kAD_Tile + wc;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int col = cu + 8 * (g >> 1) + 2 * j + (g & 1);
-        b[ks][j] = k0 + ks < steps && col < a.d_out ? __ldg(reinterpret_cast<const uint2*>(w + (long long)col * rank + 16 * (k0 + ks) + 4 * c))
-                                                    : make_uint2(0u, 0u);
+      for (int e = 0; e < 2; ++e) {
+        const int r = wr + 16 * i + 8 * e + g;
+        if (j < tiles && r < m) {
+          const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + (long long)s_tok[r] * a.y_st + col);
+          if (col < a.d_out) y_next[i][e][0] = ldg_stream(p);
+          if (col + 8 < a.d_out) y_next[i][e][1] = ldg_stream(p + 1);
+        }
       }
   };
-  weights(col0, 0);
+  fetch(0);
+  fetch(1);
+  load_y(0);
   wait_for_stream();
-  __syncthreads();
+  if (warp == 0 && rank) {
+    tmem_alloc(&s_tmem, 256);
+    tmem_relinquish();
+  }
   if (rank) {
-    for (int r = warp; r < GT; r += 8) {
-      float v[kAD_MaxRank / 32];
+    // a warp a row: lane l the ranks 2 l, 2 l + 1 (and 64 more)
+    for (int r = warp; r < kAD_Group; r += 8) {
+      float2 v[C::Atoms];
       float big = 0.f;
 #pragma unroll
-      for (int i = 0; i < kAD_MaxRank / 32; ++i) {
-        v[i] = 0.f;
-        if (r < m && 32 * i + lane < rank)
-          for (int s = 0; s < a.splits; ++s) v[i] += a.h[((size_t)s * a.T + s_tok[r]) * a.rmax + 32 * i + lane];
-        big = fmaxf(big, fabsf(v[i]));
+      for (int i = 0; i < C::Atoms; ++i) {
+        v[i] = make_float2(0.f, 0.f);
+        if (r < m && 64 * i + 2 * lane < rank)
+          for (int s = 0; s < a.splits; ++s) {
+            const float2 x = *reinterpret_cast<const float2*>(a.h + ((size_t)s * a.T + s_tok[r]) * a.rmax + 64 * i + 2 * lane);
+            v[i].x += x.x;
+            v[i].y += x.y;
+          }
+        // (a NaN is no maximum, but its row becomes NaN by itself)
+        big = fmaxf(big, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
       }
       big = warp_max(big);
       // a power of two that takes the row's largest to [2^13, 2^14): both parts then keep all of their bits in fp16 too
       const int ex = big > 0.f && big < INFINITY ? min(max((int)(__float_as_uint(big) >> 23), 14), 253) : 140;
       const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-      T* hi = reinterpret_cast<T*>(s_h + r * kRow);
 #pragma unroll
-      for (int i = 0; i < kAD_MaxRank / 32; ++i) {
-        if (32 * i + lane < rank) {
-          const float z = v[i] * up;
-          const T p = (T)z;
-          hi[32 * i + lane] = p;
-          hi[rank + 32 * i + lane] = (T)(z - (float)p);
-        }
+      for (int i = 0; i < C::Atoms; ++i) {
+        const float x = v[i].x * up, y = v[i].y * up;
+        const T hi[2] = {(T)x, (T)y}, lo[2] = {(T)(x - (float)hi[0]), (T)(y - (float)hi[1])};
+        uint8_t* to = s_h + i * (kAD_Group * 128) + sw128_offset(r, 2 * lane);
+        *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(hi);
+        *reinterpret_cast<uint32_t*>(to + C::HBytes / 2) = *reinterpret_cast<const uint32_t*>(lo);
       }
-      if (lane == 0) s_scale[r] = id < a.n ? a.scale[id] * __uint_as_float((uint32_t)(ex - 13) << 23) : 0.f;
+      if (lane == 0) s_scale[r] = a.scale[id] * __uint_as_float((uint32_t)(ex - 13) << 23);
     }
   }
-  __syncthreads();
-  for (int u = 0; u < a.units; ++u) {
-    const int cu = col0 + u * 256;
-    if (cu >= a.d_out) break;
-    if (u && steps <= KS) weights(cu, 0);
-    const bool in = cu + 8 * c < a.d_out;
+  const uint32_t idesc = idesc_f16(128, kAD_Tile, kIsBf16<T>);
+  uint32_t tmem = 0;
+  auto products = [&](int j) {             // by one thread
+    tc_fence_after();
+    const uint32_t b = bs + (j % C::Ring) * C::BBytes;
 #pragma unroll 1
-    for (int rt = 0; rt < GT && rt < m; rt += 16) {
-      uint4 yv[2];
-      long long at[2];
+    for (int part = 0; part < 2; ++part)
+#pragma unroll 1
+      for (int ks = 0; ks < steps; ++ks) {
+        const uint32_t k = (ks >> 2) * (128 * 128) + (ks & 3) * 32;      // both operands have 128 rows
+        umma_f16_ss(tmem + (j & 1) * kAD_Tile, sdesc_sw128(hs + part * (C::HBytes / 2) + k), sdesc_sw128(b + k), idesc, part > 0 || ks > 0);
+      }
+    umma_commit(s_bar + (j & 1));
+  };
+  bool ok = true;
+#pragma unroll 1
+  for (int j = -1; j < tiles && ok; ++j) {
+    // tile j + 1's rows of B have landed, everybody is done with tile j - 1
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    if (j < 0 && rank) {
+      tc_fence_after();
+      tmem = s_tmem;
+    }
+    if (tid == 0 && rank && j + 1 < tiles) products(j + 1);
+    if (j < 0) {
+      fetch(2);
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) yv[i][e][q] = y_next[i][e][q];
+    load_y(j + 1);
+    if (rank) {
+      ok = mbar_wait_warp_small(s_bar + (j & 1), (j >> 1) & 1, abort, 0x82);
+      if (!ok) break;
+      tc_fence_after();
+    }
+    fetch(j + 3);          // in the place of tile j, whose products are done
+    const int col = col0 + j * kAD_Tile + wc;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (wr + 16 * i >= m) break;
+      uint32_t d[32];
+      if (rank) {
+        tmem_ld_16x256b_x8(tmem + (j & 1) * kAD_Tile + 64 * (warp >> 2) + ((uint32_t)(wr + 16 * i) << 16), d);
+        tmem_wait_ld();
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = rt + g + 8 * e;
-        if (r < m && in) {
-          yv[e] = ldg_stream(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + (long long)s_tok[r] * a.y_st + cu + 8 * c));
-          at[e] = (long long)s_tok[r] * a.o_st + cu + 8 * c;
+        const int r = wr + 16 * i + 8 * e + g;
+        if (r >= m) continue;
+        if (rank) {
+          const float sc = s_scale[r];
+          T* v = reinterpret_cast<T*>(yv[i][e]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) v[2 * k + q] = (T)fmaf(__uint_as_float(d[4 * k + 2 * e + q]), sc, (float)v[2 * k + q]);
         }
-      }
-      float acc[4][4] = {};
-      for (int k0 = 0; k0 < steps; k0 += KS) {
-        if (steps > KS) weights(cu, k0);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          if (k0 + ks < steps) {
-            const uint8_t* p0 = s_h + (rt + g) * kRow + (16 * (k0 + ks) + 4 * c) * 2;
-            const uint2 h0 = *reinterpret_cast<const uint2*>(p0), h1 = *reinterpret_cast<const uint2*>(p0 + 8 * kRow);
-            const uint2 l0 = *reinterpret_cast<const uint2*>(p0 + 2 * rank), l1 = *reinterpret_cast<const uint2*>(p0 + 8 * kRow + 2 * rank);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              mma16816<T>(acc[j], h0.x, h1.x, h0.y, h1.y, b[ks][j].x, b[ks][j].y);
-              mma16816<T>(acc[j], l0.x, l1.x, l0.y, l1.y, b[ks][j].x, b[ks][j].y);
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = rt + g + 8 * e;
-        if (r < m && in) {
-          const float sc = rank ? s_scale[r] : 0.f;
-          T* v = reinterpret_cast<T*>(&yv[e]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-              if (rank) v[2 * j + q] = (T)fmaf(acc[j][2 * e + q], sc, (float)v[2 * j + q]);
-          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at[e]) = yv[e];
-        }
+        uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (long long)s_tok[r] * a.o_st + col);
+        if (col < a.d_out) to[0] = yv[i][e][0];
+        if (col + 8 < a.d_out) to[1] = yv[i][e][1];
       }
     }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0) report_abort(abort, a.err);
+  if (warp == 0 && rank) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -463,31 +686,41 @@ static long long adapter_groups(int T, int n) { return T / kAD_Group + (n + 1 < 
 
 template <typename T, int RM, int ST>
 static int launch_shrink(const AdapterArgs& a, unsigned groups, cudaStream_t stream) {
-  constexpr int smem = (kAD_Group + RM) * 128 * ST;
+  constexpr int smem = (kAD_Group + RM) * 128 * ST + 1024;
   const int rc = ensure_smem_attr((const void*)adapter_shrink_kernel<T, RM, ST>, smem);
   return rc ? rc : launch_early(adapter_shrink_kernel<T, RM, ST>, dim3(groups, a.splits), 256, smem, stream, a);
 }
 
+template <typename T, int RM>
+static int launch_expand(const AdapterArgs& a, unsigned groups, cudaStream_t stream) {
+  using C = ExpandCfg<T, RM>;
+  const int rc = ensure_smem_attr((const void*)adapter_expand_kernel<T, RM>, C::Smem);
+  return rc ? rc : launch_early(adapter_expand_kernel<T, RM>, dim3(groups, (a.d_out + kAD_Tile * a.units - 1) / (kAD_Tile * a.units)), 256, C::Smem, stream, a);
+}
+
 template <typename T>
 static int launch_adapters(AdapterArgs a, int sms, cudaStream_t stream) {
-  constexpr int kRow = kAD_MaxRank * 4 + 32;
   int rc;
   if (a.T <= kAD_Few) {
     rc = launch_early(adapter_shrink_few_kernel<T>, dim3(a.T, a.splits, a.rmax / 16), 256, 0, stream, a);
     if (rc) return rc;
-    a.units = 2;
-    return launch_early(adapter_expand_kernel<T, 16>, dim3(a.T, (a.d_out + 256 * a.units - 1) / (256 * a.units)), 256, 16 * kRow, stream, a);
+    // about four CTAs per SM if every token has an adapter of its own
+    const int blocks = (a.d_out + 511) / 512, cut = (4 * sms + a.T - 1) / a.T;
+    a.units = (blocks + cut - 1) / cut;
+    return launch_early(adapter_expand_few_kernel<T>, dim3(a.T, (blocks + a.units - 1) / a.units), 256, 0, stream, a);
   }
   const unsigned groups = (unsigned)adapter_groups(a.T, a.n);
-  if ((rc = launch_early(adapter_route_kernel, dim3(1), 1024, (size_t)(2 * (a.n + 2)) * 4, stream, a))) return rc;
-  rc = a.rmax <= 32 ? launch_shrink<T, 32, 6>(a, groups, stream)
-       : a.rmax <= 64 ? launch_shrink<T, 64, 6>(a, groups, stream) : launch_shrink<T, 128, 4>(a, groups, stream);
+  if ((rc = ensure_smem_attr((const void*)adapter_route_kernel, 2 * (kAD_MaxAdapters + 2) * 4 + kAD_RouteIds))) return rc;
+  if ((rc = launch_early(adapter_route_kernel, dim3(1), 1024, (size_t)(2 * (a.n + 2)) * 4 + kAD_RouteIds, stream, a))) return rc;
+  rc = a.rmax <= 32 ? launch_shrink<T, 32, 5>(a, groups, stream)
+       : a.rmax <= 64 ? launch_shrink<T, 64, 4>(a, groups, stream) : launch_shrink<T, 128, 3>(a, groups, stream);
   if (rc) return rc;
-  // columns per CTA: h's parts are made once for all of them, but there have to be enough CTAs
+  // tiles per CTA: h's parts are made once for all of them, but there have to be enough CTAs
   const long long real = (a.T + kAD_Group - 1) / kAD_Group;
-  a.units = 4;
-  while (a.units > 1 && real * ((a.d_out + 256 * a.units - 1) / (256 * a.units)) < 4LL * sms) a.units >>= 1;
-  return launch_early(adapter_expand_kernel<T, 64>, dim3(groups, (a.d_out + 256 * a.units - 1) / (256 * a.units)), 256, 64 * kRow, stream, a);
+  const int blocks = (a.d_out + kAD_Tile - 1) / kAD_Tile;
+  a.units = 16;
+  while (a.units > 1 && real * ((blocks + a.units - 1) / a.units) < 4LL * sms) a.units >>= 1;
+  return a.rmax <= 64 ? launch_expand<T, 64>(a, groups, stream) : launch_expand<T, 128>(a, groups, stream);
 }
 
 }  // namespace bfb
@@ -523,6 +756,7 @@ int bf_adapter_add(const void* x, long long x_st, const int32_t* ids, int T, int
   a.x_st = x_st; a.y_st = y_st; a.o_st = o_st;
   a.ids = ids; a.row = row; a.scale = scale;
   a.A = A; a.B = B;
+  a.err = st.err;
   a.n = n; a.T = T; a.d_in = d_in; a.d_out = d_out; a.rmax = rmax;
   adapter_split(T, d_in, 148, &a.splits, &a.kper);
   uint8_t* p = static_cast<uint8_t*>(ws);
