@@ -38,7 +38,10 @@ struct AdapterArgs {
   const void *A, *B;               // A [row[n]][d_in]; B: adapter a's [d_out][r_a] from element row[a] d_out on
   int n, T, d_in, d_out, rmax, splits, kper, units;
   unsigned int* err;
-  float* h;                        // [splits][T][rmax]
+  float* h;                        // [splits][T][rmax]; many tokens: by their place in perm
+  void* parts;                     // [T][2][rmax] h's two parts, by place in perm
+  float* back;                     // [T] the scale that undoes theirs, times the adapter's
+  int32_t* arrived;                // [groups] splits that are done
   int32_t* perm;                   // [T] tokens by adapter
   int4* groups;                    // (adapter or n, first of perm, tokens, -)
   int32_t* n_groups;
@@ -157,11 +160,22 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, buckets = a.n + 1;
   for (int i = tid; i < buckets + 1; i += 1024) s_at[i] = 0;
-  const int per = min((a.T + 1023) / 1024, kAD_RoutePer);
+  int per_log = 0;                    // a power of two of tokens per thread: no divisions
+  while (per_log < 5 && (1024 << per_log) < a.T) ++per_log;
+  const int per = 1 << per_log;
   auto load = [&](int t0) {
     const int n = min(a.T - t0, 1024 * per);
     __syncthreads();
-    for (int i = tid; i < n; i += 1024) s_id[i / per * (kAD_RoutePer + 2) + i % per] = (uint16_t)adapter_of(a, __ldg(a.ids + t0 + i));
+    for (int i0 = 0; i0 < n; i0 += 8192) {
+      int v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = i0 + k * 1024 + tid < n ? __ldg(a.ids + t0 + i0 + k * 1024 + tid) : -1;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = i0 + k * 1024 + tid;
+        if (i < n) s_id[(i >> per_log) * (kAD_RoutePer + 2) + (i & (per - 1))] = (uint16_t)adapter_of(a, v[k]);
+      }
+    }
     __syncthreads();
   };
   const uint16_t* mine_id = s_id + tid * (kAD_RoutePer + 2);
@@ -235,6 +249,7 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     }
     const int first = s_at[b] + (k - s_grp[b]) * kAD_Group;
     a.groups[k] = make_int4(b, first, min(kAD_Group, s_at[b + 1] - first), 0);
+    a.arrived[k] = 0;
   }
   if (tid == 0) *a.n_groups = total;
   __syncthreads();
@@ -261,8 +276,8 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     __syncthreads();
     // the tokens of whole warps, in their order
     for (int i = tid; i < min(a.T - t0, 1024 * per); i += 1024) {
-      const int to = s_base[i / per];
-      if (to >= 0) a.perm[to + i % per] = t0 + i;
+      const int to = s_base[i >> per_log];
+      if (to >= 0) a.perm[to + (i & (per - 1))] = t0 + i;
     }
   }
 }
@@ -277,7 +292,7 @@ __global__ void __launch_bounds__(256) adapter_shrink_kernel(AdapterArgs a) {
   __shared__ int s_tok[kAD_Group];
   __shared__ uint64_t s_bar[ST];
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort;
+  __shared__ int s_abort, s_last;
   volatile int* abort = &s_abort;
   wait_for_stream();
   let_next_start();
@@ -347,7 +362,7 @@ __global__ void __launch_bounds__(256) adapter_shrink_kernel(AdapterArgs a) {
   tc_fence_after();
   if (warp < 4 && ok) {
     const int r = 32 * warp + lane;
-    float* to = a.h + ((size_t)blockIdx.y * a.T + s_tok[r]) * a.rmax;
+    float* to = a.h + ((size_t)blockIdx.y * a.T + grp.y + r) * a.rmax;
 #pragma unroll 1
     for (int c = 0; c < rank; c += 16) {
       uint32_t v[16];
@@ -359,8 +374,57 @@ __global__ void __launch_bounds__(256) adapter_shrink_kernel(AdapterArgs a) {
       }
     }
   }
+  // the CTA that is the last to bring its split adds them all, in their order, and makes the two parts: a warp four rows at a time, lane l the
+  // ranks 2 l, 2 l + 1 (and 64 more)
+  __threadfence();
   tc_fence_before();
   __syncthreads();
+  if (tid == 0) s_last = atomicAdd(a.arrived + blockIdx.x, 1) == a.splits - 1;
+  __syncthreads();
+  if (s_last) {
+    __threadfence();
+    constexpr int kPairs = RM <= 64 ? 1 : 2;
+    const float scale = a.scale[grp.x];
+    for (int rb = 4 * warp; rb < m; rb += 32) {
+      float2 v[4][kPairs];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[q][i] = make_float2(0.f, 0.f);
+#pragma unroll 2
+      for (int sp = 0; sp < a.splits; ++sp)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < kPairs; ++i)
+            if (rb + q < m && 64 * i + 2 * lane < rank) {
+              const float2 x = __ldcg(reinterpret_cast<const float2*>(a.h + ((size_t)sp * a.T + grp.y + rb + q) * a.rmax + 64 * i + 2 * lane));
+              v[q][i].x += x.x;
+              v[q][i].y += x.y;
+            }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (rb + q >= m) break;
+        float big = 0.f;           // (a NaN is no maximum, but its row becomes NaN by itself)
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) big = fmaxf(big, fmaxf(fabsf(v[q][i].x), fabsf(v[q][i].y)));
+        big = warp_max(big);
+        // a power of two that takes the row's largest to [2^13, 2^14): both parts then keep all of their bits in fp16 too
+        const int ex = big > 0.f && big < INFINITY ? min(max((int)(__float_as_uint(big) >> 23), 14), 253) : 140;
+        const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
+        T* to = static_cast<T*>(a.parts) + (size_t)(grp.y + rb + q) * 2 * a.rmax;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+          if (64 * i + 2 * lane < rank) {
+            const float x = v[q][i].x * up, y = v[q][i].y * up;
+            const T hi[2] = {(T)x, (T)y}, lo[2] = {(T)(x - (float)hi[0]), (T)(y - (float)hi[1])};
+            *reinterpret_cast<uint32_t*>(to + 64 * i + 2 * lane) = *reinterpret_cast<const uint32_t*>(hi);
+            *reinterpret_cast<uint32_t*>(to + a.rmax + 64 * i + 2 * lane) = *reinterpret_cast<const uint32_t*>(lo);
+          }
+        if (lane == 0) a.back[grp.y + rb + q] = scale * __uint_as_float((uint32_t)(ex - 13) << 23);
+      }
+    }
+  }
   if (tid == 0) report_abort(abort, a.err);
   if (warp == 0) {
     tc_fence_after();
@@ -375,27 +439,39 @@ template <typename T, int M>       // M: 1 or 4 tokens at most
 __device__ __forceinline__ void expand_few(const AdapterArgs& a, const T* w, int rank, int m, const int* s_tok, const float* s_h, float scale, int col0,
                                            int units) {
   const int lane = threadIdx.x & 31;
+  uint32_t y[M], y_next[M];
+  uint4 b[4];
+  const uint4 *p, *q;
+  auto begin = [&](int u) {        // unit u's y and first 16 ranks
+    const int col = col0 + 512 * u + 2 * lane;
+    if (u >= units || col >= a.d_out) return;
+#pragma unroll
+    for (int t = 0; t < M; ++t)
+      if (t < m) y_next[t] = __ldcs(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.y) + (long long)s_tok[t] * a.y_st + col));
+    p = reinterpret_cast<const uint4*>(w + (long long)col * rank);
+    q = reinterpret_cast<const uint4*>(w + (long long)(col + 1) * rank);
+    b[0] = __ldg(p), b[1] = __ldg(p + 1), b[2] = __ldg(q), b[3] = __ldg(q + 1);
+  };
+  begin(0);
 #pragma unroll 1
   for (int u = 0; u < units; ++u) {
     const int col = col0 + 512 * u + 2 * lane;
     if (col >= a.d_out) return;
-    uint32_t y[M];
-#pragma unroll
-    for (int t = 0; t < M; ++t)
-      if (t < m) y[t] = __ldcs(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.y) + (long long)s_tok[t] * a.y_st + col));
     uint64_t acc[M][2];
 #pragma unroll
-    for (int t = 0; t < M; ++t) acc[t][0] = acc[t][1] = 0;
-    const uint4* p = reinterpret_cast<const uint4*>(w + (long long)col * rank);
-    const uint4* q = reinterpret_cast<const uint4*>(w + (long long)(col + 1) * rank);
-    uint4 b[4] = {ldg_stream(p), ldg_stream(p + 1), ldg_stream(q), ldg_stream(q + 1)};
+    for (int t = 0; t < M; ++t) {
+      acc[t][0] = acc[t][1] = 0;
+      y[t] = y_next[t];
+    }
 #pragma unroll 1
     for (int r = 0; r < rank; r += 16) {
       uint4 now[4] = {b[0], b[1], b[2], b[3]};
       if (r + 16 < rank) {
         p += 2;
         q += 2;
-        b[0] = ldg_stream(p), b[1] = ldg_stream(p + 1), b[2] = ldg_stream(q), b[3] = ldg_stream(q + 1);
+        b[0] = __ldg(p), b[1] = __ldg(p + 1), b[2] = __ldg(q), b[3] = __ldg(q + 1);
+      } else {
+        begin(u + 1);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -466,7 +542,9 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
   for (int i = tid; i < m * rank; i += 256) {
     const int t = i / rank, r = i - t * rank;
     float v = 0.f;
-    for (int s = 0; s < a.splits; ++s) v += a.h[((size_t)s * a.T + s_tok[t]) * a.rmax + r];
+    const float* p = a.h + (size_t)s_tok[t] * a.rmax + r;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) v += p[(size_t)s * a.T * a.rmax];
     s_h[t * kAD_MaxRank + r] = v;
   }
   __syncthreads();
@@ -557,37 +635,16 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
     tmem_relinquish();
   }
   if (rank) {
-    // a warp a row: lane l the ranks 2 l, 2 l + 1 (and 64 more)
-    for (int r = warp; r < kAD_Group; r += 8) {
-      float2 v[C::Atoms];
-      float big = 0.f;
+    // two threads to a row; rows that are not there repeat the last one, nobody reads their sums
+    const T* src = static_cast<const T*>(a.parts) + (size_t)(grp.y + min(brow, m - 1)) * 2 * a.rmax;
+    const uint32_t dst = hs + brow * 128;
+    for (int p = tid & 1; p < pieces; p += 2)
 #pragma unroll
-      for (int i = 0; i < C::Atoms; ++i) {
-        v[i] = make_float2(0.f, 0.f);
-        if (r < m && 64 * i + 2 * lane < rank)
-          for (int s = 0; s < a.splits; ++s) {
-            const float2 x = *reinterpret_cast<const float2*>(a.h + ((size_t)s * a.T + s_tok[r]) * a.rmax + 64 * i + 2 * lane);
-            v[i].x += x.x;
-            v[i].y += x.y;
-          }
-        // (a NaN is no maximum, but its row becomes NaN by itself)
-        big = fmaxf(big, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
-      }
-      big = warp_max(big);
-      // a power of two that takes the row's largest to [2^13, 2^14): both parts then keep all of their bits in fp16 too
-      const int ex = big > 0.f && big < INFINITY ? min(max((int)(__float_as_uint(big) >> 23), 14), 253) : 140;
-      const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-#pragma unroll
-      for (int i = 0; i < C::Atoms; ++i) {
-        const float x = v[i].x * up, y = v[i].y * up;
-        const T hi[2] = {(T)x, (T)y}, lo[2] = {(T)(x - (float)hi[0]), (T)(y - (float)hi[1])};
-        uint8_t* to = s_h + i * (kAD_Group * 128) + sw128_offset(r, 2 * lane);
-        *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(hi);
-        *reinterpret_cast<uint32_t*>(to + C::HBytes / 2) = *reinterpret_cast<const uint32_t*>(lo);
-      }
-      if (lane == 0) s_scale[r] = a.scale[id] * __uint_as_float((uint32_t)(ex - 13) << 23);
-    }
+      for (int part = 0; part < 2; ++part)
+        copy16(dst + part * (C::HBytes / 2) + (p >> 3) * (kAD_Group * 128) + (((p & 7) ^ (brow & 7)) << 4), src + part * a.rmax + 8 * p, true);
+    if (tid < m) s_scale[tid] = a.back[grp.y + tid];
   }
+  asm volatile("cp.async.commit_group;" ::: "memory");
   const uint32_t idesc = idesc_f16(128, kAD_Tile, kIsBf16<T>);
   uint32_t tmem = 0;
   auto products = [&](int j) {             // by one thread
@@ -606,7 +663,7 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
 #pragma unroll 1
   for (int j = -1; j < tiles && ok; ++j) {
     // tile j + 1's rows of B have landed, everybody is done with tile j - 1
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (j < 0) asm volatile("cp.async.wait_group 0;" ::: "memory"); else asm volatile("cp.async.wait_group 1;" ::: "memory");
     fence_async_smem();
     tc_fence_before();
     __syncthreads();
@@ -669,20 +726,49 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
   }
 }
 
-// how d_in is split: few tokens in parts of kAD_KFew; many so that there are about six CTAs for every SM
-static void adapter_split(int T, int d_in, int sms, int* splits, int* kper) {
+// how d_in is split: few tokens in parts of kAD_KFew; many so that the rounds of CTAs (two to an SM) times what each reads, plus 512 values' worth for its
+// start and end, are fewest
+static void adapter_split(int T, int d_in, int* splits, int* kper) {
+  int s = 1;
   if (T <= kAD_Few) {
     *kper = kAD_KFew;
   } else {
-    const int groups = (T + kAD_Group - 1) / kAD_Group, most = (d_in + 511) / 512;
-    int s = (6 * sms + groups - 1) / groups;
-    s = s < 1 ? 1 : s > most ? most : s;
+    const long long groups = (T + kAD_Group - 1) / kAD_Group, slots = 2 * 148;
+    long long best = 1ll << 62;
+    for (int k = 1; k <= 16 && k <= (d_in + 255) / 256; ++k) {
+      const long long cost = (groups * k + slots - 1) / slots * (d_in / k + 512);
+      if (cost < best) {
+        best = cost;
+        s = k;
+      }
+    }
     *kper = ((d_in + s - 1) / s + 63) / 64 * 64;
   }
   *splits = (d_in + *kper - 1) / *kper;
 }
 
 static long long adapter_groups(int T, int n) { return T / kAD_Group + (n + 1 < T ? n + 1 : T); }
+
+// the workspace: its bytes, and the arrays in it
+static size_t adapter_layout(AdapterArgs& a, uint8_t* ws) {
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* p = ws ? ws + at : nullptr;
+    at += (bytes + 15) / 16 * 16;
+    return p;
+  };
+  if (a.T > kAD_Few) {
+    const size_t groups = (size_t)adapter_groups(a.T, a.n);
+    a.n_groups = reinterpret_cast<int32_t*>(take(4));
+    a.groups = reinterpret_cast<int4*>(take(groups * sizeof(int4)));
+    a.arrived = reinterpret_cast<int32_t*>(take(groups * 4));
+    a.perm = reinterpret_cast<int32_t*>(take((size_t)a.T * 4));
+    a.back = reinterpret_cast<float*>(take((size_t)a.T * 4));
+    a.parts = take((size_t)a.T * 2 * a.rmax * 2);
+  }
+  a.h = reinterpret_cast<float*>(take((size_t)a.splits * a.T * a.rmax * 4));
+  return at;
+}
 
 template <typename T, int RM, int ST>
 static int launch_shrink(const AdapterArgs& a, unsigned groups, cudaStream_t stream) {
@@ -732,8 +818,10 @@ extern "C" {
 size_t bf_adapter_workspace(int T, int n, int d_in, int rmax) {
   if (T <= 0 || n <= 0 || n > kAD_MaxAdapters || d_in <= 0 || rmax <= 0 || rmax > kAD_MaxRank) return 0;
   int splits, kper;
-  adapter_split(T, d_in, 148, &splits, &kper);
-  return 16 + (size_t)adapter_groups(T, n) * sizeof(int4) + ((size_t)T * 4 + 15) / 16 * 16 + (size_t)splits * T * rmax * 4;
+  adapter_split(T, d_in, &splits, &kper);
+  AdapterArgs a{};
+  a.T = T; a.n = n; a.rmax = rmax; a.splits = splits;
+  return adapter_layout(a, nullptr);
 }
 
 int bf_adapter_add(const void* x, long long x_st, const int32_t* ids, int T, int d_in, int d_out, const void* A, const void* B,
@@ -758,13 +846,8 @@ int bf_adapter_add(const void* x, long long x_st, const int32_t* ids, int T, int
   a.A = A; a.B = B;
   a.err = st.err;
   a.n = n; a.T = T; a.d_in = d_in; a.d_out = d_out; a.rmax = rmax;
-  adapter_split(T, d_in, 148, &a.splits, &a.kper);
-  uint8_t* p = static_cast<uint8_t*>(ws);
-  a.n_groups = reinterpret_cast<int32_t*>(p);
-  a.groups = reinterpret_cast<int4*>(p + 16);
-  p += 16 + (size_t)adapter_groups(T, n) * sizeof(int4);
-  a.perm = reinterpret_cast<int32_t*>(p);
-  a.h = reinterpret_cast<float*>(p + ((size_t)T * 4 + 15) / 16 * 16);
+  adapter_split(T, d_in, &a.splits, &a.kper);
+  adapter_layout(a, static_cast<uint8_t*>(ws));
   return dtype == BF_BF16 ? launch_adapters<__nv_bfloat16>(a, st.sm_count, stream) : launch_adapters<__half>(a, st.sm_count, stream);
 }
 
