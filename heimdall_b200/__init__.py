@@ -12,7 +12,7 @@ Public API (mirrors of the reference ``heimdall`` package):
   window_attention                   heimdall/hibrit.py:336-361 (the math of _window_fp32)
   prompt_attention                   heimdall/hibrit.py:275-290 (a kept layer's causal attention, packed prompts)
   norm_rope_heads                    heimdall/hibrit.py:254-268 (_proj's norm and rotation, positions on several axes)
-  PagedKV                            a kept layer's cache in 8-bit pages: append, attend, fork, free, compact
+  PagedKV                            a kept layer's cache in 8-bit pages: append, attend, fork, share, free, compact
   Adapters                           low-rank adapters of many requests beside a shared projection
   BifrostLayer.student               heimdall/hibrit.py:363-424 (HybridAttention._student)
   BifrostLayer.mem_inputs            heimdall/hibrit.py:327-334

@@ -60,6 +60,10 @@ SIGNATURES = {
     "bf_paged_append": [_P, _I, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _I, _I, _P],
     "bf_paged_attend_workspace": [_I, _I, _I, _I, _I],
     "bf_paged_attend": [_P, _I, _P, _L, _L, _L, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P, _P, _Z, _P],
+    "bf_share_words": [_I],
+    "bf_page_table_share": [_P, _P, _I, _I, _P, _P, _P],
+    "bf_paged_attend_shared_workspace": [_I, _I, _I, _I, _I],
+    "bf_paged_attend_shared": [_P, _I, _P, _L, _L, _L, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P, _P, _Z, _P],
     "bf_paged_pages": [_P, _P, _I, _P, _I, _P, _I, _P, _I, _P],
     "bf_page_table_reserve": [_P, _P, _P, _I, _P, _P, _P],
     "bf_page_table_free": [_P, _P, _I, _P],
@@ -75,7 +79,7 @@ _RESTYPE = {"bf_strerror": ctypes.c_char_p, "bf_last_cuda_error": ctypes.c_char_
             "bf_layer_prefill_sp_workspace": _Z,
             "bf_gdn_segment_workspace": _Z, "bf_llama_state_floats": _Z,
             "bf_ret_decode_workspace": _Z, "bf_paged_attend_workspace": _Z, "bf_gdn_bwd_workspace": _Z,
-            "bf_adapter_workspace": _Z}
+            "bf_adapter_workspace": _Z, "bf_share_words": _Z, "bf_paged_attend_shared_workspace": _Z}
 
 _lock = threading.Lock()
 _lib = None

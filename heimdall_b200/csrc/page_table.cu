@@ -3,7 +3,10 @@
 // sequence can be partly filled, and a partly filled page belongs to one sequence (fork copies it, truncate too).
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "bifrost_b200.h"
+#include "paged_kv.h"
 
 namespace {
 
@@ -203,6 +206,87 @@ int bf_page_table_truncate(bf_page_table* t, const int64_t* slots, const int64_t
   }
   *n_fork = copies;
   *n_set = at / 2;
+  return BF_OK;
+}
+
+size_t bf_share_words(int n) { return n > 0 ? (size_t)bfb::plan_words(n) : 0; }
+
+// Sequences that come from one another share their first full pages: sorted by their pages, those with a page in common are neighbours, and the
+// runs of pages that the same sequences share are the edges of their prefix tree (only a fork shares pages, so two sequences that have a page in common
+// have all pages before it in common too).  A run that saves reading fewer than
+// min_saved tokens is left to the runs behind it, or to the sequences' tails.
+int bf_page_table_share(const bf_page_table* t, const int64_t* slots, int n, int min_saved, int32_t* plan, int32_t* scratch, int* info) {
+  if (bad(t, slots, n, info) || n < 1 || !plan || !scratch || min_saved < 1) return BF_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i < n; ++i)
+    if (slots[i] < 0 || slots[i] >= t->slots) return reject(info, BF_PAGES_SLOT_RANGE);
+  int32_t *s = plan + bfb::kPS_Head, *order = s + n, *place = order + n, *last = place + n, *skip = last + n, *runs = skip + n;
+  int32_t *lcp = scratch, *node = lcp + n, *stack = node + 3 * (int64_t)n, *depth = stack + 2 * (int64_t)n;
+  const auto full = [&](int b) { return (int)(t->lens[s[b]] / t->page); };
+  const auto common = [&](int a, int b) {      // full pages that two sequences have in common
+    const int32_t *x = row(t, s[a]), *y = row(t, s[b]);
+    int lo = 0, hi = std::min(full(a), full(b));
+    if (s[a] == s[b]) return hi;
+    while (lo < hi) {
+      const int m = (lo + hi + 1) >> 1;
+      if (x[m - 1] == y[m - 1]) lo = m; else hi = m - 1;
+    }
+    return lo;
+  };
+  for (int i = 0; i < n; ++i) {
+    s[i] = (int32_t)slots[i];
+    order[i] = i;
+  }
+  std::sort(order, order + n, [&](int a, int b) {
+    const int c = common(a, b), fa = full(a), fb = full(b);
+    if (c < fa && c < fb) return row(t, s[a])[c] < row(t, s[b])[c];
+    return fa != fb ? fa < fb : a < b;
+  });
+  for (int i = 0; i < n; ++i) {
+    place[order[i]] = i;
+    lcp[i] = i + 1 < n ? common(order[i], order[i + 1]) : 0;
+    last[i] = -1;
+    depth[i] = 0;
+    skip[i] = 0;
+  }
+  // the tree's inner nodes (first place, places, depth in pages), children before parents
+  int nodes = 0, top = 0;
+  for (int i = 0; i < n; ++i) {
+    int left = i;
+    while (top > 0 && stack[2 * top - 1] > lcp[i]) {
+      --top;
+      left = stack[2 * top];
+      node[3 * nodes] = left;
+      node[3 * nodes + 1] = i - left + 1;
+      node[3 * nodes + 2] = stack[2 * top + 1];
+      ++nodes;
+    }
+    if (lcp[i] > 0 && (top == 0 || stack[2 * top - 1] < lcp[i])) {
+      stack[2 * top] = left;
+      stack[2 * top + 1] = lcp[i];
+      ++top;
+    }
+  }
+  int count = 0;
+  for (int k = nodes - 1; k >= 0; --k) {
+    const int first = node[3 * k], many = node[3 * k + 1], end = node[3 * k + 2], lead = order[first], from = skip[lead];
+    if ((int64_t)(end - from) * t->page * (many - 1) < min_saved || depth[lead] >= bfb::kPS_Depth) continue;
+    int32_t* r = runs + bfb::kPS_Run * (int64_t)count;
+    r[0] = first;
+    r[1] = many;
+    r[2] = from;
+    r[3] = end;
+    r[4] = last[lead];
+    r[5] = 0;
+    for (int i = first; i < first + many; ++i) {
+      last[order[i]] = count;
+      skip[order[i]] = end;
+      ++depth[order[i]];
+    }
+    ++count;
+  }
+  plan[0] = count;
+  plan[1] = n;
+  plan[2] = plan[3] = 0;
   return BF_OK;
 }
 

@@ -12,7 +12,12 @@ host and can be captured into a CUDA graph:
         c.append(layer, k, v, slot_ids)       # device
         o, _ = c.attend(layer, q, slot_ids)   # device
 
-``fork`` shares pages between sequences, ``free`` and ``truncate`` give them back, ``compact`` closes the pool up.
+``fork`` shares pages between sequences, ``free`` and ``truncate`` give them back, ``compact`` closes the pool up.  Where a batch has forks of
+one prompt, or of a tree of them, ``share`` finds which pages its sequences have in common, and ``attend`` reads those once for all:
+
+    plan = c.share(slots)                     # host: again after a free or truncate
+    o, _ = c.attend(layer, q, shared=plan)    # device
+
 Calls on one cache belong on one stream, or on streams that the caller orders, and on one host thread at a time.  There is no
 CPU path.
 """
@@ -30,6 +35,7 @@ from .structs import BfPagePool, BfPageTable
 
 PAGE_SIZES = (16, 32, 64, 128)
 MAX_GROUP = 24                  # query heads per KV head of attend
+MIN_SAVED = 1024                # tokens that a shared run has to save
 
 
 _REASONS = {1: "a slot is outside [0, {slots})", 2: "a slot is named twice", 3: "a number of tokens is negative",
@@ -118,9 +124,32 @@ class PageTable:
                    self._n1, self._info)
         return {"fork": self._fork[:self._out[4]], "set": self._set[:self._out[5]]}
 
+    def share(self, slots, min_saved: int) -> np.ndarray:
+        s = self._whole(slots)
+        if s.size < 1:
+            raise ValueError("share needs at least one sequence")
+        plan, scratch = np.empty(self._lib.bf_share_words(s.size), np.int32), np.empty(7 * s.size, np.int32)
+        self._call("bf_page_table_share", s.ctypes.data, s.size, min_saved, plan.ctypes.data, scratch.ctypes.data, self._info)
+        return plan
+
     def compact(self) -> dict:
         self._call("bf_page_table_compact", self._to_move, self._n0)
         return {"move": self._move[:self._out[4]]}
+
+
+class SharedPages:
+    """Which pages the sequences of a batch have in common (``PagedKV.share``): ``slots``, in the order of the batch, and ``runs``, the number of
+    page runs that are read once for several sequences."""
+
+    def __init__(self, cache: "PagedKV", slots: np.ndarray, plan: np.ndarray):
+        self.cache = cache
+        self.n = slots.size
+        self.plan = torch.empty(plan.size, dtype=torch.int32, device=cache.device)
+        self._fill(slots, plan)
+
+    def _fill(self, slots: np.ndarray, plan: np.ndarray) -> None:
+        self.slots, self.runs, self.version = slots.tolist(), int(plan[0]), self.cache._shrunk
+        self.plan.copy_(torch.from_numpy(plan))
 
 
 class PagedKV:
@@ -158,7 +187,8 @@ class PagedKV:
         self._pool = BfPagePool(ptr(self.k_pages), ptr(self.v_pages), ptr(self.k_scale), ptr(self.v_scale), ptr(self.table),
                                 ptr(self.lens), layers, pages, heads, page, dim, slots, width)
         self._pool_ptr = ctypes.addressof(self._pool)
-        self._ws = {}                       # workspace bytes by (B, t, H)
+        self._ws = {}                       # workspace bytes by (B, t, H), with True behind them for shared pages
+        self._shrunk = 0                    # calls of free and truncate: plans of shared pages from before are not good
         self._ended = False                 # a change has reached the host's table and not the device's
         self._appended = set()              # layers that the caller's own append has written, for as long as no layer() is out
         self._progress = None               # what retrieval.teacher has written, from the first layer() on
@@ -207,6 +237,7 @@ class PagedKV:
     def free(self, slots) -> None:
         """End the sequences of these slots: their pages return to the pool unless another sequence shares them."""
         self._apply(self.host.free, slots)
+        self._shrunk += 1
         if self._progress is not None:
             self._progress.free(slots)
 
@@ -221,6 +252,7 @@ class PagedKV:
         """Shorten the sequences of these slots to lens tokens (rejected drafts); a shared page that becomes partly filled
         is copied.  The scale of the page that is cut stays as it is."""
         self._apply(self.host.truncate, slots, lens)
+        self._shrunk += 1
         if self._progress is not None:
             self._progress.truncate(slots, lens)
 
@@ -229,6 +261,30 @@ class PagedKV:
         pool is in use from page 0 on.  Returns the number of live pages."""
         self._apply(self.host.compact)
         return self.host.pages - self.host.n_free
+
+    def share(self, slots, into: SharedPages = None, min_saved: int = MIN_SAVED) -> SharedPages:
+        """Which pages these sequences (slots, a list of whole numbers; one may come several times) have in common, for ``attend(shared=)``: the
+        runs of pages that are read once for several of them.  The plan is good until a slot is freed or truncated (attend refuses it after that);
+        reserve, append, fork and compact leave it good, though sequences forked later are not in it.  ``into``: a plan of as many sequences,
+        whose device memory takes the new one, so that a captured attend goes on with it.  Runs that save fewer than
+        ``min_saved`` tokens of reading ((sequences - 1) * tokens) are not worth their start and are left out.  At most four
+        runs to a sequence; deeper ones are read sequence by sequence."""
+        self._check()
+        if into is not None and (not isinstance(into, SharedPages) or into.cache is not self):
+            raise ValueError("into must be a plan of this cache")
+        if min_saved < 1:
+            raise ValueError("min_saved must be positive")
+        slots = self.host._whole(slots)
+        if into is not None and into.n != slots.size:
+            raise ValueError(f"into is a plan of {into.n} sequences, not of {slots.size}")
+        with on_device(self.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("heimdall_b200: what is shared is found on the host: share cannot be captured into a CUDA graph")
+            plan = self.host.share(slots, min(int(min_saved), 2 ** 31 - 1))
+            if into is None:
+                return SharedPages(self, slots, plan)
+            into._fill(slots, plan)
+        return into
 
     # -------------------------------------------------------------------------------------------- keys and values
     def _layer(self, layer: int) -> int:
@@ -284,7 +340,7 @@ class PagedKV:
                       stream_handle())
         return B if shape[-3] else 0        # the sequences that tokens may have been written of
 
-    def attend(self, layer: int, q, slots=None, scale=None, with_lse: bool = False):
+    def attend(self, layer: int, q, slots=None, scale=None, with_lse: bool = False, shared: SharedPages = None):
         """Attention of each sequence's last t tokens over its pages: q [B,t,H,D] (bf16 or fp16; H a multiple of the KV
         heads) at the positions lens - t .. lens - 1, each seeing the positions up to its own.  Returns o [B,t,H,D] in q's
         dtype and lse [B,H,t] fp32 (None unless ``with_lse``); a token that sees nothing has o = 0 and lse = -inf.  What the
@@ -292,7 +348,12 @@ class PagedKV:
         tokens.  A component of q is held to 2^-25 of the largest of its row and head (exactly, where it is above about 2^-14 of
         that).  A token's weight times its V scale is held to 2^-11 of itself or 2^-26 of (largest weight) * (largest V scale) among
         the 128 tokens of its tile, whichever is more.  Made for decode steps and drafts: 24 rows (tokens times query heads per KV
-        head) share one way through the pages, so t tokens take as long as t / floor(24 / (H / G)) of them."""
+        head) share one way through the pages, so t tokens take as long as t / floor(24 / (H / G)) of them.
+
+        ``shared``: a plan of ``share`` in the place of slots: its sequences, in its order, each shared page read once for all of them.  There a
+        component of q is held to 2^-17 of the largest of its row and head (exactly, where its own bits do not end below that), a token's weight times
+        its V scale to 2^-9 (fp16: 2^-12) of itself or 2^-18 of the largest among the 128 tokens of its tile, and V scales of
+        a sequence may be 2^100 apart."""
         self._check()
         dev = serving_inputs("PagedKV.attend", self.k_pages, q)
         layer, shape = self._layer(layer), q.shape
@@ -302,11 +363,23 @@ class PagedKV:
         if H // self.heads > MAX_GROUP:
             raise NotImplementedError(f"attend takes at most {MAX_GROUP} query heads per KV head")
         scale = score_scale(scale, D)
+        if shared is not None:
+            self._check_plan(shared, slots, B)
         with on_device(dev):
-            ids = self._ids(slots, B)
+            if shared is not None and not shared.runs:
+                slots, shared = shared.plan[4:4 + B], None           # nothing to share
+            ids = None if shared is not None else self._ids(slots, B)
             q, qp, qs = heads_16bit("q", q)
             o = q.new_empty(shape)
             lse = q.new_empty((B, H, t), dtype=torch.float32) if with_lse else None
+            if shared is not None:
+                nws = self._ws.get((B, t, H, True))
+                if nws is None:
+                    nws = self._ws[B, t, H, True] = max(_lib.size("bf_paged_attend_shared_workspace", B, t, H, self.heads, D), 16)
+                ws = q.new_empty((nws,), dtype=torch.uint8)
+                _lib.call("bf_paged_attend_shared", self._pool_ptr, layer, qp, *qs, shared.plan.data_ptr(), B, t, H, kernel_dtype(q), scale,
+                          o.data_ptr(), ptr(lse), ws.data_ptr(), nws, stream_handle())
+                return o, lse
             nws = self._ws.get((B, t, H))
             if nws is None:
                 nws = self._ws[B, t, H] = max(_lib.size("bf_paged_attend_workspace", B, t, H, self.heads, D), 16)
@@ -314,6 +387,16 @@ class PagedKV:
             _lib.call("bf_paged_attend", self._pool_ptr, layer, qp, *qs, ptr(ids), B, t, H, kernel_dtype(q), scale, o.data_ptr(),
                       ptr(lse), ws.data_ptr(), nws, stream_handle())
         return o, lse
+
+    def _check_plan(self, shared, slots, B: int) -> None:
+        if not isinstance(shared, SharedPages) or shared.cache is not self:
+            raise ValueError("shared must be a plan of this cache's share")
+        if slots is not None:
+            raise ValueError("the plan of shared pages has its own slots")
+        if shared.n != B:
+            raise ValueError(f"the plan is of {shared.n} sequences, not of {B}")
+        if shared.version != self._shrunk:
+            raise ValueError("slots were freed or truncated since this plan was made: share again")
 
     def layer(self, layer: int) -> "PagedLayer":
         """This cache as one kept layer's ``cache`` argument of ``retrieval.teacher`` (slots 0 .. B-1).  How far the layer

@@ -265,3 +265,80 @@ def test_a_layers_progress_follows_the_page_table():
     host.free([0, 3])
     p.free([0, 3])
     assert p.n[:, [0, 1, 3]].tolist() == [[0] * 3] * 3
+
+
+# ------------------------------------------------------------------------------------------------ plans of shared pages
+def _plan(t, slots, min_saved=1):
+    n = len(slots)
+    p = t.share(slots, min_saved).tolist()
+    parts = [p[4 + k * n:4 + (k + 1) * n] for k in range(5)]
+    runs = [p[4 + 5 * n + 6 * k:10 + 5 * n + 6 * k] for k in range(p[0])]
+    assert p[1] == n
+    return parts, runs
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_plan_of_shared_pages_against_the_table(seed):
+    """Every run lies in the rows of all its sequences, the runs on a sequence's way follow one another, and what two sequences have in common is
+    shared unless a sequence's four runs are used up."""
+    rng = random.Random(seed)
+    for _ in range(30):
+        L, slots = rng.choice([16, 64, 128]), rng.choice([3, 12, 40])
+        t, live = PageTable(4000, slots, L, 64), []
+        for s in range(slots):
+            if live and rng.random() < 0.7:
+                t.fork([rng.choice(live)], [s])
+            t.reserve([s], [min(rng.choice([0, 1, rng.randrange(L * 6)]), 64 * L - int(t.lens[s]))])
+            live.append(s)
+        s = rng.choice(live)
+        t.truncate([s], [rng.randrange(int(t.lens[s]) + 1)])
+        b, least = [rng.randrange(slots) for _ in range(rng.choice([1, 2, 7, 30]))], rng.choice([1, 3 * L])
+        (sl, order, place, last, skip), runs = _plan(t, b, least)
+        assert sl == b and [order[p] for p in place] == list(range(len(b))) and len(runs) < len(b)
+        ways = []
+        for i in range(len(b)):
+            r, way = last[i], []
+            while r >= 0:
+                assert runs[r][0] <= place[i] < runs[r][0] + runs[r][1]
+                way.insert(0, r)
+                r = runs[r][4]
+            assert len(way) <= 4 and [runs[r][2] for r in way] == [0] * bool(way) + [runs[r][3] for r in way[:-1]]
+            assert skip[i] == (runs[way[-1]][3] if way else 0) and skip[i] * L <= t.lens[b[i]]
+            ways.append(way)
+        for first, many, begin, end, *_ in runs:
+            rows = {tuple(t.table[b[order[k]], :end].tolist()) for k in range(first, first + many)}
+            assert many > 1 and len(rows) == 1 and (end - begin) * L * (many - 1) >= least
+        for i in range(len(b)):
+            for j in range(i if least == 1 else 0):
+                same = 0
+                while same < min(t.lens[b[i]], t.lens[b[j]]) // L and t.table[b[i], same] == t.table[b[j], same]:
+                    same += 1
+                both = [r for r in ways[i] if r in ways[j]]
+                found = runs[both[-1]][3] if both else 0
+                assert found == same or (found < same and len(ways[i]) == len(ways[j]) == 4)
+
+
+def test_plan_refusals():
+    t = PageTable(10, 3, 16, 8)
+    t.reserve([0], [40])
+    for bad in ([], [3], [-1], [0.5], [[0, 1]]):
+        with pytest.raises(ValueError):
+            t.share(bad, 1)
+    with pytest.raises(ValueError, match="outside"):
+        t.share([0, 7], 1)
+    assert t.share([0, 0, 1], 1)[0] == 1 and t.share([1, 2], 1)[0] == 0
+    assert _lib.size("bf_share_words", 0) == 0 and _lib.size("bf_share_words", 5) == 4 + 11 * 5
+    ws = lambda *a: _lib.size("bf_paged_attend_shared_workspace", *a)
+    assert ws(0, 1, 4, 2, 256) == ws(1, 1, 4, 3, 256) == ws(1, 1, 25, 1, 256) == ws(1, 1, 4, 2, 128) == 0 and ws(64, 1, 24, 4, 256) > 0
+
+
+@pytest.mark.parametrize("code,kw", [(1, {"n": -1}), (1, {"H": 5}), (1, {"plan": 0}), (1, {"q": 0}), (1, {"scale": 0.0}), (2, {"dtype": 0}),
+                                     (2, {"H": 50}), (3, {"q": 8}), (3, {"plan": 8}), (4, {"ws": 0}), (4, {"nws": 1000}), (2, {"n": 1 << 27})])
+def test_c_entry_of_shared_attend_refuses(code, kw):
+    a = dict(q=16, plan=16, n=2, t=1, H=4, dtype=1, scale=0.1, ws=16, nws=1 << 40)
+    a.update(kw)
+    pool = BfPagePool(16, 16, 16, 16, 16, 16, 1, 8, 2, 16, 256, 4, 4)
+    with pytest.raises(_lib.BifrostError) as e:
+        _lib.call("bf_paged_attend_shared", ctypes.addressof(pool), 0, a["q"], 256, 256, 256, a["plan"], a["n"], a["t"], a["H"], a["dtype"],
+                  a["scale"], 16, 0, a["ws"], a["nws"], 0)
+    assert e.value.code == code
