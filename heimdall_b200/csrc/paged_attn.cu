@@ -41,7 +41,6 @@
 #include "capi_internal.h"
 #include "common.cuh"
 #include "launch_early.h"
-#include "paged_attn.h"
 #include "paged_kv.h"
 #include "tmap.h"
 
@@ -49,7 +48,9 @@ namespace bfb {
 
 constexpr int kPA_Tile = 128;                        // tokens per tile
 constexpr int kPA_Unit = kPA_Tile * kPG_D;           // bytes of one K or V tile
+constexpr int kPA_MaxCtas = 160;
 constexpr int kPA_MaxRows = 24;
+constexpr int kPA_Part = kPG_D + 4;                  // floats of a row's partial: accumulator, maximum, sum, two to keep it aligned
 
 struct PagedAttnArgs {
   PagePool p;
@@ -66,10 +67,6 @@ struct PagedAttnArgs {
   float* lse;
   int4* desc;           // [ctas] (first CTA of the cut segment that ends here or -1, b, chunk, KV head)
   float* part;          // [ctas][2][RP][kPA_Part]
-  // the tails of sequences whose first pages another kernel reads (paged_shared.cu), to be merged with what that finds:
-  const int32_t* skip;  // [B] pages that are not this call's
-  float* tail;          // [B,t,H][kPA_Part] segments inside one CTA's run
-  int2* seg;            // [B][chunks][KV heads] of the others: their first and last CTA; -1 for those in `tail`
   unsigned int* err;
 };
 
@@ -88,14 +85,11 @@ struct PagedCfg {
   static constexpr int Smem = Units * kPA_Unit + 2 * QBytes + 2 * PBytes + 5120 + 1024;
 };
 
-// slot (-1: none) and visible length of sequence b; of a tail: without the skipped pages
-template <bool Tail>
+// slot (-1: none) and visible length of sequence b
 __device__ __forceinline__ int2 paged_seq(const PagedAttnArgs& a, int b) {
   const int slot = a.slots ? a.slots[b] : b;
   const bool ok = slot >= 0 && slot < a.p.slots;
-  int len = ok ? max(0, min(a.p.lens[slot], a.cap)) : 0;
-  if constexpr (Tail) len = max(0, len - a.skip[b] * a.p.page);
-  return make_int2(ok ? slot : -1, len);
+  return make_int2(ok ? slot : -1, ok ? max(0, min(a.p.lens[slot], a.cap)) : 0);
 }
 // tiles of a sequence: at least one, so that a segment that sees nothing has a CTA that writes its zeros
 __device__ __forceinline__ int paged_tiles(int len) { return max(1, (len + kPA_Tile - 1) / kPA_Tile); }
@@ -109,13 +103,12 @@ __device__ __forceinline__ int2 paged_row(const PagedAttnArgs& a, int r) {
 // a CTA's walk over its run of tiles; the run's first kPA_Seqs sequences are in shared memory, a load from L2 on every warp's
 // way to the next sequence would cost as much as half a tile
 constexpr int kPA_Seqs = 192;
-template <bool Tail>
 struct PagedWalk {
   int b, c, g, tile, ntiles, len, slot;
   int b0;
   const int2* seqs;      // (slot, length) of sequences b0, b0 + 1, ...
   __device__ __forceinline__ void enter(const PagedAttnArgs& a) {
-    const int2 x = b - b0 < kPA_Seqs ? seqs[b - b0] : paged_seq<Tail>(a, b);
+    const int2 x = b - b0 < kPA_Seqs ? seqs[b - b0] : paged_seq(a, b);
     slot = x.x;
     len = x.y;
     ntiles = paged_tiles(len);
@@ -167,7 +160,7 @@ __device__ __forceinline__ constexpr int col_row(int c) {
   return c % n * PagedCfg<RP>::Groups + c / n;
 }
 
-template <typename T, int RP, bool Tail>
+template <typename T, int RP>
 __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, PagedAttnArgs a) {
   using C = PagedCfg<RP>;
@@ -235,7 +228,7 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
   for (int i = 0; i < per; ++i) {
     const int b = tid * per + i;
     if (b < a.B) {
-      const int2 q = paged_seq<Tail>(a, b);
+      const int2 q = paged_seq(a, b);
       mine += (paged_tiles(q.y) + C::Start) * segs;
       if (known) s_seqs[b] = q;
     }
@@ -261,7 +254,7 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
   if (u0 < u1 && before <= u0 && u0 < before + mine) {
     int at = before;
     for (int b = tid * per;; ++b) {
-      const int n = paged_tiles(known ? s_seqs[b].y : paged_seq<Tail>(a, b).y) + C::Start;
+      const int n = paged_tiles(known ? s_seqs[b].y : paged_seq(a, b).y) + C::Start;
       if (u0 < at + n * segs) {
         s_start[0] = b;
         s_start[1] = (u0 - at) / n;
@@ -273,10 +266,10 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
   }
   __syncthreads();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  PagedWalk<Tail> w{};
+  PagedWalk w{};
   int count = 0;                  // tiles of the run
   if (!known) {
-    for (int i = tid; u0 < u1 && i < kPA_Seqs && s_start[0] + i < a.B; i += C::Threads) s_seqs[i] = paged_seq<Tail>(a, s_start[0] + i);
+    for (int i = tid; u0 < u1 && i < kPA_Seqs && s_start[0] + i < a.B; i += C::Threads) s_seqs[i] = paged_seq(a, s_start[0] + i);
     __syncthreads();
   }
   if (u0 < u1) {
@@ -288,7 +281,7 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
     w.enter(a);
     w.tile = max(s_start[2] - C::Start, 0);
     // walk the run's segments: the units of each that are tiles
-    PagedWalk<Tail> x = w;
+    PagedWalk x = w;
     for (int u = u0 - s_start[2]; u < u1;) {
       count += max(min(u + C::Start + x.ntiles, u1) - max(u + C::Start, u0), 0);
       u += x.ntiles + C::Start;
@@ -299,10 +292,10 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
   count = __shfl_sync(0xffffffffu, count, 0);
   const int L = a.p.page, ppt = kPA_Tile >> a.page_log;       // pages per tile
   // the page of this tile's page number `i`, -1 where there is none
-  auto page_of = [&](const PagedWalk<Tail>& x, int i) -> int {
+  auto page_of = [&](const PagedWalk& x, int i) -> int {
     const int j = x.tile * ppt + i;
     if (i >= ppt || (long long)j * L >= x.len) return -1;
-    const int page = a.p.table[(size_t)x.slot * a.p.width + j + (Tail ? a.skip[x.b] : 0)];
+    const int page = a.p.table[(size_t)x.slot * a.p.width + j];
     return page >= 0 && page < a.p.pages ? page : -1;
   };
 
@@ -463,7 +456,7 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
     // the queries: warp w of the 4 SG takes rows w, w + 4 SG, ..., lane l dims 8 l .. 8 l + 7
     constexpr int QW = 4 * SG;
     uint4 qraw[RP / QW];
-    auto q_load = [&](const PagedWalk<Tail>& nx) {
+    auto q_load = [&](const PagedWalk& nx) {
       const int i0 = nx.c * a.tc, nx_rows = min(a.tc, a.t - i0) * a.R;
 #pragma unroll
       for (int i = 0; i < RP / QW; ++i) {
@@ -476,7 +469,7 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
     };
     // the queries in qraw, of segment nx, which begins with tile `at` of the run; then nx and qraw are the next segment's.  Rows from
     // nx_rows on stay as they are, nothing reads their scores
-    auto q_store = [&](PagedWalk<Tail>& nx, int& at, int buf) {
+    auto q_store = [&](PagedWalk& nx, int& at, int buf) {
       const int nx_rows = min(a.tc, a.t - nx.c * a.tc) * a.R;
       uint8_t* dst = sQ + buf * C::QBytes + (lane >> 4) * (NP * 128) + (lane & 1) * 8;
 #pragma unroll
@@ -520,7 +513,7 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
       const int s = j & 1;
       if (first) {
         // store the next segment's queries (and, at the run's start, this one's before them)
-        PagedWalk<Tail> nx = w;
+        PagedWalk nx = w;
         int at = j;
         if (j) at += nx.skip(a);
 #pragma unroll 1
@@ -693,7 +686,6 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
         const int i0 = w.c * a.tc, rows = min(a.tc, a.t - i0) * a.R;
         const bool whole = from_start && last;
         float* part = a.part + ((size_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * RP * kPA_Part;
-        const bool to_out = whole && !Tail;
         // lane c: row of column c, its sum, maximum and place in the output
         const int rc = col_row<RP>(min(lane, RP - 1));
         const int2 ih = paged_row(a, rc);
@@ -706,8 +698,8 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
         const int row = ((w.b * a.t + i0 + ih.x) * a.H) + w.g * a.R + ih.y;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;       // nothing seen: zeros
         if (mine_row && warp == 4 + 4 * SG) {
-          if (!to_out)
-            *reinterpret_cast<float2*>((whole ? a.tail + (size_t)row * kPA_Part : part + rc * kPA_Part) + kPG_D) = make_float2(m, sum);
+          if (!whole)
+            *reinterpret_cast<float2*>(part + rc * kPA_Part + kPG_D) = make_float2(m, sum);
           else if (a.lse)
             a.lse[((size_t)w.b * a.H + w.g * a.R + ih.y) * a.t + i0 + ih.x] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
         }
@@ -718,9 +710,7 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
           const float f = __shfl_sync(0xffffffffu, inv, c);
           const int to = __shfl_sync(0xffffffffu, row, c), r = __shfl_sync(0xffffffffu, rc, c);
           if (r < rows) {
-            if (to_out) out[(size_t)to * kPG_D] = (T)(acc[0] * f);
-            else if (Tail && whole) a.tail[(size_t)to * kPA_Part + d] = acc[0];
-            else part[r * kPA_Part + d] = acc[0];
+            if (whole) out[(size_t)to * kPG_D] = (T)(acc[0] * f); else part[r * kPA_Part + d] = acc[0];
           }
 #pragma unroll
           for (int k = 0; k + 1 < RP; ++k) acc[k] = acc[k + 1];
@@ -731,8 +721,6 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
           const int t0 = unit - (w.ntiles - 1), longer = more * (each + 1);
           desc = make_int4(t0 < longer ? t0 / (each + 1) : more + (t0 - longer) / each, w.b, w.c, w.g);
         }
-        if (Tail && last && d == 0)
-          a.seg[((size_t)w.b * a.nqc + w.c) * a.p.heads + w.g] = whole ? make_int2(-1, -1) : make_int2(desc.x, (int)blockIdx.x);
         __syncwarp();
         if (lane == 0) mbar_arrive(seg_free + (seg & 1));
         ++seg;
@@ -742,7 +730,7 @@ __global__ void __launch_bounds__(PagedCfg<RP>::Threads, 1)
       ++unit;
       w.next(a);
     }
-    if (!Tail && d == 0) a.desc[blockIdx.x] = ok ? desc : make_int4(-1, 0, 0, 0);
+    if (d == 0) a.desc[blockIdx.x] = ok ? desc : make_int4(-1, 0, 0, 0);
   }
   tc_fence_before();
   __syncthreads();
@@ -827,76 +815,12 @@ static void paged_chunks(int t, int R, int* tc, int* nqc, int* rp) {
   *rp = (*tc * R + 7) / 8 * 8;
 }
 
-template <typename T, int RP, bool Tail>
+template <typename T, int RP>
 static int launch_paged(const CUtensorMap& kmap, const CUtensorMap& vmap, const PagedAttnArgs& a, int ctas, cudaStream_t stream) {
-  int rc = ensure_smem_attr((const void*)paged_attn_kernel<T, RP, Tail>, PagedCfg<RP>::Smem);
+  int rc = ensure_smem_attr((const void*)paged_attn_kernel<T, RP>, PagedCfg<RP>::Smem);
   if (rc) return rc;
-  rc = launch_early(paged_attn_kernel<T, RP, Tail>, dim3(ctas), PagedCfg<RP>::Threads, PagedCfg<RP>::Smem, stream, kmap, vmap, a);
-  if (rc || Tail) return rc;
-  return launch_early(paged_combine_kernel<T, RP>, dim3(ctas, 4), 256, 0, stream, a);
-}
-
-template <bool Tail>
-static int launch_paged(const PagedAttnArgs& a, int rp, int dtype, const DeviceState& st, cudaStream_t stream) {
-  CUtensorMap kmap, vmap;
-  int rc = paged_maps(a.p, &kmap, &vmap);
-  if (rc) return rc;
-  const int ctas = st.sm_count < kPA_MaxCtas ? st.sm_count : kPA_MaxCtas;
-  if (dtype == BF_BF16) {
-    if (rp == 8) return launch_paged<__nv_bfloat16, 8, Tail>(kmap, vmap, a, ctas, stream);
-    if (rp == 16) return launch_paged<__nv_bfloat16, 16, Tail>(kmap, vmap, a, ctas, stream);
-    return launch_paged<__nv_bfloat16, 24, Tail>(kmap, vmap, a, ctas, stream);
-  }
-  if (rp == 8) return launch_paged<__half, 8, Tail>(kmap, vmap, a, ctas, stream);
-  if (rp == 16) return launch_paged<__half, 16, Tail>(kmap, vmap, a, ctas, stream);
-  return launch_paged<__half, 24, Tail>(kmap, vmap, a, ctas, stream);
-}
-
-// the arguments that both forms share, after their checks; BF_ERR_UNSUPPORTED where 32 bits do not count the work
-static int paged_args(PagedAttnArgs& a, const void* q, long long q_sb, long long q_st, long long q_sh, const int32_t* slots, int B, int t, int H,
-                      float scale, unsigned int* err, int* rp) {
-  a.q = q;
-  a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
-  a.slots = slots;
-  a.B = B; a.t = t; a.H = H; a.R = H / a.p.heads;
-  paged_chunks(t, a.R, &a.tc, &a.nqc, rp);
-  a.page_log = a.p.page == 16 ? 4 : a.p.page == 32 ? 5 : a.p.page == 64 ? 6 : 7;
-  a.cap = (int)((long long)a.p.width * a.p.page < 0x7fffff00LL ? (long long)a.p.width * a.p.page : 0x7fffff00LL);
-  a.by_r = (65536u + a.R - 1) / a.R;
-  a.c2 = scale * kLog2e;
-  a.err = err;
-  // the tiles of all segments are counted, and the output's rows numbered, in 32 bits
-  if ((long long)B * a.nqc * a.p.heads * (a.cap / kPA_Tile + 4) > 0x7fffffffLL || (long long)B * t * H > 0x7fffffffLL) return BF_ERR_UNSUPPORTED;
-  return BF_OK;
-}
-
-int paged_maps(const PagePool& p, CUtensorMap* kmap, CUtensorMap* vmap) {
-  const uint64_t dims[2] = {(uint64_t)kPG_D, (uint64_t)p.pages * p.heads * p.page}, strides[1] = {(uint64_t)kPG_D};
-  const uint32_t box[2] = {128, (uint32_t)p.page};
-  const int rc = make_tmap(kmap, p.k, kTmapU8, 2, dims, strides, box, true);
-  return rc ? rc : make_tmap(vmap, p.v, kTmapU8, 2, dims, strides, box, true);
-}
-
-size_t paged_tail_workspace(int B, int t, int H, int G) {
-  int tc, nqc, rp;
-  paged_chunks(t, H / G, &tc, &nqc, &rp);
-  const size_t seg = ((size_t)B * nqc * G * sizeof(int2) + 15) / 16 * 16;
-  return seg + ((size_t)kPA_MaxCtas * 2 * rp + (size_t)B * t * H) * kPA_Part * 4;
-}
-
-int paged_tail(const PagePool& p, const void* q, long long q_sb, long long q_st, long long q_sh, const int32_t* slots, const int32_t* skip, int B,
-               int t, int H, int dtype, float scale, void* ws, const DeviceState& st, cudaStream_t stream, PagedTail* out) {
-  PagedAttnArgs a{};
-  a.p = p;
-  const int rc = paged_args(a, q, q_sb, q_st, q_sh, slots, B, t, H, scale, st.err, &out->rp);
-  if (rc) return rc;
-  a.skip = skip;
-  a.seg = static_cast<int2*>(ws);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + ((size_t)B * a.nqc * p.heads * sizeof(int2) + 15) / 16 * 16);
-  a.tail = a.part + (size_t)kPA_MaxCtas * 2 * out->rp * kPA_Part;
-  out->seg = a.seg; out->part = a.part; out->tail = a.tail;
-  out->tc = a.tc; out->nqc = a.nqc;
-  return launch_paged<true>(a, out->rp, dtype, st, stream);
+  rc = launch_early(paged_attn_kernel<T, RP>, dim3(ctas), PagedCfg<RP>::Threads, PagedCfg<RP>::Smem, stream, kmap, vmap, a);
+  return rc ? rc : launch_early(paged_combine_kernel<T, RP>, dim3(ctas, 4), 256, 0, stream, a);
 }
 
 }  // namespace bfb
@@ -928,13 +852,38 @@ int bf_paged_attend(const bf_page_pool* pool, int layer, const void* q, long lon
   if (!aligned16(ws)) return BF_ERR_ALIGNMENT;
   DeviceState st;
   if ((rc = device_state(&st))) return rc;
+  a.q = q;
+  a.q_sb = q_sb; a.q_st = q_st; a.q_sh = q_sh;
+  a.slots = slots;
+  a.B = B; a.t = t; a.H = H; a.R = H / a.p.heads;
   int rp;
-  if ((rc = paged_args(a, q, q_sb, q_st, q_sh, slots, B, t, H, scale, st.err, &rp))) return rc;
+  paged_chunks(t, a.R, &a.tc, &a.nqc, &rp);
+  a.page_log = a.p.page == 16 ? 4 : a.p.page == 32 ? 5 : a.p.page == 64 ? 6 : 7;
+  a.cap = (int)((long long)a.p.width * a.p.page < 0x7fffff00LL ? (long long)a.p.width * a.p.page : 0x7fffff00LL);
+  a.by_r = (65536u + a.R - 1) / a.R;
+  // the tiles of all segments are counted, and the output's rows numbered, in 32 bits
+  if ((long long)B * a.nqc * a.p.heads * (a.cap / kPA_Tile + 4) > 0x7fffffffLL || (long long)B * t * H > 0x7fffffffLL)
+    return BF_ERR_UNSUPPORTED;
+  a.c2 = scale * kLog2e;
   a.o = o;
   a.lse = lse;
   a.desc = static_cast<int4*>(ws);
   a.part = reinterpret_cast<float*>(a.desc + kPA_MaxCtas);
-  return launch_paged<false>(a, rp, dtype, st, stream);
+  a.err = st.err;
+  CUtensorMap kmap, vmap;
+  const uint64_t dims[2] = {(uint64_t)kPG_D, (uint64_t)a.p.pages * a.p.heads * a.p.page}, strides[1] = {(uint64_t)kPG_D};
+  const uint32_t box[2] = {128, (uint32_t)a.p.page};
+  if ((rc = make_tmap(&kmap, a.p.k, kTmapU8, 2, dims, strides, box, true))) return rc;
+  if ((rc = make_tmap(&vmap, a.p.v, kTmapU8, 2, dims, strides, box, true))) return rc;
+  const int ctas = st.sm_count < kPA_MaxCtas ? st.sm_count : kPA_MaxCtas;
+  if (dtype == BF_BF16) {
+    if (rp == 8) return launch_paged<__nv_bfloat16, 8>(kmap, vmap, a, ctas, stream);
+    if (rp == 16) return launch_paged<__nv_bfloat16, 16>(kmap, vmap, a, ctas, stream);
+    return launch_paged<__nv_bfloat16, 24>(kmap, vmap, a, ctas, stream);
+  }
+  if (rp == 8) return launch_paged<__half, 8>(kmap, vmap, a, ctas, stream);
+  if (rp == 16) return launch_paged<__half, 16>(kmap, vmap, a, ctas, stream);
+  return launch_paged<__half, 24>(kmap, vmap, a, ctas, stream);
 }
 
 }  // extern "C"
