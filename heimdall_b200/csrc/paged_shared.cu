@@ -19,8 +19,8 @@
 // Kernels: paged_queries_kernel makes the query parts, paged_shared_kernel the partials, paged_merge_kernel the output, in a fixed order.
 // Work of the second: the tiles of all (run or tail, KV head, row block) in one line, cut into equal pieces, one CTA per SM; an item's start counts as
 // kSH_Start tiles.
-// Warps: 0 the walk along the line, TMA of the queries and of K; 1 the products S; 2 TMA of V; 3 the products O; two warpgroups of softmax (thread = row),
-// every other tile each; two of accumulators (thread = row and half of the dims).  What the others have to know of a tile (pages, scales, where
+// Warps: 0 the walk along the line, TMA of the queries and of K; 1 the products S; 2 TMA of V; 3 the products O; two warpgroups of softmax (thread = row
+// and half of the tokens: what a tile waits for is one thread's way through its scores, 4600 cycles for all 128); two of accumulators (thread = row and half of the dims).  What the others have to know of a tile (pages, scales, where
 // an item begins and ends) comes from warp 0 through a ring of four entries.
 #include "bifrost_b200.h"
 #include "capi_internal.h"
@@ -67,7 +67,7 @@ struct SharedSmem {
   using C = SharedCfg<T>;
   static constexpr int Q = C::Parts * 2 * kSH_Unit;
   static constexpr int Tiles = (C::NK + C::NV) * kSH_Unit + Q;
-  static constexpr int Bytes = Tiles + 512 + 4 * (int)sizeof(SharedTile) + 2 * kSH_M * 8 + 1024;
+  static constexpr int Bytes = Tiles + 512 + 4 * (int)sizeof(SharedTile) + 8 * kSH_M * 8 + 1024;
 };
 static_assert(SharedSmem<__half>::Bytes <= 232448 && SharedSmem<__nv_bfloat16>::Bytes <= 232448, "shared memory");
 
@@ -121,18 +121,15 @@ struct Stretch {
   __device__ __forceinline__ int units(int heads) const { return tokens > 0 ? heads * blocks() * (tiles() + kSH_Start) : 0; }
 };
 
-// two values as e4m3 parts that add up; each remainder is exact in fp16
-template <int Parts>
-__device__ __forceinline__ void split_sum(__half2 x, uint16_t (&part)[Parts]) {
-#pragma unroll
-  for (int i = 0; i < Parts; ++i) {
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(part[i]) : "r"(*reinterpret_cast<uint32_t*>(&x)));
-    if (i + 1 < Parts) {
-      uint32_t f;
-      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(f) : "h"(part[i]));
-      x = __hsub2(x, *reinterpret_cast<__half2*>(&f));
-    }
-  }
+__device__ __forceinline__ uint16_t to_e4m3(__half2 x) {      // two values
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<uint32_t*>(&x)));
+  return r;
+}
+__device__ __forceinline__ __half2 from_e4m3(uint16_t x) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(x));
+  return *reinterpret_cast<__half2*>(&r);
 }
 
 // The query parts: a warp a row, in the order of the plan's places, lane l dims 8 l .. 8 l + 7.
@@ -160,7 +157,13 @@ __global__ void __launch_bounds__(256) paged_queries_kernel(SharedArgs a) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const T* e = reinterpret_cast<const T*>(&v[k]);
-    split_sum<Parts>(__floats2half2_rn(fin ? (float)e[0] * up : 0.f, fin ? (float)e[1] * up : 0.f), c[k]);
+    // parts that add up; each remainder is exact in fp16
+    __half2 x = __floats2half2_rn(fin ? (float)e[0] * up : 0.f, fin ? (float)e[1] * up : 0.f);
+#pragma unroll
+    for (int p = 0; p < Parts; ++p) {
+      c[k][p] = to_e4m3(x);
+      x = __hsub2(x, from_e4m3(c[k][p]));
+    }
   }
   const size_t at = (size_t)g * rows + row;
 #pragma unroll
@@ -182,10 +185,7 @@ __device__ __forceinline__ void umma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uin
 __device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
-// x * f + acc * al, in its place among the volatile instructions around it: pure ones would all be computed ahead, in registers that there are not
-__device__ __forceinline__ void rescale_add(uint64_t& acc, uint64_t al, uint64_t x, uint64_t f) {
-  asm volatile("mul.rn.f32x2 %0, %0, %1;\n\tfma.rn.f32x2 %0, %2, %3, %0;" : "+l"(acc) : "l"(al), "l"(x), "l"(f));
-}
+__device__ __forceinline__ uint64_t scale2(uint64_t a, float f) { return pair2(lo_hi(a, 0) * f, lo_hi(a, 1) * f); }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   int* s_sum = reinterpret_cast<int*>(bars + 38);      // [20][2] per-warp totals
   int* s_start = reinterpret_cast<int*>(bars + 59);    // stretch, unit in it, rows before it
   SharedTile* s_tile = reinterpret_cast<SharedTile*>(bars + 64);  // [4]
-  float2* s_ml = reinterpret_cast<float2*>(s_tile + 4);           // [2][128] a tile's maxima and sums
+  float2* s_ml = reinterpret_cast<float2*>(s_tile + 4);           // [4][2][128] a tile's maxima and sums, of both halves of its tokens
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 4; ++i) {
@@ -219,11 +219,11 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
       mbar_init(v_full + i, 1);
       mbar_init(v_empty + i, 1);
       mbar_init(t_full + i, 1);
-      mbar_init(t_free + i, 15);       // V, S, O, four of softmax, eight accumulators
+      mbar_init(t_free + i, 19);       // V, S, O, eight of softmax, eight accumulators
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 4);
+      mbar_init(p_full + i, 8);
       mbar_init(p_free + i, 1);
       mbar_init(o_free + i, 8);
     }
@@ -414,10 +414,8 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
           in = 0;
         }
       }
-      // the end of the line, for both warpgroups of softmax
-#pragma unroll 1
-      for (int end = j + 2; j < end && ok; ++j) {
-        if (j >= 4 && !(ok = mbar_wait_warp_small(t_free + (j & 3), ((j >> 2) - 1) & 1, abort, 0x92))) break;
+      // the end of the line
+      if (ok && (j < 4 || (ok = mbar_wait_warp_small(t_free + (j & 3), ((j >> 2) - 1) & 1, abort, 0x92)))) {
         if (lane == 0) {
           s_tile[j & 3].stop = 1;
           mbar_arrive(t_full + (j & 3));
@@ -436,9 +434,8 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         if (lane == 0) mbar_arrive(t_free + (j & 3));
         if (first && !(ok = mbar_wait_warp_small(q_full, items & 1, abort, 0x94))) break;
         items += first;
-        // tile j - 2's weights, which lie over S, have been read, and the accumulators have its maxima
+        // tile j - 2's weights, which lie over S, have been read
         if (j >= 2 && !(ok = mbar_wait_warp_small(p_free + s, ((j >> 1) - 1) & 1, abort, 0x95))) break;
-        if (j >= 2 && !(ok = mbar_wait_warp_small(o_free + s, ((j >> 1) - 1) & 1, abort, 0x96))) break;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           if (!(ok = mbar_wait_warp_small(k_full + u, uphase, abort, 0x97))) break;
@@ -534,16 +531,17 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   } else {
     const int wq = warp & 3, r = wq * 32 + lane;      // this thread's row
     if (warp < 12) {
-      // ---------------------------------------------------------------- softmax: thread = row, every other tile
+      // ---------------------------------------------------------------- softmax: thread = row and half of the tokens
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSH_RegsSoftmax));
-      const int s = (warp - 4) >> 2;
-      const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + s * kSH_N;
+      const int hh = (warp - 4) >> 2, c0 = 64 * hh;
       float qs = 0.f;
       int limit = -1, rows = 0, item = 0;            // the last position that the row sees
 #pragma unroll 1
-      for (int j = s; tile(j); j += 2) {
+      for (int j = 0; tile(j); ++j) {
+        const int s = j & 1;
+        const uint32_t trow = tmem + ((uint32_t)(wq * 32) << 16) + s * kSH_N;
         const SharedTile& d = s_tile[j & 3];
-        if (d.item != item) {                         // an item that this warpgroup has not met
+        if (d.item != item) {
           item = d.item;
           rows = d.rows;
           limit = -1;
@@ -562,26 +560,22 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         const bool all = whole && __all_sync(0xffffffffu, vis == kSH_N || r >= rows);
         if (!whole) {
           // the values of tokens that are not there may be anything (a weight of 0 times NaN would be NaN): zeros
-#pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
-            const int n = 2 * j + half, u = n % NV;
-            if (!(ok = mbar_wait_warp_small(v_full + u, (n / NV) & 1, abort, 0x9c))) break;
-            if (r >= valid || !((have >> (r >> a.page_log)) & 1u)) {
-              uint4* row = reinterpret_cast<uint4*>(ring + (NK + u) * kSH_Unit + r * 128);
+          const int n = 2 * j + hh, u = n % NV;
+          if (!(ok = mbar_wait_warp_small(v_full + u, (n / NV) & 1, abort, 0x9c))) break;
+          if (r >= valid || !((have >> (r >> a.page_log)) & 1u)) {
+            uint4* row = reinterpret_cast<uint4*>(ring + (NK + u) * kSH_Unit + r * 128);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) row[(i + r) & 7] = make_uint4(0u, 0u, 0u, 0u);     // rows are as long as all banks
-            }
+            for (int i = 0; i < 8; ++i) row[(i + r) & 7] = make_uint4(0u, 0u, 0u, 0u);     // rows are as long as all banks
           }
-          if (!ok) break;
           fence_async_smem();
         }
         if (!(ok = mbar_wait_warp_small(s_full + s, (j >> 1) & 1, abort, 0x9d))) break;
         tc_fence_after();
-        float mt = -INFINITY, lt = 0.f;
         if (busy) {
           // two ways through the row's scores (they do not fit the registers): its largest, then the weights
+          float mt = -INFINITY, lt = 0.f;
 #pragma unroll 1
-          for (int c = 0; c < kSH_N; c += 32) {
+          for (int c = c0; c < c0 + 64; c += 32) {
             uint32_t x[32];
             tmem_ld32(trow + c, x);
             tmem_wait_ld();
@@ -602,43 +596,66 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
               mt = fmaxf(mt, fmaf(fmaxf(m0, m1), d.ks[pi] * qs, d.e[pi]));
             }
           }
+          // the row's maximum of both halves (the two warps of these rows meet)
+          float2* ml = s_ml + (j & 3) * 2 * kSH_M + r;
+          ml[hh * kSH_M].x = mt;
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + wq) : "memory");
+          mt = fmaxf(mt, ml[(hh ^ 1) * kSH_M].x);
           const float ref = 8.f - (mt == -INFINITY ? 0.f : mt);       // the largest weight becomes 2^8
+          // 16 tokens at a time, the next 16 scores on their way; every step for all of them before the next one, a value's own way through the
+          // steps takes 60 cycles
+          uint32_t x[16];
+          tmem_ld16(trow + c0, x);
+          tmem_wait_ld();
 #pragma unroll 1
-          for (int c = 0; c < kSH_N; c += 32) {
-            uint32_t x[32];
-            tmem_ld32(trow + c, x);
-            tmem_wait_ld();
+          for (int c = c0; c < c0 + 64; c += 16) {
+            const int pi = c >> a.page_log;
             if (!all) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c + i >= vis || !((have >> ((c + i) >> a.page_log)) & 1u)) x[i] = 0xff800000u;
+              for (int i = 0; i < 16; ++i)
+                if (c + i >= vis || !((have >> pi) & 1u)) x[i] = 0xff800000u;
             }
+            const float f = d.ks[pi] * qs, off = d.e[pi] + ref;
+            const uint64_t f2 = pair2(f, f), off2 = pair2(off, off);
+            float w[16];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int pi = (c + 16 * q) >> a.page_log;
-              const float f = d.ks[pi] * qs, off = d.e[pi] + ref;
-              const uint64_t f2 = pair2(f, f), off2 = pair2(off, off);
-              uint64_t sum = 0;
-              uint32_t out[Parts][4];
+            for (int i = 0; i < 8; ++i) {
+              const uint64_t y = fma2(pair2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f2, off2);
+              w[2 * i] = lo_hi(y, 0);
+              w[2 * i + 1] = lo_hi(y, 1);
+            }
+            if (c + 16 < c0 + 64) tmem_ld16(trow + c + 16, x);
 #pragma unroll
-              for (int i = 0; i < 16; i += 2) {
-                const uint64_t y = fma2(pair2(__uint_as_float(x[16 * q + i]), __uint_as_float(x[16 * q + i + 1])), f2, off2);
-                const float w0 = ex2_approx(lo_hi(y, 0)), w1 = ex2_approx(lo_hi(y, 1));
-                sum = add2(sum, pair2(w0, w1));
-                uint16_t pt[Parts];
-                split_sum<Parts>(__floats2half2_rn(w0, w1), pt);
+            for (int i = 0; i < 16; ++i) w[i] = ex2_approx(w[i]);
+            uint64_t sum = 0;
+            __half2 h[8];
 #pragma unroll
-                for (int p = 0; p < Parts; ++p) out[p][i >> 2] = (i & 2) ? out[p][i >> 2] | ((uint32_t)pt[p] << 16) : pt[p];
+            for (int i = 0; i < 8; ++i) {
+              sum = add2(sum, pair2(w[2 * i], w[2 * i + 1]));
+              h[i] = __floats2half2_rn(w[2 * i], w[2 * i + 1]);
+            }
+            lt = fmaf(lo_hi(sum, 0) + lo_hi(sum, 1), d.inv[pi], lt);
+            uint32_t out[Parts][4];
+#pragma unroll
+            for (int p = 0; p < Parts; ++p) {
+              uint16_t e[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) e[i] = to_e4m3(h[i]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) out[p][i] = e[2 * i] | ((uint32_t)e[2 * i + 1] << 16);
+              if (p + 1 < Parts) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[i] = __hsub2(h[i], from_e4m3(e[i]));
               }
-              lt = fmaf(lo_hi(sum, 0) + lo_hi(sum, 1), d.inv[pi], lt);
-              // the 32 tokens' parts take the place of their scores
-#pragma unroll
-              for (int p = 0; p < Parts; ++p) tmem_st4(trow + c + 8 * p + 4 * q, out[p]);
             }
+            // the tokens' parts take the place of scores that have been read: of 32 tokens in the columns of those
+            tmem_wait_ld();
+#pragma unroll
+            for (int p = 0; p < Parts; ++p) tmem_st4(trow + (c & ~31) + 8 * p + ((c >> 2) & 4), out[p]);
           }
           tmem_wait_st();
+          ml[hh * kSH_M].y = lt;
         }
-        s_ml[s * kSH_M + r] = make_float2(mt, lt);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -652,7 +669,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
       const int half = (warp - 12) >> 2;
       const uint32_t trow = tmem + 256 + half * 128 + ((uint32_t)(wq * 32) << 16);
       uint64_t acc[64];
-      float m_run = -INFINITY, l = 0.f;
+      float m_ref = -INFINITY, l = 0.f;
 #pragma unroll
       for (int i = 0; i < 64; ++i) acc[i] = 0;
 #pragma unroll 1
@@ -660,33 +677,42 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         const int rows = s_tile[j & 3].rows, base = s_tile[j & 3].base;
         const bool end = s_tile[j & 3].last, busy = wq * 32 < rows;
         if (s_tile[j & 3].first) {       // (zeroed at the end of an item instead, the compiler keeps the accumulators twice)
-          m_run = -INFINITY;
+          m_ref = -INFINITY;
           l = 0.f;
 #pragma unroll
           for (int i = 0; i < 64; ++i) acc[i] = 0;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(t_free + (j & 3));
         if (!(ok = mbar_wait_warp_small(p_full + (j & 1), (j >> 1) & 1, abort, 0x9e))) break;      // the tile's maxima
         float2 t = make_float2(-INFINITY, 0.f);
-        if (busy) t = s_ml[(j & 1) * kSH_M + r];
-        const float mn = fmaxf(m_run, t.x);
+        if (busy) {
+          const float2 *ml = s_ml + (j & 3) * 2 * kSH_M + r, t0 = ml[0], t1 = ml[kSH_M];
+          t = make_float2(fmaxf(t0.x, t1.x), t0.y + t1.y);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(t_free + (j & 3));      // the entry and the maxima may be written over
+        // the accumulators are relative to the first tile's maximum, until one is 2^40 times it: then to that
+        if (t.x > m_ref + 40.f) {
+          const float al = m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - t.x);
+          l *= al;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) acc[i] = scale2(acc[i], al);
+          m_ref = t.x;
+        }
         // (a tile without a maximum holds zeros, or NaN to be passed on)
-        const float alf = m_run == -INFINITY ? 0.f : ex2_approx(m_run - mn), ff = t.x == -INFINITY ? 1.f / 256.f : ex2_approx(t.x - mn) * (1.f / 256.f);
-        l = l * alf + t.y * ff;
-        m_run = mn;
-        const uint64_t al = pair2(alf, alf), f = pair2(ff, ff);
+        const float ff = t.x == -INFINITY ? 1.f / 256.f : ex2_approx(t.x - m_ref) * (1.f / 256.f);
+        l = fmaf(t.y, ff, l);
+        const uint64_t f = pair2(ff, ff);
         if (!(ok = mbar_wait_warp_small(o_full, j & 1, abort, 0x9f))) break;
         tc_fence_after();
         if (busy) {
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            uint32_t x[8];
-            tmem_ld8(trow + 8 * c, x);
+          for (int c = 0; c < 8; ++c) {
+            uint32_t x[16];
+            tmem_ld16(trow + 16 * c, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              rescale_add(acc[4 * c + i], al, pair2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f);
+            for (int i = 0; i < 8; ++i)
+              acc[8 * c + i] = fma2(pair2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), f, acc[8 * c + i]);
           }
         }
         tc_fence_before();
@@ -696,7 +722,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
           if (r < rows) {
             // a piece lies dim by dim, so that 32 rows are neighbours
             const size_t row0 = (size_t)blockIdx.x * kSH_M + base;
-            if (half == 0) a.ml[row0 + r] = make_float2(m_run, l);
+            if (half == 0) a.ml[row0 + r] = make_float2(m_ref, l);
             float* to = a.part + row0 * kPG_D + (size_t)half * 128 * rows + r;
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
