@@ -36,7 +36,7 @@ constexpr int kSH_MaxGroup = 24;                     // query heads per KV head,
 constexpr int kSH_M = 128, kSH_N = 128;              // rows, tokens of a tile
 constexpr int kSH_Unit = 128 * 128;                  // bytes of half a K or V tile: 128 tokens, 128 dims
 constexpr int kSH_Threads = 640;
-constexpr int kSH_Start = 2;
+constexpr int kSH_Start = 1;
 // register split (setmaxnreg) of the 96 per thread at launch
 constexpr uint32_t kSH_RegsCtl = 48, kSH_RegsSoftmax = 64, kSH_RegsAcc = 152;
 static_assert(kSH_RegsCtl + 2 * kSH_RegsSoftmax + 2 * kSH_RegsAcc <= 5 * 96, "register split");
@@ -71,6 +71,12 @@ struct SharedSmem {
 };
 static_assert(SharedSmem<__half>::Bytes <= 232448 && SharedSmem<__nv_bfloat16>::Bytes <= 232448, "shared memory");
 
+struct SharedRecord {
+  int unit, before;     // its first unit, the rows before it
+  int rows, tiles;      // its rows per KV head, its tiles (0: no pieces)
+  int first, next;      // its first place, the run before it on its sequences' way (-1: none)
+  int pad[2];
+};
 struct SharedArgs {
   PagePool p;
   const void* q;
@@ -82,7 +88,7 @@ struct SharedArgs {
   uint8_t* qp;          // [KV heads][n t R rows, in the plan's order][parts][256]
   float* qs;            // [KV heads][n t R] the rows' scales
   int4* head;           // units per CTA, CTAs with one more, -, -
-  int2* at;             // [runs + n] the first unit of a run, or of the tail of the sequence at a place, and the rows before it
+  SharedRecord* at;     // [runs + n] where a run, or the tail of the sequence at a place, lies in the line
   float* part;          // [CTAs * 128 + rows][256], a piece's rows x dims transposed
   float2* ml;           // [CTAs * 128 + rows] maximum, sum
   void* o;
@@ -283,7 +289,11 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
       if (e >= stretches) break;
       const Stretch x(a, pl, e);
       const int units = x.units(a.p.heads);
-      if (blockIdx.x == 0) a.at[e] = at;
+      if (blockIdx.x == 0) {
+        SharedRecord* to = a.at + e;
+        *reinterpret_cast<int4*>(to) = make_int4(at.x, at.y, x.rows, x.tiles());
+        *reinterpret_cast<int2*>(&to->first) = make_int2(x.first, e < pl.n_runs ? pl.runs[(size_t)e * kPS_Run + 4] : pl.last[pl.order[x.first]]);
+      }
       if (u0 < u1 && at.x <= u0 && u0 < at.x + units) {
         s_start[0] = e;
         s_start[1] = u0 - at.x;
@@ -572,6 +582,21 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         if (!(ok = mbar_wait_warp_small(s_full + s, (j >> 1) & 1, abort, 0x9d))) break;
         tc_fence_after();
         if (busy) {
+          if (!all) {
+            // scores of what the row does not see: -infinity, in a way of its own (in the loops below it would cost every tile)
+#pragma unroll 1
+            for (int c = c0; c < c0 + 64; c += 16) {
+              uint32_t x[16];
+              tmem_ld16(trow + c, x);
+              tmem_wait_ld();
+              const int seen = (have >> (c >> a.page_log)) & 1u ? vis - c : 0;
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (i >= seen) x[i] = 0xff800000u;
+              tmem_st16(trow + c, x);
+            }
+            tmem_wait_st();
+          }
           // two ways through the row's scores (they do not fit the registers): its largest, then the weights
           float mt = -INFINITY, lt = 0.f;
 #pragma unroll 1
@@ -579,11 +604,6 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
             uint32_t x[32];
             tmem_ld32(trow + c, x);
             tmem_wait_ld();
-            if (!all) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c + i >= vis || !((have >> ((c + i) >> a.page_log)) & 1u)) x[i] = 0xff800000u;
-            }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               float m0 = __uint_as_float(x[16 * q]), m1 = __uint_as_float(x[16 * q + 1]);
@@ -610,11 +630,6 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
 #pragma unroll 1
           for (int c = c0; c < c0 + 64; c += 16) {
             const int pi = c >> a.page_log;
-            if (!all) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (c + i >= vis || !((have >> pi) & 1u)) x[i] = 0xff800000u;
-            }
             const float f = d.ks[pi] * qs, off = d.e[pi] + ref;
             const uint64_t f2 = pair2(f, f), off2 = pair2(off, off);
             float w[16];
@@ -745,70 +760,113 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   }
 }
 
-// Output rows: a warp has 32 neighbouring rows of one KV head, in the plan's order (they are neighbours in every piece too), and 16 dims; a lane adds its
-// row's pieces run by run, CTA by CTA, the tail first, then the runs from the last one up.
-template <typename T>
+// Output rows: a block has 32 neighbouring rows of one KV head, in the plan's order (they are neighbours in every piece too), and 16 dims for each of its
+// 8 / Split groups of warps; a lane has a row, and the row's pieces (tail, then its runs from the last one up, CTA by CTA) are dealt to a group's
+// Split warps, whose sums are added in order.  The first warp finds where the rows' pieces lie.  (With one warp for all pieces of its rows, the 37 of a long
+// document took 40 us one after the other; split over eight, the 13 of 64 sequences took longer than over four.)
+constexpr int kSH_MergeDims = 16;
+template <typename T, int Split>
 __global__ void __launch_bounds__(256) paged_merge_kernel(SharedArgs a) {
+  constexpr int Groups = 8 / Split, Ways = kPS_Depth + 1;
+  __shared__ float s_acc[8][kSH_MergeDims][32];
+  __shared__ float2 s_sum[8][32];
+  __shared__ int4 s_way[Ways][32];       // first CTA, pieces, rows of a piece, row of it
+  __shared__ int s_base[Ways][32], s_out[32];
   wait_for_stream();
   let_next_start();
-  const int lane = threadIdx.x & 31, d0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * 16, g = blockIdx.z;
-  const Plan pl(a.plan, a.n);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = warp / Split, split = warp % Split;
+  const int d0 = (blockIdx.y * Groups + group) * kSH_MergeDims, g = blockIdx.z;
   const int per_seq = a.t * a.R;
   const long long sr = (long long)blockIdx.x * 32 + lane;
-  if (sr >= (long long)a.n * per_seq) return;
-  const int place = (int)(sr / per_seq), rem = (int)(sr - (long long)place * per_seq), i = rem / a.R, hh = rem - i * a.R;
-  const int b = pl.order[place], h = g * a.R + hh;
-  const int4 head = *a.head;
-  const int each = head.x, more = head.y, longer = more * (each + 1);
-  auto cta_of = [&](int u) { return u < longer ? u / (each + 1) : more + (u - longer) / each; };
-  float m = -INFINITY, sum = 0.f, acc[16];
+  const bool on = sr < (long long)a.n * per_seq;
+  if (warp == 0) {
+    const Plan pl(a.plan, a.n);
+    const int place = on ? (int)(sr / per_seq) : 0, rem = on ? (int)(sr - (long long)place * per_seq) : 0, i = rem / a.R;
+    const int4 head = *a.head;
+    const int each = head.x, more = head.y, longer = more * (each + 1);
+    auto cta_of = [&](int u) { return u < longer ? u / (each + 1) : more + (u - longer) / each; };
+    int e = on ? pl.n_runs + place : -1;
 #pragma unroll
-  for (int k = 0; k < 16; ++k) acc[k] = 0.f;
-  auto add = [&](float2 ml, const float (&v)[16]) {
-    // a partial without a maximum holds zeros, or NaN to be passed on
-    const float mn = fmaxf(m, ml.x);
-    const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mn);
-#pragma unroll
-    for (int k = 0; k < 16; ++k) acc[k] = acc[k] * al + v[k] * f;
-    sum = sum * al + ml.y * f;
-    m = mn;
-  };
-  for (int e = pl.n_runs + place, guard = 0; guard <= kPS_Depth; ++guard) {
-    const Stretch x(a, pl, e);
-    if (x.tokens > 0) {
-      const int blocks = x.blocks(), idx = (place - x.first) * per_seq + rem, rb = idx / kSH_M, in = idx - rb * kSH_M;
-      const int ntiles = x.tiles(), block_rows = min(kSH_M, x.rows - rb * kSH_M);
-      const int2 at = a.at[e];
-      const int u = at.x + (g * blocks + rb) * (ntiles + kSH_Start) + kSH_Start;
-      const size_t base = (size_t)at.y + (size_t)g * x.rows + rb * kSH_M;
-      const int c1 = cta_of(u + ntiles - 1);
-      for (int c = cta_of(u); c <= c1; c += 2) {
-        float v[2][16];
-        float2 ml[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const size_t row0 = (size_t)min(c + k, c1) * kSH_M + base;
-          ml[k] = a.ml[row0 + in];
-          const float* p = a.part + row0 * kPG_D + (size_t)d0 * block_rows + in;
-#pragma unroll
-          for (int q = 0; q < 16; ++q) v[k][q] = p[(size_t)q * block_rows];
+    for (int k = 0; k < Ways; ++k) {
+      int4 way = make_int4(0, 0, 1, 0);
+      int base = 0;
+      if (e >= 0 && e < pl.n_runs + a.n) {
+        const int4 x = *reinterpret_cast<const int4*>(a.at + e);
+        const int2 y = *reinterpret_cast<const int2*>(&a.at[e].first);
+        if (x.w > 0) {
+          const int blocks = (x.z + kSH_M - 1) / kSH_M, idx = (place - y.x) * per_seq + rem, rb = idx / kSH_M;
+          const int u = x.x + (g * blocks + rb) * (x.w + kSH_Start) + kSH_Start, c0 = cta_of(u);
+          way = make_int4(c0, cta_of(u + x.w - 1) - c0 + 1, min(kSH_M, x.z - rb * kSH_M), idx - rb * kSH_M);
+          base = x.y + g * x.z + rb * kSH_M;
         }
-        add(ml[0], v[0]);
-        if (c < c1) add(ml[1], v[1]);
+        e = y.y < pl.n_runs ? y.y : -1;
       }
+      s_way[k][lane] = way;
+      s_base[k][lane] = base;
     }
-    e = e >= pl.n_runs ? pl.last[b] : pl.runs[(size_t)e * kPS_Run + 4];
-    if (e < 0 || e >= pl.n_runs) break;
+    s_out[lane] = (pl.order[place] * a.t + i) * a.H + g * a.R + rem - i * a.R;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;       // nothing seen: zeros
-  uint4 out[2];
-  T* o = reinterpret_cast<T*>(out);
+  __syncthreads();
+  float m = -INFINITY, sum = 0.f, acc[kSH_MergeDims];
 #pragma unroll
-  for (int k = 0; k < 16; ++k) o[k] = (T)(acc[k] * inv);
-  uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + (((size_t)b * a.t + i) * a.H + h) * kPG_D + d0);
-  to[0] = out[0];
-  to[1] = out[1];
-  if (a.lse && d0 == 0) a.lse[((size_t)b * a.H + h) * a.t + i] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * kLn2;
+  for (int k = 0; k < kSH_MergeDims; ++k) acc[k] = 0.f;
+  int mine = split;                        // pieces until this warp's next one
+  for (int k = 0; k < Ways; ++k) {
+    const int4 way = s_way[k][lane];
+    const int base = s_base[k][lane];
+#pragma unroll 2
+    for (; mine < way.y; mine += Split) {
+      const size_t row0 = (size_t)(way.x + mine) * kSH_M + base;
+      const float2 ml = a.ml[row0 + way.w];
+      const float* p = a.part + row0 * kPG_D + (size_t)d0 * way.z + way.w;
+      float v[kSH_MergeDims];
+#pragma unroll
+      for (int q = 0; q < kSH_MergeDims; ++q) v[q] = p[(size_t)q * way.z];
+      // a partial without a maximum holds zeros, or NaN to be passed on
+      const float mn = fmaxf(m, ml.x);
+      const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mn);
+#pragma unroll
+      for (int q = 0; q < kSH_MergeDims; ++q) acc[q] = acc[q] * al + v[q] * f;
+      sum = sum * al + ml.y * f;
+      m = mn;
+    }
+    mine -= way.y;
+  }
+#pragma unroll
+  for (int k = 0; k < kSH_MergeDims; ++k) s_acc[warp][k][lane] = acc[k];
+  s_sum[warp][lane] = make_float2(m, sum);
+  __syncthreads();
+  // each warp 16 / Split of its group's dims
+  constexpr int Dims = kSH_MergeDims / Split;
+  const int w0 = group * Split;
+  float f[Split], l = 0.f;
+  m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < Split; ++k) m = fmaxf(m, s_sum[w0 + k][lane].x);
+#pragma unroll
+  for (int k = 0; k < Split; ++k) {
+    const float2 x = s_sum[w0 + k][lane];
+    f[k] = x.x == -INFINITY ? 1.f : ex2_approx(x.x - m);
+    l = fmaf(x.y, f[k], l);
+  }
+  if (!on) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;       // nothing seen: zeros
+  __align__(16) T out[Dims];
+#pragma unroll
+  for (int d = 0; d < Dims; ++d) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < Split; ++k) x = fmaf(s_acc[w0 + k][split * Dims + d][lane], f[k], x);
+    out[d] = (T)(x * inv);
+  }
+  const int row = s_out[lane];
+  T* to = static_cast<T*>(a.o) + (size_t)row * kPG_D + d0 + split * Dims;
+#pragma unroll
+  for (int d = 0; d < Dims; d += 2) *reinterpret_cast<uint32_t*>(to + d) = *reinterpret_cast<const uint32_t*>(out + d);
+  if (a.lse && d0 == 0 && split == 0) {
+    const int h = row % a.H, bt = row / a.H, b = bt / a.t;
+    a.lse[((size_t)b * a.H + h) * a.t + bt - b * a.t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  }
 }
 
 template <typename T>
@@ -827,7 +885,13 @@ static int launch_shared(const SharedArgs& a, int ctas, cudaStream_t stream) {
   const unsigned per_head = (unsigned)(rows / a.p.heads);
   if ((rc = launch_early(paged_queries_kernel<T>, dim3((per_head + 7) / 8, a.p.heads), 256, 0, stream, a))) return rc;
   if ((rc = launch_early(paged_shared_kernel<T>, dim3(ctas), kSH_Threads, SharedSmem<T>::Bytes, stream, kmap, vmap, qmap, a))) return rc;
-  return launch_early(paged_merge_kernel<T>, dim3((per_head + 31) / 32, 2, a.p.heads), 256, 0, stream, a);
+  // a row's pieces are dealt to so many warps that there are about 3072 of them
+  const unsigned blocks = (per_head + 31) / 32, warps = blocks * a.p.heads * (kPG_D / kSH_MergeDims);
+  auto merge = [&](auto kernel, int split) { return launch_early(kernel, dim3(blocks, kPG_D / kSH_MergeDims * split / 8, a.p.heads), 256, 0, stream, a); };
+  if (warps >= 2304) return merge(paged_merge_kernel<T, 1>, 1);
+  if (warps >= 1152) return merge(paged_merge_kernel<T, 2>, 2);
+  if (warps >= 576) return merge(paged_merge_kernel<T, 4>, 4);
+  return merge(paged_merge_kernel<T, 8>, 8);
 }
 
 // the workspace: its bytes, and the arrays in it
@@ -840,7 +904,7 @@ static size_t shared_layout(SharedArgs& a, int n, int t, int H, int parts, uint8
   };
   const size_t heads_rows = (size_t)n * t * H, rows = (size_t)kSH_MaxCtas * kSH_M + (kPS_Depth + 1) * heads_rows;
   a.head = reinterpret_cast<int4*>(take(sizeof(int4)));
-  a.at = reinterpret_cast<int2*>(take((size_t)2 * n * sizeof(int2)));
+  a.at = reinterpret_cast<SharedRecord*>(take((size_t)2 * n * sizeof(SharedRecord)));
   a.qs = reinterpret_cast<float*>(take(heads_rows * 4));
   a.qp = take(heads_rows * parts * kPG_D);
   a.ml = reinterpret_cast<float2*>(take(rows * sizeof(float2)));
