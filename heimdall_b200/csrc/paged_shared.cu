@@ -179,6 +179,45 @@ __global__ void __launch_bounds__(256) paged_queries_kernel(SharedArgs a) {
   if (lane == 0) a.qs[at] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
 }
 
+// Barriers and the abort word by their addresses in shared memory: through pointers every one of the many uses makes its address anew, in a kernel whose
+// warps wait for their instructions as it is (87 -> XX us for 16 x 131072 shared tokens).
+struct Bar {
+  uint32_t at;
+  __device__ __forceinline__ Bar operator+(int i) const { return Bar{at + 8u * i}; }
+  __device__ __forceinline__ void init(uint32_t count) const { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(at), "r"(count) : "memory"); }
+  __device__ __forceinline__ void arrive() const { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(at) : "memory"); }
+  __device__ __forceinline__ void expect(uint32_t bytes) const {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(at), "r"(bytes) : "memory");
+  }
+  __device__ __forceinline__ void commit() const {      // arrive once this thread's products so far are done
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(at) : "memory");
+  }
+};
+struct Waits {
+  uint32_t abort;          // the address of the CTA's abort word
+  __device__ __forceinline__ int aborted() const {
+    int x;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(x) : "r"(abort) : "memory");
+    return x;
+  }
+  // as mbar_wait_warp_small
+  __device__ __forceinline__ bool operator()(Bar bar, uint32_t parity, int site) const {
+    bool ok = mbar_try_wait(bar.at, parity);
+    if (!ok) {
+      const long long t0 = clock64();
+#pragma unroll 1
+      while (!(ok = mbar_try_wait(bar.at, parity)) && !aborted()) {
+        if (clock64() - t0 > kWaitCycles) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort), "r"(site) : "memory");
+      }
+    }
+    return __all_sync(0xffffffffu, ok) != 0;
+  }
+};
+__device__ __forceinline__ void load_2d(uint32_t dst, const void* tmap, Bar bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar.at), "r"(c0), "r"(c1) : "memory");
+}
+
 // D[tmem] (+)= A[tmem] * B[smem desc], 8-bit operands: row m of A in lane m, four values to a 32-bit column, 8 columns to a step of K = 32
 __device__ __forceinline__ void umma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -208,11 +247,13 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));   // K's half tiles, then V's
   uint8_t* sQ = ring + (NK + NV) * kSH_Unit;           // [parts][2 atoms][128 rows][128]
   uint64_t* bars = reinterpret_cast<uint64_t*>(sQ + SharedSmem<T>::Q);
-  uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 12, *s_full = bars + 16, *p_full = bars + 18,
-           *p_free = bars + 20, *o_free = bars + 22, *o_full = bars + 24, *q_full = bars + 25, *q_free = bars + 26, *t_full = bars + 28,
-           *t_free = bars + 32;
+  const Bar k_full{smem_u32(bars)}, k_empty = k_full + 4, v_full = k_full + 8, v_empty = k_full + 12, s_full = k_full + 16, p_full = k_full + 18,
+            p_free = k_full + 20, o_free = k_full + 22, o_full = k_full + 24, q_full = k_full + 25, q_free = k_full + 26, t_full = k_full + 28,
+            t_free = k_full + 32;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 36);
   volatile int* abort = reinterpret_cast<volatile int*>(bars + 37);
+  const Waits wait{smem_u32(bars + 37)};
+  const uint32_t ring_at = smem_u32(ring), q_at = smem_u32(sQ);
   int* s_sum = reinterpret_cast<int*>(bars + 38);      // [20][2] per-warp totals
   int* s_start = reinterpret_cast<int*>(bars + 59);    // stretch, unit in it, rows before it
   SharedTile* s_tile = reinterpret_cast<SharedTile*>(bars + 64);  // [4]
@@ -220,22 +261,22 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < 4; ++i) {
-      mbar_init(k_full + i, 1);
-      mbar_init(k_empty + i, 1);
-      mbar_init(v_full + i, 1);
-      mbar_init(v_empty + i, 1);
-      mbar_init(t_full + i, 1);
-      mbar_init(t_free + i, 19);       // V, S, O, eight of softmax, eight accumulators
+      (k_full + i).init(1);
+      (k_empty + i).init(1);
+      (v_full + i).init(1);
+      (v_empty + i).init(1);
+      (t_full + i).init(1);
+      (t_free + i).init(19);       // V, S, O, eight of softmax, eight accumulators
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + i, 1);
-      mbar_init(p_full + i, 8);
-      mbar_init(p_free + i, 1);
-      mbar_init(o_free + i, 8);
+      (s_full + i).init(1);
+      (p_full + i).init(8);
+      (p_free + i).init(1);
+      (o_free + i).init(8);
     }
-    mbar_init(o_full, 1);
-    mbar_init(q_full, 1);
-    mbar_init(q_free, 1);
+    o_full.init(1);
+    q_full.init(1);
+    q_free.init(1);
     *abort = 0;
     fence_barrier_init();
   }
@@ -316,7 +357,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   bool ok = true;
   // every role: wait for tile j's entry (false: no more tiles, or a wait gave up)
   auto tile = [&](int j) {
-    ok = mbar_wait_warp_small(t_full + (j & 3), (j >> 2) & 1, abort, 0x90);
+    ok = wait(t_full + (j & 3), (j >> 2) & 1, 0x90);
     return ok && !s_tile[j & 3].stop;
   };
 
@@ -344,14 +385,14 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
             const int k1 = min(ntiles, k + u1 - unit);
             if (k >= k1) continue;
             unit += k1 - k;
-            if (items && !(ok = mbar_wait_warp_small(q_free, (items - 1) & 1, abort, 0x91))) break;
+            if (items && !(ok = wait(q_free, (items - 1) & 1, 0x91))) break;
             ++items;
             const int from = g * a.n * per_seq + x.first * per_seq + rb * kSH_M;
-            if (lane == 0) mbar_expect_tx(q_full, Parts * 2 * kSH_Unit);
+            if (lane == 0) q_full.expect(Parts * 2 * kSH_Unit);
             __syncwarp();
             if (elect_one()) {
 #pragma unroll
-              for (int p = 0; p < 2 * Parts; ++p) tma_load_2d(sQ + p * kSH_Unit, &qmap, q_full, p * 128, from);
+              for (int p = 0; p < 2 * Parts; ++p) load_2d(q_at + p * kSH_Unit, &qmap, q_full, p * 128, from);
             }
             __syncwarp();
             // lane i: page i of the tile, loaded a tile ahead
@@ -374,7 +415,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
                 ks = a.p.ks[(size_t)page * a.p.heads + g];
                 ex = max((int)(__float_as_uint(a.p.vs[(size_t)page * a.p.heads + g]) >> 23) - 127, -120);      // scales are powers of two
               }
-              if (j >= 4 && !(ok = mbar_wait_warp_small(t_free + (j & 3), ((j >> 2) - 1) & 1, abort, 0x92))) break;
+              if (j >= 4 && !(ok = wait(t_free + (j & 3), ((j >> 2) - 1) & 1, 0x92))) break;
               SharedTile* d = s_tile + (j & 3);
               if (lane < 8) {
                 d->ks[lane] = ks;
@@ -396,18 +437,18 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
                 d->stop = 0;
               }
               __syncwarp();
-              if (lane == 0) mbar_arrive(t_full + (j & 3));
+              if (lane == 0) (t_full + (j & 3)).arrive();
 #pragma unroll 1
               for (int half = 0; half < 2; ++half) {
-                if (used >= NK && !(ok = mbar_wait_warp_small(k_empty + u, uphase, abort, 0x93))) break;
+                if (used >= NK && !(ok = wait(k_empty + u, uphase, 0x93))) break;
                 if (lane == 0) {
-                  if (have) mbar_expect_tx(k_full + u, (uint32_t)__popc(have) * L * 128); else mbar_arrive(k_full + u);
+                  if (have) (k_full + u).expect((uint32_t)__popc(have) * L * 128); else (k_full + u).arrive();
                 }
                 __syncwarp();
 #pragma unroll 1
                 for (int i = 0; i < ppt; ++i) {
                   const int r = __shfl_sync(0xffffffffu, row, i);
-                  if (((have >> i) & 1u) && elect_one()) tma_load_2d(ring + u * kSH_Unit + i * L * 128, &kmap, k_full + u, 128 * half, r);
+                  if (((have >> i) & 1u) && elect_one()) load_2d(ring_at + u * kSH_Unit + i * L * 128, &kmap, k_full + u, 128 * half, r);
                   __syncwarp();
                 }
                 ++used;
@@ -425,30 +466,30 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         }
       }
       // the end of the line
-      if (ok && (j < 4 || (ok = mbar_wait_warp_small(t_free + (j & 3), ((j >> 2) - 1) & 1, abort, 0x92)))) {
+      if (ok && (j < 4 || (ok = wait(t_free + (j & 3), ((j >> 2) - 1) & 1, 0x92)))) {
         if (lane == 0) {
           s_tile[j & 3].stop = 1;
-          mbar_arrive(t_full + (j & 3));
+          (t_full + (j & 3)).arrive();
         }
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- S = sum_p Q_p K^T
       constexpr uint32_t id = idesc_e4m3(kSH_M, kSH_N);
-      const uint64_t dk0 = sdesc_sw128(smem_u32(ring)), dq0 = sdesc_sw128(smem_u32(sQ));
+      const uint64_t dk0 = sdesc_sw128(ring_at), dq0 = sdesc_sw128(q_at);
       int u = 0, uphase = 0, items = 0;
 #pragma unroll 1
       for (int j = 0; tile(j); ++j) {
         const int s = j & 1;
         const bool first = s_tile[j & 3].first, last = s_tile[j & 3].last;
         __syncwarp();
-        if (lane == 0) mbar_arrive(t_free + (j & 3));
-        if (first && !(ok = mbar_wait_warp_small(q_full, items & 1, abort, 0x94))) break;
+        if (lane == 0) (t_free + (j & 3)).arrive();
+        if (first && !(ok = wait(q_full, items & 1, 0x94))) break;
         items += first;
         // tile j - 2's weights, which lie over S, have been read
-        if (j >= 2 && !(ok = mbar_wait_warp_small(p_free + s, ((j >> 1) - 1) & 1, abort, 0x95))) break;
+        if (j >= 2 && !(ok = wait(p_free + s, ((j >> 1) - 1) & 1, 0x95))) break;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-          if (!(ok = mbar_wait_warp_small(k_full + u, uphase, abort, 0x97))) break;
+          if (!(ok = wait(k_full + u, uphase, 0x97))) break;
           tc_fence_after();
           if (elect_one()) {
             const uint64_t dk = dk0 + (uint32_t)(u * (kSH_Unit >> 4));
@@ -457,10 +498,10 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
 #pragma unroll
               for (int ks = 0; ks < 4; ++ks)
                 umma_f8_ss(tmem + s * kSH_N, dq0 + (uint32_t)((p * 2 + half) * (kSH_Unit >> 4) + ks * 2), dk + ks * 2, id, half > 0 || p > 0 || ks > 0);
-            umma_commit(k_empty + u);
+            (k_empty + u).commit();
             if (half) {
-              umma_commit(s_full + s);
-              if (last) umma_commit(q_free);
+              (s_full + s).commit();
+              if (last) q_free.commit();
             }
           }
           __syncwarp();
@@ -479,18 +520,18 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         const unsigned have = s_tile[j & 3].have;
         const int row = s_tile[j & 3].prow[lane & 7];
         __syncwarp();
-        if (lane == 0) mbar_arrive(t_free + (j & 3));
+        if (lane == 0) (t_free + (j & 3)).arrive();
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-          if (used >= NV && !(ok = mbar_wait_warp_small(v_empty + u, uphase, abort, 0x98))) break;
+          if (used >= NV && !(ok = wait(v_empty + u, uphase, 0x98))) break;
           if (lane == 0) {
-            if (have) mbar_expect_tx(v_full + u, (uint32_t)__popc(have) * L * 128); else mbar_arrive(v_full + u);
+            if (have) (v_full + u).expect((uint32_t)__popc(have) * L * 128); else (v_full + u).arrive();
           }
           __syncwarp();
 #pragma unroll 1
           for (int i = 0; i < ppt; ++i) {
             const int r = __shfl_sync(0xffffffffu, row, i);
-            if (((have >> i) & 1u) && elect_one()) tma_load_2d(ring + (NK + u) * kSH_Unit + i * L * 128, &vmap, v_full + u, 128 * half, r);
+            if (((have >> i) & 1u) && elect_one()) load_2d(ring_at + (NK + u) * kSH_Unit + i * L * 128, &vmap, v_full + u, 128 * half, r);
             __syncwarp();
           }
           ++used;
@@ -504,17 +545,18 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
     } else {
       // ---------------------------------------------------------------- O = sum_p P_p V
       constexpr uint32_t id = idesc_e4m3(kSH_M, 128) | kIdescBMn;
-      const uint64_t dv0 = sdesc_sw128_mn(smem_u32(ring + NK * kSH_Unit), 16384);
+      const uint64_t dv0 = sdesc_sw128_mn(ring_at + NK * kSH_Unit, 16384);
       int u = 0, uphase = 0;
 #pragma unroll 1
       for (int j = 0; tile(j); ++j) {
         const int s = j & 1;
-        if (lane == 0) mbar_arrive(t_free + (j & 3));
-        if (!(ok = mbar_wait_warp_small(p_full + s, (j >> 1) & 1, abort, 0x99))) break;
-        if (j >= 1 && !(ok = mbar_wait_warp_small(o_free + (s ^ 1), ((j - 1) >> 1) & 1, abort, 0x9a))) break;
+        __syncwarp();
+        if (lane == 0) (t_free + (j & 3)).arrive();
+        if (!(ok = wait(p_full + s, (j >> 1) & 1, 0x99))) break;
+        if (j >= 1 && !(ok = wait(o_free + (s ^ 1), ((j - 1) >> 1) & 1, 0x9a))) break;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-          if (!(ok = mbar_wait_warp_small(v_full + u, uphase, abort, 0x9b))) break;
+          if (!(ok = wait(v_full + u, uphase, 0x9b))) break;
           tc_fence_after();
           if (elect_one()) {
             const uint64_t dv = dv0 + (uint32_t)(u * (kSH_Unit >> 4));
@@ -523,10 +565,10 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
 #pragma unroll
               for (int ks = 0; ks < 4; ++ks)
                 umma_f8_ts(tmem + 256 + half * 128, tmem + s * kSH_N + 32 * ks + 8 * p, dv + ks * (4096 >> 4), id, p > 0 || ks > 0);
-            umma_commit(v_empty + u);
+            (v_empty + u).commit();
             if (half) {
-              umma_commit(p_free + s);
-              umma_commit(o_full);
+              (p_free + s).commit();
+              o_full.commit();
             }
           }
           __syncwarp();
@@ -571,7 +613,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         if (!whole) {
           // the values of tokens that are not there may be anything (a weight of 0 times NaN would be NaN): zeros
           const int n = 2 * j + hh, u = n % NV;
-          if (!(ok = mbar_wait_warp_small(v_full + u, (n / NV) & 1, abort, 0x9c))) break;
+          if (!(ok = wait(v_full + u, (n / NV) & 1, 0x9c))) break;
           if (r >= valid || !((have >> (r >> a.page_log)) & 1u)) {
             uint4* row = reinterpret_cast<uint4*>(ring + (NK + u) * kSH_Unit + r * 128);
 #pragma unroll
@@ -579,7 +621,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
           }
           fence_async_smem();
         }
-        if (!(ok = mbar_wait_warp_small(s_full + s, (j >> 1) & 1, abort, 0x9d))) break;
+        if (!(ok = wait(s_full + s, (j >> 1) & 1, 0x9d))) break;
         tc_fence_after();
         if (busy) {
           if (!all) {
@@ -674,8 +716,8 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(t_free + (j & 3));
-          mbar_arrive(p_full + s);
+          (t_free + (j & 3)).arrive();
+          (p_full + s).arrive();
         }
       }
     } else {
@@ -697,14 +739,14 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
 #pragma unroll
           for (int i = 0; i < 64; ++i) acc[i] = 0;
         }
-        if (!(ok = mbar_wait_warp_small(p_full + (j & 1), (j >> 1) & 1, abort, 0x9e))) break;      // the tile's maxima
+        if (!(ok = wait(p_full + (j & 1), (j >> 1) & 1, 0x9e))) break;      // the tile's maxima
         float2 t = make_float2(-INFINITY, 0.f);
         if (busy) {
           const float2 *ml = s_ml + (j & 3) * 2 * kSH_M + r, t0 = ml[0], t1 = ml[kSH_M];
           t = make_float2(fmaxf(t0.x, t1.x), t0.y + t1.y);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(t_free + (j & 3));      // the entry and the maxima may be written over
+        if (lane == 0) (t_free + (j & 3)).arrive();      // the entry and the maxima may be written over
         // the accumulators are relative to the first tile's maximum, until one is 2^40 times it: then to that
         if (t.x > m_ref + 40.f) {
           const float al = m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - t.x);
@@ -717,7 +759,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         const float ff = t.x == -INFINITY ? 1.f / 256.f : ex2_approx(t.x - m_ref) * (1.f / 256.f);
         l = fmaf(t.y, ff, l);
         const uint64_t f = pair2(ff, ff);
-        if (!(ok = mbar_wait_warp_small(o_full, j & 1, abort, 0x9f))) break;
+        if (!(ok = wait(o_full, j & 1, 0x9f))) break;
         tc_fence_after();
         if (busy) {
 #pragma unroll
@@ -732,7 +774,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(o_free + (j & 1));
+        if (lane == 0) (o_free + (j & 1)).arrive();
         if (end) {
           if (r < rows) {
             // a piece lies dim by dim, so that 32 rows are neighbours
