@@ -276,7 +276,7 @@ int bf_page_table_share(const bf_page_table* t, const int64_t* slots, int n, int
     r[2] = from;
     r[3] = end;
     r[4] = last[lead];
-    r[5] = 0;
+    r[5] = depth[lead];
     for (int i = first; i < first + many; ++i) {
       last[order[i]] = count;
       skip[order[i]] = end;

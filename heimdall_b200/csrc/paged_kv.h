@@ -18,7 +18,7 @@ struct PagePool {
 
 // A plan of shared pages (bf_page_table_share), int32: kPS_Head words (runs, sequences), then, n entries each, the sequences' slots, their order, their
 // places in it, each sequence's last run (-1: none) and the pages that its runs cover, then n runs of kPS_Run words: first place, sequences, first
-// page, page behind the last, the run before it on its sequences' way (-1: none), 0.
+// page, page behind the last, the run before it on its sequences' way (-1: none), the number of those.
 constexpr int kPS_Head = 4, kPS_Run = 6, kPS_Depth = 4;      // a sequence has at most kPS_Depth runs
 inline long long plan_words(long long n) { return kPS_Head + 5 * n + kPS_Run * n; }
 

@@ -37,6 +37,7 @@ constexpr int kSH_M = 128, kSH_N = 128;              // rows, tokens of a tile
 constexpr int kSH_Unit = 128 * 128;                  // bytes of half a K or V tile: 128 tokens, 128 dims
 constexpr int kSH_Threads = 640;
 constexpr int kSH_Start = 1;
+constexpr int kSH_Ways = kPS_Depth + 1;              // pieces of the line that a sequence can have
 // register split (setmaxnreg) of the 96 per thread at launch
 constexpr uint32_t kSH_RegsCtl = 48, kSH_RegsSoftmax = 64, kSH_RegsAcc = 152;
 static_assert(kSH_RegsCtl + 2 * kSH_RegsSoftmax + 2 * kSH_RegsAcc <= 5 * 96, "register split");
@@ -71,11 +72,11 @@ struct SharedSmem {
 };
 static_assert(SharedSmem<__half>::Bytes <= 232448 && SharedSmem<__nv_bfloat16>::Bytes <= 232448, "shared memory");
 
-struct SharedRecord {
+// where a run, or a tail, lies in the line, for the sequence at a place that has it
+struct SharedWay {
   int unit, before;     // its first unit, the rows before it
   int rows, tiles;      // its rows per KV head, its tiles (0: no pieces)
-  int first, next;      // its first place, the run before it on its sequences' way (-1: none)
-  int pad[2];
+  int first, pad[3];    // its first place
 };
 struct SharedArgs {
   PagePool p;
@@ -88,7 +89,7 @@ struct SharedArgs {
   uint8_t* qp;          // [KV heads][n t R rows, in the plan's order][parts][256]
   float* qs;            // [KV heads][n t R] the rows' scales
   int4* head;           // units per CTA, CTAs with one more, -, -
-  SharedRecord* at;     // [runs + n] where a run, or the tail of the sequence at a place, lies in the line
+  SharedWay* ways;      // [n places][kSH_Ways]: the tail, then the runs
   float* part;          // [CTAs * 128 + rows][256], a piece's rows x dims transposed
   float2* ml;           // [CTAs * 128 + rows] maximum, sum
   void* o;
@@ -330,10 +331,19 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
       if (e >= stretches) break;
       const Stretch x(a, pl, e);
       const int units = x.units(a.p.heads);
-      if (blockIdx.x == 0) {
-        SharedRecord* to = a.at + e;
-        *reinterpret_cast<int4*>(to) = make_int4(at.x, at.y, x.rows, x.tiles());
-        *reinterpret_cast<int2*>(&to->first) = make_int2(x.first, e < pl.n_runs ? pl.runs[(size_t)e * kPS_Run + 4] : pl.last[pl.order[x.first]]);
+      if (e % (int)gridDim.x == (int)blockIdx.x) {      // for paged_merge_kernel: every CTA writes some stretches' part
+        const bool run = e < pl.n_runs;
+        const int32_t* r = pl.runs + (size_t)e * kPS_Run;
+        const int k = run ? 1 + r[5] : 0, many = run ? r[1] : 1, tiles = x.tiles();
+        for (int i = 0; i < many; ++i) {
+          int4* to = reinterpret_cast<int4*>(a.ways + (size_t)(x.first + i) * kSH_Ways + k);
+          to[0] = make_int4(at.x, at.y, x.rows, tiles);
+          to[1] = make_int4(x.first, 0, 0, 0);
+        }
+        if (!run) {                                     // and that there are no more than its sequence's runs
+          const int last = pl.last[pl.order[x.first]];
+          for (int i = last >= 0 ? 2 + pl.runs[(size_t)last * kPS_Run + 5] : 1; i < kSH_Ways; ++i) a.ways[(size_t)x.first * kSH_Ways + i].tiles = 0;
+        }
       }
       if (u0 < u1 && at.x <= u0 && u0 < at.x + units) {
         s_start[0] = e;
@@ -803,13 +813,12 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
 }
 
 // Output rows: a block has 32 neighbouring rows of one KV head, in the plan's order (they are neighbours in every piece too), and 16 dims for each of its
-// 8 / Split groups of warps; a lane has a row, and the row's pieces (tail, then its runs from the last one up, CTA by CTA) are dealt to a group's
-// Split warps, whose sums are added in order.  The first warp finds where the rows' pieces lie.  (With one warp for all pieces of its rows, the 37 of a long
-// document took 40 us one after the other; split over eight, the 13 of 64 sequences took longer than over four.)
+// 8 / Split groups of warps; a lane has a row, and the row's pieces (tail, then its runs, CTA by CTA) are dealt to a group's
+// Split warps, whose sums are added in order.  The first warp finds where the rows' pieces lie.
 constexpr int kSH_MergeDims = 16;
 template <typename T, int Split>
 __global__ void __launch_bounds__(256) paged_merge_kernel(SharedArgs a) {
-  constexpr int Groups = 8 / Split, Ways = kPS_Depth + 1;
+  constexpr int Groups = 8 / Split, Ways = kSH_Ways;
   __shared__ float s_acc[8][kSH_MergeDims][32];
   __shared__ float2 s_sum[8][32];
   __shared__ int4 s_way[Ways][32];       // first CTA, pieces, rows of a piece, row of it
@@ -827,21 +836,17 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(SharedArgs a) {
     const int4 head = *a.head;
     const int each = head.x, more = head.y, longer = more * (each + 1);
     auto cta_of = [&](int u) { return u < longer ? u / (each + 1) : more + (u - longer) / each; };
-    int e = on ? pl.n_runs + place : -1;
 #pragma unroll
     for (int k = 0; k < Ways; ++k) {
+      const int4* p = reinterpret_cast<const int4*>(a.ways + (size_t)place * Ways + k);
+      const int4 x = p[0], y = p[1];
       int4 way = make_int4(0, 0, 1, 0);
       int base = 0;
-      if (e >= 0 && e < pl.n_runs + a.n) {
-        const int4 x = *reinterpret_cast<const int4*>(a.at + e);
-        const int2 y = *reinterpret_cast<const int2*>(&a.at[e].first);
-        if (x.w > 0) {
-          const int blocks = (x.z + kSH_M - 1) / kSH_M, idx = (place - y.x) * per_seq + rem, rb = idx / kSH_M;
-          const int u = x.x + (g * blocks + rb) * (x.w + kSH_Start) + kSH_Start, c0 = cta_of(u);
-          way = make_int4(c0, cta_of(u + x.w - 1) - c0 + 1, min(kSH_M, x.z - rb * kSH_M), idx - rb * kSH_M);
-          base = x.y + g * x.z + rb * kSH_M;
-        }
-        e = y.y < pl.n_runs ? y.y : -1;
+      if (on && x.w > 0) {
+        const int blocks = (x.z + kSH_M - 1) / kSH_M, idx = (place - y.x) * per_seq + rem, rb = idx / kSH_M;
+        const int u = x.x + (g * blocks + rb) * (x.w + kSH_Start) + kSH_Start, c0 = cta_of(u);
+        way = make_int4(c0, cta_of(u + x.w - 1) - c0 + 1, min(kSH_M, x.z - rb * kSH_M), idx - rb * kSH_M);
+        base = x.y + g * x.z + rb * kSH_M;
       }
       s_way[k][lane] = way;
       s_base[k][lane] = base;
@@ -852,27 +857,36 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(SharedArgs a) {
   float m = -INFINITY, sum = 0.f, acc[kSH_MergeDims];
 #pragma unroll
   for (int k = 0; k < kSH_MergeDims; ++k) acc[k] = 0.f;
-  int mine = split;                        // pieces until this warp's next one
+  int seen = 0;                            // pieces of the ways before
   for (int k = 0; k < Ways; ++k) {
     const int4 way = s_way[k][lane];
     const int base = s_base[k][lane];
-#pragma unroll 2
-    for (; mine < way.y; mine += Split) {
-      const size_t row0 = (size_t)(way.x + mine) * kSH_M + base;
-      const float2 ml = a.ml[row0 + way.w];
-      const float* p = a.part + row0 * kPG_D + (size_t)d0 * way.z + way.w;
-      float v[kSH_MergeDims];
+    // a few pieces at a time, the loads of all of them before the first sum
+    constexpr int Batch = 3;
+    for (int mine = (split - seen) & (Split - 1); mine < way.y; mine += Batch * Split) {
+      float v[Batch][kSH_MergeDims];
+      float2 ml[Batch];
 #pragma unroll
-      for (int q = 0; q < kSH_MergeDims; ++q) v[q] = p[(size_t)q * way.z];
-      // a partial without a maximum holds zeros, or NaN to be passed on
-      const float mn = fmaxf(m, ml.x);
-      const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - mn);
+      for (int x = 0; x < Batch; ++x) {
+        const size_t row0 = (size_t)(way.x + min(mine + x * Split, way.y - 1)) * kSH_M + base;
+        ml[x] = a.ml[row0 + way.w];
+        const float* p = a.part + row0 * kPG_D + (size_t)d0 * way.z + way.w;
 #pragma unroll
-      for (int q = 0; q < kSH_MergeDims; ++q) acc[q] = acc[q] * al + v[q] * f;
-      sum = sum * al + ml.y * f;
-      m = mn;
+        for (int q = 0; q < kSH_MergeDims; ++q) v[x][q] = p[(size_t)q * way.z];
+      }
+#pragma unroll
+      for (int x = 0; x < Batch; ++x) {
+        if (mine + x * Split >= way.y) break;
+        // a partial without a maximum holds zeros, or NaN to be passed on
+        const float mn = fmaxf(m, ml[x].x);
+        const float al = m == -INFINITY ? 1.f : ex2_approx(m - mn), f = ml[x].x == -INFINITY ? 1.f : ex2_approx(ml[x].x - mn);
+#pragma unroll
+        for (int q = 0; q < kSH_MergeDims; ++q) acc[q] = acc[q] * al + v[x][q] * f;
+        sum = sum * al + ml[x].y * f;
+        m = mn;
+      }
     }
-    mine -= way.y;
+    seen += way.y;
   }
 #pragma unroll
   for (int k = 0; k < kSH_MergeDims; ++k) s_acc[warp][k][lane] = acc[k];
@@ -927,12 +941,13 @@ static int launch_shared(const SharedArgs& a, int ctas, cudaStream_t stream) {
   const unsigned per_head = (unsigned)(rows / a.p.heads);
   if ((rc = launch_early(paged_queries_kernel<T>, dim3((per_head + 7) / 8, a.p.heads), 256, 0, stream, a))) return rc;
   if ((rc = launch_early(paged_shared_kernel<T>, dim3(ctas), kSH_Threads, SharedSmem<T>::Bytes, stream, kmap, vmap, qmap, a))) return rc;
-  // a row's pieces are dealt to so many warps that there are about 3072 of them
+  // a row's pieces are dealt to so many warps that there are 600 to 1200 of them: with few rows the pieces' way is what takes time (whole call, 16 x 24 rows of
+  // 37 pieces each: 100, 90, 85 and 86 us over 1, 2, 4 and 8), with many the blocks (64 x 24 rows of 13: 48, 52, 53 and 62)
   const unsigned blocks = (per_head + 31) / 32, warps = blocks * a.p.heads * (kPG_D / kSH_MergeDims);
   auto merge = [&](auto kernel, int split) { return launch_early(kernel, dim3(blocks, kPG_D / kSH_MergeDims * split / 8, a.p.heads), 256, 0, stream, a); };
-  if (warps >= 2304) return merge(paged_merge_kernel<T, 1>, 1);
-  if (warps >= 1152) return merge(paged_merge_kernel<T, 2>, 2);
-  if (warps >= 576) return merge(paged_merge_kernel<T, 4>, 4);
+  if (warps >= 576) return merge(paged_merge_kernel<T, 1>, 1);
+  if (warps >= 288) return merge(paged_merge_kernel<T, 2>, 2);
+  if (warps >= 144) return merge(paged_merge_kernel<T, 4>, 4);
   return merge(paged_merge_kernel<T, 8>, 8);
 }
 
@@ -946,7 +961,7 @@ static size_t shared_layout(SharedArgs& a, int n, int t, int H, int parts, uint8
   };
   const size_t heads_rows = (size_t)n * t * H, rows = (size_t)kSH_MaxCtas * kSH_M + (kPS_Depth + 1) * heads_rows;
   a.head = reinterpret_cast<int4*>(take(sizeof(int4)));
-  a.at = reinterpret_cast<SharedRecord*>(take((size_t)2 * n * sizeof(SharedRecord)));
+  a.ways = reinterpret_cast<SharedWay*>(take((size_t)n * kSH_Ways * sizeof(SharedWay)));
   a.qs = reinterpret_cast<float*>(take(heads_rows * 4));
   a.qp = take(heads_rows * parts * kPG_D);
   a.ml = reinterpret_cast<float2*>(take(rows * sizeof(float2)));
