@@ -556,8 +556,8 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
 // out of a group of 128 tokens: CTA = (group, `units` tiles of 128 columns).  h's two parts are made once in shared memory (A operand, K-major); the tiles'
 // rows of B (N operand) come through a ring of three, D alternates between two halves of 256 TMEM columns, and the next tile's y is in
 // registers while this one's sums leave TMEM.  TMEM is read 16 lanes by 64 columns at a time, where a thread has two columns of every eight: the
-// rows of B are dealt so that column n = 8 k + 2 c + e of such a block is column 16 c + 2 k + e of y, and a thread ends with 16 consecutive
-// columns of a row, four threads with 128 bytes.
+// rows of B are dealt so that column n = 8 k + 2 c + e of 32 is column 8 c + 2 k + e of y, and a thread ends with 8 consecutive columns of a
+// row, four threads with 64 bytes, whole sectors (16 columns to a thread and 128 bytes to four put half a sector into each access: 99 against XX us).
 constexpr int kAD_Tile = 128;
 template <typename T, int RM>
 struct ExpandCfg {
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
   using C = ExpandCfg<T, RM>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* s_h = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int s_tok[kAD_Group];
+  __shared__ longlong2 s_row[kAD_Group];       // where the tokens' rows of y and out begin, in elements
   __shared__ float s_scale[kAD_Group];
   __shared__ uint64_t s_bar[2];
   __shared__ uint32_t s_tmem;
@@ -584,7 +584,10 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
   const int4 grp = a.groups[blockIdx.x];
   const int id = grp.x, m = grp.z;
   if (id == a.n && a.out == a.y) return;
-  if (tid < m) s_tok[tid] = a.perm[grp.y + tid];
+  if (tid < m) {
+    const long long t = a.perm[grp.y + tid];
+    s_row[tid] = make_longlong2(t * a.y_st, t * a.o_st);
+  }
   if (tid == 0) {
     mbar_init(s_bar, 1);
     mbar_init(s_bar + 1, 1);
@@ -596,9 +599,9 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
   const int col0 = blockIdx.y * a.units * kAD_Tile, tiles = min(a.units, (a.d_out - col0 + kAD_Tile - 1) / kAD_Tile);
   const T* w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
   const uint32_t hs = smem_u32(s_h), bs = hs + C::HBytes;
-  // B's rows of a tile: row n of the operand is column 64 (n / 64) + 16 c + 2 k + e of the tile, n % 64 = 8 k + 2 c + e
+  // B's rows of a tile: row n of the operand is column 32 (n / 32) + 8 c + 2 k + e of the tile, n % 32 = 8 k + 2 c + e
   const int pieces = rank / 8;             // of 16 bytes in a row: two threads to a row, each every second piece
-  const int brow = tid >> 1, bcol = (brow & 64) + 16 * ((brow >> 1) & 3) + 2 * ((brow >> 3) & 7) + (brow & 1);
+  const int brow = tid >> 1, bcol = (brow & 96) + 8 * ((brow >> 1) & 3) + 2 * ((brow >> 3) & 3) + (brow & 1);
   auto fetch = [&](int j) {
     if (j < tiles) {
       const int col = col0 + j * kAD_Tile + bcol;
@@ -609,8 +612,8 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // a thread's part of y: rows 32 (warp % 4) + 16 i + 8 e + g, columns 64 (warp / 4) + 16 c .. + 15
-  const int wr = 32 * (warp & 3), wc = 64 * (warp >> 2) + 16 * c;
+  // a thread's part of y: rows 32 (warp % 4) + 16 i + 8 e + g, columns 64 (warp / 4) + 32 q + 8 c .. + 7
+  const int wr = 32 * (warp & 3), wc = 64 * (warp >> 2) + 8 * c;
   uint4 yv[2][2][2], y_next[2][2][2];
   auto load_y = [&](int j) {
     const int col = col0 + j * kAD_Tile + wc;
@@ -620,9 +623,9 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
       for (int e = 0; e < 2; ++e) {
         const int r = wr + 16 * i + 8 * e + g;
         if (j < tiles && r < m) {
-          const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + (long long)s_tok[r] * a.y_st + col);
+          const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + s_row[r].x + col);
           if (col < a.d_out) y_next[i][e][0] = ldg_stream(p);
-          if (col + 8 < a.d_out) y_next[i][e][1] = ldg_stream(p + 1);
+          if (col + 32 < a.d_out) y_next[i][e][1] = ldg_stream(p + 4);
         }
       }
   };
@@ -710,9 +713,9 @@ __global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(A
 #pragma unroll
             for (int q = 0; q < 2; ++q) v[2 * k + q] = (T)fmaf(__uint_as_float(d[4 * k + 2 * e + q]), sc, (float)v[2 * k + q]);
         }
-        uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (long long)s_tok[r] * a.o_st + col);
+        uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + s_row[r].y + col);
         if (col < a.d_out) to[0] = yv[i][e][0];
-        if (col + 8 < a.d_out) to[1] = yv[i][e][1];
+        if (col + 32 < a.d_out) to[4] = yv[i][e][1];
       }
     }
   }
