@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     a.groups[k] = make_int4(b, first, min(kAD_Group, s_at[b + 1] - first), 0);
     a.arrived[k] = 0;
   }
-  if (tid == 0) *a.n_groups = total;
+  if (tid == 0) *a.n_groups = a.out == a.y ? s_grp[a.n] : total;      // tokens without an adapter come last: in place they are done
   __syncthreads();
   for (int t0 = 0; t0 < a.T; t0 += 1024 * per) {
     if (a.T > 1024 * per) load(t0);
@@ -553,179 +553,241 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
     for (int t = 0; t < m; t += 4) expand_few<T, 4>(a, w, rank, min(4, m - t), s_tok + t, s_h + t * kAD_MaxRank, scale, col0, a.units);
 }
 
-// out of a group of 128 tokens: CTA = (group, `units` tiles of 128 columns).  h's two parts are made once in shared memory (A operand, K-major); the tiles'
-// rows of B (N operand) come through a ring of three, D alternates between two halves of 256 TMEM columns, and the next tile's y is in
-// registers while this one's sums leave TMEM.  TMEM is read 16 lanes by 64 columns at a time, where a thread has two columns of every eight: the
-// rows of B are dealt so that column n = 8 k + 2 c + e of 32 is column 8 c + 2 k + e of y, and a thread ends with 8 consecutive columns of a
-// row, four threads with 64 bytes, whole sectors (16 columns to a thread and 128 bytes to four put half a sector into each access: 99 against XX us).
-constexpr int kAD_Tile = 128;
+// out of many tokens: tiles of a group (128 tokens) and 128 columns, group by group, an equal run of them to each SM's one CTA.  Four warps bring y's rows into
+// a ring of shared memory (256 bytes a copy), two bring B's rows (N operand, K-major) and, when the group changes, h's two parts (M operand), a thread issues
+// the products, and eight warps add D (TMEM, two of them) to y where it lies and send the rows out; a thread has half a row.
+// HBM under reads and writes at once wants about 130 KB of reads in flight per SM, whatever the products do (a bare copy of 8192 x 12288 by
+// such tiles: 72 us with four tiles of y on their way, 106 to 112 with two or three).  So y goes through shared memory: 85 us for those sizes and ranks up to 64,
+// against 106 with y in registers, two or three CTAs to an SM.  A warp issues a copy of its own bytes about every 70 cycles: one warp for all rows
+// took 198 us, and rows going out by such copies too 206.
+constexpr int kAD_Tile = 128, kAD_Pitch = 272;      // bytes from row to row of y in shared memory: no two of eight neighbouring rows in the same banks
 template <typename T, int RM>
 struct ExpandCfg {
-  static constexpr int Atoms = RM <= 64 ? 1 : 2;                  // of 64 ranks
-  static constexpr int HBytes = 2 * Atoms * kAD_Group * 128, BBytes = Atoms * kAD_Tile * 128, Ring = 3;
-  static constexpr int Smem = HBytes + Ring * BBytes + 1024;
+  static constexpr int Atoms = RM <= 64 ? 1 : 2, Ring = RM <= 64 ? 4 : 2;       // of 64 ranks; tiles of y
+  static constexpr int HBytes = 2 * Atoms * kAD_Group * 128, BBytes = Atoms * kAD_Tile * 128, YBytes = kAD_Group * kAD_Pitch;
+  static constexpr int Smem = HBytes + 2 * BBytes + Ring * YBytes + 1024;
 };
 
 template <typename T, int RM>
-__global__ void __launch_bounds__(256, RM <= 64 ? 2 : 1) adapter_expand_kernel(AdapterArgs a) {
+__global__ void __launch_bounds__(480, 1) adapter_expand_kernel(AdapterArgs a) {
   using C = ExpandCfg<T, RM>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* s_h = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ longlong2 s_row[kAD_Group];       // where the tokens' rows of y and out begin, in elements
-  __shared__ float s_scale[kAD_Group];
-  __shared__ uint64_t s_bar[2];
+  uint8_t* s_y = s_h + C::HBytes + 2 * C::BBytes;
+  const uint32_t hs = smem_u32(s_h), bs = hs + C::HBytes;
+  // full: bytes of y; 64 threads' copies of B (and h); the products.  free: eight warps' stores; the products; eight warps' reads of D
+  __shared__ uint64_t y_full[C::Ring], y_free[C::Ring], b_full[2], b_free[2], d_full[2], d_free[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   volatile int* abort = &s_abort;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   let_next_start();
-  // the groups are older than the kernel before this one, which began by waiting for what was before it
-  if ((int)blockIdx.x >= *a.n_groups) return;
-  const int4 grp = a.groups[blockIdx.x];
-  const int id = grp.x, m = grp.z;
-  if (id == a.n && a.out == a.y) return;
-  if (tid < m) {
-    const long long t = a.perm[grp.y + tid];
-    s_row[tid] = make_longlong2(t * a.y_st, t * a.o_st);
-  }
   if (tid == 0) {
-    mbar_init(s_bar, 1);
-    mbar_init(s_bar + 1, 1);
+    for (int i = 0; i < C::Ring; ++i) {
+      mbar_init(y_full + i, 4);
+      mbar_init(y_free + i, 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(b_full + i, 64);
+      mbar_init(b_free + i, 1);
+      mbar_init(d_full + i, 1);
+      mbar_init(d_free + i, 8);
+    }
     s_abort = 0;
     fence_barrier_init();
   }
   __syncthreads();
-  const int r0 = id < a.n ? a.row[id] : 0, rank = id < a.n ? a.row[id + 1] - r0 : 0, steps = rank / 16;
-  const int col0 = blockIdx.y * a.units * kAD_Tile, tiles = min(a.units, (a.d_out - col0 + kAD_Tile - 1) / kAD_Tile);
-  const T* w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
-  const uint32_t hs = smem_u32(s_h), bs = hs + C::HBytes;
-  // B's rows of a tile: row n of the operand is column 32 (n / 32) + 8 c + 2 k + e of the tile, n % 32 = 8 k + 2 c + e
-  const int pieces = rank / 8;             // of 16 bytes in a row: two threads to a row, each every second piece
-  const int brow = tid >> 1, bcol = (brow & 96) + 8 * ((brow >> 1) & 3) + 2 * ((brow >> 3) & 3) + (brow & 1);
-  auto fetch = [&](int j) {
-    if (j < tiles) {
-      const int col = col0 + j * kAD_Tile + bcol;
-      const bool in = col < a.d_out;
-      const T* src = w + (long long)(in ? col : 0) * rank;
-      const uint32_t dst = bs + (j % C::Ring) * C::BBytes + brow * 128;
-      for (int p = tid & 1; p < pieces; p += 2) copy16(dst + (p >> 3) * (kAD_Tile * 128) + (((p & 7) ^ (brow & 7)) << 4), src + 8 * p, in);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  // a thread's part of y: rows 32 (warp % 4) + 16 i + 8 e + g, columns 64 (warp / 4) + 32 q + 8 c .. + 7
-  const int wr = 32 * (warp & 3), wc = 64 * (warp >> 2) + 8 * c;
-  uint4 yv[2][2][2], y_next[2][2][2];
-  auto load_y = [&](int j) {
-    const int col = col0 + j * kAD_Tile + wc;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = wr + 16 * i + 8 * e + g;
-        if (j < tiles && r < m) {
-          const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + s_row[r].x + col);
-          if (col < a.d_out) y_next[i][e][0] = ldg_stream(p);
-          if (col + 32 < a.d_out) y_next[i][e][1] = ldg_stream(p + 4);
-        }
-      }
-  };
-  fetch(0);
-  fetch(1);
-  load_y(0);
-  wait_for_stream();
-  if (warp == 0 && rank) {
-    tmem_alloc(&s_tmem, 256);
-    tmem_relinquish();
-  }
-  if (rank) {
-    // two threads to a row; rows that are not there repeat the last one, nobody reads their sums
-    const T* src = static_cast<const T*>(a.parts) + (size_t)(grp.y + min(brow, m - 1)) * 2 * a.rmax;
-    const uint32_t dst = hs + brow * 128;
-    for (int p = tid & 1; p < pieces; p += 2)
-#pragma unroll
-      for (int part = 0; part < 2; ++part)
-        copy16(dst + part * (C::HBytes / 2) + (p >> 3) * (kAD_Group * 128) + (((p & 7) ^ (brow & 7)) << 4), src + part * a.rmax + 8 * p, true);
-    if (tid < m) s_scale[tid] = a.back[grp.y + tid];
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  const uint32_t idesc = idesc_f16(128, kAD_Tile, kIsBf16<T>);
-  uint32_t tmem = 0;
-  auto products = [&](int j) {             // by one thread
-    tc_fence_after();
-    const uint32_t b = bs + (j % C::Ring) * C::BBytes;
-#pragma unroll 1
-    for (int part = 0; part < 2; ++part)
-#pragma unroll 1
-      for (int ks = 0; ks < steps; ++ks) {
-        const uint32_t k = (ks >> 2) * (128 * 128) + (ks & 3) * 32;      // both operands have 128 rows
-        umma_f16_ss(tmem + (j & 1) * kAD_Tile, sdesc_sw128(hs + part * (C::HBytes / 2) + k), sdesc_sw128(b + k), idesc, part > 0 || ks > 0);
-      }
-    umma_commit(s_bar + (j & 1));
-  };
+  // y and the groups are older than the kernel before this one, which began by waiting for what was before it
+  const int tpg = (a.d_out + kAD_Tile - 1) / kAD_Tile;
+  const long long total = (long long)*a.n_groups * tpg;
+  const long long first = total * blockIdx.x / gridDim.x;
+  const int n = (int)(total * (blockIdx.x + 1) / gridDim.x - first), g0 = (int)(first / tpg), c0 = (int)(first - (long long)g0 * tpg);
   bool ok = true;
+  if (warp < 4) {
+    const int r = tid;
+    const T* src = nullptr;
+    int m = 0;
 #pragma unroll 1
-  for (int j = -1; j < tiles && ok; ++j) {
-    // tile j + 1's rows of B have landed, everybody is done with tile j - 1
-    if (j < 0) asm volatile("cp.async.wait_group 0;" ::: "memory"); else asm volatile("cp.async.wait_group 1;" ::: "memory");
-    fence_async_smem();
-    tc_fence_before();
-    __syncthreads();
-    if (j < 0 && rank) {
-      tc_fence_after();
-      tmem = s_tmem;
-    }
-    if (tid == 0 && rank && j + 1 < tiles) products(j + 1);
-    if (j < 0) {
-      fetch(2);
-      continue;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) yv[i][e][q] = y_next[i][e][q];
-    load_y(j + 1);
-    if (rank) {
-      ok = mbar_wait_warp_small(s_bar + (j & 1), (j >> 1) & 1, abort, 0x82);
-      if (!ok) break;
-      tc_fence_after();
-    }
-    fetch(j + 3);          // in the place of tile j, whose products are done
-    const int col = col0 + j * kAD_Tile + wc;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (wr + 16 * i >= m) break;
-      uint32_t d[32];
-      if (rank) {
-        tmem_ld_16x256b_x8(tmem + (j & 1) * kAD_Tile + 64 * (warp >> 2) + ((uint32_t)(wr + 16 * i) << 16), d);
-        tmem_wait_ld();
+    for (int j = 0, g = g0, c = c0; j < n; ++j) {
+      if (j == 0 || c == 0) {
+        const int4 grp = a.groups[g];
+        m = grp.z;
+        if (r < m) src = static_cast<const T*>(a.y) + (long long)a.perm[grp.y + r] * a.y_st;
       }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = wr + 16 * i + 8 * e + g;
-        if (r >= m) continue;
-        if (rank) {
-          const float sc = s_scale[r];
-          T* v = reinterpret_cast<T*>(yv[i][e]);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-#pragma unroll
-            for (int q = 0; q < 2; ++q) v[2 * k + q] = (T)fmaf(__uint_as_float(d[4 * k + 2 * e + q]), sc, (float)v[2 * k + q]);
+      const int s = j % C::Ring, bytes = 2 * min(kAD_Tile, a.d_out - c * kAD_Tile);
+      if (!mbar_wait_warp_small(y_free + s, (j / C::Ring & 1) ^ 1, abort, 0x82)) break;
+      if (lane == 0) mbar_expect_tx(y_full + s, min(max(m - r, 0), 32) * bytes);
+      __syncwarp();
+      if (r < m) bulk_load_1d(s_y + s * C::YBytes + r * kAD_Pitch, src + c * kAD_Tile, bytes, y_full + s);
+      if (++c == tpg) {
+        c = 0;
+        ++g;
+      }
+    }
+  } else if (warp < 6) {
+    wait_for_stream();
+    const int t = tid - 128, half = t & 1, row0 = t >> 1;      // two threads to a row, each every second piece of 16 bytes
+    const T* w = nullptr;
+    int rank = 0;
+#pragma unroll 1
+    for (int j = 0, g = g0, c = c0; j < n; ++j) {
+      bool sent = j == 0;          // tile j - 1 has been handed on
+      auto send = [&]() {
+        fence_async_smem();
+        mbar_arrive(b_full + ((j - 1) & 1));
+        sent = true;
+      };
+      if (j == 0 || c == 0) {
+        const int4 grp = a.groups[g];
+        const int r0 = grp.x < a.n ? a.row[grp.x] : 0;
+        rank = grp.x < a.n ? a.row[grp.x + 1] - r0 : 0;
+        w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
+        if (!sent) {               // h is in use until the products of tile j - 1 are done
+          asm volatile("cp.async.wait_group 0;" ::: "memory");
+          send();
+          if (!(ok = mbar_wait_small(b_free + ((j - 1) & 1), (j - 1) >> 1 & 1, abort, 0x83))) break;
         }
-        uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + s_row[r].y + col);
-        if (col < a.d_out) to[0] = yv[i][e][0];
-        if (col + 32 < a.d_out) to[4] = yv[i][e][1];
+        for (int r = row0; r < kAD_Group; r += 32) {
+          // rows that are not there repeat the last one, nobody reads their sums
+          const T* src = static_cast<const T*>(a.parts) + (size_t)(grp.y + min(r, grp.z - 1)) * 2 * a.rmax;
+          for (int p = half; p < rank / 8; p += 2)
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+              copy16(hs + r * 128 + part * (C::HBytes / 2) + (p >> 3) * (kAD_Group * 128) + (((p & 7) ^ (r & 7)) << 4), src + part * a.rmax + 8 * p, true);
+        }
+      }
+      if (!(ok = mbar_wait_small(b_free + (j & 1), (j >> 1 & 1) ^ 1, abort, 0x84))) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = row0 + 32 * i, col = c * kAD_Tile + r;
+        const bool in = col < a.d_out;
+        const T* src = w + (long long)(in ? col : 0) * rank;
+        const uint32_t dst = bs + (j & 1) * C::BBytes + r * 128;
+        for (int p = half; p < rank / 8; p += 2) copy16(dst + (p >> 3) * (kAD_Tile * 128) + (((p & 7) ^ (r & 7)) << 4), src + 8 * p, in);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (!sent) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        send();
+      }
+      if (++c == tpg) {
+        c = 0;
+        ++g;
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (ok && n) {
+      fence_async_smem();
+      mbar_arrive(b_full + ((n - 1) & 1));
+    }
+  } else {
+    wait_for_stream();
+    if (warp == 6) {
+      tmem_alloc(&s_tmem, 2 * kAD_Tile);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 1, 288;" ::: "memory");       // warps 6 to 14
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    if (warp == 6) {
+      const uint32_t idesc = idesc_f16(128, kAD_Tile, kIsBf16<T>);
+      int steps = 0;
+#pragma unroll 1
+      for (int j = 0, g = g0, c = c0; j < n; ++j) {
+        if (j == 0 || c == 0) {
+          const int id = a.groups[g].x;
+          steps = id < a.n ? (a.row[id + 1] - a.row[id]) / 16 : 0;
+        }
+        if (!mbar_wait_warp_small(d_free + (j & 1), (j >> 1 & 1) ^ 1, abort, 0x85)) break;
+        if (!mbar_wait_warp_small(b_full + (j & 1), j >> 1 & 1, abort, 0x86)) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t b = bs + (j & 1) * C::BBytes, d = tmem + (j & 1) * kAD_Tile;
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part)
+#pragma unroll 1
+            for (int ks = 0; ks < steps; ++ks) {
+              const uint32_t k = (ks >> 2) * (128 * 128) + (ks & 3) * 32;      // both operands have 128 rows
+              umma_f16_ss(d, sdesc_sw128(hs + part * (C::HBytes / 2) + k), sdesc_sw128(b + k), idesc, part > 0 || ks > 0);
+            }
+          umma_commit(b_free + (j & 1));
+          umma_commit(d_full + (j & 1));
+        }
+        __syncwarp();
+        if (++c == tpg) {
+          c = 0;
+          ++g;
+        }
+      }
+    } else {
+      const int row0 = 32 * (warp & 3), r = row0 + lane, at = 64 * ((warp - 7) >> 2);
+      const uint8_t* from = s_y + (row0 + (lane >> 3)) * kAD_Pitch + 2 * at + 16 * (lane & 7);      // eight lanes write a row
+      T* out = nullptr;
+      float scale = 0.f;
+      int m = 0;
+      bool adapted = false;
+#pragma unroll 1
+      for (int j = 0, g = g0, c = c0; j < n; ++j) {
+        if (j == 0 || c == 0) {
+          const int4 grp = a.groups[g];
+          m = grp.z;
+          adapted = grp.x < a.n;
+          if (r < m) {
+            out = static_cast<T*>(a.out) + (long long)a.perm[grp.y + r] * a.o_st + at;
+            if (adapted) scale = a.back[grp.y + r];
+          }
+        }
+        const int s = j % C::Ring, cols = min(64, a.d_out - c * kAD_Tile - at);
+        if (!mbar_wait_warp_small(d_full + (j & 1), j >> 1 & 1, abort, 0x87)) break;
+        if (!mbar_wait_warp_small(y_full + s, j / C::Ring & 1, abort, 0x88)) break;
+        tc_fence_after();
+        uint8_t* y = s_y + s * C::YBytes + r * kAD_Pitch + 2 * at;
+        if (adapted && row0 < m) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (16 * k >= cols) break;
+            uint32_t d[16];
+            tmem_ld16(tmem + (j & 1) * kAD_Tile + at + 16 * k + ((uint32_t)row0 << 16), d);
+            tmem_wait_ld();
+            if (r < m) {
+              // (behind d_out the second eight are no values: they go nowhere)
+              uint4 v[2] = {*reinterpret_cast<const uint4*>(y + 32 * k), *reinterpret_cast<const uint4*>(y + 32 * k + 16)};
+              T* x = reinterpret_cast<T*>(v);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = (T)fmaf(__uint_as_float(d[i]), scale, (float)x[i]);
+              *reinterpret_cast<uint4*>(y + 32 * k) = v[0];
+              *reinterpret_cast<uint4*>(y + 32 * k + 16) = v[1];
+            }
+          }
+        }
+        tc_fence_before();
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(d_free + (j & 1));
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const uint4*>(from + s * C::YBytes + 4 * i * kAD_Pitch);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(y_free + s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), 4 * i + (lane >> 3)));
+          if (row0 + 4 * i + (lane >> 3) < m && 8 * (lane & 7) < cols) *reinterpret_cast<uint4*>(to + c * kAD_Tile + 8 * (lane & 7)) = v[i];
+        }
+        if (++c == tpg) {
+          c = 0;
+          ++g;
+        }
       }
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   if (tid == 0) report_abort(abort, a.err);
-  if (warp == 0 && rank) {
+  if (warp == 6) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(s_tmem, 2 * kAD_Tile);
   }
 }
 
@@ -781,10 +843,10 @@ static int launch_shrink(const AdapterArgs& a, unsigned groups, cudaStream_t str
 }
 
 template <typename T, int RM>
-static int launch_expand(const AdapterArgs& a, unsigned groups, cudaStream_t stream) {
+static int launch_expand(const AdapterArgs& a, int sms, cudaStream_t stream) {
   using C = ExpandCfg<T, RM>;
   const int rc = ensure_smem_attr((const void*)adapter_expand_kernel<T, RM>, C::Smem);
-  return rc ? rc : launch_early(adapter_expand_kernel<T, RM>, dim3(groups, (a.d_out + kAD_Tile * a.units - 1) / (kAD_Tile * a.units)), 256, C::Smem, stream, a);
+  return rc ? rc : launch_early(adapter_expand_kernel<T, RM>, dim3(sms), 480, C::Smem, stream, a);
 }
 
 template <typename T>
@@ -804,12 +866,7 @@ static int launch_adapters(AdapterArgs a, int sms, cudaStream_t stream) {
   rc = a.rmax <= 32 ? launch_shrink<T, 32, 5>(a, groups, stream)
        : a.rmax <= 64 ? launch_shrink<T, 64, 4>(a, groups, stream) : launch_shrink<T, 128, 3>(a, groups, stream);
   if (rc) return rc;
-  // tiles per CTA: h's parts are made once for all of them, but there have to be enough CTAs
-  const long long real = (a.T + kAD_Group - 1) / kAD_Group;
-  const int blocks = (a.d_out + kAD_Tile - 1) / kAD_Tile;
-  a.units = 16;
-  while (a.units > 1 && real * ((blocks + a.units - 1) / a.units) < 4LL * sms) a.units >>= 1;
-  return a.rmax <= 64 ? launch_expand<T, 64>(a, groups, stream) : launch_expand<T, 128>(a, groups, stream);
+  return a.rmax <= 64 ? launch_expand<T, 64>(a, sms, stream) : launch_expand<T, 128>(a, sms, stream);
 }
 
 }  // namespace bfb
