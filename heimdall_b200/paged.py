@@ -15,7 +15,7 @@ host and can be captured into a CUDA graph:
 ``fork`` shares pages between sequences, ``free`` and ``truncate`` give them back, ``compact`` closes the pool up.  Where a batch has forks of
 one prompt, or of a tree of them, ``share`` finds which pages its sequences have in common, and ``attend`` reads those once for all:
 
-    plan = c.share(slots)                     # host: again after a free or truncate
+    plan = c.share(slots)                     # host: again after forks, and when the plan is no longer good
     o, _ = c.attend(layer, q, shared=plan)    # device
 
 Calls on one cache belong on one stream, or on streams that the caller orders, and on one host thread at a time.  There is no
@@ -24,6 +24,7 @@ CPU path.
 from __future__ import annotations
 
 import ctypes
+import weakref
 
 import numpy as np
 import torch
@@ -35,7 +36,12 @@ from .structs import BfPagePool, BfPageTable
 
 PAGE_SIZES = (16, 32, 64, 128)
 MAX_GROUP = 24                  # query heads per KV head of attend
-MIN_SAVED = 1024                # tokens that a shared run has to save
+# Tokens of reading that a shared run has to save, and all runs of n sequences together: WORTH[0] + WORTH[1] n.  The way over shared pages has more to start
+# (15 us against 8 for the smallest calls) and spends more on each sequence's own tokens.  Decode steps, us without and with a plan: 24 heads
+# of 4, two sequences that share 16384 tokens 21 and 25; eight, 28672 saved 19 and 21, 57344 saved 27 and 23; 64, 32256 saved 22 and 28, 64512 saved 32 and 30 (with 1000
+# tokens of their own 47 and 56, then at 129024 64 and 54); 24 heads of one, 32 sequences, 31744 saved 20 and 21, 126976 saved 30 and 26.
+# (24 heads of one and up to eight sequences gain from 2000 on, 26 against 17: min_saved is for those.)
+MIN_SAVED, WORTH = 1024, (32768, 512)
 
 
 _REASONS = {1: "a slot is outside [0, {slots})", 2: "a slot is named twice", 3: "a number of tokens is negative",
@@ -146,10 +152,17 @@ class SharedPages:
         self.n = slots.size
         self.plan = torch.empty(plan.size, dtype=torch.int32, device=cache.device)
         self._fill(slots, plan)
+        cache._plans.add(self)
 
     def _fill(self, slots: np.ndarray, plan: np.ndarray) -> None:
-        self.slots, self.runs, self.version = slots.tolist(), int(plan[0]), self.cache._shrunk
+        self.slots, self.runs, self.good = slots.tolist(), int(plan[0]), True
+        # the tokens of each slot that are read as shared pages
+        self._covered = dict(zip(self.slots, (plan[4 + 4 * self.n:4 + 5 * self.n] * self.cache.page).tolist()))
         self.plan.copy_(torch.from_numpy(plan))
+
+    def _cut(self, slots, lens) -> None:
+        if any(n < self._covered.get(s, 0) for s, n in zip(slots, lens)):
+            self.good = False
 
 
 class PagedKV:
@@ -188,7 +201,9 @@ class PagedKV:
                                 ptr(self.lens), layers, pages, heads, page, dim, slots, width)
         self._pool_ptr = ctypes.addressof(self._pool)
         self._ws = {}                       # workspace bytes by (B, t, H), with True behind them for shared pages
-        self._shrunk = 0                    # calls of free and truncate: plans of shared pages from before are not good
+        self._plans = weakref.WeakSet()     # plans of shared pages, good until a slot is cut below what they cover of it
+        self._layer_plans = {}              # those of layer(share=True) by the number of sequences, with the forks that they know of
+        self._forks = 0
         self._ended = False                 # a change has reached the host's table and not the device's
         self._appended = set()              # layers that the caller's own append has written, for as long as no layer() is out
         self._progress = None               # what retrieval.teacher has written, from the first layer() on
@@ -237,7 +252,7 @@ class PagedKV:
     def free(self, slots) -> None:
         """End the sequences of these slots: their pages return to the pool unless another sequence shares them."""
         self._apply(self.host.free, slots)
-        self._shrunk += 1
+        self._cut(slots)
         if self._progress is not None:
             self._progress.free(slots)
 
@@ -245,6 +260,7 @@ class PagedKV:
         """The (empty) slots dst continue the sequences of src: full pages are shared, the tokens of a partly filled last
         page are copied, in every layer."""
         self._apply(self.host.fork, src, dst)
+        self._forks += 1
         if self._progress is not None:
             self._progress.fork(src, dst)
 
@@ -252,9 +268,16 @@ class PagedKV:
         """Shorten the sequences of these slots to lens tokens (rejected drafts); a shared page that becomes partly filled
         is copied.  The scale of the page that is cut stays as it is."""
         self._apply(self.host.truncate, slots, lens)
-        self._shrunk += 1
+        self._cut(slots, lens)
         if self._progress is not None:
             self._progress.truncate(slots, lens)
+
+    def _cut(self, slots, lens=0) -> None:
+        if self._plans:
+            slots = self.host._whole(slots)
+            lens = self.host._whole(lens, slots).tolist()
+            for plan in self._plans:
+                plan._cut(slots.tolist(), lens)
 
     def compact(self) -> int:
         """Move the live pages at or above their number into the holes below it (both in ascending order), so that the
@@ -262,17 +285,18 @@ class PagedKV:
         self._apply(self.host.compact)
         return self.host.pages - self.host.n_free
 
-    def share(self, slots, into: SharedPages = None, min_saved: int = MIN_SAVED) -> SharedPages:
+    def share(self, slots, into: SharedPages = None, min_saved: int = None) -> SharedPages:
         """Which pages these sequences (slots, a list of whole numbers; one may come several times) have in common, for ``attend(shared=)``: the
-        runs of pages that are read once for several of them.  The plan is good until a slot is freed or truncated (attend refuses it after that);
-        reserve, append, fork and compact leave it good, though sequences forked later are not in it.  ``into``: a plan of as many sequences,
+        runs of pages that are read once for several of them.  The plan is good until a slot of it is freed or truncated into the pages that it
+        shares (attend refuses it after that); everything else leaves it good, though sequences forked later are not in it.  ``into``: a plan of as many sequences,
         whose device memory takes the new one, so that a captured attend goes on with it.  Runs that save fewer than
-        ``min_saved`` tokens of reading ((sequences - 1) * tokens) are not worth their start and are left out.  At most four
+        ``min_saved`` tokens of reading ((sequences - 1) * tokens) are left out; None: those that are not worth their start, which is all of them if
+        together they save fewer than 32768 and 512 for each sequence (attend is then the call without a plan).  At most four
         runs to a sequence; deeper ones are read sequence by sequence."""
         self._check()
         if into is not None and (not isinstance(into, SharedPages) or into.cache is not self):
             raise ValueError("into must be a plan of this cache")
-        if min_saved < 1:
+        if min_saved is not None and min_saved < 1:
             raise ValueError("min_saved must be positive")
         slots = self.host._whole(slots)
         if into is not None and into.n != slots.size:
@@ -280,7 +304,12 @@ class PagedKV:
         with on_device(self.device):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("heimdall_b200: what is shared is found on the host: share cannot be captured into a CUDA graph")
-            plan = self.host.share(slots, min(int(min_saved), 2 ** 31 - 1))
+            plan = self.host.share(slots, MIN_SAVED if min_saved is None else min(int(min_saved), 2 ** 31 - 1))
+            if min_saved is None:
+                n = slots.size
+                runs = plan[4 + 5 * n:4 + 5 * n + 6 * int(plan[0])].reshape(-1, 6).astype(np.int64)
+                if ((runs[:, 1] - 1) * (runs[:, 3] - runs[:, 2])).sum() * self.page < WORTH[0] + WORTH[1] * n:
+                    plan = self.host.share(slots, 2 ** 31 - 1)
             if into is None:
                 return SharedPages(self, slots, plan)
             into._fill(slots, plan)
@@ -395,13 +424,23 @@ class PagedKV:
             raise ValueError("the plan of shared pages has its own slots")
         if shared.n != B:
             raise ValueError(f"the plan is of {shared.n} sequences, not of {B}")
-        if shared.version != self._shrunk:
-            raise ValueError("slots were freed or truncated since this plan was made: share again")
+        if not shared.good:
+            raise ValueError("slots were freed, or truncated into shared pages, since this plan was made: share again")
 
-    def layer(self, layer: int) -> "PagedLayer":
+    def layer(self, layer: int, share: bool = False) -> "PagedLayer":
         """This cache as one kept layer's ``cache`` argument of ``retrieval.teacher`` (slots 0 .. B-1).  How far the layer
-        is belongs to the cache: fetched once or for every call, a layer goes on where it was."""
-        return PagedLayer(self, self._layer(layer))
+        is belongs to the cache: fetched once or for every call, a layer goes on where it was.  ``share``: pages that
+        the sequences have in common are read once for all of them (``attend(shared=)``, with its precision there); the plan, one for
+        all layers, is made at the first call that needs it and after forks, and again when it is no longer good.  That is host work: before such a call is captured,
+        one has to have run."""
+        return PagedLayer(self, self._layer(layer), share)
+
+    def _layer_plan(self, B: int):
+        plan, forks = self._layer_plans.get(B, (None, -1))
+        if forks != self._forks or not plan.good:
+            plan = self.share(range(B), into=plan)
+            self._layer_plans[B] = plan, self._forks
+        return plan if plan.runs else None
 
 
 class _Progress:
@@ -452,8 +491,8 @@ class PagedLayer:
     teacher, an ``append`` to sequences whose room the caller reserved waits for its slot numbers to be read back.)  Replays of a captured
     call are not seen by the host; what was captured goes on by replays, or anew after ``free``."""
 
-    def __init__(self, cache: PagedKV, layer: int):
-        self.cache, self.index = cache, layer
+    def __init__(self, cache: PagedKV, layer: int, share: bool = False):
+        self.cache, self.index, self.share = cache, layer, bool(share)
         if cache._progress is None:
             cache._progress = _Progress(cache)
 
@@ -509,7 +548,7 @@ class PagedLayer:
         q, k, v = qr.transpose(1, 2).to(dt), kr.transpose(1, 2).to(dt), v.to(dt)
         c._append(self.index, k, v)
         if later:
-            return c.attend(self.index, q)[0].to(qr.dtype)
+            return c.attend(self.index, q, shared=c._layer_plan(B) if self.share else None)[0].to(qr.dtype)
         # a whole prompt: attention over the keys and values as they are, not over their codes
         cu = torch.arange(B + 1, device=qr.device, dtype=torch.int32) * t
         o, _ = prompt_attention(q.reshape(B * t, H, D), k.reshape(B * t, c.heads, D), v.reshape(B * t, c.heads, D), cu)

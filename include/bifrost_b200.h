@@ -472,7 +472,7 @@ int bf_paged_attend(const bf_page_pool* pool, int layer, const void* q, long lon
 /* Sequences with pages in common (forks of one another), each shared page read once for all of them.
  * bf_page_table_share: HOST; which runs of pages the n sequences (slots, one may come several times) share, as a plan of bf_share_words(n) int32 for the
  *   device: runs that save reading at least min_saved tokens ((sequences - 1) * tokens), at most 4 to a sequence; scratch [7 n] int32.
- *   It holds no pages, only which slots share how many: it is good until a slot of it is freed or truncated.
+ *   It holds no pages, only which slots share how many: it is good until a slot of it is freed or truncated into them.
  * bf_paged_attend_shared: bf_paged_attend of the plan's n sequences (q [n,t,H,D] in the order of the slots given).  plan on the device, 16-byte aligned.
  *   Within shared pages a component of q is held exactly (BF_BF16: 8, BF_F16: 11 bits) where that does not need more than 2^-17 of its row's largest, and
  *   to 2^-17 of that otherwise; a weight times its V scale to 2^-9 (BF_F16: 2^-12) of itself or 2^-18 of the largest among the 128 tokens of its tile,
