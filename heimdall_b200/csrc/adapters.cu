@@ -36,15 +36,15 @@ struct AdapterArgs {
   const int32_t* row;              // [n + 1] the adapters' first rows in A, multiples of 16
   const float* scale;              // [n]
   const void *A, *B;               // A [row[n]][d_in]; B: adapter a's [d_out][r_a] from element row[a] d_out on
-  int n, T, d_in, d_out, rmax, splits, kper, units;
+  int n, T, d_in, d_out, rmax, splits, units;
   unsigned int* err;
-  float* h;                        // [splits][T][rmax]; many tokens: by their place in perm
+  float* h;                        // few tokens: [splits][T][rmax]; many: two places per CTA of [kAD_Group][rmax rounded up to 32, 64, 128]
   void* parts;                     // [T][2][rmax] h's two parts, by place in perm
   float* back;                     // [T] the scale that undoes theirs, times the adapter's
-  int32_t* arrived;                // [groups] splits that are done
+  int32_t* arrived;                // [groups] parts of h that are done
   int32_t* perm;                   // [T] tokens by adapter
   int4* groups;                    // (adapter or n, first of perm, tokens, -)
-  int32_t* n_groups;
+  int32_t* n_groups;               // all that out needs, and those of adapters
 };
 
 template <typename T>
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(AdapterArgs a) 
   if (m == 0 || id == a.n) return;
   const int r0 = a.row[id], rank = a.row[id + 1] - r0, rc = blockIdx.z * 16;
   if (rc >= rank) return;
-  const int k0 = blockIdx.y * a.kper, k1 = min(k0 + a.kper, a.d_in);
+  const int k0 = blockIdx.y * kAD_KFew, k1 = min(k0 + kAD_KFew, a.d_in);
   const T* x0 = static_cast<const T*>(a.x) + (long long)s_tok[min(g, m - 1)] * a.x_st + 8 * c;
   const T* x1 = static_cast<const T*>(a.x) + (long long)s_tok[min(g + 8, m - 1)] * a.x_st + 8 * c;
   const T* w0 = static_cast<const T*>(a.A) + (long long)(r0 + rc + g) * a.d_in + 8 * c;
@@ -251,7 +251,10 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     a.groups[k] = make_int4(b, first, min(kAD_Group, s_at[b + 1] - first), 0);
     a.arrived[k] = 0;
   }
-  if (tid == 0) *a.n_groups = a.out == a.y ? s_grp[a.n] : total;      // tokens without an adapter come last: in place they are done
+  if (tid == 0) {
+    a.n_groups[1] = s_grp[a.n];       // tokens without an adapter come last: they have no h, and in place they are done
+    a.n_groups[0] = a.out == a.y ? s_grp[a.n] : total;
+  }
   __syncthreads();
   for (int t0 = 0; t0 < a.T; t0 += 1024 * per) {
     if (a.T > 1024 * per) load(t0);
@@ -282,153 +285,225 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   }
 }
 
-// h of a group of 128 tokens: CTA = (group, part of d_in).  x rows (gathered) and A rows come 64 values at a time through a ring in shared memory
-// (K-major, 128-byte swizzle), all threads copying; one thread issues the products of a stage, D in TMEM is the group's h.
-template <typename T, int RM, int ST>
-__global__ void __launch_bounds__(256) adapter_shrink_kernel(AdapterArgs a) {
-  constexpr int kStage = (kAD_Group + RM) * 128, kCols = RM < 32 ? 32 : RM;
+// h of many tokens: the groups' steps of 128 values of d_in, group by group, an equal run of them to each CTA, one per SM.  x rows (gathered) and A rows come
+// through a ring in shared memory (K-major, 128-byte swizzle; eight warps copy); a thread issues the products, D in TMEM (two of them) is the group's h.  A run
+// that has part of a group leaves its sums in one of the CTA's two places (its first group, begun by others; its last, ended by others); the CTA that is the
+// last to bring a group's part adds them all, in their order, and makes the two parts.  (A grid of groups and parts of d_in, two CTAs per SM: 25480 tokens of
+// 6144 took 92 us, 8192 of 5120 37, against XX and XX.)
+constexpr int kAD_Ctas = 148, kAD_Step = 128, kAD_MinSteps = 8;
+template <int RM>
+struct ShrinkCfg {
+  static constexpr int Stage = (kAD_Group + RM) * 256, Ring = RM <= 32 ? 5 : RM <= 64 ? 4 : 3, Smem = Stage * Ring + 1024;
+};
+
+template <typename T, int RM>
+__global__ void __launch_bounds__(416, 1) adapter_shrink_kernel(AdapterArgs a) {
+  using C = ShrinkCfg<RM>;
+  constexpr int ST = C::Ring, kLag = ST - 2;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int s_tok[kAD_Group];
-  __shared__ uint64_t s_bar[ST];
+  const uint32_t ring_at = (smem_u32(smem_raw) + 1023) & ~1023u;
+  __shared__ uint64_t x_full[ST], x_free[ST], d_full[2], d_free[2], h_full, h_told;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_last;
   volatile int* abort = &s_abort;
   wait_for_stream();
   let_next_start();
-  if ((int)blockIdx.x >= *a.n_groups) return;
-  const int4 grp = a.groups[blockIdx.x];
-  if (grp.x == a.n) return;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, m = grp.z;
-  const int r0 = a.row[grp.x], rank = a.row[grp.x + 1] - r0;
-  if (tid < kAD_Group) s_tok[tid] = a.perm[grp.y + min(tid, m - 1)];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int spg = (a.d_in + kAD_Step - 1) / kAD_Step;
+  const long long total = (long long)a.n_groups[1] * spg, ctas = max(1ll, min((long long)kAD_Ctas, total / kAD_MinSteps));
+  if ((int)blockIdx.x >= ctas || total == 0) return;
+  const long long first = total * blockIdx.x / ctas;
+  const int n = (int)(total * (blockIdx.x + 1) / ctas - first), g0 = (int)(first / spg), k0 = (int)(first - (long long)g0 * spg);
   if (tid == 0) {
-    for (int i = 0; i < ST; ++i) mbar_init(s_bar + i, 1);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(x_full + i, 256);
+      mbar_init(x_free + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(d_full + i, 1);
+      mbar_init(d_free + i, 4);
+    }
+    mbar_init(&h_full, 4);
+    mbar_init(&h_told, 1);
     s_abort = 0;
     fence_barrier_init();
   }
-  if (warp == 0) {
-    tmem_alloc(&s_tmem, kCols);
+  if (warp == 8) {
+    tmem_alloc(&s_tmem, 2 * RM);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem, ring_at = smem_u32(ring);
-  const int k0 = blockIdx.y * a.kper, k1 = min(k0 + a.kper, a.d_in), stages = (k1 - k0 + 63) / 64;
-  // a thread's pieces of 16 bytes: piece tid % 8 of the rows tid / 8 + 32 i, x rows first.  Rows of tokens that are not there repeat the last one
-  const int piece = tid & 7, prow = tid >> 3;
-  const T* src[(kAD_Group + RM) / 32];
-#pragma unroll
-  for (int i = 0; i < (kAD_Group + RM) / 32; ++i) {
-    const int r = prow + 32 * i;
-    src[i] = (r < kAD_Group ? static_cast<const T*>(a.x) + (long long)s_tok[r] * a.x_st
-                            : static_cast<const T*>(a.A) + (long long)(r0 + min(r - kAD_Group, rank - 1)) * a.d_in) + 8 * piece;
-  }
-  auto fetch = [&](int s) {
-    if (s < stages) {
-      const int k = k0 + 64 * s;
-      const bool in = k + 8 * piece < k1;
-      const uint32_t dst = ring_at + (s % ST) * kStage + prow * 128 + ((piece ^ (prow & 7)) << 4);
-#pragma unroll
-      for (int i = 0; i < (kAD_Group + RM) / 32; ++i)
-        if (32 * i + prow < kAD_Group + rank) copy16(dst + i * 4096, in ? src[i] + k : src[i], in);
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int s = 0; s < ST - 1; ++s) fetch(s);
-  const uint32_t idesc = idesc_f16(128, rank, kIsBf16<T>);
-  bool ok = true;
-  for (int s = 0; s < stages && ok; ++s) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
-    fence_async_smem();
-    __syncthreads();
-    if (tid == 0) {
-      tc_fence_after();
-      const uint32_t xs = ring_at + (s % ST) * kStage;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        umma_f16_ss(tmem, sdesc_sw128(xs + ks * 32), sdesc_sw128(xs + kAD_Group * 128 + ks * 32), idesc, s > 0 || ks > 0);
-      umma_commit(s_bar + s % ST);
-    }
-    // stage s + ST - 1 takes the place of s - 1, whose products were issued a stage ago
-    if (s > 0 && s + ST - 1 < stages) ok = mbar_wait_small(s_bar + (s - 1) % ST, ((s - 1) / ST) & 1, abort, 0x80);
-    fetch(s + ST - 1);
-  }
-  ok = ok && mbar_wait_small(s_bar + (stages - 1) % ST, ((stages - 1) / ST) & 1, abort, 0x81);
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  ok = __all_sync(0xffffffffu, ok) != 0;
-  tc_fence_after();
-  if (warp < 4 && ok) {
-    const int r = 32 * warp + lane;
-    float* to = a.h + ((size_t)blockIdx.y * a.T + grp.y + r) * a.rmax;
+  const uint32_t tmem = s_tmem;
+  if (warp < 8) {
+    // a thread's pieces of 16 bytes: piece tid % 16 of the rows tid / 16 + 16 i, x rows first.  Rows of tokens that are not there repeat the last one
+    const int piece = tid & 15, prow = tid >> 4;
+    const uint32_t to = ring_at + (piece >> 3) * (kAD_Group * 128) + prow * 128 + (((piece & 7) ^ (prow & 7)) << 4);
+    const uint32_t toA = ring_at + kAD_Group * 256 + (piece >> 3) * (RM * 128) + prow * 128 + (((piece & 7) ^ (prow & 7)) << 4);
+    const T* src[8] = {};
+    const T* srcA = nullptr;
+    int rank = 0;
 #pragma unroll 1
-    for (int c = 0; c < rank; c += 16) {
-      uint32_t v[16];
-      tmem_ld16(tmem + ((uint32_t)(32 * warp) << 16) + c, v);
-      tmem_wait_ld();
-      if (r < m) {
+    for (int j = 0, g = g0, k = k0; j < n + kLag; ++j) {
+      if (j < n) {
+        if (j == 0 || k == 0) {
+          const int4 grp = a.groups[g];
+          const int r0 = a.row[grp.x];
+          rank = a.row[grp.x + 1] - r0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(to + c)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          for (int i = 0; i < 8; ++i)
+            src[i] = static_cast<const T*>(a.x) + (long long)a.perm[grp.y + min(prow + 16 * i, grp.z - 1)] * a.x_st + 8 * piece;
+          srcA = static_cast<const T*>(a.A) + (long long)(r0 + prow) * a.d_in + 8 * piece;
+        }
+        if (!mbar_wait_small(x_free + j % ST, (j / ST & 1) ^ 1, abort, 0x80)) break;
+        const bool in = kAD_Step * k + 8 * piece < a.d_in;
+        const int at = in ? kAD_Step * k : 0;
+        const uint32_t stage = (j % ST) * C::Stage;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) copy16(to + stage + i * 2048, in ? src[i] + at : static_cast<const T*>(a.x), in);
+        const T* w = in ? srcA + at : static_cast<const T*>(a.A);
+#pragma unroll
+        for (int i = 0; i < RM / 16; ++i, w += in ? 16 * (long long)a.d_in : 0)
+          if (16 * i < rank) copy16(toA + stage + i * 2048, w, in);
+        if (++k == spg) {
+          k = 0;
+          ++g;
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (j >= kLag) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+        fence_async_smem();
+        mbar_arrive(x_full + (j - kLag) % ST);
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (warp == 8) {
+    uint32_t idesc = 0;
+    int parts = 0;            // begun
+#pragma unroll 1
+    for (int j = 0, g = g0, k = k0; j < n; ++j) {
+      const bool begins = j == 0 || k == 0, ends = j == n - 1 || k == spg - 1;
+      if (begins) {
+        const int id = a.groups[g].x;
+        idesc = idesc_f16(128, a.row[id + 1] - a.row[id], kIsBf16<T>);
+        if (!mbar_wait_warp_small(d_free + (parts & 1), (parts >> 1 & 1) ^ 1, abort, 0x81)) break;
+        ++parts;
+      }
+      if (!mbar_wait_warp_small(x_full + j % ST, j / ST & 1, abort, 0x89)) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t xs = ring_at + (j % ST) * C::Stage, as = xs + kAD_Group * 256, d = tmem + ((parts - 1) & 1) * RM;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+          umma_f16_ss(d, sdesc_sw128(xs + (ks >> 2) * (kAD_Group * 128) + (ks & 3) * 32), sdesc_sw128(as + (ks >> 2) * (RM * 128) + (ks & 3) * 32), idesc,
+                      !begins || ks > 0);
+        umma_commit(x_free + j % ST);
+        if (ends) umma_commit(d_full + ((parts - 1) & 1));
+      }
+      __syncwarp();
+      if (++k == spg) {
+        k = 0;
+        ++g;
+      }
+    }
+  } else {
+    // thread = row of the group; sums of part of d_in lie rank by rank, so that rows are neighbours
+    const int row0 = 32 * (warp & 3), r = row0 + lane;
+    // the CTA that has step i (no run is empty)
+    auto cta_of = [&](long long i) { return (int)(((i + 1) * ctas + total - 1) / total) - 1; };
+    uint32_t shared = 0;               // groups that are other CTAs' too
+#pragma unroll 1
+    for (int p = 0, g = g0, left = n, k = k0; left > 0; ++p, ++g, left -= spg - k, k = 0) {
+      const int4 grp = a.groups[g];
+      const int m = grp.z, rank = a.row[grp.x + 1] - a.row[grp.x];
+      const int b0 = cta_of((long long)g * spg), b1 = cta_of((long long)(g + 1) * spg - 1);
+      const float scale = a.scale[grp.x];
+      if (!mbar_wait_warp_small(d_full + (p & 1), p >> 1 & 1, abort, 0x8a)) break;
+      tc_fence_after();
+      float v[RM];
+#pragma unroll
+      for (int c = 0; c < RM; c += 16)
+        if (c < rank) {
+          uint32_t x[16];
+          tmem_ld16(tmem + (p & 1) * RM + ((uint32_t)row0 << 16) + c, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[c + i] = __uint_as_float(x[i]);
+        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(d_free + (p & 1));
+      if (b0 < b1) {
+        auto place = [&](int b) { return a.h + (size_t)(2 * b + (b == b0)) * kAD_Group * RM + r; };
+        float* to = place(blockIdx.x);
+#pragma unroll
+        for (int c = 0; c < RM; ++c)
+          if (c < rank) __stcg(to + c * kAD_Group, v[c]);
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&h_full);
+        const uint32_t phase = shared++ & 1;
+        if (warp == 9) {
+          if (!mbar_wait_warp_small(&h_full, phase, abort, 0x8b)) break;
+          if (lane == 0) {
+            s_last = atomicAdd(a.arrived + g, 1) == b1 - b0;
+            mbar_arrive(&h_told);
+          }
+          __syncwarp();
+        }
+        if (!mbar_wait_warp_small(&h_told, phase, abort, 0x8c)) break;
+        if (!s_last) continue;         // (s_last is written again when all four warps are behind the next part's stores)
+        __threadfence();
+        // 32 loads at a time, those of ranks that are not there too
+#pragma unroll
+        for (int c = 0; c < RM; c += 32)
+          if (c < rank) {
+#pragma unroll 1
+            for (int b = b0; b <= b1; ++b) {
+              const float* from = place(b) + c * kAD_Group;
+              float x[32];
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = __ldcg(from + i * kAD_Group);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[c + i] = b == b0 ? x[i] : v[c + i] + x[i];
+            }
+          }
+      }
+      float big = 0.f;           // (a NaN is no maximum, but its row becomes NaN by itself)
+#pragma unroll
+      for (int c = 0; c < RM; ++c)
+        if (c < rank) big = fmaxf(big, fabsf(v[c]));
+      // a power of two that takes the row's largest to [2^13, 2^14): both parts then keep all of their bits in fp16 too
+      const int ex = big > 0.f && big < INFINITY ? min(max((int)(__float_as_uint(big) >> 23), 14), 253) : 140;
+      const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
+      if (r < m) {
+        T* to = static_cast<T*>(a.parts) + (size_t)(grp.y + r) * 2 * a.rmax;
+#pragma unroll
+        for (int c = 0; c < RM; c += 8)
+          if (c < rank) {
+            uint4 h, l;
+            T *hi = reinterpret_cast<T*>(&h), *lo = reinterpret_cast<T*>(&l);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float x = v[c + i] * up;
+              hi[i] = (T)x;
+              lo[i] = (T)(x - (float)hi[i]);
+            }
+            *reinterpret_cast<uint4*>(to + c) = h;
+            *reinterpret_cast<uint4*>(to + a.rmax + c) = l;
+          }
+        a.back[grp.y + r] = scale * __uint_as_float((uint32_t)(ex - 13) << 23);
       }
     }
   }
-  // the CTA that is the last to bring its split adds them all, in their order, and makes the two parts: a warp four rows at a time, lane l the
-  // ranks 2 l, 2 l + 1 (and 64 more)
-  __threadfence();
   tc_fence_before();
   __syncthreads();
-  if (tid == 0) s_last = atomicAdd(a.arrived + blockIdx.x, 1) == a.splits - 1;
-  __syncthreads();
-  if (s_last) {
-    __threadfence();
-    constexpr int kPairs = RM <= 64 ? 1 : 2;
-    const float scale = a.scale[grp.x];
-    for (int rb = 4 * warp; rb < m; rb += 32) {
-      float2 v[4][kPairs];
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) v[q][i] = make_float2(0.f, 0.f);
-#pragma unroll 2
-      for (int sp = 0; sp < a.splits; ++sp)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int i = 0; i < kPairs; ++i)
-            if (rb + q < m && 64 * i + 2 * lane < rank) {
-              const float2 x = __ldcg(reinterpret_cast<const float2*>(a.h + ((size_t)sp * a.T + grp.y + rb + q) * a.rmax + 64 * i + 2 * lane));
-              v[q][i].x += x.x;
-              v[q][i].y += x.y;
-            }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (rb + q >= m) break;
-        float big = 0.f;           // (a NaN is no maximum, but its row becomes NaN by itself)
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) big = fmaxf(big, fmaxf(fabsf(v[q][i].x), fabsf(v[q][i].y)));
-        big = warp_max(big);
-        // a power of two that takes the row's largest to [2^13, 2^14): both parts then keep all of their bits in fp16 too
-        const int ex = big > 0.f && big < INFINITY ? min(max((int)(__float_as_uint(big) >> 23), 14), 253) : 140;
-        const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
-        T* to = static_cast<T*>(a.parts) + (size_t)(grp.y + rb + q) * 2 * a.rmax;
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i)
-          if (64 * i + 2 * lane < rank) {
-            const float x = v[q][i].x * up, y = v[q][i].y * up;
-            const T hi[2] = {(T)x, (T)y}, lo[2] = {(T)(x - (float)hi[0]), (T)(y - (float)hi[1])};
-            *reinterpret_cast<uint32_t*>(to + 64 * i + 2 * lane) = *reinterpret_cast<const uint32_t*>(hi);
-            *reinterpret_cast<uint32_t*>(to + a.rmax + 64 * i + 2 * lane) = *reinterpret_cast<const uint32_t*>(lo);
-          }
-        if (lane == 0) a.back[grp.y + rb + q] = scale * __uint_as_float((uint32_t)(ex - 13) << 23);
-      }
-    }
-  }
   if (tid == 0) report_abort(abort, a.err);
-  if (warp == 0) {
+  if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tmem, kCols);
+    tmem_dealloc(tmem, 2 * RM);
   }
 }
 
@@ -791,27 +866,6 @@ __global__ void __launch_bounds__(480, 1) adapter_expand_kernel(AdapterArgs a) {
   }
 }
 
-// how d_in is split: few tokens in parts of kAD_KFew; many so that the rounds of CTAs (two to an SM) times what each reads, plus 512 values' worth for its
-// start and end, are fewest
-static void adapter_split(int T, int d_in, int* splits, int* kper) {
-  int s = 1;
-  if (T <= kAD_Few) {
-    *kper = kAD_KFew;
-  } else {
-    const long long groups = (T + kAD_Group - 1) / kAD_Group, slots = 2 * 148;
-    long long best = 1ll << 62;
-    for (int k = 1; k <= 16 && k <= (d_in + 255) / 256; ++k) {
-      const long long cost = (groups * k + slots - 1) / slots * (d_in / k + 512);
-      if (cost < best) {
-        best = cost;
-        s = k;
-      }
-    }
-    *kper = ((d_in + s - 1) / s + 63) / 64 * 64;
-  }
-  *splits = (d_in + *kper - 1) / *kper;
-}
-
 static long long adapter_groups(int T, int n) { return T / kAD_Group + (n + 1 < T ? n + 1 : T); }
 
 // the workspace: its bytes, and the arrays in it
@@ -824,22 +878,23 @@ static size_t adapter_layout(AdapterArgs& a, uint8_t* ws) {
   };
   if (a.T > kAD_Few) {
     const size_t groups = (size_t)adapter_groups(a.T, a.n);
-    a.n_groups = reinterpret_cast<int32_t*>(take(4));
+    a.n_groups = reinterpret_cast<int32_t*>(take(8));
     a.groups = reinterpret_cast<int4*>(take(groups * sizeof(int4)));
     a.arrived = reinterpret_cast<int32_t*>(take(groups * 4));
     a.perm = reinterpret_cast<int32_t*>(take((size_t)a.T * 4));
     a.back = reinterpret_cast<float*>(take((size_t)a.T * 4));
     a.parts = take((size_t)a.T * 2 * a.rmax * 2);
+    a.h = reinterpret_cast<float*>(take((size_t)2 * kAD_Ctas * kAD_Group * (a.rmax <= 32 ? 32 : a.rmax <= 64 ? 64 : 128) * 4));
+  } else {
+    a.h = reinterpret_cast<float*>(take((size_t)a.splits * a.T * a.rmax * 4));
   }
-  a.h = reinterpret_cast<float*>(take((size_t)a.splits * a.T * a.rmax * 4));
   return at;
 }
 
-template <typename T, int RM, int ST>
-static int launch_shrink(const AdapterArgs& a, unsigned groups, cudaStream_t stream) {
-  constexpr int smem = (kAD_Group + RM) * 128 * ST + 1024;
-  const int rc = ensure_smem_attr((const void*)adapter_shrink_kernel<T, RM, ST>, smem);
-  return rc ? rc : launch_early(adapter_shrink_kernel<T, RM, ST>, dim3(groups, a.splits), 256, smem, stream, a);
+template <typename T, int RM>
+static int launch_shrink(const AdapterArgs& a, cudaStream_t stream) {
+  const int rc = ensure_smem_attr((const void*)adapter_shrink_kernel<T, RM>, ShrinkCfg<RM>::Smem);
+  return rc ? rc : launch_early(adapter_shrink_kernel<T, RM>, dim3(kAD_Ctas), 416, ShrinkCfg<RM>::Smem, stream, a);
 }
 
 template <typename T, int RM>
@@ -860,11 +915,9 @@ static int launch_adapters(AdapterArgs a, int sms, cudaStream_t stream) {
     a.units = (blocks + cut - 1) / cut;
     return launch_early(adapter_expand_few_kernel<T>, dim3(a.T, (blocks + a.units - 1) / a.units), 256, 0, stream, a);
   }
-  const unsigned groups = (unsigned)adapter_groups(a.T, a.n);
   if ((rc = ensure_smem_attr((const void*)adapter_route_kernel, 2 * (kAD_MaxAdapters + 2) * 4 + kAD_RouteIds))) return rc;
   if ((rc = launch_early(adapter_route_kernel, dim3(1), 1024, (size_t)(2 * (a.n + 2)) * 4 + kAD_RouteIds, stream, a))) return rc;
-  rc = a.rmax <= 32 ? launch_shrink<T, 32, 5>(a, groups, stream)
-       : a.rmax <= 64 ? launch_shrink<T, 64, 4>(a, groups, stream) : launch_shrink<T, 128, 3>(a, groups, stream);
+  rc = a.rmax <= 32 ? launch_shrink<T, 32>(a, stream) : a.rmax <= 64 ? launch_shrink<T, 64>(a, stream) : launch_shrink<T, 128>(a, stream);
   if (rc) return rc;
   return a.rmax <= 64 ? launch_expand<T, 64>(a, sms, stream) : launch_expand<T, 128>(a, sms, stream);
 }
@@ -877,10 +930,8 @@ extern "C" {
 
 size_t bf_adapter_workspace(int T, int n, int d_in, int rmax) {
   if (T <= 0 || n <= 0 || n > kAD_MaxAdapters || d_in <= 0 || rmax <= 0 || rmax > kAD_MaxRank) return 0;
-  int splits, kper;
-  adapter_split(T, d_in, &splits, &kper);
   AdapterArgs a{};
-  a.T = T; a.n = n; a.rmax = rmax; a.splits = splits;
+  a.T = T; a.n = n; a.rmax = rmax; a.splits = (d_in + kAD_KFew - 1) / kAD_KFew;
   return adapter_layout(a, nullptr);
 }
 
@@ -906,7 +957,7 @@ int bf_adapter_add(const void* x, long long x_st, const int32_t* ids, int T, int
   a.A = A; a.B = B;
   a.err = st.err;
   a.n = n; a.T = T; a.d_in = d_in; a.d_out = d_out; a.rmax = rmax;
-  adapter_split(T, d_in, &a.splits, &a.kper);
+  a.splits = (d_in + kAD_KFew - 1) / kAD_KFew;
   adapter_layout(a, static_cast<uint8_t*>(ws));
   return dtype == BF_BF16 ? launch_adapters<__nv_bfloat16>(a, st.sm_count, stream) : launch_adapters<__half>(a, st.sm_count, stream);
 }
