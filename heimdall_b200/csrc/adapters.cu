@@ -155,7 +155,6 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   int* s_grp = s_dyn + a.n + 2;       // [n + 2] first group
   uint16_t* s_id = reinterpret_cast<uint16_t*>(s_dyn + 2 * (a.n + 2));
   __shared__ int2 s_warp[32];
-  __shared__ int s_base[1024];
   wait_for_stream();
   let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, buckets = a.n + 1;
@@ -166,14 +165,25 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   auto load = [&](int t0) {
     const int n = min(a.T - t0, 1024 * per);
     __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += 8192) {
-      int v[8];
+    auto put = [&](int i, int id) { s_id[(i >> per_log) * (kAD_RoutePer + 2) + (i & (per - 1))] = (uint16_t)adapter_of(a, id); };
+    const int head = min(n, (int)(-(reinterpret_cast<uintptr_t>(a.ids + t0) >> 2) & 3)), quads = (n - head) / 4;      // to a 16-byte boundary
+    if (tid < head) put(tid, a.ids[t0 + tid]);
+    if (tid < n - head - 4 * quads) put(head + 4 * quads + tid, a.ids[t0 + head + 4 * quads + tid]);
+    const int4* from = reinterpret_cast<const int4*>(a.ids + t0 + head);
+    for (int i0 = 0; i0 < quads; i0 += 8192) {
+      int4 v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = i0 + k * 1024 + tid < n ? __ldg(a.ids + t0 + i0 + k * 1024 + tid) : -1;
+      for (int k = 0; k < 8; ++k)
+        if (i0 + k * 1024 + tid < quads) v[k] = __ldg(from + i0 + k * 1024 + tid);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int i = i0 + k * 1024 + tid;
-        if (i < n) s_id[(i >> per_log) * (kAD_RoutePer + 2) + (i & (per - 1))] = (uint16_t)adapter_of(a, v[k]);
+        if (i < quads) {
+          put(head + 4 * i, v[k].x);
+          put(head + 4 * i + 1, v[k].y);
+          put(head + 4 * i + 2, v[k].z);
+          put(head + 4 * i + 3, v[k].w);
+        }
       }
     }
     __syncthreads();
@@ -184,7 +194,14 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     n = max(0, min(per, a.T - t0 - tid * per));
     const int first = n > 0 ? mine_id[0] : -1, of_warp = __shfl_sync(0xffffffffu, first, 0);
     bool same = n > 0 && first == of_warp;
-    for (int i = 1; i < n; ++i) same = same && mine_id[i] == first;
+    if (n == kAD_RoutePer) {
+      uint32_t differ = 0;             // two at a time
+#pragma unroll
+      for (int i = 0; i < kAD_RoutePer / 2; ++i) differ |= reinterpret_cast<const uint32_t*>(mine_id)[i] ^ ((uint32_t)first * 0x10001u);
+      same = same && differ == 0;
+    } else {
+      for (int i = 1; i < n; ++i) same = same && mine_id[i] == first;
+    }
     return __all_sync(0xffffffffu, same) ? of_warp : -1;
   };
   auto warp_total = [&](int n) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)n); };
@@ -260,11 +277,20 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     if (a.T > 1024 * per) load(t0);
     int n;
     const int one = whole(t0, n);
-    int base = -1;
     if (one >= 0) {
-      const int sum = warp_total(n);
+      // the warp's tokens follow one another, and so do their places: four at a time, from a 16-byte boundary on
+      const int sum = warp_total(n), t = t0 + 32 * warp * per;
+      int base = 0;
       if (lane == 0) base = atomicAdd(&s_at[one], sum);
-      base = __shfl_sync(0xffffffffu, base, 0) + lane * per;      // only the last lane with tokens can have fewer
+      base = __shfl_sync(0xffffffffu, base, 0);
+      int* to = a.perm + base;
+      const int head = min(sum, -base & 3), quads = (sum - head) / 4, rest = sum - head - 4 * quads;
+      if (lane < head) to[lane] = t + lane;
+      if (lane < rest) to[head + 4 * quads + lane] = t + head + 4 * quads + lane;
+      for (int q = lane; q < quads; q += 32) {
+        const int x = t + head + 4 * q;
+        *reinterpret_cast<int4*>(to + head + 4 * q) = make_int4(x, x + 1, x + 2, x + 3);
+      }
     } else {
       const int first = t0 + tid * per;
       for (int i = 0, begin = 0; i < n; ++i) {
@@ -274,13 +300,6 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
           begin = i + 1;
         }
       }
-    }
-    s_base[tid] = base;
-    __syncthreads();
-    // the tokens of whole warps, in their order
-    for (int i = tid; i < min(a.T - t0, 1024 * per); i += 1024) {
-      const int to = s_base[i >> per_log];
-      if (to >= 0) a.perm[to + (i & (per - 1))] = t0 + i;
     }
   }
 }
