@@ -52,7 +52,9 @@ class Adapters:
         with torch.no_grad():
             for x, y, r, lo, hi in zip(a, b, ranks, rows, rows[1:]):
                 self.a[lo:lo + r] = x
-                self.b[lo * d_out:hi * d_out].view(d_out, hi - lo)[:, :r] = y
+                part = torch.zeros(d_out, hi - lo, dtype=dtype, device=dev)       # in blocks of 8 columns and 8 ranks, as the tensor core reads them
+                part[:, :r] = y
+                self.b[lo * d_out:hi * d_out] = part.view(d_out // 8, 8, -1, 8).transpose(1, 2).reshape(-1)
         self.device = self.a.device
         self.rows = torch.tensor(rows, dtype=torch.int32, device=dev)
         self.scale = torch.tensor(scale, dtype=torch.float32, device=dev)

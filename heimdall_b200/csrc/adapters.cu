@@ -35,14 +35,14 @@ struct AdapterArgs {
   const int32_t* ids;
   const int32_t* row;              // [n + 1] the adapters' first rows in A, multiples of 16
   const float* scale;              // [n]
-  const void *A, *B;               // A [row[n]][d_in]; B: adapter a's [d_out][r_a] from element row[a] d_out on
+  const void *A, *B;               // A [row[n]][d_in]; B: adapter a's [d_out / 8][r_a / 8][8 columns][8 ranks] from element row[a] d_out on
   int n, T, d_in, d_out, rmax, splits, units;
   unsigned int* err;
   float* h;                        // few tokens: [splits][T][rmax]; many: two places per CTA of [kAD_Group][rmax rounded up to 32, 64, 128]
-  void* parts;                     // [T][2][rmax] h's two parts, by place in perm
-  float* back;                     // [T] the scale that undoes theirs, times the adapter's
+  void* parts;                     // h's two parts: a group's from its first place times 2 rmax on, [2][tokens / 8][r / 8][8 tokens][8 ranks]
+  float* back;                     // by place: the scale that undoes theirs, times the adapter's
   int32_t* arrived;                // [groups] parts of h that are done
-  int32_t* perm;                   // [T] tokens by adapter
+  int32_t* perm;                   // tokens by adapter, each adapter's from a multiple of 8 places on
   int4* groups;                    // (adapter or n, first of perm, tokens, -)
   int32_t* n_groups;               // all that out needs, and those of adapters
 };
@@ -151,14 +151,15 @@ constexpr int kAD_RoutePer = 32;                                        // token
 constexpr int kAD_RouteIds = 1024 * (kAD_RoutePer + 2) * 2;              // bytes of their adapters' numbers, two more per thread against bank conflicts
 __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   extern __shared__ int s_dyn[];
-  int* s_at = s_dyn;                  // [n + 2] count, then first place in perm of each adapter (n: none)
-  int* s_grp = s_dyn + a.n + 2;       // [n + 2] first group
-  uint16_t* s_id = reinterpret_cast<uint16_t*>(s_dyn + 2 * (a.n + 2));
+  int* s_count = s_dyn;               // [n + 2] tokens of each adapter (n: none)
+  int* s_at = s_count + a.n + 2;      // first place in perm
+  int* s_grp = s_at + a.n + 2;        // first group
+  uint16_t* s_id = reinterpret_cast<uint16_t*>(s_grp + a.n + 2);
   __shared__ int2 s_warp[32];
   wait_for_stream();
   let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, buckets = a.n + 1;
-  for (int i = tid; i < buckets + 1; i += 1024) s_at[i] = 0;
+  for (int i = tid; i < buckets; i += 1024) s_count[i] = 0;
   int per_log = 0;                    // a power of two of tokens per thread: no divisions
   while (per_log < 5 && (1024 << per_log) < a.T) ++per_log;
   const int per = 1 << per_log;
@@ -211,11 +212,11 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     const int one = whole(t0, n);
     if (one >= 0) {
       const int sum = warp_total(n);
-      if (lane == 0) atomicAdd(&s_at[one], sum);
+      if (lane == 0) atomicAdd(&s_count[one], sum);
     } else {
       for (int i = 0, begin = 0; i < n; ++i) {
         if (i + 1 == n || mine_id[i + 1] != mine_id[i]) {
-          atomicAdd(&s_at[mine_id[i]], i + 1 - begin);
+          atomicAdd(&s_count[mine_id[i]], i + 1 - begin);
           begin = i + 1;
         }
       }
@@ -226,8 +227,8 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   const int each = (buckets + 1023) / 1024, lo = min(tid * each, buckets), hi = min(lo + each, buckets);
   int2 mine = make_int2(0, 0);
   for (int b = lo; b < hi; ++b) {
-    mine.x += s_at[b];
-    mine.y += (s_at[b] + kAD_Group - 1) / kAD_Group;
+    mine.x += (s_count[b] + 7) & ~7;
+    mine.y += (s_count[b] + kAD_Group - 1) / kAD_Group;
   }
   int2 incl = mine;
 #pragma unroll
@@ -246,16 +247,12 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     at.y += s_warp[w].y;
   }
   for (int b = lo; b < hi; ++b) {
-    const int n = s_at[b];
     s_at[b] = at.x;
     s_grp[b] = at.y;
-    at.x += n;
-    at.y += (n + kAD_Group - 1) / kAD_Group;
+    at.x += (s_count[b] + 7) & ~7;
+    at.y += (s_count[b] + kAD_Group - 1) / kAD_Group;
   }
-  if (lo < hi && hi == buckets) {
-    s_at[buckets] = at.x;
-    s_grp[buckets] = at.y;
-  }
+  if (lo < hi && hi == buckets) s_grp[buckets] = at.y;
   __syncthreads();
   const int total = s_grp[buckets];
   for (int k = tid; k < total; k += 1024) {
@@ -264,8 +261,8 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
       const int mid = (b + e) >> 1;
       if (s_grp[mid] <= k) b = mid; else e = mid;
     }
-    const int first = s_at[b] + (k - s_grp[b]) * kAD_Group;
-    a.groups[k] = make_int4(b, first, min(kAD_Group, s_at[b + 1] - first), 0);
+    const int skip = (k - s_grp[b]) * kAD_Group;
+    a.groups[k] = make_int4(b, s_at[b] + skip, min(kAD_Group, s_count[b] - skip), 0);
     a.arrived[k] = 0;
   }
   if (tid == 0) {
@@ -308,7 +305,7 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
 // through a ring in shared memory (K-major, 128-byte swizzle; eight warps copy); a thread issues the products, D in TMEM (two of them) is the group's h.  A run
 // that has part of a group leaves its sums in one of the CTA's two places (its first group, begun by others; its last, ended by others); the CTA that is the
 // last to bring a group's part adds them all, in their order, and makes the two parts.  (A grid of groups and parts of d_in, two CTAs per SM: 25480 tokens of
-// 6144 took 92 us, 8192 of 5120 37, against XX and XX.)
+// 6144 took 92 us, 8192 of 5120 37, against 69 and 32.)
 constexpr int kAD_Ctas = 148, kAD_Step = 128, kAD_MinSteps = 8;
 template <int RM>
 struct ShrinkCfg {
@@ -498,7 +495,8 @@ __global__ void __launch_bounds__(416, 1) adapter_shrink_kernel(AdapterArgs a) {
       const int ex = big > 0.f && big < INFINITY ? min(max((int)(__float_as_uint(big) >> 23), 14), 253) : 140;
       const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
       if (r < m) {
-        T* to = static_cast<T*>(a.parts) + (size_t)(grp.y + r) * 2 * a.rmax;
+        T* to = static_cast<T*>(a.parts) + (size_t)grp.y * 2 * a.rmax + (r >> 3) * 8 * rank + (r & 7) * 8;
+        const int other = ((m + 7) & ~7) * rank;
 #pragma unroll
         for (int c = 0; c < RM; c += 8)
           if (c < rank) {
@@ -510,8 +508,8 @@ __global__ void __launch_bounds__(416, 1) adapter_shrink_kernel(AdapterArgs a) {
               hi[i] = (T)x;
               lo[i] = (T)(x - (float)hi[i]);
             }
-            *reinterpret_cast<uint4*>(to + c) = h;
-            *reinterpret_cast<uint4*>(to + a.rmax + c) = l;
+            *reinterpret_cast<uint4*>(to + 8 * c) = h;
+            *reinterpret_cast<uint4*>(to + other + 8 * c) = l;
           }
         a.back[grp.y + r] = scale * __uint_as_float((uint32_t)(ex - 13) << 23);
       }
@@ -533,37 +531,43 @@ template <typename T, int M>       // M: 1 or 4 tokens at most
 __device__ __forceinline__ void expand_few(const AdapterArgs& a, const T* w, int rank, int m, const int* s_tok, const float* s_h, float scale, int col0,
                                            int units) {
   const int lane = threadIdx.x & 31;
-  uint32_t y[M], y_next[M];
+  T y[M][2], y_next[M][2];
   uint4 b[4];
   const uint4 *p, *q;
-  auto begin = [&](int u) {        // unit u's y and first 16 ranks
-    const int col = col0 + 512 * u + 2 * lane;
+  // unit u's y and first 16 ranks
+  auto begin = [&](int u) {
+    const int col = col0 + 512 * u + lane;
     if (u >= units || col >= a.d_out) return;
+    const bool two = col + 32 < a.d_out;
 #pragma unroll
     for (int t = 0; t < M; ++t)
-      if (t < m) y_next[t] = __ldcs(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.y) + (long long)s_tok[t] * a.y_st + col));
-    p = reinterpret_cast<const uint4*>(w + (long long)col * rank);
-    q = reinterpret_cast<const uint4*>(w + (long long)(col + 1) * rank);
-    b[0] = __ldg(p), b[1] = __ldg(p + 1), b[2] = __ldg(q), b[3] = __ldg(q + 1);
+      if (t < m) {
+        const T* from = static_cast<const T*>(a.y) + (long long)s_tok[t] * a.y_st + col;
+        y_next[t][0] = from[0];
+        if (two) y_next[t][1] = from[32];
+      }
+    p = reinterpret_cast<const uint4*>(w + (long long)(col >> 3) * 8 * rank + (col & 7) * 8);
+    q = two ? p + 4 * rank : p;
+    b[0] = __ldg(p), b[1] = __ldg(p + 8), b[2] = __ldg(q), b[3] = __ldg(q + 8);
   };
   begin(0);
 #pragma unroll 1
   for (int u = 0; u < units; ++u) {
-    const int col = col0 + 512 * u + 2 * lane;
+    const int col = col0 + 512 * u + lane;
     if (col >= a.d_out) return;
     uint64_t acc[M][2];
 #pragma unroll
     for (int t = 0; t < M; ++t) {
       acc[t][0] = acc[t][1] = 0;
-      y[t] = y_next[t];
+      y[t][0] = y_next[t][0], y[t][1] = y_next[t][1];
     }
 #pragma unroll 1
     for (int r = 0; r < rank; r += 16) {
       uint4 now[4] = {b[0], b[1], b[2], b[3]};
       if (r + 16 < rank) {
-        p += 2;
-        q += 2;
-        b[0] = __ldg(p), b[1] = __ldg(p + 1), b[2] = __ldg(q), b[3] = __ldg(q + 1);
+        p += 16;
+        q += 16;
+        b[0] = __ldg(p), b[1] = __ldg(p + 8), b[2] = __ldg(q), b[3] = __ldg(q + 8);
       } else {
         begin(u + 1);
       }
@@ -591,10 +595,10 @@ __device__ __forceinline__ void expand_few(const AdapterArgs& a, const T* w, int
 #pragma unroll
     for (int t = 0; t < M; ++t) {
       if (t < m) {
-        T* e = reinterpret_cast<T*>(&y[t]);
+        T* to = static_cast<T*>(a.out) + (long long)s_tok[t] * a.o_st + col;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) e[k] = (T)fmaf(lo_hi(acc[t][k], 0) + lo_hi(acc[t][k], 1), scale, (float)e[k]);
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (long long)s_tok[t] * a.o_st + col) = y[t];
+        for (int k = 0; k < 2; ++k)
+          if (k == 0 || col + 32 < a.d_out) to[32 * k] = (T)fmaf(lo_hi(acc[t][k], 0) + lo_hi(acc[t][k], 1), scale, (float)y[t][k]);
       }
     }
   }
@@ -626,12 +630,6 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
   const int r0 = a.row[id], rank = a.row[id + 1] - r0;
   const float scale = a.scale[id];
   const T* w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
-  // the CTA's weights on their way to L2
-  for (int u = 0; u < a.units; ++u) {
-    const int col = col0 + 512 * u + 2 * lane;
-    if (col < a.d_out)
-      for (int r = 0; r < 2 * rank; r += 64) prefetch_l2(w + (long long)col * rank + r);
-  }
   wait_for_stream();
   for (int i = tid; i < m * rank; i += 256) {
     const int t = i / rank, r = i - t * rank;
@@ -648,13 +646,18 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
 }
 
 // out of many tokens: tiles of a group (128 tokens) and 128 columns, group by group, an equal run of them to each SM's one CTA.  Four warps bring y's rows into
-// a ring of shared memory (256 bytes a copy), two bring B's rows (N operand, K-major) and, when the group changes, h's two parts (M operand), a thread issues
+// a ring of shared memory (256 bytes a copy), one
+// thread B's columns (N operand) and, when the group changes, h's two parts (M operand), both of which lie in memory as the products read them; a thread issues
 // the products, and eight warps add D (TMEM, two of them) to y where it lies and send the rows out; a thread has half a row.
 // HBM under reads and writes at once wants about 130 KB of reads in flight per SM, whatever the products do (a bare copy of 8192 x 12288 by
-// such tiles: 72 us with four tiles of y on their way, 106 to 112 with two or three).  So y goes through shared memory: 85 us for those sizes and ranks up to 64,
-// against 106 with y in registers, two or three CTAs to an SM.  A warp issues a copy of its own bytes about every 70 cycles: one warp for all rows
-// took 198 us, and rows going out by such copies too 206.
+// such tiles: 72 us with four tiles of y on their way, 106 to 112 with two or three).  So y goes through shared memory: 68 us for those sizes and ranks up to 64,
+// against 106 with y in registers, two or three CTAs to an SM, and 85 with B and h gathered and swizzled by threads (cp.async) in the place of one copy a tile.  A warp issues a copy of its own bytes about every 70 cycles: one warp for all rows
+// of y took 198 us.
 constexpr int kAD_Tile = 128, kAD_Pitch = 272;      // bytes from row to row of y in shared memory: no two of eight neighbouring rows in the same banks
+// an operand [rows / 8][steps][2][8 rows][8 values]: blocks of 8 rows of 16 bytes, 128 bytes from block to block along K, 256 steps bytes along the rows
+__device__ __forceinline__ uint64_t sdesc_core(uint32_t addr, int steps) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(16 * steps) << 32 | 1ull << 46;
+}
 template <typename T, int RM>
 struct ExpandCfg {
   static constexpr int Atoms = RM <= 64 ? 1 : 2, Ring = RM <= 64 ? 4 : 2;       // of 64 ranks; tiles of y
@@ -663,13 +666,13 @@ struct ExpandCfg {
 };
 
 template <typename T, int RM>
-__global__ void __launch_bounds__(480, 1) adapter_expand_kernel(AdapterArgs a) {
+__global__ void __launch_bounds__(448, 1) adapter_expand_kernel(AdapterArgs a) {
   using C = ExpandCfg<T, RM>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* s_h = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_y = s_h + C::HBytes + 2 * C::BBytes;
   const uint32_t hs = smem_u32(s_h), bs = hs + C::HBytes;
-  // full: bytes of y; 64 threads' copies of B (and h); the products.  free: eight warps' stores; the products; eight warps' reads of D
+  // full: bytes of y; bytes of B (and h); the products.  free: eight warps' stores; the products; eight warps' reads of D
   __shared__ uint64_t y_full[C::Ring], y_free[C::Ring], b_full[2], b_free[2], d_full[2], d_free[2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
@@ -682,7 +685,7 @@ __global__ void __launch_bounds__(480, 1) adapter_expand_kernel(AdapterArgs a) {
       mbar_init(y_free + i, 8);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(b_full + i, 64);
+      mbar_init(b_full + i, 1);
       mbar_init(b_free + i, 1);
       mbar_init(d_full + i, 1);
       mbar_init(d_free + i, 8);
@@ -718,73 +721,51 @@ __global__ void __launch_bounds__(480, 1) adapter_expand_kernel(AdapterArgs a) {
         ++g;
       }
     }
-  } else if (warp < 6) {
+  } else if (warp == 4) {
     wait_for_stream();
-    const int t = tid - 128, half = t & 1, row0 = t >> 1;      // two threads to a row, each every second piece of 16 bytes
     const T* w = nullptr;
     int rank = 0;
 #pragma unroll 1
     for (int j = 0, g = g0, c = c0; j < n; ++j) {
-      bool sent = j == 0;          // tile j - 1 has been handed on
-      auto send = [&]() {
-        fence_async_smem();
-        mbar_arrive(b_full + ((j - 1) & 1));
-        sent = true;
-      };
+      int rows = 0;                  // of h
+      const T* h = nullptr;
       if (j == 0 || c == 0) {
         const int4 grp = a.groups[g];
         const int r0 = grp.x < a.n ? a.row[grp.x] : 0;
         rank = grp.x < a.n ? a.row[grp.x + 1] - r0 : 0;
         w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
-        if (!sent) {               // h is in use until the products of tile j - 1 are done
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-          send();
-          if (!(ok = mbar_wait_small(b_free + ((j - 1) & 1), (j - 1) >> 1 & 1, abort, 0x83))) break;
+        h = static_cast<const T*>(a.parts) + (size_t)grp.y * 2 * a.rmax;
+        rows = (grp.z + 7) & ~7;     // (rows that are not there are left as they were: nobody reads their sums)
+        // h is in use until the products of tile j - 1 are done
+        if (j > 0 && !mbar_wait_warp_small(b_free + ((j - 1) & 1), (j - 1) >> 1 & 1, abort, 0x83)) break;
+      }
+      if (!mbar_wait_warp_small(b_free + (j & 1), (j >> 1 & 1) ^ 1, abort, 0x84)) break;
+      if (lane == 0) {
+        const uint32_t bytes = 2 * rank * min(kAD_Tile, a.d_out - c * kAD_Tile), part = 2 * rank * rows;
+        mbar_expect_tx(b_full + (j & 1), bytes + 2 * part);
+        if (bytes) bulk_load_1d(s_h + C::HBytes + (j & 1) * C::BBytes, w + (long long)c * kAD_Tile * rank, bytes, b_full + (j & 1));
+        if (part) {
+          bulk_load_1d(s_h, h, part, b_full + (j & 1));
+          bulk_load_1d(s_h + C::HBytes / 2, h + rows * rank, part, b_full + (j & 1));
         }
-        for (int r = row0; r < kAD_Group; r += 32) {
-          // rows that are not there repeat the last one, nobody reads their sums
-          const T* src = static_cast<const T*>(a.parts) + (size_t)(grp.y + min(r, grp.z - 1)) * 2 * a.rmax;
-          for (int p = half; p < rank / 8; p += 2)
-#pragma unroll
-            for (int part = 0; part < 2; ++part)
-              copy16(hs + r * 128 + part * (C::HBytes / 2) + (p >> 3) * (kAD_Group * 128) + (((p & 7) ^ (r & 7)) << 4), src + part * a.rmax + 8 * p, true);
-        }
       }
-      if (!(ok = mbar_wait_small(b_free + (j & 1), (j >> 1 & 1) ^ 1, abort, 0x84))) break;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = row0 + 32 * i, col = c * kAD_Tile + r;
-        const bool in = col < a.d_out;
-        const T* src = w + (long long)(in ? col : 0) * rank;
-        const uint32_t dst = bs + (j & 1) * C::BBytes + r * 128;
-        for (int p = half; p < rank / 8; p += 2) copy16(dst + (p >> 3) * (kAD_Tile * 128) + (((p & 7) ^ (r & 7)) << 4), src + 8 * p, in);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (!sent) {
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        send();
-      }
+      __syncwarp();
       if (++c == tpg) {
         c = 0;
         ++g;
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    if (ok && n) {
-      fence_async_smem();
-      mbar_arrive(b_full + ((n - 1) & 1));
-    }
   } else {
     wait_for_stream();
-    if (warp == 6) {
+    if (warp == 5) {
       tmem_alloc(&s_tmem, 2 * kAD_Tile);
       tmem_relinquish();
     }
     tc_fence_before();
-    asm volatile("bar.sync 1, 288;" ::: "memory");       // warps 6 to 14
+    asm volatile("bar.sync 1, 288;" ::: "memory");       // warps 5 to 13
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    if (warp == 6) {
+    if (warp == 5) {
       const uint32_t idesc = idesc_f16(128, kAD_Tile, kIsBf16<T>);
       int steps = 0;
 #pragma unroll 1
@@ -802,8 +783,7 @@ __global__ void __launch_bounds__(480, 1) adapter_expand_kernel(AdapterArgs a) {
           for (int part = 0; part < 2; ++part)
 #pragma unroll 1
             for (int ks = 0; ks < steps; ++ks) {
-              const uint32_t k = (ks >> 2) * (128 * 128) + (ks & 3) * 32;      // both operands have 128 rows
-              umma_f16_ss(d, sdesc_sw128(hs + part * (C::HBytes / 2) + k), sdesc_sw128(b + k), idesc, part > 0 || ks > 0);
+              umma_f16_ss(d, sdesc_core(hs + part * (C::HBytes / 2) + 256 * ks, steps), sdesc_core(b + 256 * ks, steps), idesc, part > 0 || ks > 0);
             }
           umma_commit(b_free + (j & 1));
           umma_commit(d_full + (j & 1));
@@ -815,7 +795,7 @@ __global__ void __launch_bounds__(480, 1) adapter_expand_kernel(AdapterArgs a) {
         }
       }
     } else {
-      const int row0 = 32 * (warp & 3), r = row0 + lane, at = 64 * ((warp - 7) >> 2);
+      const int row0 = 32 * (warp & 3), r = row0 + lane, at = 64 * ((warp - 6) >> 2);
       const uint8_t* from = s_y + (row0 + (lane >> 3)) * kAD_Pitch + 2 * at + 16 * (lane & 7);      // eight lanes write a row
       T* out = nullptr;
       float scale = 0.f;
@@ -879,7 +859,7 @@ __global__ void __launch_bounds__(480, 1) adapter_expand_kernel(AdapterArgs a) {
   tc_fence_before();
   __syncthreads();
   if (tid == 0) report_abort(abort, a.err);
-  if (warp == 6) {
+  if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(s_tmem, 2 * kAD_Tile);
   }
@@ -900,9 +880,10 @@ static size_t adapter_layout(AdapterArgs& a, uint8_t* ws) {
     a.n_groups = reinterpret_cast<int32_t*>(take(8));
     a.groups = reinterpret_cast<int4*>(take(groups * sizeof(int4)));
     a.arrived = reinterpret_cast<int32_t*>(take(groups * 4));
-    a.perm = reinterpret_cast<int32_t*>(take((size_t)a.T * 4));
-    a.back = reinterpret_cast<float*>(take((size_t)a.T * 4));
-    a.parts = take((size_t)a.T * 2 * a.rmax * 2);
+    const size_t places = (size_t)a.T + 7 * (size_t)(a.n + 1 < a.T ? a.n + 1 : a.T) + 8;
+    a.perm = reinterpret_cast<int32_t*>(take(places * 4));
+    a.back = reinterpret_cast<float*>(take(places * 4));
+    a.parts = take(places * 2 * a.rmax * 2);
     a.h = reinterpret_cast<float*>(take((size_t)2 * kAD_Ctas * kAD_Group * (a.rmax <= 32 ? 32 : a.rmax <= 64 ? 64 : 128) * 4));
   } else {
     a.h = reinterpret_cast<float*>(take((size_t)a.splits * a.T * a.rmax * 4));
@@ -920,7 +901,7 @@ template <typename T, int RM>
 static int launch_expand(const AdapterArgs& a, int sms, cudaStream_t stream) {
   using C = ExpandCfg<T, RM>;
   const int rc = ensure_smem_attr((const void*)adapter_expand_kernel<T, RM>, C::Smem);
-  return rc ? rc : launch_early(adapter_expand_kernel<T, RM>, dim3(sms), 480, C::Smem, stream, a);
+  return rc ? rc : launch_early(adapter_expand_kernel<T, RM>, dim3(sms), 448, C::Smem, stream, a);
 }
 
 template <typename T>
@@ -934,8 +915,8 @@ static int launch_adapters(AdapterArgs a, int sms, cudaStream_t stream) {
     a.units = (blocks + cut - 1) / cut;
     return launch_early(adapter_expand_few_kernel<T>, dim3(a.T, (blocks + a.units - 1) / a.units), 256, 0, stream, a);
   }
-  if ((rc = ensure_smem_attr((const void*)adapter_route_kernel, 2 * (kAD_MaxAdapters + 2) * 4 + kAD_RouteIds))) return rc;
-  if ((rc = launch_early(adapter_route_kernel, dim3(1), 1024, (size_t)(2 * (a.n + 2)) * 4 + kAD_RouteIds, stream, a))) return rc;
+  if ((rc = ensure_smem_attr((const void*)adapter_route_kernel, 3 * (kAD_MaxAdapters + 2) * 4 + kAD_RouteIds))) return rc;
+  if ((rc = launch_early(adapter_route_kernel, dim3(1), 1024, (size_t)(3 * (a.n + 2)) * 4 + kAD_RouteIds, stream, a))) return rc;
   rc = a.rmax <= 32 ? launch_shrink<T, 32>(a, stream) : a.rmax <= 64 ? launch_shrink<T, 64>(a, stream) : launch_shrink<T, 128>(a, stream);
   if (rc) return rc;
   return a.rmax <= 64 ? launch_expand<T, 64>(a, sms, stream) : launch_expand<T, 128>(a, sms, stream);

@@ -279,7 +279,7 @@ int bf_norm_rope(const void* qg, long long q_sb, long long q_st, long long q_sh,
  *   out_t = y_t + scale[a] B_a (A_a x_t), a = ids[t]; out_t = y_t where ids[t] is outside [0, n).
  *   x [T,d_in], y, out [T,d_out] dtype BF_BF16 or BF_F16 with row strides in elements (multiples of 8; out may be y); ids [T] int32; row [n + 1]
  *   int32: adapter a has the rows row[a] .. row[a + 1] - 1 of A [row[n],d_in], its rank, a multiple of 16 (zeros where its own is not) of at
- *   most rmax; its B_a [d_out, rank] begins at element row[a] d_out of B; scale [n] fp32.  All on the device.
+ *   most rmax; its B_a, as [d_out / 8][rank / 8][8 columns][8 ranks], begins at element row[a] d_out of B; scale [n] fp32.  All on the device.
  * A x is summed in fp32 and enters the second product as two parts of dtype (2^-16 of itself in BF_BF16, 2^-22 in BF_F16); out is rounded once.  A token whose
  * A x is not finite gets NaN.  d_in and d_out multiples of 8, rmax a multiple of 16 of at most 128, n at most 4096, T at most 2^28.
  * Workspace: bf_adapter_workspace().
