@@ -180,8 +180,7 @@ __global__ void __launch_bounds__(256) paged_queries_kernel(SharedArgs a) {
   if (lane == 0) a.qs[at] = fin ? __uint_as_float((uint32_t)(ex - 7) << 23) * a.c2 : NAN;
 }
 
-// Barriers and the abort word by their addresses in shared memory: through pointers every one of the many uses makes its address anew, in a kernel whose
-// warps wait for their instructions as it is (87 -> XX us for 16 x 131072 shared tokens).
+// Barriers and the abort word by their addresses in shared memory: through pointers every one of the many uses makes its address anew.
 struct Bar {
   uint32_t at;
   __device__ __forceinline__ Bar operator+(int i) const { return Bar{at + 8u * i}; }
@@ -250,13 +249,13 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(sQ + SharedSmem<T>::Q);
   const Bar k_full{smem_u32(bars)}, k_empty = k_full + 4, v_full = k_full + 8, v_empty = k_full + 12, s_full = k_full + 16, p_full = k_full + 18,
             p_free = k_full + 20, o_free = k_full + 22, o_full = k_full + 24, q_full = k_full + 25, q_free = k_full + 26, t_full = k_full + 28,
-            t_free = k_full + 32;
+            t_free = k_full + 32, met = k_full + 60;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 36);
   volatile int* abort = reinterpret_cast<volatile int*>(bars + 37);
   const Waits wait{smem_u32(bars + 37)};
   const uint32_t ring_at = smem_u32(ring), q_at = smem_u32(sQ);
   int* s_sum = reinterpret_cast<int*>(bars + 38);      // [20][2] per-warp totals
-  int* s_start = reinterpret_cast<int*>(bars + 59);    // stretch, unit in it, rows before it
+  int* s_start = reinterpret_cast<int*>(bars + 58);    // stretch, unit in it, rows before it
   SharedTile* s_tile = reinterpret_cast<SharedTile*>(bars + 64);  // [4]
   float2* s_ml = reinterpret_cast<float2*>(s_tile + 4);           // [4][2][128] a tile's maxima and sums, of both halves of its tokens
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -278,6 +277,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
     o_full.init(1);
     q_full.init(1);
     q_free.init(1);
+    for (int i = 0; i < 4; ++i) (met + i).init(2);       // the two warps of softmax that have the same rows
     *abort = 0;
     fence_barrier_init();
   }
@@ -598,6 +598,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
       const int hh = (warp - 4) >> 2, c0 = 64 * hh;
       float qs = 0.f;
       int limit = -1, rows = 0, item = 0;            // the last position that the row sees
+      uint32_t meetings = 0;
 #pragma unroll 1
       for (int j = 0; tile(j); ++j) {
         const int s = j & 1;
@@ -671,7 +672,9 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
           // the row's maximum of both halves (the two warps of these rows meet)
           float2* ml = s_ml + (j & 3) * 2 * kSH_M + r;
           ml[hh * kSH_M].x = mt;
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + wq) : "memory");
+          __syncwarp();
+          if (lane == 0) (met + wq).arrive();
+          if (!(ok = wait(met + wq, meetings++ & 1, 0xa3))) break;
           mt = fmaxf(mt, ml[(hh ^ 1) * kSH_M].x);
           const float ref = 8.f - (mt == -INFINITY ? 0.f : mt);       // the largest weight becomes 2^8
           // 16 tokens at a time, the next 16 scores on their way; every step for all of them before the next one, a value's own way through the
