@@ -81,8 +81,9 @@ class Adapters:
                 # numbers above 31 bits name no adapter either
                 ids = ids.to(device=dev).clamp(-1, self.n).to(torch.int32).contiguous()
             T = ids.numel()
-            x, xp, xs = heads_16bit("x", x.reshape(T, self.d_in))
-            y2, yp, ys = heads_16bit("y", y.reshape(T, self.d_out))
+            flat = len(lead) == 1
+            x, xp, xs = heads_16bit("x", x if flat else x.reshape(T, self.d_in))
+            y2, yp, ys = heads_16bit("y", y if flat else y.reshape(T, self.d_out))
             if out is None:
                 out = y.new_empty(y.shape)
             elif (out.data_ptr() != yp or (T > 1 and ys[0] != self.d_out)) and _overlap(out, y2):

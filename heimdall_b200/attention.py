@@ -75,9 +75,17 @@ class BifrostAttention:
         y = F.linear(x, getattr(self, name + "_w"), getattr(self, name + "_b"))
         if ids is None or name not in self.adapters:
             return y
-        if ids.dim() == 1 and x.dim() == 3:
-            ids = ids[:, None].expand(x.shape[:2])
         return self.adapters[name].add(y, x, ids, out=y)
+
+    def _ids(self, x, ids):
+        """Adapter ids [B] or [B,t] as int32 [B,t], once for all projections (numbers above 31 bits name no adapter either)."""
+        if ids is None or not self.adapters:
+            return None
+        if ids.dim() == 1:
+            ids = ids[:, None].expand(x.shape[:2])
+        if ids.dtype == torch.int64:
+            ids = ids.clamp(-1, 2 ** 31 - 1)
+        return ids.to(device=x.device, dtype=torch.int32).contiguous() if ids.dtype in (torch.int32, torch.int64) else ids
 
     def project(self, x, start: int = 0, positions=None, adapter_ids=None):
         """``HybridAttention._proj`` (heimdall/hibrit.py:254-268): x [B,t,d] -> (q, k, v, qr, kr, qg) with q
@@ -89,10 +97,10 @@ class BifrostAttention:
         L = self.layer
         B, t = x.shape[:2]
         H, G, D = L.H, L.G, L.D
-        xb = x.to(torch.bfloat16)
-        qg = self._linear("q", xb, adapter_ids).contiguous()
-        kl = self._linear("k", xb, adapter_ids).contiguous()
-        v = self._linear("v", xb, adapter_ids).view(B, t, G, D)
+        xb, ids = x.to(torch.bfloat16), self._ids(x, adapter_ids)
+        qg = self._linear("q", xb, ids).contiguous()
+        kl = self._linear("k", xb, ids).contiguous()
+        v = self._linear("v", xb, ids).view(B, t, G, D)
         if positions is not None:
             q, k, qr, kr = norm_rope_heads(qg.view(B, t, H, -1), kl.view(B, t, G, D), self.q_norm_w, self.k_norm_w, positions,
                                            self.inv_freq if self.rot else None, self.axes if positions.dim() == 3 else None, self.eps,
@@ -116,7 +124,7 @@ class BifrostAttention:
         y = torch.empty(B, t, L.H * L.D, device=x.device, dtype=torch.bfloat16)
         _lib.call("bf_attn_epilogue", ptr(o.contiguous()), ptr(qg), 1 if self.gated else 0, B, t, L.H, L.D, ptr(y),
                   stream_handle())
-        return self._linear("o", y.view(B, t, L.H * L.D), adapter_ids)
+        return self._linear("o", y.view(B, t, L.H * L.D), self._ids(x, adapter_ids))
 
     def forward(self, x, cache=None, start: int = 0, positions=None, adapter_ids=None):
         """``HybridAttention.forward`` of a converted layer (heimdall/hibrit.py:426-432): x [B,t,d] -> [B,t,d] bf16,
