@@ -81,8 +81,10 @@ class BifrostAttention:
         """Adapter ids [B] or [B,t] as int32 [B,t], once for all projections (numbers above 31 bits name no adapter either)."""
         if ids is None or not self.adapters:
             return None
-        if ids.dim() == 1:
+        if ids.dim() == 1 and ids.shape[0] == x.shape[0]:
             ids = ids[:, None].expand(x.shape[:2])
+        if ids.shape != x.shape[:2]:
+            raise ValueError("adapter_ids must be [B] or [B,t]")
         if ids.dtype == torch.int64:
             ids = ids.clamp(-1, 2 ** 31 - 1)
         return ids.to(device=x.device, dtype=torch.int32).contiguous() if ids.dtype in (torch.int32, torch.int64) else ids

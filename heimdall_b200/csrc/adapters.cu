@@ -12,8 +12,7 @@
 //   * more: adapter_route_kernel sorts the tokens by adapter and lists groups of 128, one M = 128 tile of the tensor core (tcgen05).
 // h = A x is split over d_in so that every SM has work; each split's sums are written on their own and added in order.  For many tokens h enters the
 // second product as two 16-bit parts of its row's power-of-two scale (hi + lo, 16 bits of bf16, 22 of fp16), so that the only rounding of
-// consequence is that of out; for few it stays fp32.  The order of a group's tokens, which the sort leaves to chance, has no part in
-// their values.
+// consequence is that of out; for few it stays fp32.
 // (With mma.sync in the place of tcgen05 both kernels of many tokens were bound by its rate, about 32 cycles per m16n8k16 and scheduler:
 // 25480 tokens 6144 -> 5120, rank 64: 148 + 324 us.)
 #include "capi_internal.h"
@@ -144,93 +143,69 @@ __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(AdapterArgs a) 
   }
 }
 
-// The sorted list of many tokens and their groups, by one CTA.  The adapters' numbers go through shared memory, so that a thread can take
-// consecutive tokens, whose adapters come in runs, and count whole runs; a warp whose tokens are all of one adapter counts at once.  (With
-// each thread reading and writing its own tokens in global memory, 25480 tokens took 26 us.)
-constexpr int kAD_RoutePer = 32;                                        // tokens per thread at a time, at most
-constexpr int kAD_RouteIds = 1024 * (kAD_RoutePer + 2) * 2;              // bytes of their adapters' numbers, two more per thread against bank conflicts
-__global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
+// Many tokens: one CTA sorts them by adapter, in their order (a group's place among the others decides where its sums are cut, so a token's group must not
+// be left to chance), and lists the groups.  Each of up to 32 warps counts the adapters of a stretch of tokens, 32 at a time, in a row of its own; a running
+// sum over the rows then says where each warp's tokens of each adapter begin, and the warps go the same way again.
+constexpr int kAD_RouteWords = 55000;           // of shared memory
+static int adapter_route_warps(int n) { return min(32, (kAD_RouteWords - 3 * (n + 2)) / (n + 1)); }
+__global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a, int warps) {
   extern __shared__ int s_dyn[];
   int* s_count = s_dyn;               // [n + 2] tokens of each adapter (n: none)
   int* s_at = s_count + a.n + 2;      // first place in perm
   int* s_grp = s_at + a.n + 2;        // first group
-  uint16_t* s_id = reinterpret_cast<uint16_t*>(s_grp + a.n + 2);
+  int* s_row = s_grp + a.n + 2;       // [warps][n + 1] a warp's tokens of each adapter, then those of the warps before it
   __shared__ int2 s_warp[32];
   wait_for_stream();
   let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, buckets = a.n + 1;
-  for (int i = tid; i < buckets; i += 1024) s_count[i] = 0;
-  int per_log = 0;                    // a power of two of tokens per thread: no divisions
-  while (per_log < 5 && (1024 << per_log) < a.T) ++per_log;
-  const int per = 1 << per_log;
-  auto load = [&](int t0) {
-    const int n = min(a.T - t0, 1024 * per);
-    __syncthreads();
-    auto put = [&](int i, int id) { s_id[(i >> per_log) * (kAD_RoutePer + 2) + (i & (per - 1))] = (uint16_t)adapter_of(a, id); };
-    const int head = min(n, (int)(-(reinterpret_cast<uintptr_t>(a.ids + t0) >> 2) & 3)), quads = (n - head) / 4;      // to a 16-byte boundary
-    if (tid < head) put(tid, a.ids[t0 + tid]);
-    if (tid < n - head - 4 * quads) put(head + 4 * quads + tid, a.ids[t0 + head + 4 * quads + tid]);
-    const int4* from = reinterpret_cast<const int4*>(a.ids + t0 + head);
-    for (int i0 = 0; i0 < quads; i0 += 8192) {
-      int4 v[8];
+  for (int i = tid; i < warps * buckets; i += 1024) s_row[i] = 0;
+  __syncthreads();
+  const int per = ((a.T + 31) / 32 + warps - 1) / warps * 32;
+  const long long begin = (long long)warp * per;
+  const int end = warp < warps ? (int)min(begin + per, (long long)a.T) : 0;
+  int* mine = s_row + warp * buckets;
+  // what(token, adapter, tokens of it before this one in the warp's stretch), in the order of the tokens
+  auto walk = [&](auto what) {
+    for (long long t0 = begin; t0 < end; t0 += 256) {
+      int id[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (i0 + k * 1024 + tid < quads) v[k] = __ldg(from + i0 + k * 1024 + tid);
+      for (int k = 0; k < 8; ++k) id[k] = t0 + 32 * k + lane < end ? adapter_of(a, __ldg(a.ids + t0 + 32 * k + lane)) : -1;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int i = i0 + k * 1024 + tid;
-        if (i < quads) {
-          put(head + 4 * i, v[k].x);
-          put(head + 4 * i + 1, v[k].y);
-          put(head + 4 * i + 2, v[k].z);
-          put(head + 4 * i + 3, v[k].w);
+        if (t0 + 32 * k >= end) break;
+        const unsigned same = __match_any_sync(0xffffffffu, id[k]);
+        const int before = id[k] >= 0 ? mine[id[k]] : 0;
+        __syncwarp();
+        if (id[k] >= 0) {
+          what((int)t0 + 32 * k + lane, id[k], before + __popc(same & ((1u << lane) - 1u)));
+          if (lane == __ffs(same) - 1) mine[id[k]] = before + __popc(same);
         }
+        __syncwarp();
       }
     }
-    __syncthreads();
   };
-  const uint16_t* mine_id = s_id + tid * (kAD_RoutePer + 2);
-  // this thread's tokens: how many, and whether the warp's are all of one adapter
-  auto whole = [&](int t0, int& n) {
-    n = max(0, min(per, a.T - t0 - tid * per));
-    const int first = n > 0 ? mine_id[0] : -1, of_warp = __shfl_sync(0xffffffffu, first, 0);
-    bool same = n > 0 && first == of_warp;
-    if (n == kAD_RoutePer) {
-      uint32_t differ = 0;             // two at a time
+  walk([](int, int, int) {});
+  __syncthreads();
+  for (int b = warp; b < buckets; b += 32) {
+    const int n = lane < warps ? s_row[lane * buckets + b] : 0;
+    int incl = n;
 #pragma unroll
-      for (int i = 0; i < kAD_RoutePer / 2; ++i) differ |= reinterpret_cast<const uint32_t*>(mine_id)[i] ^ ((uint32_t)first * 0x10001u);
-      same = same && differ == 0;
-    } else {
-      for (int i = 1; i < n; ++i) same = same && mine_id[i] == first;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
     }
-    return __all_sync(0xffffffffu, same) ? of_warp : -1;
-  };
-  auto warp_total = [&](int n) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)n); };
-  for (int t0 = 0; t0 < a.T; t0 += 1024 * per) {
-    load(t0);
-    int n;
-    const int one = whole(t0, n);
-    if (one >= 0) {
-      const int sum = warp_total(n);
-      if (lane == 0) atomicAdd(&s_count[one], sum);
-    } else {
-      for (int i = 0, begin = 0; i < n; ++i) {
-        if (i + 1 == n || mine_id[i + 1] != mine_id[i]) {
-          atomicAdd(&s_count[mine_id[i]], i + 1 - begin);
-          begin = i + 1;
-        }
-      }
-    }
+    if (lane < warps) s_row[lane * buckets + b] = incl - n;
+    if (lane == 31) s_count[b] = incl;
   }
   __syncthreads();
   // both running sums over the adapters, thread i holding `each` of them
   const int each = (buckets + 1023) / 1024, lo = min(tid * each, buckets), hi = min(lo + each, buckets);
-  int2 mine = make_int2(0, 0);
+  int2 sum = make_int2(0, 0);
   for (int b = lo; b < hi; ++b) {
-    mine.x += (s_count[b] + 7) & ~7;
-    mine.y += (s_count[b] + kAD_Group - 1) / kAD_Group;
+    sum.x += (s_count[b] + 7) & ~7;
+    sum.y += (s_count[b] + kAD_Group - 1) / kAD_Group;
   }
-  int2 incl = mine;
+  int2 incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, incl.x, o), y = __shfl_up_sync(0xffffffffu, incl.y, o);
@@ -241,7 +216,7 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
   }
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
-  int2 at = make_int2(incl.x - mine.x, incl.y - mine.y);
+  int2 at = make_int2(incl.x - sum.x, incl.y - sum.y);
   for (int w = 0; w < warp; ++w) {
     at.x += s_warp[w].x;
     at.y += s_warp[w].y;
@@ -269,36 +244,7 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a) {
     a.n_groups[1] = s_grp[a.n];       // tokens without an adapter come last: they have no h, and in place they are done
     a.n_groups[0] = a.out == a.y ? s_grp[a.n] : total;
   }
-  __syncthreads();
-  for (int t0 = 0; t0 < a.T; t0 += 1024 * per) {
-    if (a.T > 1024 * per) load(t0);
-    int n;
-    const int one = whole(t0, n);
-    if (one >= 0) {
-      // the warp's tokens follow one another, and so do their places: four at a time, from a 16-byte boundary on
-      const int sum = warp_total(n), t = t0 + 32 * warp * per;
-      int base = 0;
-      if (lane == 0) base = atomicAdd(&s_at[one], sum);
-      base = __shfl_sync(0xffffffffu, base, 0);
-      int* to = a.perm + base;
-      const int head = min(sum, -base & 3), quads = (sum - head) / 4, rest = sum - head - 4 * quads;
-      if (lane < head) to[lane] = t + lane;
-      if (lane < rest) to[head + 4 * quads + lane] = t + head + 4 * quads + lane;
-      for (int q = lane; q < quads; q += 32) {
-        const int x = t + head + 4 * q;
-        *reinterpret_cast<int4*>(to + head + 4 * q) = make_int4(x, x + 1, x + 2, x + 3);
-      }
-    } else {
-      const int first = t0 + tid * per;
-      for (int i = 0, begin = 0; i < n; ++i) {
-        if (i + 1 == n || mine_id[i + 1] != mine_id[i]) {
-          const int to = atomicAdd(&s_at[mine_id[i]], i + 1 - begin);
-          for (int j = begin; j <= i; ++j) a.perm[to + j - begin] = first + j;
-          begin = i + 1;
-        }
-      }
-    }
-  }
+  walk([&](int t, int id, int nth) { a.perm[s_at[id] + nth] = t; });
 }
 
 // h of many tokens: the groups' steps of 128 values of d_in, group by group, an equal run of them to each CTA, one per SM.  x rows (gathered) and A rows come
@@ -915,8 +861,9 @@ static int launch_adapters(AdapterArgs a, int sms, cudaStream_t stream) {
     a.units = (blocks + cut - 1) / cut;
     return launch_early(adapter_expand_few_kernel<T>, dim3(a.T, (blocks + a.units - 1) / a.units), 256, 0, stream, a);
   }
-  if ((rc = ensure_smem_attr((const void*)adapter_route_kernel, 3 * (kAD_MaxAdapters + 2) * 4 + kAD_RouteIds))) return rc;
-  if ((rc = launch_early(adapter_route_kernel, dim3(1), 1024, (size_t)(3 * (a.n + 2)) * 4 + kAD_RouteIds, stream, a))) return rc;
+  const int warps = adapter_route_warps(a.n);
+  if ((rc = ensure_smem_attr((const void*)adapter_route_kernel, kAD_RouteWords * 4))) return rc;
+  if ((rc = launch_early(adapter_route_kernel, dim3(1), 1024, (size_t)(3 * (a.n + 2) + warps * (a.n + 1)) * 4, stream, a, warps))) return rc;
   rc = a.rmax <= 32 ? launch_shrink<T, 32>(a, stream) : a.rmax <= 64 ? launch_shrink<T, 64>(a, stream) : launch_shrink<T, 128>(a, stream);
   if (rc) return rc;
   return a.rmax <= 64 ? launch_expand<T, 64>(a, sms, stream) : launch_expand<T, 128>(a, sms, stream);

@@ -546,9 +546,10 @@ class PagedLayer:
         c, (B, H, t, D) = self.cache, qr.shape
         dt = kr.dtype if kr.dtype == torch.float16 else torch.bfloat16
         q, k, v = qr.transpose(1, 2).to(dt), kr.transpose(1, 2).to(dt), v.to(dt)
+        plan = c._layer_plan(B) if later and self.share else None      # (a capture that has none is refused before it writes)
         c._append(self.index, k, v)
         if later:
-            return c.attend(self.index, q, shared=c._layer_plan(B) if self.share else None)[0].to(qr.dtype)
+            return c.attend(self.index, q, shared=plan)[0].to(qr.dtype)
         # a whole prompt: attention over the keys and values as they are, not over their codes
         cu = torch.arange(B + 1, device=qr.device, dtype=torch.int32) * t
         o, _ = prompt_attention(q.reshape(B * t, H, D), k.reshape(B * t, c.heads, D), v.reshape(B * t, c.heads, D), cu)

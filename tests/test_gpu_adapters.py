@@ -1,8 +1,8 @@
 """Adapters.add against its formula in 64 bits.
 
 Tolerance.  u is half a step of the output type, S = |s| sum_r |B_r| sum_i |A_ri x_i|, P = |s| sum_r |B_r h_r|:
-  * a chain of products for h has at most d_in / 32 + 32 additions (steps of 16 values of half of d_in, then warps and splits), each off by at most
-    2^-22 of the sum of the magnitudes: (d_in / 32 + 32) 2^-22 S;
+  * a chain of sums for h has at most d_in / 16 + 64 additions (steps of 16 values, then warps and parts), each off by at most 2^-23 of the sum of the
+    magnitudes: (d_in / 32 + 32) 2^-22 S;
   * h enters as two parts: 2^-16 (bf16) or 2^-21 (fp16) of itself; the second product has at most 16 additions: 2^-18 P in all;
   * out is rounded once: u |out|, and 2^-25 in fp16 below its normal range.
 With whole numbers that all sums hold exactly, out is the rounded exact value."""
@@ -55,6 +55,20 @@ def test_against_the_formula(T, ranks, d_in, d_out, dtype):
     for ids in (torch.randint(-1, len(ranks), (T,), generator=g), torch.arange(T) * len(ranks) // T, torch.full((T,), len(ranks) - 1)):
         ids = ids.cuda()
         _check(ad.add(y, x, ids), x, y, ids, a, b, s)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,ranks,d_in,d_out", [(5000, [128, 64, 16, 1], 4104, 392), (2600, [64] * 7, 8, 8), (2049, [8], 1160, 136), (20100, [32, 16], 1032, 264)])
+def test_groups_that_several_ctas_share(T, ranks, d_in, d_out, dtype):
+    """More steps than CTAs, groups cut anywhere, groups of a CTA's own between two that it shares, and groups of one step."""
+    ad, a, b, s = _make(ranks, d_in, d_out, dtype)
+    x, y = _data(T, d_in, d_out, dtype, seed=T)
+    ids = torch.randint(-1, len(ranks), (T,), generator=torch.Generator().manual_seed(T)).cuda()
+    ids[T // 3:T // 2] = 0
+    first = ad.add(y, x, ids)
+    _check(first, x, y, ids, a, b, s)
+    assert torch.equal(first, ad.add(y, x, ids))           # the parts are added in their order, whoever is last
+    assert torch.equal(first, ad.add(y, x, ids, out=y))
 
 
 @pytest.mark.parametrize("T", [40, 700])
@@ -208,3 +222,7 @@ def test_layer_with_adapters():
     assert torch.equal(A.forward(x, {}, 0)[1], y[1])
     with pytest.raises(ValueError):
         layer(w, adapters={"q": Adapters(*low["k"])})
+    for bad in (ids[:2], ids.float(), ids[:, None].expand(3, 4)):
+        with pytest.raises(ValueError):
+            A.project(x, 0, adapter_ids=bad)
+    assert torch.equal(A.project(x, 0, adapter_ids=ids.int())[5], A.project(x, 0, adapter_ids=ids[:, None].expand(3, 90))[5])

@@ -273,6 +273,38 @@ def test_captured_and_replayed_with_a_new_plan():
         _check_out(c, plan, q.cpu(), o, lse)
 
 
+def test_replayed_with_a_plan_that_has_no_runs():
+    """And with one that is no longer good: what the pages then hold is not the sequences', but the replay ends and the others are right."""
+    c, slots = _tree(64, 1000, [0], [4], [3, 9, 1, 2], spare=10)
+    q = _rand(4, 1, 8, D, seed=13).cuda()
+    plan, none = c.share(slots, min_saved=1), c.share(slots)
+    assert plan.runs == 1 and none.runs == 0
+    for p in (plan, none):
+        c.attend(0, q, shared=p)
+    g, h = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o, lse = c.attend(0, q, shared=plan, with_lse=True)
+    with torch.cuda.graph(h):
+        o2, lse2 = c.attend(0, q, shared=none, with_lse=True)
+    c.share(slots, plan)
+    c.share(slots[::-1], none, min_saved=1)
+    assert plan.runs == 0 and none.runs == 1
+    g.replay()
+    h.replay()
+    torch.cuda.synchronize()
+    _check_out(c, plan, q.cpu(), o, lse)
+    _check_out(c, none, q.cpu(), o2, lse2)
+    c.share(slots, plan, min_saved=1)
+    c.free([slots[1]])
+    assert not plan.good
+    g.replay()
+    torch.cuda.synchronize()
+    assert not o[1].any() and (lse[1] == -float("inf")).all()
+    plan.slots[1] = plan.slots[0]
+    o[1], lse[1], q[1] = o[0], lse[0], q[0]
+    _check_out(c, plan, q.cpu(), o, lse)
+
+
 def test_refused_calls():
     c, slots = _tree(16, 100, [0], [3], [1, 1, 1])
     other, _ = _tree(16, 100, [0], [3], [1, 1, 1])
