@@ -170,6 +170,20 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a, int 
       int id[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) id[k] = t0 + 32 * k + lane < end ? adapter_of(a, __ldg(a.ids + t0 + 32 * k + lane)) : -1;
+      // 256 tokens of one adapter at once
+      const int one = __shfl_sync(0xffffffffu, id[0], 0);
+      bool alike = one >= 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) alike = alike && id[k] == one;
+      if (__all_sync(0xffffffffu, alike)) {
+        const int before = mine[one];
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) what((int)t0 + 32 * k + lane, one, before + 32 * k + lane);
+        if (lane == 0) mine[one] = before + 256;
+        __syncwarp();
+        continue;
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         if (t0 + 32 * k >= end) break;
