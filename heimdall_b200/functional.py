@@ -350,15 +350,15 @@ def norm_rope_heads(qg, kl, q_norm_w, k_norm_w, positions, inv_freq, axes=None, 
     dev = serving_inputs("norm_rope_heads", qg, kl, q_norm_w, k_norm_w)
     if qg.dim() != 4 or kl.dim() != 4 or qg.shape[:2] != kl.shape[:2] or qg.dtype != kl.dtype:
         raise ValueError("norm_rope_heads takes qg [B,t,H,(2) D] and kl [B,t,G,D] of one dtype")
-    B, t, H, _ = qg.shape
-    G, D = kl.shape[2], kl.shape[3]
+    (B, t, H, width), (_, _, G, D) = qg.shape, kl.shape
     if D != 256:
         raise NotImplementedError("norm_rope_heads is built for head dim 256")
-    if qg.shape[3] != (2 * D if gated else D) or q_norm_w.shape != (D,) or k_norm_w.shape != (D,) or H < 1 or G < 1:
+    if width != (2 * D if gated else D) or q_norm_w.shape != (D,) or k_norm_w.shape != (D,) or H < 1 or G < 1:
         raise ValueError("the heads' and norm weights' shapes do not match")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.shape[-2:] != (B, t) or positions.dim() not in (2, 3):
+    where, wide = positions.shape, positions.dtype is torch.int64
+    if not (wide or positions.dtype is torch.int32) or len(where) not in (2, 3) or where[-2:] != (B, t):
         raise ValueError("positions must be an int32 or int64 tensor [B,t] or [axes,B,t]")
-    n = positions.shape[0] if positions.dim() == 3 else 1
+    n = where[0] if len(where) == 3 else 1
     F = 0 if inv_freq is None else inv_freq.numel()
     if not 1 <= n <= 4 or (axes is None and n > 1):
         raise ValueError("positions have one to four axes, and with more than one the axis of each frequency is needed")
@@ -368,16 +368,23 @@ def norm_rope_heads(qg, kl, q_norm_w, k_norm_w, positions, inv_freq, axes=None, 
     if len(code) != F or (F and max(code) >= n):
         raise ValueError("axes needs one of the positions' axes for each frequency")
     with on_device(dev):
-        on = lambda x, dt: x if x.dtype == dt and x.device == dev and x.is_contiguous() else x.to(device=dev, dtype=dt).contiguous()
-        q_norm_w, k_norm_w = on(q_norm_w, torch.float32), on(k_norm_w, torch.float32)
-        inv_freq = None if not F else on(inv_freq, torch.float32)
-        positions = on(positions, positions.dtype)
+        f32 = torch.float32
+        if q_norm_w.dtype is not f32 or not q_norm_w.is_contiguous():
+            q_norm_w = q_norm_w.to(f32).contiguous()
+        if k_norm_w.dtype is not f32 or not k_norm_w.is_contiguous():
+            k_norm_w = k_norm_w.to(f32).contiguous()
+        if F == 0:
+            inv_freq = None
+        elif inv_freq.dtype is not f32 or inv_freq.device != dev or not inv_freq.is_contiguous():
+            inv_freq = inv_freq.to(device=dev, dtype=f32).contiguous()
+        if positions.device != dev or not positions.is_contiguous():
+            positions = positions.to(dev).contiguous()
         qg, qp, qs = heads_16bit("qg", qg)
         kl, kp, ks = heads_16bit("kl", kl)
         q, k = (qg.new_empty((B, t, H, D)), qg.new_empty((B, t, G, D))) if memory else (None, None)
         qr, kr = qg.new_empty((B, H, t, D)), qg.new_empty((B, G, t, D))
         _lib.call("bf_norm_rope", qp, *qs, kp, *ks, ptr(q_norm_w), ptr(k_norm_w), ptr(inv_freq), F, code, n, ptr(positions),
-                  int(positions.dtype == torch.int64), eps, B, t, H, G, D, kernel_dtype(qg), ptr(q), ptr(k), ptr(qr), ptr(kr),
+                  wide, eps, B, t, H, G, D, kernel_dtype(qg), ptr(q), ptr(k), ptr(qr), ptr(kr),
                   stream_handle())
     return q, k, qr, kr
 
