@@ -85,7 +85,7 @@ class Adapters:
             x, xp, xs = heads_16bit("x", x if flat else x.reshape(T, self.d_in))
             y2, yp, ys = heads_16bit("y", y if flat else y.reshape(T, self.d_out))
             if out is None:
-                out = y.new_empty(y.shape)
+                out = torch.empty_like(y, memory_format=torch.contiguous_format)
             elif (out.data_ptr() != yp or (T > 1 and ys[0] != self.d_out)) and _overlap(out, y2):
                 raise ValueError("out may be y, but not overlap it")
             nws = self._ws.get(T)

@@ -21,7 +21,7 @@ def check_cuda(*ts) -> None:
 
 def stream_handle() -> int:
     """The current stream of the current device (torch.cuda.current_stream() builds an object around it: 2 us)."""
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def ptr(t) -> int:
@@ -234,7 +234,10 @@ def serving_inputs(name: str, *ts) -> torch.device:
 
 def on_device(dev: torch.device):
     """The tensors' device as the current one (no guard where it is already: the guard costs a few microseconds)."""
-    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+
+
+_HERE = nullcontext()
 
 
 def heads_16bit(name: str, t):
@@ -244,6 +247,8 @@ def heads_16bit(name: str, t):
     if t.dtype != torch.bfloat16 and t.dtype != torch.float16:
         raise NotImplementedError(f"{name} is {t.dtype}: built for bfloat16 and float16")
     at, st = t.data_ptr(), t.stride()
+    if at % 16 == 0 and t.shape[-1] % 8 == 0 and t.is_contiguous():
+        return t, at, list(st[:-1])
     ok = st[-1] == 1 and at % 16 == 0
     out = []
     for s, n in zip(st[:-1], t.shape):

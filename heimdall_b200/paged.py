@@ -151,6 +151,7 @@ class SharedPages:
         self.cache = cache
         self.n = slots.size
         self.plan = torch.empty(plan.size, dtype=torch.int32, device=cache.device)
+        self._slot_ids = self.plan[4:4 + self.n]
         self._fill(slots, plan)
         cache._plans.add(self)
 
@@ -395,9 +396,10 @@ class PagedKV:
         if shared is not None:
             self._check_plan(shared, slots, B)
         with on_device(dev):
-            if shared is not None and not shared.runs:
-                slots, shared = shared.plan[4:4 + B], None           # nothing to share
-            ids = None if shared is not None else self._ids(slots, B)
+            if shared is None:
+                ids = self._ids(slots, B)
+            elif not shared.runs:
+                ids, shared = shared._slot_ids, None                 # nothing to share
             q, qp, qs = heads_16bit("q", q)
             o = q.new_empty(shape)
             lse = q.new_empty((B, H, t), dtype=torch.float32) if with_lse else None
