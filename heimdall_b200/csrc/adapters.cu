@@ -71,28 +71,63 @@ __device__ __forceinline__ uint4 ldg_stream(const uint4* p) { return __ldcs(p); 
 // an adapter's number, n for none
 __device__ __forceinline__ int adapter_of(const AdapterArgs& a, int id) { return id >= 0 && id < a.n ? id : a.n; }
 
-// Few tokens: the group that token `lead` begins, if it begins one: the 16 tokens of its adapter from it on, in s_tok.  Returns how many
-// (0: another CTA's), and the adapter.  All 256 threads.
-__device__ __forceinline__ int few_group(const AdapterArgs& a, int lead, int* s_tok, unsigned* s_mask, int& id) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  id = adapter_of(a, a.ids[lead]);
-  const bool mine = tid < a.T && adapter_of(a, a.ids[tid]) == id;
-  const unsigned m = __ballot_sync(0xffffffffu, mine);
-  if (lane == 0) s_mask[warp] = m;
-  __syncthreads();
-  int before_lead = 0, before_me = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const unsigned x = s_mask[w];
-    total += __popc(x);
-    before_lead += w < (lead >> 5) ? __popc(x) : w == (lead >> 5) ? __popc(x & ((1u << (lead & 31)) - 1u)) : 0;
-    before_me += w < warp ? __popc(x) : w == warp ? __popc(x & ((1u << lane) - 1u)) : 0;
+// h as two parts: a power of two takes the row's largest to [2^13, 2^14), so that both keep all of their bits in fp16 too.  (A NaN is no maximum, but its
+// row becomes NaN by itself.)
+struct RowScale {
+  int ex;
+  __device__ __forceinline__ explicit RowScale(float big) { ex = big > 0.f && big < INFINITY ? min(max((int)(__float_as_uint(big) >> 23), 14), 253) : 140; }
+  template <typename T>
+  __device__ __forceinline__ void parts(float h, T& hi, T& lo) const {
+    const float x = h * __uint_as_float((uint32_t)(267 - ex) << 23);
+    hi = (T)x;
+    lo = (T)(x - (float)hi);
   }
-  if (before_lead & 15) return 0;
-  if (mine && before_me >= before_lead && before_me < before_lead + 16) s_tok[before_me - before_lead] = tid;
+  __device__ __forceinline__ float back() const { return __uint_as_float((uint32_t)(ex - 13) << 23); }
+};
+
+// Few tokens: group x, the groups being 16 tokens of an adapter in their order, in the order of their first tokens: its tokens in s_tok.  Returns how
+// many (0: there are fewer groups), and the adapter.  All 256 threads, thread = token.
+struct FewSmem {
+  int4 id[kAD_Few / 4];
+  unsigned leads[8];
+  int first, nth;
+};
+__device__ __forceinline__ int few_group(const AdapterArgs& a, int x, int* s_tok, FewSmem& s, int& id) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int mine = tid < a.T ? adapter_of(a, a.ids[tid]) : -1;
+  reinterpret_cast<int*>(s.id)[tid] = mine;
+  if (tid == 0) s.first = -1;
   __syncthreads();
-  return min(16, total - before_lead);
+  int nth = 0;                 // of its adapter's tokens
+  if (32 * warp < a.T) {
+#pragma unroll 1
+    for (int w = 0; w < warp; ++w)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int4 v = s.id[8 * w + i];
+        nth += (v.x == mine) + (v.y == mine) + (v.z == mine) + (v.w == mine);
+      }
+    nth += __popc(__match_any_sync(0xffffffffu, mine) & ((1u << lane) - 1u));
+  }
+  const bool lead = mine >= 0 && (nth & 15) == 0;
+  const unsigned leads = __ballot_sync(0xffffffffu, lead);
+  if (lane == 0) s.leads[warp] = leads;
+  __syncthreads();
+  int before = __popc(leads & ((1u << lane) - 1u));
+  for (int w = 0; w < warp; ++w) before += __popc(s.leads[w]);
+  if (lead && before == x) {
+    s.first = tid;
+    s.nth = nth;
+  }
+  __syncthreads();
+  if (s.first < 0) return 0;
+  id = reinterpret_cast<const int*>(s.id)[s.first];
+  const bool member = mine == id && nth >= s.nth && nth < s.nth + 16;
+  if (member) s_tok[nth - s.nth] = tid;
+  return __syncthreads_count(member);
 }
+// no more than so many groups
+static int few_groups(int T, int n) { return min(T, T / 16 + min(n + 1, T)); }
 
 // h of a few tokens: CTA = (group, part of d_in, 16 ranks).  A warp takes every eighth 32 values of d_in: lane (g, c) loads the 16 bytes at
 // 8 c of x rows g and g + 8 and of ranks g and g + 8, the fragments of two steps (a sum over d_in may take its values in any order as
@@ -100,13 +135,13 @@ __device__ __forceinline__ int few_group(const AdapterArgs& a, int lead, int* s_
 template <typename T>
 __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(AdapterArgs a) {
   __shared__ int s_tok[16];
-  __shared__ unsigned s_mask[8];
+  __shared__ FewSmem s_few;
   __shared__ float s_sum[8][16][17];
   wait_for_stream();
   let_next_start();        // only now: what the next kernel reads before its own wait is older than this one
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   int id;
-  const int m = few_group(a, blockIdx.x, s_tok, s_mask, id);
+  const int m = few_group(a, blockIdx.x, s_tok, s_few, id);
   if (m == 0 || id == a.n) return;
   const int r0 = a.row[id], rank = a.row[id + 1] - r0, rc = blockIdx.z * 16;
   if (rc >= rank) return;
@@ -447,13 +482,11 @@ __global__ void __launch_bounds__(416, 1) adapter_shrink_kernel(AdapterArgs a) {
             }
           }
       }
-      float big = 0.f;           // (a NaN is no maximum, but its row becomes NaN by itself)
+      float big = 0.f;
 #pragma unroll
       for (int c = 0; c < RM; ++c)
         if (c < rank) big = fmaxf(big, fabsf(v[c]));
-      // a power of two that takes the row's largest to [2^13, 2^14): both parts then keep all of their bits in fp16 too
-      const int ex = big > 0.f && big < INFINITY ? min(max((int)(__float_as_uint(big) >> 23), 14), 253) : 140;
-      const float up = __uint_as_float((uint32_t)(267 - ex) << 23);
+      const RowScale rs(big);
       if (r < m) {
         T* to = static_cast<T*>(a.parts) + (size_t)grp.y * 2 * a.rmax + (r >> 3) * 8 * rank + (r & 7) * 8;
         const int other = ((m + 7) & ~7) * rank;
@@ -463,15 +496,11 @@ __global__ void __launch_bounds__(416, 1) adapter_shrink_kernel(AdapterArgs a) {
             uint4 h, l;
             T *hi = reinterpret_cast<T*>(&h), *lo = reinterpret_cast<T*>(&l);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float x = v[c + i] * up;
-              hi[i] = (T)x;
-              lo[i] = (T)(x - (float)hi[i]);
-            }
+            for (int i = 0; i < 8; ++i) rs.parts(v[c + i], hi[i], lo[i]);
             *reinterpret_cast<uint4*>(to + 8 * c) = h;
             *reinterpret_cast<uint4*>(to + other + 8 * c) = l;
           }
-        a.back[grp.y + r] = scale * __uint_as_float((uint32_t)(ex - 13) << 23);
+        a.back[grp.y + r] = scale * rs.back();
       }
     }
   }
@@ -484,14 +513,14 @@ __global__ void __launch_bounds__(416, 1) adapter_shrink_kernel(AdapterArgs a) {
   }
 }
 
-// out of a few tokens: CTA = (group, `units` times 512 columns).  A lane has two columns, whose rows of B (r values) it loads whole, 16 bytes at a
-// time and the next 16 ranks ahead, and up to four of the group's tokens: with one token per adapter most of a tensor-core tile would be empty, and
-// fp32 products of up to 16 tokens cost no more than mma.sync of two parts.
-template <typename T, int M>       // M: 1 or 4 tokens at most
-__device__ __forceinline__ void expand_few(const AdapterArgs& a, const T* w, int rank, int m, const int* s_tok, const float* s_h, float scale, int col0,
-                                           int units) {
+// out of a few tokens: CTA = (group, `units` times 512 columns), a warp 64 of them.  One token: a lane has columns l and l + 32, whose ranks it loads 16 bytes at a
+// time, the next 16 ranks ahead, and h in fp32: most of a tensor-core tile would be empty.
+template <typename T>
+__device__ __forceinline__ void expand_one(const AdapterArgs& a, const T* w, int rank, int tok, const float* s_h, float scale, int col0, int units) {
   const int lane = threadIdx.x & 31;
-  T y[M][2], y_next[M][2];
+  const T* y0 = static_cast<const T*>(a.y) + (long long)tok * a.y_st;
+  T* out0 = static_cast<T*>(a.out) + (long long)tok * a.o_st;
+  T y[2], y_next[2];
   uint4 b[4];
   const uint4 *p, *q;
   // unit u's y and first 16 ranks
@@ -499,13 +528,8 @@ __device__ __forceinline__ void expand_few(const AdapterArgs& a, const T* w, int
     const int col = col0 + 512 * u + lane;
     if (u >= units || col >= a.d_out) return;
     const bool two = col + 32 < a.d_out;
-#pragma unroll
-    for (int t = 0; t < M; ++t)
-      if (t < m) {
-        const T* from = static_cast<const T*>(a.y) + (long long)s_tok[t] * a.y_st + col;
-        y_next[t][0] = from[0];
-        if (two) y_next[t][1] = from[32];
-      }
+    y_next[0] = y0[col];
+    if (two) y_next[1] = y0[col + 32];
     p = reinterpret_cast<const uint4*>(w + (long long)(col >> 3) * 8 * rank + (col & 7) * 8);
     q = two ? p + 4 * rank : p;
     b[0] = __ldg(p), b[1] = __ldg(p + 8), b[2] = __ldg(q), b[3] = __ldg(q + 8);
@@ -515,12 +539,8 @@ __device__ __forceinline__ void expand_few(const AdapterArgs& a, const T* w, int
   for (int u = 0; u < units; ++u) {
     const int col = col0 + 512 * u + lane;
     if (col >= a.d_out) return;
-    uint64_t acc[M][2];
-#pragma unroll
-    for (int t = 0; t < M; ++t) {
-      acc[t][0] = acc[t][1] = 0;
-      y[t][0] = y_next[t][0], y[t][1] = y_next[t][1];
-    }
+    uint64_t acc[2] = {0, 0};
+    y[0] = y_next[0], y[1] = y_next[1];
 #pragma unroll 1
     for (int r = 0; r < rank; r += 16) {
       uint4 now[4] = {b[0], b[1], b[2], b[3]};
@@ -533,47 +553,93 @@ __device__ __forceinline__ void expand_few(const AdapterArgs& a, const T* w, int
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint64_t wf[2][4];
+        const ulonglong2* h = reinterpret_cast<const ulonglong2*>(s_h + r + 8 * i);
+        const ulonglong2 h0 = h[0], h1 = h[1];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const T* e = reinterpret_cast<const T*>(&now[2 * k + i]);
+          uint64_t wf[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) wf[k][x] = pair2((float)e[2 * x], (float)e[2 * x + 1]);
-        }
-#pragma unroll
-        for (int t = 0; t < M; ++t) {
-          if (t < m) {
-            const ulonglong2* h = reinterpret_cast<const ulonglong2*>(s_h + t * kAD_MaxRank + r + 8 * i);
-            const ulonglong2 h0 = h[0], h1 = h[1];
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-              acc[t][k] = fma2(wf[k][3], h1.y, fma2(wf[k][2], h1.x, fma2(wf[k][1], h0.y, fma2(wf[k][0], h0.x, acc[t][k]))));
-          }
+          for (int x = 0; x < 4; ++x) wf[x] = pair2((float)e[2 * x], (float)e[2 * x + 1]);
+          acc[k] = fma2(wf[3], h1.y, fma2(wf[2], h1.x, fma2(wf[1], h0.y, fma2(wf[0], h0.x, acc[k]))));
         }
       }
     }
 #pragma unroll
-    for (int t = 0; t < M; ++t) {
-      if (t < m) {
-        T* to = static_cast<T*>(a.out) + (long long)s_tok[t] * a.o_st + col;
+    for (int k = 0; k < 2; ++k)
+      if (k == 0 || col + 32 < a.d_out) out0[col + 32 * k] = (T)fmaf(lo_hi(acc[k], 0) + lo_hi(acc[k], 1), scale, (float)y[k]);
+  }
+}
+
+// 2 to 16 tokens: mma.sync with h's two parts (as for many tokens), 32 columns at a time.  Column 8 (n / 2) + 2 j + n % 2 of them is column n of product j, so
+// that a lane ends with 8 consecutive columns of two tokens.
+constexpr int kAD_FewPitch = kAD_MaxRank + 8;       // from row to row of h's parts in shared memory
+template <typename T>
+__device__ __forceinline__ void expand_several(const AdapterArgs& a, const T* w, int rank, int m, const int* s_tok, const T* s_parts, const float* s_back, int col0,
+                                               int units) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  auto col_of = [&](int u) { return col0 + 512 * (u >> 1) + 32 * (u & 1); };
+  uint32_t b[8];                   // product j's two values of k 0 .. 7 and 8 .. 15
+  auto load = [&](int u, int r) {
+    const int col = col_of(u) + 8 * (g >> 1);
+    const T* from = w + (long long)(col >> 3) * 8 * rank + 8 * r + 8 * (g & 1) + 2 * c;
+    const bool in = u < 2 * units && col < a.d_out;
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (k == 0 || col + 32 < a.d_out) to[32 * k] = (T)fmaf(lo_hi(acc[t][k], 0) + lo_hi(acc[t][k], 1), scale, (float)y[t][k]);
+    for (int j = 0; j < 4; ++j) {
+      b[2 * j] = in ? __ldg(reinterpret_cast<const uint32_t*>(from + 16 * j)) : 0u;
+      b[2 * j + 1] = in ? __ldg(reinterpret_cast<const uint32_t*>(from + 16 * j + 64)) : 0u;
+    }
+  };
+  load(0, 0);
+#pragma unroll 1
+  for (int u = 0; u < 2 * units; ++u) {
+    if (col_of(u) >= a.d_out) return;
+    const int col = col_of(u) + 8 * c;
+    uint4 y[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (g + 8 * e < m && col < a.d_out)
+        y[e] = ldg_stream(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + (long long)s_tok[g + 8 * e] * a.y_st + col));
+    float acc[4][4] = {};
+#pragma unroll 1
+    for (int r = 0; r < rank; r += 16) {
+      uint32_t now[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) now[j] = b[j];
+      if (r + 16 < rank) load(u, r + 16); else load(u + 1, 0);
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        const T* h = s_parts + (part * 16 + g) * kAD_FewPitch + r + 2 * c;
+        const uint32_t a0 = *reinterpret_cast<const uint32_t*>(h), a1 = *reinterpret_cast<const uint32_t*>(h + 8 * kAD_FewPitch),
+                       a2 = *reinterpret_cast<const uint32_t*>(h + 8), a3 = *reinterpret_cast<const uint32_t*>(h + 8 * kAD_FewPitch + 8);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma16816<T>(acc[j], a0, a1, a2, a3, now[2 * j], now[2 * j + 1]);
       }
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (g + 8 * e < m && col < a.d_out) {
+        const float back = s_back[g + 8 * e];
+        T* x = reinterpret_cast<T*>(&y[e]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (T)fmaf(acc[i >> 1][2 * e + (i & 1)], back, (float)x[i]);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (long long)s_tok[g + 8 * e] * a.o_st + col) = y[e];
+      }
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs a) {
-  __shared__ __align__(16) float s_h[16 * kAD_MaxRank];
+  __shared__ __align__(16) float s_h[kAD_MaxRank];
+  __shared__ __align__(16) T s_parts[2 * 16 * kAD_FewPitch];
+  __shared__ float s_back[16];
   __shared__ int s_tok[16];
-  __shared__ unsigned s_mask[8];
+  __shared__ FewSmem s_few;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   let_next_start();
   int id;
   // the ids are older than the kernel before this one, which began by waiting for what was before it
-  const int m = few_group(a, blockIdx.x, s_tok, s_mask, id);
+  const int m = few_group(a, blockIdx.x, s_tok, s_few, id);
   if (m == 0 || (id == a.n && a.out == a.y)) return;
   const int col0 = blockIdx.y * a.units * 512 + warp * 64;
   if (id == a.n) {
@@ -591,18 +657,38 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
   const float scale = a.scale[id];
   const T* w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
   wait_for_stream();
-  for (int i = tid; i < m * rank; i += 256) {
-    const int t = i / rank, r = i - t * rank;
-    float v = 0.f;
-    const float* p = a.h + (size_t)s_tok[t] * a.rmax + r;
+  // a warp a token at a time, lane l the ranks l, l + 32, ...
+  for (int t = warp; t < m; t += 8) {
+    float v[kAD_MaxRank / 32], big = 0.f;
+#pragma unroll
+    for (int k = 0; k < kAD_MaxRank / 32; ++k) {
+      v[k] = 0.f;
+      const float* p = a.h + (size_t)s_tok[t] * a.rmax + 32 * k + lane;
+      if (32 * k + lane < rank) {
 #pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) v += p[(size_t)s * a.T * a.rmax];
-    s_h[t * kAD_MaxRank + r] = v;
+        for (int i = 0; i < a.splits; ++i) v[k] += p[(size_t)i * a.T * a.rmax];
+      }
+      big = fmaxf(big, fabsf(v[k]));
+    }
+    if (m == 1) {
+#pragma unroll
+      for (int k = 0; k < kAD_MaxRank / 32; ++k)
+        if (32 * k + lane < rank) s_h[32 * k + lane] = v[k];
+    } else {
+      const RowScale rs(warp_max(big));
+#pragma unroll
+      for (int k = 0; k < kAD_MaxRank / 32; ++k)
+        if (32 * k + lane < rank) {
+          T* to = s_parts + t * kAD_FewPitch + 32 * k + lane;
+          rs.parts(v[k], to[0], to[16 * kAD_FewPitch]);
+        }
+      if (lane == 0) s_back[t] = scale * rs.back();
+    }
   }
+  // rows of tokens that are not there: anything finite or not, nobody reads their sums
   __syncthreads();
-  if (m == 1) expand_few<T, 1>(a, w, rank, 1, s_tok, s_h, scale, col0, a.units);
-  else
-    for (int t = 0; t < m; t += 4) expand_few<T, 4>(a, w, rank, min(4, m - t), s_tok + t, s_h + t * kAD_MaxRank, scale, col0, a.units);
+  if (m == 1) expand_one<T>(a, w, rank, s_tok[0], s_h, scale, col0, a.units);
+  else expand_several<T>(a, w, rank, m, s_tok, s_parts, s_back, col0, a.units);
 }
 
 // out of many tokens: tiles of a group (128 tokens) and 128 columns, group by group, an equal run of them to each SM's one CTA.  Four warps bring y's rows into
@@ -868,12 +954,13 @@ template <typename T>
 static int launch_adapters(AdapterArgs a, int sms, cudaStream_t stream) {
   int rc;
   if (a.T <= kAD_Few) {
-    rc = launch_early(adapter_shrink_few_kernel<T>, dim3(a.T, a.splits, a.rmax / 16), 256, 0, stream, a);
+    const int groups = few_groups(a.T, a.n);
+    rc = launch_early(adapter_shrink_few_kernel<T>, dim3(groups, a.splits, a.rmax / 16), 256, 0, stream, a);
     if (rc) return rc;
-    // about four CTAs per SM if every token has an adapter of its own
-    const int blocks = (a.d_out + 511) / 512, cut = (4 * sms + a.T - 1) / a.T;
+    // about four CTAs per SM if there are as many groups as there can be
+    const int blocks = (a.d_out + 511) / 512, cut = (4 * sms + groups - 1) / groups;
     a.units = (blocks + cut - 1) / cut;
-    return launch_early(adapter_expand_few_kernel<T>, dim3(a.T, (blocks + a.units - 1) / a.units), 256, 0, stream, a);
+    return launch_early(adapter_expand_few_kernel<T>, dim3(groups, (blocks + a.units - 1) / a.units), 256, 0, stream, a);
   }
   const int warps = adapter_route_warps(a.n);
   if ((rc = ensure_smem_attr((const void*)adapter_route_kernel, kAD_RouteWords * 4))) return rc;
