@@ -11,7 +11,7 @@
 //   * more: adapter_route_kernel sorts the tokens by adapter and lists groups of 128, one M = 128 tile of the tensor core (tcgen05).
 // h = A x is split over d_in so that every SM has work; each split's sums are written on their own and added in order.  For many tokens h enters the
 // second product as two 16-bit parts of its row's power-of-two scale (hi + lo, 16 bits of bf16, 22 of fp16), so that the only rounding of
-// consequence is that of out; for few it stays fp32.
+// consequence is that of out; of few tokens those that share an adapter are taken so too, one alone keeps fp32.
 // (With mma.sync in the place of tcgen05 both kernels of many tokens were bound by its rate, about 32 cycles per m16n8k16 and scheduler:
 // 25480 tokens 6144 -> 5120, rank 64: 148 + 324 us.)
 #include "capi_internal.h"
