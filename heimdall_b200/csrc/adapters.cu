@@ -516,8 +516,8 @@ __global__ void __launch_bounds__(416, 1) adapter_shrink_kernel(AdapterArgs a) {
 
 // out of a few tokens: CTA = (group, `units` times 512 columns), a warp 64 of them.  One token: a lane has columns l and l + 32, whose ranks it loads 16 bytes at a
 // time, the next 16 ranks ahead, and h in fp32: most of a tensor-core tile would be empty.
-template <typename T>
-__device__ __forceinline__ void expand_one(const AdapterArgs& a, const T* w, int rank, int tok, const float* s_h, float scale, int col0, int units) {
+template <typename T, typename F>
+__device__ __forceinline__ void expand_one(const AdapterArgs& a, const T* w, int rank, int tok, const float* s_h, float scale, int col0, int units, F h_there) {
   const int lane = threadIdx.x & 31;
   const T* y0 = static_cast<const T*>(a.y) + (long long)tok * a.y_st;
   T* out0 = static_cast<T*>(a.out) + (long long)tok * a.o_st;
@@ -536,6 +536,7 @@ __device__ __forceinline__ void expand_one(const AdapterArgs& a, const T* w, int
     b[0] = __ldg(p), b[1] = __ldg(p + 8), b[2] = __ldg(q), b[3] = __ldg(q + 8);
   };
   begin(0);
+  h_there();
 #pragma unroll 1
   for (int u = 0; u < units; ++u) {
     const int col = col0 + 512 * u + lane;
@@ -575,9 +576,9 @@ __device__ __forceinline__ void expand_one(const AdapterArgs& a, const T* w, int
 // 2 to 16 tokens: mma.sync with h's two parts (as for many tokens), 32 columns at a time.  Column 8 (n / 2) + 2 j + n % 2 of them is column n of product j, so
 // that a lane ends with 8 consecutive columns of two tokens.
 constexpr int kAD_FewPitch = kAD_MaxRank + 8;       // from row to row of h's parts in shared memory
-template <typename T>
+template <typename T, typename F>
 __device__ __forceinline__ void expand_several(const AdapterArgs& a, const T* w, int rank, int m, const int* s_tok, const T* s_parts, const float* s_back, int col0,
-                                               int units) {
+                                               int units, F h_there) {
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   auto col_of = [&](int u) { return col0 + 512 * (u >> 1) + 32 * (u & 1); };
   uint32_t b[8];                   // product j's two values of k 0 .. 7 and 8 .. 15
@@ -592,6 +593,7 @@ __device__ __forceinline__ void expand_several(const AdapterArgs& a, const T* w,
     }
   };
   load(0, 0);
+  h_there();
 #pragma unroll 1
   for (int u = 0; u < 2 * units; ++u) {
     if (col_of(u) >= a.d_out) return;
@@ -657,39 +659,41 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
   const int r0 = a.row[id], rank = a.row[id + 1] - r0;
   const float scale = a.scale[id];
   const T* w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
-  wait_for_stream();
-  // a warp a token at a time, lane l the ranks l, l + 32, ...
-  for (int t = warp; t < m; t += 8) {
-    float v[kAD_MaxRank / 32], big = 0.f;
+  // B, and y, which is older than the kernel before this one, are on their way before h is there
+  auto h_there = [&]() {
+    wait_for_stream();
+    // a warp a token at a time, lane l the ranks l, l + 32, ...
+    for (int t = warp; t < m; t += 8) {
+      float v[kAD_MaxRank / 32], big = 0.f;
 #pragma unroll
-    for (int k = 0; k < kAD_MaxRank / 32; ++k) {
-      v[k] = 0.f;
-      const float* p = a.h + (size_t)s_tok[t] * a.rmax + 32 * k + lane;
-      if (32 * k + lane < rank) {
-#pragma unroll 8
-        for (int i = 0; i < a.splits; ++i) v[k] += p[(size_t)i * a.T * a.rmax];
-      }
-      big = fmaxf(big, fabsf(v[k]));
-    }
-    if (m == 1) {
-#pragma unroll
-      for (int k = 0; k < kAD_MaxRank / 32; ++k)
-        if (32 * k + lane < rank) s_h[32 * k + lane] = v[k];
-    } else {
-      const RowScale rs(warp_max(big));
-#pragma unroll
-      for (int k = 0; k < kAD_MaxRank / 32; ++k)
+      for (int k = 0; k < kAD_MaxRank / 32; ++k) {
+        v[k] = 0.f;
+        const float* p = a.h + (size_t)s_tok[t] * a.rmax + 32 * k + lane;
         if (32 * k + lane < rank) {
-          T* to = s_parts + t * kAD_FewPitch + 32 * k + lane;
-          rs.parts(v[k], to[0], to[16 * kAD_FewPitch]);
+#pragma unroll 8
+          for (int i = 0; i < a.splits; ++i) v[k] += p[(size_t)i * a.T * a.rmax];
         }
-      if (lane == 0) s_back[t] = scale * rs.back();
+        big = fmaxf(big, fabsf(v[k]));
+      }
+      if (m == 1) {
+#pragma unroll
+        for (int k = 0; k < kAD_MaxRank / 32; ++k)
+          if (32 * k + lane < rank) s_h[32 * k + lane] = v[k];
+      } else {
+        const RowScale rs(warp_max(big));
+#pragma unroll
+        for (int k = 0; k < kAD_MaxRank / 32; ++k)
+          if (32 * k + lane < rank) {
+            T* to = s_parts + t * kAD_FewPitch + 32 * k + lane;
+            rs.parts(v[k], to[0], to[16 * kAD_FewPitch]);
+          }
+        if (lane == 0) s_back[t] = scale * rs.back();
+      }
     }
-  }
-  // rows of tokens that are not there: anything finite or not, nobody reads their sums
-  __syncthreads();
-  if (m == 1) expand_one<T>(a, w, rank, s_tok[0], s_h, scale, col0, a.units);
-  else expand_several<T>(a, w, rank, m, s_tok, s_parts, s_back, col0, a.units);
+    __syncthreads();               // (of h's parts, rows of tokens that are not there are left as they were: nobody reads their sums)
+  };
+  if (m == 1) expand_one<T>(a, w, rank, s_tok[0], s_h, scale, col0, a.units, h_there);
+  else expand_several<T>(a, w, rank, m, s_tok, s_parts, s_back, col0, a.units, h_there);
 }
 
 // out of many tokens: tiles of a group (128 tokens) and 128 columns, group by group, an equal run of them to each SM's one CTA.  Four warps bring y's rows into
