@@ -90,7 +90,7 @@ struct SharedArgs {
   float* qs;            // [KV heads][n t R] the rows' scales
   int4* head;           // units per CTA, CTAs with one more, -, -
   SharedWay* ways;      // [n places][kSH_Ways]: the tail, then the runs
-  float* part;          // [CTAs * 128 + rows][256], a piece's rows x dims transposed
+  float* part;          // [CTAs * 128 + rows][256], a piece as [64][rows][4 dims]
   float2* ml;           // [CTAs * 128 + rows] maximum, sum
   void* o;
   float* lse;
@@ -790,15 +790,13 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         if (lane == 0) (o_free + (j & 1)).arrive();
         if (end) {
           if (r < rows) {
-            // a piece lies dim by dim, so that 32 rows are neighbours
+            // a piece lies by four dims, so that 32 rows are neighbours
             const size_t row0 = (size_t)blockIdx.x * kSH_M + base;
             if (half == 0) a.ml[row0 + r] = make_float2(m_ref, l);
-            float* to = a.part + row0 * kPG_D + (size_t)half * 128 * rows + r;
+            ulonglong2* to = reinterpret_cast<ulonglong2*>(a.part + row0 * kPG_D + (size_t)half * 128 * rows) + r;
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              *to = lo_hi(acc[i], 0);
-              to += rows;
-              *to = lo_hi(acc[i], 1);
+            for (int i = 0; i < 64; i += 2) {
+              *to = make_ulonglong2(acc[i], acc[i + 1]);
               to += rows;
             }
           }
@@ -818,7 +816,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
 // Output rows: a block has 32 neighbouring rows of one KV head, in the plan's order (they are neighbours in every piece too), and 16 dims for each of its
 // 8 / Split groups of warps; a lane has a row, and the row's pieces (tail, then its runs, CTA by CTA) are dealt to a group's
 // Split warps, whose sums are added in order.  The first warp finds where the rows' pieces lie.
-constexpr int kSH_MergeDims = 16;
+constexpr int kSH_MergeDims = 16, kSH_MergeSmem = 23552;       // bytes of static shared memory, at least
 template <typename T, int Split>
 __global__ void __launch_bounds__(256) paged_merge_kernel(SharedArgs a) {
   constexpr int Groups = 8 / Split, Ways = kSH_Ways;
@@ -873,9 +871,12 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(SharedArgs a) {
       for (int x = 0; x < Batch; ++x) {
         const size_t row0 = (size_t)(way.x + min(mine + x * Split, way.y - 1)) * kSH_M + base;
         ml[x] = a.ml[row0 + way.w];
-        const float* p = a.part + row0 * kPG_D + (size_t)d0 * way.z + way.w;
+        const float4* p = reinterpret_cast<const float4*>(a.part + row0 * kPG_D + (size_t)d0 * way.z) + way.w;
 #pragma unroll
-        for (int q = 0; q < kSH_MergeDims; ++q) v[x][q] = p[(size_t)q * way.z];
+        for (int q = 0; q < kSH_MergeDims; q += 4) {
+          const float4 y = p[(size_t)(q / 4) * way.z];
+          v[x][q] = y.x, v[x][q + 1] = y.y, v[x][q + 2] = y.z, v[x][q + 3] = y.w;
+        }
       }
 #pragma unroll
       for (int x = 0; x < Batch; ++x) {
@@ -947,7 +948,14 @@ static int launch_shared(const SharedArgs& a, int ctas, cudaStream_t stream) {
   // a row's pieces are dealt to so many warps that there are 600 to 1200 of them: with few rows the pieces' way is what takes time (whole call, 16 x 24 rows of
   // 37 pieces each: 100, 90, 85 and 86 us over 1, 2, 4 and 8), with many the blocks (64 x 24 rows of 13: 48, 52, 53 and 62)
   const unsigned blocks = (per_head + 31) / 32, warps = blocks * a.p.heads * (kPG_D / kSH_MergeDims);
-  auto merge = [&](auto kernel, int split) { return launch_early(kernel, dim3(blocks, kPG_D / kSH_MergeDims * split / 8, a.p.heads), 256, 0, stream, a); };
+  // Its CTAs come as those of the kernel before them leave their SMs: each takes so much shared memory that no SM has more than its share of them, or the
+  // first SMs that are free would take them all (16 x 131072: XX us against XX).
+  auto merge = [&](auto kernel, int split) {
+    const unsigned ctas_y = kPG_D / kSH_MergeDims * split / 8, each = (blocks * ctas_y * a.p.heads + ctas - 1) / ctas;
+    const int idle = each < 8 ? (232448 / (int)each - 1024) / 1024 * 1024 - kSH_MergeSmem : 0;
+    const int e = ensure_smem_attr((const void*)kernel, 232448 - 1024 - kSH_MergeSmem);
+    return e ? e : launch_early(kernel, dim3(blocks, ctas_y, a.p.heads), 256, idle, stream, a);
+  };
   if (warps >= 576) return merge(paged_merge_kernel<T, 1>, 1);
   if (warps >= 288) return merge(paged_merge_kernel<T, 2>, 2);
   if (warps >= 144) return merge(paged_merge_kernel<T, 4>, 4);
