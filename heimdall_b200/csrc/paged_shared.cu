@@ -107,7 +107,8 @@ struct Plan {
 
 // a piece of the line: run e, or, behind the runs, the tail of the sequence at place e - n_runs
 struct Stretch {
-  int first, rows, page0, tokens;
+  int first, rows, page0, tokens, lead;      // first place; lead: the slot whose table names its pages
+  Stretch() = default;
   __device__ __forceinline__ Stretch(const SharedArgs& a, const Plan& pl, int e) {
     if (e < pl.n_runs) {
       const int32_t* r = pl.runs + (size_t)e * kPS_Run;
@@ -115,11 +116,13 @@ struct Stretch {
       rows = r[1] * a.t * a.R;
       page0 = r[2];
       tokens = (r[3] - r[2]) << a.page_log;
+      lead = pl.slots[pl.order[first]];
     } else {
       first = e - pl.n_runs;
       const int b = pl.order[first], slot = pl.slots[b];
       rows = a.t * a.R;
       page0 = pl.skip[b];
+      lead = slot;
       tokens = slot >= 0 && slot < a.p.slots ? max(0, min(a.p.lens[slot], a.cap) - (page0 << a.page_log)) : 0;
     }
   }
@@ -254,7 +257,8 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   volatile int* abort = reinterpret_cast<volatile int*>(bars + 37);
   const Waits wait{smem_u32(bars + 37)};
   const uint32_t ring_at = smem_u32(ring), q_at = smem_u32(sQ);
-  int* s_sum = reinterpret_cast<int*>(bars + 38);      // [20][2] per-warp totals
+  int* s_sum = reinterpret_cast<int*>(bars + 38);      // [16][2] totals of the warps that scan
+  Stretch* s_first = reinterpret_cast<Stretch*>(bars + 54);       // the stretch that this CTA begins in
   int* s_start = reinterpret_cast<int*>(bars + 58);    // stretch, unit in it, rows before it
   SharedTile* s_tile = reinterpret_cast<SharedTile*>(bars + 64);  // [4]
   float2* s_ml = reinterpret_cast<float2*>(s_tile + 4);           // [4][2][128] a tile's maxima and sums, of both halves of its tokens
@@ -287,15 +291,17 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   }
   if (warp == 2 && lane == 0) tma_prefetch(&vmap);
   let_next_start();
-  // this CTA's part of the line: the stretches' units summed over the block, thread i holding `per` consecutive ones.  (The plan and the lengths are
-  // older than the kernel before this one, which began by waiting for what was before it.)
+  // this CTA's part of the line: the stretches' units summed over the warps of softmax and accumulators, thread i holding `per` consecutive ones.  (The plan and
+  // the lengths are older than the kernel before this one, which began by waiting for what was before it.)
+  constexpr int kScan = kSH_Threads - 128;
   const Plan pl(a.plan, a.n);
-  const int stretches = pl.n_runs + a.n, per = (stretches + kSH_Threads - 1) / kSH_Threads;
+  const int stretches = pl.n_runs + a.n, per = (stretches + kScan - 1) / kScan, e0 = (tid - 128) * per;
+  Stretch mine0;                       // thread's first
   int2 mine = make_int2(0, 0);
-  for (int i = 0; i < per; ++i) {
-    const int e = tid * per + i;
-    if (e < stretches) {
-      const Stretch x(a, pl, e);
+  if (warp >= 4) {
+    for (int i = 0; i < per && e0 + i < stretches; ++i) {
+      const Stretch x(a, pl, e0 + i);
+      if (i == 0) mine0 = x;
       mine.x += x.units(a.p.heads);
       mine.y += x.rows * a.p.heads;
     }
@@ -309,29 +315,54 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
       incl.y += y;
     }
   }
-  if (lane == 31) {
-    s_sum[2 * warp] = incl.x;
-    s_sum[2 * warp + 1] = incl.y;
+  if (warp >= 4 && lane == 31) {
+    s_sum[2 * (warp - 4)] = incl.x;
+    s_sum[2 * (warp - 4) + 1] = incl.y;
   }
   __syncthreads();
-  int total = lane < kSH_Threads / 32 ? s_sum[2 * lane] : 0;
-  const int rows_w = lane < kSH_Threads / 32 ? s_sum[2 * lane + 1] : 0;
-  int2 before = make_int2(lane < warp ? total : 0, lane < warp ? rows_w : 0);
+  int total = lane < kScan / 32 ? s_sum[2 * lane] : 0;
+  const int rows_w = lane < kScan / 32 ? s_sum[2 * lane + 1] : 0;
+  int2 before = make_int2(lane < warp - 4 ? total : 0, lane < warp - 4 ? rows_w : 0);
   total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
   before.x = (int)__reduce_add_sync(0xffffffffu, (unsigned)before.x) + incl.x - mine.x;
   before.y = (int)__reduce_add_sync(0xffffffffu, (unsigned)before.y) + incl.y - mine.y;
   const int ctas = max(1, min(total, (int)gridDim.x)), each = total / ctas, more = total - each * ctas;
   const int u0 = min((int)blockIdx.x, ctas) * each + min((int)blockIdx.x, more);
   const int u1 = u0 + ((int)blockIdx.x < ctas ? each + ((int)blockIdx.x < more ? 1 : 0) : 0);
+  if (warp >= 4 && u0 < u1 && before.x <= u0 && u0 < before.x + mine.x) {
+    int2 at = before;
+    for (int i = 0; i < per && e0 + i < stretches; ++i) {
+      const Stretch x = i == 0 ? mine0 : Stretch(a, pl, e0 + i);
+      const int units = x.units(a.p.heads);
+      if (at.x <= u0 && u0 < at.x + units) {
+        s_start[0] = e0 + i;
+        s_start[1] = u0 - at.x;
+        s_start[2] = at.y;
+        *s_first = x;
+      }
+      at.x += units;
+      at.y += x.rows * a.p.heads;
+    }
+  }
   wait_for_stream();
-  {
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  if (warp >= 4) {
+    // for paged_merge_kernel: every CTA writes some stretches' part
     int2 at = before;
     for (int i = 0; i < per; ++i) {
-      const int e = tid * per + i;
+      const int e = e0 + i;
       if (e >= stretches) break;
-      const Stretch x(a, pl, e);
-      const int units = x.units(a.p.heads);
-      if (e % (int)gridDim.x == (int)blockIdx.x) {      // for paged_merge_kernel: every CTA writes some stretches' part
+      const bool here = e % (int)gridDim.x == (int)blockIdx.x;
+      if (!here && per == 1) break;
+      const Stretch x = i == 0 ? mine0 : Stretch(a, pl, e);
+      if (here) {
         const bool run = e < pl.n_runs;
         const int32_t* r = pl.runs + (size_t)e * kPS_Run;
         const int k = run ? 1 + r[5] : 0, many = run ? r[1] : 1, tiles = x.tiles();
@@ -345,24 +376,12 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
           for (int i = last >= 0 ? 2 + pl.runs[(size_t)last * kPS_Run + 5] : 1; i < kSH_Ways; ++i) a.ways[(size_t)x.first * kSH_Ways + i].tiles = 0;
         }
       }
-      if (u0 < u1 && at.x <= u0 && u0 < at.x + units) {
-        s_start[0] = e;
-        s_start[1] = u0 - at.x;
-        s_start[2] = at.y;
-      }
-      at.x += units;
+      at.x += x.units(a.p.heads);
       at.y += x.rows * a.p.heads;
     }
-    if (blockIdx.x == 0 && tid == 0) *a.head = make_int4(each, more, 0, 0);
+    if (blockIdx.x == 0 && tid == 128) *a.head = make_int4(each, more, 0, 0);
+    __syncwarp();
   }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int L = a.p.page, ppt = kSH_N >> a.page_log, per_seq = a.t * a.R;
   bool ok = true;
   // every role: wait for tile j's entry (false: no more tiles, or a wait gave up)
@@ -380,10 +399,10 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         int e = s_start[0], base = s_start[2], in = s_start[1];
 #pragma unroll 1
         for (; e < stretches && unit < u1 && ok; ++e) {
-          const Stretch x(a, pl, e);
+          const Stretch x = e == s_start[0] ? *s_first : Stretch(a, pl, e);
           const int ntiles = x.tiles(), len = ntiles + kSH_Start, blocks = x.blocks(), n_items = x.tokens > 0 ? a.p.heads * blocks : 0;
-          const int lead = pl.slots[pl.order[x.first]], pages = (x.tokens + L - 1) >> a.page_log;
-          const int32_t* table = a.p.table + (size_t)max(lead, 0) * a.p.width + x.page0;
+          const int pages = (x.tokens + L - 1) >> a.page_log;
+          const int32_t* table = a.p.table + (size_t)max(x.lead, 0) * a.p.width + x.page0;
           int item = in / len;
           in -= item * len;
 #pragma unroll 1
@@ -949,7 +968,7 @@ static int launch_shared(const SharedArgs& a, int ctas, cudaStream_t stream) {
   // 37 pieces each: 100, 90, 85 and 86 us over 1, 2, 4 and 8), with many the blocks (64 x 24 rows of 13: 48, 52, 53 and 62)
   const unsigned blocks = (per_head + 31) / 32, warps = blocks * a.p.heads * (kPG_D / kSH_MergeDims);
   // Its CTAs come as those of the kernel before them leave their SMs: each takes so much shared memory that no SM has more than its share of them, or the
-  // first SMs that are free would take them all (16 x 131072: XX us against XX).
+  // first SMs that are free would take them all (16 x 131072: 84 us against 93).
   auto merge = [&](auto kernel, int split) {
     const unsigned ctas_y = kPG_D / kSH_MergeDims * split / 8, each = (blocks * ctas_y * a.p.heads + ctas - 1) / ctas;
     const int idle = each < 8 ? (232448 / (int)each - 1024) / 1024 * 1024 - kSH_MergeSmem : 0;
