@@ -643,6 +643,10 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
         if (!whole) {
           // the values of tokens that are not there may be anything (a weight of 0 times NaN would be NaN): zeros
           const int n = 2 * j + hh, u = n % NV;
+          // half n - NV was in this place before, of tile j - 2 (four places) or j - 1 (three): while it is on its way, a wait for half n would take n - 2 NV
+          // for it.  (The products of tile j - 3 are done: the scores of tile j - 1 were there.)
+          constexpr int kBefore = NV < 4 ? 1 : 2;
+          if (j >= kBefore && !(ok = wait(p_free + ((j - kBefore) & 1), ((j - kBefore) >> 1) & 1, 0xa4))) break;
           if (!(ok = wait(v_full + u, (n / NV) & 1, 0x9c))) break;
           if (r >= valid || !((have >> (r >> a.page_log)) & 1u)) {
             uint4* row = reinterpret_cast<uint4*>(ring + (NK + u) * kSH_Unit + r * 128);

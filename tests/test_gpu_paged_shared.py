@@ -9,6 +9,8 @@ So |o - o*| <= (u + w + 2^-12 S + 2 E + 2^-18) A + 2^-11 max|v| with w = 2^-9 + 
 2^-16 (1 + |lse*|).  The term 2^-11 max|v| is a bound on what 128 roundings of one sign could do; that they do not add up so is the second check: the
 error's 2-norm stays below (u + w) of A's.  (Not of the output's: every term of the first bound is in units of A, and where a value of -1 of weight 0.503
 stands against thousands of +1, u |o| + w A with |o| = 0.007 and A = 1 is 0.0025, 60 times (u + w) |o|.)"""
+import random
+
 import pytest
 import torch
 
@@ -303,6 +305,44 @@ def test_replayed_with_a_plan_that_has_no_runs():
     plan.slots[1] = plan.slots[0]
     o[1], lse[1], q[1] = o[0], lse[0], q[0]
     _check_out(c, plan, q.cpu(), o, lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_same_bits_again_and_again(dtype):
+    """Ends of tiles, where what the pages hold behind a sequence (NaN here) is blotted out while the values of the tile before may still be on their way."""
+    rng = random.Random(7)
+    for tree in range(60):
+        page, G, R, t = rng.choice([16, 32, 64, 128]), rng.choice([1, 2, 4]), rng.choice([1, 2, 6, 8, 24]), rng.choice([1, 1, 1, 2, 5])
+        docs = [rng.choice([0, page, rng.randint(0, 600)]) for _ in range(rng.randint(1, 4))]
+        ways = [rng.randint(1, 9) for _ in docs]
+        c, slots = _tree(page, rng.choice([page, rng.randint(page, 1500)]), docs, ways, [rng.randint(0, 300) for _ in range(sum(ways))], G)
+        plan = c.share(slots, min_saved=1)
+        q = _rand(len(slots), t, G * R, D, seed=tree, dtype=dtype)
+        if not plan.runs:
+            continue
+        calls = [c.attend(0, q.cuda(), shared=plan, with_lse=True) for _ in range(24)]
+        for o, lse in calls:
+            assert torch.equal(o, calls[0][0]) and torch.equal(lse, calls[0][1]), tree
+        if tree % 10 == 0:
+            _check_out(c, plan, q, *calls[0])
+
+
+@pytest.mark.parametrize("page,common,docs,ways,R,t,tails,slots", [
+    (32, 1095, [159, 441, 0], [3, 9, 9], 24, 5, [3, 181, 105, 175, 10, 2, 190, 3, 3, 103, 0, 231, 3, 0, 2, 42, 0, 2, 3, 3, 3],
+     [16, 11, 5, 8, 14, 2, 13, 12, 6, 7, 1, 17, 10, 15, 4, 19, 3, 0, 18, 20, 9]),
+    (128, 128, [232, 128, 215, 358], [6, 9, 3, 8], 1, 1,
+     [0, 1, 111, 171, 0, 3, 83, 129, 0, 276, 1, 288, 12, 2, 2, 2, 0, 245, 1, 260, 5, 0, 2, 38, 51, 2],
+     [14, 11, 5, 16, 0, 19, 21, 4, 6, 3, 7, 10, 12, 15, 2, 8, 25, 13, 9, 22, 23, 17, 20, 18, 24, 1])])
+def test_values_of_the_tile_before_on_their_way(page, common, docs, ways, R, t, tails, slots):
+    """Two batches whose last tiles were blotted out too early (the values behind a sequence came after it) in one call of some tens."""
+    c, _ = _tree(page, common, docs, ways, tails, 4)
+    plan = c.share(slots, min_saved=100)
+    q = _rand(len(slots), t, 4 * R, D, dtype=torch.float16)
+    calls = []
+    for _ in range(300):
+        calls = calls[:1] + [c.attend(0, q.cuda(), shared=plan, with_lse=True)]
+        assert torch.equal(calls[-1][0], calls[0][0]) and torch.equal(calls[-1][1], calls[0][1])
+    _check_out(c, plan, q, *calls[0])
 
 
 def test_refused_calls():
