@@ -248,7 +248,8 @@ def heads_16bit(name: str, t):
         raise NotImplementedError(f"{name} is {t.dtype}: built for bfloat16 and float16")
     at, st = t.data_ptr(), t.stride()
     if at % 16 == 0 and t.shape[-1] % 8 == 0 and t.is_contiguous():
-        return t, at, list(st[:-1])
+        # (contiguous says nothing of the strides of dimensions of one: those of a row cut out of a wider one can be any)
+        return t, at, [s if n > 1 else 0 for s, n in zip(st[:-1], t.shape)]
     ok = st[-1] == 1 and at % 16 == 0
     out = []
     for s, n in zip(st[:-1], t.shape):
