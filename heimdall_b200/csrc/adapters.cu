@@ -665,6 +665,7 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
     // a warp a token at a time, lane l the ranks l, l + 32, ...
     for (int t = warp; t < m; t += 8) {
       float v[kAD_MaxRank / 32], big = 0.f;
+      bool finite = true;
 #pragma unroll
       for (int k = 0; k < kAD_MaxRank / 32; ++k) {
         v[k] = 0.f;
@@ -674,11 +675,14 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
           for (int i = 0; i < a.splits; ++i) v[k] += p[(size_t)i * a.T * a.rmax];
         }
         big = fmaxf(big, fabsf(v[k]));
+        finite = finite && fabsf(v[k]) < INFINITY;
       }
       if (m == 1) {
+        // NaN for all ranks where one is not finite, as the parts of several tokens give it
+        finite = __all_sync(0xffffffffu, finite);
 #pragma unroll
         for (int k = 0; k < kAD_MaxRank / 32; ++k)
-          if (32 * k + lane < rank) s_h[32 * k + lane] = v[k];
+          if (32 * k + lane < rank) s_h[32 * k + lane] = finite ? v[k] : NAN;
       } else {
         const RowScale rs(warp_max(big));
 #pragma unroll

@@ -226,3 +226,29 @@ def test_layer_with_adapters():
         with pytest.raises(ValueError):
             A.project(x, 0, adapter_ids=bad)
     assert torch.equal(A.project(x, 0, adapter_ids=ids.int())[5], A.project(x, 0, adapter_ids=ids[:, None].expand(3, 90))[5])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,rank", [(1, 16), (1, 3), (24, 16), (24, 48), (300, 16)])
+def test_a_token_alone_with_its_adapter_that_is_not_finite(T, rank, dtype):
+    """A x of infinities, or of sums beyond fp32, makes the whole row NaN, as it does beside other tokens of the adapter.  (Weights of one sign: infinities
+    of both signs would become NaN by themselves.)"""
+    from heimdall_b200 import Adapters
+    _, a, b, s = _make([rank] * T, 64, 48, dtype)
+    a, b = [t.abs() + 2.0 ** -6 for t in a], [t.abs() + 2.0 ** -6 for t in b]
+    ad = Adapters(a, b, s)
+    x, y = _data(T, 64, 48, dtype)
+    ids = torch.arange(T).cuda()
+    clean = ad.add(y, x, ids)
+    for row, value in ((T // 2, float("nan")), (T - 1, -float("inf")), (0, float("inf"))):
+        x[row, 5] = value
+    bad = sorted({0, T // 2, T - 1})
+    got = ad.add(y, x, ids)
+    assert got[bad].isnan().all()
+    rest = [t for t in range(T) if t not in bad]
+    assert torch.equal(got[rest], clean[rest])
+    if dtype == torch.bfloat16:                  # finite values whose A x is beyond fp32
+        x, y = _data(T, 64, 48)
+        x[0] = 3e38
+        got = Adapters([16 * t + 1 for t in a], b, s).add(y, x, ids)
+        assert got[0].isnan().all() and got[1:].isfinite().all()
