@@ -145,20 +145,25 @@ class PageTable:
 
 class SharedPages:
     """Which pages the sequences of a batch have in common (``PagedKV.share``): ``slots``, in the order of the batch, and ``runs``, the number of
-    page runs that are read once for several sequences."""
+    page runs that are read once for several sequences.  A plan does not keep its cache: ``cache`` is None once that is gone."""
 
     def __init__(self, cache: "PagedKV", slots: np.ndarray, plan: np.ndarray):
-        self.cache = cache
+        self._cache = weakref.ref(cache)         # the cache has plans of its own: with references both ways the pool would wait for the cycle collector
+        self._page = cache.page
         self.n = slots.size
         self.plan = torch.empty(plan.size, dtype=torch.int32, device=cache.device)
         self._slot_ids = self.plan[4:4 + self.n]
         self._fill(slots, plan)
         cache._plans.add(self)
 
+    @property
+    def cache(self):
+        return self._cache()
+
     def _fill(self, slots: np.ndarray, plan: np.ndarray) -> None:
         self.slots, self.runs, self.good = slots.tolist(), int(plan[0]), True
         # the tokens of each slot that are read as shared pages
-        self._covered = dict(zip(self.slots, (plan[4 + 4 * self.n:4 + 5 * self.n] * self.cache.page).tolist()))
+        self._covered = dict(zip(self.slots, (plan[4 + 4 * self.n:4 + 5 * self.n] * self._page).tolist()))
         self.plan.copy_(torch.from_numpy(plan))
 
     def _cut(self, slots, lens) -> None:

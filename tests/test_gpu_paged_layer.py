@@ -188,3 +188,25 @@ def test_appends_of_nothing_leave_no_doubt():
     none()
     _teacher(qr, kr, v, layer, None)
     assert c.lens.tolist() == [3, 3] and layer.n == 3
+
+
+def test_a_cache_ends_with_its_last_reference():
+    """Plans of shared pages, the layers' own and the caller's, do not keep the pool: it is freed at once, not when cycles are collected."""
+    import gc
+    import weakref
+    c = _cache(1, 4)
+    qr, kr, v = _qkv(4, 40, 1)
+    _teacher(qr, kr, v, c.layer(0), None)
+    qr, kr, v = _qkv(4, 1, 2)
+    _teacher(qr, kr, v, c.layer(0, share=True), None)
+    plan = c.share(range(4), min_saved=1)
+    assert c._layer_plans and plan.cache is c
+    gone = weakref.ref(c)
+    gc.disable()
+    try:
+        del c
+        assert gone() is None and plan.cache is None
+    finally:
+        gc.enable()
+    with pytest.raises(ValueError, match="plan of this cache"):
+        _cache(1, 4).attend(0, qr.transpose(1, 2), shared=plan)

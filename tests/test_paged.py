@@ -342,3 +342,27 @@ def test_c_entry_of_shared_attend_refuses(code, kw):
         _lib.call("bf_paged_attend_shared", ctypes.addressof(pool), 0, a["q"], 256, 256, 256, a["plan"], a["n"], a["t"], a["H"], a["dtype"],
                   a["scale"], 16, 0, a["ws"], a["nws"], 0)
     assert e.value.code == code
+
+
+def test_a_plan_does_not_keep_its_cache():
+    import types
+    import weakref
+    from heimdall_b200.paged import SharedPages
+    t = PageTable(40, 3, 16, 20)
+    t.reserve([0], [70])
+    t.fork([0, 0], [1, 2])
+
+    class Cache(types.SimpleNamespace):
+        __hash__ = object.__hash__
+    cache = Cache(device="cpu", page=16, _plans=weakref.WeakSet())
+    s = t._whole([2, 0, 1])
+    plan = SharedPages(cache, s, t.share(s, 1))
+    assert plan.cache is cache and list(cache._plans) == [plan] and (plan.runs, plan.slots, plan.n) == (1, [2, 0, 1], 3)
+    plan._cut([1, 2], [64, 65])
+    assert plan.good
+    plan._cut([1, 2], [64, 63])
+    assert not plan.good
+    plan._fill(s, t.share(s, 1))
+    assert plan.good
+    del cache
+    assert plan.cache is None
