@@ -167,7 +167,7 @@ class SharedPages:
         self.plan.copy_(torch.from_numpy(plan))
 
     def _cut(self, slots, lens) -> None:
-        if any(n < self._covered.get(s, 0) for s, n in zip(slots, lens)):
+        if self.good and any(n < self._covered.get(s, 0) for s, n in zip(slots, lens)):
             self.good = False
 
 

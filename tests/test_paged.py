@@ -366,3 +366,24 @@ def test_a_plan_does_not_keep_its_cache():
     assert plan.good
     del cache
     assert plan.cache is None
+
+
+def test_a_plan_that_is_no_longer_good_is_not_looked_through_again():
+    import types
+    import weakref
+    from heimdall_b200.paged import SharedPages
+    t = PageTable(40, 2, 16, 20)
+    t.reserve([0], [70])
+    t.fork([0], [1])
+
+    class Cache(types.SimpleNamespace):
+        __hash__ = object.__hash__
+    cache, s = Cache(device="cpu", page=16, _plans=weakref.WeakSet()), t._whole([0, 1])
+    plan = SharedPages(cache, s, t.share(s, 1))
+    plan._cut([1], [63])
+    assert not plan.good
+    plan._cut(None, None)                        # (would raise)
+    plan._fill(s, t.share(s, 1))
+    assert plan.good
+    plan._cut([0], [0])
+    assert not plan.good
