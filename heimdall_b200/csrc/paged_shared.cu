@@ -708,7 +708,8 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
 #pragma unroll 1
           for (int c = c0; c < c0 + 64; c += 16) {
             const int pi = c >> a.page_log;
-            const float f = d.ks[pi] * qs, off = d.e[pi] + ref;
+            // (never 0, which would make NaN of the -infinity of what the row does not see; 2^25 times 1e-38 is nothing to a score)
+            const float f = fmaf(d.ks[pi], qs, 1e-38f), off = d.e[pi] + ref;
             const uint64_t f2 = pair2(f, f), off2 = pair2(off, off);
             float w[16];
 #pragma unroll

@@ -357,3 +357,15 @@ def test_refused_calls():
         with pytest.raises(ValueError):
             bad()
     assert c.attend(0, q[:, :0], shared=plan)[0].shape == (3, 0, 4, D)
+
+
+@pytest.mark.parametrize("t,dtype", [(1, torch.bfloat16), (3, torch.float16)])
+def test_scores_below_what_fp32_holds(t, dtype):
+    """Scales and queries so small that every score is 0: what a row does not see still has no weight, and all the others are alike."""
+    c, slots = _tree(32, 200, [0], [3], [t, t + 40, t + 3], 2)
+    plan = c.share(slots, min_saved=1)
+    _check(c, plan, _rand(3, t, 4, D, seed=14, dtype=dtype), scale=1e-44)
+    q = _rand(3, t, 4, D, seed=15, dtype=dtype) * 2.0 ** (-100 if dtype == torch.bfloat16 else -20)
+    q[0] = 0
+    c.k_scale[c.k_scale.isfinite()] = 2.0 ** -64       # the scale of pages of zeros, and the smallest there is
+    _check(c, plan, q, scale=1e-20)
