@@ -442,7 +442,10 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
               int ex = 0;
               if (there) {
                 ks = a.p.ks[(size_t)page * a.p.heads + g];
-                ex = max((int)(__float_as_uint(a.p.vs[(size_t)page * a.p.heads + g]) >> 23) - 127, -120);      // scales are powers of two
+                // scales are powers of two, 2^-64 at least; 0 where nothing was written, whose codes are 0 too: any scale does, but its inverse times 2^8,
+                // summed over the tokens, has to stay in fp32
+                const int e8 = (int)(__float_as_uint(a.p.vs[(size_t)page * a.p.heads + g]) >> 23);
+                ex = e8 ? max(e8 - 127, -110) : -64;
               }
               if (j >= 4 && !(ok = wait(t_free + (j & 3), ((j >> 2) - 1) & 1, 0x92))) break;
               SharedTile* d = s_tile + (j & 3);

@@ -369,3 +369,12 @@ def test_scores_below_what_fp32_holds(t, dtype):
     q[0] = 0
     c.k_scale[c.k_scale.isfinite()] = 2.0 ** -64       # the scale of pages of zeros, and the smallest there is
     _check(c, plan, q, scale=1e-20)
+
+
+def test_pages_that_nothing_was_written_to():
+    """Scales of 0 and codes of 0, as in a call made before the first append: zeros, each token with the same weight."""
+    c = _cache(1, 20, 1, 3, page=32, max_len=320)
+    c.reserve([0], 200)
+    c.fork([0, 0], [1, 2])
+    c.reserve([0, 1, 2], [1, 70, 2])
+    _check(c, c.share([0, 1, 2], min_saved=1), _rand(3, 1, 4, D, seed=16))
