@@ -169,3 +169,20 @@ def test_layer_with_positions_on_several_axes():
     assert y.shape == (2, 50, 512) and y.isfinite().all()
     with pytest.raises(ValueError):
         BifrostAttention(pp.q_w, pp.k_w, pp.v_w, pp.o_w, pp.q_norm_w, pp.k_norm_w, L, pp.rot, pp.theta, pp.eps, pp.gated, rope_sections=(11, 11, 11))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("F,memory", [(32, True), (32, False), (8, True), (64, False), (0, True)])
+def test_infinities_reach_what_the_formula_says(F, memory, dtype):
+    """An infinity makes its own dim NaN, its partner where both are turned, and the rest of its head 0."""
+    from heimdall_b200 import norm_rope_heads
+    args = _inputs(1, 3, 2, 1, F, 1, dtype=dtype)
+    for t, at in enumerate((3, 200, 2 * F)):
+        args[0][0, t, 0, at] = float("inf")
+    args[1][0, 1, 0, 255] = -float("inf")
+    out = norm_rope_heads(*args[:5], args[5] if F else None, axes=args[6] or None, memory=memory)
+    for x, w, plain, turned in ((args[0][..., :D], args[2], out[0], out[2]), (args[1], args[3], out[1], out[3])):
+        y, o, size = _formula(x, w, args[4], args[5], args[6])
+        for got, want, mag in ((turned, o, size),) + (((plain, y, y.abs()),) if memory else ()):
+            assert torch.equal(got.isnan(), want.isnan())
+            _check(got[~got.isnan()], want[~want.isnan()], mag[~want.isnan()])
