@@ -225,9 +225,12 @@ extern "C" int bf_norm_rope(const void* qg, long long q_sb, long long q_st, long
   }
   if (B == 0 || T == 0) return BF_OK;
   if (!qg || !kl || !q_norm_w || !k_norm_w || !qr || !kr || (freqs > 0 && (!inv_freq || !pos))) return BF_ERR_INVALID_ARGUMENT;
-  const void* ptrs[] = {qg, kl, q_norm_w, k_norm_w, q, k, qr, kr};
+  const void* ptrs[] = {qg, kl, q, k, qr, kr};
   for (const void* p : ptrs)
     if (!aligned16(p)) return BF_ERR_ALIGNMENT;
+  // these are read one at a time
+  const auto off = [](const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; };
+  if (off(q_norm_w, 4) || off(k_norm_w, 4) || off(inv_freq, 4) || off(pos, pos64 ? 8 : 4)) return BF_ERR_ALIGNMENT;
   if ((q_sb | q_st | q_sh | k_sb | k_st | k_sh) & 7) return BF_ERR_ALIGNMENT;
   DeviceState st;
   const int rc = device_state(&st);

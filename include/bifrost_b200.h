@@ -267,7 +267,8 @@ int bf_attn_epilogue(const float* o, const void* qg, int gated, int B, int T, in
  *   bytes: the axis of each frequency, below n_axes (1 to 4); pos [n_axes,B,T] int32, or int64 when pos64
  *   -> y = x rsqrt(mean x^2 + eps) (1 + w); q [B,T,H,D], k [B,T,G,D] (y, both NULL: not written); qr [B,H,T,D], kr [B,G,T,D]
  *   (y with dims f and f + freqs turned by the angle pos[axes[f]] * inv_freq[f]), contiguous, each rounded to dtype once.  The
- *   angle is computed in 64 bits.  D = 256, freqs a multiple of 8, at most 128.
+ *   angle is computed in 64 bits.  D = 256, freqs a multiple of 8, at most 128.  The heads are 16-byte aligned; weights, frequencies
+ *   and positions as their type.
  */
 int bf_norm_rope(const void* qg, long long q_sb, long long q_st, long long q_sh, const void* kl, long long k_sb, long long k_st,
                  long long k_sh, const float* q_norm_w, const float* k_norm_w, const float* inv_freq, int freqs,

@@ -186,3 +186,14 @@ def test_infinities_reach_what_the_formula_says(F, memory, dtype):
         for got, want, mag in ((turned, o, size),) + (((plain, y, y.abs()),) if memory else ()):
             assert torch.equal(got.isnan(), want.isnan())
             _check(got[~got.isnan()], want[~want.isnan()], mag[~want.isnan()])
+
+
+def test_weights_and_positions_on_any_boundary():
+    """The norm weights, the frequencies and the positions may begin anywhere in a larger buffer."""
+    from heimdall_b200 import norm_rope_heads
+    args = _inputs(2, 5, 4, 2, 32, 3)
+    want = norm_rope_heads(*args[:6], axes=args[6])
+    off = [torch.cat([z.new_zeros(1), z.reshape(-1)])[1:].view(z.shape) for z in args[2:6]]
+    assert off[0].data_ptr() % 16 and off[2].is_contiguous()
+    for a, b in zip(norm_rope_heads(*args[:2], *off, axes=args[6]), want):
+        assert torch.equal(a, b)

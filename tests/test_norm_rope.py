@@ -42,3 +42,13 @@ def test_c_entry_refuses(code, kw):
 def test_c_entry_takes_no_tokens():
     _call(T=0, qg=0, kl=0)
     _call(B=0)
+
+
+@pytest.mark.parametrize("kw", [{"w": 18}, {"pos": 18}, {"pos": 20, "pos64": 1}])
+def test_c_entry_refuses_what_is_not_on_its_types_boundary(kw):
+    a = dict(w=20, pos=20, pos64=0)
+    a.update(kw)
+    with pytest.raises(_lib.BifrostError) as e:
+        _lib.call("bf_norm_rope", 16, 0, 0, 256, 16, 0, 0, 256, a["w"], a["w"], 20, 8, bytes(8), 1, a["pos"], a["pos64"], 1e-6, 1, 1, 1, 1, 256, 1,
+                  16, 16, 16, 16, 0)
+    assert e.value.code == 3
