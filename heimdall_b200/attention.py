@@ -78,16 +78,21 @@ class BifrostAttention:
         return self.adapters[name].add(y, x, ids, out=y)
 
     def _ids(self, x, ids):
-        """Adapter ids [B] or [B,t] as int32 [B,t], once for all projections (numbers above 31 bits name no adapter either)."""
-        if ids is None or not self.adapters:
+        """Adapter ids [B] or [B,t] as int32 [B,t], once for all projections (numbers above 31 bits name no adapter either); None where the layer
+        has no adapters."""
+        if ids is None:
             return None
+        if ids.dtype not in (torch.int32, torch.int64):
+            raise ValueError("adapter_ids must be int32 or int64")
         if ids.dim() == 1 and ids.shape[0] == x.shape[0]:
             ids = ids[:, None].expand(x.shape[:2])
         if ids.shape != x.shape[:2]:
             raise ValueError("adapter_ids must be [B] or [B,t]")
+        if not self.adapters:
+            return None
         if ids.dtype == torch.int64:
             ids = ids.clamp(-1, 2 ** 31 - 1)
-        return ids.to(device=x.device, dtype=torch.int32).contiguous() if ids.dtype in (torch.int32, torch.int64) else ids
+        return ids.to(device=x.device, dtype=torch.int32).contiguous()
 
     def project(self, x, start: int = 0, positions=None, adapter_ids=None):
         """``HybridAttention._proj`` (heimdall/hibrit.py:254-268): x [B,t,d] -> (q, k, v, qr, kr, qg) with q

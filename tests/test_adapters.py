@@ -48,3 +48,19 @@ def test_workspace_and_no_tokens():
     assert size(0, 2, 64, 16) == size(4, 4097, 64, 16) == size(4, 2, 64, 144) == 0
     assert size(64, 61, 5120, 32) >= 5 * 64 * 32 * 4
     assert size(8192, 4, 5120, 64) >= 8192 * 64 * 4 + 8192 * 4
+
+
+@pytest.mark.parametrize("adapters", [{}, {"q": None}])
+def test_adapter_ids_are_checked_with_and_without_adapters(adapters):
+    from heimdall_b200 import BifrostAttention
+    layer = BifrostAttention.__new__(BifrostAttention)
+    layer.adapters = adapters
+    x = torch.zeros(3, 90, 8)
+    for bad in (torch.zeros(2), torch.zeros(2, dtype=torch.int64), torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3), torch.zeros(3, 90, dtype=torch.bool)):
+        with pytest.raises(ValueError, match="adapter_ids"):
+            layer._ids(x, bad)
+    ids = torch.tensor([2 ** 40, -1, 2])
+    got = layer._ids(x, ids)
+    assert layer._ids(x, None) is None and (got is None) == (not adapters)
+    if adapters:
+        assert got.dtype == torch.int32 and got.is_contiguous() and got[:, 7].tolist() == [2 ** 31 - 1, -1, 2]
