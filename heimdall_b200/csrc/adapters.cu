@@ -93,9 +93,10 @@ struct FewSmem {
   unsigned leads[8];
   int first, nth;
 };
+template <bool Early>        // before the wait: past L1
 __device__ __forceinline__ int few_group(const AdapterArgs& a, int x, int* s_tok, FewSmem& s, int& id) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int mine = tid < a.T ? adapter_of(a, a.ids[tid]) : -1;
+  const int mine = tid < a.T ? adapter_of(a, Early ? __ldcg(a.ids + tid) : a.ids[tid]) : -1;
   reinterpret_cast<int*>(s.id)[tid] = mine;
   if (tid == 0) s.first = -1;
   __syncthreads();
@@ -138,11 +139,10 @@ __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(AdapterArgs a) 
   __shared__ int s_tok[16];
   __shared__ FewSmem s_few;
   __shared__ float s_sum[8][16][17];
-  wait_for_stream();
-  let_next_start();        // only now: what the next kernel reads before its own wait is older than this one
+  wait_then_let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   int id;
-  const int m = few_group(a, blockIdx.x, s_tok, s_few, id);
+  const int m = few_group<false>(a, blockIdx.x, s_tok, s_few, id);
   if (m == 0 || id == a.n) return;
   const int r0 = a.row[id], rank = a.row[id + 1] - r0, rc = blockIdx.z * 16;
   if (rc >= rank) return;
@@ -318,8 +318,7 @@ __global__ void __launch_bounds__(416, 1) adapter_shrink_kernel(AdapterArgs a) {
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_last;
   volatile int* abort = &s_abort;
-  wait_for_stream();
-  let_next_start();
+  wait_then_let_next_start();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int spg = (a.d_in + kAD_Step - 1) / kAD_Step;
   const long long total = (long long)a.n_groups[1] * spg, ctas = max(1ll, min((long long)kAD_Ctas, total / kAD_MinSteps));
@@ -641,9 +640,13 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   let_next_start();
   int id;
-  // the ids are older than the kernel before this one, which began by waiting for what was before it
-  const int m = few_group(a, blockIdx.x, s_tok, s_few, id);
-  if (m == 0 || (id == a.n && a.out == a.y)) return;
+  // ids and y are older than the kernel before this one (launch_early.h; y past L1 takes 0.2 us more of 64 tokens' 20)
+  if (tid == 255) acquire_early(a.ids);
+  const int m = few_group<true>(a, blockIdx.x, s_tok, s_few, id);
+  if (m == 0 || (id == a.n && a.out == a.y)) {
+    if (blockIdx.x == 0) wait_for_stream();
+    return;
+  }
   const int col0 = blockIdx.y * a.units * 512 + warp * 64;
   if (id == a.n) {
     wait_for_stream();
@@ -659,7 +662,7 @@ __global__ void __launch_bounds__(256, 3) adapter_expand_few_kernel(AdapterArgs 
   const int r0 = a.row[id], rank = a.row[id + 1] - r0;
   const float scale = a.scale[id];
   const T* w = static_cast<const T*>(a.B) + (long long)r0 * a.d_out;
-  // B, and y, which is older than the kernel before this one, are on their way before h is there
+  // B, and y, which is older than the kernel before this one (launch_early.h), are on their way before h is there
   auto h_there = [&]() {
     wait_for_stream();
     // a warp a token at a time, lane l the ranks l, l + 32, ...
@@ -749,9 +752,9 @@ __global__ void __launch_bounds__(448, 1) adapter_expand_kernel(AdapterArgs a) {
     fence_barrier_init();
   }
   __syncthreads();
-  // y and the groups are older than the kernel before this one, which began by waiting for what was before it
+  // y and the groups are older than the kernel before this one: warps 0 to 3 read them before the others' wait is over (launch_early.h)
   const int tpg = (a.d_out + kAD_Tile - 1) / kAD_Tile;
-  const long long total = (long long)*a.n_groups * tpg;
+  const long long total = (long long)__ldcg(a.n_groups) * tpg;
   const long long first = total * blockIdx.x / gridDim.x;
   const int n = (int)(total * (blockIdx.x + 1) / gridDim.x - first), g0 = (int)(first / tpg), c0 = (int)(first - (long long)g0 * tpg);
   bool ok = true;
@@ -762,9 +765,9 @@ __global__ void __launch_bounds__(448, 1) adapter_expand_kernel(AdapterArgs a) {
 #pragma unroll 1
     for (int j = 0, g = g0, c = c0; j < n; ++j) {
       if (j == 0 || c == 0) {
-        const int4 grp = a.groups[g];
+        const int4 grp = __ldcg(a.groups + g);
         m = grp.z;
-        if (r < m) src = static_cast<const T*>(a.y) + (long long)a.perm[grp.y + r] * a.y_st;
+        if (r < m) src = static_cast<const T*>(a.y) + (long long)__ldcg(a.perm + grp.y + r) * a.y_st;
       }
       const int s = j % C::Ring, bytes = 2 * min(kAD_Tile, a.d_out - c * kAD_Tile);
       if (!mbar_wait_warp_small(y_free + s, (j / C::Ring & 1) ^ 1, abort, 0x82)) break;

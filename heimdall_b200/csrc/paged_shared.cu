@@ -101,8 +101,8 @@ struct SharedArgs {
 struct Plan {
   const int32_t *slots, *order, *last, *skip, *runs;
   int n_runs;
-  __device__ __forceinline__ Plan(const int32_t* p, int n)
-      : slots(p + kPS_Head), order(slots + n), last(order + 2 * (size_t)n), skip(last + n), runs(skip + n), n_runs(min(max(p[0], 0), n)) {}
+  __device__ __forceinline__ Plan(const int32_t* p, int n, int runs_said)
+      : slots(p + kPS_Head), order(slots + n), last(order + 2 * (size_t)n), skip(last + n), runs(skip + n), n_runs(min(max(runs_said, 0), n)) {}
 };
 
 // a piece of the line: run e, or, behind the runs, the tail of the sequence at place e - n_runs
@@ -146,12 +146,11 @@ __device__ __forceinline__ __half2 from_e4m3(uint16_t x) {
 template <typename T>
 __global__ void __launch_bounds__(256) paged_queries_kernel(SharedArgs a) {
   constexpr int Parts = SharedCfg<T>::Parts;
-  wait_for_stream();
-  let_next_start();        // only now: what the next kernel reads before its own wait is older than this one
+  wait_then_let_next_start();
   const int lane = threadIdx.x & 31, g = blockIdx.y, per_seq = a.t * a.R;
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (long long)a.n * per_seq;
   if (row >= rows) return;
-  const Plan pl(a.plan, a.n);
+  const Plan pl(a.plan, a.n, a.plan[0]);
   const int place = (int)(row / per_seq), rem = (int)(row - (long long)place * per_seq), i = rem / a.R, h = g * a.R + rem - i * a.R;
   const uint4 raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + pl.order[place] * a.q_sb + i * a.q_st + h * a.q_sh + 8 * lane));
   const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -259,7 +258,7 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   const uint32_t ring_at = smem_u32(ring), q_at = smem_u32(sQ);
   int* s_sum = reinterpret_cast<int*>(bars + 38);      // [16][2] totals of the warps that scan
   Stretch* s_first = reinterpret_cast<Stretch*>(bars + 54);       // the stretch that this CTA begins in
-  int* s_start = reinterpret_cast<int*>(bars + 58);    // stretch, unit in it, rows before it
+  int* s_start = reinterpret_cast<int*>(bars + 58);    // stretch, unit in it, rows before it; the plan's runs
   SharedTile* s_tile = reinterpret_cast<SharedTile*>(bars + 64);  // [4]
   float2* s_ml = reinterpret_cast<float2*>(s_tile + 4);           // [4][2][128] a tile's maxima and sums, of both halves of its tokens
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -291,10 +290,12 @@ __global__ void __launch_bounds__(kSH_Threads, 1)
   }
   if (warp == 2 && lane == 0) tma_prefetch(&vmap);
   let_next_start();
+  if (tid == 96) s_start[3] = acquire_early(a.plan);
+  __syncthreads();
   // this CTA's part of the line: the stretches' units summed over the warps of softmax and accumulators, thread i holding `per` consecutive ones.  (The plan and
-  // the lengths are older than the kernel before this one, which began by waiting for what was before it.)
+  // the lengths are older than the kernel before this one: launch_early.h.)
   constexpr int kScan = kSH_Threads - 128;
-  const Plan pl(a.plan, a.n);
+  const Plan pl(a.plan, a.n, s_start[3]);
   const int stretches = pl.n_runs + a.n, per = (stretches + kScan - 1) / kScan, e0 = (tid - 128) * per;
   Stretch mine0;                       // thread's first
   int2 mine = make_int2(0, 0);
@@ -859,7 +860,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(SharedArgs a) {
   const long long sr = (long long)blockIdx.x * 32 + lane;
   const bool on = sr < (long long)a.n * per_seq;
   if (warp == 0) {
-    const Plan pl(a.plan, a.n);
+    const Plan pl(a.plan, a.n, a.plan[0]);
     const int place = on ? (int)(sr / per_seq) : 0, rem = on ? (int)(sr - (long long)place * per_seq) : 0, i = rem / a.R;
     const int4 head = *a.head;
     const int each = head.x, more = head.y, longer = more * (each + 1);
