@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(AdapterArgs a) 
 #pragma unroll 4
   for (int k = k0 + 32 * warp; k < k1; k += 256) {
     const bool in = k + 8 * c < k1;      // whole 16 bytes: d_in and the parts are multiples of 8
-    const uint4 a0 = in && g < m ? __ldg(reinterpret_cast<const uint4*>(x0 + k)) : none;
-    const uint4 a1 = in && g + 8 < m ? __ldg(reinterpret_cast<const uint4*>(x1 + k)) : none;
+    const uint4 a0 = in && g < m ? *reinterpret_cast<const uint4*>(x0 + k) : none;
+    const uint4 a1 = in && g + 8 < m ? *reinterpret_cast<const uint4*>(x1 + k) : none;
     const uint4 b0 = in ? ldg_stream(reinterpret_cast<const uint4*>(w0 + k)) : none;
     const uint4 b1 = in ? ldg_stream(reinterpret_cast<const uint4*>(w1 + k)) : none;
     mma16816<T>(acc[0], a0.x, a1.x, a0.y, a1.y, b0.x, b0.y);
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a, int 
     for (long long t0 = begin; t0 < end; t0 += 256) {
       int id[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) id[k] = t0 + 32 * k + lane < end ? adapter_of(a, __ldg(a.ids + t0 + 32 * k + lane)) : -1;
+      for (int k = 0; k < 8; ++k) id[k] = t0 + 32 * k + lane < end ? adapter_of(a, a.ids[t0 + 32 * k + lane]) : -1;
       // 256 tokens of one adapter at once
       const int one = __shfl_sync(0xffffffffu, id[0], 0);
       bool alike = one >= 0;

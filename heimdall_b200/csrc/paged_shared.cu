@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(256) paged_queries_kernel(SharedArgs a) {
   if (row >= rows) return;
   const Plan pl(a.plan, a.n, a.plan[0]);
   const int place = (int)(row / per_seq), rem = (int)(row - (long long)place * per_seq), i = rem / a.R, h = g * a.R + rem - i * a.R;
-  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + pl.order[place] * a.q_sb + i * a.q_st + h * a.q_sh + 8 * lane));
+  const uint4 raw = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + pl.order[place] * a.q_sb + i * a.q_st + h * a.q_sh + 8 * lane);
   const uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
   // the largest value of the row, as 16-bit patterns without their sign
   const uint32_t m2 = __vmaxu2(__vmaxu2(v[0] & 0x7fff7fffu, v[1] & 0x7fff7fffu), __vmaxu2(v[2] & 0x7fff7fffu, v[3] & 0x7fff7fffu));
