@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(1024) adapter_route_kernel(AdapterArgs a, int 
 // through a ring in shared memory (K-major, 128-byte swizzle; eight warps copy); a thread issues the products, D in TMEM (two of them) is the group's h.  A run
 // that has part of a group leaves its sums in one of the CTA's two places (its first group, begun by others; its last, ended by others); the CTA that is the
 // last to bring a group's part adds them all, in their order, and makes the two parts.  (A grid of groups and parts of d_in, two CTAs per SM: 25480 tokens of
-// 6144 took 92 us, 8192 of 5120 37, against 69 and 32.)
+// 6144 took 92 us, 8192 of 5120 37, against 69 and 32; these and the next kernel's times in bursts at 1965 MHz.)
 constexpr int kAD_Ctas = 148, kAD_Step = 128, kAD_MinSteps = 8;
 template <int RM>
 struct ShrinkCfg {

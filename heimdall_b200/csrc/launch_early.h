@@ -11,8 +11,8 @@ namespace bfb {
 // let_next_start(): from the moment that all of this kernel's CTAs run, the next kernel's may take what is left of the SMs.
 //
 // The rule: wait_for_stream() in every thread, before its first read or write of global memory.  Such a kernel may let the next one start at any time.
-// What the kernel before may have written is read by plain loads, not by __ldg: that says that nobody writes it while this kernel runs, which begins before its
-// wait, and leaves the compiler free to take it earlier.
+// What the kernel before may have written is read by plain loads, unless the address itself comes from behind the wait: __ldg says that nobody writes it while this kernel
+// runs, which begins before its wait, and leaves the compiler free to take it earlier.
 //
 // The exception, within one call: a kernel that reads before its wait what is older than the kernel before it.
 //   * The kernel before it calls wait_then_let_next_start() in every thread, first of all: then all that is older has ended when the reader starts.  No

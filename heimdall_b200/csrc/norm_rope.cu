@@ -11,7 +11,7 @@
 // are not turned (cos 1, sin 0): no value changes lanes, at the price of 8-byte accesses.  The rotated heads are made from y in fp32, so
 // each output is rounded once.
 // The instructions of a head come next to HBM as a bound: with the partner's values by shuffles and 64-bit divisions for every four heads it
-// took 75 us for 8191 tokens of 24 + 4 heads and 446 for 65536 without q and k, now 65 (5.4 TB/s) and 345 (5.5).  Two heads at a time on three or
+// took 75 us for 8191 tokens of 24 + 4 heads and 446 for 65536 without q and k, now 65 (5.4 TB/s) and 345 (5.5; sustained, at the board's power cap, 66 and 352 to 364).  Two heads at a time on three or
 // four CTAs per SM, which costs spills, 72 to 80 and 394 to 426; 16 tokens per CTA 65 and 350.
 #include "capi_internal.h"
 #include "common.cuh"
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(256, 2) norm_rope_kernel(NormRopeArgs a) {
     }
   }
   // An infinity (and no NaN) in a head makes its own dim NaN and the others 0, and 0 times that NaN has made NaN of dims that are not turned.  Those are y
-  // itself: written once more, by the lane that has both.  (Told apart in every head, that takes 370 us for 65536 tokens without q and k, against 361.)
+  // itself: written once more, by the lane that has both.  (Told apart in every head, that takes 370 us for 65536 tokens without q and k, against 361, sustained.)
   if (most < INFINITY) return;
   t = 0;
   j = warp;

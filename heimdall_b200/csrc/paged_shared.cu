@@ -973,11 +973,11 @@ static int launch_shared(const SharedArgs& a, int ctas, cudaStream_t stream) {
   const unsigned per_head = (unsigned)(rows / a.p.heads);
   if ((rc = launch_early(paged_queries_kernel<T>, dim3((per_head + 7) / 8, a.p.heads), 256, 0, stream, a))) return rc;
   if ((rc = launch_early(paged_shared_kernel<T>, dim3(ctas), kSH_Threads, SharedSmem<T>::Bytes, stream, kmap, vmap, qmap, a))) return rc;
-  // a row's pieces are dealt to so many warps that there are 600 to 1200 of them: with few rows the pieces' way is what takes time (whole call, 16 x 24 rows of
+  // a row's pieces are dealt to so many warps that there are 600 to 1200 of them: with few rows the pieces' way is what takes time (whole call, in bursts at 1965 MHz, 16 x 24 rows of
   // 37 pieces each: 100, 90, 85 and 86 us over 1, 2, 4 and 8), with many the blocks (64 x 24 rows of 13: 48, 52, 53 and 62)
   const unsigned blocks = (per_head + 31) / 32, warps = blocks * a.p.heads * (kPG_D / kSH_MergeDims);
   // Its CTAs come as those of the kernel before them leave their SMs: each takes so much shared memory that no SM has more than its share of them, or the
-  // first SMs that are free would take them all (16 x 131072: 84 us against 93).
+  // first SMs that are free would take them all (16 x 131072, in bursts: 84 us against 93).
   auto merge = [&](auto kernel, int split) {
     const unsigned ctas_y = kPG_D / kSH_MergeDims * split / 8, each = (blocks * ctas_y * a.p.heads + ctas - 1) / ctas;
     const int idle = each < 8 ? (232448 / (int)each - 1024) / 1024 * 1024 - kSH_MergeSmem : 0;

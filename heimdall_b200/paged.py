@@ -439,7 +439,7 @@ class PagedKV:
         is belongs to the cache: fetched once or for every call, a layer goes on where it was.  ``share``: pages that
         the sequences have in common are read once for all of them (``attend(shared=)``, with its precision there); the plan, one for
         all layers, is made at the first call that needs it and after forks, and again when it is no longer good.  That is host work: before such a call is captured,
-        one has to have run."""
+        one has to have run.  One plan is kept for each number of sequences, for the calls captured with it."""
         return PagedLayer(self, self._layer(layer), share)
 
     def _layer_plan(self, B: int):
